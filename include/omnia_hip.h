@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define OMNIA_ABI_VERSION 15
+#define OMNIA_ABI_VERSION 16
 
 /* Version of this ABI (OMNIA_ABI_VERSION). Pure; touches no device. */
 int32_t omnia_abi_version(void);
@@ -643,6 +643,103 @@ int32_t omnia_attention_prefill(const uint16_t* queries, const uint16_t* keys,
  * copy of B / 2 bytes) and that scales the HBM byte counters. */
 int32_t omnia_stream_copy(const void* src, void* dst, int64_t bytes, int32_t vectors_per_thread,
                           hipStream_t stream);
+
+/* Pages of a cache that many sequences share.
+ *
+ * A pool is `keys` and `values` [layers, pages, kv_heads, page_rows, D] bf16. Sequence s lies
+ * on the pages tables[s][0 ..], the same in every layer (row r is row r % page_rows of page
+ * tables[s][r / page_rows]; -1 for no page), and holds lengths[s] rows. tables [sequences,
+ * width] and lengths [sequences] are int32, on the device.
+ * No counterpart in the reference, whose caches hold a sequence each (core/cache/kv.py). */
+
+/* Most moves and edits one call takes: they travel in the kernel's arguments. */
+#define OMNIA_PAGES_MOVES 256
+#define OMNIA_PAGES_EDITS 128
+
+/* Copies the first rows of pages, in every layer, keys and values: moves [count, 3] int32 in
+ * HOST memory (from, to, rows: 1 to page_rows of every head; the rest of the page stays as it
+ * is). With `tables` (`entries` of them, else null) every entry that names `from` is renamed
+ * to `to`; the moves are then sorted by `from`. No page may be written twice, or both read
+ * and written. head_dim a multiple of 8. */
+int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages,
+                         int64_t kv_heads, int64_t page_rows, int64_t head_dim,
+                         const int32_t* moves, int64_t count, int32_t* tables, int64_t entries,
+                         hipStream_t stream);
+
+/* Edits of tables and lengths: edits [count, 5] int32 in HOST memory (kind, sequence, a, b, c):
+ *   OMNIA_PAGES_ENTRY   tables[sequence][a] = b
+ *   OMNIA_PAGES_LENGTH  lengths[sequence] = a
+ *   OMNIA_PAGES_FORK    tables[sequence] = the first b entries of sequence a, then page c (or
+ *                       -1), then -1; lengths[sequence] = lengths[a]
+ *   OMNIA_PAGES_CLEAR   tables[sequence] = -1, lengths[sequence] = 0 (b 0, c -1)
+ * No edit may write what another one of the call writes or reads. */
+#define OMNIA_PAGES_ENTRY 0
+#define OMNIA_PAGES_LENGTH 1
+#define OMNIA_PAGES_FORK 2
+#define OMNIA_PAGES_CLEAR 3
+int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t sequences, int64_t width,
+                         int64_t pages, const int32_t* edits, int64_t count, hipStream_t stream);
+
+/* lengths[chosen[i]] += rows[i] for i < count, all on the device; the chosen are distinct. An
+ * index outside [0, sequences) is passed over. */
+int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* chosen,
+                            const int32_t* rows, int64_t count, hipStream_t stream);
+
+/* The prologue of an attention layer over the new tokens of a batch of sequences: token t is
+ * its sequence's token_map[t] = (sequence, j), at position p = lengths[sequence] + j, and
+ *   n = x * w / sqrt(sum x^2 / D + eps)                  (n = x without a gain)
+ *   a, b = n_i * mscale, n_{i+P} * mscale                 i < P = rotary_pairs
+ *   y_i = a cos[p][i] - b sin[p][i], y_{i+P} = a sin[p][i] + b cos[p][i], y_d = n_d beyond
+ * in fp32, rounded once to bf16 (omnia_attention_project rounds in between as well, as the
+ * single sequence's chain does). Queries go to queries [tokens, heads, D], keys and values to
+ * row p of the sequence's pages, of one layer: keys, values [pages, kv_heads, page_rows, D].
+ * A token whose sequence, position or page is not there stores no key and no value; a
+ * position past the angle rows reads the last of them. raw_queries [tokens, heads * D],
+ * raw_keys / raw_values [tokens, kv_heads * D], rows their strides apart; cos_rows, sin_rows
+ * [angle_rows, P] fp32, `table_stride` floats apart (null with P = 0).
+ * Beside: core/kernels/attention/default.py:85-131 (one sequence's).
+ * head_dim 64 or 128; rotary_pairs a multiple of 8 with 2P <= D; page_rows 16, 32, 64, 128 or
+ * 256. */
+int32_t omnia_attention_batch_project(
+    const uint16_t* raw_queries, int64_t query_stride, const uint16_t* raw_keys,
+    int64_t key_stride, const uint16_t* raw_values, int64_t value_stride,
+    const uint16_t* query_weight, const uint16_t* key_weight, const float* cos_rows,
+    const float* sin_rows, int64_t table_stride, int64_t angle_rows, int64_t rotary_pairs,
+    float mscale, float eps, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+    uint16_t* queries, uint16_t* keys, uint16_t* values, int64_t pages, int64_t page_rows,
+    const int32_t* tables, int64_t sequences, int64_t width, const int32_t* lengths,
+    const int32_t* token_map, hipStream_t stream);
+
+/* Workspace bytes omnia_attention_batch needs. -EINVAL for a bad geometry. Pure; touches no
+ * device. */
+int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
+                                              int64_t head_dim, int64_t prefix, int64_t own_rows,
+                                              int64_t own_tiles);
+
+/* Attention of a batch's new tokens over their sequences' pages (rows written by
+ * omnia_attention_batch_project), the rows that all of them share taken once:
+ *   token t = (s, j) = token_map[t] sees rows r <= lengths[s] + j of sequence s,
+ *   out[t, h] = sum_r exp(x - M) v[r] / (exp(sink[h] - M) + sum_r exp(x - M)),
+ *   x = scale * (q[t, h] . k[r, h / gqa])
+ * in fp32, the weights rounded to bf16 for their product with the values, the result once to
+ * bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
+ * prefix) must be the same pages in every token's sequence: they are read through the first
+ * token's. own_rows bounds the rows past them of every sequence, this step's included; tiles
+ * [own_tiles, 2] int32 (device) are runs [first, end) of query rows of one sequence, at most
+ * 128 long, that cover every row once (of each kv head, row r is token r / gqa, head r % gqa).
+ * A row on no page (-1, or outside the pool) is not seen. queries, out [tokens, heads, D];
+ * workspace: at least omnia_attention_batch_workspace_bytes, 16-byte aligned.
+ * Beside: core/kernels/attention/default.py:132-156 (one sequence's).
+ * head_dim 64 or 128; heads a multiple of kv_heads; scale positive and finite. */
+int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t* keys,
+                              const uint16_t* values, int64_t pages, int64_t page_rows,
+                              const int32_t* tables, int64_t sequences, int64_t width,
+                              const int32_t* lengths, const int32_t* token_map, int64_t tokens,
+                              const int32_t* tiles, int64_t own_tiles, int64_t prefix,
+                              int64_t own_rows, int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, const uint16_t* sinks, float scale,
+                              void* workspace, int64_t workspace_bytes, uint16_t* out,
+                              hipStream_t stream);
 
 #ifdef __cplusplus
 }

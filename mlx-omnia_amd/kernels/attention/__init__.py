@@ -35,12 +35,16 @@ from .._device import hip_device
 from ..qkv_rope.atlas import AngleAtlas
 from ..qkv_rope.kernel import AngleTable
 from ..resolve import record_fallback, resolve
+from .batch import (BatchAttentionStep, BatchAttentionStepStrategy, DefaultBatchAttentionStep,
+                    HipBatchAttentionStep, batch_step_applies)
 from .cache import FixedKVCache, KVCache, RingKVCache
+from .pages import PagedBatch, PagedKVCache
 from .prefill import prefill, project, project_served
 
-__all__ = ["AttentionStep", "AttentionStepStrategy", "DefaultAttentionStep", "FixedKVCache",
-           "HipAttentionStep", "HipSinkAttentionStep", "KVCache", "RingKVCache", "attention_step_applies",
-           "sink_step_applies"]
+__all__ = ["AttentionStep", "AttentionStepStrategy", "BatchAttentionStep", "BatchAttentionStepStrategy",
+           "DefaultAttentionStep", "DefaultBatchAttentionStep", "FixedKVCache", "HipAttentionStep",
+           "HipBatchAttentionStep", "HipSinkAttentionStep", "KVCache", "PagedBatch", "PagedKVCache", "RingKVCache",
+           "attention_step_applies", "batch_step_applies", "sink_step_applies"]
 
 HEAD_DIM = 128
 

@@ -14,7 +14,7 @@ import threading
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "libomnia_hip.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -97,6 +97,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_attention_prefill_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "omnia_attention_prefill": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _P, _I64,
                                        _P, _F32, _P, _I64, _P, _P]),
+    "omnia_pages_copy": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "omnia_pages_edit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "omnia_pages_advance": (_I32, [_P, _I64, _P, _P, _I64, _P]),
+    "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
+                                             _F32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _I64,
+                                             _P, _P, _P]),
+    "omnia_attention_batch_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "omnia_attention_batch": (_I32, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
+                                     _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
     "omnia_embed_atlas": (
         _I32,
         [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P],

@@ -9,6 +9,7 @@ fit.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -1150,6 +1151,204 @@ def attention_prefill(
     call("omnia_attention_prefill", queries.data_ptr(), keys.data_ptr(), values.data_ptr(), key_stride,
          value_stride, heads, kv_heads, head_dim, length, rows, int(causal),
          mask.data_ptr() if mask is not None else None, mask_stride,
+         sinks.data_ptr() if sinks is not None else None, float(scale),
+         workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
+    return out
+
+
+PAGES_MOVES, PAGES_EDITS = 256, 128   # OMNIA_PAGES_MOVES, OMNIA_PAGES_EDITS
+PAGES_ENTRY, PAGES_LENGTH, PAGES_FORK, PAGES_CLEAR = 0, 1, 2, 3
+
+
+def _int_lines(lines, width: int, name: str):
+    """Lists of `width` whole numbers that fit 32 bits, as one array the library reads."""
+    flat = [int(n) for line in lines for n in line]
+    if len(flat) != width * len(lines):
+        raise ValueError(f"{name}: every one is {width} numbers")
+    if flat and not (-(1 << 31) <= min(flat) and max(flat) < 1 << 31):
+        raise ValueError(f"{name}: a number outside 32 bits")
+    return (ctypes.c_int32 * len(flat))(*flat)
+
+
+def _page_tables(tables: torch.Tensor, lengths: torch.Tensor, name: str) -> tuple[int, int]:
+    if not (tables.dtype == lengths.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous()
+            and lengths.is_contiguous() and tuple(lengths.shape) == (tables.shape[0],)):
+        raise ValueError(f"{name}: tables must be contiguous int32 [sequences, width] and lengths [sequences]")
+    return tables.shape
+
+
+def pages_copy(keys: torch.Tensor, values: torch.Tensor, moves, *, tables: torch.Tensor | None = None) -> None:
+    """Copy pages of the pool `keys`, `values` [layers, pages, kv_heads, page_rows, D] in every
+    layer: moves are (from, to, rows), rows the first of the page that are copied. No page may
+    be written twice, or read and written. With `tables` (int32, on the device) the entries
+    that name a page left are renamed, and moves are sorted by it; see `omnia_pages_copy`."""
+    _require(keys.dim() == 5 and keys.shape == values.shape and keys.dtype == values.dtype,
+             "pages_copy: keys and values must be [layers, pages, kv_heads, page_rows, head_dim]")
+    for pool, name in ((keys, "keys"), (values, "values")):
+        _dense(pool, keys.dtype, name)
+    layers, pages, kv_heads, page_rows, head_dim = keys.shape
+    width = head_dim * keys.element_size()
+    _require(width % 16 == 0, "pages_copy: rows must be whole 16-byte vectors")
+    tensors = [keys, values]
+    if tables is not None:
+        _require(tables.dtype == torch.int32 and tables.is_contiguous(), "pages_copy: tables must be contiguous int32")
+        tensors.append(tables)
+    _require(on_rocm(*tensors), "pages_copy: tensors must share one ROCm device")
+    moves = list(moves)
+    if len(moves) > PAGES_MOVES:   # within one call the library asks this itself
+        written = {to for _, to, _ in moves}
+        if len(written) < len(moves) or not written.isdisjoint(source for source, _, _ in moves):
+            raise ValueError("pages_copy: a page is written twice, or both read and written")
+        if tables is not None and any(a[0] >= b[0] for a, b in zip(moves, moves[1:])):
+            raise ValueError("pages_copy: moves that rename have to be sorted by the page they leave")
+    stream = _stream(keys)
+    for first in range(0, len(moves), PAGES_MOVES):
+        some = moves[first : first + PAGES_MOVES]
+        call("omnia_pages_copy", keys.data_ptr(), values.data_ptr(), layers, pages, kv_heads, page_rows, width // 2,
+             _int_lines(some, 3, "moves"), len(some), tables.data_ptr() if tables is not None else None,
+             tables.numel() if tables is not None else 0, stream)
+
+
+def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -> None:
+    """Edits of page tables on the device, each (kind, sequence, a, b, c); see
+    `omnia_pages_edit`. More than PAGES_EDITS are made in turn, as many at a time."""
+    sequences, width = _page_tables(tables, lengths, "pages_edit")
+    _require(on_rocm(tables, lengths), "pages_edit: tensors must share one ROCm device")
+    edits, stream = list(edits), _stream(tables)
+    for first in range(0, len(edits), PAGES_EDITS):
+        some = edits[first : first + PAGES_EDITS]
+        call("omnia_pages_edit", tables.data_ptr(), lengths.data_ptr(), sequences, width, pages,
+             _int_lines(some, 5, "edits"), len(some), stream)
+
+
+def pages_advance(lengths: torch.Tensor, chosen: torch.Tensor, rows: torch.Tensor) -> None:
+    """lengths[chosen[i]] += rows[i], all int32 on the device, the chosen distinct."""
+    for t, name in ((lengths, "lengths"), (chosen, "chosen"), (rows, "rows")):
+        if not (t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()):
+            raise ValueError(f"{name}: must be contiguous int32, one axis")
+    _require(chosen.shape == rows.shape, "pages_advance: as many rows as sequences chosen")
+    _require(on_rocm(lengths, chosen, rows), "pages_advance: tensors must share one ROCm device")
+    call("omnia_pages_advance", lengths.data_ptr(), lengths.numel(), chosen.data_ptr(), rows.data_ptr(),
+         chosen.numel(), _stream(lengths))
+
+
+def _layer_pool(keys: torch.Tensor, values: torch.Tensor, name: str) -> tuple[int, int, int, int]:
+    """(pages, kv_heads, page_rows, D) of one layer's pool."""
+    if keys.dim() != 4 or keys.shape != values.shape:
+        raise ValueError(f"{name}: keys and values must be [pages, kv_heads, page_rows, head_dim]")
+    _dense(keys, BF16, "keys")
+    _dense(values, BF16, "values")
+    return keys.shape
+
+
+def _token_map(token_map: torch.Tensor, tokens: int, name: str) -> None:
+    if not (token_map.dtype == torch.int32 and token_map.is_contiguous() and tuple(token_map.shape) == (tokens, 2)):
+        raise ValueError(f"{name}: token_map must be contiguous int32 [tokens, 2]")
+
+
+def attention_batch_project(
+    raw_queries: torch.Tensor,
+    raw_keys: torch.Tensor,
+    raw_values: torch.Tensor,
+    query_weight: torch.Tensor | None,
+    key_weight: torch.Tensor | None,
+    angles: tuple[torch.Tensor, torch.Tensor] | None,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    tables: torch.Tensor,
+    lengths: torch.Tensor,
+    token_map: torch.Tensor,
+    *,
+    heads: int,
+    eps: float,
+    mscale: float = 1.0,
+    queries: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The norms, the rotation and the page writes of a batch's new tokens in one launch; see
+    `omnia_attention_batch_project`. raw_queries [(1,) N, heads * D], raw_keys and raw_values
+    [(1,) N, kv_heads * D] bf16 rows, weights [D] or None, angles the (cos, sin) tables
+    [positions, pairs] fp32 or None, keys and values a layer's pool [pages, kv_heads,
+    page_rows, D], tables and lengths as the cache holds them, token_map [N, 2] -> the
+    queries [N, heads, D]."""
+    pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch_project")
+    tokens, q_stride = _token_rows(raw_queries, heads * head_dim, "raw_queries")
+    k_tokens, k_stride = _token_rows(raw_keys, kv_heads * head_dim, "raw_keys")
+    v_tokens, v_stride = _token_rows(raw_values, kv_heads * head_dim, "raw_values")
+    _require(k_tokens == tokens and v_tokens == tokens, "attention_batch_project: q, k, v differ in length")
+    sequences, width = _page_tables(tables, lengths, "attention_batch_project")
+    _token_map(token_map, tokens, "attention_batch_project")
+    tensors = [raw_queries, raw_keys, raw_values, keys, values, tables, lengths, token_map]
+    for weight, name in ((query_weight, "query_weight"), (key_weight, "key_weight")):
+        if weight is not None:
+            _dense(weight, BF16, name)
+            if not (weight.numel() == head_dim):
+                raise ValueError(f"{name}: must be [head_dim]")
+            tensors.append(weight)
+    pairs = table_stride = angle_rows = 0
+    if angles is not None:
+        cos, sin = angles
+        angle_rows, pairs = cos.shape
+        for rows, name in ((cos, "cos"), (sin, "sin")):
+            if not (rows.dtype == F32 and rows.shape == cos.shape and rows.stride(-1) == 1
+                    and rows.data_ptr() % 16 == 0):
+                raise ValueError(f"{name}: fp32 [positions, pairs], 16-byte aligned with unit inner stride")
+        table_stride = cos.stride(0) if angle_rows > 1 else pairs
+        _require(angle_rows <= 1 or sin.stride(0) == table_stride,
+                 "attention_batch_project: cos and sin row strides differ")
+        tensors += [cos, sin]
+    _require(on_rocm(*tensors), "attention_batch_project: tensors must share one ROCm device")
+    queries = _out(queries, raw_queries, (tokens, heads, head_dim), BF16, "queries")
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    call("omnia_attention_batch_project", raw_queries.data_ptr(), q_stride, raw_keys.data_ptr(), k_stride,
+         raw_values.data_ptr(), v_stride, ptr(query_weight), ptr(key_weight),
+         cos.data_ptr() if angles is not None else None, sin.data_ptr() if angles is not None else None,
+         table_stride, angle_rows, pairs, float(mscale), float(eps), tokens, heads, kv_heads, head_dim,
+         queries.data_ptr(), keys.data_ptr(), values.data_ptr(), pages, page_rows, tables.data_ptr(), sequences,
+         width, lengths.data_ptr(), token_map.data_ptr(), _stream(raw_queries))
+    return queries
+
+
+def attention_batch(
+    queries: torch.Tensor,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    tables: torch.Tensor,
+    lengths: torch.Tensor,
+    token_map: torch.Tensor,
+    tiles: torch.Tensor,
+    *,
+    prefix: int,
+    own_rows: int,
+    scale: float,
+    sinks: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a batch's new tokens, queries [N, heads, D], over a layer's pages; see
+    `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence,
+    own_rows bounds the rows past them, tiles [n, 2] are runs of one sequence's query rows;
+    sinks [heads] bf16 or None -> [N, heads, D]."""
+    pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
+    _dense(queries, BF16, "queries")
+    _require(queries.dim() == 3 and queries.shape[2] == head_dim, "attention_batch: queries must be [N, heads, D]")
+    tokens, heads, _ = queries.shape
+    sequences, width = _page_tables(tables, lengths, "attention_batch")
+    _token_map(token_map, tokens, "attention_batch")
+    _require(tiles.dtype == torch.int32 and tiles.is_contiguous() and tiles.dim() == 2 and tiles.shape[1] == 2,
+             "attention_batch: tiles must be contiguous int32 [n, 2]")
+    tensors = [queries, keys, values, tables, lengths, token_map, tiles]
+    if sinks is not None:
+        _require(sinks.dtype == BF16 and sinks.is_contiguous() and sinks.numel() == heads,
+                 "attention_batch: sinks must be contiguous bf16 [heads]")
+        tensors.append(sinks)
+    _require(on_rocm(*tensors), "attention_batch: tensors must share one ROCm device")
+    nbytes = library().omnia_attention_batch_workspace_bytes(tokens, heads, kv_heads, head_dim, prefix, own_rows,
+                                                             tiles.shape[0])
+    _require(nbytes >= 0, "attention_batch: geometry not served")
+    workspace = torch.empty(nbytes // 4, dtype=F32, device=queries.device) if nbytes else None
+    out = _out(out, queries, (tokens, heads, head_dim), BF16, "out")
+    call("omnia_attention_batch", queries.data_ptr(), keys.data_ptr(), values.data_ptr(), pages, page_rows,
+         tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), tokens, tiles.data_ptr(),
+         tiles.shape[0], prefix, own_rows, heads, kv_heads, head_dim,
          sinks.data_ptr() if sinks is not None else None, float(scale),
          workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
     return out

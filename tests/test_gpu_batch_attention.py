@@ -1,0 +1,514 @@
+"""The cache of pages and the batch step on the device, against the float64 oracle.
+
+Tolerances, from the roundings the kernels make (half a step of bf16 is 2^-8 of the value):
+- a query or key row is rounded once, after fp32 operations whose errors are a few 2^-24 of
+  the head's largest element: 2^-8 |want| + 2^-19 max |head|;
+- a context is taken from the kernel's own bf16 queries and pages: the weights are rounded
+  once (2^-8 of the mean of |v| under them) and the result once (2^-8 |want|). The fp32 sums
+  add less than 2^-12 of that mean: a score is a sum of at most 128 exact products of a total
+  size below 64 here, in fp32 (128 halves of 2^-23 times 64 is below 2^-11 at worst and some
+  2^-15 in effect, halved by the softmax's normalisation), and exp2 and the merges a few 2^-22.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_omnia_amd.kernels.attention import BatchAttentionStep, HipBatchAttentionStep, PagedKVCache
+from mlx_omnia_amd.kernels.qkv_rope import AngleAtlas, AngleTable
+from mlx_omnia_amd.kernels.resolve import FALLBACKS
+from mlx_omnia_amd.runtime import ops
+from oracle.batch_attention import attend, turned
+from paged_model import PagedModel, random_calls
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8
+
+
+def wide(t: torch.Tensor) -> np.ndarray:
+    return t.detach().float().cpu().numpy()
+
+
+class Case:
+    """A cache of random pages with the rows of some sequences, a batch of them, a layer."""
+
+    def __init__(self, *, heads, kv_heads, head_dim, page_rows=16, pairs=0, norms=False, sinks=False, prefix=0,
+                 own=(1,), tokens=1, layers=2, layer=1, seed=0, spare=float("nan"), mscale=1.0, scale=None):
+        rng = np.random.default_rng(seed)
+        self.gen = torch.Generator(device="cuda").manual_seed(seed)
+        counts = [tokens] * len(own) if isinstance(tokens, int) else list(tokens)
+        most = prefix + max(o + t for o, t in zip(own, counts)) + 2 * page_rows
+        pages = prefix // page_rows + sum(-(-(o + t) // page_rows) + 2 for o, t in zip(own, counts)) + 4
+        shape = (layers, pages, kv_heads, page_rows, head_dim)
+        self.cache = PagedKVCache(torch.full(shape, spare, dtype=torch.bfloat16, device="cuda"),
+                                  torch.full(shape, spare, dtype=torch.bfloat16, device="cuda"),
+                                  sequences=len(own) + 3, rows=most)
+        # Pages in no order: some are taken first and given back.
+        holes = [self.cache.open(page_rows) for _ in range(2)]
+        parent = self.cache.open(prefix)
+        self.cache.free(holes[:1])
+        kids = self.cache.fork(parent, len(own) - 1) if prefix % page_rows == 0 and len(own) > 1 else []
+        self.chosen = [parent, *kids]
+        for s, more in zip(self.chosen, own):
+            self.cache.reserve(s, prefix + more)
+        lengths = [prefix + more for more in own]
+        # Those rows are the sequences': the cache is taken up again with them.
+        tables = self.cache.tables.cpu().numpy()
+        held = np.zeros(len(tables), dtype=int)
+        held[self.chosen] = lengths
+        held[holes[1]] = page_rows
+        self.cache = PagedKVCache(self.cache.keys, self.cache.values, tables=tables, lengths=held,
+                                  opened=[*self.chosen, holes[1]])
+        for s, n in zip(self.chosen, lengths):
+            at = torch.arange(n, device="cuda")
+            page = self.cache.tables[s, at // page_rows].long()
+            for pool in (self.cache.keys, self.cache.values):
+                new = self.normal(layers, n, kv_heads, head_dim)
+                if s != parent:   # the shared rows are the parent's
+                    new[:, :prefix] = pool[:, page[:prefix], :, at[:prefix] % page_rows].transpose(0, 1)
+                for i in range(layers):
+                    pool[i, page, :, at % page_rows] = new[i]
+        self.heads, self.kv_heads, self.head_dim, self.layer = heads, kv_heads, head_dim, layer
+        self.scale = head_dim ** -0.5 if scale is None else scale
+        self.qw, self.kw = [(1 + 0.2 * self.normal(head_dim).float()).bfloat16() if norms else None for _ in range(2)]
+        self.sinks = self.normal(heads) if sinks else None
+        self.pairs, self.mscale = pairs, mscale
+        theta = rng.uniform(0, 6.3, (most, pairs))
+        self.cos, self.sin = (torch.from_numpy(f(theta).astype(np.float32)).cuda() for f in (np.cos, np.sin))
+        self.batch = self.cache.batch(self.chosen, tokens=counts)
+        self.raw = [self.normal(self.batch.total, n * head_dim) for n in (heads, kv_heads, kv_heads)]
+        self.step = self.make(self.cache)
+
+    def normal(self, *shape):
+        return torch.randn(shape, generator=self.gen, device="cuda").bfloat16()
+
+    def make(self, cache, **more):
+        step = BatchAttentionStep(
+            cache, layer=self.layer, heads=self.heads, kv_heads=self.kv_heads, head_dim=self.head_dim,
+            scale=self.scale, dtype=torch.bfloat16, query_weight=self.qw, key_weight=self.kw, eps=1e-6,
+            rotary_pairs=self.pairs, mscale=self.mscale,
+            angles=AngleTable(self.cos, self.sin) if self.pairs else None, sinks=self.sinks, **more)
+        if not more:
+            assert isinstance(step.strategy, HipBatchAttentionStep)
+        return step
+
+    def check_rows(self, queries, lengths):
+        """Queries, and the key and value rows of the batch's tokens, against the oracle."""
+        raw = [wide(t) for t in self.raw]
+        gains = [None if w is None else wide(w) for w in (self.qw, self.kw)]
+        cos, sin = wide(self.cos), wide(self.sin)
+        tables, size = self.cache.tables.cpu().numpy(), self.cache.page_rows
+        keys, values = wide(self.cache.keys[self.layer]), wide(self.cache.values[self.layer])
+        for t, (s, j) in enumerate(self.batch.token_map.cpu().numpy()):
+            p = int(lengths[s]) + j
+            angles = (cos[p], sin[p]) if self.pairs else (None, None)
+            page = tables[s, p // size]
+            for got, source, gain in ((wide(queries[t]), raw[0][t], gains[0]),
+                                      (keys[page, :, p % size], raw[1][t], gains[1])):
+                want = turned(source.reshape(-1, self.head_dim), gain, *angles, 1e-6, self.mscale)
+                bound = HALF * np.abs(want) + 2.0 ** -19 * np.abs(want).max(axis=1, keepdims=True)
+                assert np.all(np.abs(got - want) <= bound), (t, np.abs(got - want).max())
+            assert np.array_equal(values[page, :, p % size], raw[2][t].reshape(-1, self.head_dim))
+
+    def check_context(self, context, queries, lengths, rows=None):
+        pick = np.arange(self.batch.total) if rows is None else np.asarray(rows)
+        sinks = None if self.sinks is None else wide(self.sinks)
+        want, size = attend(wide(queries)[pick], wide(self.cache.keys[self.layer]), wide(self.cache.values[self.layer]),
+                            self.cache.tables.cpu().numpy(), lengths, self.batch.token_map.cpu().numpy()[pick],
+                            self.scale, sinks)
+        bad = np.abs(wide(context)[pick] - want) > HALF * np.abs(want) + (HALF + 2.0 ** -12) * size
+        assert not bad.any(), (int(bad.sum()), bad.size, np.argwhere(bad)[:4].tolist())
+
+    def check(self, rows=None):
+        before = [p[1 - self.layer].clone() for p in (self.cache.keys, self.cache.values)]
+        lengths = self.cache.lengths.cpu().numpy()
+        queries = self.step.project(self.batch, *self.raw)
+        self.check_rows(queries, lengths)
+        context = self.step(self.batch, *self.raw)
+        assert context.shape == (self.batch.total, self.heads, self.head_dim)
+        self.check_context(context, queries, lengths, rows)
+        again = self.step(self.batch, *self.raw)
+        assert torch.equal(context.view(torch.int16), again.view(torch.int16))   # the same to the last bit
+        for kept, pool in zip(before, (self.cache.keys, self.cache.values)):
+            assert torch.equal(kept.view(torch.int16), pool[1 - self.layer].view(torch.int16))
+        return context
+
+
+GEOMETRIES = [
+    # one token each: groups of 1 to 16, both head sizes, odd batches, every page size
+    dict(heads=2, kv_heads=2, head_dim=128, own=(1,)),
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, own=(0,)),
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=208, own=(1, 20)),
+    dict(heads=32, kv_heads=8, head_dim=128, pairs=64, norms=True, page_rows=64, prefix=640, own=(3, 70, 0, 128, 64)),
+    dict(heads=16, kv_heads=2, head_dim=64, pairs=32, sinks=True, prefix=48, own=tuple(range(0, 33, 3))),
+    dict(heads=9, kv_heads=3, head_dim=64, pairs=8, norms=True, page_rows=32, prefix=2016, own=(5, 300)),
+    dict(heads=5, kv_heads=1, head_dim=128, pairs=32, page_rows=128, prefix=1024, own=(17, 0, 130), mscale=1.3),
+    dict(heads=16, kv_heads=1, head_dim=128, page_rows=256, prefix=256, own=(255, 256, 257, 1)),
+    dict(heads=64, kv_heads=8, head_dim=64, pairs=32, sinks=True, page_rows=16, prefix=2000, own=(333, 90, 4)),
+    dict(heads=4, kv_heads=1, head_dim=128, page_rows=16, prefix=0, own=(5000,)),
+    dict(heads=8, kv_heads=8, head_dim=64, page_rows=16, prefix=16, own=tuple((i * 37) % 61 for i in range(70))),
+    # prompts: one and several tokens, a prompt into an empty sequence, tiles that end anywhere
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, own=(0,), tokens=2),
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, own=(0,), tokens=200),
+    dict(heads=8, kv_heads=2, head_dim=64, sinks=True, page_rows=32, prefix=320, own=(0, 7, 33), tokens=(40, 1, 129)),
+    dict(heads=12, kv_heads=4, head_dim=128, pairs=64, page_rows=64, prefix=128, own=(65, 0), tokens=(3, 70)),
+    dict(heads=16, kv_heads=1, head_dim=128, page_rows=16, prefix=0, own=(777,), tokens=33),
+    dict(heads=129, kv_heads=1, head_dim=64, page_rows=16, prefix=32, own=(3, 9), tokens=(2, 3)),
+]
+
+
+@pytest.mark.parametrize("case", GEOMETRIES, ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", ""))
+def test_step(case):
+    made = Case(**case)
+    made.check(None if made.batch.total * made.heads < 2000 else np.arange(0, made.batch.total, 7))
+
+
+def test_rows_in_use_may_hold_anything_where_nobody_looks():
+    """Pages and page ends nobody holds are NaN in every case here; infinities as well."""
+    for spare in (float("inf"), -3.0e38):
+        Case(heads=8, kv_heads=2, head_dim=128, prefix=96, own=(5, 1, 40), tokens=(1, 3, 1), spare=spare).check()
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_a_value_that_is_not_finite_reaches_only_who_sees_it(head_dim, value):
+    case = Case(heads=8, kv_heads=2, head_dim=head_dim, prefix=32, own=(9, 3), tokens=(50, 20))
+    clean = case.step(case.batch, *case.raw)
+    v = case.raw[2].view(case.batch.total, 2, head_dim)
+    v[30, 1, 5] = value
+    v[60, 0, 7] = value
+    out = case.step(case.batch, *case.raw)
+    touched = torch.zeros_like(out, dtype=torch.bool)
+    touched[30:50, 4:, 5] = True
+    touched[60:70, :4, 7] = True
+    assert torch.equal(out[~touched], clean[~touched])
+    assert (torch.isnan if value != value else lambda t: t == value)(out[touched]).all()
+
+
+def test_infinite_sinks_and_scores():
+    case = Case(heads=4, kv_heads=2, head_dim=64, prefix=16, own=(3, 5), sinks=True)
+    case.sinks[0], case.sinks[1] = -float("inf"), 80.0
+    case.step = case.make(case.cache)
+    out = case.check()
+    assert out[:, 1].abs().max() < 1e-20   # e^80 in the denominator
+    large = Case(heads=4, kv_heads=2, head_dim=64, prefix=16, own=(30, 5), scale=8.0)
+    large.check()   # scores of some hundreds: nearly one weight a row
+
+
+def test_tokens_of_no_sequence_and_pages_of_no_pool():
+    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=64, own=(40, 40, 40))
+    cache, batch = case.cache, case.batch
+    queries = case.step.project(batch, *case.raw)
+    tables, token_map = cache.tables.clone(), batch.token_map.clone()
+    s = case.chosen[1]
+    tables[s, 4] = -1             # rows 64 .. 79 of one sequence are nowhere
+    tables[s, 5] = cache.pages    # nor are 80 .. 95
+    tables[case.chosen[2], 6] = -7
+    token_map[0, 0] = cache.tables.shape[0] + 5
+    # The first token's sequence gives the shared rows: here the second's.
+    token_map[[0, 1]] = token_map[[1, 0]]
+    tiles = batch.tiles(4)
+    lengths = cache.lengths.cpu().numpy()
+    out = ops.attention_batch(queries, cache.keys[1], cache.values[1], tables, cache.lengths, token_map, tiles,
+                              prefix=64, own_rows=41, scale=case.scale)
+    assert (out[1] == 0).all()
+    want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), tables.cpu().numpy(), lengths,
+                        token_map.cpu().numpy(), case.scale)
+    assert np.all(np.abs(wide(out) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
+    # Nothing is written for them either.
+    before = cache.keys.clone()
+    gone = torch.full_like(cache.tables, -1)
+    ops.attention_batch_project(*case.raw, None, None, None, cache.keys[1], cache.values[1], gone, cache.lengths,
+                                batch.token_map, heads=8, eps=1e-6)
+    assert torch.equal(before.view(torch.int16), cache.keys.view(torch.int16))
+
+
+def test_sequences_shorter_than_the_shared_rows():
+    """A plan that is not the cache's own: a sequence that ends inside the shared rows sees its
+    rows of them and no more."""
+    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=160, own=(9, 4, 1))
+    cache, batch = case.cache, case.batch
+    queries = case.step.project(batch, *case.raw)
+    lengths = cache.lengths.clone()
+    lengths[case.chosen[1]], lengths[case.chosen[2]] = 70, -1
+    out = ops.attention_batch(queries, cache.keys[1], cache.values[1], cache.tables, lengths, batch.token_map,
+                              batch.tiles(4), prefix=160, own_rows=10, scale=case.scale)
+    want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), cache.tables.cpu().numpy(),
+                        lengths.cpu().numpy(), batch.token_map.cpu().numpy(), case.scale)
+    assert (out[2] == 0).all()
+    assert np.all(np.abs(wide(out) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
+
+
+def test_raw_rows_are_read_where_they_lie():
+    case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=32, own=(5, 9, 2), tokens=(1, 4, 2))
+    want = case.step(case.batch, *case.raw)
+    fused = torch.cat(case.raw, dim=1)
+    parts = torch.split(fused, [1024, 256, 256], dim=1)
+    assert torch.equal(case.step(case.batch, *parts), want)
+    assert torch.equal(case.step(case.batch, *(p[None] for p in parts)), want)
+    odd = [torch.cat([p.new_zeros(p.shape[0], 3), p], dim=1)[:, 3:] for p in parts]
+    assert torch.equal(case.step(case.batch, *odd), want)
+
+
+def test_reference_and_kernels_agree():
+    case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, norms=True, sinks=True, prefix=64, own=(33, 2), tokens=(5, 9))
+    want = case.make(case.cache, reference=True)(case.batch, *case.raw)
+    got = case.step(case.batch, *case.raw)
+    # The queries may round to either side of a half step, once more than the kernel alone.
+    assert (got.float() - want.float()).abs().max() <= 4 * HALF * want.float().abs().max()
+
+
+def test_a_call_that_autograd_follows_runs_in_torch():
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
+    q = case.raw[0].clone().requires_grad_()
+    before = dict(FALLBACKS)
+    case.step(case.batch, q, *case.raw[1:]).float().sum().backward()
+    assert q.grad is not None and torch.isfinite(q.grad).all()
+    assert FALLBACKS != before
+
+
+def test_steps_that_are_captured():
+    """A step and its advance, captured once and replayed, with eager work between the replays,
+    against the same steps taken eagerly; a page boundary on the way, and another graph."""
+    case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=64, own=(10, 25, 14))
+    twin = PagedKVCache(case.cache.keys.clone(), case.cache.values.clone(), tables=case.cache.tables.cpu().numpy(),
+                        lengths=case.cache.lengths.cpu().numpy(), opened=[*case.chosen, 1])
+    steps = 9
+    inputs = [[torch.empty_like(t).normal_(generator=case.gen) for t in case.raw] for _ in range(steps)]
+    eager, eager_batch = case.make(twin), twin.batch(case.chosen)
+    want = []
+    for raw in inputs:
+        want.append(eager(eager_batch, *raw))
+        twin.advance(eager_batch)
+    step, batch, cache = case.step, case.batch, case.cache
+    with pytest.raises(ValueError):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(batch, *case.raw)
+    torch.cuda.synchronize()
+    step.prepare_capture(batch, steps)
+    graphs = []
+    for advancing in (True, False):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(batch, *case.raw)
+            if advancing:
+                cache.advance(batch)
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    assert cache.rows(case.chosen[0]) == 74
+    for raw, expected in zip(inputs, want):
+        for held, new in zip(case.raw, raw):
+            held.copy_(new)
+        graphs[1][0].replay()   # the same step without the advance, from the other graph
+        torch.empty(1000, device="cuda").normal_().sum().item()
+        graphs[0][0].replay()
+        assert torch.equal(graphs[1][1], graphs[0][1])
+        # The captured plan cuts the keys for all the rows it was prepared for.
+        assert (graphs[0][1].float() - expected.float()).abs().max() <= 4 * HALF * expected.float().abs().max()
+    cache.account(batch, steps)
+    assert torch.equal(cache.lengths, twin.lengths)
+    for s in case.chosen:
+        n = cache.rows(s)
+        at = torch.arange(n, device="cuda")
+        # Pages reserved ahead are others than those taken a step at a time.
+        mine, theirs = (c.keys[1, c.tables[s, at // 16].long(), :, at % 16] for c in (cache, twin))
+        assert torch.equal(mine, theirs)
+    for raw in inputs[:1]:
+        assert torch.equal(step(batch, *raw), eager(eager_batch, *raw))
+
+
+def test_what_cannot_be_captured_is_refused():
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
+    cache = case.cache
+    refused = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.open(3), lambda: cache.fork(case.chosen[0]), lambda: cache.free(case.chosen[0]),
+                     lambda: cache.truncate(case.chosen[0], 1), cache.compact, lambda: cache.resize(500),
+                     lambda: cache.batch(case.chosen), lambda: cache.reserve(case.chosen[0], 60)):
+            try:
+                call()
+            except ValueError as error:
+                refused.append("captured" in str(error))
+        torch.zeros(1, device="cuda")
+    assert refused == [True] * 8
+
+
+def test_another_stream():
+    case = Case(heads=32, kv_heads=8, head_dim=128, pairs=64, norms=True, page_rows=64, prefix=1024, own=(3, 70, 9))
+    want = case.step(case.batch, *case.raw)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [case.step(case.batch, *case.raw) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_pools_past_32_bits():
+    """Pages whose elements lie past 2^31 of their pool, and past 2^32 bytes."""
+    kv_heads, head_dim, size = 8, 128, 256
+    pages = (1 << 31) // (kv_heads * head_dim * size) + 60
+    pool = torch.empty((1, pages, kv_heads, size, head_dim), dtype=torch.bfloat16, device="cuda")
+    cache = PagedKVCache(pool, torch.empty_like(pool), sequences=4, rows=2048)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    normal = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()  # noqa: E731
+    tables = np.full((4, 8), -1, dtype=np.int32)
+    tables[0, :4], tables[1, :3], tables[1, 3] = [pages - 1, 2, pages - 3, pages - 5], [pages - 1, 2, pages - 3], pages - 2
+    for page in [pages - 1, 2, pages - 3, pages - 5, pages - 2]:
+        for p in (cache.keys, cache.values):
+            p[0, page] = normal(kv_heads, size, head_dim)
+    cache = PagedKVCache(cache.keys, cache.values, tables=tables, lengths=np.array([800, 900, 0, 0]), opened=[0, 1])
+    batch = cache.batch([0, 1])
+    assert batch.prefix == 768
+    step = BatchAttentionStep(cache, layer=0, heads=32, kv_heads=8, head_dim=128, scale=128 ** -0.5, dtype=torch.bfloat16)
+    raw = [normal(2, n * 128) for n in (32, 8, 8)]
+    out = step(batch, *raw)
+    # The same rows in a pool of their own.
+    names = {page: i for i, page in enumerate([pages - 1, 2, pages - 3, pages - 5, pages - 2])}
+    small = [torch.stack([p[0, page] for page in names])[None] for p in (cache.keys, cache.values)]
+    near = np.array([[names.get(page, -1) for page in row] for row in tables])
+    twin = PagedKVCache(*small, tables=near, lengths=np.array([800, 900, 0, 0]), opened=[0, 1])
+    other = BatchAttentionStep(twin, layer=0, heads=32, kv_heads=8, head_dim=128, scale=128 ** -0.5, dtype=torch.bfloat16)
+    assert torch.equal(other(twin.batch([0, 1]), *raw), out)
+    kids = cache.fork(1, 2)   # the last page copied, to the front of the pool
+    for kid in kids:
+        assert torch.equal(cache.keys[0, cache.pages_of(kid)[3], :, :132], cache.keys[0, pages - 2, :, :132])
+    cache.free([0, *kids])
+    want = cache.keys[0, [pages - 1, 2, pages - 3]].clone()
+    assert cache.compact() == 4
+    assert torch.equal(cache.keys[0, cache.pages_of(1)[:3]], want)
+    assert cache.tables[1, :4].tolist() == cache.pages_of(1)
+
+
+# The cache's own kernels ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_any_order_of_calls_keeps_every_sequence(seed):
+    rng = np.random.default_rng(seed)
+    cache = PagedKVCache.empty(int(rng.integers(1, 4)), int(rng.integers(8, 30)), 16, 2, 16, device="cuda",
+                               sequences=int(rng.integers(2, 9)), rows=100)
+    random_calls(cache, PagedModel(), rng, 60, check_every=5)
+
+
+@pytest.mark.parametrize("dtype,head_dim", [(torch.bfloat16, 8), (torch.bfloat16, 128), (torch.float32, 24)])
+def test_copies_of_many_pages(dtype, head_dim):
+    """More moves than one launch takes, whole and partial rows, and the tables renamed."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    shape = (3, 700, 3, 16, head_dim)
+    keys, values = (torch.randn(shape, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    before = keys.clone(), values.clone()
+    moves = [(350 + i, 349 - i, 1 + i % 16) for i in range(340)]
+    tables = torch.randint(-1, 700, (40, 33), generator=gen, device="cuda", dtype=torch.int32)
+    old = tables.clone()
+    ops.pages_copy(keys, values, moves, tables=tables)
+    names = torch.arange(-1, 700, device="cuda", dtype=torch.int32)
+    for source, target, rows in moves:
+        names[source + 1] = target
+        for was, now in zip(before, (keys, values)):
+            was[:, target, :, :rows] = was[:, source, :, :rows]
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+    assert torch.equal(tables, names[old.long() + 1])
+
+
+def test_ops_refuse():
+    case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, prefix=32, own=(3, 4))
+    cache, batch, tiles = case.cache, case.batch, case.batch.tiles(4)
+    q = case.step.project(batch, *case.raw)
+    keys, values = cache.keys[1], cache.values[1]
+    base = dict(prefix=32, own_rows=5, scale=1.0)
+    calls = [
+        lambda: ops.attention_batch(q.float(), keys, values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q[:, ::2], keys, values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q, keys.float(), values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables.long(), cache.lengths, batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths[:2], batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map[:1], tiles, **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles[:, :1], **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles.cpu(), **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles, prefix=-1,
+                                    own_rows=5, scale=1.0),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles, prefix=32,
+                                    own_rows=5, scale=0.0),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles,
+                                    sinks=torch.zeros(7, device="cuda").bfloat16(), **base),
+        lambda: ops.attention_batch_project(case.raw[0][:1], *case.raw[1:], None, None, None, keys, values,
+                                            cache.tables, cache.lengths, batch.token_map, heads=8, eps=1e-6),
+        lambda: ops.attention_batch_project(*case.raw, None, None, (case.cos, case.sin[:, :32]), keys, values,
+                                            cache.tables, cache.lengths, batch.token_map, heads=8, eps=1e-6),
+        lambda: ops.pages_copy(cache.keys[:, ::2], cache.values[:, ::2], [(0, 1, 1)]),
+        lambda: ops.pages_copy(cache.keys, cache.values, [(0, cache.pages, 1)]),
+        lambda: ops.pages_copy(cache.keys, cache.values, [(0, 1, 1), (2, 1, 1)] * 200),
+        lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0, 1 << 40, 0)]),
+        lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0)]),
+        lambda: ops.pages_advance(cache.lengths, batch.chosen, batch.rows[:1]),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    short = BatchAttentionStep(cache, layer=0, heads=8, kv_heads=2, head_dim=128, scale=1.0, dtype=torch.bfloat16,
+                               rotary_pairs=64, angles=AngleTable(case.cos[:20], case.sin[:20]))
+    with pytest.raises(ValueError, match="angle table"):
+        short(batch, *case.raw)
+
+
+# A run of them together -----------------------------------------------------------------------
+
+
+def test_answers_sampled_from_one_prompt():
+    """Two layers: a prompt taken in, forked, stepped, some answers freed, the pool compacted
+    and the rest stepped on, against the same sequences with pages of their own and against the
+    oracle; the angles an atlas that grows on the way."""
+    heads, kv_heads, d, layers = 8, 2, 128, 2
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    normal = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()  # noqa: E731
+    gains = [(1 + 0.1 * normal(d).float()).bfloat16() for _ in range(2)]
+    atlas = AngleAtlas(64, base=1e6, rows=64, device="cuda")
+
+    def layered(share):
+        cache = PagedKVCache.empty(layers, 90, 32, kv_heads, d, device="cuda", sequences=9, rows=400)
+        steps = [BatchAttentionStep(cache, layer=i, heads=heads, kv_heads=kv_heads, head_dim=d, scale=d ** -0.5,
+                                    dtype=torch.bfloat16, query_weight=gains[0], key_weight=gains[1],
+                                    rotary_pairs=64, angles=atlas) for i in range(layers)]
+        return cache, steps, share
+
+    def advance(cache, steps, batch, raw):
+        outs = [step(batch, *(t * (i + 1) for t in raw)) for i, step in enumerate(steps)]
+        cache.advance(batch)
+        return torch.stack(outs)
+
+    worlds = [layered(True), layered(False)]
+    prompt = [normal(150, n * d) for n in (heads, kv_heads, kv_heads)]
+    first = []
+    for cache, steps, _ in worlds:
+        assert cache.open() == 0
+        first.append(advance(cache, steps, cache.batch([0], tokens=150), prompt))
+    assert torch.equal(*first)
+    kids = [cache.fork(0, 5, share=share) for cache, _, share in worlds]
+    assert kids[0] == kids[1] and worlds[0][0].free_pages > worlds[1][0].free_pages
+    batches = [cache.batch(kids[0]) for cache, _, _ in worlds]
+    assert batches[0].prefix == 128 and batches[1].prefix == 0
+    close = lambda a, b: (a.float() - b.float()).abs().max() <= 4 * HALF * b.float().abs().max()  # noqa: E731
+    for turn in range(40):
+        if turn == 15:
+            for cache, _, _ in worlds:
+                cache.free([kids[0][1], 0])
+                cache.compact()
+            batches = [cache.batch([kids[0][i] for i in (4, 0, 2, 3)]) for cache, _, _ in worlds]
+            assert batches[0].prefix == 128
+        raw = [normal(batches[0].total, n * d) for n in (heads, kv_heads, kv_heads)]
+        outs = [advance(cache, steps, batch, raw) for (cache, steps, _), batch in zip(worlds, batches)]
+        assert close(*outs), turn
+    cache = worlds[0][0]
+    assert cache.rows(kids[0][0]) == 190 and atlas.rows >= 190
+    queries = worlds[0][1][1].project(batches[0], *raw)
+    got = worlds[0][1][1](batches[0], *raw)
+    want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), cache.tables.cpu().numpy(),
+                        cache.lengths.cpu().numpy(), batches[0].token_map.cpu().numpy(), d ** -0.5)
+    assert np.all(np.abs(wide(got) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)

@@ -1,0 +1,326 @@
+"""The cache of pages and the batch step on the CPU: what the tables say after every kind of
+call, refusals, and the Core chain against the float64 oracle."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_omnia_amd.kernels.attention import (BatchAttentionStep, DefaultBatchAttentionStep, PagedKVCache,
+                                             batch_step_applies)
+from mlx_omnia_amd.kernels.qkv_rope import AngleAtlas, AngleTable
+from mlx_omnia_amd.runtime import ops
+from oracle.batch_attention import attend, turned
+from paged_model import PagedModel, check_against, random_calls
+
+
+def small(pages=12, page_rows=16, sequences=6, rows=96, layers=2, kv_heads=2, head_dim=8):
+    return PagedKVCache.empty(layers, pages, page_rows, kv_heads, head_dim, sequences=sequences, rows=rows)
+
+
+def test_pages_are_handed_out_lowest_first():
+    cache = small()
+    a, b = cache.open(40), cache.open(1)
+    assert (a, b) == (0, 1) and cache.pages_of(a) == [0, 1, 2] and cache.pages_of(b) == [3]
+    cache.free(a)
+    assert cache.open(17) == 0 and cache.pages_of(0) == [0, 1]
+    assert cache.tables[0].tolist() == [0, 1, -1, -1, -1, -1] and cache.lengths.tolist() == [17, 1, 0, 0, 0, 0]
+    assert cache.free_pages == 9
+
+
+def test_fork_shares_full_pages_and_copies_the_rest():
+    cache = small()
+    cache.keys.copy_(torch.arange(cache.keys.numel()).reshape(cache.keys.shape))
+    parent = cache.open(40)
+    before = cache.keys.clone()
+    one, two = cache.fork(parent, 2)
+    assert cache.pages_of(one) == [0, 1, 3] and cache.pages_of(two) == [0, 1, 4]
+    assert torch.equal(cache.keys[:, 3, :, :8], before[:, 2, :, :8])
+    assert torch.equal(cache.keys[:, 3, :, 8:], before[:, 3, :, 8:])   # rows past the last, left alone
+    cache.free([parent, one])
+    assert cache.pages_of(two) == [0, 1, 4] and cache.free_pages == 9
+    (whole,) = cache.fork(two, 1, share=False)
+    assert cache.pages_of(whole) == [2, 3, 5] and cache.rows(whole) == 40
+
+
+@pytest.mark.parametrize("rows", [0, 16, 32])
+def test_fork_at_a_page_end_copies_nothing(rows):
+    cache = small()
+    parent = cache.open(rows)
+    cache.reserve(parent, rows + 20)
+    (kid,) = cache.fork(parent)
+    assert cache.pages_of(kid) == cache.pages_of(parent)[: rows // 16] and cache.rows(kid) == rows
+
+
+def test_a_shared_page_is_copied_before_it_is_written():
+    cache = small()
+    parent = cache.open(32)
+    kids = cache.fork(parent, 2)
+    for s in (parent, *kids):
+        cache.truncate(s, 20)
+    assert cache.pages_of(parent) == [0, 1] == cache.pages_of(kids[0])
+    batch = cache.batch([parent, *kids])
+    assert batch.prefix == 16
+    cache.ready(batch)
+    # The last of the three keeps the page; the others have copies.
+    assert [cache.pages_of(s) for s in (parent, *kids)] == [[0, 2], [0, 3], [0, 1]]
+    assert cache.ready(batch) == 21 and cache.pages_of(parent) == [0, 2]
+
+
+def test_a_page_that_others_keep_is_copied_for_all():
+    cache = small()
+    parent = cache.open(32)
+    kids = cache.fork(parent, 2)
+    cache.truncate(kids[0], 17)
+    cache.ready(cache.batch([kids[0]]))
+    assert cache.pages_of(kids[0]) == [0, 2] and cache.pages_of(kids[1]) == [0, 1] == cache.pages_of(parent)
+
+
+def test_compact_and_resize():
+    cache = small()
+    cache.keys.copy_(torch.arange(cache.keys.numel()).reshape(cache.keys.shape))
+    first, second, third = cache.open(30), cache.open(20), cache.open(16)
+    held = cache.keys[:, [2, 3, 4]].clone()
+    cache.free(first)
+    with pytest.raises(ValueError, match="too few"):
+        cache.resize(3)
+    assert cache.compact() == 3
+    assert cache.pages_of(second) == [2, 0] and cache.pages_of(third) == [1]
+    assert cache.tables[second, :3].tolist() == [2, 0, -1] and cache.tables[third, 0] == 1
+    assert torch.equal(cache.keys[:, [2, 0, 1]], held)
+    assert cache.compact() == 3 and cache.pages_of(second) == [2, 0]
+    cache.resize(3)
+    assert cache.pages == 3 and cache.free_pages == 0 and torch.equal(cache.keys[:, [2, 0, 1]], held)
+    cache.resize(5)
+    assert cache.free_pages == 2 and torch.equal(cache.keys[:, [2, 0, 1]], held)
+
+
+def test_batches_find_what_their_sequences_share():
+    cache = small(pages=20)
+    parent = cache.open(50)
+    kids = cache.fork(parent, 3)
+    other = cache.open(33)
+    assert cache.batch(kids).prefix == 48 and cache.batch([parent]).prefix == 0
+    assert cache.batch([*kids, other]).prefix == 0
+    cache.truncate(kids[1], 40)
+    assert cache.batch(kids).prefix == 32
+    batch = cache.batch([kids[0], kids[2]], tokens=[3, 1])
+    assert batch.token_map.tolist() == [[kids[0], 0], [kids[0], 1], [kids[0], 2], [kids[2], 0]]
+    assert batch.tiles(50).tolist() == [[0, 128], [128, 150], [150, 200]]
+
+
+def test_full_pools_and_tables_leave_everything_as_it_was():
+    cache = small(pages=4, sequences=3, rows=64)
+    a = cache.open(40)
+    state = lambda: (cache.tables.clone(), cache.lengths.clone(), cache.free_pages)  # noqa: E731
+    before = state()
+    for call, text in ((lambda: cache.open(40), "2 more|3 more pages"), (lambda: cache.open(65), "at most 64"),
+                       (lambda: cache.reserve(a, 65), "at most 64"), (lambda: cache.fork(a, 2), "2 more pages"),
+                       (lambda: cache.fork(a, 3), "3 more sequences"), (lambda: cache.fork(a, 1, share=False), "pages"),
+                       (lambda: cache.ready(cache.batch([a], tokens=30)), "at most 64")):
+        with pytest.raises(ValueError, match=text):
+            call()
+        after = state()
+        assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1]) and before[2] == after[2]
+
+
+def test_refusals():
+    cache = small()
+    a, b = cache.open(20), cache.open(20)
+    for call in (lambda: cache.open(-1), lambda: cache.free([a, a]), lambda: cache.free(5), lambda: cache.fork(5),
+                 lambda: cache.fork(a, -1), lambda: cache.truncate(a, 21), lambda: cache.truncate(a, -1),
+                 lambda: cache.batch([]), lambda: cache.batch([a, a]), lambda: cache.batch([a, 5]),
+                 lambda: cache.batch([a, b], tokens=[1]), lambda: cache.batch([a], tokens=0),
+                 lambda: cache.batch([-1]), lambda: cache.rows(-1)):
+        with pytest.raises(ValueError):
+            call()
+    batch = cache.batch([a, b])
+    with pytest.raises(ValueError, match="another cache"):
+        small().advance(batch)
+    with pytest.raises(ValueError, match="more steps"):
+        cache.account(batch, 13)
+    with pytest.raises(ValueError, match="at least once"):
+        cache.prepare_capture(batch, 0)
+    cache.free(b)
+    for call in (lambda: cache.ready(batch), lambda: cache.advance(batch)):
+        with pytest.raises(ValueError, match="freed or truncated"):
+            call()
+    cache.open()
+    with pytest.raises(ValueError, match="freed or truncated"):   # the slot is another sequence now
+        cache.advance(batch)
+
+
+@pytest.mark.parametrize("change", [
+    dict(tables=np.full((2, 2), -1)), dict(tables=np.zeros((2, 2), int), lengths=np.zeros(2, int)), dict(sequences=2),
+    dict(tables=np.array([[5, -1]]), lengths=np.array([1]), opened=[0]),
+    dict(tables=np.array([[-1, 1]]), lengths=np.array([1]), opened=[0]),
+    dict(tables=np.array([[1, 1]]), lengths=np.array([1]), opened=[0]),
+    dict(tables=np.array([[1, -1]]), lengths=np.array([17]), opened=[0]),
+    dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[]),
+    dict(tables=np.array([[1, -2]]), lengths=np.array([3]), opened=[0]), dict(sequences=0, rows=3),
+    dict(sequences=2, rows=16, opened=[0])])
+def test_tables_that_do_not_hold_together_are_refused(change):
+    pool = torch.zeros((1, 4, 2, 16, 8))
+    with pytest.raises(ValueError):
+        PagedKVCache(pool, pool.clone(), **change)
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 24, 8), (1, 4, 2, 512, 8), (1, 4, 2, 16, 12), (4, 2, 16, 8), (1, 0, 2, 16, 8)])
+def test_pools_of_other_shapes_are_refused(shape):
+    pool = torch.zeros(shape)
+    with pytest.raises(ValueError):
+        PagedKVCache(pool, pool.clone(), sequences=2, rows=16)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_any_order_of_calls_keeps_every_sequence(seed):
+    """Rows are numbered as they are written; after each of 120 random calls every open
+    sequence holds the rows that a list a sequence says it holds."""
+    rng = np.random.default_rng(seed)
+    cache = small(pages=int(rng.integers(8, 30)), page_rows=16, sequences=int(rng.integers(2, 9)), rows=100)
+    random_calls(cache, PagedModel(), rng, 120)
+
+
+def test_a_cache_is_taken_up_as_it_was_left():
+    rng = np.random.default_rng(3)
+    cache, model = small(pages=20), PagedModel()
+    random_calls(cache, model, rng, 60)
+    again = PagedKVCache(cache.keys.clone(), cache.values.clone(), tables=cache.tables.numpy(),
+                         lengths=cache.lengths.numpy(), opened=list(model.rows))
+    check_against(again, model)
+    random_calls(again, model, rng, 60)
+
+
+# The Core chain -----------------------------------------------------------------------------
+
+
+def filled(rng, cache):
+    for pool in (cache.keys, cache.values):
+        pool.copy_(torch.from_numpy(rng.standard_normal(tuple(pool.shape)).astype(np.float32)))
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,pairs,norms,sinks,tokens", [
+    (4, 2, 8, 4, True, False, 1), (6, 2, 8, 0, False, True, [3, 1, 5]), (3, 3, 16, 8, True, True, [1, 17, 2])])
+def test_core_chain_against_the_oracle(heads, kv_heads, head_dim, pairs, norms, sinks, tokens):
+    rng = np.random.default_rng(heads)
+    cache = PagedKVCache.empty(2, 24, 16, kv_heads, head_dim, sequences=5, rows=90, dtype=torch.float32)
+    filled(rng, cache)
+    parent = cache.open(37)
+    chosen = [*cache.fork(parent, 2), cache.open(0)] if heads == 6 else cache.fork(parent, 3)
+    batch = cache.batch(chosen, tokens=tokens)
+    raw = [rng.standard_normal((batch.total, n * head_dim)) for n in (heads, kv_heads, kv_heads)]
+    gains = [1 + 0.1 * rng.standard_normal(head_dim) for _ in range(2)] if norms else [None, None]
+    cos, sin = (np.cos(rng.uniform(0, 6, (90, pairs))), np.sin(rng.uniform(0, 6, (90, pairs))))
+    logits = rng.standard_normal(heads) if sinks else None
+    tensor = lambda a: None if a is None else torch.from_numpy(np.asarray(a)).float()  # noqa: E731
+    step = BatchAttentionStep(
+        cache, layer=1, heads=heads, kv_heads=kv_heads, head_dim=head_dim, scale=0.3, dtype=torch.float32,
+        query_weight=tensor(gains[0]), key_weight=tensor(gains[1]), eps=1e-6, rotary_pairs=pairs, mscale=1.25,
+        angles=AngleTable(tensor(cos), tensor(sin)) if pairs else None, sinks=tensor(logits))
+    assert isinstance(step.strategy, DefaultBatchAttentionStep)
+    untouched = cache.keys[0].clone()
+    context = step(batch, *(tensor(a) for a in raw))
+    assert torch.equal(cache.keys[0], untouched)
+    token_map, lengths = batch.token_map.numpy(), cache.lengths.numpy()
+    f32 = np.float32(1) * 2.0 ** -18   # a few dozen operations of half a step of 2^-24 each
+    queries = np.zeros((batch.total, heads, head_dim))
+    for t, (s, j) in enumerate(token_map):
+        p = lengths[s] + j
+        angles = (cos[p].astype(np.float32), sin[p].astype(np.float32)) if pairs else (None, None)
+        f = lambda a: None if a is None else np.asarray(a, dtype=np.float32)  # noqa: E731
+        queries[t] = turned(f(raw[0][t]).reshape(heads, -1), f(gains[0]), *angles, 1e-6, 1.25)
+        key = turned(f(raw[1][t]).reshape(kv_heads, -1), f(gains[1]), *angles, 1e-6, 1.25)
+        page = cache.tables[s, p // 16]
+        assert np.abs(cache.keys[1, page, :, p % 16].numpy() - key).max() <= f32 * (1 + np.abs(key).max())
+        assert np.array_equal(cache.values[1, page, :, p % 16].numpy(), f(raw[2][t]).reshape(kv_heads, -1))
+    want, size = attend(queries, cache.keys[1].numpy(), cache.values[1].numpy(), cache.tables.numpy(), lengths,
+                        token_map, 0.3, f(logits) if sinks else None)
+    assert np.all(np.abs(context.numpy() - want) <= 2.0 ** -14 * (size + 1e-3))
+
+
+def test_core_chain_keeps_a_later_tokens_infinity_from_an_earlier_one():
+    cache = PagedKVCache.empty(1, 4, 16, 1, 8, sequences=1, rows=40, dtype=torch.float32)
+    cache.open(5)
+    batch = cache.batch([0], tokens=3)
+    step = BatchAttentionStep(cache, layer=0, heads=1, kv_heads=1, head_dim=8, scale=1.0, dtype=torch.float32)
+    v = torch.ones(3, 8)
+    v[2, 3] = float("inf")
+    out = step(batch, torch.ones(3, 8), torch.ones(3, 8), v)
+    assert torch.isfinite(out[:2]).all() and torch.isinf(out[2, 0, 3]) and torch.isfinite(out[2, 0, :3]).all()
+
+
+def test_step_declarations():
+    cache = small(head_dim=64)
+    kind = dict(scale=1.0, dtype=torch.bfloat16)
+    for bad in (dict(layer=2, heads=4, kv_heads=2, head_dim=64), dict(layer=0, heads=5, kv_heads=2, head_dim=64),
+                dict(layer=0, heads=4, kv_heads=4, head_dim=64), dict(layer=0, heads=4, kv_heads=2, head_dim=128),
+                dict(layer=0, heads=4, kv_heads=2, head_dim=64, rotary_pairs=32)):
+        with pytest.raises(ValueError):
+            BatchAttentionStep(cache, **bad, **kind)
+    step = BatchAttentionStep(cache, layer=0, heads=4, kv_heads=2, head_dim=64, rotary_pairs=32, base=1e4, **kind)
+    assert isinstance(step.strategy, DefaultBatchAttentionStep) and isinstance(step.strategy.angles, AngleAtlas)
+    cache.open(3)
+    batch = cache.batch([0])
+    good = [torch.zeros(1, 256), torch.zeros(1, 128), torch.zeros(1, 128)]
+    assert step(batch, *good).shape == (1, 4, 64)
+    for i in range(3):
+        bad = list(good)
+        bad[i] = torch.zeros(2, bad[i].shape[1])
+        with pytest.raises(ValueError, match="tokens"):
+            step(batch, *bad)
+    with pytest.raises(ValueError, match="captured"):
+        step.prepare_capture(batch, 3)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,pairs,served", [
+    (32, 8, 128, 64, True), (64, 8, 64, 32, True), (5, 5, 128, 0, True), (10, 2, 64, 8, True), (32, 8, 96, 32, False),
+    (32, 8, 128, 60, False), (32, 8, 64, 40, False), (32, 5, 64, 32, False), (8192, 8, 64, 32, False)])
+def test_what_the_kernels_serve(heads, kv_heads, head_dim, pairs, served):
+    assert batch_step_applies(heads, kv_heads, head_dim, pairs) == served
+
+
+# What the library refuses, before it looks for a device ---------------------------------------
+
+
+def test_workspace_bytes():
+    from mlx_omnia_amd.runtime import library
+    nbytes = library().omnia_attention_batch_workspace_bytes
+    assert nbytes(0, 32, 8, 128, 0, 1, 0) == 0
+    assert nbytes(64, 32, 8, 128, 8192, 700, 64) % (64 * 32 * 130 * 4) == 0
+    for bad in ((1, 32, 8, 96, 0, 1, 1), (1, 32, 5, 128, 0, 1, 1), (1, 32, 8, 128, -1, 1, 1),
+                (1, 32, 8, 128, 0, 1 << 30, 1), (1 << 28, 32, 8, 128, 0, 1, 1), (1, 8192, 8, 128, 0, 1, 1)):
+        assert nbytes(*bad) < 0
+
+
+def _copy(moves, *, layers=1, pages=8, heads=2, rows=16, dim=64, tables=None, entries=0):
+    from mlx_omnia_amd.runtime import library, loader
+    flat = ops._int_lines(moves, 3, "moves")
+    rc = library().omnia_pages_copy(4096, 8192, layers, pages, heads, rows, dim, flat, len(moves), tables, entries, None)
+    return rc, loader.last_error()
+
+
+@pytest.mark.parametrize("moves,text,more", [
+    ([(0, 8, 1)], "no such page", {}), ([(-1, 2, 1)], "no such page", {}), ([(1 << 30, 2, 1)], "no such page", {}),
+    ([(0, 1, 0)], "rows outside", {}), ([(0, 1, 17)], "rows outside", {}), ([(0, 1, 4), (2, 1, 4)], "two moves", {}),
+    ([(0, 1, 4), (1, 2, 4)], "both read", {}), ([(3, 3, 4)], "both read", {}),
+    ([(4, 0, 4), (3, 1, 4)], "sorted", dict(tables=4096, entries=4)), ([(0, 1, 1)], "bad page", dict(dim=60)),
+    ([(0, 1, 1)], "bad pool", dict(layers=0)), ([(0, 1, 1)] * 257, "more moves", {})])
+def test_pages_copy_refuses(moves, text, more):
+    rc, message = _copy(moves, **more)
+    assert rc == -22 and text in message
+
+
+@pytest.mark.parametrize("edits,text", [
+    ([(0, 4, 0, 0, 0)], "no such sequence"), ([(0, -1, 0, 0, 0)], "no such sequence"),
+    ([(0, 0, 6, 0, 0)], "no such entry"), ([(0, 0, 0, 9, 0)], "no such entry"), ([(0, 0, 0, -2, 0)], "no such entry"),
+    ([(1, 0, -1, 0, 0)], "below zero"), ([(2, 0, 4, 1, 1)], "to fork"), ([(2, 1, 1, 1, 1)], "to fork"),
+    ([(2, 0, 1, 7, 1)], "no such entry"), ([(2, 0, 1, 2, 9)], "no such entry"), ([(4, 0, 0, 0, -1)], "no such edit"),
+    ([(3, 0, 0, 2, -1)], "no such edit"), ([(0, 0, 1, 1, 0), (0, 0, 1, 2, 0)], "two edits"),
+    ([(2, 0, 1, 2, -1), (0, 1, 0, 3, 0)], "two edits"), ([(3, 1, 0, 0, -1), (1, 1, 2, 0, 0)], "two edits"),
+    ([(3, 1, 0, 0, -1), (2, 0, 1, 2, -1)], "two edits")])
+def test_pages_edit_refuses(edits, text):
+    from mlx_omnia_amd.runtime import library, loader
+    flat = ops._int_lines(edits, 5, "edits")
+    assert library().omnia_pages_edit(4096, 8192, 4, 6, 9, flat, len(edits), None) == -22
+    assert text in loader.last_error()
