@@ -38,6 +38,10 @@ struct PageTables {
     const int id = tables[static_cast<int64_t>(sequence) * width + index];
     return id < pages ? id : -1;
   }
+  // A kv head's row of a page, counted in rows of the pool.
+  __device__ __forceinline__ int64_t row_of(int page, int kv_heads, int kv_head, int row) const {
+    return ((static_cast<int64_t>(page) * kv_heads + kv_head) << page_shift) + (row & ((1 << page_shift) - 1));
+  }
 };
 
 // ---- prologue -------------------------------------------------------------------------
@@ -116,10 +120,30 @@ __global__ __launch_bounds__(256) void attention_batch_project_kernel(BatchProje
   }
   const int page = position < 0 ? -1 : a.at.page(whose.x, position);
   if (page < 0) return;
-  const int row = position & ((1 << a.at.page_shift) - 1);
-  const int64_t to = ((static_cast<int64_t>(page) * a.kv_heads + head) << a.at.page_shift) + row;
-  *reinterpret_cast<u32x4*>(a.pool[part - 1] + to * D + lane * 8) = v;
+  *reinterpret_cast<u32x4*>(a.pool[part - 1] + a.at.row_of(page, a.kv_heads, head, position) * D + lane * 8) = v;
 }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A head's sink logit in the denominator: its own weight is 1, or 0 where it is -inf (or there
+// is none), or NaN where it is +inf or a NaN. (Its maximum stays finite, so that it compares
+// and cancels.)
+struct SinkTerm {
+  float top, weight;
+  __device__ __forceinline__ SinkTerm(const uint16_t* sinks, int head) {
+    const float logit = sinks != nullptr ? bf16_to_f32(sinks[head]) : -INFINITY;
+    top = logit == -INFINITY ? -INFINITY : fminf(fmaxf(logit * kLog2e, -FLT_MAX), FLT_MAX);
+    weight = __builtin_amdgcn_exp2f(logit - fmaxf(logit, -FLT_MAX));
+  }
+  // 1 / (total + sink) for a sum over the maximum `base` has; nothing attended gives 0.
+  __device__ __forceinline__ float inverse(float base, float total) const {
+    const float most = fmaxf(base, top);
+    const float shift = most == -INFINITY ? 0.0f : most;
+    const float shrink = __builtin_amdgcn_exp2f(base - shift);
+    const float sum = __builtin_fmaf(total, shrink, weight * __builtin_amdgcn_exp2f(top - shift));
+    return sum == 0.0f ? 0.0f : shrink / sum;
+  }
+};
 
 // ---- attention ------------------------------------------------------------------------
 
@@ -138,294 +162,559 @@ struct BatchArgs {
 };
 
 constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileKeys = 64;
+constexpr int kLdsElements = 4 * 64 * 128;
 
 // A query row is one head of one token: of a kv head, row r is head r % group of token
-// r / group. A workgroup takes 128 of them (32 a wave) and walks its piece's keys in tiles of
-// 64 through two LDS buffers, the next tile's rows in registers while this one is multiplied.
+// r / group. A wave holds 32 of them.
 //
-// Scores are taken transposed, S^T = K Q^T on 32x32x16 MFMA: a lane then holds 32 scores of
-// one row (column lane % 32), so the softmax needs one cross-lane step, its state is a scalar
-// a lane, and P^T is the B operand of O^T = V^T P^T as it stands: the MFMA's k index of lane
-// half h, element j names key 8 (j / 4) + 4 h + j % 4, for both operands. V^T comes out of LDS
-// by the transposing read.
+// Scores are taken transposed, S^T = K Q^T on 32x32x16 MFMA: a lane then holds 16 scores of
+// one row (column lane % 32) for each 32 keys, so the softmax needs one cross-lane step, its
+// state is a scalar a lane, and P^T is the B operand of O^T = V^T P^T as it stands: the MFMA's
+// k index of lane half h, element j names key 8 (j / 4) + 4 h + j % 4, for both operands. V^T
+// comes out of LDS by the transposing read.
 //
-// The weights are rounded to bf16 for that product, half a step of 2^-8 each, once more than
-// the result's own rounding; their sum is taken before it, in fp32. (The weights' errors are
-// independent and average out over the attended rows.)
-//
-// Tiles start at multiples of 64 rows and pages hold 16 or more, so 16 rows from a multiple of
-// 16 lie in one page: its id is looked up once for them.
+// The weights go into that product as two bf16 parts, 16 of their 24 bits: what is cut off is
+// below 2^-15 of a weight, against the 2^-8 of the result's own rounding (one part alone made
+// the results' error 0.0028 of their size where the rounding makes 0.0017).
 template <int D>
-__global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
-  constexpr int kSteps = D / 16, kBlocks = D / 32, kChunks = D / 8;
-  constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread stages, each of K and V
-  constexpr int kTile = kTileKeys * D;                // elements of one tile
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kTile];   // K, V of two stages
-  __shared__ unsigned long long odd_rows[3];   // of a stage: rows whose values are not all finite
+struct WaveRows {
+  static constexpr int kSteps = D / 16, kBlocks = D / 32, kChunks = D / 8;
+  s16x8 q[kSteps];          // Q^T as the B operand: column = row, k = 8 half + j of each 16-wide step
+  f32x16 out[kBlocks];      // O^T: d = 32 b + 8 (e / 4) + 4 half + e % 4 of the column's row
+  float top, total;         // running maximum (the whole row's) and sum (this lane's keys)
+  int key_at, value_at[kBlocks];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int column = lane % 32, half = lane / 32;
+  __device__ __forceinline__ void start(const uint16_t* row, int lane) {
+    const int column = lane % 32, half = lane / 32;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const s16x8*>(row + 8 * half + 16 * s);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) out[b] = f32x16{};
+    top = -INFINITY;
+    total = 0.0f;
+    // Where this lane reads: K row `column`, chunk 2 s + half; V keys 4 half + sub / 4, 4
+    // values from 16 (lane / 16 % 2) + 4 (sub % 4) of each 32-wide block.
+    key_at = column * D + ((half ^ turn_k(column)) * 8);
+    const int sub = lane % 16;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const int r = sub / 4;
+      const int piece = (b * 4 + 2 * (lane / 16 % 2) + (sub % 4) / 2) ^ turn_v(r);
+      value_at[b] = (4 * half + r) * D + piece * 8 + (sub % 2) * 4;
+    }
+  }
+  // Chunks are permuted in LDS so that both operands' reads touch every bank once: K's 16
+  // rows of one chunk, V's four rows of one 64-byte group.
+  static __device__ __forceinline__ int turn_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int turn_v(int row) { return D == 128 ? (row & 3) << 2 : (row & 2) << 1; }
+
+  // One tile of 32 * kKeyBlocks keys from LDS. With `edge`, keys outside [low, high), from
+  // `limit` on (the lane's own) or in a sixteen that `absent` marks do not count.
+  template <int kKeyBlocks>
+  __device__ __forceinline__ void take(const uint16_t* tile_k, const uint16_t* tile_v, float scale_log2, bool edge,
+                                        int key0, int low, int high, int limit, uint32_t absent, int half) {
+    f32x16 s[kKeyBlocks];
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb) s[kb] = f32x16{};
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+#pragma unroll
+      for (int kb = 0; kb < kKeyBlocks; ++kb) {
+        const s16x8 k = *reinterpret_cast<const s16x8*>(tile_k + kb * 32 * D + (key_at ^ (step * 16)));
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
+                                                        __builtin_bit_cast(bf16x8, q[step]), s[kb], 0, 0, 0);
+      }
+    }
+    if (edge) {
+      const int first = max(low - key0, 0), last = min(high, limit) - key0;   // keys of the tile that count
+#pragma unroll
+      for (int e = 0; e < 16 * kKeyBlocks; ++e) {
+        const int in = (e / 16) * 32 + 8 * ((e % 16) / 4) + 4 * half + e % 4;
+        const bool keep = in >= first && in < last && ((absent >> (in / 16)) & 1u) == 0;
+        s[e / 16][e % 16] = keep ? s[e / 16][e % 16] : -INFINITY;
+      }
+    }
+    float best = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 16 * kKeyBlocks; ++e) best = fmaxf(best, s[e / 16][e % 16]);
+    uint32_t lower, upper;
+    half_pair(__float_as_uint(best), lower, upper);
+    best = fmaxf(__uint_as_float(lower), __uint_as_float(upper)) * scale_log2;
+    const float next = fmaxf(top, best);
+    const float base = next == -INFINITY ? 0.0f : next;
+    if (__ballot(next > top) != 0) {
+      const float shrink = __builtin_amdgcn_exp2f(top - base);
+      total *= shrink;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
+      top = next;
+    }
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int step = 0; step < 2 * kKeyBlocks; ++step) {   // 16 keys each
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][(step % 2) * 8 + j], scale_log2, -base));
+        sums[j % 4] += p[j];
+      }
+      u32x4 weights[2];
+      split_weights(p, weights);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
+        const uint16_t* at = tile_v + step * 16 * D + value_at[b];
+        const s16x4_lds v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
+        const s16x4_lds v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * D));
+        const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
+                                                           __builtin_bit_cast(bf16x8, weights[part]), out[b], 0, 0, 0);
+        }
+      }
+    }
+    total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+
+  // The values that were taken out of keys [low, end), for a row that sees those keys: they
+  // have positive weights, so an infinity stays one and a NaN a NaN, whatever the weights are.
+  template <typename ValueRow>
+  __device__ __forceinline__ void put_odd(int low, int end, int half, const ValueRow& value_row) {
+    for (int key = low; key < end; ++key) {
+      const uint16_t* value = value_row(key);
+      if (value == nullptr) continue;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float v = bf16_to_f32(value[b * 32 + 8 * (e / 4) + 4 * half + e % 4]);
+          out[b][e] += fabsf(v) <= FLT_MAX ? 0.0f : v;
+        }
+      }
+    }
+  }
+
+  // The row's sum, from both halves' keys.
+  __device__ __forceinline__ float whole_total() const {
+    uint32_t lower, upper;
+    half_pair(__float_as_uint(total), lower, upper);
+    return __uint_as_float(lower) + __uint_as_float(upper);
+  }
+};
+
+// Takes the values that are not finite out of eight; whether there were any.
+__device__ __forceinline__ bool take_out_odd(u32x4& v) {
+  bool found = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t word = v[j];
+    const bool lo = (word & 0x7f80u) == 0x7f80u, hi = (word & 0x7f800000u) == 0x7f800000u;
+    v[j] = word & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+    found = found || lo || hi;
+  }
+  return found;
+}
+
+// The pages of a sequence as a wave walks its rows upwards. Tiles start at multiples of 16
+// rows and pages hold 16 or more, so 16 rows from a multiple of 16 lie in one page; lane l
+// holds the page of the l-th sixteen of 1,024 rows, and the ones of the next 1,024 are on
+// their way before they are asked for.
+struct PageWalk {
+  const PageTables& at;
+  int sequence, window, now, next;
+
+  __device__ __forceinline__ int fetch(int w) const {
+    const int row = w * 1024 + static_cast<int>(threadIdx.x) % kWave * 16;
+    return row < 0 ? -1 : at.page(sequence, row);
+  }
+  __device__ __forceinline__ PageWalk(const PageTables& tables, int s, int row) : at(tables), sequence(s) {
+    window = row / 1024;
+    now = fetch(window);
+    next = fetch(window + 1);
+  }
+  // Before rows of `row`'s window are asked for (no further than the next one's).
+  __device__ __forceinline__ void reach(int row) {
+    if (row / 1024 == window) return;
+    window = row / 1024;
+    now = next;
+    next = fetch(window + 1);
+  }
+  // The page of the sixteen at `row` (the same in every lane), below 0 for none.
+  __device__ __forceinline__ int page(int row) const { return __builtin_amdgcn_readlane(now, row / 16 % 64); }
+};
+
+// What a workgroup does: which rows of which kv head with which keys of whose pages.
+struct Piece {
+  bool shared, mixed;       // mixed: rows that see different keys
+  int first_row, end_row, kv_head, split, low, high, sequence;
+};
+
+__device__ __forceinline__ bool find_piece(const BatchArgs& a, Piece& p) {
   const int rows = a.tokens * a.group;
-
-  // Which piece: the shared rows' first, for a kv head and a split the row tiles side by side.
-  const int prefix_blocks = a.kv_heads * a.prefix_splits * a.prefix_tiles;
-  int block = xcd_contiguous_block(blockIdx.x, gridDim.x);
-  const bool shared = block < prefix_blocks;
-  int first_row, end_row, split, kv_head;
-  if (shared) {
-    first_row = block % a.prefix_tiles * kTileRows;
-    end_row = min(first_row + kTileRows, rows);
-    block /= a.prefix_tiles;
-    split = block % a.prefix_splits;
-    kv_head = block / a.prefix_splits;
+  const int pairs = a.kv_heads * a.prefix_splits;
+  const int prefix_blocks = pairs * a.prefix_tiles;
+  int block = blockIdx.x;
+  p.shared = block < prefix_blocks;
+  if (p.shared) {
+    // The row tiles that read the same keys go to one XCD, one after another.
+    int pair;
+    if (pairs % kXcds == 0) {
+      const int turn = block / kXcds;
+      pair = block % kXcds + turn / a.prefix_tiles * kXcds;
+      p.first_row = turn % a.prefix_tiles * kTileRows;
+    } else {
+      pair = block % pairs;
+      p.first_row = block / pairs * kTileRows;
+    }
+    p.end_row = min(p.first_row + kTileRows, rows);
+    p.kv_head = pair % a.kv_heads;
+    p.split = pair / a.kv_heads;
+    p.low = p.split * a.prefix_keys;
+    p.high = min(p.low + a.prefix_keys, a.prefix);
+    p.sequence = a.at.tokens[0].x;
+    p.mixed = false;
   } else {
     block -= prefix_blocks;
-    split = block % a.own_splits;
-    block /= a.own_splits;
-    kv_head = block % a.kv_heads;
-    const int2 tile = a.tiles[block / a.kv_heads];
-    first_row = min(max(tile.x, 0), rows - 1);
-    end_row = min(min(max(tile.y, first_row + 1), rows), first_row + kTileRows);
-  }
-  // This lane's row, and the rows it may see; a workgroup's keys end where the last one's do.
-  const int row = min(first_row + wave * kWaveRows + column, end_row - 1);
-  const bool live = first_row + wave * kWaveRows + column < end_row;
-  const int token = row / a.group, head = kv_head * a.group + row % a.group;
-  const int2 whose = a.at.tokens[token];
-  const int limit = min(a.at.before(whose) + 1, shared ? a.prefix : INT32_MAX);
-  const int low = shared ? split * a.prefix_keys : a.prefix + split * a.own_keys;
-  int high;   // past the last key of any row
-  bool mixed; // rows that see different keys
-  int sequence;
-  {
-    const int2 first = a.at.tokens[first_row / a.group], last = a.at.tokens[(end_row - 1) / a.group];
-    sequence = first.x;
-    if (shared) {
-      high = min(low + a.prefix_keys, a.prefix);
-      mixed = false;
-    } else {
-      high = min(low + a.own_keys, a.at.before(last) + 1);
-      mixed = last.y != first.y;
+    p.kv_head = block % a.kv_heads;
+    block /= a.kv_heads;
+    p.split = block / a.own_tiles;
+    const int2 tile = a.tiles[block % a.own_tiles];
+    p.first_row = min(max(tile.x, 0), rows - 1);
+    p.end_row = min(min(max(tile.y, p.first_row + 1), rows), p.first_row + kTileRows);
+    const int2 first = a.at.tokens[p.first_row / a.group], last = a.at.tokens[(p.end_row - 1) / a.group];
+    p.low = a.prefix + p.split * a.own_keys;
+    p.high = min(p.low + a.own_keys, a.at.before(last) + 1);
+    p.sequence = first.x;
+    p.mixed = last.y != first.y;
+    if (p.low >= p.high) {
+      // No row of the tile reaches this split, nor is it merged; where it is the only one, its
+      // rows come as zeros.
+      if (a.prefix_splits + a.own_splits > 1) return false;
+      p.high = p.low;
     }
-    sequence = shared ? a.at.tokens[0].x : sequence;
-    if (sequence < 0 || sequence >= a.at.sequences) high = low;
   }
+  if (p.sequence < 0 || p.sequence >= a.at.sequences) p.high = p.low;
+  return true;
+}
+
+// The values of a sequence's row, or null for a row on no page.
+template <int D>
+__device__ __forceinline__ auto value_row(const BatchArgs& a, const Piece& p) {
+  return [&a, &p](int key) -> const uint16_t* {
+    const int page = a.at.page(p.sequence, key);
+    return page < 0 ? nullptr : a.values + a.at.row_of(page, a.kv_heads, p.kv_head, key) * D;
+  };
+}
+
+// What a piece leaves of row `at` (of token, head and split) for the merge.
+template <int D>
+__device__ __forceinline__ void store_part(const BatchArgs& a, int64_t at, int d, const f32x4& v) {
+  *reinterpret_cast<f32x4*>(a.partial + at * D + d) = v;
+}
+template <int D>
+__device__ __forceinline__ void store_state(const BatchArgs& a, int64_t at, float top, float total) {
+  const int64_t splits = a.prefix_splits + a.own_splits;
+  *reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(a.tokens) * a.heads * splits * D + 2 * at) =
+      float2{top, total};
+}
+
+// Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS
+// buffers, the next tile's rows in registers while this one is multiplied.
+template <int D>
+__device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t* lds, int* odd) {
+  using Rows = WaveRows<D>;
+  constexpr int kChunks = D / 8;
+  constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread stages, each of K and V
+  constexpr int kTile = kTileKeys * D;                // elements of one tile
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int column = lane % 32, half = lane / 32;
+  const int row = min(p.first_row + wave * kWaveRows + column, p.end_row - 1);
+  const bool live = p.first_row + wave * kWaveRows + column < p.end_row;
+  const bool working = p.first_row + wave * kWaveRows < p.end_row;   // the wave
+  const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
+  const int limit = a.at.before(a.at.tokens[token]) + 1;
+  const uint16_t* query = a.q + (static_cast<int64_t>(token) * a.heads + head) * D;
   // Rows that stop before the shared ones end are not expected of a plan, but served.
-  if (shared && __syncthreads_or(limit < high)) mixed = true;
-  if (!shared && low >= high) return;   // no row of the tile reaches this split, nor is it merged
+  if (p.shared && __syncthreads_or(limit < p.high)) p.mixed = true;
 
-  // Q^T as the B operand: column = row, k = 8 half + j of each 16-wide step.
-  s16x8 q[kSteps];
-  {
-    const uint16_t* from = a.q + (static_cast<int64_t>(token) * a.heads + head) * D + 8 * half;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const s16x8*>(from + 16 * s);
-  }
+  PageWalk walk(a.at, p.sequence, p.low);
+  Rows rows;
+  rows.start(query, lane);
 
-  // Staging: thread t's vector i is row (t + 256 i) / kChunks, chunk t % kChunks of the tile.
-  // Chunks are permuted in LDS so that both operands' reads touch every bank once: K's 16
-  // rows of one chunk, V's four rows of one 64-byte group. A row outside [low, high), or of no
-  // page, comes as zeros (a zero weight times what the page happens to hold could be a NaN).
+  // Staging: thread t's vector i is row (t + 256 i) / kChunks, chunk t % kChunks of the tile: of
+  // one sixteen for the whole wave. A row outside [low, high), or of no page, comes as zeros (a
+  // zero weight times what the page happens to hold could be a NaN).
   const int chunk = threadIdx.x % kChunks;
+  const int stage_row = threadIdx.x / kChunks;   // of vector 0
   u32x4 stage_k[kLoads], stage_v[kLoads];
+  bool whole;            // of the tile that is staged: every row there
+  uint32_t absent;       // its sixteens without a page
   auto load_tile = [&](int tile) {
+    const int key0 = tile * kTileKeys;
+    walk.reach(key0);
+    absent = 0;
+    int64_t first[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int page = walk.page(key0 + 16 * i);
+      absent |= page < 0 ? 1u << i : 0u;
+      first[i] = a.at.row_of(max(page, 0), a.kv_heads, p.kv_head, key0 + 16 * i) * D;
+    }
+    whole = absent == 0 && key0 >= p.low && key0 + kTileKeys <= p.high;
+    const uint32_t offset = (stage_row % 16) * D + chunk * 8;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int key = tile * kTileKeys + (static_cast<int>(threadIdx.x) + 256 * i) / kChunks;
-      const int sixteen = __builtin_amdgcn_readfirstlane(key & ~15);   // of the whole wave
-      const int page = sixteen < high ? a.at.page(sequence, sixteen) : -1;
-      const int64_t first = ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kv_head) << a.at.page_shift) +
-                            (sixteen & ((1 << a.at.page_shift) - 1));
-      const int64_t at = (first + (key & 15)) * D + chunk * 8;
-      stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
-      if (page >= 0 && key >= low && key < high) {
-        stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + at);
-        stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + at);
+      // D = 128: vector i is in sixteen i; D = 64: in sixteen 2 i or, the upper waves, 2 i + 1.
+      int64_t base;
+      int key;
+      bool there;
+      if constexpr (D == 128) {
+        base = first[i];
+        key = key0 + 16 * i + stage_row;
+        there = ((absent >> i) & 1u) == 0;
+      } else {
+        const bool upper = wave >= 2;
+        base = upper ? first[2 * i + 1] : first[2 * i];
+        key = key0 + 32 * i + stage_row;
+        there = ((absent >> (2 * i + (upper ? 1 : 0))) & 1u) == 0;
+      }
+      if (whole) {
+        stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
+        stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+      } else {
+        stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
+        if (there && key >= p.low && key < p.high) {
+          stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
+          stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+        }
       }
     }
   };
-  // Where rows see different keys, a value that is not finite is taken out and its row marked:
-  // a row that does not see it would have zero times it, a NaN.
-  auto store_tile = [&](int stage, int mark) {
+  // Where rows see different keys, a value that is not finite is taken out, and put to the rows
+  // that see it at the end: one that does not would have zero times it, a NaN.
+  auto store_tile = [&](int stage) {
     uint16_t* tile_k = lds + stage * 2 * kTile;
     uint16_t* tile_v = tile_k + kTile;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int at = (static_cast<int>(threadIdx.x) + 256 * i) / kChunks;
-      const int turn_k = D == 128 ? at & 15 : (at >> 1) & 7;
-      const int turn_v = D == 128 ? (at & 3) << 2 : (at & 2) << 1;
-      if (mixed) {
-        bool found = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t word = stage_v[i][j];
-          const bool lo = (word & 0x7f80u) == 0x7f80u, hi = (word & 0x7f800000u) == 0x7f800000u;
-          stage_v[i][j] = word & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
-          found = found || lo || hi;
-        }
-        if (found) atomicOr(&odd_rows[mark], 1ull << at);
-      }
-      *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ turn_k) * 8) = stage_k[i];
-      *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ turn_v) * 8) = stage_v[i];
+      const int at = stage_row + 256 / kChunks * i;
+      if (p.mixed && take_out_odd(stage_v[i])) *odd = 1;
+      *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ Rows::turn_k(at)) * 8) = stage_k[i];
+      *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ Rows::turn_v(at)) * 8) = stage_v[i];
     }
   };
 
-  // Where this lane reads: K row `column`, chunk 2 s + half; V keys 4 half + sub / 4, 4
-  // values from 16 (lane / 16 % 2) + 4 (sub % 4) of each 32-wide block.
-  const int turn_k = D == 128 ? column & 15 : (column >> 1) & 7;
-  const int key_at = column * D + ((half ^ turn_k) * 8);
-  const int sub = lane % 16;
-  int value_at[kBlocks];
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b) {
-    const int r = sub / 4;
-    const int turn = D == 128 ? r << 2 : (r & 2) << 1;
-    const int piece = (b * 4 + 2 * (lane / 16 % 2) + (sub % 4) / 2) ^ turn;
-    value_at[b] = (4 * half + r) * D + piece * 8 + (sub % 2) * 4;
-  }
-
-  f32x16 out[kBlocks];
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b) out[b] = f32x16{};
-  float top = -INFINITY, total = 0.0f;
-
-  const int tiles = (high + kTileKeys - 1) / kTileKeys;   // past the last
-  int tile = low / kTileKeys;
-  if (threadIdx.x < 3) odd_rows[threadIdx.x] = 0;
+  const int tiles = (p.high + kTileKeys - 1) / kTileKeys;   // past the last
+  int tile = p.low / kTileKeys;
+  if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
   if (tile < tiles) {
     load_tile(tile);
-    store_tile(0, 0);
+    store_tile(0);
   }
   lds_barrier();
-  int mark = 0;
   for (int turn = 0; tile < tiles; turn ^= 1, ++tile) {
+    const bool edge = p.mixed || !whole;
+    const uint32_t holes = absent;
     const bool more = tile + 1 < tiles;
     if (more) load_tile(tile + 1);
-    const int next_mark = mark == 2 ? 0 : mark + 1;
-    // The mark after the next one was last read a tile ago, behind a barrier.
-    if (threadIdx.x == 0) odd_rows[next_mark == 2 ? 0 : next_mark + 1] = 0;
-    const int key0 = tile * kTileKeys;
-    if (first_row + wave * kWaveRows < end_row) {   // the same for the whole wave
+    if (working) {
       const uint16_t* tile_k = lds + turn * 2 * kTile;
-      const uint16_t* tile_v = tile_k + kTile;
-      f32x16 s[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const s16x8 k = *reinterpret_cast<const s16x8*>(tile_k + kb * 32 * D + (key_at ^ (step * 16)));
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
-                                                          __builtin_bit_cast(bf16x8, q[step]), s[kb], 0, 0, 0);
-        }
-      }
-      // Keys that count: of this piece, seen by the row, on a page that is there.
-      uint32_t absent = 0;   // sixteens of the tile without a page
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 16 * i;
-        absent |= key < high && a.at.page(sequence, key) < 0 ? 1u << i : 0u;
-      }
-      if (mixed || key0 < low || key0 + kTileKeys > high || absent != 0) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int in = (e / 16) * 32 + 8 * ((e % 16) / 4) + 4 * half + e % 4;
-          const int key = key0 + in;
-          const bool keep = key >= low && key < high && key < limit && ((absent >> (in / 16)) & 1u) == 0;
-          s[e / 16][e % 16] = keep ? s[e / 16][e % 16] : -INFINITY;
-        }
-      }
-      float best = s[0][0];
-#pragma unroll
-      for (int e = 1; e < 32; ++e) best = fmaxf(best, s[e / 16][e % 16]);
-      uint32_t lower, upper;
-      half_pair(__float_as_uint(best), lower, upper);
-      best = fmaxf(__uint_as_float(lower), __uint_as_float(upper)) * a.scale_log2;
-      const float next = fmaxf(top, best);
-      const float base = next == -INFINITY ? 0.0f : next;
-      if (__ballot(next > top) != 0) {
-        const float shrink = __builtin_amdgcn_exp2f(top - base);
-        total *= shrink;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
-        top = next;
-      }
-      float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {   // 16 keys each
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          p[j] = __builtin_amdgcn_exp2f(
-              __builtin_fmaf(s[step / 2][(step % 2) * 8 + j], a.scale_log2, -base));
-          sums[j % 4] += p[j];
-        }
-        const u32x4 weights = pack8(p);
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
-          const uint16_t* at = tile_v + step * 16 * D + value_at[b];
-          const s16x4_lds v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
-          const s16x4_lds v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * D));
-          const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-          out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
-                                                           __builtin_bit_cast(bf16x8, weights), out[b], 0, 0, 0);
-        }
-      }
-      total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-      // The values that were taken out, for the rows that see them: the weight once more from
-      // its score, times the value as it is.
-      if (mixed) {
-        unsigned long long marked = odd_rows[mark];
-        while (marked != 0) {
-          const int key = key0 + __builtin_ctzll(marked);
-          marked &= marked - 1;
-          if (key >= limit) continue;
-          const int page = a.at.page(sequence, key);   // it was read from there
-          const int64_t at = ((((static_cast<int64_t>(page) * a.kv_heads + kv_head) << a.at.page_shift) +
-                               (key & ((1 << a.at.page_shift) - 1))) * D);
-          const uint16_t* mine = a.q + (static_cast<int64_t>(token) * a.heads + head) * D;
-          float score = 0.0f;
-          for (int d = 0; d < D; ++d) {
-            score = __builtin_fmaf(bf16_to_f32(mine[d]), bf16_to_f32(a.keys[at + d]), score);
-          }
-          const float weight =
-              fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(score, a.scale_log2, -base)), FLT_MIN);
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float v = bf16_to_f32(a.values[at + b * 32 + 8 * (e / 4) + 4 * half + e % 4]);
-              out[b][e] += fabsf(v) <= FLT_MAX ? 0.0f : weight * v;
-            }
-          }
-        }
-      }
+      rows.template take<2>(tile_k, tile_k + kTile, a.scale_log2, edge, tile * kTileKeys, p.low, p.high, limit, holes,
+                            half);
     }
-    if (more) store_tile(turn ^ 1, next_mark);
-    mark = next_mark;
+    if (more) store_tile(turn ^ 1);
     lds_barrier();
   }
+  if (*odd != 0) rows.put_odd(p.low, min(p.high, limit), half, value_row<D>(a, p));
 
-  uint32_t lower, upper;
-  half_pair(__float_as_uint(total), lower, upper);
-  total = __uint_as_float(lower) + __uint_as_float(upper);
+  const float total = rows.whole_total();
   if (!live) return;
-  const int64_t splits = a.prefix_splits + a.own_splits;
-  const int64_t at = (static_cast<int64_t>(token) * a.heads + head) * splits + (shared ? split : a.prefix_splits + split);
-  float* to = a.partial + at * D + 4 * half;
+  const int splits = a.prefix_splits + a.own_splits;
+  const int64_t at = static_cast<int64_t>(token) * a.heads + head;
+  if (splits > 1) {
+    const int64_t part = at * splits + (p.shared ? p.split : a.prefix_splits + p.split);
 #pragma unroll
-  for (int b = 0; b < kBlocks; ++b) {
+    for (int b = 0; b < Rows::kBlocks; ++b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        store_part<D>(a, part, b * 32 + 8 * i + 4 * half,
+                      f32x4{rows.out[b][4 * i], rows.out[b][4 * i + 1], rows.out[b][4 * i + 2], rows.out[b][4 * i + 3]});
+      }
+    }
+    if (half == 0) store_state<D>(a, part, rows.top, total);
+    return;
+  }
+  const SinkTerm sink(a.sinks, head);
+  const float inverse = sink.inverse(rows.top, total);
+#pragma unroll
+  for (int b = 0; b < Rows::kBlocks; ++b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<f32x4*>(to + b * 32 + 8 * i) =
-          f32x4{out[b][4 * i], out[b][4 * i + 1], out[b][4 * i + 2], out[b][4 * i + 3]};
+      uint2 packed;
+      packed.x = pack_bf16(rows.out[b][4 * i] * inverse, rows.out[b][4 * i + 1] * inverse);
+      packed.y = pack_bf16(rows.out[b][4 * i + 2] * inverse, rows.out[b][4 * i + 3] * inverse);
+      *reinterpret_cast<uint2*>(a.out + at * D + b * 32 + 8 * i + 4 * half) = packed;
     }
   }
-  if (half == 0) {
-    float* state = a.partial + static_cast<int64_t>(a.tokens) * a.heads * splits * D + 2 * at;
-    state[0] = top;
-    state[1] = total;
+}
+
+// Up to 32 rows: the four waves hold the same rows and take every fourth tile of keys each,
+// through an LDS buffer of their own without a barrier, and merge at the end.
+template <int D>
+__device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16_t* lds) {
+  using Rows = WaveRows<D>;
+  constexpr int kKeyBlocks = D == 128 ? 1 : 2, kKeys = 32 * kKeyBlocks;
+  constexpr int kChunks = D / 8, kRowsALoad = kWave / kChunks;   // 4 or 8
+  constexpr int kLoads = kKeys / kRowsALoad;                     // 8: 16-byte vectors a lane stages, each of K and V
+  constexpr int kTile = kKeys * D;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int column = lane % 32, half = lane / 32;
+  const int row = min(p.first_row + column, p.end_row - 1);
+  const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
+  const int limit = a.at.before(a.at.tokens[token]) + 1;
+  const uint16_t* query = a.q + (static_cast<int64_t>(token) * a.heads + head) * D;
+  if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
+
+  const int tiles = (p.high + kKeys - 1) / kKeys;   // past the last
+  int tile = p.low / kKeys + wave;
+  PageWalk walk(a.at, p.sequence, tile * kKeys);
+  Rows rows;
+  rows.start(query, lane);
+  uint16_t* tile_k = lds + wave * 2 * kTile;
+  uint16_t* tile_v = tile_k + kTile;
+  const int chunk = lane % kChunks, stage_row = lane / kChunks;
+  u32x4 stage_k[kLoads], stage_v[kLoads];
+  bool whole;
+  uint32_t absent;
+  auto load_tile = [&](int t) {
+    const int key0 = t * kKeys;
+    walk.reach(key0);
+    absent = 0;
+    int64_t first[kKeys / 16];
+#pragma unroll
+    for (int i = 0; i < kKeys / 16; ++i) {
+      const int page = walk.page(key0 + 16 * i);
+      absent |= page < 0 ? 1u << i : 0u;
+      first[i] = a.at.row_of(max(page, 0), a.kv_heads, p.kv_head, key0 + 16 * i) * D;
+    }
+    whole = absent == 0 && key0 >= p.low && key0 + kKeys <= p.high;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int in = i * kRowsALoad;   // of the tile, the load's first row
+      const int64_t base = first[in / 16] + (in % 16) * D;
+      const uint32_t offset = stage_row * D + chunk * 8;
+      if (whole) {
+        stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
+        stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+      } else {
+        const int key = key0 + in + stage_row;
+        stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
+        if (((absent >> (in / 16)) & 1u) == 0 && key >= p.low && key < p.high) {
+          stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
+          stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+        }
+      }
+    }
+  };
+
+  bool odd = false;   // a value of this wave's keys was taken out, by this lane
+  if (tile < tiles) load_tile(tile);
+  while (tile < tiles) {
+    const int key0 = tile * kKeys;
+    const bool edge = p.mixed || !whole;
+    const uint32_t holes = absent;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * kRowsALoad + stage_row;
+      if (p.mixed) odd = take_out_odd(stage_v[i]) || odd;
+      *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ Rows::turn_k(at)) * 8) = stage_k[i];
+      *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ Rows::turn_v(at)) * 8) = stage_v[i];
+    }
+    const int following = tile + kWaves;
+    if (following < tiles) load_tile(following);
+    // The wave's lanes read what the others stored: LDS takes a wave's operations in order.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    rows.template take<kKeyBlocks>(tile_k, tile_v, a.scale_log2, edge, key0, p.low, p.high, limit, holes, half);
+    tile = following;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  }
+
+  // A wave that took any out puts back its own keys' (every fourth tile's).
+  if (__ballot(odd) != 0) {
+    const auto any = value_row<D>(a, p);
+    rows.put_odd(p.low, min(p.high, limit), half, [&](int key) {
+      return (key / kKeys - p.low / kKeys) % kWaves == wave ? any(key) : nullptr;
+    });
+  }
+
+  // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c], its top
+  // and sum behind the four.
+  const float total = rows.whole_total();
+  const int count = p.end_row - p.first_row;
+  float* parts = reinterpret_cast<float*>(lds);
+  float2* states = reinterpret_cast<float2*>(parts + kWaves * kWaveRows * D);
+  lds_barrier();
+  if (column < count) {
+#pragma unroll
+    for (int b = 0; b < Rows::kBlocks; ++b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<f32x4*>(parts + (wave * kWaveRows + column) * D + b * 32 + 8 * i + 4 * half) =
+            f32x4{rows.out[b][4 * i], rows.out[b][4 * i + 1], rows.out[b][4 * i + 2], rows.out[b][4 * i + 3]};
+      }
+    }
+    if (half == 0) states[wave * kWaveRows + column] = float2{rows.top, total};
+  }
+  lds_barrier();
+  const int splits = a.prefix_splits + a.own_splits;
+  for (int item = threadIdx.x; item < count * (D / 4); item += 256) {
+    const int r = item / (D / 4), d = item % (D / 4) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, states[w * kWaveRows + r].x);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 state = states[w * kWaveRows + r];
+      const float factor = __builtin_amdgcn_exp2f(state.x - base);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(parts + (w * kWaveRows + r) * D + d);
+      sum = __builtin_fmaf(state.y, factor, sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(part[i], factor, v[i]);
+    }
+    const int global = p.first_row + r;
+    const int h = p.kv_head * a.group + global % a.group;
+    const int64_t at = static_cast<int64_t>(global / a.group) * a.heads + h;
+    if (splits > 1) {
+      const int64_t part = at * splits + (p.shared ? p.split : a.prefix_splits + p.split);
+      store_part<D>(a, part, d, v);
+      if (d == 0) store_state<D>(a, part, top, sum);
+    } else {
+      const SinkTerm sink(a.sinks, h);
+      const float inverse = sink.inverse(top, sum);
+      uint2 packed;
+      packed.x = pack_bf16(v[0] * inverse, v[1] * inverse);
+      packed.y = pack_bf16(v[2] * inverse, v[3] * inverse);
+      *reinterpret_cast<uint2*>(a.out + at * D + d) = packed;
+    }
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElements + kWaves * kWaveRows * 4];
+  __shared__ int odd;   // a value was taken out
+  Piece p;
+  if (!find_piece(a, p)) return;
+  if (p.end_row - p.first_row <= kWaveRows) {
+    narrow_piece<D>(a, p, lds);
+  } else {
+    wide_piece<D>(a, p, lds, &odd);
   }
 }
 
@@ -444,17 +733,11 @@ __global__ __launch_bounds__(256) void attention_batch_merge_kernel(BatchArgs a)
   const float2* states =
       reinterpret_cast<const float2*>(a.partial + static_cast<int64_t>(a.tokens) * a.heads * splits * D) + row * splits;
   const float* parts = a.partial + row * splits * D + column;
-  const float sink = a.sinks != nullptr ? bf16_to_f32(a.sinks[row - token * a.heads]) : -INFINITY;
-  constexpr float kLog2e = 1.4426950408889634f;
-  float top = fminf(fmaxf(sink, -FLT_MAX), FLT_MAX) * kLog2e;
-  top = sink == -INFINITY ? -INFINITY : fminf(fmaxf(top, -FLT_MAX), FLT_MAX);
-  // The sink's own weight: 1, or 0 where it is -inf, or NaN where it is +inf or a NaN. (Its
-  // maximum stays finite, so that it compares and cancels.)
-  const float sink_top = top;
-  const float sink_weight = __builtin_amdgcn_exp2f(sink - fmaxf(sink, -FLT_MAX));
+  const SinkTerm sink(a.sinks, static_cast<int>(row - token * a.heads));
+  float top = -INFINITY;
   for (int s = 0; s < count; ++s) top = fmaxf(top, states[s].x);
   const float base = top == -INFINITY ? 0.0f : top;
-  float total = a.sinks != nullptr ? sink_weight * __builtin_amdgcn_exp2f(sink_top - base) : 0.0f;
+  float total = 0.0f;
   f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int s = 0; s < count; ++s) {
@@ -465,7 +748,7 @@ __global__ __launch_bounds__(256) void attention_batch_merge_kernel(BatchArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], factor, sum[i]);
   }
-  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+  const float inverse = sink.inverse(top, total);
   uint2 packed;
   packed.x = pack_bf16(sum[0] * inverse, sum[1] * inverse);
   packed.y = pack_bf16(sum[2] * inverse, sum[3] * inverse);
@@ -473,38 +756,36 @@ __global__ __launch_bounds__(256) void attention_batch_merge_kernel(BatchArgs a)
 }
 
 // How the keys are cut: the shared rows and the sequences' own each into pieces of a multiple
-// of 64 keys, as many as give every CU a workgroup, each of at least four tiles.
+// of 64 keys. A wide piece leaves 128 rows of context for the merge, so there are about two
+// workgroups a CU of them, of at least four tiles; a narrow one leaves a few rows and is short,
+// so that sequences of different lengths fill the card evenly.
 struct Plan {
   int64_t prefix_tiles, prefix_splits, prefix_keys, own_splits, own_keys;
 };
 
-constexpr int kTargetBlocks = 256, kMinSplitTiles = 4, kMaxSplits = 64;
+constexpr int64_t kWideBlocks = 512, kWideKeys = 256, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
 
-int64_t split_count(int64_t blocks, int64_t keys) {
+// Pieces of `keys` keys for each of `blocks` workgroups, and the keys of one.
+int64_t cut(int64_t blocks, int64_t keys, bool narrow, int64_t& each) {
+  each = kTileKeys;
   if (keys <= 0 || blocks <= 0) return 0;
-  const int64_t by_blocks = (kTargetBlocks + blocks - 1) / blocks;
-  const int64_t by_tiles = (keys + kTileKeys - 1) / kTileKeys / kMinSplitTiles;
-  const int64_t splits = by_blocks < by_tiles ? by_blocks : by_tiles;
-  return splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
-}
-
-// Keys of one of `splits` pieces, and as many pieces as that leaves.
-int64_t piece_keys(int64_t keys, int64_t& splits) {
-  if (splits == 0) return kTileKeys;
+  const int64_t target = narrow ? kNarrowBlocks : kWideBlocks, least = narrow ? kNarrowKeys : kWideKeys;
+  int64_t splits = (target + blocks - 1) / blocks;
+  const int64_t by_keys = keys / least;
+  splits = splits < by_keys ? splits : by_keys;
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
-  const int64_t each = (tiles + splits - 1) / splits;
-  splits = (tiles + each - 1) / each;
-  return each * kTileKeys;
+  const int64_t of_one = (tiles + splits - 1) / splits;
+  each = of_one * kTileKeys;
+  return (tiles + of_one - 1) / of_one;
 }
 
 Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t own_rows, int64_t own_tiles) {
   Plan p{};
   const int64_t rows = tokens * (heads / kv_heads);
   p.prefix_tiles = prefix > 0 ? (rows + kTileRows - 1) / kTileRows : 0;
-  p.prefix_splits = split_count(kv_heads * p.prefix_tiles, prefix);
-  p.prefix_keys = piece_keys(prefix, p.prefix_splits);
-  p.own_splits = split_count(kv_heads * own_tiles, own_rows);
-  p.own_keys = piece_keys(own_rows, p.own_splits);
+  p.prefix_splits = cut(kv_heads * p.prefix_tiles, prefix, rows <= kWaveRows, p.prefix_keys);
+  p.own_splits = cut(kv_heads * own_tiles, own_rows, rows <= kWaveRows * own_tiles, p.own_keys);
   return p;
 }
 
@@ -576,7 +857,8 @@ extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t
   using namespace omnia;
   if (!geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles)) return -EINVAL;
   const Plan p = plan_for(tokens, heads, kv_heads, prefix, own_rows, own_tiles);
-  return (p.prefix_splits + p.own_splits) * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  const int64_t splits = p.prefix_splits + p.own_splits;
+  return splits == 1 ? 0 : splits * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t* keys, const uint16_t* values,
@@ -607,7 +889,6 @@ extern "C" int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
   const Plan p = plan_for(tokens, heads, kv_heads, prefix, own_rows, own_tiles);
-  constexpr float kLog2e = 1.4426950408889634f;
   const BatchArgs a{queries, keys, values, reinterpret_cast<const int2*>(tiles), sinks, out,
                     static_cast<float*>(workspace),
                     {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
@@ -623,7 +904,9 @@ extern "C" int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t
     const auto kernel = head_dim == 64 ? attention_batch_kernel<64> : attention_batch_kernel<128>;
     kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
   }
-  const auto merge = head_dim == 64 ? attention_batch_merge_kernel<64> : attention_batch_merge_kernel<128>;
-  merge<<<dim3(static_cast<unsigned>(merges)), 256, 0, stream>>>(a);
+  if (p.prefix_splits + p.own_splits != 1) {
+    const auto merge = head_dim == 64 ? attention_batch_merge_kernel<64> : attention_batch_merge_kernel<128>;
+    merge<<<dim3(static_cast<unsigned>(merges)), 256, 0, stream>>>(a);
+  }
   return launched("attention_batch");
 }
