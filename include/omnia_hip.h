@@ -691,8 +691,8 @@ int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* 
  *   a, b = n_i * mscale, n_{i+P} * mscale                 i < P = rotary_pairs
  *   y_i = a cos[p][i] - b sin[p][i], y_{i+P} = a sin[p][i] + b cos[p][i], y_d = n_d beyond
  * in fp32, rounded once to bf16 (omnia_attention_project rounds in between as well, as the
- * single sequence's chain does). Queries go to queries [tokens, heads, D], keys and values to
- * row p of the sequence's pages, of one layer: keys, values [pages, kv_heads, page_rows, D].
+ * single sequence's chain does). Queries go to queries [tokens, heads, D] (with wide_queries 1
+ * as fp32, not rounded), keys and values to row p of the sequence's pages, of one layer: keys, values [pages, kv_heads, page_rows, D].
  * A token whose sequence, position or page is not there stores no key and no value; a
  * position past the angle rows reads the last of them. raw_queries [tokens, heads * D],
  * raw_keys / raw_values [tokens, kv_heads * D], rows their strides apart; cos_rows, sin_rows
@@ -706,8 +706,8 @@ int32_t omnia_attention_batch_project(
     const uint16_t* query_weight, const uint16_t* key_weight, const float* cos_rows,
     const float* sin_rows, int64_t table_stride, int64_t angle_rows, int64_t rotary_pairs,
     float mscale, float eps, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
-    uint16_t* queries, uint16_t* keys, uint16_t* values, int64_t pages, int64_t page_rows,
-    const int32_t* tables, int64_t sequences, int64_t width, const int32_t* lengths,
+    void* queries, int32_t wide_queries, uint16_t* keys, uint16_t* values, int64_t pages,
+    int64_t page_rows, const int32_t* tables, int64_t sequences, int64_t width, const int32_t* lengths,
     const int32_t* token_map, hipStream_t stream);
 
 /* Workspace bytes omnia_attention_batch needs. -EINVAL for a bad geometry. Pure; touches no
@@ -727,12 +727,13 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  * token's. own_rows bounds the rows past them of every sequence, this step's included; tiles
  * [own_tiles, 2] int32 (device) are runs [first, end) of query rows of one sequence, at most
  * 128 long, that cover every row once (of each kv head, row r is token r / gqa, head r % gqa).
- * A row on no page (-1, or outside the pool) is not seen. queries, out [tokens, heads, D];
+ * A row on no page (-1, or outside the pool) is not seen. queries [tokens, heads, D] bf16, or
+ * fp32 with wide_queries 1; out [tokens, heads, D] bf16;
  * workspace: at least omnia_attention_batch_workspace_bytes, 16-byte aligned.
  * Beside: core/kernels/attention/default.py:132-156 (one sequence's).
  * head_dim 64 or 128; heads a multiple of kv_heads; scale positive and finite. */
-int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t* keys,
-                              const uint16_t* values, int64_t pages, int64_t page_rows,
+int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
+                              const uint16_t* keys, const uint16_t* values, int64_t pages, int64_t page_rows,
                               const int32_t* tables, int64_t sequences, int64_t width,
                               const int32_t* lengths, const int32_t* token_map, int64_t tokens,
                               const int32_t* tiles, int64_t own_tiles, int64_t prefix,

@@ -53,10 +53,10 @@ struct BatchProjectArgs {
   const float* cos;         // [angle_rows, pairs] rows `table_stride` floats apart
   const float* sin;
   int64_t table_stride, angle_rows;
-  uint16_t* queries;        // [tokens, heads, D]
+  void* queries;            // [tokens, heads, D] bf16, or fp32 with `wide`
   uint16_t* pool[2];        // a layer's keys and values [pages, kv_heads, page_rows, D]
   PageTables at;
-  int heads, kv_heads, tokens, pairs;
+  int heads, kv_heads, tokens, pairs, wide;
   float mscale, eps;
 };
 
@@ -76,8 +76,8 @@ __global__ __launch_bounds__(256) void attention_batch_project_kernel(BatchProje
   u32x4 v = *reinterpret_cast<const u32x4*>(a.raw[part] + token * a.stride[part] + head * D + lane * 8);
   const int2 whose = a.at.tokens[token];
   const int position = a.at.before(whose);
+  float x[8];
   if (part < 2) {
-    float x[8];
     unpack8(v, x);
     const uint16_t* gain = a.gain[part];
     if (gain != nullptr) {
@@ -115,7 +115,14 @@ __global__ __launch_bounds__(256) void attention_batch_project_kernel(BatchProje
     v = pack8(x);
   }
   if (part == 0) {
-    *reinterpret_cast<u32x4*>(a.queries + (token * a.heads + head) * D + lane * 8) = v;
+    const int64_t at = (token * a.heads + head) * D + lane * 8;
+    if (a.wide != 0) {
+      float* to = static_cast<float*>(a.queries) + at;
+      *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.queries) + at) = v;
+    }
     return;
   }
   const int page = position < 0 ? -1 : a.at.page(whose.x, position);
@@ -148,7 +155,7 @@ struct SinkTerm {
 // ---- attention ------------------------------------------------------------------------
 
 struct BatchArgs {
-  const uint16_t* q;        // [tokens, heads, D]
+  const void* q;            // [tokens, heads, D] bf16 or fp32
   const uint16_t* keys;     // a layer's [pages, kv_heads, page_rows, D]
   const uint16_t* values;
   const int2* tiles;        // own pieces: query rows [x, y) of one sequence
@@ -161,33 +168,82 @@ struct BatchArgs {
   float scale_log2;
 };
 
-constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileKeys = 64;
+constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileKeys = 64, kNarrowRows = 16;
 constexpr int kLdsElements = 4 * 64 * 128;
 
 // A query row is one head of one token: of a kv head, row r is head r % group of token
-// r / group. A wave holds 32 of them.
+// r / group.
 //
-// Scores are taken transposed, S^T = K Q^T on 32x32x16 MFMA: a lane then holds 16 scores of
-// one row (column lane % 32) for each 32 keys, so the softmax needs one cross-lane step, its
-// state is a scalar a lane, and P^T is the B operand of O^T = V^T P^T as it stands: the MFMA's
-// k index of lane half h, element j names key 8 (j / 4) + 4 h + j % 4, for both operands. V^T
-// comes out of LDS by the transposing read.
+// Scores are taken transposed, S^T = K Q^T on the matrix cores: a lane then holds the scores of
+// one row, its state is a scalar a lane, and P^T is the B operand of O^T = V^T P^T as it stands,
+// with the keys that a lane holds as the product's k index, in that order for both operands.
+// V^T comes out of LDS by the transposing read.
 //
-// The weights go into that product as two bf16 parts, 16 of their 24 bits: what is cut off is
-// below 2^-15 of a weight, against the 2^-8 of the result's own rounding (one part alone made
-// the results' error 0.0028 of their size where the rounding makes 0.0017).
-template <int D>
-struct WaveRows {
-  static constexpr int kSteps = D / 16, kBlocks = D / 32, kChunks = D / 8;
-  s16x8 q[kSteps];          // Q^T as the B operand: column = row, k = 8 half + j of each 16-wide step
+// Queries of 32 bits go into the product as two bf16 parts, 16 of their 24 bits (queries of bf16
+// are one). The weights are rounded to bf16, half a step of 2^-8 each; their sum is taken before
+// that, in fp32. So the results' error is 0.0024 of their size, where rounding them alone makes
+// 0.0017; with the queries rounded as well it was 0.0028. Both parts of the weights instead of
+// the queries' give the same, and cost four vector operations a score more.
+//
+// The maximum that the weights are taken under is raised only where a score passes it by more
+// than 2^8: the sums have the room, and the rescaling of a row's context, which a growing
+// maximum would ask for in nearly every tile, is rare.
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ u32x4 low_part(const float (&x)[8], const u32x4& high) {
+  float h[8], rest[8];
+  unpack8(high, h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = x[i] - h[i];
+  return pack8(rest);
+}
+
+// Eight consecutive values of a query as bf16 operands, in kParts parts.
+template <int kParts>
+__device__ __forceinline__ void load_query(const void* q, int64_t at, s16x8 (&parts)[kParts]) {
+  if constexpr (kParts == 1) {
+    parts[0] = *reinterpret_cast<const s16x8*>(static_cast<const uint16_t*>(q) + at);
+  } else {
+    const float* from = static_cast<const float*>(q) + at;
+    float x[8];
+    *reinterpret_cast<f32x4*>(x) = *reinterpret_cast<const f32x4*>(from);
+    *reinterpret_cast<f32x4*>(x + 4) = *reinterpret_cast<const f32x4*>(from + 4);
+    const u32x4 high = pack8(x);
+    parts[0] = __builtin_bit_cast(s16x8, high);
+    parts[1] = __builtin_bit_cast(s16x8, low_part(x, high));
+  }
+}
+
+__device__ __forceinline__ s16x8 read_transposed(const uint16_t* first, const uint16_t* second) {
+  typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
+  const s16x4_lds v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(first));
+  const s16x4_lds v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(second));
+  return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Raises the maximum where it has to be; the factor for what was summed under the old one.
+__device__ __forceinline__ bool raise(float& top, float best, float& shrink) {
+  if (__ballot(best > top + kSlack || (top == -INFINITY && best > top)) == 0) return false;
+  const float next = fmaxf(top, best);
+  shrink = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
+  top = next;
+  return true;
+}
+
+// 32 rows on 32x32x16 MFMA: row = column lane % 32; of 32 keys lane half h holds the keys
+// 8 i + 4 h + j, i and j below 4.
+template <int D, int kParts>
+struct WideRows {
+  static constexpr int kSteps = D / 16, kBlocks = D / 32;
+  s16x8 q[kSteps][kParts];  // Q^T as the B operand: k = 8 half + j of each 16-wide step
   f32x16 out[kBlocks];      // O^T: d = 32 b + 8 (e / 4) + 4 half + e % 4 of the column's row
-  float top, total;         // running maximum (the whole row's) and sum (this lane's keys)
+  float top, total;         // the maximum (the whole row's) and the sum (this lane's keys)
   int key_at, value_at[kBlocks];
 
-  __device__ __forceinline__ void start(const uint16_t* row, int lane) {
+  __device__ __forceinline__ void start(const void* queries, int64_t row, int lane) {
     const int column = lane % 32, half = lane / 32;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const s16x8*>(row + 8 * half + 16 * s);
+    for (int s = 0; s < kSteps; ++s) load_query<kParts>(queries, row * D + 8 * half + 16 * s, q[s]);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = f32x16{};
     top = -INFINITY;
@@ -208,27 +264,27 @@ struct WaveRows {
   static __device__ __forceinline__ int turn_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
   static __device__ __forceinline__ int turn_v(int row) { return D == 128 ? (row & 3) << 2 : (row & 2) << 1; }
 
-  // One tile of 32 * kKeyBlocks keys from LDS. With `edge`, keys outside [low, high), from
-  // `limit` on (the lane's own) or in a sixteen that `absent` marks do not count.
-  template <int kKeyBlocks>
+  // A tile of 64 keys from LDS. With `edge`, keys outside [first, last) of it or in a sixteen
+  // that `absent` marks do not count.
   __device__ __forceinline__ void take(const uint16_t* tile_k, const uint16_t* tile_v, float scale_log2, bool edge,
-                                        int key0, int low, int high, int limit, uint32_t absent, int half) {
-    f32x16 s[kKeyBlocks];
-#pragma unroll
-    for (int kb = 0; kb < kKeyBlocks; ++kb) s[kb] = f32x16{};
+                                       int first, int last, uint32_t absent, int half) {
+    f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
 #pragma unroll
-      for (int kb = 0; kb < kKeyBlocks; ++kb) {
+      for (int kb = 0; kb < 2; ++kb) {
         const s16x8 k = *reinterpret_cast<const s16x8*>(tile_k + kb * 32 * D + (key_at ^ (step * 16)));
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
-                                                        __builtin_bit_cast(bf16x8, q[step]), s[kb], 0, 0, 0);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
+                                                          __builtin_bit_cast(bf16x8, q[step][part]), s[kb], 0, 0, 0);
+        }
       }
     }
     if (edge) {
-      const int first = max(low - key0, 0), last = min(high, limit) - key0;   // keys of the tile that count
+      asm volatile("");   // a branch: as selects its compares ran in every tile
 #pragma unroll
-      for (int e = 0; e < 16 * kKeyBlocks; ++e) {
+      for (int e = 0; e < 32; ++e) {
         const int in = (e / 16) * 32 + 8 * ((e % 16) / 4) + 4 * half + e % 4;
         const bool keep = in >= first && in < last && ((absent >> (in / 16)) & 1u) == 0;
         s[e / 16][e % 16] = keep ? s[e / 16][e % 16] : -INFINITY;
@@ -236,42 +292,32 @@ struct WaveRows {
     }
     float best = s[0][0];
 #pragma unroll
-    for (int e = 1; e < 16 * kKeyBlocks; ++e) best = fmaxf(best, s[e / 16][e % 16]);
+    for (int e = 1; e < 32; ++e) best = fmaxf(best, s[e / 16][e % 16]);
     uint32_t lower, upper;
     half_pair(__float_as_uint(best), lower, upper);
     best = fmaxf(__uint_as_float(lower), __uint_as_float(upper)) * scale_log2;
-    const float next = fmaxf(top, best);
-    const float base = next == -INFINITY ? 0.0f : next;
-    if (__ballot(next > top) != 0) {
-      const float shrink = __builtin_amdgcn_exp2f(top - base);
+    float shrink;
+    if (raise(top, best, shrink)) {
       total *= shrink;
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
-      top = next;
     }
+    const float base = top == -INFINITY ? 0.0f : top;
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int step = 0; step < 2 * kKeyBlocks; ++step) {   // 16 keys each
+    for (int step = 0; step < 4; ++step) {   // 16 keys each
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][(step % 2) * 8 + j], scale_log2, -base));
         sums[j % 4] += p[j];
       }
-      u32x4 weights[2];
-      split_weights(p, weights);
+      const u32x4 weights = pack8(p);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
         const uint16_t* at = tile_v + step * 16 * D + value_at[b];
-        const s16x4_lds v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
-        const s16x4_lds v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * D));
-        const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v),
-                                                           __builtin_bit_cast(bf16x8, weights[part]), out[b], 0, 0, 0);
-        }
+        out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, read_transposed(at, at + 8 * D)),
+                                                         __builtin_bit_cast(bf16x8, weights), out[b], 0, 0, 0);
       }
     }
     total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
@@ -300,6 +346,114 @@ struct WaveRows {
     uint32_t lower, upper;
     half_pair(__float_as_uint(total), lower, upper);
     return __uint_as_float(lower) + __uint_as_float(upper);
+  }
+};
+
+// 16 rows on 16x16x32 MFMA: row = column lane % 16; of 32 keys the lane quarter h holds the
+// keys 16 i + 4 h + j, i below 2 and j below 4.
+template <int D, int kParts>
+struct NarrowRows {
+  static constexpr int kSteps = D / 32, kBlocks = D / 16;
+  s16x8 q[kSteps][kParts];  // Q^T as the B operand: k = 8 quarter + j of each 32-wide step
+  f32x4 out[kBlocks];       // O^T: d = 16 b + 4 quarter + e of the column's row
+  float top, total;
+  int key_at, value_at;
+
+  __device__ __forceinline__ void start(const void* queries, int64_t row, int lane) {
+    const int column = lane % 16, quarter = lane / 16;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) load_query<kParts>(queries, row * D + 8 * quarter + 32 * s, q[s]);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) out[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    top = -INFINITY;
+    total = 0.0f;
+    // Where this lane reads: K row `column`, chunk 4 s + quarter; V key 4 quarter + column / 4,
+    // 4 values from 4 (column % 4) of each 16-wide block (whose two chunks are 2 b and 2 b + 1).
+    key_at = column * D + ((quarter ^ turn_k(column)) * 8);
+    const int r = 4 * quarter + column / 4;
+    value_at = r * D + ((column % 4 / 2) ^ turn_v(r)) * 8 + column % 2 * 4;
+  }
+  // Chunks are permuted in LDS so that both operands' reads touch every bank once: K's 16 rows
+  // of one chunk, V's eight rows of two. (Rows 16 on are turned as the first 16.)
+  static __device__ __forceinline__ int turn_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int turn_v(int row) { return D == 128 ? (row & 7) << 1 : (row & 6); }
+
+  // A tile of 32 keys from LDS, as above.
+  __device__ __forceinline__ void take(const uint16_t* tile_k, const uint16_t* tile_v, float scale_log2, bool edge,
+                                       int first, int last, uint32_t absent, int quarter) {
+    f32x4 s[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const s16x8 k = *reinterpret_cast<const s16x8*>(tile_k + kb * 16 * D + (key_at ^ (step * 32)));
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
+                                                          __builtin_bit_cast(bf16x8, q[step][part]), s[kb], 0, 0, 0);
+        }
+      }
+    }
+    if (edge) {
+      asm volatile("");   // a branch: as selects its compares ran in every tile
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int in = (e / 4) * 16 + 4 * quarter + e % 4;
+        const bool keep = in >= first && in < last && ((absent >> (in / 16)) & 1u) == 0;
+        s[e / 4][e % 4] = keep ? s[e / 4][e % 4] : -INFINITY;
+      }
+    }
+    float best = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) best = fmaxf(best, s[e / 4][e % 4]);
+    uint32_t x, y;
+    row_pair(__float_as_uint(best), x, y);
+    best = fmaxf(__uint_as_float(x), __uint_as_float(y));
+    half_pair(__float_as_uint(best), x, y);
+    best = fmaxf(__uint_as_float(x), __uint_as_float(y)) * scale_log2;
+    float shrink;
+    if (raise(top, best, shrink)) {
+      total *= shrink;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], scale_log2, -base));
+    total += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    const u32x4 weights = pack8(p);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const uint16_t* at = tile_v + (value_at ^ (b * 16));
+      out[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, read_transposed(at, at + 16 * D)),
+                                                       __builtin_bit_cast(bf16x8, weights), out[b], 0, 0, 0);
+    }
+  }
+
+  template <typename ValueRow>
+  __device__ __forceinline__ void put_odd(int low, int end, int quarter, const ValueRow& value_row) {
+    for (int key = low; key < end; ++key) {
+      const uint16_t* value = value_row(key);
+      if (value == nullptr) continue;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = bf16_to_f32(value[b * 16 + 4 * quarter + e]);
+          out[b][e] += fabsf(v) <= FLT_MAX ? 0.0f : v;
+        }
+      }
+    }
+  }
+
+  // The row's sum, from the four quarters' keys.
+  __device__ __forceinline__ float whole_total() const {
+    uint32_t x, y;
+    row_pair(__float_as_uint(total), x, y);
+    const float two = __uint_as_float(x) + __uint_as_float(y);
+    half_pair(__float_as_uint(two), x, y);
+    return __uint_as_float(x) + __uint_as_float(y);
   }
 };
 
@@ -421,9 +575,9 @@ __device__ __forceinline__ void store_state(const BatchArgs& a, int64_t at, floa
 
 // Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS
 // buffers, the next tile's rows in registers while this one is multiplied.
-template <int D>
+template <int D, int kParts>
 __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t* lds, int* odd) {
-  using Rows = WaveRows<D>;
+  using Rows = WideRows<D, kParts>;
   constexpr int kChunks = D / 8;
   constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread stages, each of K and V
   constexpr int kTile = kTileKeys * D;                // elements of one tile
@@ -434,13 +588,12 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   const bool working = p.first_row + wave * kWaveRows < p.end_row;   // the wave
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int limit = a.at.before(a.at.tokens[token]) + 1;
-  const uint16_t* query = a.q + (static_cast<int64_t>(token) * a.heads + head) * D;
   // Rows that stop before the shared ones end are not expected of a plan, but served.
   if (p.shared && __syncthreads_or(limit < p.high)) p.mixed = true;
 
   PageWalk walk(a.at, p.sequence, p.low);
   Rows rows;
-  rows.start(query, lane);
+  rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
 
   // Staging: thread t's vector i is row (t + 256 i) / kChunks, chunk t % kChunks of the tile: of
   // one sixteen for the whole wave. A row outside [low, high), or of no page, comes as zeros (a
@@ -515,14 +668,14 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   }
   lds_barrier();
   for (int turn = 0; tile < tiles; turn ^= 1, ++tile) {
-    const bool edge = p.mixed || !whole;
+    const bool edge = __builtin_amdgcn_readfirstlane(p.mixed || !whole ? 1 : 0) != 0;
     const uint32_t holes = absent;
+    const int key0 = tile * kTileKeys;
     const bool more = tile + 1 < tiles;
     if (more) load_tile(tile + 1);
     if (working) {
       const uint16_t* tile_k = lds + turn * 2 * kTile;
-      rows.template take<2>(tile_k, tile_k + kTile, a.scale_log2, edge, tile * kTileKeys, p.low, p.high, limit, holes,
-                            half);
+      rows.take(tile_k, tile_k + kTile, a.scale_log2, edge, p.low - key0, min(p.high, limit) - key0, holes, half);
     }
     if (more) store_tile(turn ^ 1);
     lds_barrier();
@@ -560,34 +713,34 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   }
 }
 
-// Up to 32 rows: the four waves hold the same rows and take every fourth tile of keys each,
+// Up to 16 rows: the four waves hold the same rows and take every fourth tile of 32 keys each,
 // through an LDS buffer of their own without a barrier, and merge at the end.
-template <int D>
+template <int D, int kParts>
 __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16_t* lds) {
-  using Rows = WaveRows<D>;
-  constexpr int kKeyBlocks = D == 128 ? 1 : 2, kKeys = 32 * kKeyBlocks;
+  using Rows = NarrowRows<D, kParts>;
+  constexpr int kKeys = 32;
   constexpr int kChunks = D / 8, kRowsALoad = kWave / kChunks;   // 4 or 8
-  constexpr int kLoads = kKeys / kRowsALoad;                     // 8: 16-byte vectors a lane stages, each of K and V
+  constexpr int kLoads = kKeys / kRowsALoad;                     // 16-byte vectors a lane stages, each of K and V
   constexpr int kTile = kKeys * D;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int column = lane % 32, half = lane / 32;
+  const int column = lane % 16, quarter = lane / 16;
   const int row = min(p.first_row + column, p.end_row - 1);
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int limit = a.at.before(a.at.tokens[token]) + 1;
-  const uint16_t* query = a.q + (static_cast<int64_t>(token) * a.heads + head) * D;
   if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
 
   const int tiles = (p.high + kKeys - 1) / kKeys;   // past the last
   int tile = p.low / kKeys + wave;
   PageWalk walk(a.at, p.sequence, tile * kKeys);
   Rows rows;
-  rows.start(query, lane);
+  rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
   uint16_t* tile_k = lds + wave * 2 * kTile;
   uint16_t* tile_v = tile_k + kTile;
   const int chunk = lane % kChunks, stage_row = lane / kChunks;
+  const uint32_t offset = stage_row * D + chunk * 8;
   u32x4 stage_k[kLoads], stage_v[kLoads];
-  bool whole;
-  uint32_t absent;
+  bool whole = false;
+  uint32_t absent = 0;
   auto load_tile = [&](int t) {
     const int key0 = t * kKeys;
     walk.reach(key0);
@@ -599,21 +752,21 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
       absent |= page < 0 ? 1u << i : 0u;
       first[i] = a.at.row_of(max(page, 0), a.kv_heads, p.kv_head, key0 + 16 * i) * D;
     }
-    whole = absent == 0 && key0 >= p.low && key0 + kKeys <= p.high;
+    whole = __builtin_amdgcn_readfirstlane(absent == 0 && key0 >= p.low && key0 + kKeys <= p.high ? 1 : 0) != 0;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int in = i * kRowsALoad;   // of the tile, the load's first row
-      const int64_t base = first[in / 16] + (in % 16) * D;
-      const uint32_t offset = stage_row * D + chunk * 8;
+      const uint16_t* from_k = a.keys + first[in / 16] + (in % 16) * D;
+      const uint16_t* from_v = a.values + first[in / 16] + (in % 16) * D;
       if (whole) {
-        stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
-        stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+        stage_k[i] = *reinterpret_cast<const u32x4*>(from_k + offset);
+        stage_v[i] = *reinterpret_cast<const u32x4*>(from_v + offset);
       } else {
         const int key = key0 + in + stage_row;
         stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
         if (((absent >> (in / 16)) & 1u) == 0 && key >= p.low && key < p.high) {
-          stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
-          stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
+          stage_k[i] = *reinterpret_cast<const u32x4*>(from_k + offset);
+          stage_v[i] = *reinterpret_cast<const u32x4*>(from_v + offset);
         }
       }
     }
@@ -623,7 +776,7 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
   if (tile < tiles) load_tile(tile);
   while (tile < tiles) {
     const int key0 = tile * kKeys;
-    const bool edge = p.mixed || !whole;
+    const bool edge = __builtin_amdgcn_readfirstlane(p.mixed || !whole ? 1 : 0) != 0;
     const uint32_t holes = absent;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -637,36 +790,31 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
     // The wave's lanes read what the others stored: LDS takes a wave's operations in order.
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-    rows.template take<kKeyBlocks>(tile_k, tile_v, a.scale_log2, edge, key0, p.low, p.high, limit, holes, half);
+    rows.take(tile_k, tile_v, a.scale_log2, edge, p.low - key0, min(p.high, limit) - key0, holes, quarter);
     tile = following;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
   }
-
   // A wave that took any out puts back its own keys' (every fourth tile's).
   if (__ballot(odd) != 0) {
     const auto any = value_row<D>(a, p);
-    rows.put_odd(p.low, min(p.high, limit), half, [&](int key) {
+    rows.put_odd(p.low, min(p.high, limit), quarter, [&](int key) {
       return (key / kKeys - p.low / kKeys) % kWaves == wave ? any(key) : nullptr;
     });
   }
 
   // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c], its top
-  // and sum behind the four.
+  // and sum behind them all.
   const float total = rows.whole_total();
   const int count = p.end_row - p.first_row;
   float* parts = reinterpret_cast<float*>(lds);
-  float2* states = reinterpret_cast<float2*>(parts + kWaves * kWaveRows * D);
+  float2* states = reinterpret_cast<float2*>(parts + kWaves * kNarrowRows * D);
   lds_barrier();
   if (column < count) {
 #pragma unroll
     for (int b = 0; b < Rows::kBlocks; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        *reinterpret_cast<f32x4*>(parts + (wave * kWaveRows + column) * D + b * 32 + 8 * i + 4 * half) =
-            f32x4{rows.out[b][4 * i], rows.out[b][4 * i + 1], rows.out[b][4 * i + 2], rows.out[b][4 * i + 3]};
-      }
+      *reinterpret_cast<f32x4*>(parts + (wave * kNarrowRows + column) * D + b * 16 + 4 * quarter) = rows.out[b];
     }
-    if (half == 0) states[wave * kWaveRows + column] = float2{rows.top, total};
+    if (quarter == 0) states[wave * kNarrowRows + column] = float2{rows.top, total};
   }
   lds_barrier();
   const int splits = a.prefix_splits + a.own_splits;
@@ -674,15 +822,15 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
     const int r = item / (D / 4), d = item % (D / 4) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, states[w * kWaveRows + r].x);
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, states[w * kNarrowRows + r].x);
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float2 state = states[w * kWaveRows + r];
+      const float2 state = states[w * kNarrowRows + r];
       const float factor = __builtin_amdgcn_exp2f(state.x - base);
-      const f32x4 part = *reinterpret_cast<const f32x4*>(parts + (w * kWaveRows + r) * D + d);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(parts + (w * kNarrowRows + r) * D + d);
       sum = __builtin_fmaf(state.y, factor, sum);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(part[i], factor, v[i]);
@@ -705,16 +853,16 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
   }
 }
 
-template <int D>
+template <int D, int kParts>
 __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElements + kWaves * kWaveRows * 4];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElements];
   __shared__ int odd;   // a value was taken out
   Piece p;
   if (!find_piece(a, p)) return;
-  if (p.end_row - p.first_row <= kWaveRows) {
-    narrow_piece<D>(a, p, lds);
+  if (p.end_row - p.first_row <= kNarrowRows) {
+    narrow_piece<D, kParts>(a, p, lds);
   } else {
-    wide_piece<D>(a, p, lds, &odd);
+    wide_piece<D, kParts>(a, p, lds, &odd);
   }
 }
 
@@ -784,8 +932,8 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, i
   Plan p{};
   const int64_t rows = tokens * (heads / kv_heads);
   p.prefix_tiles = prefix > 0 ? (rows + kTileRows - 1) / kTileRows : 0;
-  p.prefix_splits = cut(kv_heads * p.prefix_tiles, prefix, rows <= kWaveRows, p.prefix_keys);
-  p.own_splits = cut(kv_heads * own_tiles, own_rows, rows <= kWaveRows * own_tiles, p.own_keys);
+  p.prefix_splits = cut(kv_heads * p.prefix_tiles, prefix, rows <= kNarrowRows, p.prefix_keys);
+  p.own_splits = cut(kv_heads * own_tiles, own_rows, rows <= kNarrowRows * own_tiles, p.own_keys);
   return p;
 }
 
@@ -811,8 +959,8 @@ extern "C" int32_t omnia_attention_batch_project(
     const uint16_t* raw_queries, int64_t query_stride, const uint16_t* raw_keys, int64_t key_stride,
     const uint16_t* raw_values, int64_t value_stride, const uint16_t* query_weight, const uint16_t* key_weight,
     const float* cos_rows, const float* sin_rows, int64_t table_stride, int64_t angle_rows, int64_t rotary_pairs,
-    float mscale, float eps, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, uint16_t* queries,
-    uint16_t* keys, uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
+    float mscale, float eps, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, void* queries,
+    int32_t wide_queries, uint16_t* keys, uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
     int64_t width, const int32_t* lengths, const int32_t* token_map, hipStream_t stream) {
   using namespace omnia;
   OMNIA_REQUIRE(geometry_served(tokens, heads, kv_heads, head_dim, 0, 0, 0), "attention_batch_project: bad geometry");
@@ -844,7 +992,7 @@ extern "C" int32_t omnia_attention_batch_project(
                            {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
                             static_cast<int>(width), static_cast<int>(pages), shift},
                            static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(tokens),
-                           static_cast<int>(rotary_pairs), mscale, eps};
+                           static_cast<int>(rotary_pairs), wide_queries != 0 ? 1 : 0, mscale, eps};
   const int64_t threads = tokens * (heads + 2 * kv_heads) * (head_dim / 8);
   const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
   (head_dim == 64 ? attention_batch_project_kernel<64> : attention_batch_project_kernel<128>)<<<grid, 256, 0, stream>>>(a);
@@ -861,8 +1009,8 @@ extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t
   return splits == 1 ? 0 : splits * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t* keys, const uint16_t* values,
-                                         int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
+extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queries, const uint16_t* keys,
+                                         const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
                                          int64_t width, const int32_t* lengths, const int32_t* token_map,
                                          int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
                                          int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -901,7 +1049,9 @@ extern "C" int32_t omnia_attention_batch(const uint16_t* queries, const uint16_t
   const int64_t merges = (tokens * heads * (head_dim / 4) + 255) / 256;
   OMNIA_REQUIRE(blocks < (int64_t{1} << 31) && merges < (int64_t{1} << 31), "attention_batch: too many tiles");
   if (blocks > 0) {
-    const auto kernel = head_dim == 64 ? attention_batch_kernel<64> : attention_batch_kernel<128>;
+    const bool wide = wide_queries != 0;
+    const auto kernel = head_dim == 64 ? (wide ? attention_batch_kernel<64, 2> : attention_batch_kernel<64, 1>)
+                                       : (wide ? attention_batch_kernel<128, 2> : attention_batch_kernel<128, 1>);
     kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
   }
   if (p.prefix_splits + p.own_splits != 1) {

@@ -212,7 +212,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
             table = table.table()
         return table.cos, table.sin
 
-    def _project(self, batch: PagedBatch, raw_queries, raw_keys, raw_values) -> tuple[torch.Tensor, int]:
+    def _project(self, batch: PagedBatch, raw_queries, raw_keys, raw_values, wide: bool) -> tuple[torch.Tensor, int]:
         core, cache = self.core, self.core.cache
         last = cache.ready(batch)
         angles = self._angles(last)
@@ -222,7 +222,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         queries = ops.attention_batch_project(
             _readable(raw_queries), _readable(raw_keys), _readable(raw_values), core.query_weight, core.key_weight,
             angles, cache.keys[core.layer], cache.values[core.layer], cache.tables, cache.lengths, batch.token_map,
-            heads=core.heads, eps=core.eps, mscale=core.mscale)
+            heads=core.heads, eps=core.eps, mscale=core.mscale, wide_queries=wide)
         return queries, last
 
     def _followed(self, *raw: torch.Tensor) -> bool:
@@ -237,7 +237,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         _check_rows(batch, raw_queries, core.heads * core.head_dim, "raw_queries")
         if self._followed(raw_queries, raw_keys, raw_values):
             return core.project(batch, raw_queries, raw_keys, raw_values)
-        return self._project(batch, raw_queries, raw_keys, raw_values)[0]
+        return self._project(batch, raw_queries, raw_keys, raw_values, False)[0]
 
     def __call__(self, batch, raw_queries, raw_keys, raw_values):
         core, cache = self.core, self.core.cache
@@ -245,7 +245,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         if self._followed(raw_queries, raw_keys, raw_values):
             return core(batch, raw_queries, raw_keys, raw_values)
         tiles = batch.tiles(core.heads // core.kv_heads)
-        queries, last = self._project(batch, raw_queries, raw_keys, raw_values)
+        queries, last = self._project(batch, raw_queries, raw_keys, raw_values, True)
         return ops.attention_batch(
             queries, cache.keys[core.layer], cache.values[core.layer], cache.tables, cache.lengths, batch.token_map,
             tiles, prefix=batch.prefix, own_rows=last - batch.prefix, scale=core.scale, sinks=core.sinks)

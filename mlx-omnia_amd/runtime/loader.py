@@ -101,10 +101,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_pages_edit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "omnia_pages_advance": (_I32, [_P, _I64, _P, _P, _I64, _P]),
     "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
-                                             _F32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _I64,
-                                             _P, _P, _P]),
+                                             _F32, _I64, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _P, _I64,
+                                             _I64, _P, _P, _P]),
     "omnia_attention_batch_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
-    "omnia_attention_batch": (_I32, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
+    "omnia_attention_batch": (_I32, [_P, _I32, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
                                      _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
     "omnia_embed_atlas": (
         _I32,

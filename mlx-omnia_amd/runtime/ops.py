@@ -1262,6 +1262,7 @@ def attention_batch_project(
     heads: int,
     eps: float,
     mscale: float = 1.0,
+    wide_queries: bool = False,
     queries: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """The norms, the rotation and the page writes of a batch's new tokens in one launch; see
@@ -1269,7 +1270,7 @@ def attention_batch_project(
     [(1,) N, kv_heads * D] bf16 rows, weights [D] or None, angles the (cos, sin) tables
     [positions, pairs] fp32 or None, keys and values a layer's pool [pages, kv_heads,
     page_rows, D], tables and lengths as the cache holds them, token_map [N, 2] -> the
-    queries [N, heads, D]."""
+    queries [N, heads, D], bf16 or, not rounded, fp32."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch_project")
     tokens, q_stride = _token_rows(raw_queries, heads * head_dim, "raw_queries")
     k_tokens, k_stride = _token_rows(raw_keys, kv_heads * head_dim, "raw_keys")
@@ -1297,14 +1298,14 @@ def attention_batch_project(
                  "attention_batch_project: cos and sin row strides differ")
         tensors += [cos, sin]
     _require(on_rocm(*tensors), "attention_batch_project: tensors must share one ROCm device")
-    queries = _out(queries, raw_queries, (tokens, heads, head_dim), BF16, "queries")
+    queries = _out(queries, raw_queries, (tokens, heads, head_dim), F32 if wide_queries else BF16, "queries")
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     call("omnia_attention_batch_project", raw_queries.data_ptr(), q_stride, raw_keys.data_ptr(), k_stride,
          raw_values.data_ptr(), v_stride, ptr(query_weight), ptr(key_weight),
          cos.data_ptr() if angles is not None else None, sin.data_ptr() if angles is not None else None,
          table_stride, angle_rows, pairs, float(mscale), float(eps), tokens, heads, kv_heads, head_dim,
-         queries.data_ptr(), keys.data_ptr(), values.data_ptr(), pages, page_rows, tables.data_ptr(), sequences,
-         width, lengths.data_ptr(), token_map.data_ptr(), _stream(raw_queries))
+         queries.data_ptr(), int(wide_queries), keys.data_ptr(), values.data_ptr(), pages, page_rows,
+         tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), _stream(raw_queries))
     return queries
 
 
@@ -1323,12 +1324,12 @@ def attention_batch(
     sinks: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """Attention of a batch's new tokens, queries [N, heads, D], over a layer's pages; see
+    """Attention of a batch's new tokens, queries [N, heads, D] bf16 or fp32, over a layer's pages; see
     `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence,
     own_rows bounds the rows past them, tiles [n, 2] are runs of one sequence's query rows;
-    sinks [heads] bf16 or None -> [N, heads, D]."""
+    sinks [heads] bf16 or None -> [N, heads, D] bf16."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
-    _dense(queries, BF16, "queries")
+    _dense(queries, F32 if queries.dtype == F32 else BF16, "queries")
     _require(queries.dim() == 3 and queries.shape[2] == head_dim, "attention_batch: queries must be [N, heads, D]")
     tokens, heads, _ = queries.shape
     sequences, width = _page_tables(tables, lengths, "attention_batch")
@@ -1346,7 +1347,7 @@ def attention_batch(
     _require(nbytes >= 0, "attention_batch: geometry not served")
     workspace = torch.empty(nbytes // 4, dtype=F32, device=queries.device) if nbytes else None
     out = _out(out, queries, (tokens, heads, head_dim), BF16, "out")
-    call("omnia_attention_batch", queries.data_ptr(), keys.data_ptr(), values.data_ptr(), pages, page_rows,
+    call("omnia_attention_batch", queries.data_ptr(), int(queries.dtype == F32), keys.data_ptr(), values.data_ptr(), pages, page_rows,
          tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), tokens, tiles.data_ptr(),
          tiles.shape[0], prefix, own_rows, heads, kv_heads, head_dim,
          sinks.data_ptr() if sinks is not None else None, float(scale),

@@ -3,8 +3,9 @@
 Tolerances, from the roundings the kernels make (half a step of bf16 is 2^-8 of the value):
 - a query or key row is rounded once, after fp32 operations whose errors are a few 2^-24 of
   the head's largest element: 2^-8 |want| + 2^-19 max |head|;
-- a context is taken from the kernel's own bf16 queries and pages: the weights are rounded
-  once (2^-8 of the mean of |v| under them) and the result once (2^-8 |want|). The fp32 sums
+- a context is taken from the kernel's own queries (fp32, of which the product takes 16 bits)
+  and pages: the weights are rounded once (2^-8 of the mean of |v| under them) and the result
+  once (2^-8 |want|). The fp32 sums
   add less than 2^-12 of that mean: a score is a sum of at most 128 exact products of a total
   size below 64 here, in fp32 (128 halves of 2^-23 times 64 is below 2^-11 at worst and some
   2^-15 in effect, halved by the softmax's normalisation), and exp2 and the merges a few 2^-22.
@@ -95,6 +96,14 @@ class Case:
             assert isinstance(step.strategy, HipBatchAttentionStep)
         return step
 
+    def wide_queries(self):
+        """The queries that the step's attention takes, before any rounding."""
+        angles = (self.cos, self.sin) if self.pairs else None
+        return ops.attention_batch_project(
+            *self.raw, self.qw, self.kw, angles, self.cache.keys[self.layer], self.cache.values[self.layer],
+            self.cache.tables, self.cache.lengths, self.batch.token_map, heads=self.heads, eps=1e-6,
+            mscale=self.mscale, wide_queries=True)
+
     def check_rows(self, queries, lengths):
         """Queries, and the key and value rows of the batch's tokens, against the oracle."""
         raw = [wide(t) for t in self.raw]
@@ -127,6 +136,8 @@ class Case:
         lengths = self.cache.lengths.cpu().numpy()
         queries = self.step.project(self.batch, *self.raw)
         self.check_rows(queries, lengths)
+        rounded, queries = queries, self.wide_queries()
+        assert torch.equal(rounded, queries.bfloat16())
         context = self.step(self.batch, *self.raw)
         assert context.shape == (self.batch.total, self.heads, self.head_dim)
         self.check_context(context, queries, lengths, rows)
@@ -423,7 +434,7 @@ def test_ops_refuse():
     keys, values = cache.keys[1], cache.values[1]
     base = dict(prefix=32, own_rows=5, scale=1.0)
     calls = [
-        lambda: ops.attention_batch(q.float(), keys, values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
+        lambda: ops.attention_batch(q.half(), keys, values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
         lambda: ops.attention_batch(q[:, ::2], keys, values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
         lambda: ops.attention_batch(q, keys.float(), values, cache.tables, cache.lengths, batch.token_map, tiles, **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables.long(), cache.lengths, batch.token_map, tiles, **base),
@@ -507,7 +518,10 @@ def test_answers_sampled_from_one_prompt():
         assert close(*outs), turn
     cache = worlds[0][0]
     assert cache.rows(kids[0][0]) == 190 and atlas.rows >= 190
-    queries = worlds[0][1][1].project(batches[0], *raw)
+    table = atlas.table()
+    queries = ops.attention_batch_project(
+        *raw, *gains, (table.cos, table.sin), cache.keys[1], cache.values[1], cache.tables, cache.lengths,
+        batches[0].token_map, heads=heads, eps=1e-6, wide_queries=True)
     got = worlds[0][1][1](batches[0], *raw)
     want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), cache.tables.cpu().numpy(),
                         cache.lengths.cpu().numpy(), batches[0].token_map.cpu().numpy(), d ** -0.5)
