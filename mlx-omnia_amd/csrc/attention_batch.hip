@@ -169,7 +169,6 @@ struct BatchArgs {
 };
 
 constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileKeys = 64, kNarrowRows = 16;
-constexpr int kLdsElements = 4 * 64 * 128;
 
 // A query row is one head of one token: of a kv head, row r is head r % group of token
 // r / group.
@@ -282,10 +281,14 @@ struct WideRows {
       }
     }
     if (edge) {
-      asm volatile("");   // a branch: as selects its compares ran in every tile
+      // This lane's keys are 4 half and a constant each: compared with constants, since 32 keys
+      // of its own were held in registers throughout the walk.
+      first -= 4 * half;
+      last -= 4 * half;
+      asm volatile("" : "+v"(first), "+v"(last));
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const int in = (e / 16) * 32 + 8 * ((e % 16) / 4) + 4 * half + e % 4;
+        const int in = (e / 16) * 32 + 8 * ((e % 16) / 4) + e % 4;
         const bool keep = in >= first && in < last && ((absent >> (in / 16)) & 1u) == 0;
         s[e / 16][e % 16] = keep ? s[e / 16][e % 16] : -INFINITY;
       }
@@ -395,10 +398,12 @@ struct NarrowRows {
       }
     }
     if (edge) {
-      asm volatile("");   // a branch: as selects its compares ran in every tile
+      first -= 4 * quarter;
+      last -= 4 * quarter;
+      asm volatile("" : "+v"(first), "+v"(last));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int in = (e / 4) * 16 + 4 * quarter + e % 4;
+        const int in = (e / 4) * 16 + e % 4;
         const bool keep = in >= first && in < last && ((absent >> (in / 16)) & 1u) == 0;
         s[e / 4][e % 4] = keep ? s[e / 4][e % 4] : -INFINITY;
       }
@@ -573,13 +578,20 @@ __device__ __forceinline__ void store_state(const BatchArgs& a, int64_t at, floa
       float2{top, total};
 }
 
-// Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS
-// buffers, the next tile's rows in registers while this one is multiplied.
+// 16 bytes a lane from global memory straight to LDS: lane l's come to `to` + 16 l.
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) {
+  typedef __attribute__((address_space(1))) const void* Global;
+  typedef __attribute__((address_space(3))) void* Local;
+  __builtin_amdgcn_global_load_lds((Global)from, (Local)to, 16, 0, 0);
+}
+
+// Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS stages;
+// the next tile is on its way to the one while the other is multiplied.
 template <int D, int kParts>
-__device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t* lds, int* odd) {
+__device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t* stage0, uint16_t* stage1, int* odd) {
   using Rows = WideRows<D, kParts>;
   constexpr int kChunks = D / 8;
-  constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread stages, each of K and V
+  constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread brings, each of K and V
   constexpr int kTile = kTileKeys * D;                // elements of one tile
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int column = lane % 32, half = lane / 32;
@@ -588,74 +600,71 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   const bool working = p.first_row + wave * kWaveRows < p.end_row;   // the wave
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int limit = a.at.before(a.at.tokens[token]) + 1;
-  // Rows that stop before the shared ones end are not expected of a plan, but served.
-  if (p.shared && __syncthreads_or(limit < p.high)) p.mixed = true;
+  // Up to here every row sees the keys: up to the first row's limit, or for the shared rows
+  // (that a sequence stops before their end is not expected of a plan, but served) nowhere.
+  int common = p.mixed ? a.at.before(a.at.tokens[p.first_row / a.group]) + 1 : p.high;
+  if (p.shared && __syncthreads_or(limit < p.high)) common = 0;
+  common = __builtin_amdgcn_readfirstlane(common);
 
   PageWalk walk(a.at, p.sequence, p.low);
   Rows rows;
   rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
 
-  // Staging: thread t's vector i is row (t + 256 i) / kChunks, chunk t % kChunks of the tile: of
-  // one sixteen for the whole wave. A row outside [low, high), or of no page, comes as zeros (a
-  // zero weight times what the page happens to hold could be a NaN).
+  // Thread t's vector i is chunk t % kChunks of row (t + 256 i) / kChunks of a tile, of one
+  // sixteen for the whole wave.
   const int chunk = threadIdx.x % kChunks;
   const int stage_row = threadIdx.x / kChunks;   // of vector 0
-  u32x4 stage_k[kLoads], stage_v[kLoads];
-  bool whole;            // of the tile that is staged: every row there
-  uint32_t absent;       // its sixteens without a page
-  auto load_tile = [&](int tile) {
+  const uint32_t from_k = (stage_row % 16) * D + (chunk ^ Rows::turn_k(stage_row)) * 8;
+  const uint32_t from_v = (stage_row % 16) * D + (chunk ^ Rows::turn_v(stage_row)) * 8;
+  const int sixteen = D == 128 ? 0 : __builtin_amdgcn_readfirstlane(wave / 2);   // of vector 0
+  int64_t base[kLoads];
+  bool whole = false;    // of the tile asked for: every row there, and seen by all rows
+  uint32_t absent = 0;   // its sixteens without a page
+  auto ask = [&](int tile, uint16_t* stage) {
     const int key0 = tile * kTileKeys;
     walk.reach(key0);
     absent = 0;
-    int64_t first[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int page = walk.page(key0 + 16 * i);
-      absent |= page < 0 ? 1u << i : 0u;
-      first[i] = a.at.row_of(max(page, 0), a.kv_heads, p.kv_head, key0 + 16 * i) * D;
-    }
-    whole = absent == 0 && key0 >= p.low && key0 + kTileKeys <= p.high;
-    const uint32_t offset = (stage_row % 16) * D + chunk * 8;
+    for (int i = 0; i < 4; ++i) absent |= walk.page(key0 + 16 * i) < 0 ? 1u << i : 0u;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      // D = 128: vector i is in sixteen i; D = 64: in sixteen 2 i or, the upper waves, 2 i + 1.
-      int64_t base;
-      int key;
-      bool there;
-      if constexpr (D == 128) {
-        base = first[i];
-        key = key0 + 16 * i + stage_row;
-        there = ((absent >> i) & 1u) == 0;
-      } else {
-        const bool upper = wave >= 2;
-        base = upper ? first[2 * i + 1] : first[2 * i];
-        key = key0 + 32 * i + stage_row;
-        there = ((absent >> (2 * i + (upper ? 1 : 0))) & 1u) == 0;
-      }
-      if (whole) {
-        stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
-        stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
-      } else {
-        stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
-        if (there && key >= p.low && key < p.high) {
-          stage_k[i] = *reinterpret_cast<const u32x4*>(a.keys + base + offset);
-          stage_v[i] = *reinterpret_cast<const u32x4*>(a.values + base + offset);
-        }
+      const int at = key0 + 16 * (D == 128 ? i : 2 * i + sixteen);
+      base[i] = a.at.row_of(max(walk.page(at), 0), a.kv_heads, p.kv_head, at) * D;
+    }
+    whole = absent == 0 && key0 >= p.low && key0 + kTileKeys <= min(p.high, common);
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        uint16_t* to = stage + (256 * i + wave * kWave) * 8;
+        load_to_lds(a.keys + base[i] + from_k, to);
+        load_to_lds(a.values + base[i] + from_v, to + kTile);
       }
     }
   };
-  // Where rows see different keys, a value that is not finite is taken out, and put to the rows
-  // that see it at the end: one that does not would have zero times it, a NaN.
-  auto store_tile = [&](int stage) {
-    uint16_t* tile_k = lds + stage * 2 * kTile;
-    uint16_t* tile_v = tile_k + kTile;
+  // Any other tile: a row outside [low, high), or of no page, comes as zeros (a zero weight
+  // times what the page happens to hold could be a NaN), and so does a value that is not
+  // finite: a row that does not see it would have zero times it. Those that see it get it at
+  // the end.
+  auto patch = [&](int tile, uint16_t* stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = stage_row + 256 / kChunks * i;
-      if (p.mixed && take_out_odd(stage_v[i])) *odd = 1;
-      *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ Rows::turn_k(at)) * 8) = stage_k[i];
-      *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ Rows::turn_v(at)) * 8) = stage_v[i];
+      const int key = tile * kTileKeys + at;
+      const bool there = key >= p.low && key < p.high && ((absent >> (at / 16)) & 1u) == 0;
+      u32x4 k = u32x4{0, 0, 0, 0}, v = u32x4{0, 0, 0, 0};
+      if (there) {
+        k = *reinterpret_cast<const u32x4*>(a.keys + base[i] + from_k);
+        v = *reinterpret_cast<const u32x4*>(a.values + base[i] + from_v);
+      }
+      if (take_out_odd(v)) *odd = 1;
+      *reinterpret_cast<u32x4*>(stage + at * D + chunk * 8) = k;
+      *reinterpret_cast<u32x4*>(stage + kTile + at * D + chunk * 8) = v;
     }
+  };
+  // The tile asked for is in LDS, of every wave.
+  auto arrive = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    lds_barrier();
   };
 
   const int tiles = (p.high + kTileKeys - 1) / kTileKeys;   // past the last
@@ -663,22 +672,29 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
   if (tile < tiles) {
-    load_tile(tile);
-    store_tile(0);
+    ask(tile, stage0);
+    if (!whole) patch(tile, stage0);
   }
-  lds_barrier();
-  for (int turn = 0; tile < tiles; turn ^= 1, ++tile) {
-    const bool edge = __builtin_amdgcn_readfirstlane(p.mixed || !whole ? 1 : 0) != 0;
+  arrive();
+  // The stages by name, not by a turning index: the compiler then sees that what is on its way
+  // to the one is not what is read from the other, and does not wait for it.
+  auto turn = [&](const uint16_t* here, uint16_t* there) {
+    const bool edge = !whole;
     const uint32_t holes = absent;
     const int key0 = tile * kTileKeys;
     const bool more = tile + 1 < tiles;
-    if (more) load_tile(tile + 1);
+    if (more) ask(tile + 1, there);
     if (working) {
-      const uint16_t* tile_k = lds + turn * 2 * kTile;
-      rows.take(tile_k, tile_k + kTile, a.scale_log2, edge, p.low - key0, min(p.high, limit) - key0, holes, half);
+      rows.take(here, here + kTile, a.scale_log2, edge, p.low - key0, min(p.high, limit) - key0, holes, half);
     }
-    if (more) store_tile(turn ^ 1);
-    lds_barrier();
+    ++tile;
+    if (more && !whole) patch(tile, there);
+    arrive();
+  };
+  while (tile < tiles) {
+    turn(stage0, stage1);
+    if (tile >= tiles) break;
+    turn(stage1, stage0);
   }
   if (*odd != 0) rows.put_odd(p.low, min(p.high, limit), half, value_row<D>(a, p));
 
@@ -716,7 +732,7 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
 // Up to 16 rows: the four waves hold the same rows and take every fourth tile of 32 keys each,
 // through an LDS buffer of their own without a barrier, and merge at the end.
 template <int D, int kParts>
-__device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16_t* lds) {
+__device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16_t* stage0, uint16_t* stage1) {
   using Rows = NarrowRows<D, kParts>;
   constexpr int kKeys = 32;
   constexpr int kChunks = D / 8, kRowsALoad = kWave / kChunks;   // 4 or 8
@@ -734,7 +750,7 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
   PageWalk walk(a.at, p.sequence, tile * kKeys);
   Rows rows;
   rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
-  uint16_t* tile_k = lds + wave * 2 * kTile;
+  uint16_t* tile_k = (wave < 2 ? stage0 : stage1) + wave % 2 * 2 * kTile;
   uint16_t* tile_v = tile_k + kTile;
   const int chunk = lane % kChunks, stage_row = lane / kChunks;
   const uint32_t offset = stage_row * D + chunk * 8;
@@ -802,12 +818,12 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
     });
   }
 
-  // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c], its top
-  // and sum behind them all.
+  // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c] of the one
+  // stage, its top and sum in the other.
   const float total = rows.whole_total();
   const int count = p.end_row - p.first_row;
-  float* parts = reinterpret_cast<float*>(lds);
-  float2* states = reinterpret_cast<float2*>(parts + kWaves * kNarrowRows * D);
+  float* parts = reinterpret_cast<float*>(stage0);
+  float2* states = reinterpret_cast<float2*>(stage1);
   lds_barrier();
   if (column < count) {
 #pragma unroll
@@ -855,14 +871,18 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
 
 template <int D, int kParts>
 __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElements];
+  // K and V of a tile each; a narrow piece's waves have half of one each, and its contexts of
+  // four waves fill the first.
+  __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTileKeys * D], stage1[2 * kTileKeys * D];
+  static_assert(sizeof(stage0) == kWaves * kNarrowRows * D * sizeof(float) && sizeof(stage0) == 2 * 2 * 32 * D * 2,
+                "a stage holds what a narrow piece puts there");
   __shared__ int odd;   // a value was taken out
   Piece p;
   if (!find_piece(a, p)) return;
   if (p.end_row - p.first_row <= kNarrowRows) {
-    narrow_piece<D, kParts>(a, p, lds);
+    narrow_piece<D, kParts>(a, p, stage0, stage1);
   } else {
-    wide_piece<D, kParts>(a, p, lds, &odd);
+    wide_piece<D, kParts>(a, p, stage0, stage1, &odd);
   }
 }
 
