@@ -189,6 +189,9 @@ constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileK
 // maximum would ask for in nearly every tile, is rare.
 constexpr float kSlack = 8.0f;
 
+// What the scheduler is told to group (sched_group_barrier's masks).
+constexpr int kValu = 0x2, kMfma = 0x8, kDsRead = 0x100;
+
 __device__ __forceinline__ u32x4 low_part(const float (&x)[8], const u32x4& high) {
   float h[8], rest[8];
   unpack8(high, h);
@@ -280,6 +283,23 @@ struct WideRows {
         }
       }
     }
+    // The first values, read while the scores are still being multiplied.
+    s16x8 v[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) v[b] = read_transposed(tile_v + value_at[b], tile_v + value_at[b] + 8 * D);
+    // Keys two steps ahead of their products.
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+    for (int step = 0; step < kSteps - 2; ++step) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, kParts, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, 2 * kParts, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kBlocks, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, 2 * kParts, 0);
     if (edge) {
       // This lane's keys are 4 half and a constant each: compared with constants, since 32 keys
       // of its own were held in registers throughout the walk.
@@ -307,6 +327,7 @@ struct WideRows {
     }
     const float base = top == -INFINITY ? 0.0f : top;
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4 weights[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) {   // 16 keys each
       float p[8];
@@ -315,14 +336,29 @@ struct WideRows {
         p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][(step % 2) * 8 + j], scale_log2, -base));
         sums[j % 4] += p[j];
       }
-      const u32x4 weights = pack8(p);
+      weights[step] = pack8(p);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        const uint16_t* at = tile_v + step * 16 * D + value_at[b];
-        out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, read_transposed(at, at + 8 * D)),
-                                                         __builtin_bit_cast(bf16x8, weights), out[b], 0, 0, 0);
+        out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[b]),
+                                                         __builtin_bit_cast(bf16x8, weights[step]), out[b], 0, 0, 0);
+        if (step < 3) {
+          const uint16_t* at = tile_v + (step + 1) * 16 * D + value_at[b];
+          v[b] = read_transposed(at, at + 8 * D);
+        }
       }
     }
+    // A step's products beside the next one's weights (28 vector operations) and values.
+    __builtin_amdgcn_sched_group_barrier(kValu, 28, 0);
+#pragma unroll
+    for (int step = 0; step < 3; ++step) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 28 / kBlocks, 0);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, kBlocks, 0);
     total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
 
@@ -646,7 +682,7 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   // finite: a row that does not see it would have zero times it. Those that see it get it at
   // the end.
   auto patch = [&](int tile, uint16_t* stage) {
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kLoads; ++i) {
       const int at = stage_row + 256 / kChunks * i;
       const int key = tile * kTileKeys + at;
