@@ -964,7 +964,7 @@ __global__ __launch_bounds__(256) void attention_batch_merge_kernel(BatchArgs a)
 // workgroups a CU of them, of at least four tiles; a narrow one leaves a few rows and is short,
 // so that sequences of different lengths fill the card evenly.
 struct Plan {
-  int64_t prefix_tiles, prefix_splits, prefix_keys, own_splits, own_keys;
+  int64_t prefix, prefix_tiles, prefix_splits, prefix_keys, own_splits, own_keys;
 };
 
 constexpr int64_t kWideBlocks = 512, kWideKeys = 256, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
@@ -977,6 +977,8 @@ int64_t cut(int64_t blocks, int64_t keys, bool narrow, int64_t& each) {
   int64_t splits = (target + blocks - 1) / blocks;
   const int64_t by_keys = keys / least;
   splits = splits < by_keys ? splits : by_keys;
+  // Wide pieces run in rounds of as many as fit the card: fewer, where they fill theirs as well.
+  if (!narrow && splits > 1 && blocks * (splits - 1) <= target && blocks * (splits - 1) * 8 >= target * 7) --splits;
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int64_t of_one = (tiles + splits - 1) / splits;
@@ -987,8 +989,13 @@ int64_t cut(int64_t blocks, int64_t keys, bool narrow, int64_t& each) {
 Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t own_rows, int64_t own_tiles) {
   Plan p{};
   const int64_t rows = tokens * (heads / kv_heads);
-  p.prefix_tiles = prefix > 0 ? (rows + kTileRows - 1) / kTileRows : 0;
-  p.prefix_splits = cut(kv_heads * p.prefix_tiles, prefix, rows <= kNarrowRows, p.prefix_keys);
+  const int64_t shared_tiles = (rows + kTileRows - 1) / kTileRows;
+  // Where the sequences' own tiles are nearly as full as shared ones (prompts), each walks the
+  // shared rows as well: as many products, and nothing to merge.
+  p.prefix = own_tiles * 4 <= shared_tiles * 5 ? 0 : prefix;
+  own_rows += prefix - p.prefix;
+  p.prefix_tiles = p.prefix > 0 ? shared_tiles : 0;
+  p.prefix_splits = cut(kv_heads * p.prefix_tiles, p.prefix, rows <= kNarrowRows, p.prefix_keys);
   p.own_splits = cut(kv_heads * own_tiles, own_rows, rows <= kNarrowRows * own_tiles, p.own_keys);
   return p;
 }
@@ -1098,7 +1105,7 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
                     {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
                      static_cast<int>(width), static_cast<int>(pages), shift},
                     static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(heads / kv_heads),
-                    static_cast<int>(tokens), static_cast<int>(prefix), static_cast<int>(p.prefix_tiles),
+                    static_cast<int>(tokens), static_cast<int>(p.prefix), static_cast<int>(p.prefix_tiles),
                     static_cast<int>(own_tiles), static_cast<int>(p.prefix_splits), static_cast<int>(p.prefix_keys),
                     static_cast<int>(p.own_splits), static_cast<int>(p.own_keys), scale * kLog2e};
   const int64_t blocks = kv_heads * (p.prefix_tiles * p.prefix_splits + own_tiles * p.own_splits);
