@@ -725,8 +725,9 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  * bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
  * prefix) must be the same pages in every token's sequence: they are read through the first
  * token's. own_rows bounds the rows past them of every sequence, this step's included; tiles
- * [own_tiles, 2] int32 (device) are runs [first, end) of query rows of one sequence, at most
- * 128 long, that cover every row once (of each kv head, row r is token r / gqa, head r % gqa).
+ * [own_tiles, 4] int32 (device) are runs of query rows that cover every row once (of each kv
+ * head, row r is token r / gqa, head r % gqa): (first, end, s, j) for the rows [first, end), at
+ * most 128, of sequence s, whose new token j the first row is of.
  * A row on no page (-1, or outside the pool) is not seen. queries [tokens, heads, D] bf16, or
  * fp32 with wide_queries 1; out [tokens, heads, D] bf16;
  * workspace: at least omnia_attention_batch_workspace_bytes, 16-byte aligned.

@@ -71,15 +71,17 @@ class PagedBatch:
         self._tiles: dict[int, torch.Tensor] = {}
 
     def tiles(self, group: int) -> torch.Tensor:
-        """Runs of at most TILE_ROWS query rows of one sequence, with `group` rows a token."""
+        """Runs of at most TILE_ROWS query rows of one sequence, with `group` rows a token: (first
+        row, past the last, sequence, which of its new tokens the first row is of)."""
         held = self._tiles.get(group)
         if held is None:
             if _capturing(self.cache.keys.device):
                 raise ValueError("a batch's first step cannot be captured: call prepare_capture first")
             runs = []
-            for end, count in zip(self.ends * group, self.counts * group):
+            for s, end, count in zip(self.sequences, self.ends * group, self.counts * group):
                 first = np.arange(end - count, end, TILE_ROWS)
-                runs.append(np.stack([first, np.minimum(first + TILE_ROWS, end)], axis=1))
+                runs.append(np.stack([first, np.minimum(first + TILE_ROWS, end), np.full_like(first, s),
+                                      (first - (end - count)) // group], axis=1))
             flat = np.ascontiguousarray(np.concatenate(runs), dtype=np.int32)
             held = self._tiles[group] = torch.from_numpy(flat).to(self.cache.keys.device)
         return held

@@ -1326,7 +1326,7 @@ def attention_batch(
 ) -> torch.Tensor:
     """Attention of a batch's new tokens, queries [N, heads, D] bf16 or fp32, over a layer's pages; see
     `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence,
-    own_rows bounds the rows past them, tiles [n, 2] are runs of one sequence's query rows;
+    own_rows bounds the rows past them, tiles [n, 4] are runs of one sequence's query rows;
     sinks [heads] bf16 or None -> [N, heads, D] bf16."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
     _dense(queries, F32 if queries.dtype == F32 else BF16, "queries")
@@ -1334,8 +1334,8 @@ def attention_batch(
     tokens, heads, _ = queries.shape
     sequences, width = _page_tables(tables, lengths, "attention_batch")
     _token_map(token_map, tokens, "attention_batch")
-    _require(tiles.dtype == torch.int32 and tiles.is_contiguous() and tiles.dim() == 2 and tiles.shape[1] == 2,
-             "attention_batch: tiles must be contiguous int32 [n, 2]")
+    _require(tiles.dtype == torch.int32 and tiles.is_contiguous() and tiles.dim() == 2 and tiles.shape[1] == 4,
+             "attention_batch: tiles must be contiguous int32 [n, 4]")
     tensors = [queries, keys, values, tables, lengths, token_map, tiles]
     if sinks is not None:
         _require(sinks.dtype == BF16 and sinks.is_contiguous() and sinks.numel() == heads,

@@ -221,7 +221,8 @@ def test_tokens_of_no_sequence_and_pages_of_no_pool():
     token_map[0, 0] = cache.tables.shape[0] + 5
     # The first token's sequence gives the shared rows: here the second's.
     token_map[[0, 1]] = token_map[[1, 0]]
-    tiles = batch.tiles(4)
+    tiles = batch.tiles(4).clone()
+    tiles[:, 2] = token_map[:, 0]
     lengths = cache.lengths.cpu().numpy()
     out = ops.attention_batch(queries, cache.keys[1], cache.values[1], tables, cache.lengths, token_map, tiles,
                               prefix=64, own_rows=41, scale=case.scale)
@@ -440,7 +441,7 @@ def test_ops_refuse():
         lambda: ops.attention_batch(q, keys, values, cache.tables.long(), cache.lengths, batch.token_map, tiles, **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths[:2], batch.token_map, tiles, **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map[:1], tiles, **base),
-        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles[:, :1], **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles[:, :2], **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles.cpu(), **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles, prefix=-1,
                                     own_rows=5, scale=1.0),

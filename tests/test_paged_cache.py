@@ -107,7 +107,7 @@ def test_batches_find_what_their_sequences_share():
     assert cache.batch(kids).prefix == 32
     batch = cache.batch([kids[0], kids[2]], tokens=[3, 1])
     assert batch.token_map.tolist() == [[kids[0], 0], [kids[0], 1], [kids[0], 2], [kids[2], 0]]
-    assert batch.tiles(50).tolist() == [[0, 128], [128, 150], [150, 200]]
+    assert batch.tiles(50).tolist() == [[0, 128, kids[0], 0], [128, 150, kids[0], 2], [150, 200, kids[2], 0]]
 
 
 def test_full_pools_and_tables_leave_everything_as_it_was():
