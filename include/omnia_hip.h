@@ -652,8 +652,8 @@ int32_t omnia_stream_copy(const void* src, void* dst, int64_t bytes, int32_t vec
  * width] and lengths [sequences] are int32, on the device.
  * No counterpart in the reference, whose caches hold a sequence each (core/cache/kv.py). */
 
-/* Most moves and edits one call takes: they travel in the kernel's arguments. */
-#define OMNIA_PAGES_MOVES 256
+/* Most moves, children and edits one call takes: they travel in the kernel's arguments. */
+#define OMNIA_PAGES_MOVES 128
 #define OMNIA_PAGES_EDITS 128
 
 /* Copies the first rows of pages, in every layer, keys and values: moves [count, 3] int32 in
@@ -666,17 +666,25 @@ int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t layers, int64
                          const int32_t* moves, int64_t count, int32_t* tables, int64_t entries,
                          hipStream_t stream);
 
-/* Edits of tables and lengths: edits [count, 5] int32 in HOST memory (kind, sequence, a, b, c):
+/* Makes sequences the children of `parent`: kids [count, 2] int32 in HOST memory (sequence,
+ * page). A child's row of the table is the parent's first `full` entries, then its page, then
+ * -1, its length the parent's. The first `rows` rows of every head of `page` (the parent's
+ * last, partly filled one) are copied into the child's, in every layer; with rows 0 there is
+ * nothing to copy and the children's page is -1. Children and pages are distinct. */
+int32_t omnia_pages_fork(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages,
+                         int64_t kv_heads, int64_t page_rows, int64_t head_dim, int32_t* tables,
+                         int32_t* lengths, int64_t sequences, int64_t width, int64_t parent,
+                         int64_t full, int64_t page, int64_t rows, const int32_t* kids,
+                         int64_t count, hipStream_t stream);
+
+/* Edits of tables and lengths: edits [count, 4] int32 in HOST memory (kind, sequence, a, b):
  *   OMNIA_PAGES_ENTRY   tables[sequence][a] = b
  *   OMNIA_PAGES_LENGTH  lengths[sequence] = a
- *   OMNIA_PAGES_FORK    tables[sequence] = the first b entries of sequence a, then page c (or
- *                       -1), then -1; lengths[sequence] = lengths[a]
- *   OMNIA_PAGES_CLEAR   tables[sequence] = -1, lengths[sequence] = 0 (b 0, c -1)
- * No edit may write what another one of the call writes or reads. */
+ *   OMNIA_PAGES_CLEAR   tables[sequence] = -1, lengths[sequence] = 0
+ * No two edits of a call may write one place. */
 #define OMNIA_PAGES_ENTRY 0
 #define OMNIA_PAGES_LENGTH 1
-#define OMNIA_PAGES_FORK 2
-#define OMNIA_PAGES_CLEAR 3
+#define OMNIA_PAGES_CLEAR 2
 int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t sequences, int64_t width,
                          int64_t pages, const int32_t* edits, int64_t count, hipStream_t stream);
 
@@ -742,6 +750,29 @@ int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
                               int64_t head_dim, const uint16_t* sinks, float scale,
                               void* workspace, int64_t workspace_bytes, uint16_t* out,
                               hipStream_t stream);
+
+/* A batch's step of one layer in one call: omnia_attention_batch_project with fp32 queries, then
+ * omnia_attention_batch over them. The workspace holds the queries [tokens, heads, D] fp32 and,
+ * from the next multiple of 256 bytes on, what omnia_attention_batch needs:
+ * omnia_attention_batch_step_bytes. With `queries` not null only the first half runs, its
+ * queries rounded to bf16 there. Every field is as the two entries take it; `raw_*`, `queries`,
+ * `out` and `workspace` are what changes from call to call, `own_rows` from step to step. */
+typedef struct {
+  const uint16_t *raw_queries, *raw_keys, *raw_values, *query_weight, *key_weight;
+  const float *cos_rows, *sin_rows;
+  uint16_t *keys, *values;
+  const int32_t *tables, *lengths, *token_map, *tiles;
+  const uint16_t *sinks;
+  uint16_t *queries, *out;
+  void *workspace;
+  int64_t workspace_bytes, query_stride, key_stride, value_stride, table_stride, angle_rows, rotary_pairs;
+  int64_t tokens, heads, kv_heads, head_dim, pages, page_rows, sequences, width, own_tiles, prefix, own_rows;
+  float mscale, eps, scale;
+} omnia_attention_batch_step_t;
+int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t prefix, int64_t own_rows,
+                                         int64_t own_tiles);
+int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1077,6 +1077,10 @@ bool geometry_served(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t he
          own_rows < kMaxRows && own_tiles >= 0 && own_tiles < kMaxRows;
 }
 
+int64_t query_bytes(int64_t tokens, int64_t heads, int64_t head_dim) {
+  return (tokens * heads * head_dim * static_cast<int64_t>(sizeof(float)) + 255) / 256 * 256;
+}
+
 int page_shift_of(int64_t page_rows) {
   for (int shift = 4; shift <= 8; ++shift) {
     if (page_rows == int64_t{1} << shift) return shift;
@@ -1189,4 +1193,37 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
     head_dim == 64 ? launch_merge<64>(a, stream) : launch_merge<128>(a, stream);
   }
   return launched("attention_batch");
+}
+
+extern "C" int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                    int64_t prefix, int64_t own_rows, int64_t own_tiles) {
+  using namespace omnia;
+  const int64_t more = omnia_attention_batch_workspace_bytes(tokens, heads, kv_heads, head_dim, prefix, own_rows,
+                                                             own_tiles);
+  return more < 0 ? more : query_bytes(tokens, heads, head_dim) + more;
+}
+
+extern "C" int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* s, hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(s != nullptr, "attention_batch_step: null pointer");
+  const auto project = [&](void* queries, int32_t wide) {
+    return omnia_attention_batch_project(
+        s->raw_queries, s->query_stride, s->raw_keys, s->key_stride, s->raw_values, s->value_stride, s->query_weight,
+        s->key_weight, s->cos_rows, s->sin_rows, s->table_stride, s->angle_rows, s->rotary_pairs, s->mscale, s->eps,
+        s->tokens, s->heads, s->kv_heads, s->head_dim, queries, wide, s->keys, s->values, s->pages, s->page_rows,
+        s->tables, s->sequences, s->width, s->lengths, s->token_map, stream);
+  };
+  if (s->queries != nullptr) return project(s->queries, 0);
+  const int64_t need = omnia_attention_batch_step_bytes(s->tokens, s->heads, s->kv_heads, s->head_dim, s->prefix,
+                                                        s->own_rows, s->own_tiles);
+  OMNIA_REQUIRE(need >= 0, "attention_batch_step: bad geometry");
+  OMNIA_REQUIRE(need == 0 || (s->workspace && s->workspace_bytes >= need && aligned16(s->workspace)),
+                "attention_batch_step: workspace too small (omnia_attention_batch_step_bytes) or not aligned");
+  const int64_t queries = query_bytes(s->tokens, s->heads, s->head_dim);
+  const int32_t rc = project(s->workspace, 1);
+  if (rc != 0) return rc;
+  return omnia_attention_batch(s->workspace, 1, s->keys, s->values, s->pages, s->page_rows, s->tables, s->sequences,
+                               s->width, s->lengths, s->token_map, s->tokens, s->tiles, s->own_tiles, s->prefix,
+                               s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
+                               static_cast<char*>(s->workspace) + queries, s->workspace_bytes - queries, s->out, stream);
 }

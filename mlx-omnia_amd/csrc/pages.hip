@@ -6,6 +6,8 @@
 // layer. The page ids to copy and the edits come from the host in the kernel's arguments, each
 // checked before the launch: no list has to be on the device, or outlive the call, and no id
 // that a kernel here follows is one that the host has not seen.
+#include <string>
+
 #include "common.hpp"
 #include "host.hpp"
 
@@ -16,19 +18,44 @@ struct Move {
   int32_t from, to, rows;
 };
 
-struct CopyArgs {
-  uint16_t* pool[2];        // keys, values
+// A pool's pages, as far as a copy needs them.
+struct Pool {
+  uint16_t* pages[2];       // keys, values
   int64_t layer_stride;     // elements from a layer to the next
+  int heads, page_rows, head_dim, planes;   // planes: layers of both
+
+  // Page `page` of plane `plane` (layer, then keys or values).
+  __device__ __forceinline__ uint16_t* page(int plane, int32_t page) const {
+    return pages[plane & 1] + (plane >> 1) * layer_stride + static_cast<int64_t>(page) * heads * page_rows * head_dim;
+  }
+};
+
+constexpr int kPieceVectors = 1024;   // 16-byte vectors a workgroup copies, four a thread
+
+// Where thread t's i-th vector of a piece of the first `rows` rows of every head lies in a page,
+// or -1 past them.
+__device__ __forceinline__ int vector_at(const Pool& pool, int rows, int piece, int i) {
+  const int head_vectors = rows * pool.head_dim / 8;
+  const int vector = piece * kPieceVectors + i * 256 + threadIdx.x;
+  const int head = vector / head_vectors;
+  return head < pool.heads ? head * pool.page_rows * pool.head_dim + (vector - head * head_vectors) * 8 : -1;
+}
+
+int pieces_of(int64_t kv_heads, int64_t rows, int64_t head_dim) {
+  return static_cast<int>((kv_heads * rows * head_dim / 8 + kPieceVectors - 1) / kPieceVectors);
+}
+
+struct CopyArgs {
+  Pool pool;
   int32_t* tables;          // renamed from -> to where they name a moved page, or null
   int64_t entries;          // of the tables
-  int heads, page_rows, head_dim, count, layers, pieces, copies;
+  int count, pieces, copies;
   Move moves[OMNIA_PAGES_MOVES];
 };
 
-constexpr int kPieceVectors = 1024;   // 16-byte vectors a workgroup copies
-
-// One piece (16 KB) of one page of one layer of one pool a workgroup; the workgroups past the
-// copies rename table entries, 256 each.
+// One piece (16 KB) of one page of one plane a workgroup; the workgroups past the copies rename
+// table entries, 256 each. Bound by memory: nothing is read or written twice, and past the
+// caches.
 __global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
   const int block = blockIdx.x;
   if (block >= a.copies) {
@@ -49,33 +76,72 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
   }
   const int piece = block % a.pieces;
   const int rest = block / a.pieces;
-  const int move = rest % a.count;
-  const int plane = rest / a.count;   // layer, pool
-  const Move m = a.moves[move];
-  uint16_t* layer = a.pool[plane & 1] + (plane >> 1) * a.layer_stride;
-  const int64_t page_elements = static_cast<int64_t>(a.heads) * a.page_rows * a.head_dim;
-  const uint16_t* from = layer + m.from * page_elements;
-  uint16_t* to = layer + m.to * page_elements;
-  const int head_vectors = m.rows * a.head_dim / 8;   // of a head's rows in use
-  const int vectors = a.heads * head_vectors;
-  const int head_stride = a.page_rows * a.head_dim;
+  const Move m = a.moves[rest % a.count];
+  const uint16_t* from = a.pool.page(rest / a.count, m.from);
+  uint16_t* to = a.pool.page(rest / a.count, m.to);
   u32x4 v[4];
   int at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int vector = piece * kPieceVectors + i * 256 + threadIdx.x;
-    const int head = vector / head_vectors;
-    at[i] = vector < vectors ? head * head_stride + (vector - head * head_vectors) * 8 : -1;
-    if (at[i] >= 0) v[i] = *reinterpret_cast<const u32x4*>(from + at[i]);
+    at[i] = vector_at(a.pool, m.rows, piece, i);
+    if (at[i] >= 0) v[i] = load_nt(reinterpret_cast<const u32x4*>(from + at[i]));
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (at[i] >= 0) *reinterpret_cast<u32x4*>(to + at[i]) = v[i];
+    if (at[i] >= 0) store_nt(reinterpret_cast<u32x4*>(to + at[i]), v[i]);
+  }
+}
+
+struct Kid {
+  int32_t sequence, page;
+};
+
+struct ForkArgs {
+  Pool pool;
+  int32_t* tables;
+  int32_t* lengths;
+  int64_t width;
+  int parent, full, page, rows, count, pieces, groups;
+  Kid kids[OMNIA_PAGES_MOVES];
+};
+
+constexpr int kKidsAtOnce = 8;
+
+// A piece of the parent's last page, read once and written for eight children, a workgroup;
+// behind those one for each child's row of the table.
+__global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
+  const int copies = a.pieces * a.groups * a.pool.planes;
+  const int block = blockIdx.x;
+  if (block >= copies) {
+    const Kid kid = a.kids[block - copies];
+    const int32_t* source = a.tables + a.parent * a.width;
+    int32_t* row = a.tables + kid.sequence * a.width;
+    for (int64_t i = threadIdx.x; i < a.width; i += 256) row[i] = i < a.full ? source[i] : i == a.full ? kid.page : -1;
+    if (threadIdx.x == 0) a.lengths[kid.sequence] = a.lengths[a.parent];
+    return;
+  }
+  const int piece = block % a.pieces;
+  const int rest = block / a.pieces;
+  const int first = rest % a.groups * kKidsAtOnce, plane = rest / a.groups;
+  const uint16_t* from = a.pool.page(plane, a.page);
+  u32x4 v[4];
+  int at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    at[i] = vector_at(a.pool, a.rows, piece, i);
+    if (at[i] >= 0) v[i] = *reinterpret_cast<const u32x4*>(from + at[i]);
+  }
+  for (int kid = first; kid < min(first + kKidsAtOnce, a.count); ++kid) {
+    uint16_t* to = a.pool.page(plane, a.kids[kid].page);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (at[i] >= 0) store_nt(reinterpret_cast<u32x4*>(to + at[i]), v[i]);
+    }
   }
 }
 
 struct Edit {
-  int32_t kind, sequence, a, b, c;
+  int32_t kind, sequence, a, b;
 };
 
 struct EditArgs {
@@ -97,19 +163,15 @@ __global__ __launch_bounds__(256) void pages_edit_kernel(EditArgs a) {
     if (threadIdx.x == 0) a.lengths[e.sequence] = e.a;
     return;
   }
-  // A fork's row: `b` entries of sequence `a`, then page `c`. A cleared one has none.
-  const int32_t* source = a.tables + (e.kind == OMNIA_PAGES_FORK ? e.a : e.sequence) * a.width;
-  for (int64_t i = threadIdx.x; i < a.width; i += 256) row[i] = i < e.b ? source[i] : i == e.b ? e.c : -1;
-  if (threadIdx.x == 0) a.lengths[e.sequence] = e.kind == OMNIA_PAGES_FORK ? a.lengths[e.a] : 0;
+  for (int64_t i = threadIdx.x; i < a.width; i += 256) row[i] = -1;
+  if (threadIdx.x == 0) a.lengths[e.sequence] = 0;
 }
 
-// Whether one of two edits writes what the other writes or reads.
+// Whether two edits write one place.
 bool meet(const Edit& x, const Edit& y) {
-  const auto whole = [](const Edit& e) { return e.kind == OMNIA_PAGES_FORK || e.kind == OMNIA_PAGES_CLEAR; };
-  if (x.kind == OMNIA_PAGES_FORK && x.a == y.sequence) return true;
-  if (y.kind == OMNIA_PAGES_FORK && y.a == x.sequence) return true;
   if (x.sequence != y.sequence) return false;
-  return whole(x) || whole(y) || (x.kind == y.kind && (x.kind == OMNIA_PAGES_LENGTH || x.a == y.a));
+  if (x.kind == OMNIA_PAGES_CLEAR || y.kind == OMNIA_PAGES_CLEAR) return true;
+  return x.kind == y.kind && (x.kind == OMNIA_PAGES_LENGTH || x.a == y.a);
 }
 
 __global__ __launch_bounds__(256) void pages_advance_kernel(int32_t* lengths, const int32_t* sequences,
@@ -120,22 +182,44 @@ __global__ __launch_bounds__(256) void pages_advance_kernel(int32_t* lengths, co
   if (sequence >= 0 && sequence < all) lengths[sequence] += rows[i];
 }
 
-// A small set of page ids, open addressing: whether two moves meet is asked of at most
-// OMNIA_PAGES_MOVES ids, without an allocation that could fail.
-struct PageSet {
+// A small set of numbers, open addressing: whether two moves meet is asked of at most
+// OMNIA_PAGES_MOVES of them, without an allocation that could fail.
+struct SmallSet {
   static constexpr int kSlots = 4 * OMNIA_PAGES_MOVES;
   int32_t slots[kSlots];
-  PageSet() {
+  SmallSet() {
     for (int32_t& s : slots) s = -1;
   }
-  int find(int32_t page) const {
-    int at = static_cast<int>((static_cast<uint32_t>(page) * 2654435761u) >> 16) % kSlots;
-    while (slots[at] != -1 && slots[at] != page) at = (at + 1) % kSlots;
+  int find(int32_t number) const {
+    int at = static_cast<int>((static_cast<uint32_t>(number) * 2654435761u) >> 16) % kSlots;
+    while (slots[at] != -1 && slots[at] != number) at = (at + 1) % kSlots;
     return at;
   }
-  bool has(int32_t page) const { return slots[find(page)] == page; }
-  void add(int32_t page) { slots[find(page)] = page; }
+  bool has(int32_t number) const { return slots[find(number)] == number; }
+  void add(int32_t number) { slots[find(number)] = number; }
 };
+
+// A pool's checks; an error text, or null.
+const char* bad_pool(const uint16_t* keys, const uint16_t* values, int64_t layers, int64_t pages, int64_t kv_heads,
+                     int64_t page_rows, int64_t head_dim) {
+  if (layers <= 0 || layers > 65536 || pages <= 0 || pages >= (int64_t{1} << 31)) return "bad pool";
+  if (kv_heads <= 0 || kv_heads > 4096 || head_dim <= 0 || head_dim % 8 != 0 || head_dim > 2048 || page_rows <= 0 ||
+      page_rows > 4096 || kv_heads * page_rows * head_dim >= (int64_t{1} << 30)) {
+    return "bad page";
+  }
+  return keys && values && aligned16(keys) && aligned16(values) ? nullptr : "null or unaligned pointer";
+}
+
+Pool make_pool(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages, int64_t kv_heads, int64_t page_rows,
+               int64_t head_dim) {
+  return Pool{{keys, values}, pages * kv_heads * page_rows * head_dim, static_cast<int>(kv_heads),
+              static_cast<int>(page_rows), static_cast<int>(head_dim), static_cast<int>(2 * layers)};
+}
+
+bool bad_tables(int64_t sequences, int64_t width, int64_t pages) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  return sequences <= 0 || sequences >= kMost || width <= 0 || width >= kMost || pages <= 0 || pages >= kMost;
+}
 
 }  // namespace
 }  // namespace omnia
@@ -144,19 +228,15 @@ extern "C" int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t la
                                     int64_t page_rows, int64_t head_dim, const int32_t* moves, int64_t count,
                                     int32_t* tables, int64_t entries, hipStream_t stream) {
   using namespace omnia;
-  OMNIA_REQUIRE(layers > 0 && layers <= 65536 && pages > 0 && pages < (int64_t{1} << 31), "pages_copy: bad pool");
-  OMNIA_REQUIRE(kv_heads > 0 && kv_heads <= 4096 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= 1024 &&
-                    page_rows > 0 && page_rows <= 4096 && kv_heads * page_rows * head_dim < (int64_t{1} << 30),
-                "pages_copy: bad page");
   OMNIA_REQUIRE(count >= 0 && count <= OMNIA_PAGES_MOVES, "pages_copy: more moves than one call takes");
+  const char* bad = bad_pool(keys, values, layers, pages, kv_heads, page_rows, head_dim);
+  if (bad != nullptr) return fail(-EINVAL, std::string("pages_copy: ") + bad);
   if (count == 0) return 0;
-  OMNIA_REQUIRE(keys && values && moves && aligned16(keys) && aligned16(values),
-                "pages_copy: null or unaligned pointer");
+  OMNIA_REQUIRE(moves, "pages_copy: null pointer");
   OMNIA_REQUIRE(tables == nullptr || (entries >= 0 && entries < (int64_t{1} << 37)), "pages_copy: bad table");
-  CopyArgs a{{keys, values}, pages * kv_heads * page_rows * head_dim, tables, tables ? entries : 0,
-             static_cast<int>(kv_heads), static_cast<int>(page_rows), static_cast<int>(head_dim),
-             static_cast<int>(count), static_cast<int>(layers), 0, 0, {}};
-  PageSet written;
+  CopyArgs a{make_pool(keys, values, layers, pages, kv_heads, page_rows, head_dim), tables, tables ? entries : 0,
+             static_cast<int>(count), 0, 0, {}};
+  SmallSet written;
   int64_t most = 0;
   for (int64_t i = 0; i < count; ++i) {
     const Move m{moves[3 * i], moves[3 * i + 1], moves[3 * i + 2]};
@@ -174,7 +254,7 @@ extern "C" int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t la
   }
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
-  a.pieces = static_cast<int>((kv_heads * most * head_dim / 8 + kPieceVectors - 1) / kPieceVectors);
+  a.pieces = pieces_of(kv_heads, most, head_dim);
   const int64_t copies = a.pieces * count * layers * 2;
   const int64_t blocks = copies + (a.entries + 255) / 256;
   OMNIA_REQUIRE(blocks < (int64_t{1} << 31), "pages_copy: too many pieces for one launch");
@@ -183,28 +263,61 @@ extern "C" int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t la
   return launched("pages_copy");
 }
 
+extern "C" int32_t omnia_pages_fork(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages, int64_t kv_heads,
+                                    int64_t page_rows, int64_t head_dim, int32_t* tables, int32_t* lengths,
+                                    int64_t sequences, int64_t width, int64_t parent, int64_t full, int64_t page,
+                                    int64_t rows, const int32_t* kids, int64_t count, hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(count >= 0 && count <= OMNIA_PAGES_MOVES, "pages_fork: more children than one call takes");
+  const char* bad = bad_pool(keys, values, layers, pages, kv_heads, page_rows, head_dim);
+  if (bad != nullptr) return fail(-EINVAL, std::string("pages_fork: ") + bad);
+  OMNIA_REQUIRE(!bad_tables(sequences, width, pages), "pages_fork: bad tables");
+  OMNIA_REQUIRE(parent >= 0 && parent < sequences, "pages_fork: no such sequence");
+  OMNIA_REQUIRE(full >= 0 && full <= width && rows >= 0 && rows <= page_rows, "pages_fork: rows outside the table or page");
+  OMNIA_REQUIRE(rows == 0 || (full < width && page >= 0 && page < pages), "pages_fork: no such page");
+  if (count == 0) return 0;
+  OMNIA_REQUIRE(tables && lengths && kids, "pages_fork: null pointer");
+  ForkArgs a{make_pool(keys, values, layers, pages, kv_heads, page_rows, head_dim), tables, lengths, width,
+             static_cast<int>(parent), static_cast<int>(full), static_cast<int>(page), static_cast<int>(rows),
+             static_cast<int>(count), 0, static_cast<int>((count + kKidsAtOnce - 1) / kKidsAtOnce), {}};
+  SmallSet named, written;
+  for (int64_t i = 0; i < count; ++i) {
+    const Kid kid{kids[2 * i], kids[2 * i + 1]};
+    OMNIA_REQUIRE(kid.sequence >= 0 && kid.sequence < sequences && kid.sequence != parent && !named.has(kid.sequence),
+                  "pages_fork: a child is no other sequence, or named twice");
+    OMNIA_REQUIRE(rows == 0 ? kid.page == -1 : kid.page >= 0 && kid.page < pages && kid.page != page &&
+                                                   !written.has(kid.page),
+                  "pages_fork: a child's page is no other page, or named twice");
+    named.add(kid.sequence);
+    if (rows != 0) written.add(kid.page);
+    a.kids[i] = kid;
+  }
+  int32_t rc = check_device(stream);
+  if (rc != 0) return rc;
+  a.pieces = pieces_of(kv_heads, rows, head_dim);
+  const int64_t blocks = static_cast<int64_t>(a.pieces) * a.groups * a.pool.planes + count;
+  OMNIA_REQUIRE(blocks < (int64_t{1} << 31), "pages_fork: too many pieces for one launch");
+  pages_fork_kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
+  return launched("pages_fork");
+}
+
 extern "C" int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t sequences, int64_t width, int64_t pages,
                                     const int32_t* edits, int64_t count, hipStream_t stream) {
   using namespace omnia;
-  OMNIA_REQUIRE(sequences > 0 && sequences < (int64_t{1} << 31) && width > 0 && width < (int64_t{1} << 31) &&
-                    pages > 0 && pages < (int64_t{1} << 31),
-                "pages_edit: bad tables");
+  OMNIA_REQUIRE(!bad_tables(sequences, width, pages), "pages_edit: bad tables");
   OMNIA_REQUIRE(count >= 0 && count <= OMNIA_PAGES_EDITS, "pages_edit: more edits than one call takes");
   if (count == 0) return 0;
   OMNIA_REQUIRE(tables && lengths && edits, "pages_edit: null pointer");
   EditArgs a{tables, lengths, width, {}};
   for (int64_t i = 0; i < count; ++i) {
-    const Edit e{edits[5 * i], edits[5 * i + 1], edits[5 * i + 2], edits[5 * i + 3], edits[5 * i + 4]};
+    const Edit e{edits[4 * i], edits[4 * i + 1], edits[4 * i + 2], edits[4 * i + 3]};
     OMNIA_REQUIRE(e.sequence >= 0 && e.sequence < sequences, "pages_edit: no such sequence");
     if (e.kind == OMNIA_PAGES_ENTRY) {
       OMNIA_REQUIRE(e.a >= 0 && e.a < width && e.b >= -1 && e.b < pages, "pages_edit: no such entry or page");
     } else if (e.kind == OMNIA_PAGES_LENGTH) {
       OMNIA_REQUIRE(e.a >= 0, "pages_edit: a length below zero");
-    } else if (e.kind == OMNIA_PAGES_FORK) {
-      OMNIA_REQUIRE(e.a >= 0 && e.a < sequences && e.a != e.sequence, "pages_edit: no such sequence to fork");
-      OMNIA_REQUIRE(e.b >= 0 && e.b <= width && e.c >= -1 && e.c < pages, "pages_edit: no such entry or page");
     } else {
-      OMNIA_REQUIRE(e.kind == OMNIA_PAGES_CLEAR && e.b == 0 && e.c == -1, "pages_edit: no such edit");
+      OMNIA_REQUIRE(e.kind == OMNIA_PAGES_CLEAR, "pages_edit: no such edit");
     }
     for (int64_t j = 0; j < i; ++j) OMNIA_REQUIRE(!meet(a.edits[j], e), "pages_edit: two edits of one place");
     a.edits[i] = e;

@@ -149,16 +149,7 @@ class DefaultBatchAttentionStep(BatchAttentionStepStrategy):
         return self._attend(batch, self.project(batch, raw_queries, raw_keys, raw_values))
 
 
-def _readable(raw: torch.Tensor) -> torch.Tensor:
-    """The rows, copied where the kernel could not read them in place."""
-    stride = raw.stride(-2)
-    if (raw.stride(-1) != 1 or (raw.shape[-2] > 1 and (stride % 8 or stride < raw.shape[-1]))
-            or raw.data_ptr() % 16):
-        raw = raw.clone(memory_format=torch.contiguous_format)
-    return raw
-
-
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class HipBatchAttentionStep(BatchAttentionStepStrategy):
     core: DefaultBatchAttentionStep
 
@@ -200,55 +191,48 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
             self.core.angles.ensure(rows - 1)
         batch.tiles(self.core.heads // self.core.kv_heads)
 
-    def _angles(self, last: int):
-        """The (cos, sin) tables, covering positions [0, last)."""
-        core = self.core
-        if not core.rotary_pairs:
-            return None
-        table = core.angles
-        if isinstance(table, AngleAtlas):
-            if last > table.rows and not _capturing(table.atlas.device):
-                table.ensure(last - 1)
-            table = table.table()
-        return table.cos, table.sin
-
-    def _project(self, batch: PagedBatch, raw_queries, raw_keys, raw_values, wide: bool) -> tuple[torch.Tensor, int]:
+    def _plan(self, batch: PagedBatch) -> tuple[ops.BatchStepPlan, int]:
+        """The batch's plan of this layer, and the most rows a sequence has in the step."""
         core, cache = self.core, self.core.cache
         last = cache.ready(batch)
-        angles = self._angles(last)
-        if angles is not None and angles[0].shape[0] < last:
-            raise ValueError(f"a step that may reach position {last - 1} is past the angle table's "
-                             f"{angles[0].shape[0]} rows")
-        queries = ops.attention_batch_project(
-            _readable(raw_queries), _readable(raw_keys), _readable(raw_values), core.query_weight, core.key_weight,
-            angles, cache.keys[core.layer], cache.values[core.layer], cache.tables, cache.lengths, batch.token_map,
-            heads=core.heads, eps=core.eps, mscale=core.mscale, wide_queries=wide)
-        return queries, last
+        plan, pool = batch.plans.get(self, (None, None))
+        if plan is None or pool is not cache.keys or (core.rotary_pairs and last > plan.angle_rows):
+            angles = None
+            if core.rotary_pairs:
+                table = core.angles
+                if isinstance(table, AngleAtlas):
+                    if not _capturing(cache.keys.device):
+                        table.ensure(last - 1)   # grown past its last row
+                    table = table.table()
+                angles = table.cos, table.sin
+                if table.cos.shape[0] < last:
+                    raise ValueError(f"a step that may reach position {last - 1} is past the angle table's "
+                                     f"{table.cos.shape[0]} rows")
+            plan = ops.BatchStepPlan(
+                core.query_weight, core.key_weight, angles, cache.keys[core.layer], cache.values[core.layer],
+                cache.tables, cache.lengths, batch.token_map, batch.tiles(core.heads // core.kv_heads),
+                heads=core.heads, prefix=batch.prefix, scale=core.scale, eps=core.eps, mscale=core.mscale,
+                sinks=core.sinks)
+            batch.plans[self] = plan, cache.keys
+        return plan, last
 
     def _followed(self, *raw: torch.Tensor) -> bool:
         """A call that autograd follows, for the torch ops."""
-        if torch.is_grad_enabled() and any(t.requires_grad for t in raw):
+        if torch.is_grad_enabled() and (raw[0].requires_grad or raw[1].requires_grad or raw[2].requires_grad):
             record_fallback(self, self.core)
             return True
         return False
 
     def project(self, batch, raw_queries, raw_keys, raw_values):
-        core = self.core
-        _check_rows(batch, raw_queries, core.heads * core.head_dim, "raw_queries")
         if self._followed(raw_queries, raw_keys, raw_values):
-            return core.project(batch, raw_queries, raw_keys, raw_values)
-        return self._project(batch, raw_queries, raw_keys, raw_values, False)[0]
+            return self.core.project(batch, raw_queries, raw_keys, raw_values)
+        return self._plan(batch)[0].project(raw_queries, raw_keys, raw_values)
 
     def __call__(self, batch, raw_queries, raw_keys, raw_values):
-        core, cache = self.core, self.core.cache
-        _check_rows(batch, raw_queries, core.heads * core.head_dim, "raw_queries")
         if self._followed(raw_queries, raw_keys, raw_values):
-            return core(batch, raw_queries, raw_keys, raw_values)
-        tiles = batch.tiles(core.heads // core.kv_heads)
-        queries, last = self._project(batch, raw_queries, raw_keys, raw_values, True)
-        return ops.attention_batch(
-            queries, cache.keys[core.layer], cache.values[core.layer], cache.tables, cache.lengths, batch.token_map,
-            tiles, prefix=batch.prefix, own_rows=last - batch.prefix, scale=core.scale, sinks=core.sinks)
+            return self.core(batch, raw_queries, raw_keys, raw_values)
+        plan, last = self._plan(batch)
+        return plan(raw_queries, raw_keys, raw_values, last - batch.prefix)
 
 
 _STRATEGIES = (HipBatchAttentionStep, DefaultBatchAttentionStep)

@@ -60,7 +60,7 @@ class PagedBatch:
         self.counts = np.asarray(tokens, dtype=np.int64)
         self.ends = np.cumsum(self.counts)
         self.generation = cache._generation[self.index].copy()
-        self.ready = False            # the pages of the step at hand are there
+        self.clock = -1               # the cache's, at which the step's pages were made sure of
         self.reach = 0                # the most rows that captured steps were prepared for
         device = cache.keys.device
         whose = np.repeat(self.index, self.counts)
@@ -68,6 +68,9 @@ class PagedBatch:
         upload = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)  # noqa: E731
         self.token_map = upload(np.stack([whose, which], axis=1))
         self.chosen, self.rows = upload(self.index), upload(self.counts)
+        self.epoch = cache._epoch     # at which its sequences were last seen to be the same
+        self.last = 0                 # the most rows a sequence has in the step at hand
+        self.plans: dict = {}         # what a layer's binding laid out for the batch
         self._tiles: dict[int, torch.Tensor] = {}
 
     def tiles(self, group: int) -> torch.Tensor:
@@ -111,6 +114,7 @@ class PagedKVCache:
         elif lengths is None or opened is None:
             raise ValueError("PagedKVCache: tables need lengths and opened")
         self.keys, self.values = keys, values
+        self._hip = hip_device(keys)
         self._tables = np.array(tables, dtype=np.int32)
         self._rows = np.array(lengths, dtype=np.int64)
         self._open = np.zeros(len(self._tables), dtype=bool)
@@ -119,7 +123,9 @@ class PagedKVCache:
         self._check_tables()
         self._refs = np.zeros(pages, dtype=np.int64)
         np.add.at(self._refs, self._tables[self._tables >= 0], 1)
-        self._generation = np.zeros(len(self._tables), dtype=np.int64)
+        self._generation = np.zeros(len(self._tables), dtype=np.int64)   # of a slot: whose it is
+        self._epoch = 0                                                  # of them all
+        self._clock = 0                                                  # turns as sequences grow
         self.tables = torch.from_numpy(self._tables.copy()).to(keys.device)
         self.lengths = torch.from_numpy(self._rows.astype(np.int32)).to(keys.device)
 
@@ -177,32 +183,43 @@ class PagedKVCache:
         if _capturing(self.keys.device):
             raise ValueError(f"PagedKVCache: {what} cannot be captured (a replay would not repeat the host's part)")
 
-    def _edit(self, edits: list[tuple[int, int, int, int, int]]) -> None:
-        if not edits:
+    def _edit(self, edits) -> None:
+        if not len(edits):
             return
-        if hip_device(self.keys):
+        if self._hip:
             ops.pages_edit(self.tables, self.lengths, self.pages, edits)
             return
-        for kind, s, a, b, c in edits:
+        for kind, s, a, b in np.asarray(edits).tolist():
             if kind == ops.PAGES_ENTRY:
                 self.tables[s, a] = b
             elif kind == ops.PAGES_LENGTH:
                 self.lengths[s] = a
             else:
-                row = torch.full_like(self.tables[s], -1)
-                if kind == ops.PAGES_FORK:
-                    row[:b] = self.tables[a, :b]
-                    if c >= 0:
-                        row[b] = c
-                self.tables[s] = row
-                self.lengths[s] = self.lengths[a] if kind == ops.PAGES_FORK else 0
+                self.tables[s], self.lengths[s] = -1, 0
 
-    def _copy(self, moves: list[tuple[int, int, int]], rename: bool = False) -> None:
-        if not moves:
+    def _fork(self, parent: int, full: int, rows: int, kids: np.ndarray) -> None:
+        """Rows of the table for the kids (sequence, page), and `rows` rows of the parent's last
+        page for each."""
+        page = int(self._tables[parent, full]) if rows else -1
+        if self._hip:
+            ops.pages_fork(self.keys, self.values, self.tables, self.lengths, parent, full, page, rows, kids)
             return
-        if hip_device(self.keys):
+        if rows:
+            self._copy([(page, to, rows) for _, to in kids.tolist()])
+        for kid, to in kids.tolist():
+            self.tables[kid] = -1
+            self.tables[kid, :full] = self.tables[parent, :full]
+            if rows:
+                self.tables[kid, full] = to
+            self.lengths[kid] = self.lengths[parent]
+
+    def _copy(self, moves, rename: bool = False) -> None:
+        if not len(moves):
+            return
+        if self._hip:
             ops.pages_copy(self.keys, self.values, moves, tables=self.tables if rename else None)
             return
+        moves = np.asarray(moves).tolist()
         for pool in (self.keys, self.values):
             for source, target, rows in moves:
                 pool[:, target, :, :rows] = pool[:, source, :, :rows]
@@ -216,6 +233,11 @@ class PagedKVCache:
         for s in sequences:
             if not 0 <= s < len(self._open) or not self._open[s]:
                 raise ValueError(f"PagedKVCache: sequence {s} is not open")
+
+    def _renew(self, sequences) -> None:
+        """The sequences are others now: batches of the ones before are refused."""
+        self._generation[sequences] += 1
+        self._epoch += 1
 
     def _take(self, count: int) -> np.ndarray:
         """The lowest `count` free pages, still free."""
@@ -249,13 +271,21 @@ class PagedKVCache:
         (s,) = self._slots(1)
         fresh = self._take(pages)
         self._open[s] = True
-        self._generation[s] += 1
+        self._renew(s)
         self._refs[fresh] = 1
         self._tables[s, :pages] = fresh
         self._held[s], self._rows[s] = pages, rows
-        edits = [(ops.PAGES_ENTRY, s, i, page, 0) for i, page in enumerate(fresh.tolist())]
-        self._edit(edits + ([(ops.PAGES_LENGTH, s, rows, 0, 0)] if rows else []))
+        self._edit(self._entries(s, 0, fresh) if not rows else
+                   np.concatenate([self._entries(s, 0, fresh), [(ops.PAGES_LENGTH, s, rows, 0)]]))
         return s
+
+    @staticmethod
+    def _entries(sequence: int, first: int, pages: np.ndarray) -> np.ndarray:
+        """The edits that make `pages` a sequence's entries from `first` on."""
+        edits = np.empty((len(pages), 4), dtype=np.int32)
+        edits[:, 0], edits[:, 1], edits[:, 3] = ops.PAGES_ENTRY, sequence, pages
+        edits[:, 2] = np.arange(first, first + len(pages))
+        return edits
 
     def _reserve(self, index: np.ndarray, rows: np.ndarray) -> None:
         """Pages for `rows` rows of each sequence, and one of its own where it writes next."""
@@ -282,7 +312,7 @@ class PagedKVCache:
         for i, page in zip(copied, fresh.tolist()):
             s, old = int(index[i]), int(self._tables[index[i], at[i]])
             moves.append((old, page, int(now[i] % size)))
-            edits.append((ops.PAGES_ENTRY, s, int(at[i]), page, 0))
+            edits.append((ops.PAGES_ENTRY, s, int(at[i]), page))
             self._tables[s, at[i]] = page
             self._refs[old] -= 1
         self._refs[fresh] = 1
@@ -291,7 +321,7 @@ class PagedKVCache:
             s = int(index[i])
             for entry in range(self._held[s], self._held[s] + int(more[i])):
                 self._tables[s, entry] = page = next(rest)
-                edits.append((ops.PAGES_ENTRY, s, entry, page, 0))
+                edits.append((ops.PAGES_ENTRY, s, entry, page))
             self._held[s] += int(more[i])
         self._copy(moves)
         self._edit(edits)
@@ -320,23 +350,20 @@ class PagedKVCache:
         self._refs[fresh.reshape(-1)] = 1
         self._refs[parent[:full]] += count
         self._open[kids] = True
-        self._generation[kids] += 1
+        self._renew(kids)
         self._tables[kids, :full] = parent[:full]
         self._tables[kids, full : full + each] = fresh
         self._held[kids], self._rows[kids] = full + each, rows
-        if each:
-            heads = parent[full : full + each].tolist()
-            used = [size] * (each - 1) + [rest - size * (each - 1)]
-            self._copy([(page, to, n) for line in fresh.tolist() for page, to, n in zip(heads, line, used)])
         if share:
-            last = fresh[:, 0].tolist() if each else [-1] * count
-            self._edit([(ops.PAGES_FORK, kid, sequence, full, page) for kid, page in zip(kids, last)])
+            self._fork(sequence, full, rest, np.stack(
+                [kids, fresh[:, 0] if each else np.full(count, -1)], axis=1).astype(np.int32))
         else:
-            edits = []
-            for kid, line in zip(kids, fresh.tolist()):
-                edits += [(ops.PAGES_ENTRY, kid, i, page, 0) for i, page in enumerate(line)]
-                edits.append((ops.PAGES_LENGTH, kid, rows, 0, 0))
-            self._edit(edits)
+            used = np.full((count, each), size)
+            used[:, -1:] = rest - size * (each - 1)
+            self._copy(np.stack([np.broadcast_to(parent[:each], (count, each)), fresh, used], axis=-1).reshape(-1, 3))
+            self._edit(np.concatenate([np.empty((0, 4), dtype=np.int32)] + [
+                edits for kid, line in zip(kids, fresh)
+                for edits in (self._entries(kid, 0, line), [(ops.PAGES_LENGTH, kid, rows, 0)])]))
         return kids
 
     def free(self, sequences: Sequence[int] | int) -> None:
@@ -353,8 +380,10 @@ class PagedKVCache:
         self._tables[gone] = -1
         self._held[gone] = self._rows[gone] = 0
         self._open[gone] = False
-        self._generation[gone] += 1
-        self._edit([(ops.PAGES_CLEAR, s, 0, 0, -1) for s in gone])
+        self._renew(gone)
+        edits = np.zeros((len(gone), 4), dtype=np.int32)
+        edits[:, 0], edits[:, 1] = ops.PAGES_CLEAR, gone
+        self._edit(edits)
 
     def truncate(self, sequence: int, rows: int) -> None:
         """Drop the sequence's rows from `rows` on (a rejected guess), and the pages past them."""
@@ -363,13 +392,13 @@ class PagedKVCache:
         if not 0 <= rows <= self._rows[sequence]:
             raise ValueError(f"PagedKVCache: sequence {sequence} holds {self._rows[sequence]} rows, not {rows}")
         keep = self._pages_for(rows)
-        gone = range(keep, int(self._held[sequence]))
+        gone = int(self._held[sequence]) - keep
         self._refs[self._tables[sequence, keep : self._held[sequence]]] -= 1
         self._tables[sequence, keep:] = -1
         self._held[sequence], self._rows[sequence] = keep, rows
-        self._generation[sequence] += 1
-        self._edit([(ops.PAGES_ENTRY, sequence, i, -1, 0) for i in gone]
-                   + [(ops.PAGES_LENGTH, sequence, rows, 0, 0)])
+        self._renew(sequence)
+        self._edit(np.concatenate([self._entries(sequence, keep, np.full(gone, -1)),
+                                   [(ops.PAGES_LENGTH, sequence, rows, 0)]]))
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool, each that lies behind them to the
@@ -384,7 +413,7 @@ class PagedKVCache:
             names[-1], names[source] = -1, target
             self._tables = names[self._tables]
             self._refs[target], self._refs[source] = self._refs[source], 0
-            self._copy([(a, b, self.page_rows) for a, b in zip(source.tolist(), target.tolist())], rename=True)
+            self._copy(np.stack([source, target, np.full(len(source), self.page_rows)], axis=1), rename=True)
         return live
 
     def resize(self, pages: int) -> None:
@@ -428,18 +457,20 @@ class PagedKVCache:
     def _current(self, batch: PagedBatch) -> None:
         if batch.cache is not self:
             raise ValueError("PagedKVCache: the batch belongs to another cache")
-        if not np.array_equal(self._generation[batch.index], batch.generation):
-            raise ValueError("PagedKVCache: a sequence of the batch was freed or truncated; make a new batch")
+        if batch.epoch != self._epoch:
+            if not np.array_equal(self._generation[batch.index], batch.generation):
+                raise ValueError("PagedKVCache: a sequence of the batch was freed or truncated; make a new batch")
+            batch.epoch = self._epoch
 
     def ready(self, batch: PagedBatch) -> int:
         """Make sure of the pages of the batch's step; the most rows any of its sequences has
         then, or may have in the replays that were prepared for."""
         self._current(batch)
-        if not batch.ready:
-            self._reserve(batch.index, self._rows[batch.index] + batch.counts)
-            batch.ready = True
-        last = int((self._rows[batch.index] + batch.counts).max())
-        return max(last, batch.reach) if _capturing(self.keys.device) else last
+        if batch.clock != self._clock:
+            rows = self._rows[batch.index] + batch.counts
+            self._reserve(batch.index, rows)
+            batch.clock, batch.last = self._clock, int(rows.max())
+        return max(batch.last, batch.reach) if batch.reach and _capturing(self.keys.device) else batch.last
 
     def prepare_capture(self, batch: PagedBatch, steps: int) -> int:
         """Reserve the pages of the batch's next `steps` steps, before a step and its `advance`
@@ -450,7 +481,8 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: a captured step is replayed at least once")
         rows = self._rows[batch.index] + steps * batch.counts
         self._reserve(batch.index, rows)
-        batch.ready, batch.reach = True, int(rows.max())
+        batch.reach = int(rows.max())
+        self.ready(batch)
         return batch.reach
 
     def advance(self, batch: PagedBatch) -> None:
@@ -459,7 +491,7 @@ class PagedKVCache:
         self._current(batch)
         if not _capturing(self.keys.device):
             self.account(batch, 1)
-        if hip_device(self.keys):
+        if self._hip:
             ops.pages_advance(self.lengths, batch.chosen, batch.rows)
         else:
             self.lengths[batch.chosen.long()] += batch.rows
@@ -471,4 +503,4 @@ class PagedKVCache:
         if steps < 0 or (rows > self._held[batch.index] * self.page_rows).any():
             raise ValueError("PagedKVCache: more steps than the pages hold")
         self._rows[batch.index] = rows
-        batch.ready = False
+        self._clock += 1

@@ -21,6 +21,20 @@ _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F32 = ctypes.c_float
 
+
+class BatchStep(ctypes.Structure):
+    """`omnia_attention_batch_step_t`; must match include/omnia_hip.h."""
+
+    _fields_ = ([(name, _P) for name in (
+        "raw_queries", "raw_keys", "raw_values", "query_weight", "key_weight", "cos_rows", "sin_rows", "keys",
+        "values", "tables", "lengths", "token_map", "tiles", "sinks", "queries", "out", "workspace")]
+        + [(name, _I64) for name in (
+            "workspace_bytes", "query_stride", "key_stride", "value_stride", "table_stride", "angle_rows",
+            "rotary_pairs", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_rows", "sequences", "width",
+            "own_tiles", "prefix", "own_rows")]
+        + [(name, _F32) for name in ("mscale", "eps", "scale")])
+
+
 # name -> (restype, argtypes); must match include/omnia_hip.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_abi_version": (_I32, []),
@@ -98,6 +112,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_attention_prefill": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _P, _I64,
                                        _P, _F32, _P, _I64, _P, _P]),
     "omnia_pages_copy": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "omnia_pages_fork": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
+                                _I64, _P]),
     "omnia_pages_edit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "omnia_pages_advance": (_I32, [_P, _I64, _P, _P, _I64, _P]),
     "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
@@ -106,6 +122,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_attention_batch_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "omnia_attention_batch": (_I32, [_P, _I32, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
                                      _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
+    "omnia_attention_batch_step_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "omnia_attention_batch_step": (_I32, [_P, _P]),
     "omnia_embed_atlas": (
         _I32,
         [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P],

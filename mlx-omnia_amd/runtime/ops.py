@@ -12,9 +12,10 @@ from __future__ import annotations
 import ctypes
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
-from .loader import call, last_error, library
+from .loader import BatchStep, call, last_error, library
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -1156,18 +1157,35 @@ def attention_prefill(
     return out
 
 
-PAGES_MOVES, PAGES_EDITS = 256, 128   # OMNIA_PAGES_MOVES, OMNIA_PAGES_EDITS
-PAGES_ENTRY, PAGES_LENGTH, PAGES_FORK, PAGES_CLEAR = 0, 1, 2, 3
+PAGES_MOVES, PAGES_EDITS = 128, 128   # OMNIA_PAGES_MOVES, OMNIA_PAGES_EDITS
+PAGES_ENTRY, PAGES_LENGTH, PAGES_CLEAR = 0, 1, 2
 
 
-def _int_lines(lines, width: int, name: str):
-    """Lists of `width` whole numbers that fit 32 bits, as one array the library reads."""
-    flat = [int(n) for line in lines for n in line]
-    if len(flat) != width * len(lines):
-        raise ValueError(f"{name}: every one is {width} numbers")
-    if flat and not (-(1 << 31) <= min(flat) and max(flat) < 1 << 31):
-        raise ValueError(f"{name}: a number outside 32 bits")
-    return (ctypes.c_int32 * len(flat))(*flat)
+def _int_lines(lines, width: int, name: str) -> np.ndarray:
+    """Lines of `width` whole numbers that fit 32 bits, as the library reads them."""
+    try:
+        array = np.asarray(lines)
+        if array.dtype != np.int32:
+            if array.size and (array.dtype.kind not in "iu" or array.min() < -(1 << 31) or array.max() >= 1 << 31):
+                raise ValueError
+            array = array.astype(np.int32)
+    except (ValueError, OverflowError):
+        raise ValueError(f"{name}: whole numbers of 32 bits, {width} a line") from None
+    if array.size and (array.ndim != 2 or array.shape[1] != width):
+        raise ValueError(f"{name}: whole numbers of 32 bits, {width} a line")
+    return np.ascontiguousarray(array).reshape(-1, width)
+
+
+def _pool(keys: torch.Tensor, values: torch.Tensor, name: str) -> tuple[int, int, int, int, int]:
+    """(layers, pages, kv_heads, page_rows, 16-bit words of a row) of a pool of any type."""
+    _require(keys.dim() == 5 and keys.shape == values.shape and keys.dtype == values.dtype,
+             name + ": keys and values must be [layers, pages, kv_heads, page_rows, head_dim]")
+    _dense(keys, keys.dtype, "keys")
+    _dense(values, keys.dtype, "values")
+    layers, pages, kv_heads, page_rows, head_dim = keys.shape
+    width = head_dim * keys.element_size()
+    _require(width % 16 == 0, name + ": rows must be whole 16-byte vectors")
+    return layers, pages, kv_heads, page_rows, width // 2
 
 
 def _page_tables(tables: torch.Tensor, lengths: torch.Tensor, name: str) -> tuple[int, int]:
@@ -1182,43 +1200,53 @@ def pages_copy(keys: torch.Tensor, values: torch.Tensor, moves, *, tables: torch
     layer: moves are (from, to, rows), rows the first of the page that are copied. No page may
     be written twice, or read and written. With `tables` (int32, on the device) the entries
     that name a page left are renamed, and moves are sorted by it; see `omnia_pages_copy`."""
-    _require(keys.dim() == 5 and keys.shape == values.shape and keys.dtype == values.dtype,
-             "pages_copy: keys and values must be [layers, pages, kv_heads, page_rows, head_dim]")
-    for pool, name in ((keys, "keys"), (values, "values")):
-        _dense(pool, keys.dtype, name)
-    layers, pages, kv_heads, page_rows, head_dim = keys.shape
-    width = head_dim * keys.element_size()
-    _require(width % 16 == 0, "pages_copy: rows must be whole 16-byte vectors")
+    pool = _pool(keys, values, "pages_copy")
     tensors = [keys, values]
     if tables is not None:
         _require(tables.dtype == torch.int32 and tables.is_contiguous(), "pages_copy: tables must be contiguous int32")
         tensors.append(tables)
     _require(on_rocm(*tensors), "pages_copy: tensors must share one ROCm device")
-    moves = list(moves)
+    moves = _int_lines(moves, 3, "moves")
     if len(moves) > PAGES_MOVES:   # within one call the library asks this itself
-        written = {to for _, to, _ in moves}
-        if len(written) < len(moves) or not written.isdisjoint(source for source, _, _ in moves):
+        if len(np.unique(moves[:, 1])) < len(moves) or np.isin(moves[:, 1], moves[:, 0]).any():
             raise ValueError("pages_copy: a page is written twice, or both read and written")
-        if tables is not None and any(a[0] >= b[0] for a, b in zip(moves, moves[1:])):
+        if tables is not None and (np.diff(moves[:, 0]) <= 0).any():
             raise ValueError("pages_copy: moves that rename have to be sorted by the page they leave")
     stream = _stream(keys)
     for first in range(0, len(moves), PAGES_MOVES):
         some = moves[first : first + PAGES_MOVES]
-        call("omnia_pages_copy", keys.data_ptr(), values.data_ptr(), layers, pages, kv_heads, page_rows, width // 2,
-             _int_lines(some, 3, "moves"), len(some), tables.data_ptr() if tables is not None else None,
-             tables.numel() if tables is not None else 0, stream)
+        call("omnia_pages_copy", keys.data_ptr(), values.data_ptr(), *pool, some.ctypes.data, len(some),
+             tables.data_ptr() if tables is not None else None, tables.numel() if tables is not None else 0, stream)
+
+
+def pages_fork(keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, parent: int,
+               full: int, page: int, rows: int, kids) -> None:
+    """Make sequences the children of `parent`, each a (sequence, page) of kids: they share its
+    first `full` pages and get the first `rows` rows of `page` copied; see `omnia_pages_fork`."""
+    pool = _pool(keys, values, "pages_fork")
+    sequences, width = _page_tables(tables, lengths, "pages_fork")
+    _require(on_rocm(keys, values, tables, lengths), "pages_fork: tensors must share one ROCm device")
+    kids = _int_lines(kids, 2, "kids")
+    if len(kids) > PAGES_MOVES and (len(np.unique(kids[:, 0])) < len(kids)
+                                    or (rows and len(np.unique(kids[:, 1])) < len(kids))):
+        raise ValueError("pages_fork: a child or a page is named twice")
+    stream = _stream(keys)
+    for first in range(0, len(kids), PAGES_MOVES):
+        some = kids[first : first + PAGES_MOVES]
+        call("omnia_pages_fork", keys.data_ptr(), values.data_ptr(), *pool, tables.data_ptr(), lengths.data_ptr(),
+             sequences, width, parent, full, page, rows, some.ctypes.data, len(some), stream)
 
 
 def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -> None:
-    """Edits of page tables on the device, each (kind, sequence, a, b, c); see
-    `omnia_pages_edit`. More than PAGES_EDITS are made in turn, as many at a time."""
+    """Edits of page tables on the device, each (kind, sequence, a, b); see `omnia_pages_edit`.
+    More than PAGES_EDITS are made in turn, as many at a time."""
     sequences, width = _page_tables(tables, lengths, "pages_edit")
     _require(on_rocm(tables, lengths), "pages_edit: tensors must share one ROCm device")
-    edits, stream = list(edits), _stream(tables)
+    edits, stream = _int_lines(edits, 4, "edits"), _stream(tables)
     for first in range(0, len(edits), PAGES_EDITS):
         some = edits[first : first + PAGES_EDITS]
         call("omnia_pages_edit", tables.data_ptr(), lengths.data_ptr(), sequences, width, pages,
-             _int_lines(some, 5, "edits"), len(some), stream)
+             some.ctypes.data, len(some), stream)
 
 
 def pages_advance(lengths: torch.Tensor, chosen: torch.Tensor, rows: torch.Tensor) -> None:
@@ -1353,6 +1381,103 @@ def attention_batch(
          sinks.data_ptr() if sinks is not None else None, float(scale),
          workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
     return out
+
+
+class BatchStepPlan:
+    """A layer's step of one batch, its arguments checked and laid out once for
+    `omnia_attention_batch_step`: what stays the same from step to step. Calling it with the raw
+    rows and `own_rows` gives the context [N, heads, D] bf16, `project` the queries alone. The
+    arguments are those of `attention_batch_project` and `attention_batch`."""
+
+    def __init__(self, query_weight, key_weight, angles, keys, values, tables, lengths, token_map, tiles, *, heads: int,
+                 prefix: int, scale: float, eps: float, mscale: float = 1.0, sinks=None) -> None:
+        pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch_step")
+        sequences, width = _page_tables(tables, lengths, "attention_batch_step")
+        tokens = token_map.shape[0]
+        _token_map(token_map, tokens, "attention_batch_step")
+        _require(tiles.dtype == torch.int32 and tiles.is_contiguous() and tiles.dim() == 2 and tiles.shape[1] == 4,
+                 "attention_batch_step: tiles must be contiguous int32 [n, 4]")
+        held = [keys, values, tables, lengths, token_map, tiles]
+        for weight, name in ((query_weight, "query_weight"), (key_weight, "key_weight")):
+            if weight is not None:
+                _dense(weight, BF16, name)
+                if not (weight.numel() == head_dim):
+                    raise ValueError(f"{name}: must be [head_dim]")
+                held.append(weight)
+        if sinks is not None:
+            _require(sinks.dtype == BF16 and sinks.is_contiguous() and sinks.numel() == heads,
+                     "attention_batch_step: sinks must be contiguous bf16 [heads]")
+            held.append(sinks)
+        cos = sin = None
+        if angles is not None:
+            cos, sin = angles
+            for rows, name in ((cos, "cos"), (sin, "sin")):
+                if not (rows.dtype == F32 and rows.dim() == 2 and rows.shape == cos.shape and rows.stride(-1) == 1
+                        and rows.stride() == cos.stride() and rows.data_ptr() % 16 == 0):
+                    raise ValueError(f"{name}: fp32 [positions, pairs], 16-byte aligned with unit inner stride")
+            held += [cos, sin]
+        _require(on_rocm(*held), "attention_batch_step: tensors must share one ROCm device")
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        self.held, self.index = held, keys.get_device()
+        self.device = keys.device
+        self.angle_rows = cos.shape[0] if cos is not None else None
+        self.tokens, self.heads, self.kv_heads, self.head_dim = tokens, heads, kv_heads, head_dim
+        self.args = BatchStep(
+            query_weight=ptr(query_weight), key_weight=ptr(key_weight), cos_rows=ptr(cos), sin_rows=ptr(sin),
+            keys=keys.data_ptr(), values=values.data_ptr(), tables=tables.data_ptr(), lengths=lengths.data_ptr(),
+            token_map=token_map.data_ptr(), tiles=tiles.data_ptr(), sinks=ptr(sinks),
+            table_stride=0 if cos is None else cos.stride(0) if cos.shape[0] > 1 else cos.shape[1],
+            angle_rows=self.angle_rows or 0, rotary_pairs=0 if cos is None else cos.shape[1], tokens=tokens,
+            heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=pages, page_rows=page_rows, sequences=sequences,
+            width=width, own_tiles=tiles.shape[0], prefix=prefix, own_rows=-1, mscale=mscale, eps=eps, scale=scale)
+        self.sized = -1, 0   # own rows, and the workspace that they need
+
+    def _rows(self, raw: torch.Tensor, width: int, name: str) -> tuple[int, int, torch.Tensor]:
+        """(address, stride, the tensor that holds them) of the raw rows, copied where the kernel
+        could not read them in place."""
+        shape = raw.shape
+        if (raw.dtype != BF16 or len(shape) < 2 or shape[-1] != width or shape[-2] != self.tokens
+                or raw.numel() != self.tokens * width or raw.get_device() != self.index):
+            raise ValueError(f"{name}: expected the batch's {self.tokens} tokens of {width}, bf16 on {self.device}, not "
+                             f"{tuple(shape)} {raw.dtype} on {raw.device}")
+        stride, address = raw.stride(-2) if self.tokens > 1 else width, raw.data_ptr()
+        if raw.stride(-1) != 1 or stride % 8 or stride < width or address % 16:
+            raw = raw.clone(memory_format=torch.contiguous_format)
+            stride, address = width, raw.data_ptr()
+        return address, stride, raw
+
+    def _raw(self, args: BatchStep, raw_queries, raw_keys, raw_values) -> tuple:
+        d = self.head_dim
+        args.raw_queries, args.query_stride, q = self._rows(raw_queries, self.heads * d, "raw_queries")
+        args.raw_keys, args.key_stride, k = self._rows(raw_keys, self.kv_heads * d, "raw_keys")
+        args.raw_values, args.value_stride, v = self._rows(raw_values, self.kv_heads * d, "raw_values")
+        return q, k, v   # held until the call
+
+    def project(self, raw_queries, raw_keys, raw_values) -> torch.Tensor:
+        args = BatchStep.from_buffer_copy(self.args)   # of this call: two may be under way
+        held = self._raw(args, raw_queries, raw_keys, raw_values)
+        out = torch.empty((self.tokens, self.heads, self.head_dim), dtype=BF16, device=self.device)
+        args.queries = out.data_ptr()
+        call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
+        del held
+        return out
+
+    def __call__(self, raw_queries, raw_keys, raw_values, own_rows: int) -> torch.Tensor:
+        args = BatchStep.from_buffer_copy(self.args)
+        held = self._raw(args, raw_queries, raw_keys, raw_values)
+        sized, nbytes = self.sized
+        if sized != own_rows:
+            nbytes = library().omnia_attention_batch_step_bytes(self.tokens, self.heads, self.kv_heads, self.head_dim,
+                                                                args.prefix, own_rows, args.own_tiles)
+            _require(nbytes >= 0, "attention_batch_step: geometry not served")
+            self.sized = own_rows, nbytes
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        out = torch.empty((self.tokens, self.heads, self.head_dim), dtype=BF16, device=self.device)
+        args.own_rows, args.workspace_bytes, args.workspace, args.out = (own_rows, nbytes, workspace.data_ptr(),
+                                                                          out.data_ptr())
+        call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
+        del held
+        return out
 
 
 @dataclass(frozen=True)

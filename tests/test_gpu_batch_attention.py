@@ -456,7 +456,7 @@ def test_ops_refuse():
         lambda: ops.pages_copy(cache.keys[:, ::2], cache.values[:, ::2], [(0, 1, 1)]),
         lambda: ops.pages_copy(cache.keys, cache.values, [(0, cache.pages, 1)]),
         lambda: ops.pages_copy(cache.keys, cache.values, [(0, 1, 1), (2, 1, 1)] * 200),
-        lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0, 1 << 40, 0)]),
+        lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0, 1 << 40)]),
         lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0)]),
         lambda: ops.pages_advance(cache.lengths, batch.chosen, batch.rows[:1]),
     ]

@@ -296,7 +296,8 @@ def test_workspace_bytes():
 def _copy(moves, *, layers=1, pages=8, heads=2, rows=16, dim=64, tables=None, entries=0):
     from mlx_omnia_amd.runtime import library, loader
     flat = ops._int_lines(moves, 3, "moves")
-    rc = library().omnia_pages_copy(4096, 8192, layers, pages, heads, rows, dim, flat, len(moves), tables, entries, None)
+    rc = library().omnia_pages_copy(4096, 8192, layers, pages, heads, rows, dim, flat.ctypes.data, len(moves), tables,
+                                    entries, None)
     return rc, loader.last_error()
 
 
@@ -305,22 +306,73 @@ def _copy(moves, *, layers=1, pages=8, heads=2, rows=16, dim=64, tables=None, en
     ([(0, 1, 0)], "rows outside", {}), ([(0, 1, 17)], "rows outside", {}), ([(0, 1, 4), (2, 1, 4)], "two moves", {}),
     ([(0, 1, 4), (1, 2, 4)], "both read", {}), ([(3, 3, 4)], "both read", {}),
     ([(4, 0, 4), (3, 1, 4)], "sorted", dict(tables=4096, entries=4)), ([(0, 1, 1)], "bad page", dict(dim=60)),
-    ([(0, 1, 1)], "bad pool", dict(layers=0)), ([(0, 1, 1)] * 257, "more moves", {})])
+    ([(0, 1, 1)], "bad pool", dict(layers=0)), ([(0, 1, 1)] * 129, "more moves", {})])
 def test_pages_copy_refuses(moves, text, more):
     rc, message = _copy(moves, **more)
     assert rc == -22 and text in message
 
 
 @pytest.mark.parametrize("edits,text", [
-    ([(0, 4, 0, 0, 0)], "no such sequence"), ([(0, -1, 0, 0, 0)], "no such sequence"),
-    ([(0, 0, 6, 0, 0)], "no such entry"), ([(0, 0, 0, 9, 0)], "no such entry"), ([(0, 0, 0, -2, 0)], "no such entry"),
-    ([(1, 0, -1, 0, 0)], "below zero"), ([(2, 0, 4, 1, 1)], "to fork"), ([(2, 1, 1, 1, 1)], "to fork"),
-    ([(2, 0, 1, 7, 1)], "no such entry"), ([(2, 0, 1, 2, 9)], "no such entry"), ([(4, 0, 0, 0, -1)], "no such edit"),
-    ([(3, 0, 0, 2, -1)], "no such edit"), ([(0, 0, 1, 1, 0), (0, 0, 1, 2, 0)], "two edits"),
-    ([(2, 0, 1, 2, -1), (0, 1, 0, 3, 0)], "two edits"), ([(3, 1, 0, 0, -1), (1, 1, 2, 0, 0)], "two edits"),
-    ([(3, 1, 0, 0, -1), (2, 0, 1, 2, -1)], "two edits")])
+    ([(0, 4, 0, 0)], "no such sequence"), ([(0, -1, 0, 0)], "no such sequence"), ([(0, 0, 6, 0)], "no such entry"),
+    ([(0, 0, 0, 9)], "no such entry"), ([(0, 0, 0, -2)], "no such entry"), ([(1, 0, -1, 0)], "below zero"),
+    ([(3, 0, 0, 0)], "no such edit"), ([(0, 0, 1, 1), (0, 0, 1, 2)], "two edits"),
+    ([(2, 1, 0, 0), (1, 1, 2, 0)], "two edits"), ([(0, 1, 0, 3), (2, 1, 0, 0)], "two edits"),
+    ([(0, 0, 0, 0)] * 129, "more edits")])
 def test_pages_edit_refuses(edits, text):
     from mlx_omnia_amd.runtime import library, loader
-    flat = ops._int_lines(edits, 5, "edits")
-    assert library().omnia_pages_edit(4096, 8192, 4, 6, 9, flat, len(edits), None) == -22
+    flat = ops._int_lines(edits, 4, "edits")
+    assert library().omnia_pages_edit(4096, 8192, 4, 6, 9, flat.ctypes.data, len(edits), None) == -22
     assert text in loader.last_error()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(parent=4), "no such sequence"), (dict(parent=-1), "no such sequence"), (dict(full=7), "outside"),
+    (dict(full=6), "no such page"), (dict(rows=17), "outside"), (dict(rows=-1), "outside"), (dict(page=9), "no such page"),
+    (dict(page=-1), "no such page"), (dict(kids=[(4, 1)]), "no other sequence"), (dict(kids=[(0, 1)]), "no other sequence"),
+    (dict(kids=[(1, 1), (1, 2)]), "named twice"), (dict(kids=[(1, 1), (2, 1)]), "named twice"),
+    (dict(kids=[(1, 3)]), "no other page"), (dict(kids=[(1, 9)]), "no other page"), (dict(rows=0), "no other page"),
+    (dict(kids=[(1, 1)] * 129), "more children"), (dict(width=0), "bad tables")])
+def test_pages_fork_refuses(change, text):
+    from mlx_omnia_amd.runtime import library, loader
+    case = dict(width=6, parent=0, full=2, page=3, rows=5, kids=[(1, 1)], **{}) | change
+    kids = ops._int_lines(case["kids"], 2, "kids")
+    assert library().omnia_pages_fork(4096, 8192, 1, 9, 2, 16, 64, 4096, 8192, 4, case["width"], case["parent"],
+                                      case["full"], case["page"], case["rows"], kids.ctypes.data, len(kids), None) == -22
+    assert text in loader.last_error()
+
+
+def test_lines_of_numbers():
+    assert ops._int_lines([], 3, "moves").shape == (0, 3)
+    for bad in ([(1, 2)], [(1, 2, 1 << 31)], [(1, 2, -(1 << 40))], [(1.5, 2, 3)], [1, 2, 3], [(1, 2, 3), (1,)]):
+        with pytest.raises(ValueError, match="moves"):
+            ops._int_lines(bad, 3, "moves")
+
+
+def test_another_batch_of_the_same_sequences_keeps_up():
+    cache = small()
+    a = cache.open(15)
+    one, two = cache.batch([a]), cache.batch([a], tokens=2)
+    assert cache.ready(one) == 16 and cache.ready(two) == 17 and len(cache.pages_of(a)) == 2
+    for _ in range(17):
+        cache.ready(one)
+        cache.advance(one)
+    assert cache.ready(two) == 34 and len(cache.pages_of(a)) == 3
+
+
+def test_the_steps_arguments_are_laid_out_as_declared():
+    import ctypes
+    import re
+    from pathlib import Path
+
+    from mlx_omnia_amd.runtime.loader import BatchStep
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "omnia_hip.h").read_text()
+    body = re.search(r"typedef struct \{([^}]*)\} omnia_attention_batch_step_t;", text).group(1)
+    declared = []
+    for line in body.replace("const ", "").split(";"):
+        kind, _, names = line.strip().partition(" ")
+        for name in filter(None, (n.strip() for n in names.split(","))):
+            pointer = name.startswith("*")
+            declared.append((name.lstrip("*"), ctypes.c_void_p if pointer else
+                             {"int64_t": ctypes.c_int64, "float": ctypes.c_float}[kind]))
+    assert declared == list(BatchStep._fields_)
