@@ -27,6 +27,8 @@ A page id that is handed out is the lowest one free, so the same calls give the 
 
 from __future__ import annotations
 
+from array import array
+from bisect import insort
 from collections.abc import Sequence
 
 import numpy as np
@@ -114,11 +116,13 @@ class PagedKVCache:
         elif lengths is None or opened is None:
             raise ValueError("PagedKVCache: tables need lengths and opened")
         self.keys, self.values = keys, values
-        self._hip = hip_device(keys)
         self._tables = np.array(tables, dtype=np.int32)
         self._rows = np.array(lengths, dtype=np.int64)
-        self._open = np.zeros(len(self._tables), dtype=bool)
-        self._open[list(opened)] = True
+        slots = range(len(self._tables))
+        if len(set(opened)) != len(opened) or any(s not in slots for s in opened):
+            raise ValueError("PagedKVCache: opened names other sequences than the tables, or one twice")
+        self._open = [s in opened for s in slots]
+        self._closed = [s for s in slots if not self._open[s]]   # ascending
         self._held = (self._tables >= 0).sum(axis=1)
         self._check_tables()
         self._refs = np.zeros(pages, dtype=np.int64)
@@ -128,6 +132,7 @@ class PagedKVCache:
         self._clock = 0                                                  # turns as sequences grow
         self.tables = torch.from_numpy(self._tables.copy()).to(keys.device)
         self.lengths = torch.from_numpy(self._rows.astype(np.int32)).to(keys.device)
+        self._pool = ops.PagePool(keys, values, self.tables, self.lengths) if hip_device(keys) else None
 
     def _check_tables(self) -> None:
         tables, width = self._tables, self._tables.shape[1] if self._tables.ndim == 2 else 0
@@ -142,7 +147,7 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: a table's pages must come first, without gaps")
         if (self._rows < 0).any() or (self._rows > self._held * self.page_rows).any():
             raise ValueError("PagedKVCache: a length outside its sequence's pages")
-        if (self._held[~self._open] > 0).any():
+        if (self._held[self._closed] > 0).any():
             raise ValueError("PagedKVCache: a sequence that is not open holds pages")
         for row in tables:
             if len(np.unique(row[row >= 0])) != (row >= 0).sum():
@@ -183,13 +188,14 @@ class PagedKVCache:
         if _capturing(self.keys.device):
             raise ValueError(f"PagedKVCache: {what} cannot be captured (a replay would not repeat the host's part)")
 
-    def _edit(self, edits) -> None:
-        if not len(edits):
+    def _edit(self, edits: list[int]) -> None:
+        """Edits (kind, sequence, a, b), one after the other."""
+        if not edits:
             return
-        if self._hip:
-            ops.pages_edit(self.tables, self.lengths, self.pages, edits)
+        if self._pool is not None:
+            self._pool.edit(array("i", edits))
             return
-        for kind, s, a, b in np.asarray(edits).tolist():
+        for kind, s, a, b in zip(*(edits[i::4] for i in range(4))):
             if kind == ops.PAGES_ENTRY:
                 self.tables[s, a] = b
             elif kind == ops.PAGES_LENGTH:
@@ -197,29 +203,38 @@ class PagedKVCache:
             else:
                 self.tables[s], self.lengths[s] = -1, 0
 
-    def _fork(self, parent: int, full: int, rows: int, kids: np.ndarray) -> None:
-        """Rows of the table for the kids (sequence, page), and `rows` rows of the parent's last
-        page for each."""
+    @staticmethod
+    def _entries(sequence: int, first: int, pages) -> list[int]:
+        """The edits that make `pages` a sequence's entries from `first` on."""
+        return [n for i, page in enumerate(pages, first) for n in (ops.PAGES_ENTRY, sequence, i, page)]
+
+    def _fork(self, parent: int, full: int, rows: int, kids: list[int], pages: list[int]) -> None:
+        """Rows of the table for the kids, each with a page of its own, and `rows` rows of the
+        parent's last page for each."""
         page = int(self._tables[parent, full]) if rows else -1
-        if self._hip:
-            ops.pages_fork(self.keys, self.values, self.tables, self.lengths, parent, full, page, rows, kids)
+        if self._pool is not None:
+            flat = array("i", bytes(8 * len(kids)))
+            flat[0::2], flat[1::2] = array("i", kids), array("i", pages)
+            self._pool.fork(parent, full, page, rows, flat)
             return
         if rows:
-            self._copy([(page, to, rows) for _, to in kids.tolist()])
-        for kid, to in kids.tolist():
+            self._copy([(page, to, rows) for to in pages])
+        for kid, to in zip(kids, pages):
             self.tables[kid] = -1
             self.tables[kid, :full] = self.tables[parent, :full]
             if rows:
                 self.tables[kid, full] = to
             self.lengths[kid] = self.lengths[parent]
 
-    def _copy(self, moves, rename: bool = False) -> None:
-        if not len(moves):
+    def _copy(self, moves: list[tuple[int, int, int]], rename: bool = False) -> None:
+        if not moves:
             return
-        if self._hip:
-            ops.pages_copy(self.keys, self.values, moves, tables=self.tables if rename else None)
+        if self._pool is not None:
+            if rename:
+                self._pool.copy(moves, self.tables.data_ptr(), self.tables.numel())
+            else:
+                self._pool.copy(moves)
             return
-        moves = np.asarray(moves).tolist()
         for pool in (self.keys, self.values):
             for source, target, rows in moves:
                 pool[:, target, :, :rows] = pool[:, source, :, :rows]
@@ -241,19 +256,23 @@ class PagedKVCache:
 
     def _take(self, count: int) -> np.ndarray:
         """The lowest `count` free pages, still free."""
-        if count == 0:
-            return np.empty(0, dtype=np.int64)
-        found = np.flatnonzero(self._refs == 0)[:count]
+        found = (self._refs == 0).nonzero()[0][:count]
         if len(found) < count:
             raise ValueError(f"PagedKVCache: {count} more pages are needed, {len(found)} of {self.pages} are free")
         return found
 
     def _slots(self, count: int) -> list[int]:
-        found = np.flatnonzero(~self._open)[:count]
-        if len(found) < count:
-            raise ValueError(f"PagedKVCache: {count} more sequences are asked for, {len(found)} of "
+        """The lowest `count` sequences that are not open, still not."""
+        if len(self._closed) < count:
+            raise ValueError(f"PagedKVCache: {count} more sequences are asked for, {len(self._closed)} of "
                              f"{len(self._open)} are not open")
-        return found.tolist()
+        return self._closed[:count]
+
+    def _begin(self, slots: list[int]) -> None:
+        del self._closed[: len(slots)]
+        for s in slots:
+            self._open[s] = True
+        self._renew(slots)
 
     def _pages_for(self, rows: int) -> int:
         pages = -(-int(rows) // self.page_rows)
@@ -268,24 +287,14 @@ class PagedKVCache:
         if rows < 0:
             raise ValueError("PagedKVCache: a sequence of fewer than no rows")
         pages = self._pages_for(rows)
-        (s,) = self._slots(1)
-        fresh = self._take(pages)
-        self._open[s] = True
-        self._renew(s)
+        slots = self._slots(1)
+        s, fresh = slots[0], self._take(pages)
+        self._begin(slots)
         self._refs[fresh] = 1
         self._tables[s, :pages] = fresh
         self._held[s], self._rows[s] = pages, rows
-        self._edit(self._entries(s, 0, fresh) if not rows else
-                   np.concatenate([self._entries(s, 0, fresh), [(ops.PAGES_LENGTH, s, rows, 0)]]))
+        self._edit(self._entries(s, 0, fresh.tolist()) + ([ops.PAGES_LENGTH, s, rows, 0] if rows else []))
         return s
-
-    @staticmethod
-    def _entries(sequence: int, first: int, pages: np.ndarray) -> np.ndarray:
-        """The edits that make `pages` a sequence's entries from `first` on."""
-        edits = np.empty((len(pages), 4), dtype=np.int32)
-        edits[:, 0], edits[:, 1], edits[:, 3] = ops.PAGES_ENTRY, sequence, pages
-        edits[:, 2] = np.arange(first, first + len(pages))
-        return edits
 
     def _reserve(self, index: np.ndarray, rows: np.ndarray) -> None:
         """Pages for `rows` rows of each sequence, and one of its own where it writes next."""
@@ -312,7 +321,7 @@ class PagedKVCache:
         for i, page in zip(copied, fresh.tolist()):
             s, old = int(index[i]), int(self._tables[index[i], at[i]])
             moves.append((old, page, int(now[i] % size)))
-            edits.append((ops.PAGES_ENTRY, s, int(at[i]), page))
+            edits += ops.PAGES_ENTRY, s, int(at[i]), page
             self._tables[s, at[i]] = page
             self._refs[old] -= 1
         self._refs[fresh] = 1
@@ -321,7 +330,7 @@ class PagedKVCache:
             s = int(index[i])
             for entry in range(self._held[s], self._held[s] + int(more[i])):
                 self._tables[s, entry] = page = next(rest)
-                edits.append((ops.PAGES_ENTRY, s, entry, page))
+                edits += ops.PAGES_ENTRY, s, entry, page
             self._held[s] += int(more[i])
         self._copy(moves)
         self._edit(edits)
@@ -343,27 +352,31 @@ class PagedKVCache:
         full, rest = divmod(rows, size)
         if not share:
             full, rest = 0, rows
-        parent = self._tables[sequence]
         each = -(-rest // size)
-        kids = self._slots(count)
-        fresh = self._take(each * count).reshape(count, each)
-        self._refs[fresh.reshape(-1)] = 1
+        kids, fresh = self._slots(count), self._take(each * count)
+        if not count:
+            return kids
+        parent = self._tables[sequence]
+        self._refs[fresh] = 1
         self._refs[parent[:full]] += count
-        self._open[kids] = True
-        self._renew(kids)
-        self._tables[kids, :full] = parent[:full]
-        self._tables[kids, full : full + each] = fresh
-        self._held[kids], self._rows[kids] = full + each, rows
+        self._begin(kids)
+        block = self._tables[kids[0] : kids[-1] + 1] if kids[-1] - kids[0] == count - 1 else None
+        lines = self._tables[kids] if block is None else block
+        lines[:, :full] = parent[:full]
+        lines[:, full : full + each] = fresh.reshape(count, each)
+        if block is None:
+            self._tables[kids] = lines
+        self._held[kids] = full + each
+        self._rows[kids] = rows
+        pages = fresh.tolist()
         if share:
-            self._fork(sequence, full, rest, np.stack(
-                [kids, fresh[:, 0] if each else np.full(count, -1)], axis=1).astype(np.int32))
+            self._fork(sequence, full, rest, kids, pages if each else [-1] * count)
         else:
-            used = np.full((count, each), size)
-            used[:, -1:] = rest - size * (each - 1)
-            self._copy(np.stack([np.broadcast_to(parent[:each], (count, each)), fresh, used], axis=-1).reshape(-1, 3))
-            self._edit(np.concatenate([np.empty((0, 4), dtype=np.int32)] + [
-                edits for kid, line in zip(kids, fresh)
-                for edits in (self._entries(kid, 0, line), [(ops.PAGES_LENGTH, kid, rows, 0)])]))
+            used = [size] * (each - 1) + [rest - size * (each - 1)]
+            self._copy([(page, to, n) for i in range(count)
+                        for page, to, n in zip(parent.tolist(), pages[i * each : (i + 1) * each], used)])
+            self._edit([n for i, kid in enumerate(kids)
+                        for n in self._entries(kid, 0, pages[i * each : (i + 1) * each]) + [ops.PAGES_LENGTH, kid, rows, 0]])
         return kids
 
     def free(self, sequences: Sequence[int] | int) -> None:
@@ -375,15 +388,21 @@ class PagedKVCache:
         self._known(gone)
         if not gone:
             return
-        held = self._tables[gone]
-        np.subtract.at(self._refs, held[held >= 0], 1)
-        self._tables[gone] = -1
-        self._held[gone] = self._rows[gone] = 0
-        self._open[gone] = False
+        if len(gone) == 1:   # a sequence names no page twice
+            held = self._tables[gone[0], : self._held[gone[0]]]
+            self._refs[held] -= 1
+            held[:] = -1
+        else:
+            held = self._tables[gone]
+            self._refs -= np.bincount(held[held >= 0], minlength=len(self._refs))
+            self._tables[gone] = -1
+        for s in gone:
+            self._open[s] = False
+            insort(self._closed, s)
+        self._held[gone] = 0
+        self._rows[gone] = 0
         self._renew(gone)
-        edits = np.zeros((len(gone), 4), dtype=np.int32)
-        edits[:, 0], edits[:, 1] = ops.PAGES_CLEAR, gone
-        self._edit(edits)
+        self._edit([n for s in gone for n in (ops.PAGES_CLEAR, s, 0, 0)])
 
     def truncate(self, sequence: int, rows: int) -> None:
         """Drop the sequence's rows from `rows` on (a rejected guess), and the pages past them."""
@@ -397,8 +416,7 @@ class PagedKVCache:
         self._tables[sequence, keep:] = -1
         self._held[sequence], self._rows[sequence] = keep, rows
         self._renew(sequence)
-        self._edit(np.concatenate([self._entries(sequence, keep, np.full(gone, -1)),
-                                   [(ops.PAGES_LENGTH, sequence, rows, 0)]]))
+        self._edit(self._entries(sequence, keep, [-1] * gone) + [ops.PAGES_LENGTH, sequence, rows, 0])
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool, each that lies behind them to the
@@ -413,7 +431,7 @@ class PagedKVCache:
             names[-1], names[source] = -1, target
             self._tables = names[self._tables]
             self._refs[target], self._refs[source] = self._refs[source], 0
-            self._copy(np.stack([source, target, np.full(len(source), self.page_rows)], axis=1), rename=True)
+            self._copy([(a, b, self.page_rows) for a, b in zip(source.tolist(), target.tolist())], rename=True)
         return live
 
     def resize(self, pages: int) -> None:
@@ -433,6 +451,8 @@ class PagedKVCache:
         refs = np.zeros(pages, dtype=np.int64)
         refs[:kept] = self._refs[:kept]
         (self.keys, self.values), self._refs = pools, refs
+        if self._pool is not None:
+            self._pool = ops.PagePool(*pools, self.tables, self.lengths)
 
     # Steps --------------------------------------------------------------------------------
 
@@ -491,7 +511,7 @@ class PagedKVCache:
         self._current(batch)
         if not _capturing(self.keys.device):
             self.account(batch, 1)
-        if self._hip:
+        if self._pool is not None:
             ops.pages_advance(self.lengths, batch.chosen, batch.rows)
         else:
             self.lengths[batch.chosen.long()] += batch.rows

@@ -10,6 +10,7 @@ fit.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -1161,31 +1162,21 @@ PAGES_MOVES, PAGES_EDITS = 128, 128   # OMNIA_PAGES_MOVES, OMNIA_PAGES_EDITS
 PAGES_ENTRY, PAGES_LENGTH, PAGES_CLEAR = 0, 1, 2
 
 
-def _int_lines(lines, width: int, name: str) -> np.ndarray:
-    """Lines of `width` whole numbers that fit 32 bits, as the library reads them."""
-    try:
-        array = np.asarray(lines)
-        if array.dtype != np.int32:
-            if array.size and (array.dtype.kind not in "iu" or array.min() < -(1 << 31) or array.max() >= 1 << 31):
-                raise ValueError
-            array = array.astype(np.int32)
-    except (ValueError, OverflowError):
-        raise ValueError(f"{name}: whole numbers of 32 bits, {width} a line") from None
-    if array.size and (array.ndim != 2 or array.shape[1] != width):
-        raise ValueError(f"{name}: whole numbers of 32 bits, {width} a line")
-    return np.ascontiguousarray(array).reshape(-1, width)
-
-
-def _pool(keys: torch.Tensor, values: torch.Tensor, name: str) -> tuple[int, int, int, int, int]:
-    """(layers, pages, kv_heads, page_rows, 16-bit words of a row) of a pool of any type."""
-    _require(keys.dim() == 5 and keys.shape == values.shape and keys.dtype == values.dtype,
-             name + ": keys and values must be [layers, pages, kv_heads, page_rows, head_dim]")
-    _dense(keys, keys.dtype, "keys")
-    _dense(values, keys.dtype, "values")
-    layers, pages, kv_heads, page_rows, head_dim = keys.shape
-    width = head_dim * keys.element_size()
-    _require(width % 16 == 0, name + ": rows must be whole 16-byte vectors")
-    return layers, pages, kv_heads, page_rows, width // 2
+def _int_lines(lines, width: int, name: str) -> array:
+    """Lines of `width` whole numbers that fit 32 bits, one after the other, as the library
+    reads them (an array of them as it is)."""
+    if isinstance(lines, array) and lines.typecode == "i":
+        flat = lines
+    else:
+        try:
+            lines = lines.tolist() if isinstance(lines, np.ndarray) else list(lines)
+            if any(len(line) != width for line in lines):
+                raise TypeError
+            flat = array("i", [n for line in lines for n in line])
+        except (TypeError, OverflowError):
+            raise ValueError(f"{name}: whole numbers of 32 bits, {width} a line") from None
+    _require(len(flat) % width == 0, f"{name}: whole numbers of 32 bits, {width} a line")
+    return flat
 
 
 def _page_tables(tables: torch.Tensor, lengths: torch.Tensor, name: str) -> tuple[int, int]:
@@ -1195,46 +1186,78 @@ def _page_tables(tables: torch.Tensor, lengths: torch.Tensor, name: str) -> tupl
     return tables.shape
 
 
+class PagePool:
+    """A pool of pages with its tables, checked once: `copy`, `fork` and `edit` as the functions
+    below have them. (Fifteen microseconds of a fork's thirty-six were checks of tensors that a
+    cache keeps.)"""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor | None = None,
+                 lengths: torch.Tensor | None = None) -> None:
+        _require(keys.dim() == 5 and keys.shape == values.shape and keys.dtype == values.dtype,
+                 "page pool: keys and values must be [layers, pages, kv_heads, page_rows, head_dim]")
+        _dense(keys, keys.dtype, "keys")
+        _dense(values, keys.dtype, "values")
+        width = keys.shape[-1] * keys.element_size()
+        _require(width % 16 == 0, "page pool: rows must be whole 16-byte vectors")
+        self.held = [t for t in (keys, values, tables, lengths) if t is not None]
+        _require(on_rocm(*self.held), "page pool: tensors must share one ROCm device")
+        self.pool = keys.data_ptr(), values.data_ptr(), *keys.shape[:4], width // 2
+        self.index, self.pages = keys.get_device(), keys.shape[1]
+        if tables is not None and lengths is not None:
+            self.sequences, self.width = _page_tables(tables, lengths, "page pool")
+            self.tables, self.lengths = tables.data_ptr(), lengths.data_ptr()
+
+    def copy(self, moves, tables: int | None = None, entries: int = 0) -> None:
+        flat, step = _int_lines(moves, 3, "moves"), 3 * PAGES_MOVES
+        if len(flat) > step:   # within one call the library asks this itself
+            source, target = np.asarray(flat[0::3]), np.asarray(flat[1::3])
+            if len(np.unique(target)) < len(target) or np.isin(target, source).any():
+                raise ValueError("pages_copy: a page is written twice, or both read and written")
+            if tables is not None and (np.diff(source) <= 0).any():
+                raise ValueError("pages_copy: moves that rename have to be sorted by the page they leave")
+        stream, address = _raw_stream(self.index), flat.buffer_info()[0]
+        for first in range(0, len(flat), step):
+            call("omnia_pages_copy", *self.pool, address + 4 * first, min(step, len(flat) - first) // 3, tables,
+                 entries, stream)
+
+    def fork(self, parent: int, full: int, page: int, rows: int, kids) -> None:
+        flat, step = _int_lines(kids, 2, "kids"), 2 * PAGES_MOVES
+        if len(flat) > step and (len(set(flat[0::2])) < len(flat) // 2 or (rows and len(set(flat[1::2])) < len(flat) // 2)):
+            raise ValueError("pages_fork: a child or a page is named twice")
+        stream, address = _raw_stream(self.index), flat.buffer_info()[0]
+        for first in range(0, len(flat), step):
+            call("omnia_pages_fork", *self.pool, self.tables, self.lengths, self.sequences, self.width, parent, full,
+                 page, rows, address + 4 * first, min(step, len(flat) - first) // 2, stream)
+
+    def edit(self, edits) -> None:
+        _edit(self.tables, self.lengths, self.sequences, self.width, self.pages, edits, _raw_stream(self.index))
+
+
+def _edit(tables: int, lengths: int, sequences: int, width: int, pages: int, edits, stream: int) -> None:
+    flat, step = _int_lines(edits, 4, "edits"), 4 * PAGES_EDITS
+    address = flat.buffer_info()[0]
+    for first in range(0, len(flat), step):
+        call("omnia_pages_edit", tables, lengths, sequences, width, pages, address + 4 * first,
+             min(step, len(flat) - first) // 4, stream)
+
+
 def pages_copy(keys: torch.Tensor, values: torch.Tensor, moves, *, tables: torch.Tensor | None = None) -> None:
     """Copy pages of the pool `keys`, `values` [layers, pages, kv_heads, page_rows, D] in every
     layer: moves are (from, to, rows), rows the first of the page that are copied. No page may
     be written twice, or read and written. With `tables` (int32, on the device) the entries
-    that name a page left are renamed, and moves are sorted by it; see `omnia_pages_copy`."""
-    pool = _pool(keys, values, "pages_copy")
-    tensors = [keys, values]
-    if tables is not None:
-        _require(tables.dtype == torch.int32 and tables.is_contiguous(), "pages_copy: tables must be contiguous int32")
-        tensors.append(tables)
-    _require(on_rocm(*tensors), "pages_copy: tensors must share one ROCm device")
-    moves = _int_lines(moves, 3, "moves")
-    if len(moves) > PAGES_MOVES:   # within one call the library asks this itself
-        if len(np.unique(moves[:, 1])) < len(moves) or np.isin(moves[:, 1], moves[:, 0]).any():
-            raise ValueError("pages_copy: a page is written twice, or both read and written")
-        if tables is not None and (np.diff(moves[:, 0]) <= 0).any():
-            raise ValueError("pages_copy: moves that rename have to be sorted by the page they leave")
-    stream = _stream(keys)
-    for first in range(0, len(moves), PAGES_MOVES):
-        some = moves[first : first + PAGES_MOVES]
-        call("omnia_pages_copy", keys.data_ptr(), values.data_ptr(), *pool, some.ctypes.data, len(some),
-             tables.data_ptr() if tables is not None else None, tables.numel() if tables is not None else 0, stream)
+    that name a page left are renamed, and moves are sorted by it; see `omnia_pages_copy`.
+    More than PAGES_MOVES are made in turn, as many at a time."""
+    if tables is None:
+        return PagePool(keys, values).copy(moves)
+    _require(tables.dtype == torch.int32 and tables.is_contiguous(), "pages_copy: tables must be contiguous int32")
+    PagePool(keys, values, tables).copy(moves, tables.data_ptr(), tables.numel())
 
 
 def pages_fork(keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, parent: int,
                full: int, page: int, rows: int, kids) -> None:
     """Make sequences the children of `parent`, each a (sequence, page) of kids: they share its
     first `full` pages and get the first `rows` rows of `page` copied; see `omnia_pages_fork`."""
-    pool = _pool(keys, values, "pages_fork")
-    sequences, width = _page_tables(tables, lengths, "pages_fork")
-    _require(on_rocm(keys, values, tables, lengths), "pages_fork: tensors must share one ROCm device")
-    kids = _int_lines(kids, 2, "kids")
-    if len(kids) > PAGES_MOVES and (len(np.unique(kids[:, 0])) < len(kids)
-                                    or (rows and len(np.unique(kids[:, 1])) < len(kids))):
-        raise ValueError("pages_fork: a child or a page is named twice")
-    stream = _stream(keys)
-    for first in range(0, len(kids), PAGES_MOVES):
-        some = kids[first : first + PAGES_MOVES]
-        call("omnia_pages_fork", keys.data_ptr(), values.data_ptr(), *pool, tables.data_ptr(), lengths.data_ptr(),
-             sequences, width, parent, full, page, rows, some.ctypes.data, len(some), stream)
+    PagePool(keys, values, tables, lengths).fork(parent, full, page, rows, kids)
 
 
 def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -> None:
@@ -1242,11 +1265,7 @@ def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -
     More than PAGES_EDITS are made in turn, as many at a time."""
     sequences, width = _page_tables(tables, lengths, "pages_edit")
     _require(on_rocm(tables, lengths), "pages_edit: tensors must share one ROCm device")
-    edits, stream = _int_lines(edits, 4, "edits"), _stream(tables)
-    for first in range(0, len(edits), PAGES_EDITS):
-        some = edits[first : first + PAGES_EDITS]
-        call("omnia_pages_edit", tables.data_ptr(), lengths.data_ptr(), sequences, width, pages,
-             some.ctypes.data, len(some), stream)
+    _edit(tables.data_ptr(), lengths.data_ptr(), sequences, width, pages, edits, _stream(tables))
 
 
 def pages_advance(lengths: torch.Tensor, chosen: torch.Tensor, rows: torch.Tensor) -> None:

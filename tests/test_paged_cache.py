@@ -110,6 +110,17 @@ def test_batches_find_what_their_sequences_share():
     assert batch.tiles(50).tolist() == [[0, 128, kids[0], 0], [128, 150, kids[0], 2], [150, 200, kids[2], 0]]
 
 
+def test_children_in_the_slots_that_are_left():
+    cache = small(pages=20, sequences=7)
+    for _ in range(6):
+        cache.open(3)
+    cache.free([4, 1, 3])
+    assert cache.fork(0, 3) == [1, 3, 4]
+    assert [cache.pages_of(s) for s in (1, 3, 4)] == [[1], [3], [4]] and cache.pages_of(5) == [5]
+    assert cache.tables[:, 0].tolist() == [0, 1, 2, 3, 4, 5, -1] and cache.lengths.tolist() == [3] * 6 + [0]
+    assert cache.open() == 6 and cache.fork(0, 0) == []
+
+
 def test_full_pools_and_tables_leave_everything_as_it_was():
     cache = small(pages=4, sequences=3, rows=64)
     a = cache.open(40)
@@ -159,7 +170,9 @@ def test_refusals():
     dict(tables=np.array([[1, -1]]), lengths=np.array([17]), opened=[0]),
     dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[]),
     dict(tables=np.array([[1, -2]]), lengths=np.array([3]), opened=[0]), dict(sequences=0, rows=3),
-    dict(sequences=2, rows=16, opened=[0])])
+    dict(sequences=2, rows=16, opened=[0]), dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[-1]),
+    dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[0, 1]),
+    dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[0, 0])])
 def test_tables_that_do_not_hold_together_are_refused(change):
     pool = torch.zeros((1, 4, 2, 16, 8))
     with pytest.raises(ValueError):
@@ -296,7 +309,7 @@ def test_workspace_bytes():
 def _copy(moves, *, layers=1, pages=8, heads=2, rows=16, dim=64, tables=None, entries=0):
     from mlx_omnia_amd.runtime import library, loader
     flat = ops._int_lines(moves, 3, "moves")
-    rc = library().omnia_pages_copy(4096, 8192, layers, pages, heads, rows, dim, flat.ctypes.data, len(moves), tables,
+    rc = library().omnia_pages_copy(4096, 8192, layers, pages, heads, rows, dim, flat.buffer_info()[0], len(moves), tables,
                                     entries, None)
     return rc, loader.last_error()
 
@@ -321,7 +334,7 @@ def test_pages_copy_refuses(moves, text, more):
 def test_pages_edit_refuses(edits, text):
     from mlx_omnia_amd.runtime import library, loader
     flat = ops._int_lines(edits, 4, "edits")
-    assert library().omnia_pages_edit(4096, 8192, 4, 6, 9, flat.ctypes.data, len(edits), None) == -22
+    assert library().omnia_pages_edit(4096, 8192, 4, 6, 9, flat.buffer_info()[0], len(edits), None) == -22
     assert text in loader.last_error()
 
 
@@ -337,12 +350,12 @@ def test_pages_fork_refuses(change, text):
     case = dict(width=6, parent=0, full=2, page=3, rows=5, kids=[(1, 1)], **{}) | change
     kids = ops._int_lines(case["kids"], 2, "kids")
     assert library().omnia_pages_fork(4096, 8192, 1, 9, 2, 16, 64, 4096, 8192, 4, case["width"], case["parent"],
-                                      case["full"], case["page"], case["rows"], kids.ctypes.data, len(kids), None) == -22
+                                      case["full"], case["page"], case["rows"], kids.buffer_info()[0], len(kids) // 2, None) == -22
     assert text in loader.last_error()
 
 
 def test_lines_of_numbers():
-    assert ops._int_lines([], 3, "moves").shape == (0, 3)
+    assert list(ops._int_lines([], 3, "moves")) == [] and list(ops._int_lines([(1, 2, 3)], 3, "moves")) == [1, 2, 3]
     for bad in ([(1, 2)], [(1, 2, 1 << 31)], [(1, 2, -(1 << 40))], [(1.5, 2, 3)], [1, 2, 3], [(1, 2, 3), (1,)]):
         with pytest.raises(ValueError, match="moves"):
             ops._int_lines(bad, 3, "moves")
