@@ -731,8 +731,8 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  *   x = scale * (q[t, h] . k[r, h / gqa])
  * in fp32, the weights rounded to bf16 for their product with the values, the result once to
  * bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
- * prefix) must be the same pages in every token's sequence: they are read through the first
- * token's. own_rows bounds the rows past them of every sequence, this step's included; tiles
+ * prefix) must be the same pages in every token's sequence: they are read through
+ * prefix_sequence's. own_rows bounds the rows past them of every sequence, this step's included; tiles
  * [own_tiles, 4] int32 (device) are runs of query rows that cover every row once (of each kv
  * head, row r is token r / gqa, head r % gqa): (first, end, s, j) for the rows [first, end), at
  * most 128, of sequence s, whose new token j the first row is of.
@@ -746,7 +746,7 @@ int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
                               const int32_t* tables, int64_t sequences, int64_t width,
                               const int32_t* lengths, const int32_t* token_map, int64_t tokens,
                               const int32_t* tiles, int64_t own_tiles, int64_t prefix,
-                              int64_t own_rows, int64_t heads, int64_t kv_heads,
+                              int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads,
                               int64_t head_dim, const uint16_t* sinks, float scale,
                               void* workspace, int64_t workspace_bytes, uint16_t* out,
                               hipStream_t stream);
@@ -766,7 +766,8 @@ typedef struct {
   uint16_t *queries, *out;
   void *workspace;
   int64_t workspace_bytes, query_stride, key_stride, value_stride, table_stride, angle_rows, rotary_pairs;
-  int64_t tokens, heads, kv_heads, head_dim, pages, page_rows, sequences, width, own_tiles, prefix, own_rows;
+  int64_t tokens, heads, kv_heads, head_dim, pages, page_rows, sequences, width, own_tiles, prefix;
+  int64_t prefix_sequence, own_rows;
   float mscale, eps, scale;
 } omnia_attention_batch_step_t;
 int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,

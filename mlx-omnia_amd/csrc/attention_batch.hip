@@ -35,7 +35,7 @@ struct PageTables {
   // The page of a sequence's row, or -1 where there is none.
   __device__ __forceinline__ int page(int sequence, int row) const {
     const int index = row >> page_shift;
-    if (index >= width) return -1;
+    if (sequence < 0 || sequence >= sequences || index < 0 || index >= width) return -1;
     const int id = tables[static_cast<int64_t>(sequence) * width + index];
     return id < pages ? id : -1;
   }
@@ -66,18 +66,18 @@ struct BatchProjectArgs {
 // under way together. (Its angles are four times a lane's bytes of a head: read for each head
 // and with an index division, 7,000 tokens of 64 heads took 31 us.) The norm, the rotation and
 // mscale stay in fp32 and are rounded once, where they are stored. Bound by its launch at a few
-// tokens and by memory at a prompt.
-constexpr int kProjectHeads = 4;
-template <int D>
+// tokens (where a head in turn is the faster: 128 tokens of 48 heads 5.3 us for 8.1) and by
+// memory at a prompt.
+template <int D, int kHeads>
 __global__ __launch_bounds__(256) void attention_batch_project_kernel(BatchProjectArgs a) {
   constexpr int kLanes = D / 8, kGroups = 256 / kLanes;
   const int64_t token = blockIdx.x;
   const int lane = threadIdx.x % kLanes;
-  const int first = static_cast<int>(blockIdx.y) * kGroups * kProjectHeads + threadIdx.x / kLanes;
+  const int first = static_cast<int>(blockIdx.y) * kGroups * kHeads + threadIdx.x / kLanes;
   const int slots = a.heads + 2 * a.kv_heads;
-  u32x4 raw[kProjectHeads];
+  u32x4 raw[kHeads];
 #pragma unroll
-  for (int i = 0; i < kProjectHeads; ++i) {
+  for (int i = 0; i < kHeads; ++i) {
     const int slot = min(first + i * kGroups, slots - 1);
     const int part = slot < a.heads ? 0 : slot < a.heads + a.kv_heads ? 1 : 2;
     const int head = slot - (part == 0 ? 0 : part == 1 ? a.heads : a.heads + a.kv_heads);
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256) void attention_batch_project_kernel(BatchProje
     *reinterpret_cast<f32x4*>(s + 4) = *reinterpret_cast<const f32x4*>(a.sin + row + at + 4);
   }
 #pragma unroll
-  for (int i = 0; i < kProjectHeads; ++i) {
+  for (int i = 0; i < kHeads; ++i) {
     const int slot = first + i * kGroups;
     if (slot >= slots) return;   // whole groups of lanes: their shuffles stay inside
     const int part = slot < a.heads ? 0 : slot < a.heads + a.kv_heads ? 1 : 2;
@@ -181,7 +181,7 @@ struct BatchArgs {
   uint16_t* out;            // [tokens, heads, D]
   float* partial;           // [tokens * heads, splits, D] contexts, then [tokens * heads, splits, 2]
   PageTables at;
-  int heads, kv_heads, group, tokens, prefix, prefix_tiles, own_tiles;
+  int heads, kv_heads, group, tokens, prefix, prefix_sequence, prefix_tiles, own_tiles;
   int prefix_splits, prefix_keys, own_splits, own_keys;   // splits of either part, keys of one
   float scale_log2;
 };
@@ -540,8 +540,7 @@ struct PageWalk {
   int sequence, window, now, next;
 
   __device__ __forceinline__ int fetch(int w) const {
-    const int row = w * 1024 + static_cast<int>(threadIdx.x) % kWave * 16;
-    return row < 0 ? -1 : at.page(sequence, row);
+    return at.page(sequence, w * 1024 + static_cast<int>(threadIdx.x) % kWave * 16);
   }
   __device__ __forceinline__ PageWalk(const PageTables& tables, int s, int row) : at(tables), sequence(s) {
     window = row / 1024;
@@ -563,15 +562,12 @@ struct PageWalk {
 struct Piece {
   bool shared, mixed;       // mixed: rows that see different keys
   int first_row, end_row, kv_head, split, low, high, sequence;
+  int token;                // own: the first row is of this new token of the sequence
   int before;               // own: a row's token t sees the keys up to before + t
-
-  // Past the last key that a token sees.
-  __device__ __forceinline__ int limit(const BatchArgs& a, int token) const {
-    return (shared ? a.at.before(a.at.tokens[token]) : before + token) + 1;
-  }
 };
 
-__device__ __forceinline__ bool find_piece(const BatchArgs& a, Piece& p) {
+// As far as the block's number and its tile say, so that the pages are asked for at once.
+__device__ __forceinline__ void find_piece(const BatchArgs& a, Piece& p) {
   const int rows = a.tokens * a.group;
   const int pairs = a.kv_heads * a.prefix_splits;
   const int prefix_blocks = pairs * a.prefix_tiles;
@@ -593,7 +589,7 @@ __device__ __forceinline__ bool find_piece(const BatchArgs& a, Piece& p) {
     p.split = pair / a.kv_heads;
     p.low = p.split * a.prefix_keys;
     p.high = min(p.low + a.prefix_keys, a.prefix);
-    p.sequence = a.at.tokens[0].x;
+    p.sequence = a.prefix_sequence;
     p.mixed = false;
   } else {
     block -= prefix_blocks;
@@ -604,12 +600,18 @@ __device__ __forceinline__ bool find_piece(const BatchArgs& a, Piece& p) {
     p.first_row = min(max(tile.x, 0), rows - 1);
     p.end_row = min(min(max(tile.y, p.first_row + 1), rows), p.first_row + kTileRows);
     p.sequence = tile.z;
-    // Of the tokens: the tile says which they are, so that nothing waits for their map.
-    const int first = p.first_row / a.group;
-    p.before = a.at.rows_before(tile.z, tile.w) - first;
+    p.token = tile.w;
     p.low = a.prefix + p.split * a.own_keys;
-    p.high = min(p.low + a.own_keys, p.before + (p.end_row - 1) / a.group + 1);
-    p.mixed = (p.end_row - 1) / a.group != first;
+  }
+}
+
+// The keys of an own piece, by its sequence's length; whether there is anything to do.
+__device__ __forceinline__ bool find_keys(const BatchArgs& a, Piece& p) {
+  if (!p.shared) {
+    const int first = p.first_row / a.group, last = (p.end_row - 1) / a.group;
+    p.before = a.at.rows_before(p.sequence, p.token) - first;
+    p.high = min(p.low + a.own_keys, p.before + last + 1);
+    p.mixed = last != first;
     if (p.low >= p.high) {
       // No row of the tile reaches this split, nor is it merged; where it is the only one, its
       // rows come as zeros.
@@ -652,7 +654,8 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) 
 // Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS stages;
 // the next tile is on its way to the one while the other is multiplied.
 template <int D, int kParts>
-__device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t* stage0, uint16_t* stage1, int* odd) {
+__device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk& walk, uint16_t* stage0, 
+                                           uint16_t* stage1, int* odd) {
   using Rows = WideRows<D, kParts>;
   constexpr int kChunks = D / 8;
   constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread brings, each of K and V
@@ -663,16 +666,12 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   const bool live = p.first_row + wave * kWaveRows + column < p.end_row;
   const bool working = p.first_row + wave * kWaveRows < p.end_row;   // the wave
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
-  const int limit = p.limit(a, token);
-  // Up to here every row sees the keys: up to the first row's limit, or for the shared rows
-  // (that a sequence stops before their end is not expected of a plan, but served) nowhere.
-  int common = p.mixed ? p.limit(a, p.first_row / a.group) : p.high;
-  if (p.shared && __syncthreads_or(limit < p.high)) common = 0;
-  common = __builtin_amdgcn_readfirstlane(common);
-
-  PageWalk walk(a.at, p.sequence, p.low);
+  const int2 whose = p.shared ? a.at.tokens[token] : int2{0, 0};   // asked for ahead of its use
   Rows rows;
   rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
+  // Up to here every row sees the keys: up to the first row's limit, or all the shared ones
+  // (that a sequence stops before their end is not expected of a plan, but served: below).
+  int common = p.mixed ? p.before + p.first_row / a.group + 1 : p.high;
 
   // Thread t's vector i is chunk t % kChunks of row (t + 256 i) / kChunks of a tile, of one
   // sixteen for the whole wave.
@@ -735,10 +734,14 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   int tile = p.low / kTileKeys;
   if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
-  if (tile < tiles) {
-    ask(tile, stage0);
-    if (!whole) patch(tile, stage0);
+  if (tile < tiles) ask(tile, stage0);
+  const int limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
+  if (p.shared && __syncthreads_or(limit < p.high)) {
+    common = 0;
+    whole = false;
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what was asked for comes first
   }
+  if (tile < tiles && !whole) patch(tile, stage0);
   arrive();
   // The stages by name, not by a turning index: the compiler then sees that what is on its way
   // to the one is not what is read from the other, and does not wait for it.
@@ -793,34 +796,33 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, uint16_t
   }
 }
 
-// Up to 16 rows: the four waves hold the same rows and take every fourth tile of 32 keys each,
-// through an LDS buffer of their own without a barrier, and merge at the end.
-template <int D, int kParts>
-__device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16_t* stage0, uint16_t* stage1) {
+// A wave's walk over a piece with up to 16 rows: every `stride`-th tile of 32 keys from `tile`
+// on, through an LDS buffer of its own, without a barrier. Leaves the rows' state in `rows`.
+template <int D, int kParts, bool kStream>
+__device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWalk& walk, NarrowRows<D, kParts>& rows,
+                                            int tile, int stride, uint16_t* tile_k) {
   using Rows = NarrowRows<D, kParts>;
   constexpr int kKeys = 32;
   constexpr int kChunks = D / 8, kRowsALoad = kWave / kChunks;   // 4 or 8
   constexpr int kLoads = kKeys / kRowsALoad;                     // 16-byte vectors a lane stages, each of K and V
-  constexpr int kTile = kKeys * D;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int column = lane % 16, quarter = lane / 16;
+  uint16_t* tile_v = tile_k + kKeys * D;
+  const int lane = threadIdx.x % kWave, column = lane % 16, quarter = lane / 16;
   const int row = min(p.first_row + column, p.end_row - 1);
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
-  const int limit = p.limit(a, token);
-  if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
-
-  const int tiles = (p.high + kKeys - 1) / kKeys;   // past the last
-  int tile = p.low / kKeys + wave;
-  PageWalk walk(a.at, p.sequence, tile * kKeys);
-  Rows rows;
+  const int2 whose = p.shared ? a.at.tokens[token] : int2{0, 0};
   rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
-  uint16_t* tile_k = (wave < 2 ? stage0 : stage1) + wave % 2 * 2 * kTile;
-  uint16_t* tile_v = tile_k + kTile;
+
+  const int first_tile = tile, tiles = (p.high + kKeys - 1) / kKeys;   // past the last
   const int chunk = lane % kChunks, stage_row = lane / kChunks;
   const uint32_t offset = stage_row * D + chunk * 8;
   u32x4 stage_k[kLoads], stage_v[kLoads];
   bool whole = false;
   uint32_t absent = 0;
+  // (Where one of two branches' loads of an address is nontemporal the compiler makes one of
+  // them that is not.)
+  const auto load = [](const uint16_t* from) {
+    return kStream ? load_nt(reinterpret_cast<const u32x4*>(from)) : *reinterpret_cast<const u32x4*>(from);
+  };
   auto load_tile = [&](int t) {
     const int key0 = t * kKeys;
     walk.reach(key0);
@@ -839,14 +841,14 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
       const uint16_t* from_k = a.keys + first[in / 16] + (in % 16) * D;
       const uint16_t* from_v = a.values + first[in / 16] + (in % 16) * D;
       if (whole) {
-        stage_k[i] = *reinterpret_cast<const u32x4*>(from_k + offset);
-        stage_v[i] = *reinterpret_cast<const u32x4*>(from_v + offset);
+        stage_k[i] = load(from_k + offset);
+        stage_v[i] = load(from_v + offset);
       } else {
         const int key = key0 + in + stage_row;
         stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
         if (((absent >> (in / 16)) & 1u) == 0 && key >= p.low && key < p.high) {
-          stage_k[i] = *reinterpret_cast<const u32x4*>(from_k + offset);
-          stage_v[i] = *reinterpret_cast<const u32x4*>(from_v + offset);
+          stage_k[i] = load(from_k + offset);
+          stage_v[i] = load(from_v + offset);
         }
       }
     }
@@ -854,6 +856,8 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
 
   bool odd = false;   // a value of this wave's keys was taken out, by this lane
   if (tile < tiles) load_tile(tile);
+  const int limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
+  if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
   while (tile < tiles) {
     const int key0 = tile * kKeys;
     const bool edge = __builtin_amdgcn_readfirstlane(p.mixed || !whole ? 1 : 0) != 0;
@@ -865,7 +869,7 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
       *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ Rows::turn_k(at)) * 8) = stage_k[i];
       *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ Rows::turn_v(at)) * 8) = stage_v[i];
     }
-    const int following = tile + kWaves;
+    const int following = tile + stride;
     if (following < tiles) load_tile(following);
     // The wave's lanes read what the others stored: LDS takes a wave's operations in order.
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
@@ -874,13 +878,46 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
     tile = following;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
   }
-  // A wave that took any out puts back its own keys' (every fourth tile's).
+  // A wave that took any out puts back its own tiles'.
   if (__ballot(odd) != 0) {
     const auto any = value_row<D>(a, p);
-    rows.put_odd(p.low, min(p.high, limit), quarter, [&](int key) {
-      return (key / kKeys - p.low / kKeys) % kWaves == wave ? any(key) : nullptr;
+    rows.put_odd(max(p.low, first_tile * kKeys), min(p.high, limit), quarter, [&](int key) {
+      return (key / kKeys - first_tile) % stride == 0 ? any(key) : nullptr;
     });
   }
+}
+
+// Four values of a row at `d`: for the merge, or the result where there is one piece a row.
+template <int D>
+__device__ __forceinline__ void store_four(const BatchArgs& a, const Piece& p, int row, int d, float top, float total,
+                                           const f32x4& v) {
+  const int splits = a.prefix_splits + a.own_splits;
+  const int head = p.kv_head * a.group + row % a.group;
+  const int64_t at = static_cast<int64_t>(row / a.group) * a.heads + head;
+  if (splits > 1) {
+    const int64_t part = at * splits + (p.shared ? p.split : a.prefix_splits + p.split);
+    store_part<D>(a, part, d, v);
+    if (d == 0) store_state<D>(a, part, top, total);
+    return;
+  }
+  const SinkTerm sink(a.sinks, head);
+  const float inverse = sink.inverse(top, total);
+  uint2 packed;
+  packed.x = pack_bf16(v[0] * inverse, v[1] * inverse);
+  packed.y = pack_bf16(v[2] * inverse, v[3] * inverse);
+  *reinterpret_cast<uint2*>(a.out + at * D + d) = packed;
+}
+
+// Up to 16 rows: the four waves hold the same rows, take every fourth tile each and merge at the
+// end.
+template <int D, int kParts>
+__device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, PageWalk& walk, uint16_t* stage0,
+                                             uint16_t* stage1) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int column = lane % 16, quarter = lane / 16;
+  NarrowRows<D, kParts> rows;
+  narrow_walk<D, kParts, false>(a, p, walk, rows, p.low / 32 + wave, kWaves,
+                         (wave < 2 ? stage0 : stage1) + wave % 2 * 2 * 32 * D);
 
   // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c] of the one
   // stage, its top and sum in the other.
@@ -891,13 +928,12 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
   lds_barrier();
   if (column < count) {
 #pragma unroll
-    for (int b = 0; b < Rows::kBlocks; ++b) {
+    for (int b = 0; b < D / 16; ++b) {
       *reinterpret_cast<f32x4*>(parts + (wave * kNarrowRows + column) * D + b * 16 + 4 * quarter) = rows.out[b];
     }
     if (quarter == 0) states[wave * kNarrowRows + column] = float2{rows.top, total};
   }
   lds_barrier();
-  const int splits = a.prefix_splits + a.own_splits;
   for (int item = threadIdx.x; item < count * (D / 4); item += 256) {
     const int r = item / (D / 4), d = item % (D / 4) * 4;
     float top = -INFINITY;
@@ -915,21 +951,7 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, uint16
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(part[i], factor, v[i]);
     }
-    const int global = p.first_row + r;
-    const int h = p.kv_head * a.group + global % a.group;
-    const int64_t at = static_cast<int64_t>(global / a.group) * a.heads + h;
-    if (splits > 1) {
-      const int64_t part = at * splits + (p.shared ? p.split : a.prefix_splits + p.split);
-      store_part<D>(a, part, d, v);
-      if (d == 0) store_state<D>(a, part, top, sum);
-    } else {
-      const SinkTerm sink(a.sinks, h);
-      const float inverse = sink.inverse(top, sum);
-      uint2 packed;
-      packed.x = pack_bf16(v[0] * inverse, v[1] * inverse);
-      packed.y = pack_bf16(v[2] * inverse, v[3] * inverse);
-      *reinterpret_cast<uint2*>(a.out + at * D + d) = packed;
-    }
+    store_four<D>(a, p, p.first_row + r, d, top, sum, v);
   }
 }
 
@@ -942,11 +964,42 @@ __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
                 "a stage holds what a narrow piece puts there");
   __shared__ int odd;   // a value was taken out
   Piece p;
-  if (!find_piece(a, p)) return;
+  find_piece(a, p);
+  PageWalk walk(a.at, p.sequence, p.low);
+  if (!find_keys(a, p)) return;
   if (p.end_row - p.first_row <= kNarrowRows) {
-    narrow_piece<D, kParts>(a, p, stage0, stage1);
+    narrow_piece<D, kParts>(a, p, walk, stage0, stage1);
   } else {
-    wide_piece<D, kParts>(a, p, stage0, stage1, &odd);
+    wide_piece<D, kParts>(a, p, walk, stage0, stage1, &odd);
+  }
+}
+
+// Own pieces alone, a wave each, so that none waits for another: 24 sequences of up to 16,000
+// rows take 92 us, with the four waves of a workgroup on one piece 115. Bound by memory, at 5.5
+// to 6.2 TB/s; what is read is past the caches' size, so it goes by them (24 of 4,776 rows: 103
+// -> 91 us; where it fits, it may be there still, and a nontemporal load costs a tenth). Pieces
+// of a tile of more than 16 rows take them 16 at a time.
+template <int D, int kParts>
+__global__ __launch_bounds__(64, 2) void attention_own_kernel(BatchArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t tile[2 * 32 * D];
+  Piece p;
+  find_piece(a, p);
+  const int first = p.first_row, end = p.end_row, token = p.token;
+  for (int row = first; row < end; row += kNarrowRows) {
+    p.first_row = row;
+    p.end_row = min(row + kNarrowRows, end);
+    PageWalk walk(a.at, p.sequence, p.low);
+    p.token = token + row / a.group - first / a.group;
+    if (!find_keys(a, p)) continue;
+    const int column = threadIdx.x % 16, quarter = threadIdx.x / 16;
+    NarrowRows<D, kParts> rows;
+    narrow_walk<D, kParts, true>(a, p, walk, rows, p.low / 32, 1, tile);
+    const float total = rows.whole_total();
+    if (column >= p.end_row - p.first_row) continue;
+#pragma unroll
+    for (int b = 0; b < D / 16; ++b) {
+      store_four<D>(a, p, p.first_row + column, b * 16 + 4 * quarter, rows.top, total, rows.out[b]);
+    }
   }
 }
 
@@ -1051,25 +1104,38 @@ void launch_merge(const BatchArgs& a, hipStream_t stream) {
 // so that sequences of different lengths fill the card evenly.
 struct Plan {
   int64_t prefix, prefix_tiles, prefix_splits, prefix_keys, own_splits, own_keys;
+  bool own_alone;   // own pieces only, a wave each
 };
 
-constexpr int64_t kWideBlocks = 512, kWideKeys = 256, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
+constexpr int64_t kSlots = 512, kWideKeys = 256, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
+constexpr int64_t kOwnKeys = 256, kOwnPieces = 2048;
 
-// Pieces of `keys` keys for each of `blocks` workgroups, and the keys of one.
-int64_t cut(int64_t blocks, int64_t keys, bool narrow, int64_t& each) {
-  each = kTileKeys;
-  if (keys <= 0 || blocks <= 0) return 0;
-  const int64_t target = narrow ? kNarrowBlocks : kWideBlocks, least = narrow ? kNarrowKeys : kWideKeys;
-  int64_t splits = (target + blocks - 1) / blocks;
-  const int64_t by_keys = keys / least;
-  splits = splits < by_keys ? splits : by_keys;
-  // Wide pieces run in rounds of as many as fit the card: fewer, where they fill theirs as well.
-  if (!narrow && splits > 1 && blocks * (splits - 1) <= target && blocks * (splits - 1) * 8 >= target * 7) --splits;
+// `splits` pieces of whole tiles of 64 keys, or as many as those leave, and the keys of one.
+int64_t cut(int64_t keys, int64_t splits, int64_t& each) {
   splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int64_t of_one = (tiles + splits - 1) / splits;
   each = of_one * kTileKeys;
   return (tiles + of_one - 1) / of_one;
+}
+
+// Pieces of `keys` keys for each of `blocks` workgroups, and the keys of one.
+int64_t pieces(int64_t blocks, int64_t keys, bool narrow, int64_t& each) {
+  each = kTileKeys;
+  if (keys <= 0 || blocks <= 0) return 0;
+  const auto fill = [&](int64_t target, int64_t least) {
+    const int64_t splits = (target + blocks - 1) / blocks, by_keys = keys / least;
+    return splits < by_keys ? splits : by_keys;
+  };
+  if (narrow) {
+    // Short ones where the slots would be left empty, else longer.
+    const int64_t splits = fill(kNarrowBlocks, kNarrowKeys);
+    return cut(keys, blocks * splits < kSlots ? fill(kSlots, kNarrowKeys / 4) : splits, each);
+  }
+  int64_t splits = fill(kSlots, kWideKeys);
+  // They run in rounds of as many as fit the card: fewer, where they fill theirs as well.
+  if (splits > 1 && blocks * (splits - 1) <= kSlots && blocks * (splits - 1) * 8 >= kSlots * 7) --splits;
+  return cut(keys, splits, each);
 }
 
 Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t own_rows, int64_t own_tiles) {
@@ -1078,11 +1144,24 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, i
   const int64_t shared_tiles = (rows + kTileRows - 1) / kTileRows;
   // Where the sequences' own tiles are nearly as full as shared ones (prompts), each walks the
   // shared rows as well: as many products, and nothing to merge.
-  p.prefix = own_tiles * 4 <= shared_tiles * 5 ? 0 : prefix;
+  // So do a few sequences of a few rows: one piece a row, and again nothing to merge (2 of 229
+  // rows: LATER).
+  const bool few = prefix + own_rows <= kNarrowKeys && kv_heads * own_tiles <= kSlots;
+  p.prefix = own_tiles * 4 <= shared_tiles * 5 || few ? 0 : prefix;
   own_rows += prefix - p.prefix;
   p.prefix_tiles = p.prefix > 0 ? shared_tiles : 0;
-  p.prefix_splits = cut(kv_heads * p.prefix_tiles, p.prefix, rows <= kNarrowRows, p.prefix_keys);
-  p.own_splits = cut(kv_heads * own_tiles, own_rows, rows <= kNarrowRows * own_tiles, p.own_keys);
+  p.prefix_splits = pieces(kv_heads * p.prefix_tiles, p.prefix, rows <= kNarrowRows, p.prefix_keys);
+  const bool narrow = rows <= kNarrowRows * own_tiles;
+  p.own_alone = p.prefix == 0 && narrow && kv_heads * own_tiles * own_rows >= kOwnPieces * kOwnKeys;
+  if (p.own_alone) {
+    // All at once where that is possible: a wave that has done its piece leaves the others more
+    // of the memory's rate, until the last ones cannot take it.
+    const int64_t fill = (kOwnPieces + kv_heads * own_tiles - 1) / (kv_heads * own_tiles);
+    const int64_t most = own_rows / kOwnKeys, least = own_rows / (4 * kOwnKeys);
+    p.own_splits = cut(own_rows, fill > most ? most : fill < least ? least : fill, p.own_keys);
+  } else {
+    p.own_splits = pieces(kv_heads * own_tiles, own_rows, narrow, p.own_keys);
+  }
   return p;
 }
 
@@ -1146,10 +1225,13 @@ extern "C" int32_t omnia_attention_batch_project(
                             static_cast<int>(width), static_cast<int>(pages), shift},
                            static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(tokens),
                            static_cast<int>(rotary_pairs), wide_queries != 0 ? 1 : 0, mscale, eps};
-  const int64_t of_one = 256 / (head_dim / 8) * kProjectHeads;
-  const int64_t parts = (heads + 2 * kv_heads + of_one - 1) / of_one;   // at most 192
+  const int64_t turns = tokens < 512 ? 1 : 4, of_one = 256 / (head_dim / 8) * turns;
+  const int64_t parts = (heads + 2 * kv_heads + of_one - 1) / of_one;   // at most 768
   const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(parts));
-  (head_dim == 64 ? attention_batch_project_kernel<64> : attention_batch_project_kernel<128>)<<<grid, 256, 0, stream>>>(a);
+  const auto kernel = head_dim == 64
+                          ? (turns == 1 ? attention_batch_project_kernel<64, 1> : attention_batch_project_kernel<64, 4>)
+                          : (turns == 1 ? attention_batch_project_kernel<128, 1> : attention_batch_project_kernel<128, 4>);
+  kernel<<<grid, 256, 0, stream>>>(a);
   return launched("attention_batch_project");
 }
 
@@ -1167,7 +1249,7 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
                                          const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
                                          int64_t width, const int32_t* lengths, const int32_t* token_map,
                                          int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
-                                         int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                          const uint16_t* sinks, float scale, void* workspace, int64_t workspace_bytes,
                                          uint16_t* out, hipStream_t stream) {
   using namespace omnia;
@@ -1178,6 +1260,8 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
   OMNIA_REQUIRE(pages > 0 && pages < (int64_t{1} << 31) && sequences > 0 && sequences < (int64_t{1} << 31) &&
                     width > 0 && width < (int64_t{1} << 31) / page_rows,
                 "attention_batch: bad tables");
+  OMNIA_REQUIRE(prefix == 0 || (prefix_sequence >= 0 && prefix_sequence < sequences),
+                "attention_batch: no such sequence to read the shared rows through");
   OMNIA_REQUIRE(scale > 0.0f && scale < INFINITY, "attention_batch: the scale must be positive");
   if (tokens == 0) return 0;
   OMNIA_REQUIRE(queries && keys && values && tables && lengths && token_map && out && (own_tiles == 0 || tiles),
@@ -1196,13 +1280,17 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
                     {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
                      static_cast<int>(width), static_cast<int>(pages), shift},
                     static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(heads / kv_heads),
-                    static_cast<int>(tokens), static_cast<int>(p.prefix), static_cast<int>(p.prefix_tiles),
-                    static_cast<int>(own_tiles), static_cast<int>(p.prefix_splits), static_cast<int>(p.prefix_keys),
+                    static_cast<int>(tokens), static_cast<int>(p.prefix), static_cast<int>(prefix_sequence),
+                    static_cast<int>(p.prefix_tiles), static_cast<int>(own_tiles), static_cast<int>(p.prefix_splits), static_cast<int>(p.prefix_keys),
                     static_cast<int>(p.own_splits), static_cast<int>(p.own_keys), scale * kLog2e};
   const int64_t blocks = kv_heads * (p.prefix_tiles * p.prefix_splits + own_tiles * p.own_splits);
   OMNIA_REQUIRE(blocks < (int64_t{1} << 31), "attention_batch: too many tiles");
-  if (blocks > 0) {
-    const bool wide = wide_queries != 0;
+  const bool wide = wide_queries != 0;
+  if (p.own_alone) {
+    const auto kernel = head_dim == 64 ? (wide ? attention_own_kernel<64, 2> : attention_own_kernel<64, 1>)
+                                       : (wide ? attention_own_kernel<128, 2> : attention_own_kernel<128, 1>);
+    kernel<<<dim3(static_cast<unsigned>(blocks)), 64, 0, stream>>>(a);
+  } else if (blocks > 0) {
     const auto kernel = head_dim == 64 ? (wide ? attention_batch_kernel<64, 2> : attention_batch_kernel<64, 1>)
                                        : (wide ? attention_batch_kernel<128, 2> : attention_batch_kernel<128, 1>);
     kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
@@ -1242,6 +1330,6 @@ extern "C" int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t
   if (rc != 0) return rc;
   return omnia_attention_batch(s->workspace, 1, s->keys, s->values, s->pages, s->page_rows, s->tables, s->sequences,
                                s->width, s->lengths, s->token_map, s->tokens, s->tiles, s->own_tiles, s->prefix,
-                               s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
+                               s->prefix_sequence, s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
                                static_cast<char*>(s->workspace) + queries, s->workspace_bytes - queries, s->out, stream);
 }

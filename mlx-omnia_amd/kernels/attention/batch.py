@@ -211,7 +211,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
             plan = ops.BatchStepPlan(
                 core.query_weight, core.key_weight, angles, cache.keys[core.layer], cache.values[core.layer],
                 cache.tables, cache.lengths, batch.token_map, batch.tiles(core.heads // core.kv_heads),
-                heads=core.heads, prefix=batch.prefix, scale=core.scale, eps=core.eps, mscale=core.mscale,
+                heads=core.heads, prefix=batch.prefix, prefix_sequence=batch.sequences[0], scale=core.scale, eps=core.eps, mscale=core.mscale,
                 sinks=core.sinks)
             batch.plans[self] = plan, cache.keys
         return plan, last

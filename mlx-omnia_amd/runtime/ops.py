@@ -1368,12 +1368,13 @@ def attention_batch(
     prefix: int,
     own_rows: int,
     scale: float,
+    prefix_sequence: int = 0,
     sinks: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attention of a batch's new tokens, queries [N, heads, D] bf16 or fp32, over a layer's pages; see
-    `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence,
-    own_rows bounds the rows past them, tiles [n, 4] are runs of one sequence's query rows;
+    `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence
+    (read through prefix_sequence's), own_rows bounds the rows past them, tiles [n, 4] are runs of one sequence's query rows;
     sinks [heads] bf16 or None -> [N, heads, D] bf16."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
     _dense(queries, F32 if queries.dtype == F32 else BF16, "queries")
@@ -1396,7 +1397,7 @@ def attention_batch(
     out = _out(out, queries, (tokens, heads, head_dim), BF16, "out")
     call("omnia_attention_batch", queries.data_ptr(), int(queries.dtype == F32), keys.data_ptr(), values.data_ptr(), pages, page_rows,
          tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), tokens, tiles.data_ptr(),
-         tiles.shape[0], prefix, own_rows, heads, kv_heads, head_dim,
+         tiles.shape[0], prefix, prefix_sequence, own_rows, heads, kv_heads, head_dim,
          sinks.data_ptr() if sinks is not None else None, float(scale),
          workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
     return out
@@ -1409,7 +1410,7 @@ class BatchStepPlan:
     arguments are those of `attention_batch_project` and `attention_batch`."""
 
     def __init__(self, query_weight, key_weight, angles, keys, values, tables, lengths, token_map, tiles, *, heads: int,
-                 prefix: int, scale: float, eps: float, mscale: float = 1.0, sinks=None) -> None:
+                 prefix: int, prefix_sequence: int, scale: float, eps: float, mscale: float = 1.0, sinks=None) -> None:
         pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch_step")
         sequences, width = _page_tables(tables, lengths, "attention_batch_step")
         tokens = token_map.shape[0]
@@ -1448,7 +1449,8 @@ class BatchStepPlan:
             table_stride=0 if cos is None else cos.stride(0) if cos.shape[0] > 1 else cos.shape[1],
             angle_rows=self.angle_rows or 0, rotary_pairs=0 if cos is None else cos.shape[1], tokens=tokens,
             heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=pages, page_rows=page_rows, sequences=sequences,
-            width=width, own_tiles=tiles.shape[0], prefix=prefix, own_rows=-1, mscale=mscale, eps=eps, scale=scale)
+            width=width, own_tiles=tiles.shape[0], prefix=prefix,
+            prefix_sequence=prefix_sequence, own_rows=-1, mscale=mscale, eps=eps, scale=scale)
         self.sized = -1, 0   # own rows, and the workspace that they need
 
     def _rows(self, raw: torch.Tensor, width: int, name: str) -> tuple[int, int, torch.Tensor]:

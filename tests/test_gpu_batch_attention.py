@@ -209,23 +209,26 @@ def test_infinite_sinks_and_scores():
     large.check()   # scores of some hundreds: nearly one weight a row
 
 
-def test_tokens_of_no_sequence_and_pages_of_no_pool():
-    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=64, own=(40, 40, 40))
+@pytest.mark.parametrize("prefix", [64, 640])
+def test_tokens_of_no_sequence_and_pages_of_no_pool(prefix):
+    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=prefix, own=(40, 40, 40))
     cache, batch = case.cache, case.batch
     queries = case.step.project(batch, *case.raw)
     tables, token_map = cache.tables.clone(), batch.token_map.clone()
     s = case.chosen[1]
-    tables[s, 4] = -1             # rows 64 .. 79 of one sequence are nowhere
-    tables[s, 5] = cache.pages    # nor are 80 .. 95
-    tables[case.chosen[2], 6] = -7
+    first = prefix // 16
+    tables[s, first] = -1                 # the first rows of one sequence's own are nowhere
+    tables[s, first + 1] = cache.pages    # nor are the next
+    tables[case.chosen[2], first + 2] = -7
+    tables[case.chosen, 1] = -1           # nor 16 of the shared ones
     token_map[0, 0] = cache.tables.shape[0] + 5
-    # The first token's sequence gives the shared rows: here the second's.
+    # The second token's sequence gives the shared rows.
     token_map[[0, 1]] = token_map[[1, 0]]
     tiles = batch.tiles(4).clone()
     tiles[:, 2] = token_map[:, 0]
     lengths = cache.lengths.cpu().numpy()
     out = ops.attention_batch(queries, cache.keys[1], cache.values[1], tables, cache.lengths, token_map, tiles,
-                              prefix=64, own_rows=41, scale=case.scale)
+                              prefix=prefix, prefix_sequence=s, own_rows=41, scale=case.scale)
     assert (out[1] == 0).all()
     want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), tables.cpu().numpy(), lengths,
                         token_map.cpu().numpy(), case.scale)
@@ -238,16 +241,18 @@ def test_tokens_of_no_sequence_and_pages_of_no_pool():
     assert torch.equal(before.view(torch.int16), cache.keys.view(torch.int16))
 
 
-def test_sequences_shorter_than_the_shared_rows():
+@pytest.mark.parametrize("prefix,own", [(160, (9, 4, 1)), (640, (9, 4, 1)), (1600, (9, 4, 1, 30) * 4)])
+def test_sequences_shorter_than_the_shared_rows(prefix, own):
     """A plan that is not the cache's own: a sequence that ends inside the shared rows sees its
     rows of them and no more."""
-    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=160, own=(9, 4, 1))
+    case = Case(heads=8, kv_heads=2, head_dim=128, page_rows=16, prefix=prefix, own=own)
     cache, batch = case.cache, case.batch
     queries = case.step.project(batch, *case.raw)
     lengths = cache.lengths.clone()
-    lengths[case.chosen[1]], lengths[case.chosen[2]] = 70, -1
+    lengths[case.chosen[1]], lengths[case.chosen[2]] = prefix // 2 - 10, -1
     out = ops.attention_batch(queries, cache.keys[1], cache.values[1], cache.tables, lengths, batch.token_map,
-                              batch.tiles(4), prefix=160, own_rows=10, scale=case.scale)
+                              batch.tiles(4), prefix=prefix, prefix_sequence=case.chosen[0], own_rows=31,
+                              scale=case.scale)
     want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), cache.tables.cpu().numpy(),
                         lengths.cpu().numpy(), batch.token_map.cpu().numpy(), case.scale)
     assert (out[2] == 0).all()
@@ -443,6 +448,8 @@ def test_ops_refuse():
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map[:1], tiles, **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles[:, :2], **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles.cpu(), **base),
+        lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles,
+                                    prefix_sequence=cache.tables.shape[0], **base),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles, prefix=-1,
                                     own_rows=5, scale=1.0),
         lambda: ops.attention_batch(q, keys, values, cache.tables, cache.lengths, batch.token_map, tiles, prefix=32,
