@@ -9,7 +9,7 @@ of it, and a call names the `PagedBatch` that steps.
   with or without gains, a rotary table and sinks, any number of new tokens a sequence. The
   rows that the batch's sequences share are read once for all of them.
 - `DefaultBatchAttentionStep` is the Core chain, a sequence at a time in torch ops (fp32). It
-  accepts everything.
+  accepts everything, calls that autograd follows among it: gradients of the step's own q, k and v.
 
 The norm, the rotation and mscale are rounded once, as one operation (`AttentionStep` rounds
 after each, as its reference does).
@@ -94,7 +94,8 @@ class DefaultBatchAttentionStep(BatchAttentionStepStrategy):
         a, b = x[..., :p] * self.mscale, x[..., p : 2 * p] * self.mscale
         return torch.cat([a * cos - b * sin, a * sin + b * cos, x[..., 2 * p :]], dim=-1)
 
-    def project(self, batch, raw_queries, raw_keys, raw_values):
+    def _project(self, batch, raw_queries, raw_keys, raw_values):
+        """The tokens' queries, and their key and value rows as they were written."""
         d, cache, size = self.head_dim, self.cache, self.cache.page_rows
         _check_rows(batch, raw_queries, self.heads * d, "raw_queries")
         _check_rows(batch, raw_keys, self.kv_heads * d, "raw_keys")
@@ -114,19 +115,26 @@ class DefaultBatchAttentionStep(BatchAttentionStepStrategy):
         whose = torch.repeat_interleave(batch.chosen.long(), batch.rows.long())
         page = cache.tables[whose, at // size].long()
         kind = cache.keys.dtype
-        cache.keys[self.layer, page, :, at % size] = k.to(kind)
-        cache.values[self.layer, page, :, at % size] = raw_values.reshape(batch.total, -1, d).to(kind)
-        return q.to(raw_queries.dtype)
+        k, v = k.to(kind), raw_values.reshape(batch.total, -1, d).to(kind)
+        # The pool itself follows no gradient: rows of earlier steps are constants.
+        cache.keys[self.layer, page, :, at % size] = k.detach()
+        cache.values[self.layer, page, :, at % size] = v.detach()
+        return q.to(raw_queries.dtype), k, v
 
-    def _attend(self, batch: PagedBatch, queries: torch.Tensor) -> torch.Tensor:
+    def project(self, batch, raw_queries, raw_keys, raw_values):
+        return self._project(batch, raw_queries, raw_keys, raw_values)[0]
+
+    def _attend(self, batch: PagedBatch, queries: torch.Tensor, new_keys: torch.Tensor,
+                new_values: torch.Tensor) -> torch.Tensor:
         cache, d, kv = self.cache, self.head_dim, self.kv_heads
         group, out, end = self.heads // kv, [], 0
         for s, count in zip(batch.sequences, batch.tokens):
             before, first = int(cache._rows[s]), end
             rows, end = before + count, first + count
             pages = cache.tables[s, : -(-rows // cache.page_rows)].long()
-            keys, values = (pool[self.layer, pages].transpose(0, 1).reshape(kv, -1, d)[:, :rows].float()
-                            for pool in (cache.keys, cache.values))
+            keys, values = (torch.cat([pool[self.layer, pages].transpose(0, 1).reshape(kv, -1, d)[:, :before],
+                                       new[first:end].transpose(0, 1)], dim=1).float()
+                            for pool, new in ((cache.keys, new_keys), (cache.values, new_values)))
             q = queries[first:end].float().unflatten(1, (kv, group)).permute(1, 2, 0, 3).reshape(kv, group * count, d)
             scores = (q @ keys.transpose(1, 2).contiguous()).unflatten(1, (group, count)) * self.scale
             seen = (torch.arange(rows, device=q.device)[None]
@@ -146,7 +154,7 @@ class DefaultBatchAttentionStep(BatchAttentionStepStrategy):
         return torch.cat(out).to(queries.dtype)
 
     def __call__(self, batch, raw_queries, raw_keys, raw_values):
-        return self._attend(batch, self.project(batch, raw_queries, raw_keys, raw_values))
+        return self._attend(batch, *self._project(batch, raw_queries, raw_keys, raw_values))
 
 
 @dataclass(frozen=True, eq=False)
@@ -211,9 +219,11 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
             plan = ops.BatchStepPlan(
                 core.query_weight, core.key_weight, angles, cache.keys[core.layer], cache.values[core.layer],
                 cache.tables, cache.lengths, batch.token_map, batch.tiles(core.heads // core.kv_heads),
-                heads=core.heads, prefix=batch.prefix, prefix_sequence=batch.sequences[0], scale=core.scale, eps=core.eps, mscale=core.mscale,
-                sinks=core.sinks)
+                heads=core.heads, prefix=batch.prefix, prefix_sequence=batch.sequences[0], scale=core.scale,
+                eps=core.eps, mscale=core.mscale, sinks=core.sinks)
             batch.plans[self] = plan, cache.keys
+        if batch.reach and _capturing(cache.keys.device) and all(plan is not held for held in batch.captured):
+            batch.captured.append(plan)   # and with it the angles, should the atlas grow
         return plan, last
 
     def _followed(self, *raw: torch.Tensor) -> bool:

@@ -23,6 +23,8 @@ the current stream with what the kernels do.
     cache.free(answers)
 
 A page id that is handed out is the lowest one free, so the same calls give the same tables.
+One thread at a time calls a cache, and the steps over it; the kernels of its calls run on
+streams that are ordered among themselves, as with any tensor that is written.
 """
 
 from __future__ import annotations
@@ -73,6 +75,7 @@ class PagedBatch:
         self.epoch = cache._epoch     # at which its sequences were last seen to be the same
         self.last = 0                 # the most rows a sequence has in the step at hand
         self.plans: dict = {}         # what a layer's binding laid out for the batch
+        self.captured: list = []      # of those, the ones that graphs read
         self._tiles: dict[int, torch.Tensor] = {}
 
     def tiles(self, group: int) -> torch.Tensor:
@@ -127,6 +130,9 @@ class PagedKVCache:
         self._check_tables()
         self._refs = np.zeros(pages, dtype=np.int64)
         np.add.at(self._refs, self._tables[self._tables >= 0], 1)
+        spare = (np.arange(self._tables.shape[1]) >= -(-self._rows[:, None] // page_rows)) & (self._tables >= 0)
+        if (self._refs[self._tables[spare]] > 1).any():
+            raise ValueError("PagedKVCache: a page past a sequence's rows is another sequence's as well")
         self._generation = np.zeros(len(self._tables), dtype=np.int64)   # of a slot: whose it is
         self._epoch = 0                                                  # of them all
         self._clock = 0                                                  # turns as sequences grow
@@ -382,7 +388,7 @@ class PagedKVCache:
     def free(self, sequences: Sequence[int] | int) -> None:
         """Close sequences; the pages that no other one holds are free again."""
         self._refuse_capture("freeing")
-        gone = [sequences] if isinstance(sequences, int) else list(sequences)
+        gone = [int(s) for s in ([sequences] if isinstance(sequences, (int, np.integer)) else sequences)]
         if len(set(gone)) != len(gone):
             raise ValueError("PagedKVCache: a sequence to free is named twice")
         self._known(gone)
@@ -464,7 +470,7 @@ class PagedKVCache:
         if not chosen or len(set(chosen)) != len(chosen):
             raise ValueError("PagedKVCache: a batch names at least one sequence, each once")
         self._known(chosen)
-        counts = [int(tokens)] * len(chosen) if isinstance(tokens, int) else [int(n) for n in tokens]
+        counts = [int(tokens)] * len(chosen) if isinstance(tokens, (int, np.integer)) else [int(n) for n in tokens]
         if len(counts) != len(chosen) or min(counts) < 1:
             raise ValueError("PagedKVCache: every sequence of a batch has at least one new token")
         shared = 0
@@ -484,18 +490,23 @@ class PagedKVCache:
 
     def ready(self, batch: PagedBatch) -> int:
         """Make sure of the pages of the batch's step; the most rows any of its sequences has
-        then, or may have in the replays that were prepared for."""
+        then, or may have in the replays that were prepared for, if it is being captured."""
         self._current(batch)
         if batch.clock != self._clock:
             rows = self._rows[batch.index] + batch.counts
             self._reserve(batch.index, rows)
             batch.clock, batch.last = self._clock, int(rows.max())
-        return max(batch.last, batch.reach) if batch.reach and _capturing(self.keys.device) else batch.last
+        if not _capturing(self.keys.device):
+            return batch.last
+        if batch.reach < batch.last:
+            raise ValueError("a batch's step is captured after prepare_capture has reserved what its replays reach")
+        return batch.reach
 
     def prepare_capture(self, batch: PagedBatch, steps: int) -> int:
         """Reserve the pages of the batch's next `steps` steps, before a step and its `advance`
         are captured; the most rows a sequence has after them. Replays past that are outside
-        the contract (their rows are not stored)."""
+        the contract (their rows are not stored, nor those past the reach attended). The batch
+        holds what the graph reads and lives as long."""
         self._current(batch)
         if steps < 1:
             raise ValueError("PagedKVCache: a captured step is replayed at least once")

@@ -1374,8 +1374,9 @@ def attention_batch(
 ) -> torch.Tensor:
     """Attention of a batch's new tokens, queries [N, heads, D] bf16 or fp32, over a layer's pages; see
     `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence
-    (read through prefix_sequence's), own_rows bounds the rows past them, tiles [n, 4] are runs of one sequence's query rows;
-    sinks [heads] bf16 or None -> [N, heads, D] bf16."""
+    (read through prefix_sequence's), own_rows bounds the rows past them of any of its sequences
+    (rows past the bound are not attended), tiles [n, 4] are runs of one sequence's query rows, as
+    token_map has them; sinks [heads] bf16 or None -> [N, heads, D] bf16."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
     _dense(queries, F32 if queries.dtype == F32 else BF16, "queries")
     _require(queries.dim() == 3 and queries.shape[2] == head_dim, "attention_batch: queries must be [N, heads, D]")

@@ -172,7 +172,10 @@ def test_refusals():
     dict(tables=np.array([[1, -2]]), lengths=np.array([3]), opened=[0]), dict(sequences=0, rows=3),
     dict(sequences=2, rows=16, opened=[0]), dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[-1]),
     dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[0, 1]),
-    dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[0, 0])])
+    dict(tables=np.array([[1, -1]]), lengths=np.array([3]), opened=[0, 0]),
+    # a page that both sequences would write next, one shared and one not yet reached
+    dict(tables=np.array([[0, 1], [2, 1]]), lengths=np.array([16, 16]), opened=[0, 1]),
+    dict(tables=np.array([[0, 1], [2, 1]]), lengths=np.array([16, 20]), opened=[0, 1])])
 def test_tables_that_do_not_hold_together_are_refused(change):
     pool = torch.zeros((1, 4, 2, 16, 8))
     with pytest.raises(ValueError):
@@ -193,6 +196,18 @@ def test_any_order_of_calls_keeps_every_sequence(seed):
     rng = np.random.default_rng(seed)
     cache = small(pages=int(rng.integers(8, 30)), page_rows=16, sequences=int(rng.integers(2, 9)), rows=100)
     random_calls(cache, PagedModel(), rng, 120)
+
+
+def test_whole_numbers_of_numpy():
+    cache = small()
+    a, b = cache.open(np.int64(3)), cache.open(5)
+    batch = cache.batch(np.array([a, b]), tokens=np.int32(2))
+    cache.ready(batch)
+    cache.advance(batch)
+    assert cache.rows(np.int64(a)) == 5
+    cache.free(np.int64(a))
+    cache.free(np.array([b]))
+    assert cache.free_pages == cache.pages
 
 
 def test_a_cache_is_taken_up_as_it_was_left():
@@ -261,6 +276,52 @@ def test_core_chain_keeps_a_later_tokens_infinity_from_an_earlier_one():
     v[2, 3] = float("inf")
     out = step(batch, torch.ones(3, 8), torch.ones(3, 8), v)
     assert torch.isfinite(out[:2]).all() and torch.isinf(out[2, 0, 3]) and torch.isfinite(out[2, 0, :3]).all()
+
+
+def test_gradients_of_a_steps_own_rows():
+    """Against the formula in 64 bits and its central differences; earlier rows are constants, and
+    the pool keeps no graph. The step's operations are some thousand fp32 ones a number, none of
+    which cancels by more than the 2^6 that the sums of its terms' sizes allow: 2^-24 2^6 2^5."""
+    gen = torch.Generator().manual_seed(2)
+    heads, kv, d, scale = 4, 2, 8, 0.4
+    cache = PagedKVCache.empty(2, 9, 16, kv, d, sequences=3, rows=48, dtype=torch.float32)
+    for pool in (cache.keys, cache.values):
+        pool.copy_(torch.randn(pool.shape, generator=gen))
+    chosen = [cache.open(21)]
+    chosen += cache.fork(chosen[0])
+    counts = [3, 1]
+    batch = cache.batch(chosen, tokens=counts)
+    step = BatchAttentionStep(cache, layer=1, heads=heads, kv_heads=kv, head_dim=d, scale=scale, dtype=torch.float32)
+    old = [[torch.stack([pool[1, cache.tables[s, r // 16], :, r % 16] for r in range(21)]).double() for s in chosen]
+           for pool in (cache.keys, cache.values)]
+    raw = [torch.randn(batch.total, n * d, generator=gen) for n in (heads, kv, kv)]
+    weight = torch.randn(batch.total, heads, d, generator=gen)
+
+    def formula(q, k, v):
+        total, at = 0.0, 0
+        for i, n in enumerate(counts):
+            for t in range(n):
+                for h in range(heads):
+                    keys, values = (torch.cat([o[i][:, h // 2], new[at : at + t + 1].unflatten(1, (kv, d))[:, h // 2]])
+                                    for o, new in zip(old, (k, v)))
+                    p = torch.softmax(keys @ q[at + t].unflatten(0, (heads, d))[h] * scale, dim=0)
+                    total = total + (p @ values) @ weight[at + t, h].double()
+            at += n
+        return total
+
+    mine = [t.clone().requires_grad_() for t in raw]
+    (step(batch, *mine) * weight).sum().backward()
+    exact = [t.double().requires_grad_() for t in raw]
+    formula(*exact).backward()
+    for got, want in zip(mine, exact):
+        assert (got.grad.double() - want.grad).abs().max() <= 2.0 ** -13 * want.grad.abs().max()
+    along = [torch.randn(t.shape, generator=gen, dtype=torch.float64) for t in raw]
+    h = 1e-5   # the differences' own error: h^2 of a third derivative of some hundreds, 2^-52 of some tens / h
+    ends = [formula(*(t.double() + sign * h * a for t, a in zip(raw, along))) for sign in (1, -1)]
+    slope = sum((t.grad * a).sum() for t, a in zip(exact, along))
+    assert abs((ends[0] - ends[1]) / (2 * h) - slope) <= 1e-6 * (1 + abs(slope))
+    assert not cache.keys.requires_grad and not cache.values.requires_grad
+    assert torch.equal(step(batch, *raw), step(batch, *mine).detach())
 
 
 def test_step_declarations():
