@@ -1145,7 +1145,7 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, i
   // Where the sequences' own tiles are nearly as full as shared ones (prompts), each walks the
   // shared rows as well: as many products, and nothing to merge.
   // So do a few sequences of a few rows: one piece a row, and again nothing to merge (2 of 229
-  // rows: LATER).
+  // rows: 16 -> 13.4 us a step).
   const bool few = prefix + own_rows <= kNarrowKeys && kv_heads * own_tiles <= kSlots;
   p.prefix = own_tiles * 4 <= shared_tiles * 5 || few ? 0 : prefix;
   own_rows += prefix - p.prefix;

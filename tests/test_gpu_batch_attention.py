@@ -13,6 +13,8 @@ Tolerances, from the roundings the kernels make (half a step of bf16 is 2^-8 of 
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -169,6 +171,40 @@ GEOMETRIES = [
     dict(heads=16, kv_heads=1, head_dim=128, page_rows=16, prefix=0, own=(777,), tokens=33),
     dict(heads=129, kv_heads=1, head_dim=64, page_rows=16, prefix=32, own=(3, 9), tokens=(2, 3)),
 ]
+
+
+# What a plan chooses by: shared rows read once, for tiles of some rows, of many and of many tokens;
+# own rows alone, past the caches, a tile of more than 16 rows among them; steps beside prompts.
+PLANS = [
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=640, own=(5, 0, 17), tokens=(2, 1, 3)),
+    dict(heads=16, kv_heads=2, head_dim=64, sinks=True, prefix=1008, own=(3, 30, 9, 1, 70, 64), tokens=(1, 9, 1, 1, 17, 2)),
+    dict(heads=32, kv_heads=2, head_dim=128, page_rows=64, prefix=704, own=tuple(range(12)), tokens=2),
+    dict(heads=16, kv_heads=4, head_dim=128, page_rows=32, prefix=1024, own=tuple((i * 29) % 130 for i in range(40))),
+    dict(heads=8, kv_heads=1, head_dim=64, page_rows=16, prefix=4000, own=(1, 2, 3, 4), tokens=(1, 1, 1, 5)),
+    dict(heads=16, kv_heads=8, head_dim=64, pairs=32, sinks=True, page_rows=256, prefix=0, own=(3000,) * 21 + (0, 1, 256)),
+    dict(heads=24, kv_heads=8, head_dim=128, page_rows=64, prefix=0, own=(2900, 17, 0) + (2750,) * 21,
+         tokens=(1, 20, 6) + (1,) * 21),
+    dict(heads=16, kv_heads=4, head_dim=128, pairs=64, page_rows=64, prefix=0, own=(700, 0, 1500, 9, 64), tokens=(1, 300, 1, 2, 75)),
+    dict(heads=16, kv_heads=4, head_dim=64, page_rows=16, prefix=320, own=(700, 0, 9, 64), tokens=(1, 150, 1, 1)),
+]
+
+
+@pytest.mark.parametrize("case", PLANS, ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", ""))
+def test_plans(case):
+    made = Case(**case)
+    made.check(None if made.batch.total * made.heads < 2000 else np.arange(0, made.batch.total, 7))
+
+
+def test_values_that_are_not_finite_among_own_rows_alone():
+    """Rows behind a token's own are not there for it, whatever they hold, 16 rows of a tile at a time."""
+    case = Case(heads=24, kv_heads=8, head_dim=128, page_rows=64, own=(2900, 17) + (2750,) * 21, tokens=(1, 20) + (1,) * 21)
+    clean = case.step(case.batch, *case.raw)
+    v = case.raw[2].view(case.batch.total, 8, 128)
+    v[9, 3, 40] = float("inf")
+    out = case.step(case.batch, *case.raw)
+    touched = torch.zeros_like(out, dtype=torch.bool)
+    touched[9:21, 9:12, 40] = True
+    assert torch.equal(out[~touched], clean[~touched]) and (out[touched] == float("inf")).all()
 
 
 @pytest.mark.parametrize("case", GEOMETRIES, ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", ""))
@@ -338,6 +374,53 @@ def test_steps_that_are_captured():
         assert torch.equal(step(batch, *raw), eager(eager_batch, *raw))
 
 
+def test_a_step_is_not_captured_for_fewer_rows_than_it_will_have():
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
+    cache, batch, step = case.cache, case.batch, case.step
+    step.prepare_capture(batch, 1)
+    step(batch, *case.raw)
+    cache.advance(batch)   # the one step that was prepared for
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device="cuda")
+        with pytest.raises(ValueError, match="prepare_capture"):
+            step(batch, *case.raw)
+    torch.cuda.synchronize()
+
+
+def test_a_graph_keeps_the_angles_it_was_captured_with():
+    """The atlas grows, for another step, while a graph that reads its first rows lives."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
+    atlas = AngleAtlas(32, base=1e4, rows=64, device="cuda")
+    step = BatchAttentionStep(case.cache, layer=1, heads=8, kv_heads=2, head_dim=64, scale=0.1, dtype=torch.bfloat16,
+                              rotary_pairs=32, angles=atlas)
+    want = step(case.batch, *case.raw)
+    step.prepare_capture(case.batch, 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(case.batch, *case.raw)
+    assert len(case.batch.captured) == 1
+    atlas.ensure(5000)
+    case.batch.plans.clear()
+    for _ in range(3):
+        filler = [torch.full((64, 64), 3.0, device="cuda") for _ in range(50)]   # where freed rows would lie
+        graph.replay()
+        assert torch.equal(out, want) and len(filler) == 50
+        assert torch.equal(step(case.batch, *case.raw), want)
+
+
+def test_gradients_go_to_a_steps_own_rows():
+    """Against the Core chain's, whose gradients are tested against the formula: the same chain."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4), tokens=(2, 1))
+    grads = []
+    for step in (case.step, case.make(case.cache, reference=True)):
+        raw = [t.clone().requires_grad_() for t in case.raw]
+        step(case.batch, *raw).float().square().sum().backward()
+        grads.append([t.grad for t in raw])
+    assert all(torch.equal(a, b) and a.abs().max() > 0 for a, b in zip(*grads))
+    assert not case.cache.keys.requires_grad
+
+
 def test_what_cannot_be_captured_is_refused():
     case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
     cache = case.cache
@@ -364,6 +447,52 @@ def test_another_stream():
         got = [case.step(case.batch, *case.raw) for _ in range(3)]
     torch.cuda.current_stream().wait_stream(stream)
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_two_threads_with_a_cache_each():
+    made = [Case(heads=16, kv_heads=4, head_dim=128, pairs=64, page_rows=32, prefix=640, own=(3, 70 + i, 9), seed=i)
+            for i in range(2)]
+    want = [case.step(case.batch, *case.raw) for case in made]
+    got: list = [[], []]
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(made[i].step(made[i].batch, *made[i].raw))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for mine, all_of in zip(want, got):
+        assert len(all_of) == 20 and all(torch.equal(g, mine) for g in all_of)
+
+
+def test_a_pool_that_grows_and_many_forks():
+    """More children than one launch takes, then a pool of another size, then a step of them all."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, page_rows=16, prefix=0, own=(45,))
+    parent, cache = case.chosen[0], case.cache
+    wanted = cache.keys[1, cache.pages_of(parent)[2], :, :13].clone()
+    grown = PagedKVCache.empty(2, 400, 16, 2, 64, device="cuda", sequences=300, rows=100)
+    assert grown.open(45) == 0
+    for mine, theirs in ((grown.keys, cache.keys), (grown.values, cache.values)):
+        mine[:, grown.pages_of(0)] = theirs[:, cache.pages_of(parent)]
+    kids = grown.fork(0, 270)
+    assert all(torch.equal(grown.keys[1, grown.pages_of(kid)[2], :, :13], wanted) for kid in (kids[0], *kids[127:131], kids[-1]))
+    step = case.make(grown)
+    batch = grown.batch(kids)
+    raw = [case.normal(270, n * 64) for n in (8, 2, 2)]
+    want = step(batch, *raw)
+    grown.resize(600)
+    assert torch.equal(step(grown.batch(kids), *raw), want)
+    few = step(grown.batch(kids[:5]), *(t[:5] for t in raw))
+    grown.free(kids[5:])
+    assert grown.compact() == 8
+    grown.resize(8)
+    assert torch.equal(step(grown.batch(kids[:5]), *(t[:5] for t in raw)), few)
 
 
 def test_pools_past_32_bits():
