@@ -688,6 +688,34 @@ int32_t omnia_pages_fork(uint16_t* keys, uint16_t* values, int64_t layers, int64
 int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t sequences, int64_t width,
                          int64_t pages, const int32_t* edits, int64_t count, hipStream_t stream);
 
+/* A cache of pages: what the host keeps of it, beside the pool and the tables on the device. The
+ * host's arrays are the caller's, in HOST memory, and say the same as the device's:
+ *   host_tables [sequences, width], rows [sequences] (the lengths), held [sequences] (how many
+ *   pages a sequence lies on, its first entries), refs [pages] (how many sequences hold a page;
+ *   0: free), generation [sequences] (grows as a sequence begins, ends or is cut short),
+ *   open [sequences] (1 or 0).
+ * One call at a time works on a cache. */
+typedef struct {
+  uint16_t *keys, *values;
+  int32_t *tables, *lengths;
+  int32_t* host_tables;
+  int64_t *rows, *held, *refs, *generation;
+  uint8_t* open;
+  int64_t layers, pages, kv_heads, page_rows, head_dim, sequences, width;
+} omnia_paged_cache_t;
+
+/* Begins `count` sequences with the rows of `parent`: its full pages shared, the last, partly
+ * filled one copied for each (omnia_pages_fork), the pages and sequences the lowest that are
+ * free. kids [count, 2] int32 in HOST memory takes their (sequence, page). A refused call
+ * leaves everything as it was. */
+int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* cache, int64_t parent, int64_t count, int32_t* kids,
+                               hipStream_t stream);
+
+/* Ends the sequences gone [count] int32 in HOST memory: the pages that no other one holds are
+ * free. A refused call leaves everything as it was. */
+int32_t omnia_paged_cache_free(const omnia_paged_cache_t* cache, const int32_t* gone, int64_t count,
+                               hipStream_t stream);
+
 /* lengths[chosen[i]] += rows[i] for i < count, all on the device; the chosen are distinct. An
  * index outside [0, sequences) is passed over. */
 int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* chosen,

@@ -328,6 +328,123 @@ extern "C" int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t s
   return launched("pages_edit");
 }
 
+// What the host keeps of a cache changes only once the device's part has been launched, so a
+// refused or failed call leaves it as it was.
+extern "C" int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* c, int64_t parent, int64_t count, int32_t* kids,
+                                          hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(c && c->host_tables && c->rows && c->held && c->refs && c->generation && c->open,
+                "paged_cache_fork: null pointer");
+  OMNIA_REQUIRE(!bad_tables(c->sequences, c->width, c->pages) && c->page_rows > 0, "paged_cache_fork: bad tables");
+  if (parent < 0 || parent >= c->sequences || c->open[parent] == 0) {
+    return fail(-EINVAL, "paged_cache_fork: sequence " + std::to_string(parent) + " is not open");
+  }
+  OMNIA_REQUIRE(count >= 0, "paged_cache_fork: fewer than no forks");
+  if (count == 0) return 0;
+  OMNIA_REQUIRE(kids, "paged_cache_fork: null pointer");
+  const int64_t full = c->rows[parent] / c->page_rows, rest = c->rows[parent] % c->page_rows;
+  const int32_t* line = c->host_tables + parent * c->width;
+  OMNIA_REQUIRE(full + (rest > 0 ? 1 : 0) <= c->held[parent] && c->held[parent] <= c->width,
+                "paged_cache_fork: a sequence holds more rows than pages");
+  for (int64_t i = 0; i < full; ++i) {
+    OMNIA_REQUIRE(line[i] >= 0 && line[i] < c->pages, "paged_cache_fork: a table names a page outside the pool");
+  }
+  int64_t found = 0;
+  for (int64_t s = 0; s < c->sequences && found < count; ++s) {
+    if (c->open[s] == 0) kids[2 * found++] = static_cast<int32_t>(s);
+  }
+  if (found < count) {
+    return fail(-EINVAL, "paged_cache_fork: " + std::to_string(count) + " more sequences are asked for, " +
+                             std::to_string(found) + " of " + std::to_string(c->sequences) + " are not open");
+  }
+  found = 0;
+  if (rest > 0) {
+    for (int64_t p = 0; p < c->pages && found < count; ++p) {
+      if (c->refs[p] == 0) kids[2 * found++ + 1] = static_cast<int32_t>(p);
+    }
+    if (found < count) {
+      return fail(-EINVAL, "paged_cache_fork: " + std::to_string(count) + " more pages are needed, " +
+                               std::to_string(found) + " of " + std::to_string(c->pages) + " are free");
+    }
+  } else {
+    for (int64_t i = 0; i < count; ++i) kids[2 * i + 1] = -1;
+  }
+  for (int64_t first = 0; first < count; first += OMNIA_PAGES_MOVES) {
+    const int64_t some = count - first < OMNIA_PAGES_MOVES ? count - first : OMNIA_PAGES_MOVES;
+    const int32_t rc = omnia_pages_fork(c->keys, c->values, c->layers, c->pages, c->kv_heads, c->page_rows, c->head_dim,
+                                        c->tables, c->lengths, c->sequences, c->width, parent, full,
+                                        rest > 0 ? line[full] : -1, rest, kids + 2 * first, some, stream);
+    if (rc != 0) return rc;
+  }
+  for (int64_t i = 0; i < full; ++i) c->refs[line[i]] += count;
+  for (int64_t i = 0; i < count; ++i) {
+    const int32_t s = kids[2 * i], page = kids[2 * i + 1];
+    int32_t* entries = c->host_tables + s * c->width;
+    for (int64_t e = 0; e < full; ++e) entries[e] = line[e];
+    if (page >= 0) {
+      entries[full] = page;
+      c->refs[page] = 1;
+    }
+    c->held[s] = full + (page >= 0 ? 1 : 0);
+    c->rows[s] = c->rows[parent];
+    c->generation[s] += 1;
+    c->open[s] = 1;
+  }
+  return 0;
+}
+
+extern "C" int32_t omnia_paged_cache_free(const omnia_paged_cache_t* c, const int32_t* gone, int64_t count,
+                                          hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(c && c->host_tables && c->rows && c->held && c->refs && c->generation && c->open,
+                "paged_cache_free: null pointer");
+  OMNIA_REQUIRE(!bad_tables(c->sequences, c->width, c->pages), "paged_cache_free: bad tables");
+  OMNIA_REQUIRE(count >= 0, "paged_cache_free: bad count");
+  if (count == 0) return 0;
+  OMNIA_REQUIRE(gone, "paged_cache_free: null pointer");
+  // Those seen are marked in `open` until all are.
+  constexpr uint8_t kSeen = 2;
+  int64_t seen = 0;
+  int32_t rc = 0;
+  while (seen < count && rc == 0) {
+    const int32_t s = gone[seen];
+    if (s < 0 || s >= c->sequences || c->open[s] == 0) {
+      rc = fail(-EINVAL, "paged_cache_free: sequence " + std::to_string(s) + " is not open");
+    } else if (c->open[s] == kSeen) {
+      rc = fail(-EINVAL, "paged_cache_free: a sequence to free is named twice");
+    } else if (c->held[s] < 0 || c->held[s] > c->width) {
+      rc = fail(-EINVAL, "paged_cache_free: a sequence holds more pages than its table");
+    } else {
+      c->open[s] = kSeen;
+      ++seen;
+    }
+  }
+  for (int64_t i = 0; i < seen; ++i) c->open[gone[i]] = 1;
+  for (int64_t first = 0; first < count && rc == 0; first += OMNIA_PAGES_EDITS) {
+    const int64_t some = count - first < OMNIA_PAGES_EDITS ? count - first : OMNIA_PAGES_EDITS;
+    int32_t edits[4 * OMNIA_PAGES_EDITS];
+    for (int64_t i = 0; i < some; ++i) {
+      edits[4 * i] = OMNIA_PAGES_CLEAR;
+      edits[4 * i + 1] = gone[first + i];
+      edits[4 * i + 2] = edits[4 * i + 3] = 0;
+    }
+    rc = omnia_pages_edit(c->tables, c->lengths, c->sequences, c->width, c->pages, edits, some, stream);
+  }
+  if (rc != 0) return rc;
+  for (int64_t i = 0; i < count; ++i) {
+    const int32_t s = gone[i];
+    int32_t* entries = c->host_tables + s * c->width;
+    for (int64_t e = 0; e < c->held[s]; ++e) {
+      if (entries[e] >= 0 && entries[e] < c->pages) c->refs[entries[e]] -= 1;
+      entries[e] = -1;
+    }
+    c->held[s] = c->rows[s] = 0;
+    c->generation[s] += 1;
+    c->open[s] = 0;
+  }
+  return 0;
+}
+
 extern "C" int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* chosen, const int32_t* rows,
                                        int64_t count, hipStream_t stream) {
   using namespace omnia;

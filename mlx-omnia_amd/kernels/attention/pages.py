@@ -30,7 +30,6 @@ streams that are ordered among themselves, as with any tensor that is written.
 from __future__ import annotations
 
 from array import array
-from bisect import insort
 from collections.abc import Sequence
 
 import numpy as np
@@ -119,13 +118,13 @@ class PagedKVCache:
         elif lengths is None or opened is None:
             raise ValueError("PagedKVCache: tables need lengths and opened")
         self.keys, self.values = keys, values
-        self._tables = np.array(tables, dtype=np.int32)
+        self._tables = np.array(tables, dtype=np.int32, order="C")
         self._rows = np.array(lengths, dtype=np.int64)
         slots = range(len(self._tables))
         if len(set(opened)) != len(opened) or any(s not in slots for s in opened):
             raise ValueError("PagedKVCache: opened names other sequences than the tables, or one twice")
-        self._open = [s in opened for s in slots]
-        self._closed = [s for s in slots if not self._open[s]]   # ascending
+        self._open = np.zeros(len(self._tables), dtype=np.uint8)
+        self._open[list(opened)] = 1
         self._held = (self._tables >= 0).sum(axis=1)
         self._check_tables()
         self._refs = np.zeros(pages, dtype=np.int64)
@@ -138,7 +137,14 @@ class PagedKVCache:
         self._clock = 0                                                  # turns as sequences grow
         self.tables = torch.from_numpy(self._tables.copy()).to(keys.device)
         self.lengths = torch.from_numpy(self._rows.astype(np.int32)).to(keys.device)
-        self._pool = ops.PagePool(keys, values, self.tables, self.lengths) if hip_device(keys) else None
+        self._bind()
+
+    def _bind(self) -> None:
+        """The library's view of the pool, the tables and the host's arrays: on a HIP device."""
+        self._pool = None
+        if hip_device(self.keys):
+            self._pool = ops.PagePool(self.keys, self.values, self.tables, self.lengths)
+            self._pool.keep(self._tables, self._rows, self._held, self._refs, self._generation, self._open)
 
     def _check_tables(self) -> None:
         tables, width = self._tables, self._tables.shape[1] if self._tables.ndim == 2 else 0
@@ -153,7 +159,7 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: a table's pages must come first, without gaps")
         if (self._rows < 0).any() or (self._rows > self._held * self.page_rows).any():
             raise ValueError("PagedKVCache: a length outside its sequence's pages")
-        if (self._held[self._closed] > 0).any():
+        if (self._held[self._open == 0] > 0).any():
             raise ValueError("PagedKVCache: a sequence that is not open holds pages")
         for row in tables:
             if len(np.unique(row[row >= 0])) != (row >= 0).sum():
@@ -214,24 +220,6 @@ class PagedKVCache:
         """The edits that make `pages` a sequence's entries from `first` on."""
         return [n for i, page in enumerate(pages, first) for n in (ops.PAGES_ENTRY, sequence, i, page)]
 
-    def _fork(self, parent: int, full: int, rows: int, kids: list[int], pages: list[int]) -> None:
-        """Rows of the table for the kids, each with a page of its own, and `rows` rows of the
-        parent's last page for each."""
-        page = int(self._tables[parent, full]) if rows else -1
-        if self._pool is not None:
-            flat = array("i", bytes(8 * len(kids)))
-            flat[0::2], flat[1::2] = array("i", kids), array("i", pages)
-            self._pool.fork(parent, full, page, rows, flat)
-            return
-        if rows:
-            self._copy([(page, to, rows) for to in pages])
-        for kid, to in zip(kids, pages):
-            self.tables[kid] = -1
-            self.tables[kid, :full] = self.tables[parent, :full]
-            if rows:
-                self.tables[kid, full] = to
-            self.lengths[kid] = self.lengths[parent]
-
     def _copy(self, moves: list[tuple[int, int, int]], rename: bool = False) -> None:
         if not moves:
             return
@@ -269,15 +257,14 @@ class PagedKVCache:
 
     def _slots(self, count: int) -> list[int]:
         """The lowest `count` sequences that are not open, still not."""
-        if len(self._closed) < count:
-            raise ValueError(f"PagedKVCache: {count} more sequences are asked for, {len(self._closed)} of "
+        closed = (self._open == 0).nonzero()[0]
+        if len(closed) < count:
+            raise ValueError(f"PagedKVCache: {count} more sequences are asked for, {len(closed)} of "
                              f"{len(self._open)} are not open")
-        return self._closed[:count]
+        return closed[:count].tolist()
 
     def _begin(self, slots: list[int]) -> None:
-        del self._closed[: len(slots)]
-        for s in slots:
-            self._open[s] = True
+        self._open[slots] = 1
         self._renew(slots)
 
     def _pages_for(self, rows: int) -> int:
@@ -354,6 +341,12 @@ class PagedKVCache:
         self._known([sequence])
         if count < 0:
             raise ValueError("PagedKVCache: fewer than no forks")
+        if count > len(self._open):
+            self._slots(count)   # raises
+        if share and self._pool is not None:   # the same, beside the launch: 26 us a fork and a free here
+            kids = self._pool.begin(int(sequence), int(count))
+            self._epoch += 1
+            return kids
         size, rows = self.page_rows, int(self._rows[sequence])
         full, rest = divmod(rows, size)
         if not share:
@@ -366,23 +359,15 @@ class PagedKVCache:
         self._refs[fresh] = 1
         self._refs[parent[:full]] += count
         self._begin(kids)
-        block = self._tables[kids[0] : kids[-1] + 1] if kids[-1] - kids[0] == count - 1 else None
-        lines = self._tables[kids] if block is None else block
-        lines[:, :full] = parent[:full]
-        lines[:, full : full + each] = fresh.reshape(count, each)
-        if block is None:
-            self._tables[kids] = lines
+        self._tables[kids, :full] = parent[:full]
+        self._tables[kids, full : full + each] = fresh.reshape(count, each)
         self._held[kids] = full + each
         self._rows[kids] = rows
-        pages = fresh.tolist()
-        if share:
-            self._fork(sequence, full, rest, kids, pages if each else [-1] * count)
-        else:
-            used = [size] * (each - 1) + [rest - size * (each - 1)]
-            self._copy([(page, to, n) for i in range(count)
-                        for page, to, n in zip(parent.tolist(), pages[i * each : (i + 1) * each], used)])
-            self._edit([n for i, kid in enumerate(kids)
-                        for n in self._entries(kid, 0, pages[i * each : (i + 1) * each]) + [ops.PAGES_LENGTH, kid, rows, 0]])
+        used = [size] * (each - 1) + [rest - size * (each - 1)]
+        self._copy([(page, to, n) for line in fresh.reshape(count, each).tolist()
+                    for page, to, n in zip(parent[full:].tolist(), line, used)])
+        self._edit([n for kid in kids for n in self._entries(kid, 0, self._tables[kid, : full + each].tolist())
+                    + [ops.PAGES_LENGTH, kid, rows, 0]])
         return kids
 
     def free(self, sequences: Sequence[int] | int) -> None:
@@ -394,17 +379,14 @@ class PagedKVCache:
         self._known(gone)
         if not gone:
             return
-        if len(gone) == 1:   # a sequence names no page twice
-            held = self._tables[gone[0], : self._held[gone[0]]]
-            self._refs[held] -= 1
-            held[:] = -1
-        else:
-            held = self._tables[gone]
-            self._refs -= np.bincount(held[held >= 0], minlength=len(self._refs))
-            self._tables[gone] = -1
-        for s in gone:
-            self._open[s] = False
-            insort(self._closed, s)
+        if self._pool is not None:
+            self._pool.end(gone)
+            self._epoch += 1
+            return
+        held = self._tables[gone]
+        self._refs -= np.bincount(held[held >= 0], minlength=len(self._refs))
+        self._tables[gone] = -1
+        self._open[gone] = 0
         self._held[gone] = 0
         self._rows[gone] = 0
         self._renew(gone)
@@ -435,7 +417,7 @@ class PagedKVCache:
         if len(source):
             names = np.arange(self.pages + 1, dtype=np.int32)   # the last for -1
             names[-1], names[source] = -1, target
-            self._tables = names[self._tables]
+            self._tables[:] = names[self._tables]
             self._refs[target], self._refs[source] = self._refs[source], 0
             self._copy([(a, b, self.page_rows) for a, b in zip(source.tolist(), target.tolist())], rename=True)
         return live
@@ -457,8 +439,7 @@ class PagedKVCache:
         refs = np.zeros(pages, dtype=np.int64)
         refs[:kept] = self._refs[:kept]
         (self.keys, self.values), self._refs = pools, refs
-        if self._pool is not None:
-            self._pool = ops.PagePool(*pools, self.tables, self.lengths)
+        self._bind()
 
     # Steps --------------------------------------------------------------------------------
 

@@ -35,6 +35,14 @@ class BatchStep(ctypes.Structure):
         + [(name, _F32) for name in ("mscale", "eps", "scale")])
 
 
+class PagedCache(ctypes.Structure):
+    """`omnia_paged_cache_t`; must match include/omnia_hip.h."""
+
+    _fields_ = ([(name, _P) for name in ("keys", "values", "tables", "lengths", "host_tables", "rows", "held", "refs",
+                                         "generation", "open")]
+                + [(name, _I64) for name in ("layers", "pages", "kv_heads", "page_rows", "head_dim", "sequences", "width")])
+
+
 # name -> (restype, argtypes); must match include/omnia_hip.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_abi_version": (_I32, []),
@@ -115,6 +123,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_pages_fork": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
                                 _I64, _P]),
     "omnia_pages_edit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "omnia_paged_cache_fork": (_I32, [_P, _I64, _I64, _P, _P]),
+    "omnia_paged_cache_free": (_I32, [_P, _P, _I64, _P]),
     "omnia_pages_advance": (_I32, [_P, _I64, _P, _P, _I64, _P]),
     "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
                                              _F32, _I64, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _P, _I64,

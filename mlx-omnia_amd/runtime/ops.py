@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from .loader import BatchStep, call, last_error, library
+from .loader import BatchStep, PagedCache, call, last_error, library
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -1206,6 +1206,31 @@ class PagePool:
         if tables is not None and lengths is not None:
             self.sequences, self.width = _page_tables(tables, lengths, "page pool")
             self.tables, self.lengths = tables.data_ptr(), lengths.data_ptr()
+
+    def keep(self, tables: np.ndarray, rows: np.ndarray, held: np.ndarray, refs: np.ndarray, generation: np.ndarray,
+             opened: np.ndarray) -> None:
+        """The host's arrays of the cache, which `begin` and `end` change with the device's."""
+        kept = [tables, rows, held, refs, generation, opened]
+        shapes = [(self.sequences, self.width), *[(self.sequences,)] * 2, (self.pages,), *[(self.sequences,)] * 2]
+        kinds = [np.int32, *[np.int64] * 4, np.uint8]
+        _require(all(a.shape == shape and a.dtype == kind and a.flags.c_contiguous
+                     for a, shape, kind in zip(kept, shapes, kinds)), "page pool: the host's arrays")
+        keys, values, layers, pages, kv_heads, page_rows, head_dim = self.pool
+        self.kept = kept
+        self.cache = PagedCache(keys, values, self.tables, self.lengths, *(a.ctypes.data for a in kept), layers, pages,
+                                kv_heads, page_rows, head_dim, self.sequences, self.width)
+        self.cache_at = ctypes.addressof(self.cache)
+
+    def begin(self, parent: int, count: int) -> list[int]:
+        """`omnia_paged_cache_fork`: the sequences begun."""
+        kids = array("i", bytes(8 * count))
+        call("omnia_paged_cache_fork", self.cache_at, parent, count, kids.buffer_info()[0], _raw_stream(self.index))
+        return kids[0::2].tolist()
+
+    def end(self, gone: list[int]) -> None:
+        """`omnia_paged_cache_free`."""
+        flat = array("i", gone)
+        call("omnia_paged_cache_free", self.cache_at, flat.buffer_info()[0], len(flat), _raw_stream(self.index))
 
     def copy(self, moves, tables: int | None = None, entries: int = 0) -> None:
         flat, step = _int_lines(moves, 3, "moves"), 3 * PAGES_MOVES

@@ -450,3 +450,85 @@ def test_the_steps_arguments_are_laid_out_as_declared():
             declared.append((name.lstrip("*"), ctypes.c_void_p if pointer else
                              {"int64_t": ctypes.c_int64, "float": ctypes.c_float}[kind]))
     assert declared == list(BatchStep._fields_)
+
+
+def _kept(**change):
+    """The host's part of a cache of six pages of 16 rows and five sequences of at most four."""
+    state = dict(tables=np.array([[0, 1, 2, -1], [0, 4, -1, -1], *[[-1] * 4] * 3], dtype=np.int32),
+                 rows=np.array([37, 20, 0, 0, 0]), held=np.array([3, 2, 0, 0, 0]), refs=np.array([2, 1, 1, 0, 1, 0]),
+                 generation=np.zeros(5, dtype=np.int64), open=np.array([1, 1, 0, 0, 0], dtype=np.uint8))
+    for name, (at, value) in change.items():
+        state[name][at] = value
+    return state
+
+
+def _call_kept(name, state, *args):
+    import ctypes
+
+    from mlx_omnia_amd.runtime import library
+    from mlx_omnia_amd.runtime.loader import PagedCache
+    cache = PagedCache(4096, 8192, 4096, 8192, *(state[n].ctypes.data for n in ("tables", "rows", "held", "refs", "generation", "open")),
+                       1, 6, 2, 16, 64, 5, 4)
+    return getattr(library(), name)(ctypes.addressof(cache), *args, None)
+
+
+@pytest.mark.parametrize("change,parent,count,text", [
+    ({}, 2, 1, "2 is not open"), ({}, -1, 1, "-1 is not open"), ({}, 5, 1, "5 is not open"), ({}, 0, -1, "no forks"),
+    ({}, 0, 4, "4 more sequences are asked for, 3 of 5 are not open"),
+    ({}, 0, 3, "3 more pages are needed, 2 of 6 are free"),
+    (dict(held=(0, 2)), 0, 1, "more rows than pages"), (dict(held=(0, 5)), 0, 1, "more rows than pages"),
+    (dict(tables=((0, 1), -1)), 0, 1, "outside the pool"), (dict(tables=((0, 0), 6)), 0, 1, "outside the pool"),
+    (dict(tables=((0, 2), 6)), 0, 1, "no such page")])
+def test_paged_cache_fork_refuses(change, parent, count, text):
+    """And leaves everything as it was."""
+    from mlx_omnia_amd.runtime import loader
+    state, before = _kept(**change), _kept(**change)
+    kids = np.zeros(2 * max(count, 0), dtype=np.int32)
+    assert _call_kept("omnia_paged_cache_fork", state, parent, count, kids.ctypes.data) == -22
+    assert text in loader.last_error()
+    assert all(np.array_equal(state[n], before[n]) for n in state)
+
+
+@pytest.mark.parametrize("change,gone,text", [
+    ({}, [2], "2 is not open"), ({}, [0, 1, -1], "-1 is not open"), ({}, [1, 5], "5 is not open"),
+    ({}, [0, 1, 0], "named twice"), (dict(held=(1, 5)), [0, 1], "more pages than its table")])
+def test_paged_cache_free_refuses(change, gone, text):
+    """And leaves everything as it was."""
+    from mlx_omnia_amd.runtime import loader
+    state, before = _kept(**change), _kept(**change)
+    assert _call_kept("omnia_paged_cache_free", state, np.array(gone, dtype=np.int32).ctypes.data, len(gone)) == -22
+    assert text in loader.last_error()
+    assert all(np.array_equal(state[n], before[n]) for n in state)
+
+
+def test_no_forks_and_nothing_freed():
+    state = _kept()
+    assert _call_kept("omnia_paged_cache_fork", state, 0, 0, None) == 0
+    assert _call_kept("omnia_paged_cache_free", state, None, 0) == 0
+
+
+def test_the_caches_host_part_is_laid_out_as_declared():
+    import ctypes
+    import re
+    from pathlib import Path
+
+    from mlx_omnia_amd.runtime.loader import PagedCache
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "omnia_hip.h").read_text()
+    body = re.search(r"typedef struct \{([^}]*)\} omnia_paged_cache_t;", text).group(1)
+    declared = []
+    for line in body.split(";"):
+        kind, _, names = line.strip().partition(" ")
+        for name in filter(None, (n.strip() for n in names.split(","))):
+            pointer = name.startswith("*") or kind.endswith("*")
+            declared.append((name.lstrip("*"), ctypes.c_void_p if pointer else {"int64_t": ctypes.c_int64}[kind]))
+    assert declared == list(PagedCache._fields_), declared
+
+
+def test_tables_in_another_order():
+    """Arrays as numpy may lay them out: by columns, of other kinds."""
+    pool = torch.zeros((1, 6, 2, 16, 8))
+    cache = PagedKVCache(pool, pool.clone(), tables=np.asfortranarray([[0, 1], [2, -1]]), lengths=np.array([20.0, 3.0]), opened=[0, 1])
+    assert cache._tables.flags.c_contiguous and cache.rows(0) == 20 and cache.pages_of(0) == [0, 1]
+    with pytest.raises(ValueError, match="asked for"):
+        cache.fork(0, 1 << 60)
