@@ -30,7 +30,7 @@ struct Pool {
   }
 };
 
-constexpr int kPieceVectors = 1024;   // 16-byte vectors a workgroup copies, four a thread
+constexpr int kVectors = 2, kPieceVectors = 256 * kVectors;   // 16-byte vectors a thread and a workgroup copy
 
 // Where thread t's i-th vector of a piece of the first `rows` rows of every head lies in a page,
 // or -1 past them.
@@ -53,9 +53,10 @@ struct CopyArgs {
   Move moves[OMNIA_PAGES_MOVES];
 };
 
-// One piece (16 KB) of one page of one plane a workgroup; the workgroups past the copies rename
-// table entries, 256 each. Bound by memory: nothing is read or written twice, and past the
-// caches.
+// One piece (8 KB) of one page of one plane a workgroup; the workgroups past the copies rename
+// table entries, 256 each. Bound by memory: nothing is read or written twice, and what is
+// written goes past the caches (69 pages of 16 layers, 579 MB: 88 us, 6.6 TB/s; reads past them
+// as well 100 us, both through them 107; 32 KB a workgroup 94).
 __global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
   const int block = blockIdx.x;
   if (block >= a.copies) {
@@ -79,15 +80,15 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(CopyArgs a) {
   const Move m = a.moves[rest % a.count];
   const uint16_t* from = a.pool.page(rest / a.count, m.from);
   uint16_t* to = a.pool.page(rest / a.count, m.to);
-  u32x4 v[4];
-  int at[4];
+  u32x4 v[kVectors];
+  int at[kVectors];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kVectors; ++i) {
     at[i] = vector_at(a.pool, m.rows, piece, i);
-    if (at[i] >= 0) v[i] = load_nt(reinterpret_cast<const u32x4*>(from + at[i]));
+    if (at[i] >= 0) v[i] = *reinterpret_cast<const u32x4*>(from + at[i]);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kVectors; ++i) {
     if (at[i] >= 0) store_nt(reinterpret_cast<u32x4*>(to + at[i]), v[i]);
   }
 }
@@ -105,10 +106,12 @@ struct ForkArgs {
   Kid kids[OMNIA_PAGES_MOVES];
 };
 
-constexpr int kKidsAtOnce = 8;
+constexpr int kKidsAtOnce = 16;
 
-// A piece of the parent's last page, read once and written for eight children, a workgroup;
-// behind those one for each child's row of the table.
+// A piece of the parent's last page, read once and written for 16 children, a workgroup; behind
+// those one for each child's row of the table. Bound by the writes, which a step reads soon: into
+// the caches (16 children, 33 rows of 36 layers, 83 MB: 13.7 us; past them, four times the bytes
+// a workgroup and half the children 16.5).
 __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
   const int copies = a.pieces * a.groups * a.pool.planes;
   const int block = blockIdx.x;
@@ -124,18 +127,18 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
   const int rest = block / a.pieces;
   const int first = rest % a.groups * kKidsAtOnce, plane = rest / a.groups;
   const uint16_t* from = a.pool.page(plane, a.page);
-  u32x4 v[4];
-  int at[4];
+  u32x4 v[kVectors];
+  int at[kVectors];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kVectors; ++i) {
     at[i] = vector_at(a.pool, a.rows, piece, i);
     if (at[i] >= 0) v[i] = *reinterpret_cast<const u32x4*>(from + at[i]);
   }
   for (int kid = first; kid < min(first + kKidsAtOnce, a.count); ++kid) {
     uint16_t* to = a.pool.page(plane, a.kids[kid].page);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (at[i] >= 0) store_nt(reinterpret_cast<u32x4*>(to + at[i]), v[i]);
+    for (int i = 0; i < kVectors; ++i) {
+      if (at[i] >= 0) *reinterpret_cast<u32x4*>(to + at[i]) = v[i];
     }
   }
 }
