@@ -295,6 +295,15 @@ def test_sequences_shorter_than_the_shared_rows(prefix, own):
     assert np.all(np.abs(wide(out) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
 
 
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (24, 2, 128), (40, 2, 64), (70, 5, 128), (70, 7, 64),
+                                                     (60, 2, 128), (120, 4, 64)])
+def test_prompts_of_many_tokens_into_the_pages(heads, kv_heads, head_dim):
+    """One to four heads in turn, and heads that do not fill the last of them."""
+    case = Case(heads=heads, kv_heads=kv_heads, head_dim=head_dim, pairs=head_dim // 4, norms=True, page_rows=32,
+                prefix=32, own=(3, 40), tokens=(600, 501), layers=2, layer=0)
+    case.check_rows(case.step.project(case.batch, *case.raw), case.cache.lengths.cpu().numpy())
+
+
 def test_raw_rows_are_read_where_they_lie():
     case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=32, own=(5, 9, 2), tokens=(1, 4, 2))
     want = case.step(case.batch, *case.raw)
