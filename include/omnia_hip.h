@@ -716,6 +716,14 @@ int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* cache, int64_t parent,
 int32_t omnia_paged_cache_free(const omnia_paged_cache_t* cache, const int32_t* gone, int64_t count,
                                hipStream_t stream);
 
+/* Begins a sequence of `rows` rows on the lowest free pages, whose rows the caller writes itself;
+ * `sequence` in HOST memory takes which it is. A refused call leaves everything as it was. */
+int32_t omnia_paged_cache_open(const omnia_paged_cache_t* cache, int64_t rows, int32_t* sequence, hipStream_t stream);
+
+/* Moves the pages in use to the front of the pool (omnia_pages_copy), each that lies behind them
+ * to the lowest free one in turn; `live` in HOST memory takes how many are in use. */
+int32_t omnia_paged_cache_compact(const omnia_paged_cache_t* cache, int64_t* live, hipStream_t stream);
+
 /* lengths[chosen[i]] += rows[i] for i < count, all on the device; the chosen are distinct. An
  * index outside [0, sequences) is passed over. */
 int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* chosen,

@@ -219,11 +219,34 @@ Pool make_pool(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages, 
               static_cast<int>(page_rows), static_cast<int>(head_dim), static_cast<int>(2 * layers)};
 }
 
+bool bad_cache(const omnia_paged_cache_t* c) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  return !c || !c->host_tables || !c->rows || !c->held || !c->refs || !c->generation || !c->open || c->sequences <= 0 ||
+         c->sequences >= kMost || c->width <= 0 || c->width >= kMost || c->pages <= 0 || c->pages >= kMost ||
+         c->page_rows <= 0;
+}
+
+// The lowest number from `from` on below `end` whose count is none, or `end`.
+template <typename T>
+int64_t next_none(const T* counts, int64_t from, int64_t end) {
+  while (from < end && counts[from] != 0) ++from;
+  return from;
+}
+
 bool bad_tables(int64_t sequences, int64_t width, int64_t pages) {
   constexpr int64_t kMost = int64_t{1} << 31;
   return sequences <= 0 || sequences >= kMost || width <= 0 || width >= kMost || pages <= 0 || pages >= kMost;
 }
 
+}  // namespace
+}  // namespace omnia
+
+namespace omnia {
+namespace {
+int32_t too_few(const char* call, int64_t count, const char* what, int64_t found, int64_t all, const char* state) {
+  return fail(-EINVAL, std::string(call) + ": " + std::to_string(count) + " more " + what + ", " + std::to_string(found) +
+                           " of " + std::to_string(all) + " are " + state);
+}
 }  // namespace
 }  // namespace omnia
 
@@ -336,9 +359,7 @@ extern "C" int32_t omnia_pages_edit(int32_t* tables, int32_t* lengths, int64_t s
 extern "C" int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* c, int64_t parent, int64_t count, int32_t* kids,
                                           hipStream_t stream) {
   using namespace omnia;
-  OMNIA_REQUIRE(c && c->host_tables && c->rows && c->held && c->refs && c->generation && c->open,
-                "paged_cache_fork: null pointer");
-  OMNIA_REQUIRE(!bad_tables(c->sequences, c->width, c->pages) && c->page_rows > 0, "paged_cache_fork: bad tables");
+  OMNIA_REQUIRE(!bad_cache(c), "paged_cache_fork: null pointer or bad tables");
   if (parent < 0 || parent >= c->sequences || c->open[parent] == 0) {
     return fail(-EINVAL, "paged_cache_fork: sequence " + std::to_string(parent) + " is not open");
   }
@@ -353,23 +374,18 @@ extern "C" int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* c, int64_t 
     OMNIA_REQUIRE(line[i] >= 0 && line[i] < c->pages, "paged_cache_fork: a table names a page outside the pool");
   }
   int64_t found = 0;
-  for (int64_t s = 0; s < c->sequences && found < count; ++s) {
-    if (c->open[s] == 0) kids[2 * found++] = static_cast<int32_t>(s);
+  for (int64_t s = next_none(c->open, 0, c->sequences); s < c->sequences && found < count;
+       s = next_none(c->open, s + 1, c->sequences)) {
+    kids[2 * found++] = static_cast<int32_t>(s);
   }
-  if (found < count) {
-    return fail(-EINVAL, "paged_cache_fork: " + std::to_string(count) + " more sequences are asked for, " +
-                             std::to_string(found) + " of " + std::to_string(c->sequences) + " are not open");
+  if (found < count) return too_few("paged_cache_fork", count, "sequences are asked for", found, c->sequences, "not open");
+  found = rest > 0 ? 0 : count;
+  for (int64_t p = next_none(c->refs, 0, c->pages); p < c->pages && found < count;
+       p = next_none(c->refs, p + 1, c->pages)) {
+    kids[2 * found++ + 1] = static_cast<int32_t>(p);
   }
-  found = 0;
-  if (rest > 0) {
-    for (int64_t p = 0; p < c->pages && found < count; ++p) {
-      if (c->refs[p] == 0) kids[2 * found++ + 1] = static_cast<int32_t>(p);
-    }
-    if (found < count) {
-      return fail(-EINVAL, "paged_cache_fork: " + std::to_string(count) + " more pages are needed, " +
-                               std::to_string(found) + " of " + std::to_string(c->pages) + " are free");
-    }
-  } else {
+  if (found < count) return too_few("paged_cache_fork", count, "pages are needed", found, c->pages, "free");
+  if (rest == 0) {
     for (int64_t i = 0; i < count; ++i) kids[2 * i + 1] = -1;
   }
   for (int64_t first = 0; first < count; first += OMNIA_PAGES_MOVES) {
@@ -399,9 +415,7 @@ extern "C" int32_t omnia_paged_cache_fork(const omnia_paged_cache_t* c, int64_t 
 extern "C" int32_t omnia_paged_cache_free(const omnia_paged_cache_t* c, const int32_t* gone, int64_t count,
                                           hipStream_t stream) {
   using namespace omnia;
-  OMNIA_REQUIRE(c && c->host_tables && c->rows && c->held && c->refs && c->generation && c->open,
-                "paged_cache_free: null pointer");
-  OMNIA_REQUIRE(!bad_tables(c->sequences, c->width, c->pages), "paged_cache_free: bad tables");
+  OMNIA_REQUIRE(!bad_cache(c), "paged_cache_free: null pointer or bad tables");
   OMNIA_REQUIRE(count >= 0, "paged_cache_free: bad count");
   if (count == 0) return 0;
   OMNIA_REQUIRE(gone, "paged_cache_free: null pointer");
@@ -446,6 +460,101 @@ extern "C" int32_t omnia_paged_cache_free(const omnia_paged_cache_t* c, const in
     c->open[s] = 0;
   }
   return 0;
+}
+
+extern "C" int32_t omnia_paged_cache_open(const omnia_paged_cache_t* c, int64_t rows, int32_t* sequence,
+                                          hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(!bad_cache(c) && sequence, "paged_cache_open: null pointer or bad tables");
+  OMNIA_REQUIRE(rows >= 0, "paged_cache_open: a sequence of fewer than no rows");
+  const int64_t need = rows / c->page_rows + (rows % c->page_rows > 0 ? 1 : 0);
+  if (need > c->width) {
+    return fail(-EINVAL, "paged_cache_open: a sequence holds at most " + std::to_string(c->width * c->page_rows) +
+                             " rows, not " + std::to_string(rows));
+  }
+  const int64_t s = next_none(c->open, 0, c->sequences);
+  if (s == c->sequences) return too_few("paged_cache_open", 1, "sequences are asked for", 0, c->sequences, "not open");
+  int64_t found = 0;
+  for (int64_t p = next_none(c->refs, 0, c->pages); p < c->pages && found < need;
+       p = next_none(c->refs, p + 1, c->pages)) {
+    ++found;
+  }
+  if (found < need) return too_few("paged_cache_open", need, "pages are needed", found, c->pages, "free");
+  int32_t edits[4 * OMNIA_PAGES_EDITS];
+  int64_t count = 0, done = 0, page = -1;
+  int32_t rc = 0;
+  // Its entries, and the length at the end; the line is nobody's until it is open.
+  int32_t* line = c->host_tables + s * c->width;
+  for (int64_t i = 0; i <= need && rc == 0; ++i) {
+    if (i < need) {
+      page = next_none(c->refs, page + 1, c->pages);
+      line[i] = static_cast<int32_t>(page);
+    } else if (rows == 0) {
+      break;
+    }
+    const int32_t edit[4] = {i < need ? OMNIA_PAGES_ENTRY : OMNIA_PAGES_LENGTH, static_cast<int32_t>(s),
+                             static_cast<int32_t>(i < need ? i : rows), static_cast<int32_t>(i < need ? page : 0)};
+    for (int64_t j = 0; j < 4; ++j) edits[4 * count + j] = edit[j];
+    ++count;
+    done = i < need ? i + 1 : need;
+    if (count == OMNIA_PAGES_EDITS || i == need) {
+      rc = omnia_pages_edit(c->tables, c->lengths, c->sequences, c->width, c->pages, edits, count, stream);
+      count = 0;
+    }
+  }
+  if (rc != 0) {
+    for (int64_t i = 0; i < done; ++i) line[i] = -1;
+    return rc;
+  }
+  for (int64_t i = 0; i < need; ++i) c->refs[line[i]] = 1;
+  c->held[s] = need;
+  c->rows[s] = rows;
+  c->generation[s] += 1;
+  c->open[s] = 1;
+  *sequence = static_cast<int32_t>(s);
+  return 0;
+}
+
+extern "C" int32_t omnia_paged_cache_compact(const omnia_paged_cache_t* c, int64_t* live, hipStream_t stream) {
+  using namespace omnia;
+  OMNIA_REQUIRE(!bad_cache(c) && live, "paged_cache_compact: null pointer or bad tables");
+  int64_t used = 0;
+  for (int64_t p = 0; p < c->pages; ++p) used += c->refs[p] != 0 ? 1 : 0;
+  int64_t target = -1, source = used - 1;
+  int32_t rc = 0;
+  bool moved = false;
+  // As many pages in use lie behind the first `used` as free ones among them. A page that was left
+  // says where to until the tables have been renamed: -1 - target.
+  while (rc == 0) {
+    int32_t moves[3 * OMNIA_PAGES_MOVES];
+    int64_t count = 0;
+    while (count < OMNIA_PAGES_MOVES) {
+      do ++source; while (source < c->pages && c->refs[source] == 0);
+      if (source >= c->pages) break;
+      target = next_none(c->refs, target + 1, used);
+      moves[3 * count] = static_cast<int32_t>(source);
+      moves[3 * count + 1] = static_cast<int32_t>(target);
+      moves[3 * count + 2] = static_cast<int32_t>(c->page_rows);
+      ++count;
+    }
+    if (count == 0) break;
+    rc = omnia_pages_copy(c->keys, c->values, c->layers, c->pages, c->kv_heads, c->page_rows, c->head_dim, moves, count,
+                          c->tables, c->sequences * c->width, stream);
+    for (int64_t i = 0; i < count && rc == 0; ++i) {
+      c->refs[moves[3 * i + 1]] = c->refs[moves[3 * i]];
+      c->refs[moves[3 * i]] = -1 - moves[3 * i + 1];
+      moved = true;
+    }
+  }
+  if (moved) {
+    for (int64_t i = 0; i < c->sequences * c->width; ++i) {
+      const int32_t page = c->host_tables[i];
+      if (page >= used && page < c->pages && c->refs[page] < 0) c->host_tables[i] = static_cast<int32_t>(-1 - c->refs[page]);
+    }
+    for (int64_t p = used; p < c->pages; ++p) c->refs[p] = c->refs[p] < 0 ? 0 : c->refs[p];
+  }
+  if (rc == 0) *live = used;
+  return rc;
 }
 
 extern "C" int32_t omnia_pages_advance(int32_t* lengths, int64_t sequences, const int32_t* chosen, const int32_t* rows,

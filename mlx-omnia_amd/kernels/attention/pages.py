@@ -279,6 +279,10 @@ class PagedKVCache:
         self._refuse_capture("opening a sequence")
         if rows < 0:
             raise ValueError("PagedKVCache: a sequence of fewer than no rows")
+        if self._pool is not None:   # the same, beside the launch
+            s = self._pool.open(int(rows))
+            self._epoch += 1
+            return s
         pages = self._pages_for(rows)
         slots = self._slots(1)
         s, fresh = slots[0], self._take(pages)
@@ -411,6 +415,8 @@ class PagedKVCache:
         lowest free one in turn; how many are in use. Sequences and batches stay what they
         are."""
         self._refuse_capture("compacting")
+        if self._pool is not None:
+            return self._pool.compact()
         used = np.flatnonzero(self._refs > 0)
         live = len(used)
         source, target = used[used >= live], np.flatnonzero(self._refs[:live] == 0)

@@ -125,6 +125,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_pages_edit": (_I32, [_P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "omnia_paged_cache_fork": (_I32, [_P, _I64, _I64, _P, _P]),
     "omnia_paged_cache_free": (_I32, [_P, _P, _I64, _P]),
+    "omnia_paged_cache_open": (_I32, [_P, _I64, _P, _P]),
+    "omnia_paged_cache_compact": (_I32, [_P, _P, _P]),
     "omnia_pages_advance": (_I32, [_P, _I64, _P, _P, _I64, _P]),
     "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
                                              _F32, _I64, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _P, _I64,

@@ -1209,7 +1209,8 @@ class PagePool:
 
     def keep(self, tables: np.ndarray, rows: np.ndarray, held: np.ndarray, refs: np.ndarray, generation: np.ndarray,
              opened: np.ndarray) -> None:
-        """The host's arrays of the cache, which `begin` and `end` change with the device's."""
+        """The host's arrays of the cache, which `open`, `begin`, `end` and `compact` change with the
+        device's."""
         kept = [tables, rows, held, refs, generation, opened]
         shapes = [(self.sequences, self.width), *[(self.sequences,)] * 2, (self.pages,), *[(self.sequences,)] * 2]
         kinds = [np.int32, *[np.int64] * 4, np.uint8]
@@ -1226,6 +1227,18 @@ class PagePool:
         kids = array("i", bytes(8 * count))
         call("omnia_paged_cache_fork", self.cache_at, parent, count, kids.buffer_info()[0], _raw_stream(self.index))
         return kids[0::2].tolist()
+
+    def open(self, rows: int) -> int:
+        """`omnia_paged_cache_open`: the sequence begun."""
+        which = array("i", (0,))
+        call("omnia_paged_cache_open", self.cache_at, rows, which.buffer_info()[0], _raw_stream(self.index))
+        return which[0]
+
+    def compact(self) -> int:
+        """`omnia_paged_cache_compact`: the pages in use."""
+        live = array("q", (0,))
+        call("omnia_paged_cache_compact", self.cache_at, live.buffer_info()[0], _raw_stream(self.index))
+        return live[0]
 
     def end(self, gone: list[int]) -> None:
         """`omnia_paged_cache_free`."""

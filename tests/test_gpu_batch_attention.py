@@ -551,6 +551,51 @@ def test_any_order_of_calls_keeps_every_sequence(seed):
     random_calls(cache, PagedModel(), rng, 60, check_every=5)
 
 
+def test_a_cache_of_many_pages_is_the_hosts():
+    """More entries, children and moves than one launch takes: the tables, the lengths and the
+    pages of the same calls on the CPU."""
+    caches = [PagedKVCache.empty(2, 900, 16, 2, 8, device=device, sequences=400, rows=3200) for device in ("cuda", "cpu")]
+    gen = torch.Generator().manual_seed(5)
+    first = torch.randn(caches[1].keys.shape, generator=gen).bfloat16()
+    for cache in caches:
+        for pool in (cache.keys, cache.values):
+            pool.copy_(first)
+    rng = np.random.default_rng(1)
+
+    def same(call):
+        got = [call(cache) for cache in caches]
+        assert got[0] == got[1]
+        device, host = caches
+        assert torch.equal(device.tables.cpu(), host.tables) and torch.equal(device.lengths.cpu(), host.lengths)
+        assert torch.equal(device.keys.cpu(), host.keys) and torch.equal(device.values.cpu(), host.values)
+        for name in ("_tables", "_rows", "_held", "_refs", "_generation", "_open"):
+            assert np.array_equal(getattr(device, name), getattr(host, name)), name
+        assert device._epoch == host._epoch
+        return got[0]
+
+    assert same(lambda c: c.open(2500)) == 0 and same(lambda c: c.open(3200)) == 1
+    kids = same(lambda c: c.fork(0, 300))
+    gone = [int(s) for s in rng.permutation(kids)[:170]]
+    same(lambda c: c.free([1, *gone]))
+    for rows in (0, 1, 16, 17, 2080):
+        same(lambda c: c.open(rows))
+    same(lambda c: c.free(0))
+    assert same(lambda c: c.compact()) == caches[0].pages - caches[0].free_pages
+    same(lambda c: c.fork(kids[-1] if kids[-1] not in gone else [s for s in kids if s not in gone][0], 2, share=False))
+    same(lambda c: c.resize(1000))
+    same(lambda c: c.free([s for s in kids if s not in gone][:100]))
+    same(lambda c: c.compact())
+    for call in (lambda c: c.open(3201), lambda c: c.open(3200) and c.open(3200) and c.open(3200) and c.open(3200)):
+        errors = []
+        for cache in caches:
+            with pytest.raises(ValueError) as refused:
+                for _ in range(9):
+                    call(cache)
+            errors.append(str(refused.value).rsplit(": ", 1)[1].split(" (code")[0])
+        assert errors[0] == errors[1]
+    same(lambda c: c.compact())
+
+
 @pytest.mark.parametrize("dtype,head_dim", [(torch.bfloat16, 8), (torch.bfloat16, 128), (torch.float32, 24)])
 def test_copies_of_many_pages(dtype, head_dim):
     """More moves than one launch takes, whole and partial rows, and the tables renamed."""

@@ -501,6 +501,33 @@ def test_paged_cache_free_refuses(change, gone, text):
     assert all(np.array_equal(state[n], before[n]) for n in state)
 
 
+@pytest.mark.parametrize("change,rows,text", [
+    ({}, -1, "fewer than no rows"), ({}, 65, "at most 64 rows, not 65"), ({}, 1 << 62, "at most 64"),
+    ({}, 33, "3 more pages are needed, 2 of 6 are free"),
+    (dict(open=(slice(None), 1)), 1, "1 more sequences are asked for, 0 of 5 are not open")])
+def test_paged_cache_open_refuses(change, rows, text):
+    """And leaves everything as it was."""
+    from mlx_omnia_amd.runtime import loader
+    state, before = _kept(**change), _kept(**change)
+    which = np.zeros(1, dtype=np.int32)
+    assert _call_kept("omnia_paged_cache_open", state, rows, which.ctypes.data) == -22
+    assert text in loader.last_error()
+    assert all(np.array_equal(state[n], before[n]) for n in state)
+
+
+def test_an_empty_sequence_and_a_pool_that_is_packed():
+    """What launches nothing."""
+    state = _kept()
+    which, live = np.zeros(1, dtype=np.int32), np.zeros(1, dtype=np.int64)
+    assert _call_kept("omnia_paged_cache_open", state, 0, which.ctypes.data) == 0 and which[0] == 2
+    assert state["open"].tolist() == [1, 1, 1, 0, 0] and state["generation"].tolist() == [0, 0, 1, 0, 0]
+    state["refs"][:] = [2, 1, 1, 1, 0, 0]
+    state["tables"][1, 1] = 3
+    before = {n: a.copy() for n, a in state.items()}
+    assert _call_kept("omnia_paged_cache_compact", state, live.ctypes.data) == 0 and live[0] == 4
+    assert all(np.array_equal(state[n], before[n]) for n in state)
+
+
 def test_no_forks_and_nothing_freed():
     state = _kept()
     assert _call_kept("omnia_paged_cache_fork", state, 0, 0, None) == 0
