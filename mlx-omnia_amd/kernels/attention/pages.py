@@ -483,7 +483,7 @@ class PagedKVCache:
             rows = self._rows[batch.index] + batch.counts
             self._reserve(batch.index, rows)
             batch.clock, batch.last = self._clock, int(rows.max())
-        if not _capturing(self.keys.device):
+        if self._pool is None or not torch.cuda.is_current_stream_capturing():
             return batch.last
         if batch.reach < batch.last:
             raise ValueError("a batch's step is captured after prepare_capture has reserved what its replays reach")

@@ -1491,16 +1491,24 @@ class BatchStepPlan:
             width=width, own_tiles=tiles.shape[0], prefix=prefix,
             prefix_sequence=prefix_sequence, own_rows=-1, mscale=mscale, eps=eps, scale=scale)
         self.sized = -1, 0   # own rows, and the workspace that they need
+        # What results are made like, without a call's parsing of their kind and place.
+        self.keys, self.like = keys, keys.view(-1)[:1].expand(tokens, heads, head_dim)
+
+    def _context(self) -> torch.Tensor:
+        return torch.empty_like(self.like, memory_format=torch.contiguous_format)
 
     def _rows(self, raw: torch.Tensor, width: int, name: str) -> tuple[int, int, torch.Tensor]:
         """(address, stride, the tensor that holds them) of the raw rows, copied where the kernel
         could not read them in place."""
-        shape = raw.shape
+        shape, address = raw.shape, raw.data_ptr()
+        if (shape == (self.tokens, width) and raw.stride() == (width, 1) and raw.dtype is BF16
+                and raw.get_device() == self.index and address % 16 == 0):
+            return address, width, raw
         if (raw.dtype != BF16 or len(shape) < 2 or shape[-1] != width or shape[-2] != self.tokens
                 or raw.numel() != self.tokens * width or raw.get_device() != self.index):
             raise ValueError(f"{name}: expected the batch's {self.tokens} tokens of {width}, bf16 on {self.device}, not "
                              f"{tuple(shape)} {raw.dtype} on {raw.device}")
-        stride, address = raw.stride(-2) if self.tokens > 1 else width, raw.data_ptr()
+        stride = raw.stride(-2) if self.tokens > 1 else width
         if raw.stride(-1) != 1 or stride % 8 or stride < width or address % 16:
             raw = raw.clone(memory_format=torch.contiguous_format)
             stride, address = width, raw.data_ptr()
@@ -1516,7 +1524,7 @@ class BatchStepPlan:
     def project(self, raw_queries, raw_keys, raw_values) -> torch.Tensor:
         args = BatchStep.from_buffer_copy(self.args)   # of this call: two may be under way
         held = self._raw(args, raw_queries, raw_keys, raw_values)
-        out = torch.empty((self.tokens, self.heads, self.head_dim), dtype=BF16, device=self.device)
+        out = self._context()
         args.queries = out.data_ptr()
         call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
         del held
@@ -1531,8 +1539,7 @@ class BatchStepPlan:
                                                                 args.prefix, own_rows, args.own_tiles)
             _require(nbytes >= 0, "attention_batch_step: geometry not served")
             self.sized = own_rows, nbytes
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        out = torch.empty((self.tokens, self.heads, self.head_dim), dtype=BF16, device=self.device)
+        workspace, out = self.keys.new_empty(nbytes // 2), self._context()   # of bf16
         args.own_rows, args.workspace_bytes, args.workspace, args.out = (own_rows, nbytes, workspace.data_ptr(),
                                                                           out.data_ptr())
         call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
