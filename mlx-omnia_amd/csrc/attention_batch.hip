@@ -1091,8 +1091,12 @@ void launch_merge(const BatchArgs& a, hipStream_t stream) {
     const int64_t of_one = 256 / (D / 4) / groups;
     kernel<<<dim3(static_cast<unsigned>((rows + of_one - 1) / of_one)), 256, 0, stream>>>(a);
   };
-  if (a.prefix_splits + a.own_splits <= 8) {
+  // A group has four pieces under way at once.
+  const int splits = a.prefix_splits + a.own_splits;
+  if (splits <= 4) {
     launch(attention_batch_merge_kernel<D, 1>, 1);
+  } else if (splits <= 20) {
+    launch(attention_batch_merge_kernel<D, 4>, 4);
   } else {
     launch(attention_batch_merge_kernel<D, 256 / (D / 4)>, 256 / (D / 4));
   }
