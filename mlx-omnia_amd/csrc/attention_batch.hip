@@ -218,21 +218,29 @@ __device__ __forceinline__ u32x4 low_part(const float (&x)[8], const u32x4& high
   return pack8(rest);
 }
 
-// Eight consecutive values of a query as bf16 operands, in kParts parts.
+// Eight consecutive values of a query, as they come (bf16, or fp32 in kParts 2) and as bf16
+// operands, in kParts parts.
 template <int kParts>
-__device__ __forceinline__ void load_query(const void* q, int64_t at, s16x8 (&parts)[kParts]) {
-  if constexpr (kParts == 1) {
-    parts[0] = *reinterpret_cast<const s16x8*>(static_cast<const uint16_t*>(q) + at);
-  } else {
-    const float* from = static_cast<const float*>(q) + at;
-    float x[8];
-    *reinterpret_cast<f32x4*>(x) = *reinterpret_cast<const f32x4*>(from);
-    *reinterpret_cast<f32x4*>(x + 4) = *reinterpret_cast<const f32x4*>(from + 4);
-    const u32x4 high = pack8(x);
-    parts[0] = __builtin_bit_cast(s16x8, high);
-    parts[1] = __builtin_bit_cast(s16x8, low_part(x, high));
+struct QueryEight {
+  u32x4 raw[kParts];
+  __device__ __forceinline__ void load(const void* q, int64_t at) {
+    const u32x4* from = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(q) + at * kParts);
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) raw[i] = from[i];
   }
-}
+  __device__ __forceinline__ void split(s16x8 (&parts)[kParts]) const {
+    if constexpr (kParts == 1) {
+      parts[0] = __builtin_bit_cast(s16x8, raw[0]);
+    } else {
+      float x[8];
+      *reinterpret_cast<u32x4*>(x) = raw[0];
+      *reinterpret_cast<u32x4*>(x + 4) = raw[1];
+      const u32x4 high = pack8(x);
+      parts[0] = __builtin_bit_cast(s16x8, high);
+      parts[1] = __builtin_bit_cast(s16x8, low_part(x, high));
+    }
+  }
+};
 
 __device__ __forceinline__ s16x8 read_transposed(const uint16_t* first, const uint16_t* second) {
   typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
@@ -259,11 +267,18 @@ struct WideRows {
   f32x16 out[kBlocks];      // O^T: d = 32 b + 8 (e / 4) + 4 half + e % 4 of the column's row
   float top, total;         // the maximum (the whole row's) and the sum (this lane's keys)
   int key_at, value_at[kBlocks];
+  struct Queries {
+    QueryEight<kParts> of[kSteps];
+    __device__ __forceinline__ Queries(const void* queries, int64_t row, int lane) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) of[s].load(queries, row * D + 8 * (lane / 32) + 16 * s);
+    }
+  };
 
-  __device__ __forceinline__ void start(const void* queries, int64_t row, int lane) {
+  __device__ __forceinline__ void start(const Queries& queries, int lane) {
     const int column = lane % 32, half = lane / 32;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) load_query<kParts>(queries, row * D + 8 * half + 16 * s, q[s]);
+    for (int s = 0; s < kSteps; ++s) queries.of[s].split(q[s]);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = f32x16{};
     top = -INFINITY;
@@ -417,11 +432,18 @@ struct NarrowRows {
   f32x4 out[kBlocks];       // O^T: d = 16 b + 4 quarter + e of the column's row
   float top, total;
   int key_at, value_at;
+  struct Queries {
+    QueryEight<kParts> of[kSteps];
+    __device__ __forceinline__ Queries(const void* queries, int64_t row, int lane) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) of[s].load(queries, row * D + 8 * (lane / 16) + 32 * s);
+    }
+  };
 
-  __device__ __forceinline__ void start(const void* queries, int64_t row, int lane) {
+  __device__ __forceinline__ void start(const Queries& queries, int lane) {
     const int column = lane % 16, quarter = lane / 16;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) load_query<kParts>(queries, row * D + 8 * quarter + 32 * s, q[s]);
+    for (int s = 0; s < kSteps; ++s) queries.of[s].split(q[s]);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     top = -INFINITY;
@@ -533,16 +555,23 @@ __device__ __forceinline__ bool take_out_odd(u32x4& v) {
 
 // The pages of a sequence as a wave walks its rows upwards. Tiles start at multiples of 16
 // rows and pages hold 16 or more, so 16 rows from a multiple of 16 lie in one page; lane l
-// holds the page of the l-th sixteen of 1,024 rows, and the ones of the next 1,024 are on
-// their way before they are asked for.
+// holds the entry of the l-th sixteen of 1,024 rows, and the ones of the next 1,024 are on
+// their way before they are asked for. What is loaded is looked at where it is used, and checked
+// there: with the checks beside the loads each was waited for in turn, 3 us before the first keys
+// of a piece were asked for.
 struct PageWalk {
   const PageTables& at;
-  int sequence, window, now, next;
+  const int32_t* line;      // of the sequence's table, or of the first one's where there is none
+  bool known;               // whether there is
+  int window, now, next;
 
   __device__ __forceinline__ int fetch(int w) const {
-    return at.page(sequence, w * 1024 + static_cast<int>(threadIdx.x) % kWave * 16);
+    const int index = (w * 1024 + static_cast<int>(threadIdx.x) % kWave * 16) >> at.page_shift;
+    return line[min(index, at.width - 1)];
   }
-  __device__ __forceinline__ PageWalk(const PageTables& tables, int s, int row) : at(tables), sequence(s) {
+  __device__ __forceinline__ PageWalk(const PageTables& tables, int s, int row) : at(tables) {
+    known = s >= 0 && s < at.sequences;
+    line = at.tables + static_cast<int64_t>(known ? s : 0) * at.width;
     window = row / 1024;
     now = fetch(window);
     next = fetch(window + 1);
@@ -555,7 +584,10 @@ struct PageWalk {
     next = fetch(window + 1);
   }
   // The page of the sixteen at `row` (the same in every lane), below 0 for none.
-  __device__ __forceinline__ int page(int row) const { return __builtin_amdgcn_readlane(now, row / 16 % 64); }
+  __device__ __forceinline__ int page(int row) const {
+    const int id = __builtin_amdgcn_readlane(now, row / 16 % 64);
+    return known && (row >> at.page_shift) < at.width && id < at.pages ? id : -1;
+  }
 };
 
 // What a workgroup does: which rows of which kv head with which keys of whose pages.
@@ -652,10 +684,13 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) 
 }
 
 // Up to 128 rows, 32 a wave: the four waves share the tiles of 64 keys, through two LDS stages;
-// the next tile is on its way to the one while the other is multiplied.
+// the next tile is on its way to the one while the other is multiplied. (A piece of a few tiles
+// starts at the rate that a CU takes its 64 KB of queries and its keys from the caches, 3 us: with
+// the first two tiles asked for together it was none the faster, 40.5 us for 39.9.)
 template <int D, int kParts>
 __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk& walk, uint16_t* stage0, 
-                                           uint16_t* stage1, int* odd) {
+                                           uint16_t* stage1, int* flags) {
+  int *odd = flags, *short_rows = flags + 1;
   using Rows = WideRows<D, kParts>;
   constexpr int kChunks = D / 8;
   constexpr int kLoads = kTileKeys * kChunks / 256;   // 16-byte vectors a thread brings, each of K and V
@@ -667,8 +702,6 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   const bool working = p.first_row + wave * kWaveRows < p.end_row;   // the wave
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int2 whose = p.shared ? a.at.tokens[token] : int2{0, 0};   // asked for ahead of its use
-  Rows rows;
-  rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
   // Up to here every row sees the keys: up to the first row's limit, or all the shared ones
   // (that a sequence stops before their end is not expected of a plan, but served: below).
   int common = p.mixed ? p.before + p.first_row / a.group + 1 : p.high;
@@ -680,7 +713,6 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   const uint32_t from_k = (stage_row % 16) * D + (chunk ^ Rows::turn_k(stage_row)) * 8;
   const uint32_t from_v = (stage_row % 16) * D + (chunk ^ Rows::turn_v(stage_row)) * 8;
   const int sixteen = D == 128 ? 0 : __builtin_amdgcn_readfirstlane(wave / 2);   // of vector 0
-  int64_t base[kLoads];
   bool whole = false;    // of the tile asked for: every row there, and seen by all rows
   uint32_t absent = 0;   // its sixteens without a page
   auto ask = [&](int tile, uint16_t* stage) {
@@ -689,6 +721,7 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
     absent = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) absent |= walk.page(key0 + 16 * i) < 0 ? 1u << i : 0u;
+    int64_t base[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = key0 + 16 * (D == 128 ? i : 2 * i + sixteen);
@@ -711,13 +744,15 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   auto patch = [&](int tile, uint16_t* stage) {
 #pragma unroll 1
     for (int i = 0; i < kLoads; ++i) {
+      const int first = tile * kTileKeys + 16 * (D == 128 ? i : 2 * i + sixteen);
+      const int page = walk.page(first);
       const int at = stage_row + 256 / kChunks * i;
       const int key = tile * kTileKeys + at;
-      const bool there = key >= p.low && key < p.high && ((absent >> (at / 16)) & 1u) == 0;
       u32x4 k = u32x4{0, 0, 0, 0}, v = u32x4{0, 0, 0, 0};
-      if (there) {
-        k = *reinterpret_cast<const u32x4*>(a.keys + base[i] + from_k);
-        v = *reinterpret_cast<const u32x4*>(a.values + base[i] + from_v);
+      if (page >= 0 && key >= p.low && key < p.high) {
+        const int64_t base = a.at.row_of(page, a.kv_heads, p.kv_head, first) * D;
+        k = *reinterpret_cast<const u32x4*>(a.keys + base + from_k);
+        v = *reinterpret_cast<const u32x4*>(a.values + base + from_v);
       }
       if (take_out_odd(v)) *odd = 1;
       *reinterpret_cast<u32x4*>(stage + at * D + chunk * 8) = k;
@@ -732,17 +767,26 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
 
   const int tiles = (p.high + kTileKeys - 1) / kTileKeys;   // past the last
   int tile = p.low / kTileKeys;
-  if (threadIdx.x == 0) *odd = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) *odd = *short_rows = 0;
+  lds_barrier();
+  const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
   if (tile < tiles) ask(tile, stage0);
-  const int limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
-  if (p.shared && __syncthreads_or(limit < p.high)) {
-    common = 0;
-    whole = false;
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what was asked for comes first
-  }
+  const bool known = whose.x >= 0 && whose.x < a.at.sequences;
+  const int length = a.at.lengths[known ? whose.x : 0];
+  Rows rows;
+  rows.start(queries, lane);
+  const int limit = (!p.shared ? p.before + token : known ? length + whose.y : -1) + 1;
+  if (p.shared && limit < p.high) *short_rows = 1;
   if (tile < tiles && !whole) patch(tile, stage0);
   arrive();
+  if (*short_rows != 0) {
+    common = 0;
+    if (tile < tiles && whole) {
+      patch(tile, stage0);
+      lds_barrier();
+    }
+    whole = false;
+  }
   // The stages by name, not by a turning index: the compiler then sees that what is on its way
   // to the one is not what is read from the other, and does not wait for it.
   auto turn = [&](const uint16_t* here, uint16_t* there) {
@@ -810,7 +854,7 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
   const int row = min(p.first_row + column, p.end_row - 1);
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int2 whose = p.shared ? a.at.tokens[token] : int2{0, 0};
-  rows.start(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
+  const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
 
   const int first_tile = tile, tiles = (p.high + kKeys - 1) / kKeys;   // past the last
   const int chunk = lane % kChunks, stage_row = lane / kChunks;
@@ -818,8 +862,6 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
   u32x4 stage_k[kLoads], stage_v[kLoads];
   bool whole = false;
   uint32_t absent = 0;
-  // (Where one of two branches' loads of an address is nontemporal the compiler makes one of
-  // them that is not.)
   const auto load = [](const uint16_t* from) {
     return kStream ? load_nt(reinterpret_cast<const u32x4*>(from)) : *reinterpret_cast<const u32x4*>(from);
   };
@@ -835,33 +877,37 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
       first[i] = a.at.row_of(max(page, 0), a.kv_heads, p.kv_head, key0 + 16 * i) * D;
     }
     whole = __builtin_amdgcn_readfirstlane(absent == 0 && key0 >= p.low && key0 + kKeys <= p.high ? 1 : 0) != 0;
+    // Every row, counted or not (a row of any page is in the pool): without branches the queries,
+    // asked for before, are waited for alone.
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int in = i * kRowsALoad;   // of the tile, the load's first row
-      const uint16_t* from_k = a.keys + first[in / 16] + (in % 16) * D;
-      const uint16_t* from_v = a.values + first[in / 16] + (in % 16) * D;
-      if (whole) {
-        stage_k[i] = load(from_k + offset);
-        stage_v[i] = load(from_v + offset);
-      } else {
-        const int key = key0 + in + stage_row;
-        stage_k[i] = stage_v[i] = u32x4{0, 0, 0, 0};
-        if (((absent >> (in / 16)) & 1u) == 0 && key >= p.low && key < p.high) {
-          stage_k[i] = load(from_k + offset);
-          stage_v[i] = load(from_v + offset);
-        }
-      }
+      stage_k[i] = load(a.keys + first[in / 16] + (in % 16) * D + offset);
+      stage_v[i] = load(a.values + first[in / 16] + (in % 16) * D + offset);
     }
   };
 
   bool odd = false;   // a value of this wave's keys was taken out, by this lane
-  if (tile < tiles) load_tile(tile);
+  load_tile(tile);
+  rows.start(queries, lane);
   const int limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
   if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
   while (tile < tiles) {
     const int key0 = tile * kKeys;
     const bool edge = __builtin_amdgcn_readfirstlane(p.mixed || !whole ? 1 : 0) != 0;
     const uint32_t holes = absent;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int in = i * kRowsALoad, key = key0 + in + stage_row;
+        const bool there = ((absent >> (in / 16)) & 1u) == 0 && key >= p.low && key < p.high;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          stage_k[i][j] = there ? stage_k[i][j] : 0u;
+          stage_v[i][j] = there ? stage_v[i][j] : 0u;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = i * kRowsALoad + stage_row;
@@ -962,7 +1008,7 @@ __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTileKeys * D], stage1[2 * kTileKeys * D];
   static_assert(sizeof(stage0) == kWaves * kNarrowRows * D * sizeof(float) && sizeof(stage0) == 2 * 2 * 32 * D * 2,
                 "a stage holds what a narrow piece puts there");
-  __shared__ int odd;   // a value was taken out
+  __shared__ int flags[2];   // a value was taken out; a row ends before the shared ones do
   Piece p;
   find_piece(a, p);
   PageWalk walk(a.at, p.sequence, p.low);
@@ -970,7 +1016,7 @@ __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
   if (p.end_row - p.first_row <= kNarrowRows) {
     narrow_piece<D, kParts>(a, p, walk, stage0, stage1);
   } else {
-    wide_piece<D, kParts>(a, p, walk, stage0, stage1, &odd);
+    wide_piece<D, kParts>(a, p, walk, stage0, stage1, flags);
   }
 }
 
