@@ -29,6 +29,7 @@ from ..qkv_rope.atlas import AngleAtlas
 from ..qkv_rope.kernel import AngleTable
 from ..resolve import record_fallback, resolve
 from .pages import PagedBatch, PagedKVCache, _capturing
+from .prefill import unfollowed
 
 HEAD_DIMS = (64, 128)
 
@@ -160,6 +161,7 @@ class DefaultBatchAttentionStep(BatchAttentionStepStrategy):
 @dataclass(frozen=True, eq=False)
 class HipBatchAttentionStep(BatchAttentionStepStrategy):
     core: DefaultBatchAttentionStep
+    held: tuple[torch.Tensor, ...]   # the parameters and tables that autograd may follow
 
     @classmethod
     def build(cls, cache, *, layer, heads, kv_heads, head_dim, scale, dtype, query_weight, key_weight, eps,
@@ -189,7 +191,9 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         return cls(DefaultBatchAttentionStep.build(
             cache, layer=layer, heads=heads, kv_heads=kv_heads, head_dim=head_dim, scale=scale, dtype=dtype,
             query_weight=query_weight, key_weight=key_weight, eps=eps, rotary_pairs=rotary_pairs, mscale=mscale,
-            angles=angles, sinks=sinks.contiguous() if sinks is not None else None))
+            angles=angles, sinks=sinks.contiguous() if sinks is not None else None),
+            (*weights, *(() if sinks is None else (sinks,)),
+             *((angles.cos, angles.sin) if rotary_pairs and isinstance(angles, AngleTable) else ())))
 
     def prepare_capture(self, batch: PagedBatch, steps: int) -> None:
         """Before capturing a step of the batch: the pages of its next `steps` steps, the
@@ -227,11 +231,11 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         return plan, last
 
     def _followed(self, *raw: torch.Tensor) -> bool:
-        """A call that autograd follows, for the torch ops."""
-        if torch.is_grad_enabled() and (raw[0].requires_grad or raw[1].requires_grad or raw[2].requires_grad):
-            record_fallback(self, self.core)
-            return True
-        return False
+        """A call that autograd, a transform, a mode or a compiler follows, for the torch ops."""
+        if unfollowed(*raw, *self.held):
+            return False
+        record_fallback(self, self.core)
+        return True
 
     def project(self, batch, raw_queries, raw_keys, raw_values):
         if self._followed(raw_queries, raw_keys, raw_values):

@@ -28,25 +28,34 @@ from .cache import FixedKVCache, KVCache
 HEAD_DIMS = (64, 128)
 MAX_HEADS, MAX_ROWS = 4096, 1 << 24   # what the entries take: as many heads, fewer rows
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_C = torch._C
+
+
+def unfollowed(*tensors: torch.Tensor) -> bool:
+    """Ordinary tensors with nothing following the operations on them: no compiler, tracer,
+    mode, transform or autograd."""
+    # First, since a compiler follows the questions below as well.
+    if torch.compiler.is_compiling() or _C._get_tracing_state() is not None or _C._len_torch_dispatch_stack():
+        return False
+    if _C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0:
+        return False
+    if _C._len_torch_function_stack() and any(
+            type(mode) is not DeviceContext for mode in _get_current_function_mode_stack()):
+        return False
+    followed = torch.is_grad_enabled()
+    for t in tensors:
+        if type(t) not in _PLAIN or (followed and t.requires_grad):
+            return False
+    return True
 
 
 def plain_call(*tensors: torch.Tensor) -> bool:
-    """Ordinary tensors on the current ROCm device, with nothing following the operations
-    on them: a kernel may then stand in for torch ops."""
-    # First, since a compiler follows the questions below as well.
-    if torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None:
+    """Unfollowed tensors on the current ROCm device: a kernel may then stand in for torch ops."""
+    if not unfollowed(*tensors):
         return False
-    if torch._C._len_torch_dispatch_stack():
+    index = tensors[0].get_device()
+    if any(t.get_device() != index for t in tensors):
         return False
-    if torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0:
-        return False
-    if torch._C._len_torch_function_stack() and any(
-            type(mode) is not DeviceContext for mode in _get_current_function_mode_stack()):
-        return False
-    followed, index = torch.is_grad_enabled(), tensors[0].get_device()
-    for t in tensors:
-        if type(t) not in _PLAIN or t.get_device() != index or (followed and t.requires_grad):
-            return False
     return hip_device(tensors[0]) and index == torch._C._cuda_getDevice()
 
 

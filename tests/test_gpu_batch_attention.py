@@ -418,6 +418,40 @@ def test_a_graph_keeps_the_angles_it_was_captured_with():
         assert torch.equal(step(case.batch, *case.raw), want)
 
 
+def test_gains_and_sinks_that_autograd_follows():
+    case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, norms=True, sinks=True, prefix=16, own=(3, 4))
+    want = case.step(case.batch, *case.raw)
+    grads = []
+    for reference in (False, True):
+        case.qw, case.kw, case.sinks = (torch.nn.Parameter(t.detach().clone()) for t in (case.qw, case.kw, case.sinks))
+        step = case.make(case.cache, **(dict(reference=True) if reference else {}))
+        before = dict(FALLBACKS)
+        step(case.batch, *case.raw).float().square().sum().backward()
+        assert reference or FALLBACKS != before
+        grads.append([t.grad for t in (case.qw, case.kw, case.sinks)])
+        if not reference:
+            with torch.no_grad():   # nothing follows: the kernels, and the same result
+                assert torch.equal(step(case.batch, *case.raw), want)
+    assert all(torch.equal(a, b) and a.abs().max() > 0 for a, b in zip(*grads))
+
+
+def test_a_mode_that_follows_a_call_sees_its_operations():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.add(func.name())
+            return func(*args, **(kwargs or {}))
+
+    case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
+    want = case.step(case.batch, *case.raw)
+    with Names() as mode:
+        mode.seen = set()
+        got = case.step(case.batch, *case.raw)
+    assert "aten::_softmax" in mode.seen
+    assert (got.float() - want.float()).abs().max() <= 4 * HALF * want.float().abs().max()
+
+
 def test_gradients_go_to_a_steps_own_rows():
     """Against the Core chain's, whose gradients are tested against the formula: the same chain."""
     case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4), tokens=(2, 1))
