@@ -792,7 +792,10 @@ int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
  * from the next multiple of 256 bytes on, what omnia_attention_batch needs:
  * omnia_attention_batch_step_bytes. With `queries` not null only the first half runs, its
  * queries rounded to bf16 there. Every field is as the two entries take it; `raw_*`, `queries`,
- * `out` and `workspace` are what changes from call to call, `own_rows` from step to step. */
+ * `out` and `workspace` are what changes from call to call, `own_rows` from step to step.
+ * one_token_each 1 says that every token is of another sequence, with a tile of its own, and that
+ * every sequence holds all the shared rows: heads of at most 16 a kv head with 0, 32 or 64 rotary
+ * pairs are then projected where they are attended, without a launch of their own. */
 typedef struct {
   const uint16_t *raw_queries, *raw_keys, *raw_values, *query_weight, *key_weight;
   const float *cos_rows, *sin_rows;
@@ -803,7 +806,7 @@ typedef struct {
   void *workspace;
   int64_t workspace_bytes, query_stride, key_stride, value_stride, table_stride, angle_rows, rotary_pairs;
   int64_t tokens, heads, kv_heads, head_dim, pages, page_rows, sequences, width, own_tiles, prefix;
-  int64_t prefix_sequence, own_rows;
+  int64_t prefix_sequence, own_rows, one_token_each;
   float mscale, eps, scale;
 } omnia_attention_batch_step_t;
 int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,

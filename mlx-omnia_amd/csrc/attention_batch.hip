@@ -184,6 +184,7 @@ struct BatchArgs {
   int heads, kv_heads, group, tokens, prefix, prefix_sequence, prefix_tiles, own_tiles;
   int prefix_splits, prefix_keys, own_splits, own_keys;   // splits of either part, keys of one
   float scale_log2;
+  BatchProjectArgs fresh;   // with kFresh: the new tokens' raw rows, in place of q
 };
 
 constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileKeys = 64, kNarrowRows = 16;
@@ -258,6 +259,94 @@ __device__ __forceinline__ bool raise(float& top, float best, float& shrink) {
   return true;
 }
 
+// The same from a token's raw row: eights of it kStep apart, from `at` on, normed and rotated as the
+// prologue does. Its launch is spared (4 us of a step of one token a sequence); rotary pairs in
+// whole kStep, so that both halves of a pair are the lane's.
+template <int D, int kEights, int kStep>
+struct FreshQueries {
+  u32x4 raw[kEights], gain[kEights];
+  f32x4 c[kEights / 2][2], s[kEights / 2][2];
+  __device__ __forceinline__ void load(const BatchProjectArgs& a, int token, int head, int at) {
+    const uint16_t* from = a.raw[0] + token * a.stride[0] + head * D + at;
+#pragma unroll
+    for (int i = 0; i < kEights; ++i) raw[i] = *reinterpret_cast<const u32x4*>(from + kStep * i);
+    if (a.gain[0] != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kEights; ++i) gain[i] = *reinterpret_cast<const u32x4*>(a.gain[0] + at + kStep * i);
+    }
+  }
+  __device__ __forceinline__ void load_angles(const BatchProjectArgs& a, int position, int at) {
+    if (a.pairs == 0) return;
+    const int64_t row = min(static_cast<int64_t>(max(position, 0)), a.angle_rows - 1) * a.table_stride + at;
+#pragma unroll
+    for (int i = 0; i < kEights / 2; ++i) {
+      const int64_t from = row + (kStep * i < a.pairs ? kStep * i : 0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[i][h] = *reinterpret_cast<const f32x4*>(a.cos + from + 4 * h);
+        s[i][h] = *reinterpret_cast<const f32x4*>(a.sin + from + 4 * h);
+      }
+    }
+  }
+  template <int kPairs>
+  __device__ __forceinline__ void rotate(float (&x)[kEights][8], float mscale) const {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float first = x[i][j] * mscale, second = x[i + kPairs][j] * mscale;
+        x[i][j] = first * c[i][j / 4][j % 4] - second * s[i][j / 4][j % 4];
+        x[i + kPairs][j] = first * s[i][j / 4][j % 4] + second * c[i][j / 4][j % 4];
+      }
+    }
+  }
+  // `whole`: the sum over the lanes that share the row.
+  template <typename Whole>
+  __device__ __forceinline__ void split(const BatchProjectArgs& a, s16x8 (&parts)[kEights][2], const Whole& whole) const {
+    float x[kEights][8];
+#pragma unroll
+    for (int i = 0; i < kEights; ++i) unpack8(raw[i], x[i]);
+    if (a.gain[0] != nullptr) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEights; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += x[i][j] * x[i][j];
+      }
+      const float inv = 1.0f / sqrtf(whole(sum) / static_cast<float>(D) + a.eps);
+#pragma unroll
+      for (int i = 0; i < kEights; ++i) {
+        float w[8];
+        unpack8(gain[i], w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = w[j] * (x[i][j] * inv);
+      }
+    }
+    if (a.pairs == kEights / 2 * kStep) {
+      rotate<kEights / 2>(x, a.mscale);
+    } else if constexpr (kEights >= 4) {
+      if (a.pairs == kEights / 4 * kStep) rotate<kEights / 4>(x, a.mscale);
+    }
+#pragma unroll
+    for (int i = 0; i < kEights; ++i) {
+      const u32x4 high = pack8(x[i]);
+      parts[i][0] = __builtin_bit_cast(s16x8, high);
+      parts[i][1] = __builtin_bit_cast(s16x8, low_part(x[i], high));
+    }
+  }
+};
+
+__device__ __forceinline__ float pair_sum(float x) {   // over lanes l and l + 32
+  uint32_t lower, upper;
+  half_pair(__float_as_uint(x), lower, upper);
+  return __uint_as_float(lower) + __uint_as_float(upper);
+}
+__device__ __forceinline__ float quarter_sum(float x) {   // over lanes l, l + 16, l + 32 and l + 48
+  uint32_t a, b;
+  row_pair(__float_as_uint(x), a, b);
+  return pair_sum(__uint_as_float(a) + __uint_as_float(b));
+}
+
 // 32 rows on 32x32x16 MFMA: row = column lane % 32; of 32 keys lane half h holds the keys
 // 8 i + 4 h + j, i and j below 4.
 template <int D, int kParts>
@@ -275,10 +364,19 @@ struct WideRows {
     }
   };
 
+  using Fresh = FreshQueries<D, kSteps, 16>;
+
   __device__ __forceinline__ void start(const Queries& queries, int lane) {
-    const int column = lane % 32, half = lane / 32;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) queries.of[s].split(q[s]);
+    start(lane);
+  }
+  __device__ __forceinline__ void start(const Fresh& fresh, const BatchProjectArgs& a, int lane) {
+    fresh.split(a, q, pair_sum);
+    start(lane);
+  }
+  __device__ __forceinline__ void start(int lane) {
+    const int column = lane % 32, half = lane / 32;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = f32x16{};
     top = -INFINITY;
@@ -440,10 +538,19 @@ struct NarrowRows {
     }
   };
 
+  using Fresh = FreshQueries<D, kSteps, 32>;
+
   __device__ __forceinline__ void start(const Queries& queries, int lane) {
-    const int column = lane % 16, quarter = lane / 16;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) queries.of[s].split(q[s]);
+    start(lane);
+  }
+  __device__ __forceinline__ void start(const Fresh& fresh, const BatchProjectArgs& a, int lane) {
+    fresh.split(a, q, quarter_sum);
+    start(lane);
+  }
+  __device__ __forceinline__ void start(int lane) {
+    const int column = lane % 16, quarter = lane / 16;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     top = -INFINITY;
@@ -687,7 +794,7 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) 
 // the next tile is on its way to the one while the other is multiplied. (A piece of a few tiles
 // starts at the rate that a CU takes its 64 KB of queries and its keys from the caches, 3 us: with
 // the first two tiles asked for together it was none the faster, 40.5 us for 39.9.)
-template <int D, int kParts>
+template <int D, int kParts, bool kFresh>
 __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk& walk, uint16_t* stage0, 
                                            uint16_t* stage1, int* flags) {
   int *odd = flags, *short_rows = flags + 1;
@@ -769,13 +876,25 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   int tile = p.low / kTileKeys;
   if (threadIdx.x == 0) *odd = *short_rows = 0;
   lds_barrier();
-  const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
-  if (tile < tiles) ask(tile, stage0);
-  const bool known = whose.x >= 0 && whose.x < a.at.sequences;
-  const int length = a.at.lengths[known ? whose.x : 0];
   Rows rows;
-  rows.start(queries, lane);
-  const int limit = (!p.shared ? p.before + token : known ? length + whose.y : -1) + 1;
+  int limit;
+  const bool known = whose.x >= 0 && whose.x < a.at.sequences;
+  const auto last = [&](int length) { return !p.shared ? p.before + token : known ? length + whose.y : -1; };
+  if constexpr (kFresh) {
+    typename Rows::Fresh fresh;
+    fresh.load(a.fresh, token, head, 8 * half);
+    const int length = a.at.lengths[known ? whose.x : 0];
+    if (tile < tiles) ask(tile, stage0);
+    limit = last(length) + 1;
+    fresh.load_angles(a.fresh, limit - 1, 8 * half);
+    rows.start(fresh, a.fresh, lane);
+  } else {
+    const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
+    if (tile < tiles) ask(tile, stage0);
+    const int length = a.at.lengths[known ? whose.x : 0];
+    rows.start(queries, lane);
+    limit = last(length) + 1;
+  }
   if (p.shared && limit < p.high) *short_rows = 1;
   if (tile < tiles && !whole) patch(tile, stage0);
   arrive();
@@ -840,9 +959,58 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   }
 }
 
+// The row that a token adds for a kv head, 16 bytes a lane: its key in the first D / 8 lanes, normed
+// and rotated as the prologue does, its value in as many more.
+template <int D>
+struct NewRow {
+  static constexpr int kLanes = D / 8;
+  u32x4 raw, gain;
+  f32x4 c[2], s[2];
+  __device__ __forceinline__ void load(const BatchProjectArgs& a, int token, int head, int position, int lane) {
+    const int mine = lane % kLanes, part = lane / kLanes % 2, half = a.pairs / 8;
+    raw = *reinterpret_cast<const u32x4*>(a.raw[1 + part] + token * a.stride[1 + part] + head * D + mine * 8);
+    if (a.gain[1] != nullptr) gain = *reinterpret_cast<const u32x4*>(a.gain[1] + mine * 8);
+    if (a.pairs == 0) return;
+    const int64_t from = min(static_cast<int64_t>(max(position, 0)), a.angle_rows - 1) * a.table_stride +
+                         (mine < half ? mine : mine < 2 * half ? mine - half : 0) * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      c[h] = *reinterpret_cast<const f32x4*>(a.cos + from + 4 * h);
+      s[h] = *reinterpret_cast<const f32x4*>(a.sin + from + 4 * h);
+    }
+  }
+  __device__ __forceinline__ u32x4 finish(const BatchProjectArgs& a, int lane) const {
+    const int mine = lane % kLanes, part = lane / kLanes % 2, half = a.pairs / 8;
+    float x[8];
+    unpack8(raw, x);
+    if (a.gain[1] != nullptr) {
+      float sum = 0.0f, w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
+      sum = group_sum<kLanes>(sum);
+      const float inv = 1.0f / sqrtf(sum / static_cast<float>(D) + a.eps);
+      unpack8(gain, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = w[j] * (x[j] * inv);
+    }
+    if (a.pairs > 0) {
+      const bool turned = mine < 2 * half;
+      const int partner = mine < half ? mine + half : turned ? mine - half : mine;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float self = x[j] * a.mscale, other = __shfl(self, partner, kLanes);
+        const float cj = c[j / 4][j % 4], sj = s[j / 4][j % 4];
+        const float rotated = mine < half ? self * cj - other * sj : other * sj + self * cj;
+        x[j] = turned ? rotated : x[j];
+      }
+    }
+    return part == 0 ? pack8(x) : raw;
+  }
+};
+
 // A wave's walk over a piece with up to 16 rows: every `stride`-th tile of 32 keys from `tile`
 // on, through an LDS buffer of its own, without a barrier. Leaves the rows' state in `rows`.
-template <int D, int kParts, bool kStream>
+template <int D, int kParts, bool kStream, bool kFresh>
 __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWalk& walk, NarrowRows<D, kParts>& rows,
                                             int tile, int stride, uint16_t* tile_k) {
   using Rows = NarrowRows<D, kParts>;
@@ -854,7 +1022,6 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
   const int row = min(p.first_row + column, p.end_row - 1);
   const int token = row / a.group, head = p.kv_head * a.group + row % a.group;
   const int2 whose = p.shared ? a.at.tokens[token] : int2{0, 0};
-  const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
 
   const int first_tile = tile, tiles = (p.high + kKeys - 1) / kKeys;   // past the last
   const int chunk = lane % kChunks, stage_row = lane / kChunks;
@@ -888,9 +1055,37 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
   };
 
   bool odd = false;   // a value of this wave's keys was taken out, by this lane
-  load_tile(tile);
-  rows.start(queries, lane);
-  const int limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
+  int limit;
+  u32x4 new_row;   // the new token's key (lanes below D / 8) and value (as many more), and where it is
+  int new_at = -1;
+  if constexpr (kFresh) {
+    // Own rows are of one token, whose position is known: all it needs is asked for ahead of the keys.
+    typename Rows::Fresh fresh;
+    NewRow<D> added;
+    fresh.load(a.fresh, token, head, 8 * quarter);
+    const bool shared = !kStream && p.shared;
+    if (!shared) {
+      limit = p.before + token + 1;
+      const int position = __builtin_amdgcn_readfirstlane(limit - 1);
+      fresh.load_angles(a.fresh, position, 8 * quarter);
+      if (position >= p.low && position < p.high) {
+        new_at = position;
+        added.load(a.fresh, __builtin_amdgcn_readfirstlane(token), p.kv_head, position, lane);
+      }
+    }
+    load_tile(tile);
+    if (shared) {
+      limit = a.at.before(whose) + 1;
+      fresh.load_angles(a.fresh, limit - 1, 8 * quarter);
+    }
+    rows.start(fresh, a.fresh, lane);
+    if (new_at >= 0) new_row = added.finish(a.fresh, lane);
+  } else {
+    const typename Rows::Queries queries(a.q, static_cast<int64_t>(token) * a.heads + head, lane);
+    load_tile(tile);
+    rows.start(queries, lane);
+    limit = (p.shared ? a.at.before(whose) : p.before + token) + 1;
+  }
   if (p.shared && __ballot(limit < p.high) != 0) p.mixed = true;   // the same rows in every wave
   while (tile < tiles) {
     const int key0 = tile * kKeys;
@@ -914,6 +1109,17 @@ __device__ __forceinline__ void narrow_walk(const BatchArgs& a, Piece& p, PageWa
       if (p.mixed) odd = take_out_odd(stage_v[i]) || odd;
       *reinterpret_cast<u32x4*>(tile_k + at * D + (chunk ^ Rows::turn_k(at)) * 8) = stage_k[i];
       *reinterpret_cast<u32x4*>(tile_v + at * D + (chunk ^ Rows::turn_v(at)) * 8) = stage_v[i];
+    }
+    // The new row, over what its place in the pool held: this wave is its only reader here.
+    if (kFresh && new_at >= 0 && tile == new_at / kKeys) {
+      const int at = new_at % kKeys, mine = lane % kChunks, part = lane / kChunks;
+      const int turn = part == 0 ? Rows::turn_k(at) : Rows::turn_v(at);
+      const int page = walk.page(new_at);
+      if (page >= 0 && part < 2) {
+        *reinterpret_cast<u32x4*>((part == 0 ? tile_k : tile_v) + at * D + (mine ^ turn) * 8) = new_row;
+        const int64_t to = a.at.row_of(page, a.kv_heads, p.kv_head, new_at) * D + mine * 8;
+        *reinterpret_cast<u32x4*>(a.fresh.pool[part] + to) = new_row;
+      }
     }
     const int following = tile + stride;
     if (following < tiles) load_tile(following);
@@ -956,13 +1162,13 @@ __device__ __forceinline__ void store_four(const BatchArgs& a, const Piece& p, i
 
 // Up to 16 rows: the four waves hold the same rows, take every fourth tile each and merge at the
 // end.
-template <int D, int kParts>
+template <int D, int kParts, bool kFresh>
 __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, PageWalk& walk, uint16_t* stage0,
                                              uint16_t* stage1) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int column = lane % 16, quarter = lane / 16;
   NarrowRows<D, kParts> rows;
-  narrow_walk<D, kParts, false>(a, p, walk, rows, p.low / 32 + wave, kWaves,
+  narrow_walk<D, kParts, false, kFresh>(a, p, walk, rows, p.low / 32 + wave, kWaves,
                          (wave < 2 ? stage0 : stage1) + wave % 2 * 2 * 32 * D);
 
   // The waves' states and contexts meet in LDS: row c's context of wave w at [w][c] of the one
@@ -1001,7 +1207,7 @@ __device__ __forceinline__ void narrow_piece(const BatchArgs& a, Piece p, PageWa
   }
 }
 
-template <int D, int kParts>
+template <int D, int kParts, bool kFresh = false>
 __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
   // K and V of a tile each; a narrow piece's waves have half of one each, and its contexts of
   // four waves fill the first.
@@ -1014,9 +1220,9 @@ __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
   PageWalk walk(a.at, p.sequence, p.low);
   if (!find_keys(a, p)) return;
   if (p.end_row - p.first_row <= kNarrowRows) {
-    narrow_piece<D, kParts>(a, p, walk, stage0, stage1);
+    narrow_piece<D, kParts, kFresh>(a, p, walk, stage0, stage1);
   } else {
-    wide_piece<D, kParts>(a, p, walk, stage0, stage1, flags);
+    wide_piece<D, kParts, kFresh>(a, p, walk, stage0, stage1, flags);
   }
 }
 
@@ -1025,7 +1231,7 @@ __global__ __launch_bounds__(256, 2) void attention_batch_kernel(BatchArgs a) {
 // to 6.2 TB/s; what is read is past the caches' size, so it goes by them (24 of 4,776 rows: 103
 // -> 91 us; where it fits, it may be there still, and a nontemporal load costs a tenth). Pieces
 // of a tile of more than 16 rows take them 16 at a time.
-template <int D, int kParts>
+template <int D, int kParts, bool kFresh = false>
 __global__ __launch_bounds__(64, 2) void attention_own_kernel(BatchArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t tile[2 * 32 * D];
   Piece p;
@@ -1039,7 +1245,7 @@ __global__ __launch_bounds__(64, 2) void attention_own_kernel(BatchArgs a) {
     if (!find_keys(a, p)) continue;
     const int column = threadIdx.x % 16, quarter = threadIdx.x / 16;
     NarrowRows<D, kParts> rows;
-    narrow_walk<D, kParts, true>(a, p, walk, rows, p.low / 32, 1, tile);
+    narrow_walk<D, kParts, true, kFresh>(a, p, walk, rows, p.low / 32, 1, tile);
     const float total = rows.whole_total();
     if (column >= p.end_row - p.first_row) continue;
 #pragma unroll
@@ -1238,6 +1444,85 @@ int page_shift_of(int64_t page_rows) {
   return -1;
 }
 
+// Whether the attention projects a step's rows itself, without the prologue's launch: one token a
+// sequence, of up to 16 rows, with pairs that a lane holds both halves of, where the pieces run at
+// once (one a sequence and kv head counted: of more some are past its rows). Each projects its
+// queries, which costs it a microsecond or two: 33 sequences of 64 heads 28.1 -> 23.4 us, but 96
+// of 32 with 696 pieces 43.7 -> 44.6. Waves alone have several rounds and gain all the same (24
+// sequences of up to 16,000 rows: 94.5 -> 93.1).
+bool takes_fresh(const omnia_attention_batch_step_t& s) {
+  if (s.one_token_each == 0 || s.tokens <= 0 || s.own_tiles != s.tokens || s.rotary_pairs % 32 != 0 ||
+      !geometry_served(s.tokens, s.heads, s.kv_heads, s.head_dim, s.prefix, s.own_rows, s.own_tiles) ||
+      s.heads > kNarrowRows * s.kv_heads) {
+    return false;
+  }
+  const Plan p = plan_for(s.tokens, s.heads, s.kv_heads, s.prefix, s.own_rows, s.own_tiles);
+  return p.own_alone || s.kv_heads * (p.prefix_tiles * p.prefix_splits + s.own_tiles) <= kSlots;
+}
+
+// Whether a step's prologue is refused.
+int32_t project_refused(const omnia_attention_batch_step_t& s, const void* queries) {
+  OMNIA_REQUIRE(geometry_served(s.tokens, s.heads, s.kv_heads, s.head_dim, 0, 0, 0), "attention_batch_project: bad geometry");
+  OMNIA_REQUIRE(s.rotary_pairs >= 0 && s.rotary_pairs % 8 == 0 && 2 * s.rotary_pairs <= s.head_dim,
+                "attention_batch_project: rotary_pairs must be a multiple of 8 within the head");
+  OMNIA_REQUIRE(page_shift_of(s.page_rows) > 0, "attention_batch_project: page_rows must be 16, 32, 64, 128 or 256");
+  OMNIA_REQUIRE(s.pages > 0 && s.pages < (int64_t{1} << 31) && s.sequences > 0 && s.sequences < (int64_t{1} << 31) &&
+                    s.width > 0 && s.width < (int64_t{1} << 31) / s.page_rows,
+                "attention_batch_project: bad tables");
+  if (s.tokens == 0) return 0;
+  OMNIA_REQUIRE(s.raw_queries && s.raw_keys && s.raw_values && queries && s.keys && s.values && s.tables && s.lengths &&
+                    s.token_map,
+                "attention_batch_project: null pointer");
+  OMNIA_REQUIRE(aligned16(s.raw_queries) && aligned16(s.raw_keys) && aligned16(s.raw_values) && aligned16(queries) &&
+                    aligned16(s.keys) && aligned16(s.values) && aligned16(s.query_weight) && aligned16(s.key_weight),
+                "attention_batch_project: pointers must be 16-byte aligned");
+  OMNIA_REQUIRE(s.query_stride % 8 == 0 && s.key_stride % 8 == 0 && s.value_stride % 8 == 0 &&
+                    s.query_stride >= s.heads * s.head_dim && s.key_stride >= s.kv_heads * s.head_dim &&
+                    s.value_stride >= s.kv_heads * s.head_dim,
+                "attention_batch_project: row strides must be multiples of 8 covering the heads");
+  OMNIA_REQUIRE(s.rotary_pairs == 0 || (s.cos_rows && s.sin_rows && aligned16(s.cos_rows) && aligned16(s.sin_rows) &&
+                                        s.table_stride % 4 == 0 && s.table_stride >= s.rotary_pairs && s.angle_rows > 0),
+                "attention_batch_project: angle rows must be 16-byte aligned and cover the pairs");
+  return 0;
+}
+
+BatchProjectArgs project_args(const omnia_attention_batch_step_t& s, void* queries, int32_t wide) {
+  return BatchProjectArgs{{s.raw_queries, s.raw_keys, s.raw_values}, {s.query_stride, s.key_stride, s.value_stride},
+                          {s.query_weight, s.key_weight}, s.cos_rows, s.sin_rows, s.table_stride, s.angle_rows, queries,
+                          {s.keys, s.values},
+                          {s.tables, s.lengths, reinterpret_cast<const int2*>(s.token_map),
+                           static_cast<int>(s.sequences), static_cast<int>(s.width), static_cast<int>(s.pages),
+                           page_shift_of(s.page_rows)},
+                          static_cast<int>(s.heads), static_cast<int>(s.kv_heads), static_cast<int>(s.tokens),
+                          static_cast<int>(s.rotary_pairs), wide != 0 ? 1 : 0, s.mscale, s.eps};
+}
+
+int32_t project(const omnia_attention_batch_step_t& s, void* queries, int32_t wide, hipStream_t stream) {
+  int32_t rc = project_refused(s, queries);
+  if (rc != 0 || s.tokens == 0) return rc;
+  rc = check_device(stream);
+  if (rc != 0) return rc;
+  const BatchProjectArgs a = project_args(s, queries, wide);
+  // Up to four heads in turn, the same number in every workgroup of a token (7,133 tokens of 80
+  // heads of 64, 32 at once: three in turn 30.6 us, four 31.8; 4,000 of 12 heads of 128, 16 at
+  // once: one 9.9, four 13.6). Below 1,024 tokens one is the faster (900 of 80: 9.0 for 9.3).
+  const int64_t at_once = 256 / (s.head_dim / 8), rounds = (s.heads + 2 * s.kv_heads + at_once - 1) / at_once;
+  const int64_t parts = s.tokens < 1024 ? rounds : (rounds + 3) / 4;   // at most 768
+  const dim3 grid(static_cast<unsigned>(s.tokens), static_cast<unsigned>(parts));
+  const auto launch = [&](auto one, auto two, auto three, auto four) {
+    const int64_t turns = (rounds + parts - 1) / parts;
+    (turns == 1 ? one : turns == 2 ? two : turns == 3 ? three : four)<<<grid, 256, 0, stream>>>(a);
+  };
+  if (s.head_dim == 64) {
+    launch(attention_batch_project_kernel<64, 1>, attention_batch_project_kernel<64, 2>,
+           attention_batch_project_kernel<64, 3>, attention_batch_project_kernel<64, 4>);
+  } else {
+    launch(attention_batch_project_kernel<128, 1>, attention_batch_project_kernel<128, 2>,
+           attention_batch_project_kernel<128, 3>, attention_batch_project_kernel<128, 4>);
+  }
+  return launched("attention_batch_project");
+}
+
 }  // namespace
 }  // namespace omnia
 
@@ -1249,54 +1534,36 @@ extern "C" int32_t omnia_attention_batch_project(
     int32_t wide_queries, uint16_t* keys, uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
     int64_t width, const int32_t* lengths, const int32_t* token_map, hipStream_t stream) {
   using namespace omnia;
-  OMNIA_REQUIRE(geometry_served(tokens, heads, kv_heads, head_dim, 0, 0, 0), "attention_batch_project: bad geometry");
-  OMNIA_REQUIRE(rotary_pairs >= 0 && rotary_pairs % 8 == 0 && 2 * rotary_pairs <= head_dim,
-                "attention_batch_project: rotary_pairs must be a multiple of 8 within the head");
-  const int shift = page_shift_of(page_rows);
-  OMNIA_REQUIRE(shift > 0, "attention_batch_project: page_rows must be 16, 32, 64, 128 or 256");
-  OMNIA_REQUIRE(pages > 0 && pages < (int64_t{1} << 31) && sequences > 0 && sequences < (int64_t{1} << 31) &&
-                    width > 0 && width < (int64_t{1} << 31) / page_rows,
-                "attention_batch_project: bad tables");
-  if (tokens == 0) return 0;
-  OMNIA_REQUIRE(raw_queries && raw_keys && raw_values && queries && keys && values && tables && lengths && token_map,
-                "attention_batch_project: null pointer");
-  OMNIA_REQUIRE(aligned16(raw_queries) && aligned16(raw_keys) && aligned16(raw_values) && aligned16(queries) &&
-                    aligned16(keys) && aligned16(values) && aligned16(query_weight) && aligned16(key_weight),
-                "attention_batch_project: pointers must be 16-byte aligned");
-  OMNIA_REQUIRE(query_stride % 8 == 0 && key_stride % 8 == 0 && value_stride % 8 == 0 &&
-                    query_stride >= heads * head_dim && key_stride >= kv_heads * head_dim &&
-                    value_stride >= kv_heads * head_dim,
-                "attention_batch_project: row strides must be multiples of 8 covering the heads");
-  OMNIA_REQUIRE(rotary_pairs == 0 || (cos_rows && sin_rows && aligned16(cos_rows) && aligned16(sin_rows) &&
-                                      table_stride % 4 == 0 && table_stride >= rotary_pairs && angle_rows > 0),
-                "attention_batch_project: angle rows must be 16-byte aligned and cover the pairs");
-  int32_t rc = check_device(stream);
-  if (rc != 0) return rc;
-  const BatchProjectArgs a{{raw_queries, raw_keys, raw_values}, {query_stride, key_stride, value_stride},
-                           {query_weight, key_weight}, cos_rows, sin_rows, table_stride, angle_rows, queries,
-                           {keys, values},
-                           {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
-                            static_cast<int>(width), static_cast<int>(pages), shift},
-                           static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(tokens),
-                           static_cast<int>(rotary_pairs), wide_queries != 0 ? 1 : 0, mscale, eps};
-  // Up to four heads in turn, the same number in every workgroup of a token (7,133 tokens of 80
-  // heads of 64, 32 at once: three in turn 30.6 us, four 31.8; 4,000 of 12 heads of 128, 16 at
-  // once: one 9.9, four 13.6). Below 1,024 tokens one is the faster (900 of 80: 9.0 for 9.3).
-  const int64_t at_once = 256 / (head_dim / 8), rounds = (heads + 2 * kv_heads + at_once - 1) / at_once;
-  const int64_t parts = tokens < 1024 ? rounds : (rounds + 3) / 4;   // at most 768
-  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(parts));
-  const auto launch = [&](auto one, auto two, auto three, auto four) {
-    const int64_t turns = (rounds + parts - 1) / parts;
-    (turns == 1 ? one : turns == 2 ? two : turns == 3 ? three : four)<<<grid, 256, 0, stream>>>(a);
-  };
-  if (head_dim == 64) {
-    launch(attention_batch_project_kernel<64, 1>, attention_batch_project_kernel<64, 2>,
-           attention_batch_project_kernel<64, 3>, attention_batch_project_kernel<64, 4>);
-  } else {
-    launch(attention_batch_project_kernel<128, 1>, attention_batch_project_kernel<128, 2>,
-           attention_batch_project_kernel<128, 3>, attention_batch_project_kernel<128, 4>);
-  }
-  return launched("attention_batch_project");
+  omnia_attention_batch_step_t s{};
+  s.raw_queries = raw_queries;
+  s.raw_keys = raw_keys;
+  s.raw_values = raw_values;
+  s.query_stride = query_stride;
+  s.key_stride = key_stride;
+  s.value_stride = value_stride;
+  s.query_weight = query_weight;
+  s.key_weight = key_weight;
+  s.cos_rows = cos_rows;
+  s.sin_rows = sin_rows;
+  s.table_stride = table_stride;
+  s.angle_rows = angle_rows;
+  s.rotary_pairs = rotary_pairs;
+  s.mscale = mscale;
+  s.eps = eps;
+  s.tokens = tokens;
+  s.heads = heads;
+  s.kv_heads = kv_heads;
+  s.head_dim = head_dim;
+  s.keys = keys;
+  s.values = values;
+  s.pages = pages;
+  s.page_rows = page_rows;
+  s.tables = tables;
+  s.sequences = sequences;
+  s.width = width;
+  s.lengths = lengths;
+  s.token_map = token_map;
+  return project(s, queries, wide_queries, stream);
 }
 
 extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
@@ -1309,14 +1576,16 @@ extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t
   return splits == 1 ? 0 : splits * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queries, const uint16_t* keys,
+namespace omnia {
+namespace {
+// `fresh`: the step's prologue, where the kernels take the new tokens' raw rows in place of queries.
+int32_t attend(const BatchProjectArgs* fresh, const void* queries, int32_t wide_queries, const uint16_t* keys,
                                          const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
                                          int64_t width, const int32_t* lengths, const int32_t* token_map,
                                          int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
                                          int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                          const uint16_t* sinks, float scale, void* workspace, int64_t workspace_bytes,
                                          uint16_t* out, hipStream_t stream) {
-  using namespace omnia;
   OMNIA_REQUIRE(geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles),
                 "attention_batch: head_dim 64 or 128, heads a multiple of kv_heads, fewer than 2^30 rows");
   const int shift = page_shift_of(page_rows);
@@ -1346,23 +1615,38 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
                     static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(heads / kv_heads),
                     static_cast<int>(tokens), static_cast<int>(p.prefix), static_cast<int>(prefix_sequence),
                     static_cast<int>(p.prefix_tiles), static_cast<int>(own_tiles), static_cast<int>(p.prefix_splits), static_cast<int>(p.prefix_keys),
-                    static_cast<int>(p.own_splits), static_cast<int>(p.own_keys), scale * kLog2e};
+                    static_cast<int>(p.own_splits), static_cast<int>(p.own_keys), scale * kLog2e,
+                    fresh != nullptr ? *fresh : BatchProjectArgs{}};
   const int64_t blocks = kv_heads * (p.prefix_tiles * p.prefix_splits + own_tiles * p.own_splits);
   OMNIA_REQUIRE(blocks < (int64_t{1} << 31), "attention_batch: too many tiles");
   const bool wide = wide_queries != 0;
   if (p.own_alone) {
-    const auto kernel = head_dim == 64 ? (wide ? attention_own_kernel<64, 2> : attention_own_kernel<64, 1>)
-                                       : (wide ? attention_own_kernel<128, 2> : attention_own_kernel<128, 1>);
+    const auto kernel = head_dim == 64
+                            ? (fresh ? attention_own_kernel<64, 2, true> : wide ? attention_own_kernel<64, 2> : attention_own_kernel<64, 1>)
+                            : (fresh ? attention_own_kernel<128, 2, true> : wide ? attention_own_kernel<128, 2> : attention_own_kernel<128, 1>);
     kernel<<<dim3(static_cast<unsigned>(blocks)), 64, 0, stream>>>(a);
   } else if (blocks > 0) {
-    const auto kernel = head_dim == 64 ? (wide ? attention_batch_kernel<64, 2> : attention_batch_kernel<64, 1>)
-                                       : (wide ? attention_batch_kernel<128, 2> : attention_batch_kernel<128, 1>);
+    const auto kernel = head_dim == 64
+                            ? (fresh ? attention_batch_kernel<64, 2, true> : wide ? attention_batch_kernel<64, 2> : attention_batch_kernel<64, 1>)
+                            : (fresh ? attention_batch_kernel<128, 2, true> : wide ? attention_batch_kernel<128, 2> : attention_batch_kernel<128, 1>);
     kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
   }
   if (p.prefix_splits + p.own_splits != 1) {
     head_dim == 64 ? launch_merge<64>(a, stream) : launch_merge<128>(a, stream);
   }
   return launched("attention_batch");
+}
+}  // namespace
+}  // namespace omnia
+
+extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queries, const uint16_t* keys,
+                                         const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
+                                         int64_t width, const int32_t* lengths, const int32_t* token_map,
+                                         int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
+                                         int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         const uint16_t* sinks, float scale, void* workspace, int64_t workspace_bytes,
+                                         uint16_t* out, hipStream_t stream) {
+  return omnia::attend(nullptr, queries, wide_queries, keys, values, pages, page_rows, tables, sequences, width, lengths, token_map, tokens, tiles, own_tiles, prefix, prefix_sequence, own_rows, heads, kv_heads, head_dim, sinks, scale, workspace, workspace_bytes, out, stream);
 }
 
 extern "C" int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -1376,24 +1660,19 @@ extern "C" int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t head
 extern "C" int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* s, hipStream_t stream) {
   using namespace omnia;
   OMNIA_REQUIRE(s != nullptr, "attention_batch_step: null pointer");
-  const auto project = [&](void* queries, int32_t wide) {
-    return omnia_attention_batch_project(
-        s->raw_queries, s->query_stride, s->raw_keys, s->key_stride, s->raw_values, s->value_stride, s->query_weight,
-        s->key_weight, s->cos_rows, s->sin_rows, s->table_stride, s->angle_rows, s->rotary_pairs, s->mscale, s->eps,
-        s->tokens, s->heads, s->kv_heads, s->head_dim, queries, wide, s->keys, s->values, s->pages, s->page_rows,
-        s->tables, s->sequences, s->width, s->lengths, s->token_map, stream);
-  };
-  if (s->queries != nullptr) return project(s->queries, 0);
+  if (s->queries != nullptr) return project(*s, s->queries, 0, stream);
   const int64_t need = omnia_attention_batch_step_bytes(s->tokens, s->heads, s->kv_heads, s->head_dim, s->prefix,
                                                         s->own_rows, s->own_tiles);
   OMNIA_REQUIRE(need >= 0, "attention_batch_step: bad geometry");
   OMNIA_REQUIRE(need == 0 || (s->workspace && s->workspace_bytes >= need && aligned16(s->workspace)),
                 "attention_batch_step: workspace too small (omnia_attention_batch_step_bytes) or not aligned");
   const int64_t queries = query_bytes(s->tokens, s->heads, s->head_dim);
-  const int32_t rc = project(s->workspace, 1);
+  const bool fresh = takes_fresh(*s);
+  const int32_t rc = fresh ? project_refused(*s, s->workspace) : project(*s, s->workspace, 1, stream);
   if (rc != 0) return rc;
-  return omnia_attention_batch(s->workspace, 1, s->keys, s->values, s->pages, s->page_rows, s->tables, s->sequences,
-                               s->width, s->lengths, s->token_map, s->tokens, s->tiles, s->own_tiles, s->prefix,
-                               s->prefix_sequence, s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
-                               static_cast<char*>(s->workspace) + queries, s->workspace_bytes - queries, s->out, stream);
+  const BatchProjectArgs rows = project_args(*s, s->workspace, 1);
+  return attend(fresh ? &rows : nullptr, s->workspace, 1, s->keys, s->values, s->pages, s->page_rows, s->tables,
+                s->sequences, s->width, s->lengths, s->token_map, s->tokens, s->tiles, s->own_tiles, s->prefix,
+                s->prefix_sequence, s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
+                static_cast<char*>(s->workspace) + queries, s->workspace_bytes - queries, s->out, stream);
 }

@@ -224,7 +224,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
                 core.query_weight, core.key_weight, angles, cache.keys[core.layer], cache.values[core.layer],
                 cache.tables, cache.lengths, batch.token_map, batch.tiles(core.heads // core.kv_heads),
                 heads=core.heads, prefix=batch.prefix, prefix_sequence=batch.sequences[0], scale=core.scale,
-                eps=core.eps, mscale=core.mscale, sinks=core.sinks)
+                eps=core.eps, mscale=core.mscale, sinks=core.sinks, one_token_each=batch.total == len(batch.sequences))
             batch.plans[self] = plan, cache.keys
         if batch.reach and _capturing(cache.keys.device) and all(plan is not held for held in batch.captured):
             batch.captured.append(plan)   # and with it the angles, should the atlas grow

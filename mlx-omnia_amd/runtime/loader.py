@@ -31,7 +31,7 @@ class BatchStep(ctypes.Structure):
         + [(name, _I64) for name in (
             "workspace_bytes", "query_stride", "key_stride", "value_stride", "table_stride", "angle_rows",
             "rotary_pairs", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_rows", "sequences", "width",
-            "own_tiles", "prefix", "prefix_sequence", "own_rows")]
+            "own_tiles", "prefix", "prefix_sequence", "own_rows", "one_token_each")]
         + [(name, _F32) for name in ("mscale", "eps", "scale")])
 
 

@@ -1446,10 +1446,12 @@ class BatchStepPlan:
     """A layer's step of one batch, its arguments checked and laid out once for
     `omnia_attention_batch_step`: what stays the same from step to step. Calling it with the raw
     rows and `own_rows` gives the context [N, heads, D] bf16, `project` the queries alone. The
-    arguments are those of `attention_batch_project` and `attention_batch`."""
+    arguments are those of `attention_batch_project` and `attention_batch`; one_token_each says
+    that no sequence has more than one new token."""
 
     def __init__(self, query_weight, key_weight, angles, keys, values, tables, lengths, token_map, tiles, *, heads: int,
-                 prefix: int, prefix_sequence: int, scale: float, eps: float, mscale: float = 1.0, sinks=None) -> None:
+                 prefix: int, prefix_sequence: int, scale: float, eps: float, mscale: float = 1.0, sinks=None,
+                 one_token_each: bool = False) -> None:
         pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch_step")
         sequences, width = _page_tables(tables, lengths, "attention_batch_step")
         tokens = token_map.shape[0]
@@ -1489,7 +1491,8 @@ class BatchStepPlan:
             angle_rows=self.angle_rows or 0, rotary_pairs=0 if cos is None else cos.shape[1], tokens=tokens,
             heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=pages, page_rows=page_rows, sequences=sequences,
             width=width, own_tiles=tiles.shape[0], prefix=prefix,
-            prefix_sequence=prefix_sequence, own_rows=-1, mscale=mscale, eps=eps, scale=scale)
+            prefix_sequence=prefix_sequence, own_rows=-1, one_token_each=int(one_token_each), mscale=mscale, eps=eps,
+            scale=scale)
         self.sized = -1, 0   # own rows, and the workspace that they need
         # What results are made like, without a call's parsing of their kind and place.
         self.keys, self.like = keys, keys.view(-1)[:1].expand(tokens, heads, head_dim)

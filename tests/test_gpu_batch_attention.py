@@ -195,6 +195,34 @@ def test_plans(case):
     made.check(None if made.batch.total * made.heads < 2000 else np.arange(0, made.batch.total, 7))
 
 
+@pytest.mark.parametrize("case", [c for c in PLANS + GEOMETRIES if c.get("tokens", 1) == 1],
+                         ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", ""))
+def test_a_step_writes_its_rows_and_no_others(case):
+    """Without the prologue's own launch ahead of it, which would have written them."""
+    made = Case(**case)
+    cache, size, d = made.cache, made.cache.page_rows, made.head_dim
+    before = [p.clone() for p in (cache.keys, cache.values)]
+    lengths = cache.lengths.cpu().numpy()
+    context = made.step(made.batch, *made.raw)   # which takes pages where a sequence's are full
+    tables = cache.tables.cpu().numpy()
+    raw, gain = [wide(t) for t in made.raw], None if made.kw is None else wide(made.kw)
+    cos, sin = wide(made.cos), wide(made.sin)
+    for t, (s, j) in enumerate(made.batch.token_map.cpu().numpy()):
+        p = int(lengths[s]) + j
+        angles = (cos[p], sin[p]) if made.pairs else (None, None)
+        page, row = int(tables[s, p // size]), p % size
+        key, value = (wide(pool[made.layer, page, :, row]) for pool in (cache.keys, cache.values))
+        want = turned(raw[1][t].reshape(-1, d), gain, *angles, 1e-6, made.mscale)
+        assert np.all(np.abs(key - want) <= HALF * np.abs(want) + 2.0 ** -19 * np.abs(want).max(axis=1, keepdims=True))
+        assert np.array_equal(value, raw[2][t].reshape(-1, d))
+        for pool, was in zip((cache.keys, cache.values), before):
+            was[made.layer, page, :, row] = pool[made.layer, page, :, row]
+    for pool, was in zip((cache.keys, cache.values), before):
+        assert torch.equal(pool.view(torch.int16), was.view(torch.int16))
+    if made.batch.total * made.heads < 2000:
+        made.check_context(context, made.wide_queries(), lengths)
+
+
 def test_values_that_are_not_finite_among_own_rows_alone():
     """Rows behind a token's own are not there for it, whatever they hold, 16 rows of a tile at a time."""
     case = Case(heads=24, kv_heads=8, head_dim=128, page_rows=64, own=(2900, 17) + (2750,) * 21, tokens=(1, 20) + (1,) * 21)
