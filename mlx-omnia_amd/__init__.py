@@ -12,6 +12,9 @@ and registers hand-written HIP kernels ahead of the stock-op Core chains:
 - `kernels.gate_softplus.GateSoftplus`   -exp(A_log) * softplus(a + dt_bias)
 - `kernels.route.Route`                  softmax -> top-k -> renormalise
 - `kernels.route.ResidualRouter`         residual add + RMSNorm + router projection + top-k
+- `kernels.attention.AttentionStep`      one sequence's attention step over its KV cache
+- `kernels.attention.PagedKVCache`       a KV cache of pages that sequences share
+- `kernels.attention.BatchAttentionStep` a batch's attention step over that cache
 
 The kernels live in `libomnia_hip.so` (sources under `csrc/`, C ABI in
 `include/omnia_hip.h`), loaded by `runtime.library`.
