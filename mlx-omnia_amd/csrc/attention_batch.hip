@@ -1355,15 +1355,15 @@ void launch_merge(const BatchArgs& a, hipStream_t stream) {
 }
 
 // How the keys are cut: the shared rows and the sequences' own each into pieces of a multiple
-// of 64 keys. A wide piece leaves 128 rows of context for the merge, so there are about two
-// workgroups a CU of them, of at least four tiles; a narrow one leaves a few rows and is short,
-// so that sequences of different lengths fill the card evenly.
+// of 64 keys. A wide piece leaves 128 rows of context for the merge and takes a while to start; a
+// narrow one leaves a few rows and is short, so that sequences of different lengths fill the card
+// evenly.
 struct Plan {
   int64_t prefix, prefix_tiles, prefix_splits, prefix_keys, own_splits, own_keys;
   bool own_alone;   // own pieces only, a wave each
 };
 
-constexpr int64_t kSlots = 512, kWideKeys = 256, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
+constexpr int64_t kSlots = 512, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
 constexpr int64_t kOwnKeys = 256, kOwnPieces = 2048;
 
 // `splits` pieces of whole tiles of 64 keys, or as many as those leave, and the keys of one.
@@ -1375,29 +1375,82 @@ int64_t cut(int64_t keys, int64_t splits, int64_t& each) {
   return (tiles + of_one - 1) / of_one;
 }
 
-// Pieces of `keys` keys for each of `blocks` workgroups, and the keys of one; `taken` workgroups
+// What wide pieces were measured to take, in us: one on a CU waits for its keys, two share the
+// matrix cores and the start's loads.
+struct WideCost {
+  double start, tile, start_both, tile_both, tile_bytes;
+};
+constexpr WideCost kCost64{4.0, 1.2, 5.0, 1.6, 16384.0}, kCost128{5.5, 2.0, 7.5, 2.57, 32768.0};
+constexpr double kBytesPerUs = 6e6, kLaunchUs = 4.0;
+
+// `count` pieces of `tiles` tiles, of which `row_tiles` read the same keys.
+double wide_us(const WideCost& c, int64_t count, int64_t tiles, int64_t row_tiles) {
+  const auto round = [&](int64_t n) {
+    if (n <= 0) return 0.0;
+    const bool both = n > kSlots / 2;
+    const double memory = n * c.tile_bytes / row_tiles / kBytesPerUs, tile = both ? c.tile_both : c.tile;
+    return (both ? c.start_both : c.start * (0.65 + 0.7 * n / kSlots)) + tiles * (memory > tile ? memory : tile);
+  };
+  return count / kSlots * round(kSlots) + round(count % kSlots);
+}
+
+// What runs beside wide pieces and is merged with them: how many pieces, what one takes, and what
+// all of them take where they have the card to themselves. `fresh`: one token a sequence, whose
+// prologue is spared where all pieces run at once.
+struct Beside {
+  double pieces, us, all_us;
+  int64_t blocks;
+  bool fresh;
+};
+
+// Wide pieces: as many as are expected to be done first, with their partial results (`row_us` for
+// a piece of every row) and the merge's launch, and what is beside them and finds no slot
+// meanwhile. Against as many as fill the slots, of 256 keys or more (replayed): 128 tokens behind
+// 32,768 rows with up to 1,024 own each 166 -> 155 us, 128 behind 4,096 95 -> 78, 96 behind 4,000
+// 43 -> 41, 100 of two kv heads behind 8,192 34.7 -> 27.9, nine prompts of up to 100 tokens behind
+// 2,048 79 -> 60.
+int64_t wide_splits(int64_t blocks, int64_t keys, const WideCost& c, int64_t row_tiles, double row_us,
+                    const Beside& beside, int64_t& each) {
+  const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t splits = 1; splits <= kMaxSplits && splits <= tiles; ++splits) {
+    const int64_t of_one = (tiles + splits - 1) / splits;
+    if ((tiles + of_one - 1) / of_one != splits) continue;   // as another one
+    const int64_t count = blocks * splits;
+    double us = wide_us(c, count, of_one, row_tiles);
+    if (beside.pieces > 0) {
+      // Beside the others one takes a quarter longer, and with every slot taken the last wait.
+      const double meanwhile = count < kSlots ? 0.8 * (kSlots - count) * us / beside.us : 0.0;
+      if (count > kSlots / 16 * 15) us *= 1.05;
+      if (meanwhile < beside.pieces) us += (beside.pieces - meanwhile) / beside.pieces * beside.all_us;
+      if (beside.fresh && count + beside.blocks > kSlots) us += kLaunchUs;
+    }
+    if (splits > 1 || beside.pieces > 0) us += kLaunchUs + splits * row_us;
+    if (splits == 1 || us < least) {
+      least = us;
+      best = splits;
+    }
+  }
+  return cut(keys, best, each);
+}
+
+// Narrow pieces of `keys` keys for each of `blocks` workgroups, and the keys of one; `taken` workgroups
 // start before them.
-int64_t pieces(int64_t blocks, int64_t keys, bool narrow, int64_t taken, int64_t& each) {
-  each = kTileKeys;
-  if (keys <= 0 || blocks <= 0) return 0;
+int64_t narrow_splits(int64_t blocks, int64_t keys, int64_t taken, int64_t& each) {
   const auto fill = [&](int64_t target, int64_t least) {
     const int64_t splits = (target + blocks - 1) / blocks, by_keys = keys / least;
     return splits < by_keys ? splits : by_keys;
   };
-  if (narrow) {
-    // Short ones where slots that are left would be empty, else longer (384 beside 312 others: 45.0
-    // us in two pieces each, 42.5 in one).
-    const int64_t splits = fill(kNarrowBlocks, kNarrowKeys);
-    const int64_t slots = taken >= kSlots ? kSlots : taken > kSlots / 2 ? kSlots / 2 : kSlots - taken;
-    return cut(keys, blocks * splits < slots ? fill(slots, kNarrowKeys / 4) : splits, each);
-  }
-  int64_t splits = fill(kSlots, kWideKeys);
-  // They run in rounds of as many as fit the card: fewer, where they fill theirs as well.
-  if (splits > 1 && blocks * (splits - 1) <= kSlots && blocks * (splits - 1) * 8 >= kSlots * 7) --splits;
-  return cut(keys, splits, each);
+  // Short ones where slots that are left would be empty, else longer (384 beside 312 others: 45.0
+  // us in two pieces each, 42.5 in one).
+  const int64_t splits = fill(kNarrowBlocks, kNarrowKeys);
+  const int64_t slots = taken >= kSlots ? kSlots : taken > kSlots / 2 ? kSlots / 2 : kSlots - taken;
+  return cut(keys, blocks * splits < slots ? fill(slots, kNarrowKeys / 4) : splits, each);
 }
 
-Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, int64_t own_rows, int64_t own_tiles) {
+Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t prefix, int64_t own_rows,
+              int64_t own_tiles) {
   Plan p{};
   const int64_t rows = tokens * (heads / kv_heads);
   const int64_t shared_tiles = (rows + kTileRows - 1) / kTileRows;
@@ -1409,18 +1462,47 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t prefix, i
   p.prefix = own_tiles * 4 <= shared_tiles * 5 || few ? 0 : prefix;
   own_rows += prefix - p.prefix;
   p.prefix_tiles = p.prefix > 0 ? shared_tiles : 0;
-  p.prefix_splits = pieces(kv_heads * p.prefix_tiles, p.prefix, rows <= kNarrowRows, 0, p.prefix_keys);
-  const bool narrow = rows <= kNarrowRows * own_tiles;
-  p.own_alone = p.prefix == 0 && narrow && kv_heads * own_tiles * own_rows >= kOwnPieces * kOwnKeys;
+  p.prefix_keys = p.own_keys = kTileKeys;
+  const int64_t own_blocks = kv_heads * own_tiles;
+  const bool narrow = rows <= kNarrowRows * own_tiles, any_own = own_rows > 0 && own_tiles > 0;
+  const WideCost& cost = head_dim == 64 ? kCost64 : kCost128;
+  // A piece's contexts of all rows, written and read.
+  const double row_us = static_cast<double>(tokens) * heads * head_dim * 8.0 / kBytesPerUs;
+  if (p.prefix > 0 && shared_tiles > 0) {
+    const int64_t blocks = kv_heads * shared_tiles;
+    if (rows <= kNarrowRows) {
+      p.prefix_splits = narrow_splits(blocks, p.prefix, 0, p.prefix_keys);
+    } else {
+      Beside own{0.0, 1.0, 0.0, 0, false};
+      if (any_own && narrow) {
+        // The sequences' lengths are taken to be spread up to own_rows.
+        const int64_t of_one = own_rows < kNarrowKeys ? own_rows : kNarrowKeys;
+        own = {own_blocks * ((own_rows + kNarrowKeys - 1) / kNarrowKeys + 1) / 2.0, 3.0 + 0.011 * of_one, 0.0, own_blocks,
+               own_tiles == tokens && heads <= kNarrowRows * kv_heads};
+        const double bytes = own_blocks * (own_rows / 2.0) * head_dim * 4.0;
+        own.all_us = own.pieces / kSlots * own.us;
+        if (own.all_us < bytes / kBytesPerUs) own.all_us = bytes / kBytesPerUs;
+      } else if (any_own) {
+        own = {static_cast<double>(own_blocks), cost.start + (own_rows + kTileKeys - 1) / kTileKeys * cost.tile, 0.0,
+               own_blocks, false};
+        own.all_us = own.pieces / kSlots * own.us;
+      }
+      p.prefix_splits = wide_splits(blocks, p.prefix, cost, shared_tiles, row_us, own, p.prefix_keys);
+    }
+  }
+  if (!any_own) return p;
+  p.own_alone = p.prefix == 0 && narrow && own_blocks * own_rows >= kOwnPieces * kOwnKeys;
   if (p.own_alone) {
     // All at once where that is possible: a wave that has done its piece leaves the others more
     // of the memory's rate, until the last ones cannot take it.
-    const int64_t fill = (kOwnPieces + kv_heads * own_tiles - 1) / (kv_heads * own_tiles);
+    const int64_t fill = (kOwnPieces + own_blocks - 1) / own_blocks;
     const int64_t most = own_rows / kOwnKeys, least = own_rows / (4 * kOwnKeys);
     p.own_splits = cut(own_rows, fill > most ? most : fill < least ? least : fill, p.own_keys);
+  } else if (narrow) {
+    p.own_splits = narrow_splits(own_blocks, own_rows, kv_heads * p.prefix_tiles * p.prefix_splits, p.own_keys);
   } else {
-    p.own_splits = pieces(kv_heads * own_tiles, own_rows, narrow, kv_heads * p.prefix_tiles * p.prefix_splits,
-                          p.own_keys);
+    p.own_splits = wide_splits(own_blocks, own_rows, cost, own_tiles, row_us,
+                               Beside{p.prefix > 0 ? 1e-9 : 0.0, 1.0, 0.0, 0, false}, p.own_keys);
   }
   return p;
 }
@@ -1456,7 +1538,7 @@ bool takes_fresh(const omnia_attention_batch_step_t& s) {
       s.heads > kNarrowRows * s.kv_heads) {
     return false;
   }
-  const Plan p = plan_for(s.tokens, s.heads, s.kv_heads, s.prefix, s.own_rows, s.own_tiles);
+  const Plan p = plan_for(s.tokens, s.heads, s.kv_heads, s.head_dim, s.prefix, s.own_rows, s.own_tiles);
   return p.own_alone || s.kv_heads * (p.prefix_tiles * p.prefix_splits + s.own_tiles) <= kSlots;
 }
 
@@ -1571,7 +1653,7 @@ extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t
                                                          int64_t own_tiles) {
   using namespace omnia;
   if (!geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles)) return -EINVAL;
-  const Plan p = plan_for(tokens, heads, kv_heads, prefix, own_rows, own_tiles);
+  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles);
   const int64_t splits = p.prefix_splits + p.own_splits;
   return splits == 1 ? 0 : splits * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
@@ -1607,7 +1689,7 @@ int32_t attend(const BatchProjectArgs* fresh, const void* queries, int32_t wide_
                 "attention_batch: workspace too small (omnia_attention_batch_workspace_bytes) or not aligned");
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
-  const Plan p = plan_for(tokens, heads, kv_heads, prefix, own_rows, own_tiles);
+  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles);
   const BatchArgs a{queries, keys, values, reinterpret_cast<const int4*>(tiles), sinks, out,
                     static_cast<float*>(workspace),
                     {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
