@@ -1394,13 +1394,13 @@ double wide_us(const WideCost& c, int64_t count, int64_t tiles, int64_t row_tile
   return count / kSlots * round(kSlots) + round(count % kSlots);
 }
 
-// What runs beside wide pieces and is merged with them: how many pieces, what one takes, and what
-// all of them take where they have the card to themselves. `fresh`: one token a sequence, whose
-// prologue is spared where all pieces run at once.
+// What runs beside wide pieces and is merged with them: whether there is anything, how many pieces
+// start after them, what one takes, and what all of them take where they have the card to
+// themselves. `fresh`: one token a sequence, whose prologue is spared where all pieces run at once.
 struct Beside {
-  double pieces, us, all_us;
+  bool any, fresh;
   int64_t blocks;
-  bool fresh;
+  double pieces, us, all_us;
 };
 
 // Wide pieces: as many as are expected to be done first, with their partial results (`row_us` for
@@ -1426,7 +1426,7 @@ int64_t wide_splits(int64_t blocks, int64_t keys, const WideCost& c, int64_t row
       if (meanwhile < beside.pieces) us += (beside.pieces - meanwhile) / beside.pieces * beside.all_us;
       if (beside.fresh && count + beside.blocks > kSlots) us += kLaunchUs;
     }
-    if (splits > 1 || beside.pieces > 0) us += kLaunchUs + splits * row_us;
+    if (splits > 1 || beside.any) us += kLaunchUs + splits * row_us;
     if (splits == 1 || us < least) {
       least = us;
       best = splits;
@@ -1473,20 +1473,20 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
     if (rows <= kNarrowRows) {
       p.prefix_splits = narrow_splits(blocks, p.prefix, 0, p.prefix_keys);
     } else {
-      Beside own{0.0, 1.0, 0.0, 0, false};
+      Beside own{any_own, false, own_blocks, 0.0, 1.0, 0.0};
       if (any_own && narrow) {
         // The sequences' lengths are taken to be spread up to own_rows.
         const int64_t of_one = own_rows < kNarrowKeys ? own_rows : kNarrowKeys;
-        own = {own_blocks * ((own_rows + kNarrowKeys - 1) / kNarrowKeys + 1) / 2.0, 3.0 + 0.011 * of_one, 0.0, own_blocks,
-               own_tiles == tokens && heads <= kNarrowRows * kv_heads};
-        const double bytes = own_blocks * (own_rows / 2.0) * head_dim * 4.0;
-        own.all_us = own.pieces / kSlots * own.us;
-        if (own.all_us < bytes / kBytesPerUs) own.all_us = bytes / kBytesPerUs;
+        own.fresh = own_tiles == tokens && heads <= kNarrowRows * kv_heads;
+        own.pieces = own_blocks * ((own_rows + kNarrowKeys - 1) / kNarrowKeys + 1) / 2.0;
+        own.us = 3.0 + 0.011 * of_one;
       } else if (any_own) {
-        own = {static_cast<double>(own_blocks), cost.start + (own_rows + kTileKeys - 1) / kTileKeys * cost.tile, 0.0,
-               own_blocks, false};
-        own.all_us = own.pieces / kSlots * own.us;
+        own.pieces = static_cast<double>(own_blocks);
+        own.us = cost.start + (own_rows + kTileKeys - 1) / kTileKeys * cost.tile;
       }
+      own.all_us = own.pieces / kSlots * own.us;
+      const double bytes = narrow ? own_blocks * (own_rows / 2.0) * head_dim * 4.0 : 0.0;
+      if (own.all_us < bytes / kBytesPerUs) own.all_us = bytes / kBytesPerUs;
       p.prefix_splits = wide_splits(blocks, p.prefix, cost, shared_tiles, row_us, own, p.prefix_keys);
     }
   }
@@ -1502,7 +1502,7 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
     p.own_splits = narrow_splits(own_blocks, own_rows, kv_heads * p.prefix_tiles * p.prefix_splits, p.own_keys);
   } else {
     p.own_splits = wide_splits(own_blocks, own_rows, cost, own_tiles, row_us,
-                               Beside{p.prefix > 0 ? 1e-9 : 0.0, 1.0, 0.0, 0, false}, p.own_keys);
+                               Beside{p.prefix > 0, false, 0, 0.0, 1.0, 0.0}, p.own_keys);
   }
   return p;
 }
