@@ -184,6 +184,8 @@ PLANS = [
     dict(heads=16, kv_heads=8, head_dim=64, pairs=32, sinks=True, page_rows=256, prefix=0, own=(3000,) * 21 + (0, 1, 256)),
     dict(heads=24, kv_heads=8, head_dim=128, page_rows=64, prefix=0, own=(2900, 17, 0) + (2750,) * 21,
          tokens=(1, 20, 6) + (1,) * 21),
+    dict(heads=24, kv_heads=8, head_dim=128, pairs=32, norms=True, page_rows=64, prefix=0,
+         own=(2900, 0, 255, 256) + (2751,) * 20),
     dict(heads=16, kv_heads=4, head_dim=128, pairs=64, page_rows=64, prefix=0, own=(700, 0, 1500, 9, 64), tokens=(1, 300, 1, 2, 75)),
     dict(heads=16, kv_heads=4, head_dim=64, page_rows=16, prefix=320, own=(700, 0, 9, 64), tokens=(1, 150, 1, 1)),
 ]
@@ -305,6 +307,42 @@ def test_tokens_of_no_sequence_and_pages_of_no_pool(prefix):
     assert torch.equal(before.view(torch.int16), cache.keys.view(torch.int16))
 
 
+@pytest.mark.parametrize("prefix,one_each", [(64, True), (640, True), (640, False)])
+def test_a_step_with_rows_that_are_nowhere(prefix, one_each):
+    """A new row without a page is not stored and not seen; one of no sequence is zeros, and no page changes."""
+    case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, page_rows=16, prefix=prefix, own=(40, 32, 40, 3))
+    cache, batch, layer = case.cache, case.batch, case.layer
+    cache.ready(batch)
+    tables, token_map, tiles = cache.tables.clone(), batch.token_map.clone(), batch.tiles(4).clone()
+    lengths = cache.lengths.cpu().numpy()
+    tables[case.chosen[1], (prefix + 32) // 16] = -1              # where its new row would be
+    tables[case.chosen[0], prefix // 16 + 1] = cache.pages + 3    # some of its own rows
+    token_map[2, 0], tiles[2, 2] = -1, -1
+    good = case.wide_queries()   # which writes every row where it belongs
+    before = [p.clone() for p in (cache.keys, cache.values)]
+    plan = ops.BatchStepPlan(case.qw, case.kw, (case.cos, case.sin), cache.keys[layer], cache.values[layer], tables,
+                             cache.lengths, token_map, tiles, heads=8, prefix=prefix, prefix_sequence=case.chosen[3],
+                             scale=case.scale, eps=1e-6, one_token_each=one_each)
+    raw = [t + 1 for t in case.raw]   # other rows than those in the pages by now
+    out = plan(*raw, 41)
+    assert (out[2] == 0).all()
+    for pool, was in zip((cache.keys, cache.values), before):
+        for t in (0, 3):
+            s = case.chosen[t]
+            p = int(lengths[s])
+            page = int(tables[s, p // 16])
+            assert not torch.equal(pool[layer, page, :, p % 16], was[layer, page, :, p % 16])
+            was[layer, page, :, p % 16] = pool[layer, page, :, p % 16]
+        assert torch.equal(pool.view(torch.int16), was.view(torch.int16))
+    spare = [p.clone() for p in (cache.keys[layer], cache.values[layer])]
+    queries = ops.attention_batch_project(*raw, case.qw, case.kw, (case.cos, case.sin), *spare, cache.tables, cache.lengths,
+                                          batch.token_map, heads=8, eps=1e-6, wide_queries=True)
+    assert queries.shape == good.shape
+    want, size = attend(wide(queries), wide(cache.keys[layer]), wide(cache.values[layer]), tables.cpu().numpy(), lengths,
+                        token_map.cpu().numpy(), case.scale)
+    assert np.all(np.abs(wide(out) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
+
+
 @pytest.mark.parametrize("prefix,own", [(160, (9, 4, 1)), (640, (9, 4, 1)), (1600, (9, 4, 1, 30) * 4)])
 def test_sequences_shorter_than_the_shared_rows(prefix, own):
     """A plan that is not the cache's own: a sequence that ends inside the shared rows sees its
@@ -321,6 +359,15 @@ def test_sequences_shorter_than_the_shared_rows(prefix, own):
                         lengths.cpu().numpy(), batch.token_map.cpu().numpy(), case.scale)
     assert (out[2] == 0).all()
     assert np.all(np.abs(wide(out) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
+
+
+@pytest.mark.parametrize("case", [
+    dict(heads=4, kv_heads=1, head_dim=128, pairs=64, page_rows=256, own=(0,), tokens=9001),
+    dict(heads=16, kv_heads=4, head_dim=64, norms=True, page_rows=64, prefix=5120, own=(900, 0), tokens=(1, 4000)),
+    dict(heads=8, kv_heads=1, head_dim=64, sinks=True, page_rows=128, own=(70001,))], ids=["prompt", "beside", "long"])
+def test_long_ones(case):
+    made = Case(**case, layers=2)
+    made.check(np.unique(np.linspace(0, made.batch.total - 1, 9).astype(int)))
 
 
 @pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (24, 2, 128), (40, 2, 64), (70, 5, 128), (70, 7, 64),
