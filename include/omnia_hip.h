@@ -758,7 +758,7 @@ int32_t omnia_attention_batch_project(
  * device. */
 int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
                                               int64_t head_dim, int64_t prefix, int64_t own_rows,
-                                              int64_t own_tiles);
+                                              int64_t own_total, int64_t own_tiles);
 
 /* Attention of a batch's new tokens over their sequences' pages (rows written by
  * omnia_attention_batch_project), the rows that all of them share taken once:
@@ -768,7 +768,9 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  * in fp32, the weights rounded to bf16 for their product with the values, the result once to
  * bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
  * prefix) must be the same pages in every token's sequence: they are read through
- * prefix_sequence's. own_rows bounds the rows past them of every sequence, this step's included; tiles
+ * prefix_sequence's. own_rows bounds the rows past them of every sequence, this step's included;
+ * own_total is the sum of those rows over the tiles, each its sequence's, or 0: how the work is cut
+ * depends on it, the result does not beyond its rounding; tiles
  * [own_tiles, 4] int32 (device) are runs of query rows that cover every row once (of each kv
  * head, row r is token r / gqa, head r % gqa): (first, end, s, j) for the rows [first, end), at
  * most 128, of sequence s, whose new token j the first row is of.
@@ -782,7 +784,8 @@ int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
                               const int32_t* tables, int64_t sequences, int64_t width,
                               const int32_t* lengths, const int32_t* token_map, int64_t tokens,
                               const int32_t* tiles, int64_t own_tiles, int64_t prefix,
-                              int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads,
+                              int64_t prefix_sequence, int64_t own_rows, int64_t own_total,
+                              int64_t heads, int64_t kv_heads,
                               int64_t head_dim, const uint16_t* sinks, float scale,
                               void* workspace, int64_t workspace_bytes, uint16_t* out,
                               hipStream_t stream);
@@ -792,7 +795,7 @@ int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
  * from the next multiple of 256 bytes on, what omnia_attention_batch needs:
  * omnia_attention_batch_step_bytes. With `queries` not null only the first half runs, its
  * queries rounded to bf16 there. Every field is as the two entries take it; `raw_*`, `queries`,
- * `out` and `workspace` are what changes from call to call, `own_rows` from step to step.
+ * `out` and `workspace` are what changes from call to call, `own_rows` and `own_total` from step to step.
  * one_token_each 1 says that every token is of another sequence, with a tile of its own, and that
  * every sequence holds all the shared rows: heads of at most 16 a kv head with 0, 32 or 64 rotary
  * pairs are then projected where they are attended, without a launch of their own. */
@@ -806,12 +809,12 @@ typedef struct {
   void *workspace;
   int64_t workspace_bytes, query_stride, key_stride, value_stride, table_stride, angle_rows, rotary_pairs;
   int64_t tokens, heads, kv_heads, head_dim, pages, page_rows, sequences, width, own_tiles, prefix;
-  int64_t prefix_sequence, own_rows, one_token_each;
+  int64_t prefix_sequence, own_rows, own_total, one_token_each;
   float mscale, eps, scale;
 } omnia_attention_batch_step_t;
 int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
                                          int64_t head_dim, int64_t prefix, int64_t own_rows,
-                                         int64_t own_tiles);
+                                         int64_t own_total, int64_t own_tiles);
 int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hipStream_t stream);
 
 #ifdef __cplusplus

@@ -1427,13 +1427,14 @@ struct Beside {
   double pieces, us, all_us;
 };
 
-// Wide pieces: as many as are expected to be done first, with their partial results (`row_us` for
+// Wide pieces of `keys` keys, of which the part `filled` is there, for each of `blocks` workgroups:
+// as many as are expected to be done first, with their partial results (`row_us` for
 // a piece of every row) and the merge's launch, and what is beside them and finds no slot
 // meanwhile. Against as many as fill the slots, of 256 keys or more (replayed): 128 tokens behind
 // 32,768 rows with up to 1,024 own each 166 -> 155 us, 128 behind 4,096 95 -> 78, 96 behind 4,000
 // 43 -> 41, 100 of two kv heads behind 8,192 34.7 -> 27.9, nine prompts of up to 100 tokens behind
 // 2,048 79 -> 60.
-int64_t wide_splits(int64_t blocks, int64_t keys, const WideCost& c, int64_t row_tiles, double row_us,
+int64_t wide_splits(int64_t blocks, int64_t keys, double filled, const WideCost& c, int64_t row_tiles, double row_us,
                     const Beside& beside, int64_t& each) {
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   int64_t best = 1;
@@ -1441,7 +1442,8 @@ int64_t wide_splits(int64_t blocks, int64_t keys, const WideCost& c, int64_t row
   for (int64_t splits = 1; splits <= kMaxSplits && splits <= tiles; ++splits) {
     const int64_t of_one = (tiles + splits - 1) / splits;
     if ((tiles + of_one - 1) / of_one != splits) continue;   // as another one
-    const int64_t count = blocks * splits;
+    // Of pieces that are not all there, as many whole ones as they amount to.
+    const int64_t count = static_cast<int64_t>(blocks * splits * filled) + (filled < 1.0 ? 1 : 0);
     double us = wide_us(c, count, of_one, row_tiles);
     if (beside.pieces > 0) {
       // Beside the others one takes a quarter longer, and with every slot taken the last wait.
@@ -1459,9 +1461,10 @@ int64_t wide_splits(int64_t blocks, int64_t keys, const WideCost& c, int64_t row
   return cut(keys, best, each);
 }
 
-// Narrow pieces of `keys` keys for each of `blocks` workgroups, and the keys of one; `taken` workgroups
-// start before them.
-int64_t narrow_splits(int64_t blocks, int64_t keys, int64_t taken, int64_t& each) {
+// Narrow pieces of `keys` keys, of which the part `filled` is there, for each of `blocks`
+// workgroups, and the keys of one; `taken` workgroups start before them.
+int64_t narrow_splits(int64_t blocks, int64_t keys, double filled, int64_t taken, int64_t& each) {
+  if (filled < 0.5) blocks = static_cast<int64_t>(blocks * 2.0 * filled) + 1;
   const auto fill = [&](int64_t target, int64_t least) {
     const int64_t splits = (target + blocks - 1) / blocks, by_keys = keys / least;
     return splits < by_keys ? splits : by_keys;
@@ -1473,8 +1476,10 @@ int64_t narrow_splits(int64_t blocks, int64_t keys, int64_t taken, int64_t& each
   return cut(keys, blocks * splits < slots ? fill(slots, kNarrowKeys / 4) : splits, each);
 }
 
+// `own_total`: the own rows of every tile's sequence together, or 0 where they are not known and
+// taken to be spread up to own_rows (in prompts: to be as many).
 Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t prefix, int64_t own_rows,
-              int64_t own_tiles) {
+              int64_t own_total, int64_t own_tiles) {
   Plan p{};
   const int64_t rows = tokens * (heads / kv_heads);
   const int64_t shared_tiles = (rows + kTileRows - 1) / kTileRows;
@@ -1484,48 +1489,54 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
   // rows: 16 -> 13.4 us a step).
   const bool few = prefix + own_rows <= kNarrowKeys && kv_heads * own_tiles <= kSlots;
   p.prefix = own_tiles * 4 <= shared_tiles * 5 || few ? 0 : prefix;
+  if (own_total > 0) own_total += (prefix - p.prefix) * own_tiles;
   own_rows += prefix - p.prefix;
   p.prefix_tiles = p.prefix > 0 ? shared_tiles : 0;
   p.prefix_keys = p.own_keys = kTileKeys;
   const int64_t own_blocks = kv_heads * own_tiles;
   const bool narrow = rows <= kNarrowRows * own_tiles, any_own = own_rows > 0 && own_tiles > 0;
   const WideCost& cost = head_dim == 64 ? kCost64 : kCost128;
+  const double whole = static_cast<double>(own_rows) * own_tiles;
+  const double total = own_total <= 0 ? (narrow ? whole / 2.0 : whole) : own_total < whole ? own_total : whole;
+  const double filled = whole > 0.0 ? total / whole : 1.0;
   // A piece's contexts of all rows, written and read.
   const double row_us = static_cast<double>(tokens) * heads * head_dim * 8.0 / kBytesPerUs;
   if (p.prefix > 0 && shared_tiles > 0) {
     const int64_t blocks = kv_heads * shared_tiles;
     if (rows <= kNarrowRows) {
-      p.prefix_splits = narrow_splits(blocks, p.prefix, 0, p.prefix_keys);
+      p.prefix_splits = narrow_splits(blocks, p.prefix, 1.0, 0, p.prefix_keys);
     } else {
       Beside own{any_own, false, own_blocks, 0.0, 1.0, 0.0};
       if (any_own && narrow) {
-        // The sequences' lengths are taken to be spread up to own_rows.
         const int64_t of_one = own_rows < kNarrowKeys ? own_rows : kNarrowKeys;
         own.fresh = own_tiles == tokens && heads <= kNarrowRows * kv_heads;
-        own.pieces = own_blocks * ((own_rows + kNarrowKeys - 1) / kNarrowKeys + 1) / 2.0;
+        own.pieces = own_blocks * (filled * own_rows / kNarrowKeys + 0.5);
+        if (own.pieces < own_blocks) own.pieces = static_cast<double>(own_blocks);
         own.us = 3.0 + 0.011 * of_one;
       } else if (any_own) {
         own.pieces = static_cast<double>(own_blocks);
         own.us = cost.start + (own_rows + kTileKeys - 1) / kTileKeys * cost.tile;
       }
       own.all_us = own.pieces / kSlots * own.us;
-      const double bytes = narrow ? own_blocks * (own_rows / 2.0) * head_dim * 4.0 : 0.0;
+      const double bytes = narrow ? kv_heads * total * head_dim * 4.0 : 0.0;
       if (own.all_us < bytes / kBytesPerUs) own.all_us = bytes / kBytesPerUs;
-      p.prefix_splits = wide_splits(blocks, p.prefix, cost, shared_tiles, row_us, own, p.prefix_keys);
+      p.prefix_splits = wide_splits(blocks, p.prefix, 1.0, cost, shared_tiles, row_us, own, p.prefix_keys);
     }
   }
   if (!any_own) return p;
-  p.own_alone = p.prefix == 0 && narrow && own_blocks * own_rows >= kOwnPieces * kOwnKeys;
+  p.own_alone = p.prefix == 0 && narrow && 2.0 * kv_heads * total >= kOwnPieces * kOwnKeys;
   if (p.own_alone) {
     // All at once where that is possible: a wave that has done its piece leaves the others more
-    // of the memory's rate, until the last ones cannot take it.
-    const int64_t fill = (kOwnPieces + own_blocks - 1) / own_blocks;
+    // of the memory's rate, until the last ones cannot take it. Short ones where a few sequences
+    // have most of the rows (64 sequences of up to 567, but one of 4,000, of 3 tokens: 92 -> 48 us).
+    const int64_t even = filled < 0.5 ? static_cast<int64_t>(own_blocks * 2.0 * filled) + 1 : own_blocks;
+    const int64_t fill = (kOwnPieces + even - 1) / even;
     const int64_t most = own_rows / kOwnKeys, least = own_rows / (4 * kOwnKeys);
     p.own_splits = cut(own_rows, fill > most ? most : fill < least ? least : fill, p.own_keys);
   } else if (narrow) {
-    p.own_splits = narrow_splits(own_blocks, own_rows, kv_heads * p.prefix_tiles * p.prefix_splits, p.own_keys);
+    p.own_splits = narrow_splits(own_blocks, own_rows, filled, kv_heads * p.prefix_tiles * p.prefix_splits, p.own_keys);
   } else {
-    p.own_splits = wide_splits(own_blocks, own_rows, cost, own_tiles, row_us,
+    p.own_splits = wide_splits(own_blocks, own_rows, filled, cost, own_tiles, row_us,
                                Beside{p.prefix > 0, false, 0, 0.0, 1.0, 0.0}, p.own_keys);
   }
   return p;
@@ -1562,7 +1573,7 @@ bool takes_fresh(const omnia_attention_batch_step_t& s) {
       s.heads > kNarrowRows * s.kv_heads) {
     return false;
   }
-  const Plan p = plan_for(s.tokens, s.heads, s.kv_heads, s.head_dim, s.prefix, s.own_rows, s.own_tiles);
+  const Plan p = plan_for(s.tokens, s.heads, s.kv_heads, s.head_dim, s.prefix, s.own_rows, s.own_total, s.own_tiles);
   return p.own_alone || s.kv_heads * (p.prefix_tiles * p.prefix_splits + s.own_tiles) <= kSlots;
 }
 
@@ -1674,10 +1685,10 @@ extern "C" int32_t omnia_attention_batch_project(
 
 extern "C" int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads,
                                                          int64_t head_dim, int64_t prefix, int64_t own_rows,
-                                                         int64_t own_tiles) {
+                                                         int64_t own_total, int64_t own_tiles) {
   using namespace omnia;
-  if (!geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles)) return -EINVAL;
-  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles);
+  if (!geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles) || own_total < 0) return -EINVAL;
+  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_total, own_tiles);
   const int64_t splits = p.prefix_splits + p.own_splits;
   return splits == 1 ? 0 : splits * tokens * heads * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
@@ -1689,10 +1700,11 @@ int32_t attend(const BatchProjectArgs* fresh, const void* queries, int32_t wide_
                                          const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
                                          int64_t width, const int32_t* lengths, const int32_t* token_map,
                                          int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
-                                         int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t prefix_sequence, int64_t own_rows, int64_t own_total,
+                                         int64_t heads, int64_t kv_heads, int64_t head_dim,
                                          const uint16_t* sinks, float scale, void* workspace, int64_t workspace_bytes,
                                          uint16_t* out, hipStream_t stream) {
-  OMNIA_REQUIRE(geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles),
+  OMNIA_REQUIRE(geometry_served(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles) && own_total >= 0,
                 "attention_batch: head_dim 64 or 128, heads a multiple of kv_heads, fewer than 2^30 rows");
   const int shift = page_shift_of(page_rows);
   OMNIA_REQUIRE(shift > 0, "attention_batch: page_rows must be 16, 32, 64, 128 or 256");
@@ -1708,12 +1720,12 @@ int32_t attend(const BatchProjectArgs* fresh, const void* queries, int32_t wide_
   OMNIA_REQUIRE(aligned16(queries) && aligned16(keys) && aligned16(values) && aligned16(out) && aligned16(tiles),
                 "attention_batch: pointers must be 16-byte aligned");
   const int64_t need = omnia_attention_batch_workspace_bytes(tokens, heads, kv_heads, head_dim, prefix, own_rows,
-                                                             own_tiles);
+                                                             own_total, own_tiles);
   OMNIA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                 "attention_batch: workspace too small (omnia_attention_batch_workspace_bytes) or not aligned");
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
-  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_tiles);
+  const Plan p = plan_for(tokens, heads, kv_heads, head_dim, prefix, own_rows, own_total, own_tiles);
   const BatchArgs a{queries, keys, values, reinterpret_cast<const int4*>(tiles), sinks, out,
                     static_cast<float*>(workspace),
                     {tables, lengths, reinterpret_cast<const int2*>(token_map), static_cast<int>(sequences),
@@ -1749,17 +1761,21 @@ extern "C" int32_t omnia_attention_batch(const void* queries, int32_t wide_queri
                                          const uint16_t* values, int64_t pages, int64_t page_rows, const int32_t* tables, int64_t sequences,
                                          int64_t width, const int32_t* lengths, const int32_t* token_map,
                                          int64_t tokens, const int32_t* tiles, int64_t own_tiles, int64_t prefix,
-                                         int64_t prefix_sequence, int64_t own_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t prefix_sequence, int64_t own_rows, int64_t own_total,
+                                         int64_t heads, int64_t kv_heads, int64_t head_dim,
                                          const uint16_t* sinks, float scale, void* workspace, int64_t workspace_bytes,
                                          uint16_t* out, hipStream_t stream) {
-  return omnia::attend(nullptr, queries, wide_queries, keys, values, pages, page_rows, tables, sequences, width, lengths, token_map, tokens, tiles, own_tiles, prefix, prefix_sequence, own_rows, heads, kv_heads, head_dim, sinks, scale, workspace, workspace_bytes, out, stream);
+  return omnia::attend(nullptr, queries, wide_queries, keys, values, pages, page_rows, tables, sequences, width, lengths,
+                       token_map, tokens, tiles, own_tiles, prefix, prefix_sequence, own_rows, own_total, heads, kv_heads,
+                       head_dim, sinks, scale, workspace, workspace_bytes, out, stream);
 }
 
 extern "C" int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                                    int64_t prefix, int64_t own_rows, int64_t own_tiles) {
+                                                    int64_t prefix, int64_t own_rows, int64_t own_total,
+                                                    int64_t own_tiles) {
   using namespace omnia;
   const int64_t more = omnia_attention_batch_workspace_bytes(tokens, heads, kv_heads, head_dim, prefix, own_rows,
-                                                             own_tiles);
+                                                             own_total, own_tiles);
   return more < 0 ? more : query_bytes(tokens, heads, head_dim) + more;
 }
 
@@ -1768,7 +1784,7 @@ extern "C" int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t
   OMNIA_REQUIRE(s != nullptr, "attention_batch_step: null pointer");
   if (s->queries != nullptr) return project(*s, s->queries, 0, stream);
   const int64_t need = omnia_attention_batch_step_bytes(s->tokens, s->heads, s->kv_heads, s->head_dim, s->prefix,
-                                                        s->own_rows, s->own_tiles);
+                                                        s->own_rows, s->own_total, s->own_tiles);
   OMNIA_REQUIRE(need >= 0, "attention_batch_step: bad geometry");
   OMNIA_REQUIRE(need == 0 || (s->workspace && s->workspace_bytes >= need && aligned16(s->workspace)),
                 "attention_batch_step: workspace too small (omnia_attention_batch_step_bytes) or not aligned");
@@ -1779,6 +1795,6 @@ extern "C" int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t
   const BatchProjectArgs rows = project_args(*s, s->workspace, 1);
   return attend(fresh ? &rows : nullptr, s->workspace, 1, s->keys, s->values, s->pages, s->page_rows, s->tables,
                 s->sequences, s->width, s->lengths, s->token_map, s->tokens, s->tiles, s->own_tiles, s->prefix,
-                s->prefix_sequence, s->own_rows, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
+                s->prefix_sequence, s->own_rows, s->own_total, s->heads, s->kv_heads, s->head_dim, s->sinks, s->scale,
                 static_cast<char*>(s->workspace) + queries, s->workspace_bytes - queries, s->out, stream);
 }

@@ -246,7 +246,9 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         if self._followed(raw_queries, raw_keys, raw_values):
             return self.core(batch, raw_queries, raw_keys, raw_values)
         plan, last = self._plan(batch)
-        return plan(raw_queries, raw_keys, raw_values, last - batch.prefix)
+        # (What replays that go further reach in all is not known.)
+        total = batch.own_total(self.core.heads // self.core.kv_heads) if last == batch.last else 0
+        return plan(raw_queries, raw_keys, raw_values, last - batch.prefix, total)
 
 
 _STRATEGIES = (HipBatchAttentionStep, DefaultBatchAttentionStep)

@@ -75,7 +75,9 @@ class PagedBatch:
         self.last = 0                 # the most rows a sequence has in the step at hand
         self.plans: dict = {}         # what a layer's binding laid out for the batch
         self.captured: list = []      # of those, the ones that graphs read
+        self.now = None               # and each of them
         self._tiles: dict[int, torch.Tensor] = {}
+        self._totals: dict[int, tuple[int, int]] = {}
 
     def tiles(self, group: int) -> torch.Tensor:
         """Runs of at most TILE_ROWS query rows of one sequence, with `group` rows a token: (first
@@ -92,6 +94,15 @@ class PagedBatch:
             flat = np.ascontiguousarray(np.concatenate(runs), dtype=np.int32)
             held = self._tiles[group] = torch.from_numpy(flat).to(self.cache.keys.device)
         return held
+
+
+    def own_total(self, group: int) -> int:
+        """The rows past the shared ones of every tile's sequence, in the step at hand."""
+        held = self._totals.get(group)
+        if held is None or held[0] != self.clock:
+            tiles = -(-self.counts * group // TILE_ROWS)
+            held = self._totals[group] = self.clock, int(((self.now - self.prefix) * tiles).sum())
+        return held[1]
 
 
 class PagedKVCache:
@@ -482,7 +493,7 @@ class PagedKVCache:
         if batch.clock != self._clock:
             rows = self._rows[batch.index] + batch.counts
             self._reserve(batch.index, rows)
-            batch.clock, batch.last = self._clock, int(rows.max())
+            batch.clock, batch.last, batch.now = self._clock, int(rows.max()), rows
         if self._pool is None or not torch.cuda.is_current_stream_capturing():
             return batch.last
         if batch.reach < batch.last:

@@ -31,7 +31,7 @@ class BatchStep(ctypes.Structure):
         + [(name, _I64) for name in (
             "workspace_bytes", "query_stride", "key_stride", "value_stride", "table_stride", "angle_rows",
             "rotary_pairs", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_rows", "sequences", "width",
-            "own_tiles", "prefix", "prefix_sequence", "own_rows", "one_token_each")]
+            "own_tiles", "prefix", "prefix_sequence", "own_rows", "own_total", "one_token_each")]
         + [(name, _F32) for name in ("mscale", "eps", "scale")])
 
 
@@ -131,10 +131,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_attention_batch_project": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F32,
                                              _F32, _I64, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _P, _I64,
                                              _I64, _P, _P, _P]),
-    "omnia_attention_batch_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "omnia_attention_batch_workspace_bytes": (_I64, [_I64] * 8),
     "omnia_attention_batch": (_I32, [_P, _I32, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
-                                     _I64, _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
-    "omnia_attention_batch_step_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+                                     _I64, _I64, _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
+    "omnia_attention_batch_step_bytes": (_I64, [_I64] * 8),
     "omnia_attention_batch_step": (_I32, [_P, _P]),
     "omnia_embed_atlas": (
         _I32,

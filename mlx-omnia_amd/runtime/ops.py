@@ -1407,13 +1407,15 @@ def attention_batch(
     own_rows: int,
     scale: float,
     prefix_sequence: int = 0,
+    own_total: int = 0,
     sinks: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attention of a batch's new tokens, queries [N, heads, D] bf16 or fp32, over a layer's pages; see
     `omnia_attention_batch`: the first `prefix` rows are the same pages for every sequence
     (read through prefix_sequence's), own_rows bounds the rows past them of any of its sequences
-    (rows past the bound are not attended), tiles [n, 4] are runs of one sequence's query rows, as
+    (rows past the bound are not attended), own_total is their sum over the tiles' sequences or 0 for
+    not known (it says how the work is cut), tiles [n, 4] are runs of one sequence's query rows, as
     token_map has them; sinks [heads] bf16 or None -> [N, heads, D] bf16."""
     pages, kv_heads, page_rows, head_dim = _layer_pool(keys, values, "attention_batch")
     _dense(queries, F32 if queries.dtype == F32 else BF16, "queries")
@@ -1430,13 +1432,13 @@ def attention_batch(
         tensors.append(sinks)
     _require(on_rocm(*tensors), "attention_batch: tensors must share one ROCm device")
     nbytes = library().omnia_attention_batch_workspace_bytes(tokens, heads, kv_heads, head_dim, prefix, own_rows,
-                                                             tiles.shape[0])
+                                                             own_total, tiles.shape[0])
     _require(nbytes >= 0, "attention_batch: geometry not served")
     workspace = torch.empty(nbytes // 4, dtype=F32, device=queries.device) if nbytes else None
     out = _out(out, queries, (tokens, heads, head_dim), BF16, "out")
     call("omnia_attention_batch", queries.data_ptr(), int(queries.dtype == F32), keys.data_ptr(), values.data_ptr(), pages, page_rows,
          tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), tokens, tiles.data_ptr(),
-         tiles.shape[0], prefix, prefix_sequence, own_rows, heads, kv_heads, head_dim,
+         tiles.shape[0], prefix, prefix_sequence, own_rows, own_total, heads, kv_heads, head_dim,
          sinks.data_ptr() if sinks is not None else None, float(scale),
          workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
     return out
@@ -1445,7 +1447,7 @@ def attention_batch(
 class BatchStepPlan:
     """A layer's step of one batch, its arguments checked and laid out once for
     `omnia_attention_batch_step`: what stays the same from step to step. Calling it with the raw
-    rows and `own_rows` gives the context [N, heads, D] bf16, `project` the queries alone. The
+    rows, `own_rows` and `own_total` gives the context [N, heads, D] bf16, `project` the queries alone. The
     arguments are those of `attention_batch_project` and `attention_batch`; one_token_each says
     that no sequence has more than one new token."""
 
@@ -1493,7 +1495,7 @@ class BatchStepPlan:
             width=width, own_tiles=tiles.shape[0], prefix=prefix,
             prefix_sequence=prefix_sequence, own_rows=-1, one_token_each=int(one_token_each), mscale=mscale, eps=eps,
             scale=scale)
-        self.sized = -1, 0   # own rows, and the workspace that they need
+        self.sized = None, 0   # own rows and their total, and the workspace that they need
         # What results are made like, without a call's parsing of their kind and place.
         self.keys, self.like = keys, keys.view(-1)[:1].expand(tokens, heads, head_dim)
 
@@ -1533,16 +1535,17 @@ class BatchStepPlan:
         del held
         return out
 
-    def __call__(self, raw_queries, raw_keys, raw_values, own_rows: int) -> torch.Tensor:
+    def __call__(self, raw_queries, raw_keys, raw_values, own_rows: int, own_total: int = 0) -> torch.Tensor:
         args = BatchStep.from_buffer_copy(self.args)
         held = self._raw(args, raw_queries, raw_keys, raw_values)
         sized, nbytes = self.sized
-        if sized != own_rows:
+        if sized != (own_rows, own_total):
             nbytes = library().omnia_attention_batch_step_bytes(self.tokens, self.heads, self.kv_heads, self.head_dim,
-                                                                args.prefix, own_rows, args.own_tiles)
+                                                                args.prefix, own_rows, own_total, args.own_tiles)
             _require(nbytes >= 0, "attention_batch_step: geometry not served")
-            self.sized = own_rows, nbytes
+            self.sized = (own_rows, own_total), nbytes
         workspace, out = self.keys.new_empty(nbytes // 2), self._context()   # of bf16
+        args.own_total = own_total
         args.own_rows, args.workspace_bytes, args.workspace, args.out = (own_rows, nbytes, workspace.data_ptr(),
                                                                           out.data_ptr())
         call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))

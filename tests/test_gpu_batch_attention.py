@@ -826,3 +826,17 @@ def test_answers_sampled_from_one_prompt():
     want, size = attend(wide(queries), wide(cache.keys[1]), wide(cache.values[1]), cache.tables.cpu().numpy(),
                         cache.lengths.cpu().numpy(), batches[0].token_map.cpu().numpy(), d ** -0.5)
     assert np.all(np.abs(wide(got) - want) <= HALF * np.abs(want) + (HALF + 2.0 ** -12) * size)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 5])
+def test_one_long_sequence_among_short_ones(tokens):
+    """Pieces cut for what the sequences hold together, and for the longest alone where that is not known."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, page_rows=64, own=(9000, *(i % 41 for i in range(60))), tokens=tokens)
+    context = case.check(np.arange(0, case.batch.total, 13))
+    queries, group = case.wide_queries(), 4
+    tiles = case.batch.tiles(group)
+    assert case.batch.own_total(group) == sum(int(case.cache.rows(s)) + tokens for s in case.chosen)
+    other = ops.attention_batch(queries, case.cache.keys[1], case.cache.values[1], case.cache.tables, case.cache.lengths,
+                                case.batch.token_map, tiles, prefix=0, own_rows=9000 + tokens, scale=case.scale)
+    case.check_context(other, queries, case.cache.lengths.cpu().numpy(), np.arange(0, case.batch.total, 13))
+    assert (other.float() - context.float()).abs().max() <= 4 * HALF * context.float().abs().max()

@@ -360,10 +360,12 @@ def test_what_the_kernels_serve(heads, kv_heads, head_dim, pairs, served):
 def test_workspace_bytes():
     from mlx_omnia_amd.runtime import library
     nbytes = library().omnia_attention_batch_workspace_bytes
-    assert nbytes(0, 32, 8, 128, 0, 1, 0) == 0
-    assert nbytes(64, 32, 8, 128, 8192, 700, 64) % (64 * 32 * 130 * 4) == 0
-    for bad in ((1, 32, 8, 96, 0, 1, 1), (1, 32, 5, 128, 0, 1, 1), (1, 32, 8, 128, -1, 1, 1),
-                (1, 32, 8, 128, 0, 1 << 30, 1), (1 << 28, 32, 8, 128, 0, 1, 1), (1, 8192, 8, 128, 0, 1, 1)):
+    assert nbytes(0, 32, 8, 128, 0, 1, 0, 0) == 0
+    for total in (0, 1, 64 * 700, 1 << 50):
+        assert nbytes(64, 32, 8, 128, 8192, 700, total, 64) % (64 * 32 * 130 * 4) == 0
+    for bad in ((1, 32, 8, 96, 0, 1, 0, 1), (1, 32, 5, 128, 0, 1, 0, 1), (1, 32, 8, 128, -1, 1, 0, 1),
+                (1, 32, 8, 128, 0, 1 << 30, 0, 1), (1 << 28, 32, 8, 128, 0, 1, 0, 1), (1, 8192, 8, 128, 0, 1, 0, 1),
+                (1, 32, 8, 128, 0, 1, -1, 1)):
         assert nbytes(*bad) < 0
 
 
