@@ -210,6 +210,8 @@ class PagedKVCache:
     def _refuse_capture(self, what: str) -> None:
         if _capturing(self.keys.device):
             raise ValueError(f"PagedKVCache: {what} cannot be captured (a replay would not repeat the host's part)")
+        if self._pool is not None:
+            self._pool.stream()   # raises where another device is current, ahead of any change
 
     def _edit(self, edits: list[int]) -> None:
         """Edits (kind, sequence, a, b), one after the other."""
@@ -518,18 +520,25 @@ class PagedKVCache:
         """The step's tokens are rows of their sequences now: once a step, after every layer.
         Captured, it moves the device's lengths at each replay, and `account` the host's."""
         self._current(batch)
-        if not _capturing(self.keys.device):
-            self.account(batch, 1)
+        counted = not _capturing(self.keys.device)
+        if counted:
+            self._grown(batch, 1)   # raises where the pages do not hold them
         if self._pool is not None:
             ops.pages_advance(self.lengths, batch.chosen, batch.rows)
         else:
             self.lengths[batch.chosen.long()] += batch.rows
+        if counted:
+            self.account(batch, 1)
 
     def account(self, batch: PagedBatch, steps: int) -> None:
         """Count `steps` steps of the batch that the device has taken in replays."""
         self._current(batch)
+        self._rows[batch.index] = self._grown(batch, steps)
+        self._clock += 1
+
+    def _grown(self, batch: PagedBatch, steps: int) -> np.ndarray:
+        """The rows of the batch's sequences `steps` steps on."""
         rows = self._rows[batch.index] + steps * batch.counts
         if steps < 0 or (rows > self._held[batch.index] * self.page_rows).any():
             raise ValueError("PagedKVCache: more steps than the pages hold")
-        self._rows[batch.index] = rows
-        self._clock += 1
+        return rows

@@ -24,6 +24,7 @@ F32 = torch.float32
 
 _ROCM = torch.version.hip is not None
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent without a GPU build
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 # These checks run on every call, ahead of a kernel of a few microseconds: they look at
@@ -58,6 +59,14 @@ def _dense(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
 
 def _stream(t: torch.Tensor) -> int:
     return _raw_stream(t.get_device())
+
+
+def _stream_here(index: int) -> int:
+    """The current stream of device `index`, which has to be the current one: the default stream of
+    another is the same null pointer, and the kernels would run here."""
+    if _current_device() != index:
+        raise ValueError(f"the tensors are on device {index}, but {_current_device()} is current; make theirs current first")
+    return _raw_stream(index)
 
 
 def _out(out: torch.Tensor | None, like: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
@@ -1207,6 +1216,10 @@ class PagePool:
             self.sequences, self.width = _page_tables(tables, lengths, "page pool")
             self.tables, self.lengths = tables.data_ptr(), lengths.data_ptr()
 
+    def stream(self) -> int:
+        """The current stream, of the pool's device, which has to be the current one."""
+        return _stream_here(self.index)
+
     def keep(self, tables: np.ndarray, rows: np.ndarray, held: np.ndarray, refs: np.ndarray, generation: np.ndarray,
              opened: np.ndarray) -> None:
         """The host's arrays of the cache, which `open`, `begin`, `end` and `compact` change with the
@@ -1225,25 +1238,25 @@ class PagePool:
     def begin(self, parent: int, count: int) -> list[int]:
         """`omnia_paged_cache_fork`: the sequences begun."""
         kids = array("i", bytes(8 * count))
-        call("omnia_paged_cache_fork", self.cache_at, parent, count, kids.buffer_info()[0], _raw_stream(self.index))
+        call("omnia_paged_cache_fork", self.cache_at, parent, count, kids.buffer_info()[0], self.stream())
         return kids[0::2].tolist()
 
     def open(self, rows: int) -> int:
         """`omnia_paged_cache_open`: the sequence begun."""
         which = array("i", (0,))
-        call("omnia_paged_cache_open", self.cache_at, rows, which.buffer_info()[0], _raw_stream(self.index))
+        call("omnia_paged_cache_open", self.cache_at, rows, which.buffer_info()[0], self.stream())
         return which[0]
 
     def compact(self) -> int:
         """`omnia_paged_cache_compact`: the pages in use."""
         live = array("q", (0,))
-        call("omnia_paged_cache_compact", self.cache_at, live.buffer_info()[0], _raw_stream(self.index))
+        call("omnia_paged_cache_compact", self.cache_at, live.buffer_info()[0], self.stream())
         return live[0]
 
     def end(self, gone: list[int]) -> None:
         """`omnia_paged_cache_free`."""
         flat = array("i", gone)
-        call("omnia_paged_cache_free", self.cache_at, flat.buffer_info()[0], len(flat), _raw_stream(self.index))
+        call("omnia_paged_cache_free", self.cache_at, flat.buffer_info()[0], len(flat), self.stream())
 
     def copy(self, moves, tables: int | None = None, entries: int = 0) -> None:
         flat, step = _int_lines(moves, 3, "moves"), 3 * PAGES_MOVES
@@ -1253,7 +1266,7 @@ class PagePool:
                 raise ValueError("pages_copy: a page is written twice, or both read and written")
             if tables is not None and (np.diff(source) <= 0).any():
                 raise ValueError("pages_copy: moves that rename have to be sorted by the page they leave")
-        stream, address = _raw_stream(self.index), flat.buffer_info()[0]
+        stream, address = self.stream(), flat.buffer_info()[0]
         for first in range(0, len(flat), step):
             call("omnia_pages_copy", *self.pool, address + 4 * first, min(step, len(flat) - first) // 3, tables,
                  entries, stream)
@@ -1262,13 +1275,13 @@ class PagePool:
         flat, step = _int_lines(kids, 2, "kids"), 2 * PAGES_MOVES
         if len(flat) > step and (len(set(flat[0::2])) < len(flat) // 2 or (rows and len(set(flat[1::2])) < len(flat) // 2)):
             raise ValueError("pages_fork: a child or a page is named twice")
-        stream, address = _raw_stream(self.index), flat.buffer_info()[0]
+        stream, address = self.stream(), flat.buffer_info()[0]
         for first in range(0, len(flat), step):
             call("omnia_pages_fork", *self.pool, self.tables, self.lengths, self.sequences, self.width, parent, full,
                  page, rows, address + 4 * first, min(step, len(flat) - first) // 2, stream)
 
     def edit(self, edits) -> None:
-        _edit(self.tables, self.lengths, self.sequences, self.width, self.pages, edits, _raw_stream(self.index))
+        _edit(self.tables, self.lengths, self.sequences, self.width, self.pages, edits, self.stream())
 
 
 def _edit(tables: int, lengths: int, sequences: int, width: int, pages: int, edits, stream: int) -> None:
@@ -1303,7 +1316,7 @@ def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -
     More than PAGES_EDITS are made in turn, as many at a time."""
     sequences, width = _page_tables(tables, lengths, "pages_edit")
     _require(on_rocm(tables, lengths), "pages_edit: tensors must share one ROCm device")
-    _edit(tables.data_ptr(), lengths.data_ptr(), sequences, width, pages, edits, _stream(tables))
+    _edit(tables.data_ptr(), lengths.data_ptr(), sequences, width, pages, edits, _stream_here(tables.get_device()))
 
 
 def pages_advance(lengths: torch.Tensor, chosen: torch.Tensor, rows: torch.Tensor) -> None:
@@ -1314,7 +1327,7 @@ def pages_advance(lengths: torch.Tensor, chosen: torch.Tensor, rows: torch.Tenso
     _require(chosen.shape == rows.shape, "pages_advance: as many rows as sequences chosen")
     _require(on_rocm(lengths, chosen, rows), "pages_advance: tensors must share one ROCm device")
     call("omnia_pages_advance", lengths.data_ptr(), lengths.numel(), chosen.data_ptr(), rows.data_ptr(),
-         chosen.numel(), _stream(lengths))
+         chosen.numel(), _stream_here(lengths.get_device()))
 
 
 def _layer_pool(keys: torch.Tensor, values: torch.Tensor, name: str) -> tuple[int, int, int, int]:
@@ -1390,7 +1403,7 @@ def attention_batch_project(
          cos.data_ptr() if angles is not None else None, sin.data_ptr() if angles is not None else None,
          table_stride, angle_rows, pairs, float(mscale), float(eps), tokens, heads, kv_heads, head_dim,
          queries.data_ptr(), int(wide_queries), keys.data_ptr(), values.data_ptr(), pages, page_rows,
-         tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), _stream(raw_queries))
+         tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), _stream_here(raw_queries.get_device()))
     return queries
 
 
@@ -1440,7 +1453,7 @@ def attention_batch(
          tables.data_ptr(), sequences, width, lengths.data_ptr(), token_map.data_ptr(), tokens, tiles.data_ptr(),
          tiles.shape[0], prefix, prefix_sequence, own_rows, own_total, heads, kv_heads, head_dim,
          sinks.data_ptr() if sinks is not None else None, float(scale),
-         workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream(queries))
+         workspace.data_ptr() if workspace is not None else None, nbytes, out.data_ptr(), _stream_here(queries.get_device()))
     return out
 
 
@@ -1531,7 +1544,7 @@ class BatchStepPlan:
         held = self._raw(args, raw_queries, raw_keys, raw_values)
         out = self._context()
         args.queries = out.data_ptr()
-        call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
+        call("omnia_attention_batch_step", ctypes.addressof(args), _stream_here(self.index))
         del held
         return out
 
@@ -1548,7 +1561,7 @@ class BatchStepPlan:
         args.own_total = own_total
         args.own_rows, args.workspace_bytes, args.workspace, args.out = (own_rows, nbytes, workspace.data_ptr(),
                                                                           out.data_ptr())
-        call("omnia_attention_batch_step", ctypes.addressof(args), _raw_stream(self.index))
+        call("omnia_attention_batch_step", ctypes.addressof(args), _stream_here(self.index))
         del held
         return out
 

@@ -840,3 +840,24 @@ def test_one_long_sequence_among_short_ones(tokens):
                                 case.batch.token_map, tiles, prefix=0, own_rows=9000 + tokens, scale=case.scale)
     case.check_context(other, queries, case.cache.lengths.cpu().numpy(), np.arange(0, case.batch.total, 13))
     assert (other.float() - context.float()).abs().max() <= 4 * HALF * context.float().abs().max()
+
+
+def test_another_device_than_the_current_one_is_refused(monkeypatch):
+    """Before anything is launched or counted: the tensors' device would not be the one that runs."""
+    case = Case(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=64, own=(3, 4))
+    cache, tables = case.cache, case.cache.tables.clone()
+    want = case.step(case.batch, *case.raw)
+    held, rows = cache.free_pages, cache.rows(case.chosen[0])
+    with monkeypatch.context() as patch:
+        patch.setattr(ops, "_current_device", lambda: 1)
+        for call in (lambda: case.step(case.batch, *case.raw), lambda: case.step.project(case.batch, *case.raw),
+                     lambda: cache.open(20), lambda: cache.fork(case.chosen[0]), lambda: cache.free(case.chosen[0]),
+                     cache.compact, lambda: cache.advance(case.batch), lambda: cache.reserve(case.chosen[0], 99),
+                     lambda: cache.truncate(case.chosen[0], 1), lambda: cache.resize(500),
+                     lambda: cache.fork(case.chosen[0], share=False), lambda: ops.pages_advance(cache.lengths, case.batch.chosen, case.batch.rows),
+                     case.wide_queries, lambda: ops.pages_copy(cache.keys, cache.values, [(0, 1, 1)]),
+                     lambda: ops.pages_edit(cache.tables, cache.lengths, cache.pages, [(0, 0, 0, 1)])):
+            with pytest.raises(ValueError, match="is current"):
+                call()
+    assert cache.free_pages == held and cache.rows(case.chosen[0]) == rows and torch.equal(cache.tables, tables)
+    assert torch.equal(case.step(case.batch, *case.raw), want)
