@@ -1390,9 +1390,18 @@ struct Plan {
 constexpr int64_t kSlots = 512, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
 constexpr int64_t kOwnKeys = 256, kOwnPieces = 2048;
 
-// `splits` pieces of whole tiles of 64 keys, or as many as those leave, and the keys of one.
-int64_t cut(int64_t keys, int64_t splits, int64_t& each) {
-  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+// Most pieces of a row: the merge takes them one after another, but a few kv heads of a few
+// sequences have to fill the card (two of one sequence of 400,000 rows: 64 pieces each 251 us, 512 86).
+int64_t most_splits(int64_t blocks) {
+  const int64_t fill = 2 * kSlots / (blocks < 1 ? 1 : blocks);
+  return fill > kMaxSplits ? fill : kMaxSplits;
+}
+
+// `splits` pieces of whole tiles of 64 keys for each of `blocks` workgroups, or as many as those
+// leave, and the keys of one.
+int64_t cut(int64_t blocks, int64_t keys, int64_t splits, int64_t& each) {
+  const int64_t most = most_splits(blocks);
+  splits = splits < 1 ? 1 : splits > most ? most : splits;
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int64_t of_one = (tiles + splits - 1) / splits;
   each = of_one * kTileKeys;
@@ -1439,7 +1448,7 @@ int64_t wide_splits(int64_t blocks, int64_t keys, double filled, const WideCost&
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   int64_t best = 1;
   double least = 0.0;
-  for (int64_t splits = 1; splits <= kMaxSplits && splits <= tiles; ++splits) {
+  for (int64_t splits = 1; splits <= most_splits(blocks) && splits <= tiles; ++splits) {
     const int64_t of_one = (tiles + splits - 1) / splits;
     if ((tiles + of_one - 1) / of_one != splits) continue;   // as another one
     // Of pieces that are not all there, as many whole ones as they amount to.
@@ -1458,7 +1467,7 @@ int64_t wide_splits(int64_t blocks, int64_t keys, double filled, const WideCost&
       best = splits;
     }
   }
-  return cut(keys, best, each);
+  return cut(blocks, keys, best, each);
 }
 
 // Narrow pieces of `keys` keys, of which the part `filled` is there, for each of `blocks`
@@ -1473,7 +1482,7 @@ int64_t narrow_splits(int64_t blocks, int64_t keys, double filled, int64_t taken
   // us in two pieces each, 42.5 in one).
   const int64_t splits = fill(kNarrowBlocks, kNarrowKeys);
   const int64_t slots = taken >= kSlots ? kSlots : taken > kSlots / 2 ? kSlots / 2 : kSlots - taken;
-  return cut(keys, blocks * splits < slots ? fill(slots, kNarrowKeys / 4) : splits, each);
+  return cut(blocks, keys, blocks * splits < slots ? fill(slots, kNarrowKeys / 4) : splits, each);
 }
 
 // `own_total`: the own rows of every tile's sequence together, or 0 where they are not known and
@@ -1532,7 +1541,7 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
     const int64_t even = filled < 0.5 ? static_cast<int64_t>(own_blocks * 2.0 * filled) + 1 : own_blocks;
     const int64_t fill = (kOwnPieces + even - 1) / even;
     const int64_t most = own_rows / kOwnKeys, least = own_rows / (4 * kOwnKeys);
-    p.own_splits = cut(own_rows, fill > most ? most : fill < least ? least : fill, p.own_keys);
+    p.own_splits = cut(own_blocks, own_rows, fill > most ? most : fill < least ? least : fill, p.own_keys);
   } else if (narrow) {
     p.own_splits = narrow_splits(own_blocks, own_rows, filled, kv_heads * p.prefix_tiles * p.prefix_splits, p.own_keys);
   } else {
