@@ -765,8 +765,8 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  *   token t = (s, j) = token_map[t] sees rows r <= lengths[s] + j of sequence s,
  *   out[t, h] = sum_r exp(x - M) v[r] / (exp(sink[h] - M) + sum_r exp(x - M)),
  *   x = scale * (q[t, h] . k[r, h / gqa])
- * in fp32, the weights rounded to bf16 for their product with the values, the result once to
- * bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
+ * in fp32, queries of 32 bits and the weights held to 16 for their products with the keys and
+ * the values, the result rounded once to bf16; no sink term with null sinks; a token that sees nothing comes as zeros. Rows [0,
  * prefix) must be the same pages in every token's sequence: they are read through
  * prefix_sequence's. own_rows bounds the rows past them of every sequence, this step's included;
  * own_total is the sum of those rows over the tiles, each its sequence's, or 0: how the work is cut

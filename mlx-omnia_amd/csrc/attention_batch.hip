@@ -198,15 +198,33 @@ constexpr int kWaveRows = 32, kWaves = 4, kTileRows = kWaveRows * kWaves, kTileK
 // V^T comes out of LDS by the transposing read.
 //
 // Queries of 32 bits go into the product as two bf16 parts, 16 of their 24 bits (queries of bf16
-// are one). The weights are rounded to bf16, half a step of 2^-8 each; their sum is taken before
-// that, in fp32. So the results' error is 0.0024 of their size, where rounding them alone makes
-// 0.0017; with the queries rounded as well it was 0.0028. Both parts of the weights instead of
-// the queries' give the same, and cost four vector operations a score more.
+// are one), and so do the weights (split_weights_two): a weight is off by at most 2^-15 of
+// itself, 1/128 of the half step that the result is rounded by. Their sum is taken before that,
+// in fp32. The results' error is 0.0017 of their size, that of rounding them alone. One part of
+// the weights made 0.0023 of it and, replayed, 150 us for 175 behind a document of 32,768 rows
+// (128 tokens), 203 for 254 over prompts (1,828 tokens behind 4,096 rows), within 3 us where
+// memory or launches bound.
 //
 // The maximum that the weights are taken under is raised only where a score passes it by more
 // than 2^8: the sums have the room, and the rescaling of a row's context, which a growing
 // maximum would ask for in nearly every tile, is rare.
 constexpr float kSlack = 8.0f;
+
+// Eight softmax weights (each zero, or a positive normal number) as two bf16 operands: the top
+// half of the number cut off, less than 2^-7 of it left, and that rounded by at most 2^-8 of
+// itself. Neither part is negative, and of a positive weight neither is zero: times an infinite
+// value both give that infinity, as the weight itself would.
+__device__ __forceinline__ void split_weights_two(const float (&p)[8], u32x4 (&parts)[2]) {
+  float rest[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x0 = __float_as_uint(p[2 * j]), x1 = __float_as_uint(p[2 * j + 1]);
+    parts[0][j] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+    rest[2 * j] = __builtin_amdgcn_fmed3f(p[2 * j] - __uint_as_float(x0 & 0xffff0000u), p[2 * j], 0x1p-126f);
+    rest[2 * j + 1] = __builtin_amdgcn_fmed3f(p[2 * j + 1] - __uint_as_float(x1 & 0xffff0000u), p[2 * j + 1], 0x1p-126f);
+  }
+  parts[1] = pack8(rest);
+}
 
 // What the scheduler is told to group (sched_group_barrier's masks).
 constexpr int kValu = 0x2, kMfma = 0x8, kVmemRead = 0x20, kDsRead = 0x100;
@@ -465,7 +483,6 @@ struct WideRows {
     }
     const float base = top == -INFINITY ? 0.0f : top;
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4 weights[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) {   // 16 keys each
       float p[8];
@@ -474,29 +491,34 @@ struct WideRows {
         p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][(step % 2) * 8 + j], scale_log2, -base));
         sums[j % 4] += p[j];
       }
-      weights[step] = pack8(p);
+      u32x4 weights[2];
+      split_weights_two(p, weights);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[b]),
-                                                         __builtin_bit_cast(bf16x8, weights[step]), out[b], 0, 0, 0);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          out[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[b]),
+                                                           __builtin_bit_cast(bf16x8, weights[part]), out[b], 0, 0, 0);
+        }
         if (step < 3) {
           const uint16_t* at = tile_v + (step + 1) * 16 * D + value_at[b];
           v[b] = read_transposed(at, at + 8 * D);
         }
       }
     }
-    // A step's products beside the next one's weights (28 vector operations) and values.
-    __builtin_amdgcn_sched_group_barrier(kValu, 28, 0);
+    // A step's products beside the next one's weights (52 vector operations) and values; of the
+    // first step's 44 ahead of any product (with all 52 two registers spilled).
+    __builtin_amdgcn_sched_group_barrier(kValu, 44, 0);
 #pragma unroll
     for (int step = 0; step < 3; ++step) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
         __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(kValu, 28 / kBlocks, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 52 / kBlocks, 0);
       }
     }
-    __builtin_amdgcn_sched_group_barrier(kMfma, kBlocks, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, 2 * kBlocks, 0);
     total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
 
@@ -617,12 +639,17 @@ struct NarrowRows {
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], scale_log2, -base));
     total += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    const u32x4 weights = pack8(p);
+    u32x4 weights[2];
+    split_weights_two(p, weights);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const uint16_t* at = tile_v + (value_at ^ (b * 16));
-      out[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, read_transposed(at, at + 16 * D)),
-                                                       __builtin_bit_cast(bf16x8, weights), out[b], 0, 0, 0);
+      const s16x8 v = read_transposed(at, at + 16 * D);
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        out[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v),
+                                                         __builtin_bit_cast(bf16x8, weights[part]), out[b], 0, 0, 0);
+      }
     }
   }
 

@@ -197,6 +197,54 @@ def test_plans(case):
     made.check(None if made.batch.total * made.heads < 2000 else np.arange(0, made.batch.total, 7))
 
 
+# Every way that a row's weights go into their product: a wave's own rows with and without the
+# prologue's launch, shared rows for many tokens and for few, own rows alone, prompts.
+WEIGHTS = [
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, prefix=64, own=(0, 1, 5, 20)),
+    dict(heads=16, kv_heads=2, head_dim=64, pairs=8, own=(0, 1, 2, 3, 40)),
+    dict(heads=16, kv_heads=4, head_dim=128, prefix=1024, own=tuple((i * 29) % 130 for i in range(40))),
+    dict(heads=8, kv_heads=8, head_dim=64, prefix=640, own=tuple(range(0, 61)) + (9,) * 30, sinks=True),
+    dict(heads=24, kv_heads=8, head_dim=128, pairs=32, norms=True, page_rows=64, own=(0, 1, 2, 3) + (2751,) * 20),
+    dict(heads=24, kv_heads=8, head_dim=64, page_rows=64, own=(0, 1, 2, 3) + (2751,) * 20, tokens=(2, 1, 1, 1) + (1,) * 20),
+    dict(heads=8, kv_heads=2, head_dim=128, pairs=64, norms=True, own=(0,), tokens=200),
+    dict(heads=8, kv_heads=2, head_dim=64, sinks=True, page_rows=32, own=(0, 7, 33), tokens=(40, 1, 129)),
+]
+
+
+@pytest.mark.parametrize("case", WEIGHTS, ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", "")[:60])
+def test_weights_are_held_in_sixteen_bits(case):
+    """What remains beside the result's own rounding, in parts of the mean of |v|:
+    - a weight is cut to 8 bits, which leaves less than 2^-7 of it, and the rest rounded by at
+      most 2^-8 of itself: 2^-15;
+    - fp32 queries are rounded to 8 bits, what that leaves (2^-8 at most) to 8 more: 2^-16 of
+      each, and a score's 128 products are summed in fp32 (128 halves of 2^-23, 2^-17): with
+      |q . k| of the absolutes at most ||q|| ||k||, a score is off by (2^-16 + 2^-17) of that times
+      the scale, the weight by as much of itself, and so is the sum that it is divided by;
+    - n rows summed in fp32: n 2^-24 in the context and in the sum of the weights;
+    - exp2, the merges and the products of fp32 around them, of 2^-22 or less each: 2^-18."""
+    made = Case(**case, scale=0.02)
+    lengths = made.cache.lengths.cpu().numpy()
+    context, queries = made.step(made.batch, *made.raw), made.wide_queries()
+    token_map, sinks = made.batch.token_map.cpu().numpy(), None if made.sinks is None else wide(made.sinks)
+    keys, values = wide(made.cache.keys[made.layer]), wide(made.cache.values[made.layer])
+    tables = made.cache.tables.cpu().numpy()
+    seen = lengths[token_map[:, 0]] + token_map[:, 1] + 1
+    pick = np.flatnonzero((seen <= 200) | (np.arange(len(seen)) % 5 == 0))
+    longest = np.sqrt(np.nanmax((keys.astype(np.float64) ** 2).sum(axis=-1)))
+    rounded = queries.bfloat16()
+    alone = ops.attention_batch(rounded, made.cache.keys[made.layer], made.cache.values[made.layer], made.cache.tables,
+                                made.cache.lengths, made.batch.token_map, made.batch.tiles(made.heads // made.kv_heads),
+                                prefix=made.batch.prefix, prefix_sequence=made.chosen[0],
+                                own_rows=int(seen.max()) - made.batch.prefix, scale=made.scale, sinks=made.sinks)
+    for got, q, query_bits in ((context, queries, 2.0 ** -16), (alone, rounded, 0.0)):
+        want, size = attend(wide(q)[pick], keys, values, tables, lengths, token_map[pick], made.scale, sinks)
+        score = np.linalg.norm(wide(q)[pick], axis=-1, keepdims=True) * longest * made.scale
+        bound = (2.0 ** -15 + 2 * (query_bits + 2.0 ** -17) * score
+                 + 2 * seen[pick][:, None, None] * 2.0 ** -24 + 2.0 ** -18)
+        bad = np.abs(wide(got)[pick] - want) > HALF * np.abs(want) + bound * size
+        assert not bad.any(), (int(bad.sum()), bad.size, np.argwhere(bad)[:4].tolist())
+
+
 @pytest.mark.parametrize("case", [c for c in PLANS + GEOMETRIES if c.get("tokens", 1) == 1],
                          ids=lambda c: "-".join(f"{v}" for v in c.values()).replace(" ", ""))
 def test_a_step_writes_its_rows_and_no_others(case):
