@@ -207,8 +207,10 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         """The batch's plan of this layer, and the most rows a sequence has in the step."""
         core, cache = self.core, self.core.cache
         last = cache.ready(batch)
-        plan, pool = batch.plans.get(self, (None, None))
-        if plan is None or pool is not cache.keys or (core.rotary_pairs and last > plan.angle_rows):
+        plan, laid = batch.plans.get(self, (None, None))
+        # A tensor keeps its identity where a module is moved, or a parameter sharded: its address is asked.
+        lies = [t.data_ptr() for t in (cache.keys, cache.values, cache.tables, cache.lengths, *self.held)]
+        if plan is None or laid != lies or (core.rotary_pairs and last > plan.angle_rows):
             angles = None
             if core.rotary_pairs:
                 table = core.angles
@@ -225,7 +227,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
                 cache.tables, cache.lengths, batch.token_map, batch.tiles(core.heads // core.kv_heads),
                 heads=core.heads, prefix=batch.prefix, prefix_sequence=batch.sequences[0], scale=core.scale,
                 eps=core.eps, mscale=core.mscale, sinks=core.sinks, one_token_each=batch.total == len(batch.sequences))
-            batch.plans[self] = plan, cache.keys
+            batch.plans[self] = plan, lies
         if batch.reach and _capturing(cache.keys.device) and all(plan is not held for held in batch.captured):
             batch.captured.append(plan)   # and with it the angles, should the atlas grow
         return plan, last

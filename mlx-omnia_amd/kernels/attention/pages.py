@@ -152,10 +152,22 @@ class PagedKVCache:
 
     def _bind(self) -> None:
         """The library's view of the pool, the tables and the host's arrays: on a HIP device."""
-        self._pool = None
+        pool = None
         if hip_device(self.keys):
-            self._pool = ops.PagePool(self.keys, self.values, self.tables, self.lengths)
-            self._pool.keep(self._tables, self._rows, self._held, self._refs, self._generation, self._open)
+            pool = ops.PagePool(self.keys, self.values, self.tables, self.lengths)
+            pool.keep(self._tables, self._rows, self._held, self._refs, self._generation, self._open)
+        self._pool, self._kind = pool, (self.keys.shape, self.keys.dtype)
+
+    def _library(self) -> None:
+        """The same again where a tensor lies elsewhere by now: its identity does not say so
+        (`.data`, as a module that is moved sets it)."""
+        if self._kind != (self.keys.shape, self.keys.dtype):
+            raise ValueError("PagedKVCache: the pool is of another shape or kind than it was (resize changes it)")
+        tensors = self.keys, self.values, self.tables, self.lengths
+        if self._pool.addresses != [t.data_ptr() for t in tensors]:
+            if not hip_device(*tensors):
+                raise ValueError("PagedKVCache: the pool and its tables have left their device")
+            self._bind()
 
     def _check_tables(self) -> None:
         tables, width = self._tables, self._tables.shape[1] if self._tables.ndim == 2 else 0
@@ -211,6 +223,7 @@ class PagedKVCache:
         if _capturing(self.keys.device):
             raise ValueError(f"PagedKVCache: {what} cannot be captured (a replay would not repeat the host's part)")
         if self._pool is not None:
+            self._library()
             self._pool.stream()   # raises where another device is current, ahead of any change
 
     def _edit(self, edits: list[int]) -> None:

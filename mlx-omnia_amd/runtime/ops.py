@@ -1210,6 +1210,8 @@ class PagePool:
         _require(width % 16 == 0, "page pool: rows must be whole 16-byte vectors")
         self.held = [t for t in (keys, values, tables, lengths) if t is not None]
         _require(on_rocm(*self.held), "page pool: tensors must share one ROCm device")
+        self.addresses = [t.data_ptr() for t in self.held]
+        _require(all(self.addresses), "page pool: a tensor without memory")
         self.pool = keys.data_ptr(), values.data_ptr(), *keys.shape[:4], width // 2
         self.index, self.pages = keys.get_device(), keys.shape[1]
         if tables is not None and lengths is not None:
@@ -1462,7 +1464,8 @@ class BatchStepPlan:
     `omnia_attention_batch_step`: what stays the same from step to step. Calling it with the raw
     rows, `own_rows` and `own_total` gives the context [N, heads, D] bf16, `project` the queries alone. The
     arguments are those of `attention_batch_project` and `attention_batch`; one_token_each says
-    that no sequence has more than one new token."""
+    that no sequence has more than one new token. Its addresses are those of when it was made: a
+    caller asks whether the tensors still lie there."""
 
     def __init__(self, query_weight, key_weight, angles, keys, values, tables, lengths, token_map, tiles, *, heads: int,
                  prefix: int, prefix_sequence: int, scale: float, eps: float, mscale: float = 1.0, sinks=None,
@@ -1493,8 +1496,10 @@ class BatchStepPlan:
                     raise ValueError(f"{name}: fp32 [positions, pairs], 16-byte aligned with unit inner stride")
             held += [cos, sin]
         _require(on_rocm(*held), "attention_batch_step: tensors must share one ROCm device")
+        _require(all(t.data_ptr() for t in held), "attention_batch_step: a tensor without memory")
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        self.held, self.index = held, keys.get_device()
+        # The memory itself: a tensor that is given other memory must not let go of what is read here.
+        self.held, self.index = [t.detach() for t in held], keys.get_device()
         self.device = keys.device
         self.angle_rows = cos.shape[0] if cos is not None else None
         self.tokens, self.heads, self.kv_heads, self.head_dim = tokens, heads, kv_heads, head_dim

@@ -541,6 +541,29 @@ def test_a_graph_keeps_the_angles_it_was_captured_with():
         assert torch.equal(step(case.batch, *case.raw), want)
 
 
+def test_tensors_that_were_given_other_memory():
+    """Gains, sinks, angles and the pool of a batch that steps on, moved as a module moves its
+    parameters, with other numbers where they were."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, norms=True, sinks=True, prefix=64, own=(3, 40, 9))
+    want = case.step(case.batch, *case.raw)
+    held = []
+    for t in (case.qw, case.kw, case.sinks, case.cos, case.sin, case.cache.keys, case.cache.values, case.cache.tables,
+              case.cache.lengths):
+        held.append(t.data)
+        t.data = t.data.clone()
+        if t.is_floating_point():
+            held[-1].fill_(7.0)
+        assert torch.equal(case.step(case.batch, *case.raw), want)
+    table = case.cache.tables.clone()
+    kids = case.cache.fork(case.chosen[1], 2)
+    assert torch.equal(case.cache.tables[kids[0], :4], table[case.chosen[1], :4])
+    assert (held[-2] == table).all()   # the ones that were left
+    assert torch.equal(case.step(case.batch, *case.raw), want)
+    case.qw.data = case.qw.data.float()
+    with pytest.raises(ValueError, match="query_weight"):
+        case.step(case.batch, *case.raw)
+
+
 def test_gains_and_sinks_that_autograd_follows():
     case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, norms=True, sinks=True, prefix=16, own=(3, 4))
     want = case.step(case.batch, *case.raw)

@@ -561,3 +561,121 @@ def test_tables_in_another_order():
     assert cache._tables.flags.c_contiguous and cache.rows(0) == 20 and cache.pages_of(0) == [0, 1]
     with pytest.raises(ValueError, match="asked for"):
         cache.fork(0, 1 << 60)
+
+
+# Where the kernels read ------------------------------------------------------------------------
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """A device's path on CPU tensors: what the library would be called with, and nothing run."""
+    import types
+
+    from mlx_omnia_amd.kernels.attention import batch, pages
+    from mlx_omnia_amd.runtime.loader import BatchStep, PagedCache
+
+    seen = []
+
+    def call(name, *args):
+        kind = {"omnia_attention_batch_step": BatchStep, "omnia_paged_cache_fork": PagedCache,
+                "omnia_paged_cache_open": PagedCache, "omnia_paged_cache_free": PagedCache,
+                "omnia_paged_cache_compact": PagedCache}.get(name)
+        seen.append((name, kind.from_buffer_copy(kind.from_address(args[0])) if kind else args))
+
+    for module in (batch, pages):
+        monkeypatch.setattr(module, "hip_device", lambda *tensors: True)
+    monkeypatch.setattr(ops, "on_rocm", lambda *tensors: True)
+    monkeypatch.setattr(ops, "_stream_here", lambda index: 0)
+    monkeypatch.setattr(ops, "library", lambda: types.SimpleNamespace(omnia_attention_batch_step_bytes=lambda *a: 256))
+    monkeypatch.setattr(ops, "call", call)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return seen
+
+
+def _taken_up(layers=2):
+    shape = (layers, 8, 2, 16, 64)
+    return PagedKVCache(torch.zeros(shape, dtype=torch.bfloat16), torch.zeros(shape, dtype=torch.bfloat16),
+                        tables=np.array([[0, 1, -1], [0, 2, -1], [-1, -1, -1]]), lengths=np.array([20, 21, 0]), opened=[0, 1])
+
+
+def _declared(cache):
+    gen = torch.Generator().manual_seed(1)
+    made = lambda *shape, dtype=torch.bfloat16: torch.randn(shape, generator=gen).to(dtype)  # noqa: E731
+    parts = dict(query_weight=made(64), key_weight=made(64), sinks=made(8), cos_rows=made(48, 32, dtype=torch.float32),
+                 sin_rows=made(48, 32, dtype=torch.float32))
+    step = BatchAttentionStep(cache, layer=1, heads=8, kv_heads=2, head_dim=64, scale=0.1, dtype=torch.bfloat16,
+                              query_weight=parts["query_weight"], key_weight=parts["key_weight"], rotary_pairs=32,
+                              angles=AngleTable(parts["cos_rows"], parts["sin_rows"]), sinks=parts["sinks"])
+    parts |= dict(keys=cache.keys, values=cache.values, tables=cache.tables, lengths=cache.lengths)
+    return step, parts, [made(2, n * 64) for n in (8, 2, 2)]
+
+
+@pytest.mark.parametrize("name", ["query_weight", "key_weight", "sinks", "cos_rows", "sin_rows", "keys", "values", "tables",
+                                  "lengths"])
+def test_a_step_reads_its_tensors_where_they_lie_by_now(launches, name):
+    """A module that is moved, or its parameters sharded, gives the same tensors other memory."""
+    cache = _taken_up()
+    step, parts, raw = _declared(cache)
+    batch = cache.batch([0, 1])
+    for call in (step, step.project):
+        for _ in range(2):
+            call(batch, *raw)
+            parts[name].data = parts[name].data.clone()
+            call(batch, *raw)
+            got, layer = launches[-1][1], cache.keys[0].numel() * 2
+            for field, t in parts.items():
+                assert getattr(got, field) == t.data_ptr() + (layer if field in ("keys", "values") else 0), field
+
+
+def test_a_steps_tensors_are_checked_where_they_lie_by_now(launches):
+    cache = _taken_up()
+    step, parts, raw = _declared(cache)
+    batch = cache.batch([0, 1])
+    for name in ("query_weight", "key_weight", "sinks", "cos_rows"):
+        held = parts[name].data
+        others = [held.double(), held[..., :4].clone()]
+        if name.endswith("weight"):
+            others.append(held.repeat(2)[1:65])   # off the 16 bytes that are read at a time
+        for other in others:
+            step(batch, *raw)
+            count = len(launches)
+            parts[name].data = other
+            with pytest.raises(ValueError):
+                step(batch, *raw)
+            assert len(launches) == count
+            parts[name].data = held
+    parts["query_weight"].data = torch.empty(0, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        step(batch, *raw)
+    emptied = parts["key_weight"]
+    parts["query_weight"].data = emptied.data.clone()
+    step(batch, *raw)
+    emptied.untyped_storage().resize_(0)   # as a sharded parameter's between its uses: no address
+    with pytest.raises(ValueError):
+        step(batch, *raw)
+
+
+def test_a_caches_calls_name_its_pool_where_it_lies_by_now(launches):
+    cache = _taken_up()
+    calls = [lambda: cache.fork(0), lambda: cache.open(3), lambda: cache.free(1), cache.compact]
+    for name in ("keys", "values", "tables", "lengths"):
+        held = getattr(cache, name)
+        held.data = held.data.clone()
+        for call in calls if name == "tables" else calls[:2]:
+            call()
+            got = launches[-1][1]
+            assert all(getattr(got, n) == getattr(cache, n).data_ptr() for n in ("keys", "values", "tables", "lengths"))
+    cache.values = cache.values.clone()
+    cache.fork(0)
+    assert launches[-1][1].values == cache.values.data_ptr()
+    cache.reserve(0, 40)   # pages in the torch order of things, edited by the library
+    assert launches[-1][0] == "omnia_pages_edit" and launches[-1][1][0] == cache.tables.data_ptr()
+    held, count = cache.keys.data, len(launches)
+    for other in (held.view(torch.float16), held[:1].clone(), held[:, :4].clone()):
+        cache.keys.data = other
+        for call in calls:
+            with pytest.raises(ValueError):
+                call()
+    assert len(launches) == count
+    cache.keys.data = held
+    cache.fork(0)
