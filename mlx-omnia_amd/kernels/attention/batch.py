@@ -176,7 +176,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
             return None
         if sinks is not None and (sinks.dtype != dtype or sinks.numel() != heads):
             return None
-        held = [cache.keys, *weights] + ([sinks.contiguous()] if sinks is not None else [])
+        held = [cache.keys, *weights] + ([sinks] if sinks is not None else [])
         if rotary_pairs:
             if not isinstance(angles, (AngleTable, AngleAtlas)) or angles.pairs != rotary_pairs:
                 return None
@@ -191,7 +191,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
         return cls(DefaultBatchAttentionStep.build(
             cache, layer=layer, heads=heads, kv_heads=kv_heads, head_dim=head_dim, scale=scale, dtype=dtype,
             query_weight=query_weight, key_weight=key_weight, eps=eps, rotary_pairs=rotary_pairs, mscale=mscale,
-            angles=angles, sinks=sinks.contiguous() if sinks is not None else None),
+            angles=angles, sinks=sinks),
             (*weights, *(() if sinks is None else (sinks,)),
              *((angles.cos, angles.sin) if rotary_pairs and isinstance(angles, AngleTable) else ())))
 

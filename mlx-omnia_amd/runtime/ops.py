@@ -1463,9 +1463,9 @@ class BatchStepPlan:
     """A layer's step of one batch, its arguments checked and laid out once for
     `omnia_attention_batch_step`: what stays the same from step to step. Calling it with the raw
     rows, `own_rows` and `own_total` gives the context [N, heads, D] bf16, `project` the queries alone. The
-    arguments are those of `attention_batch_project` and `attention_batch`; one_token_each says
-    that no sequence has more than one new token. Its addresses are those of when it was made: a
-    caller asks whether the tensors still lie there."""
+    arguments are those of `attention_batch_project` and `attention_batch` (the sinks may lie
+    apart); one_token_each says that no sequence has more than one new token. Its addresses are
+    those of when it was made: a caller asks whether the tensors still lie there."""
 
     def __init__(self, query_weight, key_weight, angles, keys, values, tables, lengths, token_map, tiles, *, heads: int,
                  prefix: int, prefix_sequence: int, scale: float, eps: float, mscale: float = 1.0, sinks=None,
@@ -1484,9 +1484,10 @@ class BatchStepPlan:
                     raise ValueError(f"{name}: must be [head_dim]")
                 held.append(weight)
         if sinks is not None:
-            _require(sinks.dtype == BF16 and sinks.is_contiguous() and sinks.numel() == heads,
-                     "attention_batch_step: sinks must be contiguous bf16 [heads]")
+            _require(sinks.dtype == BF16 and sinks.numel() == heads, "attention_batch_step: sinks must be bf16 [heads]")
             held.append(sinks)
+        # Copied for every call where they do not lie together: they may be others by then.
+        self.strided = None if sinks is None or sinks.is_contiguous() else sinks
         cos = sin = None
         if angles is not None:
             cos, sin = angles
@@ -1564,6 +1565,9 @@ class BatchStepPlan:
             self.sized = (own_rows, own_total), nbytes
         workspace, out = self.keys.new_empty(nbytes // 2), self._context()   # of bf16
         args.own_total = own_total
+        if self.strided is not None:
+            sinks = self.strided.contiguous()
+            args.sinks = sinks.data_ptr()
         args.own_rows, args.workspace_bytes, args.workspace, args.out = (own_rows, nbytes, workspace.data_ptr(),
                                                                           out.data_ptr())
         call("omnia_attention_batch_step", ctypes.addressof(args), _stream_here(self.index))

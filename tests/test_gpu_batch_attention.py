@@ -543,9 +543,15 @@ def test_a_graph_keeps_the_angles_it_was_captured_with():
 
 def test_tensors_that_were_given_other_memory():
     """Gains, sinks, angles and the pool of a batch that steps on, moved as a module moves its
-    parameters, with other numbers where they were."""
+    parameters, with other numbers where they were; and sinks that do not lie together."""
     case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, norms=True, sinks=True, prefix=64, own=(3, 40, 9))
-    want = case.step(case.batch, *case.raw)
+    apart = torch.stack([case.sinks, case.sinks + 1], dim=1)
+    loose = BatchAttentionStep(case.cache, layer=case.layer, heads=8, kv_heads=2, head_dim=64, scale=case.scale,
+                               dtype=torch.bfloat16, query_weight=case.qw, key_weight=case.kw, rotary_pairs=32,
+                               angles=AngleTable(case.cos, case.sin), sinks=apart[:, 0])
+    assert isinstance(loose.strategy, HipBatchAttentionStep)
+    want, other = case.step(case.batch, *case.raw), loose(case.batch, *case.raw)
+    assert torch.equal(other, want)
     held = []
     for t in (case.qw, case.kw, case.sinks, case.cos, case.sin, case.cache.keys, case.cache.values, case.cache.tables,
               case.cache.lengths):
@@ -559,6 +565,10 @@ def test_tensors_that_were_given_other_memory():
     assert torch.equal(case.cache.tables[kids[0], :4], table[case.chosen[1], :4])
     assert (held[-2] == table).all()   # the ones that were left
     assert torch.equal(case.step(case.batch, *case.raw), want)
+    apart[:, 0] += 2
+    case.sinks += 2
+    assert torch.equal(loose(case.batch, *case.raw), case.step(case.batch, *case.raw))
+    assert not torch.equal(loose(case.batch, *case.raw), want)
     case.qw.data = case.qw.data.float()
     with pytest.raises(ValueError, match="query_weight"):
         case.step(case.batch, *case.raw)

@@ -655,6 +655,30 @@ def test_a_steps_tensors_are_checked_where_they_lie_by_now(launches):
         step(batch, *raw)
 
 
+def test_sinks_that_do_not_lie_together_are_read_as_they_are_now(launches):
+    import ctypes
+
+    cache = _taken_up()
+    table = torch.arange(24, dtype=torch.float32).bfloat16().reshape(8, 3)
+    step = BatchAttentionStep(cache, layer=0, heads=8, kv_heads=2, head_dim=64, scale=0.1, dtype=torch.bfloat16,
+                              sinks=table[:, 1])
+    assert type(step.strategy).__name__ == "HipBatchAttentionStep"
+    batch = cache.batch([0, 1])
+    raw = [torch.zeros(2, n * 64, dtype=torch.bfloat16) for n in (8, 2, 2)]
+    read = []
+
+    def call(name, address, stream):
+        from mlx_omnia_amd.runtime.loader import BatchStep
+        read.append(list((ctypes.c_uint16 * 8).from_address(BatchStep.from_address(address).sinks)))
+
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(ops, "call", call)
+        for change in (0.0, 1.0, 7.0):
+            table += change
+            step(batch, *raw)
+            assert read[-1] == table[:, 1].contiguous().view(torch.uint16).tolist()
+
+
 def test_a_caches_calls_name_its_pool_where_it_lies_by_now(launches):
     cache = _taken_up()
     calls = [lambda: cache.fork(0), lambda: cache.open(3), lambda: cache.free(1), cache.compact]
