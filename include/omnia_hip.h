@@ -668,9 +668,9 @@ int32_t omnia_pages_copy(uint16_t* keys, uint16_t* values, int64_t layers, int64
 
 /* Makes sequences the children of `parent`: kids [count, 2] int32 in HOST memory (sequence,
  * page). A child's row of the table is the parent's first `full` entries, then its page, then
- * -1, its length the parent's. The first `rows` rows of every head of `page` (the parent's
- * last, partly filled one) are copied into the child's, in every layer; with rows 0 there is
- * nothing to copy and the children's page is -1. Children and pages are distinct. */
+ * -1, its length full * page_rows + rows, whatever the parent's is on the device. The first `rows` rows of every head of `page` (the parent's last, partly
+ * filled one) are copied into the child's, in every layer; with rows 0 there is nothing to copy
+ * and the children's page is -1. Children and pages are distinct. */
 int32_t omnia_pages_fork(uint16_t* keys, uint16_t* values, int64_t layers, int64_t pages,
                          int64_t kv_heads, int64_t page_rows, int64_t head_dim, int32_t* tables,
                          int32_t* lengths, int64_t sequences, int64_t width, int64_t parent,

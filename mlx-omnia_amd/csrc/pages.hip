@@ -102,7 +102,7 @@ struct ForkArgs {
   int32_t* tables;
   int32_t* lengths;
   int64_t width;
-  int parent, full, page, rows, count, pieces, groups;
+  int parent, full, page, rows, count, pieces, groups, length;
   Kid kids[OMNIA_PAGES_MOVES];
 };
 
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(ForkArgs a) {
     const int32_t* source = a.tables + a.parent * a.width;
     int32_t* row = a.tables + kid.sequence * a.width;
     for (int64_t i = threadIdx.x; i < a.width; i += 256) row[i] = i < a.full ? source[i] : i == a.full ? kid.page : -1;
-    if (threadIdx.x == 0) a.lengths[kid.sequence] = a.lengths[a.parent];
+    if (threadIdx.x == 0) a.lengths[kid.sequence] = a.length;
     return;
   }
   const int piece = block % a.pieces;
@@ -300,12 +300,14 @@ extern "C" int32_t omnia_pages_fork(uint16_t* keys, uint16_t* values, int64_t la
   OMNIA_REQUIRE(!bad_tables(sequences, width, pages), "pages_fork: bad tables");
   OMNIA_REQUIRE(parent >= 0 && parent < sequences, "pages_fork: no such sequence");
   OMNIA_REQUIRE(full >= 0 && full <= width && rows >= 0 && rows <= page_rows, "pages_fork: rows outside the table or page");
+  OMNIA_REQUIRE(full * page_rows + rows < (int64_t{1} << 31), "pages_fork: rows outside the table or page");
   OMNIA_REQUIRE(rows == 0 || (full < width && page >= 0 && page < pages), "pages_fork: no such page");
   if (count == 0) return 0;
   OMNIA_REQUIRE(tables && lengths && kids, "pages_fork: null pointer");
   ForkArgs a{make_pool(keys, values, layers, pages, kv_heads, page_rows, head_dim), tables, lengths, width,
              static_cast<int>(parent), static_cast<int>(full), static_cast<int>(page), static_cast<int>(rows),
-             static_cast<int>(count), 0, static_cast<int>((count + kKidsAtOnce - 1) / kKidsAtOnce), {}};
+             static_cast<int>(count), 0, static_cast<int>((count + kKidsAtOnce - 1) / kKidsAtOnce),
+             static_cast<int>(full * page_rows + rows), {}};
   SmallSet named, written;
   for (int64_t i = 0; i < count; ++i) {
     const Kid kid{kids[2 * i], kids[2 * i + 1]};

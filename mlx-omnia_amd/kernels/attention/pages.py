@@ -365,8 +365,9 @@ class PagedKVCache:
         self._reserve(np.asarray([sequence]), np.asarray([rows]))
 
     def fork(self, sequence: int, count: int = 1, *, share: bool = True) -> list[int]:
-        """`count` new sequences with the rows of this one: its full pages shared, the last,
-        partly filled one copied for each; with `share=False` every page copied."""
+        """`count` new sequences with the rows of this one, as many as the host has counted: its
+        full pages shared, the last, partly filled one copied for each; with `share=False` every
+        page copied."""
         self._refuse_capture("forking")
         self._known([sequence])
         if count < 0:
@@ -544,7 +545,9 @@ class PagedKVCache:
             self.account(batch, 1)
 
     def account(self, batch: PagedBatch, steps: int) -> None:
-        """Count `steps` steps of the batch that the device has taken in replays."""
+        """Count `steps` steps of the batch that the device has taken in replays: before the next
+        call that names its sequences, since the host goes by what it has counted (a fork made
+        ahead of it has the rows of before the replays)."""
         self._current(batch)
         self._rows[batch.index] = self._grown(batch, steps)
         self._clock += 1

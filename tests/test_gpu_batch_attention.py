@@ -506,6 +506,32 @@ def test_steps_that_are_captured():
         assert torch.equal(step(batch, *raw), eager(eager_batch, *raw))
 
 
+def test_a_fork_between_replays_and_their_account():
+    """Its children have the rows that the host has counted, on the device as well, and step on
+    as those of a fork ahead of the replays."""
+    case = Case(heads=8, kv_heads=2, head_dim=64, pairs=32, prefix=0, own=(21,))
+    cache, batch, step = case.cache, case.batch, case.step
+    cache.free(1)   # the case's own, for its slot
+    step.prepare_capture(batch, 3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(batch, *case.raw)
+        cache.advance(batch)
+    (early,) = cache.fork(case.chosen[0])
+    for _ in range(3):
+        graph.replay()
+        torch.empty(1000, device="cuda").normal_().sum().item()
+    late = [*cache.fork(case.chosen[0]), *cache.fork(case.chosen[0], share=False)]
+    assert cache.lengths[[early, *late, case.chosen[0]]].tolist() == [21, 21, 21, 24]
+    assert [cache.rows(s) for s in (early, *late)] == [21] * 3
+    cache.account(batch, 3)
+    assert cache.rows(case.chosen[0]) == 24 and cache.lengths[[early, *late]].tolist() == [21] * 3
+    raw = [t + 1 for t in case.raw]
+    want = step(cache.batch([early]), *raw)
+    for kid in late:
+        assert torch.equal(step(cache.batch([kid]), *raw), want)
+
+
 def test_a_step_is_not_captured_for_fewer_rows_than_it_will_have():
     case = Case(heads=8, kv_heads=2, head_dim=64, prefix=16, own=(3, 4))
     cache, batch, step = case.cache, case.batch, case.step
