@@ -10,7 +10,8 @@ the parent's full pages to share and copies only the page that is still being fi
 hands back the pages that nobody else holds, `compact` moves what is in use to the front of
 the pool. Which page is whose is decided on the host, which holds the counts; `tables` and
 `lengths` say the same on the device, where the kernels read them, and change in the order of
-the current stream with what the kernels do.
+the current stream with what the kernels do. The host's arrays change once the device's part
+has been launched: a call that is refused, or whose launch fails, leaves them as they were.
 
     cache = PagedKVCache.empty(layers, pages, page_rows, kv_heads, head_dim, sequences=64, rows=32768)
     prompt = cache.open()
@@ -340,23 +341,23 @@ class PagedKVCache:
             holders.setdefault(int(self._tables[index[i], at[i]]), []).append(i)
         copied = [i for page, who in holders.items() for i in (who[:-1] if len(who) == self._refs[page] else who)]
         fresh = self._take(len(copied) + int(more.sum()))
-        edits, moves = [], []
+        entries, moves = [], []
         for i, page in zip(copied, fresh.tolist()):
             s, old = int(index[i]), int(self._tables[index[i], at[i]])
             moves.append((old, page, int(now[i] % size)))
-            edits += ops.PAGES_ENTRY, s, int(at[i]), page
-            self._tables[s, at[i]] = page
-            self._refs[old] -= 1
-        self._refs[fresh] = 1
+            entries.append((s, int(at[i]), page))
         rest = iter(fresh[len(copied):].tolist())
         for i in np.flatnonzero(more):
             s = int(index[i])
-            for entry in range(self._held[s], self._held[s] + int(more[i])):
-                self._tables[s, entry] = page = next(rest)
-                edits += ops.PAGES_ENTRY, s, entry, page
-            self._held[s] += int(more[i])
+            entries += [(s, entry, next(rest)) for entry in range(self._held[s], self._held[s] + int(more[i]))]
         self._copy(moves)
-        self._edit(edits)
+        self._edit([n for entry in entries for n in (ops.PAGES_ENTRY, *entry)])
+        for old, _, _ in moves:
+            self._refs[old] -= 1
+        self._refs[fresh] = 1
+        for s, entry, page in entries:
+            self._tables[s, entry] = page
+        self._held[index] += more
 
     def reserve(self, sequence: int, rows: int) -> None:
         """Pages for the sequence up to `rows` rows, ahead of the steps that fill them."""
@@ -386,19 +387,19 @@ class PagedKVCache:
         kids, fresh = self._slots(count), self._take(each * count)
         if not count:
             return kids
-        parent = self._tables[sequence]
+        parent = self._tables[sequence].tolist()
+        lines = fresh.reshape(count, each).tolist()
+        used = [size] * (each - 1) + [rest - size * (each - 1)]
+        self._copy([(page, to, n) for line in lines for page, to, n in zip(parent[full:], line, used)])
+        self._edit([n for kid, line in zip(kids, lines) for n in self._entries(kid, 0, parent[:full] + line)
+                    + [ops.PAGES_LENGTH, kid, rows, 0]])
         self._refs[fresh] = 1
         self._refs[parent[:full]] += count
         self._begin(kids)
-        self._tables[kids, :full] = parent[:full]
-        self._tables[kids, full : full + each] = fresh.reshape(count, each)
+        for kid, line in zip(kids, lines):
+            self._tables[kid, : full + each] = parent[:full] + line
         self._held[kids] = full + each
         self._rows[kids] = rows
-        used = [size] * (each - 1) + [rest - size * (each - 1)]
-        self._copy([(page, to, n) for line in fresh.reshape(count, each).tolist()
-                    for page, to, n in zip(parent[full:].tolist(), line, used)])
-        self._edit([n for kid in kids for n in self._entries(kid, 0, self._tables[kid, : full + each].tolist())
-                    + [ops.PAGES_LENGTH, kid, rows, 0]])
         return kids
 
     def free(self, sequences: Sequence[int] | int) -> None:
@@ -431,11 +432,11 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: sequence {sequence} holds {self._rows[sequence]} rows, not {rows}")
         keep = self._pages_for(rows)
         gone = int(self._held[sequence]) - keep
+        self._edit(self._entries(sequence, keep, [-1] * gone) + [ops.PAGES_LENGTH, sequence, rows, 0])
         self._refs[self._tables[sequence, keep : self._held[sequence]]] -= 1
         self._tables[sequence, keep:] = -1
         self._held[sequence], self._rows[sequence] = keep, rows
         self._renew(sequence)
-        self._edit(self._entries(sequence, keep, [-1] * gone) + [ops.PAGES_LENGTH, sequence, rows, 0])
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool, each that lies behind them to the

@@ -563,6 +563,35 @@ def test_tables_in_another_order():
         cache.fork(0, 1 << 60)
 
 
+@pytest.mark.parametrize("fails", ["_copy", "_edit"])
+@pytest.mark.parametrize("call", ["reserve", "ready", "fork", "truncate"])
+def test_a_launch_that_fails_leaves_the_hosts_part_as_it_was(monkeypatch, call, fails):
+    cache = small(pages=20)
+    parent = cache.open(40)
+    kids = cache.fork(parent, 2)
+    for s in (parent, *kids):
+        cache.truncate(s, 30)   # in a page that the three of them share
+    batch = cache.batch([parent, *kids], tokens=20)
+    calls = dict(reserve=lambda: cache.reserve(parent, 50), ready=lambda: cache.ready(batch),
+                 fork=lambda: cache.fork(parent, 2, share=False), truncate=lambda: cache.truncate(parent, 9))
+    names = "_tables", "_rows", "_held", "_refs", "_generation", "_open"
+    before = {name: getattr(cache, name).copy() for name in names}
+    if call != "truncate" or fails != "_copy":   # which copies nothing
+        def fail(*args, **kwargs):
+            raise RuntimeError("not launched")
+
+        with monkeypatch.context() as patch:
+            patch.setattr(cache, fails, fail)
+            with pytest.raises(RuntimeError, match="not launched"):
+                calls[call]()
+        for name in names:
+            assert np.array_equal(getattr(cache, name), before[name]), name
+    calls[call]()
+    assert any(not np.array_equal(getattr(cache, name), before[name]) for name in names)
+    for s in np.flatnonzero(cache._open):
+        assert cache.tables[s].tolist() == cache._tables[s].tolist() and cache.lengths[s] == cache.rows(s)
+
+
 # Where the kernels read ------------------------------------------------------------------------
 
 
