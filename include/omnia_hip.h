@@ -778,7 +778,7 @@ int64_t omnia_attention_batch_workspace_bytes(int64_t tokens, int64_t heads, int
  * fp32 with wide_queries 1; out [tokens, heads, D] bf16;
  * workspace: at least omnia_attention_batch_workspace_bytes, 16-byte aligned.
  * Beside: core/kernels/attention/default.py:132-156 (one sequence's).
- * head_dim 64 or 128; heads a multiple of kv_heads; scale positive and finite. */
+ * head_dim 64 or 128; heads a multiple of kv_heads; scale positive, below 2^127. */
 int32_t omnia_attention_batch(const void* queries, int32_t wide_queries,
                               const uint16_t* keys, const uint16_t* values, int64_t pages, int64_t page_rows,
                               const int32_t* tables, int64_t sequences, int64_t width,

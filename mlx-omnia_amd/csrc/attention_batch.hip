@@ -1749,7 +1749,7 @@ int32_t attend(const BatchProjectArgs* fresh, const void* queries, int32_t wide_
                 "attention_batch: bad tables");
   OMNIA_REQUIRE(prefix == 0 || (prefix_sequence >= 0 && prefix_sequence < sequences),
                 "attention_batch: no such sequence to read the shared rows through");
-  OMNIA_REQUIRE(scale > 0.0f && scale < INFINITY, "attention_batch: the scale must be positive");
+  OMNIA_REQUIRE(scale > 0.0f && scale * kLog2e < INFINITY, "attention_batch: the scale must be positive, below 2^127");
   if (tokens == 0) return 0;
   OMNIA_REQUIRE(queries && keys && values && tables && lengths && token_map && out && (own_tiles == 0 || tiles),
                 "attention_batch: null pointer");

@@ -166,7 +166,10 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
     @classmethod
     def build(cls, cache, *, layer, heads, kv_heads, head_dim, scale, dtype, query_weight, key_weight, eps,
               rotary_pairs, mscale, angles, sinks) -> "HipBatchAttentionStep | None":
-        if dtype != torch.bfloat16 or cache.keys.dtype != dtype or not 0 < scale < math.inf:
+        if dtype != torch.bfloat16 or cache.keys.dtype != dtype:
+            return None
+        # The kernels' scale is the logarithm's base more, in 32 bits.
+        if not 2.0 ** -126 <= scale < 2.0 ** 127:
             return None
         if not batch_step_applies(heads, kv_heads, head_dim, rotary_pairs):
             return None

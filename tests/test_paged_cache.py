@@ -684,6 +684,22 @@ def test_a_steps_tensors_are_checked_where_they_lie_by_now(launches):
         step(batch, *raw)
 
 
+@pytest.mark.parametrize("scale,served", [(0.1, True), (2.0 ** -126, True), (1e-39, False), (1e-50, False), (0.0, False),
+                                          (-1.0, False), (1e38, True), (3e38, False), (1e39, False), (float("nan"), False)])
+def test_scales_that_32_bits_do_not_hold(launches, scale, served):
+    """They go to the Core chain, and not to kernels that refuse every call."""
+    step = BatchAttentionStep(_taken_up(), layer=0, heads=8, kv_heads=2, head_dim=64, scale=scale, dtype=torch.bfloat16)
+    assert (type(step.strategy) is not DefaultBatchAttentionStep) == served
+
+
+@pytest.mark.parametrize("scale,rc", [(0.1, 0), (1e38, 0), (3e38, -22), (1e39, -22), (0.0, -22), (-1.0, -22), (float("nan"), -22)])
+def test_attention_batch_refuses_scales(scale, rc):
+    from mlx_omnia_amd.runtime import library
+    at = 4096   # of no tokens: nothing is looked at
+    assert library().omnia_attention_batch(at, 0, at, at, 8, 16, at, 2, 4, at, at, 0, at, 0, 0, 0, 0, 0, 8, 2, 64, None, scale,
+                                           None, 0, at, None) == rc
+
+
 def test_sinks_that_do_not_lie_together_are_read_as_they_are_now(launches):
     import ctypes
 
