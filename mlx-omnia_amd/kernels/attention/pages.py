@@ -247,21 +247,15 @@ class PagedKVCache:
         """The edits that make `pages` a sequence's entries from `first` on."""
         return [n for i, page in enumerate(pages, first) for n in (ops.PAGES_ENTRY, sequence, i, page)]
 
-    def _copy(self, moves: list[tuple[int, int, int]], rename: bool = False) -> None:
+    def _copy(self, moves: list[tuple[int, int, int]]) -> None:
         if not moves:
             return
         if self._pool is not None:
-            if rename:
-                self._pool.copy(moves, self.tables.data_ptr(), self.tables.numel())
-            else:
-                self._pool.copy(moves)
+            self._pool.copy(moves)
             return
         for pool in (self.keys, self.values):
             for source, target, rows in moves:
                 pool[:, target, :, :rows] = pool[:, source, :, :rows]
-        if rename:
-            names = {source: target for source, target, _ in moves}
-            self.tables.apply_(lambda page: names.get(page, page))
 
     # Pages --------------------------------------------------------------------------------
 
@@ -451,9 +445,10 @@ class PagedKVCache:
         if len(source):
             names = np.arange(self.pages + 1, dtype=np.int32)   # the last for -1
             names[-1], names[source] = -1, target
+            self._copy([(a, b, self.page_rows) for a, b in zip(source.tolist(), target.tolist())])
             self._tables[:] = names[self._tables]
             self._refs[target], self._refs[source] = self._refs[source], 0
-            self._copy([(a, b, self.page_rows) for a, b in zip(source.tolist(), target.tolist())], rename=True)
+            self.tables.copy_(torch.from_numpy(self._tables))
         return live
 
     def resize(self, pages: int) -> None:

@@ -1196,8 +1196,8 @@ def _page_tables(tables: torch.Tensor, lengths: torch.Tensor, name: str) -> tupl
 
 
 class PagePool:
-    """A pool of pages with its tables, checked once: `copy`, `fork` and `edit` as the functions
-    below have them. (Fifteen microseconds of a fork's thirty-six were checks of tensors that a
+    """A pool of pages with its tables, checked once: `copy` and `edit` as the functions below
+    have them. (Fifteen microseconds of a fork's thirty-six were checks of tensors that a
     cache keeps.)"""
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor | None = None,
@@ -1211,7 +1211,7 @@ class PagePool:
         self.held = [t for t in (keys, values, tables, lengths) if t is not None]
         _require(on_rocm(*self.held), "page pool: tensors must share one ROCm device")
         self.addresses = [t.data_ptr() for t in self.held]
-        _require(all(self.addresses), "page pool: a tensor without memory")
+        _require(all(at or not t.numel() for at, t in zip(self.addresses, self.held)), "page pool: a tensor without memory")
         self.pool = keys.data_ptr(), values.data_ptr(), *keys.shape[:4], width // 2
         self.index, self.pages = keys.get_device(), keys.shape[1]
         if tables is not None and lengths is not None:
@@ -1273,15 +1273,6 @@ class PagePool:
             call("omnia_pages_copy", *self.pool, address + 4 * first, min(step, len(flat) - first) // 3, tables,
                  entries, stream)
 
-    def fork(self, parent: int, full: int, page: int, rows: int, kids) -> None:
-        flat, step = _int_lines(kids, 2, "kids"), 2 * PAGES_MOVES
-        if len(flat) > step and (len(set(flat[0::2])) < len(flat) // 2 or (rows and len(set(flat[1::2])) < len(flat) // 2)):
-            raise ValueError("pages_fork: a child or a page is named twice")
-        stream, address = self.stream(), flat.buffer_info()[0]
-        for first in range(0, len(flat), step):
-            call("omnia_pages_fork", *self.pool, self.tables, self.lengths, self.sequences, self.width, parent, full,
-                 page, rows, address + 4 * first, min(step, len(flat) - first) // 2, stream)
-
     def edit(self, edits) -> None:
         _edit(self.tables, self.lengths, self.sequences, self.width, self.pages, edits, self.stream())
 
@@ -1304,13 +1295,6 @@ def pages_copy(keys: torch.Tensor, values: torch.Tensor, moves, *, tables: torch
         return PagePool(keys, values).copy(moves)
     _require(tables.dtype == torch.int32 and tables.is_contiguous(), "pages_copy: tables must be contiguous int32")
     PagePool(keys, values, tables).copy(moves, tables.data_ptr(), tables.numel())
-
-
-def pages_fork(keys: torch.Tensor, values: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, parent: int,
-               full: int, page: int, rows: int, kids) -> None:
-    """Make sequences the children of `parent`, each a (sequence, page) of kids: they share its
-    first `full` pages and get the first `rows` rows of `page` copied; see `omnia_pages_fork`."""
-    PagePool(keys, values, tables, lengths).fork(parent, full, page, rows, kids)
 
 
 def pages_edit(tables: torch.Tensor, lengths: torch.Tensor, pages: int, edits) -> None:
