@@ -1417,8 +1417,8 @@ struct Plan {
 constexpr int64_t kSlots = 512, kNarrowBlocks = 2048, kNarrowKeys = 512, kMaxSplits = 64;
 constexpr int64_t kOwnKeys = 256, kOwnPieces = 2048;
 
-// Most pieces of a row: the merge takes them one after another, but a few kv heads of a few
-// sequences have to fill the card (two of one sequence of 400,000 rows: 64 pieces each 251 us, 512 86).
+// Most pieces of a row: the merge reads them all again, up to 64 at once, but a few kv heads of a
+// few sequences have to fill the card (two of one sequence of 400,000 rows: 64 pieces each 251 us, 512 86).
 int64_t most_splits(int64_t blocks) {
   const int64_t fill = 2 * kSlots / (blocks < 1 ? 1 : blocks);
   return fill > kMaxSplits ? fill : kMaxSplits;
@@ -1436,14 +1436,19 @@ int64_t cut(int64_t blocks, int64_t keys, int64_t splits, int64_t& each) {
 }
 
 // What wide pieces were measured to take, in us: one on a CU waits for its keys, two share the
-// matrix cores and the start's loads.
+// matrix cores and the start's loads. That was with one part of the weights; with two a tile takes
+// 1.5 and 2.15, and 2.4 and 3.35. Cut by those, it comes out even (replayed): three prompts of 300
+// tokens behind 512 rows 54.8 -> 49.6, nine of 120 behind 2,048 124 -> 117, but 40 of 20 behind
+// 8,192 216 -> 230 and 128 tokens behind 32,768 181 -> 187, so they stay.
 struct WideCost {
   double start, tile, start_both, tile_both, tile_bytes;
 };
 constexpr WideCost kCost64{4.0, 1.2, 5.0, 1.6, 16384.0}, kCost128{5.5, 2.0, 7.5, 2.57, 32768.0};
 constexpr double kBytesPerUs = 6e6, kLaunchUs = 4.0;
 
-// `count` pieces of `tiles` tiles, of which `row_tiles` read the same keys.
+// `count` pieces of `tiles` tiles, of which `row_tiles` read the same keys. (Alone, the start takes
+// less where there are fewer to share the caches' rate: 256 pieces of four tiles 20.0 us, 128 and 64
+// of them 18.0, the launch included; 0.65 and 0.7 are fitted to such replays.)
 double wide_us(const WideCost& c, int64_t count, int64_t tiles, int64_t row_tiles) {
   const auto round = [&](int64_t n) {
     if (n <= 0) return 0.0;
@@ -1482,7 +1487,8 @@ int64_t wide_splits(int64_t blocks, int64_t keys, double filled, const WideCost&
     const int64_t count = static_cast<int64_t>(blocks * splits * filled) + (filled < 1.0 ? 1 : 0);
     double us = wide_us(c, count, of_one, row_tiles);
     if (beside.pieces > 0) {
-      // Beside the others one takes a quarter longer, and with every slot taken the last wait.
+      // Beside the others one takes a quarter longer, and with every slot taken the last wait: 0.8,
+      // 1.05 and 15 of 16 are fitted to the replays above together, not measured apart.
       const double meanwhile = count < kSlots ? 0.8 * (kSlots - count) * us / beside.us : 0.0;
       if (count > kSlots / 16 * 15) us *= 1.05;
       if (meanwhile < beside.pieces) us += (beside.pieces - meanwhile) / beside.pieces * beside.all_us;
@@ -1520,11 +1526,14 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
   const int64_t rows = tokens * (heads / kv_heads);
   const int64_t shared_tiles = (rows + kTileRows - 1) / kTileRows;
   // Where the sequences' own tiles are nearly as full as shared ones (prompts), each walks the
-  // shared rows as well: as many products, and nothing to merge.
+  // shared rows as well: as many products, and nothing to merge. At 1.06 as many tiles, nine
+  // prompts of 120 tokens, that is even (behind 2,048 rows 116 us shared, 117 walked, behind 8,192
+  // 307 and 309), at 1.24, of 100, it is not (98 and 110, 233 and 285), nor mostly at 1.2, of 50 (69
+  // and 62, 134 and 156).
   // So do a few sequences of a few rows: one piece a row, and again nothing to merge (2 of 229
   // rows: 16 -> 13.4 us a step).
   const bool few = prefix + own_rows <= kNarrowKeys && kv_heads * own_tiles <= kSlots;
-  p.prefix = own_tiles * 4 <= shared_tiles * 5 || few ? 0 : prefix;
+  p.prefix = own_tiles * 8 <= shared_tiles * 9 || few ? 0 : prefix;
   if (own_total > 0) own_total += (prefix - p.prefix) * own_tiles;
   own_rows += prefix - p.prefix;
   p.prefix_tiles = p.prefix > 0 ? shared_tiles : 0;
@@ -1548,7 +1557,7 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
         own.fresh = own_tiles == tokens && heads <= kNarrowRows * kv_heads;
         own.pieces = own_blocks * (filled * own_rows / kNarrowKeys + 0.5);
         if (own.pieces < own_blocks) own.pieces = static_cast<double>(own_blocks);
-        own.us = 3.0 + 0.011 * of_one;
+        own.us = 3.0 + 0.011 * of_one;   // 128 pieces, launch included: 5.8 us of 128 keys, 7.0 of 192
       } else if (any_own) {
         own.pieces = static_cast<double>(own_blocks);
         own.us = cost.start + (own_rows + kTileKeys - 1) / kTileKeys * cost.tile;
@@ -1564,7 +1573,8 @@ Plan plan_for(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
   if (p.own_alone) {
     // All at once where that is possible: a wave that has done its piece leaves the others more
     // of the memory's rate, until the last ones cannot take it. Short ones where a few sequences
-    // have most of the rows (64 sequences of up to 567, but one of 4,000, of 3 tokens: 92 -> 48 us).
+    // have most of the rows (64 sequences of up to 567, but one of 4,000, of 3 tokens: 92 -> 48 us;
+    // eight of up to 8,000, of 6 tokens, 39 -> 43).
     const int64_t even = filled < 0.5 ? static_cast<int64_t>(own_blocks * 2.0 * filled) + 1 : own_blocks;
     const int64_t fill = (kOwnPieces + even - 1) / even;
     const int64_t most = own_rows / kOwnKeys, least = own_rows / (4 * kOwnKeys);
