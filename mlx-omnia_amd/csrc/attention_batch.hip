@@ -948,7 +948,7 @@ __device__ __forceinline__ void wide_piece(const BatchArgs& a, Piece p, PageWalk
   // The stages by name, not by a turning index: the compiler then sees that what is on its way
   // to the one is not what is read from the other, and does not wait for it.
   // The next tile is asked for between the products (ahead of them, 1,828 tokens of prompts took
-  // 203 us for 196), whatever it is, without a branch that they would wait at, and patched once it
+  // 203 us for 196, with one part of the weights), whatever it is, without a branch that they would wait at, and patched once it
   // has arrived. Behind the last it is that one again: a piece of four tiles takes up to a
   // hundredth longer.
   static_assert(Rows::kSteps == 2 * kLoads, "a vector of the next tile a step of the products");
@@ -1472,9 +1472,9 @@ struct Beside {
 // as many as are expected to be done first, with their partial results (`row_us` for
 // a piece of every row) and the merge's launch, and what is beside them and finds no slot
 // meanwhile. Against as many as fill the slots, of 256 keys or more (replayed): 128 tokens behind
-// 32,768 rows with up to 1,024 own each 166 -> 155 us, 128 behind 4,096 95 -> 78, 96 behind 4,000
-// 43 -> 41, 100 of two kv heads behind 8,192 34.7 -> 27.9, nine prompts of up to 100 tokens behind
-// 2,048 79 -> 60.
+// 32,768 rows with up to 1,024 own each 202 -> 181 us, 128 behind 4,096 105 -> 81, 96 behind 4,000
+// 53 -> 50, 100 of two kv heads behind 8,192 46 -> 42, nine prompts of up to 100 tokens behind
+// 2,048 88 -> 68.
 int64_t wide_splits(int64_t blocks, int64_t keys, double filled, const WideCost& c, int64_t row_tiles, double row_us,
                     const Beside& beside, int64_t& each) {
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
