@@ -168,7 +168,7 @@ class HipBatchAttentionStep(BatchAttentionStepStrategy):
               rotary_pairs, mscale, angles, sinks) -> "HipBatchAttentionStep | None":
         if dtype != torch.bfloat16 or cache.keys.dtype != dtype:
             return None
-        # The kernels' scale is the logarithm's base more, in 32 bits.
+        # The kernels take scale * log2(e), in 32 bits.
         if not 2.0 ** -126 <= scale < 2.0 ** 127:
             return None
         if not batch_step_applies(heads, kv_heads, head_dim, rotary_pairs):

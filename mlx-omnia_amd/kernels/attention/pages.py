@@ -11,7 +11,8 @@ hands back the pages that nobody else holds, `compact` moves what is in use to t
 the pool. Which page is whose is decided on the host, which holds the counts; `tables` and
 `lengths` say the same on the device, where the kernels read them, and change in the order of
 the current stream with what the kernels do. The host's arrays change once the device's part
-has been launched: a call that is refused, or whose launch fails, leaves them as they were.
+has been launched: a call that is refused, or whose launch fails, leaves them as they were (a
+compaction of many pages keeps what it has moved by then).
 
     cache = PagedKVCache.empty(layers, pages, page_rows, kv_heads, head_dim, sequences=64, rows=32768)
     prompt = cache.open()
@@ -474,7 +475,8 @@ class PagedKVCache:
 
     def batch(self, sequences: Sequence[int], tokens: int | Sequence[int] = 1) -> PagedBatch:
         """The steps of these sequences with so many new tokens each (or each its own number).
-        The rows that all of them share are found here, from the tables."""
+        The rows that all of them share are found here, from the tables; what only some of them
+        share each reads for itself, so groups that share nothing step as batches of their own."""
         self._refuse_capture("making a batch")
         chosen = [int(s) for s in sequences]
         if not chosen or len(set(chosen)) != len(chosen):

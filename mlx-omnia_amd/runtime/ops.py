@@ -1481,7 +1481,7 @@ class BatchStepPlan:
                     raise ValueError(f"{name}: fp32 [positions, pairs], 16-byte aligned with unit inner stride")
             held += [cos, sin]
         _require(on_rocm(*held), "attention_batch_step: tensors must share one ROCm device")
-        _require(all(t.data_ptr() for t in held), "attention_batch_step: a tensor without memory")
+        _require(all(t.data_ptr() or not t.numel() for t in held), "attention_batch_step: a tensor without memory")
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         # The memory itself: a tensor that is given other memory must not let go of what is read here.
         self.held, self.index = [t.detach() for t in held], keys.get_device()

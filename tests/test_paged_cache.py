@@ -724,6 +724,15 @@ def test_sinks_that_do_not_lie_together_are_read_as_they_are_now(launches):
             assert read[-1] == table[:, 1].contiguous().view(torch.uint16).tolist()
 
 
+def test_a_plan_of_no_tokens(launches):
+    cache = _taken_up()
+    none = torch.empty((0, 2), dtype=torch.int32)
+    plan = ops.BatchStepPlan(None, None, None, cache.keys[0], cache.values[0], cache.tables, cache.lengths, none,
+                             torch.empty((0, 4), dtype=torch.int32), heads=8, prefix=0, prefix_sequence=0, scale=0.1, eps=1e-6)
+    assert plan(*(torch.empty((0, n * 64), dtype=torch.bfloat16) for n in (8, 2, 2)), 1).shape == (0, 8, 64)
+    assert launches[-1][1].tokens == 0
+
+
 def test_a_caches_calls_name_its_pool_where_it_lies_by_now(launches):
     cache = _taken_up()
     calls = [lambda: cache.fork(0), lambda: cache.open(3), lambda: cache.free(1), cache.compact]
