@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define OMNIA_ABI_VERSION 16
+#define OMNIA_ABI_VERSION 17
 
 /* Version of this ABI (OMNIA_ABI_VERSION). Pure; touches no device. */
 int32_t omnia_abi_version(void);
@@ -816,6 +816,61 @@ int64_t omnia_attention_batch_step_bytes(int64_t tokens, int64_t heads, int64_t 
                                          int64_t head_dim, int64_t prefix, int64_t own_rows,
                                          int64_t own_total, int64_t own_tiles);
 int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hipStream_t stream);
+
+/* Linear attention with a decay for each head, over the packed new tokens of a batch:
+ *   S_t = exp(g[t, h]) S_{t-1} + w[t, h] k[t, h / (heads / key_heads)] v[t, h]^T
+ *   out[t, h] = bf16(scale * q[t, h / (heads / key_heads)] S_t)
+ * for the tokens of each sequence in order, S in fp32 [key_dim, value_dim] from
+ * states[slot, h], where the last one is left. Sums are fp32.
+ * queries, keys [tokens, key_heads, key_dim], values [tokens, heads, value_dim] bf16, the heads
+ * of a token together, its rows *_stride elements apart; log_decay (g) fp32 [tokens, heads],
+ * decay_stride floats apart (0: one row [heads] for every token); strengths (w) likewise, or
+ * null (ones); states [slots, heads, key_dim, value_dim] fp32; out [tokens, heads, value_dim]
+ * bf16. steps [step_count, 3] int32 (device): the slot, first token and token count of each
+ * sequence. No slot may be named twice; an entry outside the states or the tokens is skipped.
+ * Its input is what omnia_gate_softplus gives (models/qwen3_5/layers/deltanet.py:222-224);
+ * the single-token recurrence stands where core/kernels/ssm does.
+ * key_dim, value_dim 64 or 128; heads a multiple of key_heads, at most 4096. */
+typedef struct {
+  const uint16_t *queries, *keys, *values;
+  const float *log_decay, *strengths;
+  float* states;
+  const int32_t* steps;
+  uint16_t* out;
+  int64_t query_stride, key_stride, value_stride, decay_stride, strength_stride;
+  int64_t slots, tokens, heads, key_heads, key_dim, value_dim, step_count;
+  float scale;
+} omnia_linear_attention_t;
+int32_t omnia_linear_attention(const omnia_linear_attention_t* call, hipStream_t stream);
+
+/* RMSNorm of a mixer's output in groups, with its gate:
+ *   gate_first 0:  out = bf16(x * inv * weight * act(gate)),   inv = 1 / sqrt(mean(x^2) + eps)
+ *   gate_first 1:  y = x * act(gate), out = bf16(y * inv * weight), inv of y
+ * over each `group` consecutive values of a row, in fp32, rounded once; act is
+ * z / (1 + exp(-z)) (silu 1) or 1 / (1 + exp(-z)) (silu 0). x, gate bf16 [rows, width], rows
+ * their strides apart; weight bf16 [group] (weight_width == group) or [width]; out [rows, width].
+ * The gated norm behind the mixers of models/qwen3_5 and of core/kernels/mamba_step.
+ * group a multiple of 8, at most 8192, dividing width. */
+int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t* gate,
+                             int64_t gate_stride, const uint16_t* weight, int64_t weight_width,
+                             int64_t rows, int64_t width, int64_t group, float eps, int32_t silu,
+                             int32_t gate_first, uint16_t* out, hipStream_t stream);
+
+/* The join of two blocks: the norm behind the one, its gate, both scales, the norm ahead of
+ * the other, in one pass:
+ *   y = block, or block * inv(block) * post_weight;  y = y * act(gate) with a gate
+ *   s = residual_scale * x + block_scale * y;        summed = bf16(s)
+ *   normalized = bf16(s * inv(s) * pre_weight)       inv(v) = 1 / sqrt(mean(v^2) + eps)
+ * in fp32 (s unrounded in the norm). x, block bf16 [rows, hidden] and, null for none, gate
+ * bf16 [rows, hidden], rows gate_stride apart (0: one row for all); act is 1 / (1 + exp(-z))
+ * (sigmoid 1) or z itself; post_weight [hidden] or null, pre_weight [hidden].
+ * Beside omnia_add_rms_norm, for blocks that are normed on both sides (core/kernels/add_norm).
+ * hidden a multiple of 8, at most 16384. */
+int32_t omnia_block_norm(const uint16_t* x, const uint16_t* block, const uint16_t* gate,
+                         int64_t gate_stride, int32_t sigmoid, const uint16_t* post_weight,
+                         float post_eps, const uint16_t* pre_weight, float pre_eps,
+                         float residual_scale, float block_scale, int64_t rows, int64_t hidden,
+                         uint16_t* summed, uint16_t* normalized, hipStream_t stream);
 
 #ifdef __cplusplus
 }

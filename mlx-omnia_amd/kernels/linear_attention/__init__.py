@@ -1,0 +1,217 @@
+"""Linear attention with a decay for each head: a mixer whose state stands in place of a cache.
+
+    S_t = exp(g_t) S_{t-1} + w_t k_t v_t^T,   o_t = scale * q_t S_t
+
+for each sequence's new tokens in order, S [key_dim, value_dim] fp32 of every head in a pool
+`states` [slots, heads, key_dim, value_dim]. It reads what `GateSoftplus` gives
+(models/qwen3_5/layers/deltanet.py:222-224: g = -exp(A_log) softplus(a + dt_bias)), and stands
+beside `AttentionStep` as the single-token recurrence of core/kernels/ssm stands beside
+core/kernels/attention. One call takes prompts and steps of one token alike, a batch of any
+lengths:
+
+    states = torch.zeros(slots, heads, key_dim, value_dim, device="cuda")
+    mixer = LinearAttention(states, heads=32, key_heads=16, key_dim=128, value_dim=128,
+                            scale=128 ** -0.5, dtype=torch.bfloat16)
+    batch = LinearBatch([3, 0], [900, 1])          # 900 new tokens of slot 3, one of slot 0
+    o = mixer(batch, q, k, v, g)                   # the states of both, moved on
+
+A fresh sequence's state is zeros and a fork's a copy of its parent's (`states[kid] =
+states[parent]`): both are the caller's, on the stream of the calls.
+
+- `HipLinearAttention` (`omnia_linear_attention`, csrc/linear_attention.hip): bf16 rows, heads
+  of 64 or 128, any number of heads per key head, fp32 gates and states.
+- `DefaultLinearAttention` is the Core chain in torch ops, and takes everything, calls that
+  autograd follows among it: gradients of the call's own inputs (the pool follows none).
+
+A token sees its own sequence's tokens up to itself, and nothing of the values behind them: an
+infinity or a NaN there stays with the tokens from its own on.
+"""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Sequence
+from dataclasses import dataclass
+from typing import Protocol, runtime_checkable
+
+import numpy as np
+import torch
+
+from ...runtime import ops
+from .._device import hip_device
+from ..attention.prefill import unfollowed
+from ..resolve import record_fallback, resolve
+
+__all__ = ["DefaultLinearAttention", "HipLinearAttention", "LinearAttention", "LinearAttentionStrategy",
+           "LinearBatch", "applies"]
+
+DIMS = (64, 128)
+CHUNK = 64   # tokens that the Core chain takes together
+
+
+class LinearBatch:
+    """The sequences of a call: the slots of their states, each once, and how many new tokens each
+    has (none among them). Their rows lie together in the call's tensors, in this order. Made on
+    the host and kept as long as the same slots step on."""
+
+    def __init__(self, slots: Sequence[int], tokens: Sequence[int], *, device: torch.device | str = "cuda") -> None:
+        self.slots, self.tokens = tuple(int(s) for s in slots), tuple(int(n) for n in tokens)
+        if len(self.slots) != len(self.tokens):
+            raise ValueError(f"LinearBatch: {len(self.slots)} slots with {len(self.tokens)} token counts")
+        if len(set(self.slots)) != len(self.slots) or any(s < 0 for s in self.slots):
+            raise ValueError("LinearBatch: a slot is named twice, or negative")
+        if any(n < 0 for n in self.tokens):
+            raise ValueError("LinearBatch: a negative token count")
+        self.total = sum(self.tokens)
+        if self.total >= 1 << 24:
+            raise ValueError(f"LinearBatch: {self.total} tokens, of at most {(1 << 24) - 1}")
+        self.device = torch.device(device)
+        self.plans: dict = {}   # what a layer's binding laid out for the batch
+        self._steps: torch.Tensor | None = None
+
+    def steps(self) -> torch.Tensor:
+        """[n, 3] int32 on the device: slot, first token and count of every sequence with new tokens."""
+        if self._steps is None:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise ValueError("a batch's first call cannot be captured: make one before")
+            counts = np.asarray(self.tokens, dtype=np.int64)
+            rows = np.stack([np.asarray(self.slots, dtype=np.int64), np.cumsum(counts) - counts, counts], axis=1)
+            rows = np.ascontiguousarray(rows[counts > 0], dtype=np.int32).reshape(-1, 3)
+            self._steps = torch.from_numpy(rows).to(self.device)
+        return self._steps
+
+
+@runtime_checkable
+class LinearAttentionStrategy(Protocol):
+    """A batch's N packed tokens: queries, keys [N, key_heads, key_dim], values [N, heads, value_dim],
+    log_decay and strengths [N, heads] fp32 -> the context [N, heads, value_dim]."""
+
+    def __call__(self, batch: LinearBatch, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                 log_decay: torch.Tensor | None = None, strengths: torch.Tensor | None = None) -> torch.Tensor: ...
+
+
+def applies(heads: int, key_heads: int, key_dim: int, value_dim: int) -> bool:
+    """Heads of 64 or 128, whole groups of them for a key head."""
+    return (key_dim in DIMS and value_dim in DIMS and key_heads > 0 and 0 < heads <= 4096 and heads % key_heads == 0)
+
+
+@dataclass(frozen=True)
+class DefaultLinearAttention(LinearAttentionStrategy):
+    states: torch.Tensor
+    heads: int
+    key_heads: int
+    scale: float
+    decay: torch.Tensor | None
+
+    @classmethod
+    def build(cls, states, *, heads, key_heads, key_dim, value_dim, scale, dtype, decay) -> "DefaultLinearAttention":
+        return cls(states, heads, key_heads, scale, decay)
+
+    def _gates(self, batch: LinearBatch, log_decay: torch.Tensor | None) -> torch.Tensor:
+        """[N, heads], fp64: its sums lose nothing of a slow decay behind a fast one."""
+        gates = self.decay if log_decay is None else log_decay
+        return gates.double().expand(batch.total, self.heads)
+
+    def __call__(self, batch, queries, keys, values, log_decay=None, strengths=None):
+        kind = torch.promote_types(queries.dtype, torch.float32)
+        group = self.heads // self.key_heads
+        q, k = (x.to(kind).repeat_interleave(group, dim=1) for x in (queries, keys))
+        v, gates = values.to(kind), self._gates(batch, log_decay)
+        if strengths is not None:
+            v = v * strengths.to(kind)[..., None]
+        # Zero times a value that a token does not see is a NaN where it is not finite: then one at a time.
+        chunk = CHUNK if bool(torch.isfinite(v).all()) else 1
+        out, end = [], 0
+        for slot, count in zip(batch.slots, batch.tokens):
+            state = self.states[slot].detach().to(kind, copy=True)   # the pool is written below
+            for first in range(end, end + count, chunk):
+                mine = slice(first, min(first + chunk, end + count))
+                # Never -inf, whose differences are NaN: exp(-1e5) is zero as well.
+                to = torch.cumsum(gates[mine].clamp(min=-1e5), dim=0).t()   # [heads, n]
+                seen = torch.ones(to.shape[1], to.shape[1], dtype=torch.bool, device=to.device).tril()
+                apart = torch.where(seen, to[:, :, None] - to[:, None], -math.inf)
+                qs, ks, vs = (x[mine].transpose(0, 1) for x in (q, k, v))
+                weight = torch.where(seen, qs @ ks.transpose(1, 2).contiguous(), 0) * torch.exp(apart).to(kind)
+                mixed = weight @ vs + (qs @ state) * torch.exp(to).to(kind)[..., None]
+                out.append(mixed.transpose(0, 1) * self.scale)
+                left = torch.exp(to[:, -1:] - to).to(kind)
+                state = state * torch.exp(to[:, -1]).to(kind)[:, None, None] + (
+                    ks * left[..., None]).transpose(1, 2).contiguous() @ vs
+            if count:
+                # The pool itself follows no gradient.
+                self.states[slot] = state.detach().to(self.states.dtype)
+            end += count
+        return torch.cat(out).to(queries.dtype) if out else torch.zeros_like(values)
+
+
+@dataclass(frozen=True, eq=False)
+class HipLinearAttention(LinearAttentionStrategy):
+    core: DefaultLinearAttention
+
+    @classmethod
+    def build(cls, states, *, heads, key_heads, key_dim, value_dim, scale, dtype, decay) -> "HipLinearAttention | None":
+        if dtype != torch.bfloat16 or states.dtype != torch.float32 or not states.is_contiguous():
+            return None
+        if not applies(heads, key_heads, key_dim, value_dim) or states.data_ptr() % 16:
+            return None
+        if decay is not None and (decay.dtype != torch.float32 or not decay.is_contiguous()):
+            return None
+        if not hip_device(states, *(() if decay is None else (decay,))):
+            return None
+        return cls(DefaultLinearAttention(states, heads, key_heads, scale, decay))
+
+    def __call__(self, batch, queries, keys, values, log_decay=None, strengths=None):
+        core = self.core
+        gates = core.decay if log_decay is None else log_decay
+        if not unfollowed(queries, keys, values, gates, core.states, *(() if strengths is None else (strengths,))):
+            record_fallback(self, core)
+            return core(batch, queries, keys, values, log_decay, strengths)
+        plan, at = batch.plans.get(self, (None, None))
+        if plan is None or at != core.states.data_ptr():   # a pool that was given other memory
+            plan, at = ops.LinearAttentionPlan(core.states, batch.steps(), batch.total, key_heads=core.key_heads,
+                                               scale=core.scale), core.states.data_ptr()
+            batch.plans[self] = plan, at
+        return plan(queries, keys, values, gates, strengths)
+
+
+_STRATEGIES = (HipLinearAttention, DefaultLinearAttention)
+
+
+class LinearAttention(LinearAttentionStrategy):
+    """A layer's mixer over its pool of states: picks its binding once, then forwards every call.
+
+    `decay` [heads] is a layer's fixed log decay, for calls that give none of their own."""
+
+    def __init__(self, states: torch.Tensor, *, heads: int, key_heads: int, key_dim: int, value_dim: int, scale: float,
+                 dtype: torch.dtype, decay: torch.Tensor | None = None, reference: bool = False) -> None:
+        if states.dim() != 4 or tuple(states.shape[1:]) != (heads, key_dim, value_dim):
+            raise ValueError(f"LinearAttention: states [slots, {heads}, {key_dim}, {value_dim}], not {tuple(states.shape)}")
+        if key_heads < 1 or heads < 1 or heads % key_heads:
+            raise ValueError(f"LinearAttention: {heads} heads over {key_heads} key heads")
+        if not states.is_floating_point() or states.element_size() < 4:
+            raise ValueError(f"LinearAttention: states in 32 bits or more, not {states.dtype}")
+        if decay is not None and decay.shape != (heads,):
+            raise ValueError(f"LinearAttention: a decay for each of {heads} heads, not {tuple(decay.shape)}")
+        self.shapes = (key_heads, key_dim), (heads, value_dim), heads
+        self.slots, self.decay, self.device = states.shape[0], decay, states.device
+        self.strategy: LinearAttentionStrategy = resolve(
+            (DefaultLinearAttention,) if reference else _STRATEGIES, states, heads=heads, key_heads=key_heads,
+            key_dim=key_dim, value_dim=value_dim, scale=scale, dtype=dtype, decay=decay)
+
+    def __call__(self, batch: LinearBatch, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                 log_decay: torch.Tensor | None = None, strengths: torch.Tensor | None = None) -> torch.Tensor:
+        of_keys, of_values, heads = self.shapes
+        n = batch.total
+        if queries.shape != (n, *of_keys) or keys.shape != (n, *of_keys) or values.shape != (n, *of_values):
+            raise ValueError(f"LinearAttention: the batch's {n} tokens are queries and keys {(n, *of_keys)} and values "
+                             f"{(n, *of_values)}, not {tuple(queries.shape)}, {tuple(keys.shape)} and {tuple(values.shape)}")
+        if log_decay is None:
+            if self.decay is None:
+                raise ValueError("LinearAttention: neither the layer nor the call has a decay")
+        elif log_decay.shape != (n, heads):
+            raise ValueError(f"LinearAttention: log_decay {(n, heads)}, not {tuple(log_decay.shape)}")
+        if strengths is not None and strengths.shape != (n, heads):
+            raise ValueError(f"LinearAttention: strengths {(n, heads)}, not {tuple(strengths.shape)}")
+        if batch.slots and max(batch.slots) >= self.slots:
+            raise ValueError(f"LinearAttention: slot {max(batch.slots)} of a pool of {self.slots}")
+        return self.strategy(batch, queries, keys, values, log_decay, strengths)

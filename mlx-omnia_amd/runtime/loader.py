@@ -14,7 +14,7 @@ import threading
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "libomnia_hip.so"
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -41,6 +41,16 @@ class PagedCache(ctypes.Structure):
     _fields_ = ([(name, _P) for name in ("keys", "values", "tables", "lengths", "host_tables", "rows", "held", "refs",
                                          "generation", "open")]
                 + [(name, _I64) for name in ("layers", "pages", "kv_heads", "page_rows", "head_dim", "sequences", "width")])
+
+
+class LinearAttentionCall(ctypes.Structure):
+    """`omnia_linear_attention_t`; must match include/omnia_hip.h."""
+
+    _fields_ = ([(name, _P) for name in ("queries", "keys", "values", "log_decay", "strengths", "states", "steps", "out")]
+                + [(name, _I64) for name in (
+                    "query_stride", "key_stride", "value_stride", "decay_stride", "strength_stride", "slots", "tokens",
+                    "heads", "key_heads", "key_dim", "value_dim", "step_count")]
+                + [("scale", _F32)])
 
 
 # name -> (restype, argtypes); must match include/omnia_hip.h.
@@ -136,6 +146,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                      _I64, _I64, _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
     "omnia_attention_batch_step_bytes": (_I64, [_I64] * 8),
     "omnia_attention_batch_step": (_I32, [_P, _P]),
+    "omnia_linear_attention": (_I32, [_P, _P]),
+    "omnia_gated_rms_norm": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F32, _I32, _I32, _P, _P]),
+    "omnia_block_norm": (_I32, [_P, _P, _P, _I64, _I32, _P, _F32, _P, _F32, _F32, _F32, _I64, _I64, _P, _P, _P]),
     "omnia_embed_atlas": (
         _I32,
         [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P],
