@@ -826,8 +826,16 @@ int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hip
  * of a token together, its rows *_stride elements apart; log_decay (g) fp32 [tokens, heads],
  * decay_stride floats apart (0: one row [heads] for every token); strengths (w) likewise, or
  * null (ones); states [slots, heads, key_dim, value_dim] fp32; out [tokens, heads, value_dim]
- * bf16. steps [step_count, 3] int32 (device): the slot, first token and token count of each
- * sequence. No slot may be named twice; an entry outside the states or the tokens is skipped.
+ * bf16.
+ * steps [step_count, 3] int32 (device): slot, first token and token count of the sequences that
+ * are walked a token at a time. runs [run_count, 5] int32: the others, 64 tokens at a time, each
+ * in one or several pieces: slot, first token, token count, the piece's place in the workspace (-1
+ * for a sequence in one), and 1 for a sequence's first piece + 2 for its last. The pieces of a
+ * sequence follow one another in the workspace (`pieces` of them in all); the first handed_on runs
+ * are those that are not a last piece, and chains [chain_count, 2] names the sequences of three or
+ * more: their first place and how many. No slot may be named twice; an entry outside the states,
+ * the tokens or the workspace is skipped. workspace: at least
+ * omnia_linear_attention_workspace_bytes, 16-byte aligned (null where that is 0).
  * Its input is what omnia_gate_softplus gives (models/qwen3_5/layers/deltanet.py:222-224);
  * the single-token recurrence stands where core/kernels/ssm does.
  * key_dim, value_dim 64 or 128; heads a multiple of key_heads, at most 4096. */
@@ -835,12 +843,16 @@ typedef struct {
   const uint16_t *queries, *keys, *values;
   const float *log_decay, *strengths;
   float* states;
-  const int32_t* steps;
+  const int32_t *steps, *runs, *chains;
   uint16_t* out;
-  int64_t query_stride, key_stride, value_stride, decay_stride, strength_stride;
-  int64_t slots, tokens, heads, key_heads, key_dim, value_dim, step_count;
+  void* workspace;
+  int64_t workspace_bytes, query_stride, key_stride, value_stride, decay_stride, strength_stride;
+  int64_t slots, tokens, heads, key_heads, key_dim, value_dim;
+  int64_t step_count, run_count, handed_on, chain_count, pieces;
   float scale;
 } omnia_linear_attention_t;
+int64_t omnia_linear_attention_workspace_bytes(int64_t heads, int64_t key_dim, int64_t value_dim,
+                                               int64_t pieces);
 int32_t omnia_linear_attention(const omnia_linear_attention_t* call, hipStream_t stream);
 
 /* RMSNorm of a mixer's output in groups, with its gate:

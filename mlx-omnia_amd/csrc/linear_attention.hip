@@ -6,6 +6,10 @@
 // Steps: a workgroup takes one head of one sequence with its whole state in registers (64 KB at
 // 128 x 128, 16 vectors of 16 bytes a lane, all asked for at once), so a step of one token reads
 // and writes the state once and is bound by that.
+//
+// Prompts: a workgroup takes one head of one piece of a sequence, 64 tokens at a time on the matrix
+// unit. Where the sequences are too few to fill the card each is cut into pieces: the pieces' own
+// parts of the state first (k and v alone), then the states ahead of each, then the pieces' contexts.
 #include "common.hpp"
 #include "host.hpp"
 
@@ -16,10 +20,11 @@ struct LinearArgs {
   const uint16_t *q, *k, *v;
   const float *decay, *strength;
   float* states;
-  const int32_t* steps;
+  const int32_t *steps, *runs, *chains;
   uint16_t* out;
+  float *carried, *totals;   // the workspace: states ahead of pieces, and pieces' log2 decays
   int64_t q_stride, k_stride, v_stride, decay_stride, strength_stride;
-  int slots, tokens, heads, group;
+  int slots, tokens, heads, group, pieces;
   float scale;
 };
 
@@ -92,8 +97,348 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
   for (int i = 0; i < kPasses; ++i) *reinterpret_cast<f32x4*>(state + i * kRows * DV) = s[i];
 }
 
+// ---- prompts: 64 tokens at a time ---------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4_lds __attribute__((ext_vector_type(4)));
+
+constexpr int kChunk = 64;
+constexpr double kLog2e = 1.4426950408889634074;
+
+// Where 16-byte piece `piece` of row `row` lies in its row of a tile of D columns: rows of one
+// piece (the products' operands) and four rows of one 64-byte group (the transposed reads) touch
+// every bank once.
+template <int D>
+__device__ __forceinline__ int turn_of(int row) {
+  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
+}
+
+// Eight fp32 numbers as bf16 operands of the matrix unit: the top halves, cut off (`x` keeps what
+// is left of each, exactly).
+__device__ __forceinline__ s16x8 cut(float (&x)[8]) {
+  u32x4 part;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x0 = __float_as_uint(x[2 * j]), x1 = __float_as_uint(x[2 * j + 1]);
+    part[j] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+    x[2 * j] -= __uint_as_float(x0 & 0xffff0000u);
+    x[2 * j + 1] -= __uint_as_float(x1 & 0xffff0000u);
+  }
+  return __builtin_bit_cast(s16x8, part);
+}
+
+__device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ double prefix_sum(double value, int lane) {
+#pragma unroll
+  for (int step = 1; step < kWave; step *= 2) {
+    const double before = __shfl_up(value, step, kWave);
+    value += lane >= step ? before : 0.0;
+  }
+  return value;
+}
+
+// A piece of a sequence, for one head: a wave holds 32 columns of the state in the matrix unit's
+// accumulators over all of the piece's chunks, lane (half, c) its column c and of each 32 rows the
+// rows 8 i + 4 half + 0..3. In a chunk, with G the sums of g up to a token in it:
+//   P[t, s] = exp(G_t - G_s) w_s (q_t . k_s), s <= t              each 32 x 32 of it by one wave
+//   o_t = scale (exp(G_t) q_t S + P v),   S' = exp(G_end) S + k^T (exp(G_end - G_s) w_s v_s)
+// The accumulators' order of rows is that of the products' operands over 16 rows: S is an operand
+// of q S, and the columns of P that a wave has made one of P v, as they are. S enters its product
+// as two bf16 parts (16 bits; the result is rounded to 8), P as two, the scaled v, whose sums the
+// state keeps, as three, which hold all of its 24 bits. G is summed in fp64 and held in two floats: its
+// differences are what counts, and a fast decay ahead of a slow one would swallow them.
+// kOutputs false leaves out q, P and the context: the piece's own part of the state, for the
+// pieces behind it.
+template <int DK, int DV, bool kOutputs>
+__global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
+  constexpr int kWaves = DV / 32, kThreads = 64 * kWaves;
+  constexpr int kTiles = DK / 32, kSteps = DK / 16;
+  constexpr int kKeyPieces = DK / 8, kValuePieces = DV / 8;
+  __shared__ __attribute__((aligned(16))) uint16_t tile_q[kOutputs ? kChunk * DK : 8];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_k[kChunk * DK];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * DV];
+  __shared__ u32x4 weights[kOutputs ? 2 : 1][kOutputs ? 6 : 1][kWave];   // P^T: parts, (t tile, 16 s), lanes
+  __shared__ __attribute__((aligned(16))) float sum_hi[kChunk], sum_lo[kChunk], strength[kChunk], left[kChunk], rate[kChunk];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int half = lane / 32, column = lane % 32;
+  const int entry = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+  const int32_t* run = a.runs + 5 * entry;
+  const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
+  if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < -1 ||
+      in + ((kind & 2) == 0) >= a.pieces || (in < 0 && kind != 3) || (!kOutputs && (kind & 2) != 0)) {
+    return;
+  }
+  const int shared = head / a.group;
+  constexpr int64_t kState = DK * DV;
+  const int64_t state_at = (static_cast<int64_t>(slot) * a.heads + head) * kState;
+  float* carried = a.carried + (static_cast<int64_t>(in < 0 ? 0 : in) * a.heads + head) * kState;
+  const int64_t mine = 4 * half * DV + 32 * wave + column;   // this lane's first row and its column
+
+  f32x16 s[kTiles];
+  {
+    const float* from = kOutputs ? (in < 0 ? a.states + state_at : carried) : a.states + state_at;
+    const bool zero = !kOutputs && (kind & 1) == 0;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t at = mine + (32 * i + 8 * (e / 4) + e % 4) * DV;
+        s[i][e] = zero ? 0.0f : from[at];
+        if (!kOutputs && !zero) carried[at] = s[i][e];   // what the first piece's context starts from
+      }
+    }
+  }
+  double total = 0.0;   // of the piece's log2 decays (the first wave's)
+
+  // Where this lane reads: rows `column` of a piece, and transposed, rows 4 half + sub / 4 (+ 8).
+  const int sub = lane % 16;
+  const int turned_k = turn_of<DK>(column), turned_rows = turn_of<DK>(4 * half + sub / 4);
+  const int turned_v = turn_of<DV>(4 * half + sub / 4);
+  const int piece = 2 * (lane / 16 % 2) + (sub % 4) / 2;
+  const int row_k = (4 * half + sub / 4) * DK + (sub % 2) * 4, row_v = (4 * half + sub / 4) * DV + (sub % 2) * 4;
+  typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
+  auto transposed = [&](const uint16_t* tile, int width, int row_at, int block, int turn, int step) {
+    const uint16_t* at = tile + row_at + step * 16 * width;
+    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + ((block * 4 + piece) ^ turn) * 8));
+    const s16x4_lds high =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * width + ((block * 4 + piece) ^ turn ^ 2) * 8));
+    return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  for (int chunk = 0; chunk < count; chunk += kChunk) {
+    const int64_t token0 = first + chunk;
+    const int tokens = min(kChunk, count - chunk);
+    // Rows past the last are zeros: they add nothing to the state, and nobody reads their context.
+    for (int i = threadIdx.x; i < kChunk * kKeyPieces; i += kThreads) {
+      const int row = i / kKeyPieces, at = i % kKeyPieces;
+      const int64_t offset = (token0 + min(row, tokens - 1));
+      u32x4 kv = *reinterpret_cast<const u32x4*>(a.k + offset * a.k_stride + shared * DK + at * 8);
+      if (row >= tokens) kv = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(tile_k + row * DK + (at ^ turn_of<DK>(row)) * 8) = kv;
+      if constexpr (kOutputs) {
+        // q's columns in the operands' order: 16-byte piece 2 s + h has columns 16 s + 4 h + 0..3 and those 8 on.
+        const u32x4 qv = *reinterpret_cast<const u32x4*>(a.q + offset * a.q_stride + shared * DK + at * 8);
+        uint16_t* to = tile_q + row * DK + (at % 2) * 4;
+        const int turn = turn_of<DK>(row);
+        *reinterpret_cast<uint2*>(to + (((at & ~1) + 0) ^ turn) * 8) = make_uint2(qv.x, qv.y);
+        *reinterpret_cast<uint2*>(to + (((at & ~1) + 1) ^ turn) * 8) = make_uint2(qv.z, qv.w);
+      }
+    }
+    for (int i = threadIdx.x; i < kChunk * kValuePieces; i += kThreads) {
+      const int row = i / kValuePieces, at = i % kValuePieces;
+      u32x4 vv = *reinterpret_cast<const u32x4*>(a.v + (token0 + min(row, tokens - 1)) * a.v_stride + head * DV + at * 8);
+      if (row >= tokens) vv = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(tile_v + row * DV + (at ^ turn_of<DV>(row)) * 8) = vv;
+    }
+    if (wave == 0) {
+      const bool there = lane < tokens;
+      const int64_t token = token0 + min(lane, tokens - 1);
+      const float g = there ? a.decay[token * a.decay_stride + head] : 0.0f;
+      const float w = a.strength != nullptr ? a.strength[token * a.strength_stride + head] : 1.0f;
+      // A decay past 2^-512 leaves nothing of 32 bits, as that does; sums of -inf would differ by NaN.
+      const double log2 = g < -354.0f ? -512.0 : g * kLog2e;
+      const double sum = prefix_sum(log2, lane);
+      const double end = __shfl(sum, kWave - 1, kWave);
+      total += end;
+      const float hi = static_cast<float>(sum);
+      sum_hi[lane] = hi;
+      sum_lo[lane] = static_cast<float>(sum - hi);
+      strength[lane] = w * a.scale;
+      left[lane] = __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w;
+      rate[lane] = static_cast<float>(log2);
+    }
+    lds_barrier();
+
+    f32x16 o[2] = {f32x16{}, f32x16{}};
+    if constexpr (kOutputs) {
+      // P^T of 32 tokens t by 32 s: (0, 0) and (1, 1) by the waves 0 and 1, (1, 0) by the last.
+      for (int tile = wave; tile < 3; tile += kWaves) {
+        const int tt = tile == 0 ? 0 : 1, ts = tile == 1 ? 1 : 0;
+        const uint16_t* rows_q = tile_q + (32 * tt + column) * DK;
+        const uint16_t* rows_k = tile_k + (32 * ts + column) * DK + 4 * half;
+        f32x16 p = f32x16{};
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          const s16x8 qf = *reinterpret_cast<const s16x8*>(rows_q + ((2 * step + half) ^ turned_k) * 8);
+          const s16x4 k0 = *reinterpret_cast<const s16x4*>(rows_k + ((2 * step) ^ turned_k) * 8);
+          const s16x4 k1 = *reinterpret_cast<const s16x4*>(rows_k + ((2 * step + 1) ^ turned_k) * 8);
+          p = product(__builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7), qf, p);
+        }
+        const int t = 32 * tt + column;
+        const float hi = sum_hi[t], lo = sum_lo[t];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = 32 * ts + 16 * j + 8 * (e / 4) + 4 * half + e % 4;
+            const float apart = (hi - sum_hi[at]) + (lo - sum_lo[at]);
+            // Chosen, not multiplied by zero: a later token's key may not be finite.
+            x[e] = at <= t ? p[8 * j + e] * (__builtin_amdgcn_exp2f(apart) * strength[at]) : 0.0f;
+          }
+          const int frag = (tt == 0 ? 0 : 2) + 2 * ts + j;
+          weights[0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
+          weights[1][frag][lane] = pack8(x);
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
+        const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const s16x8 qf =
+              *reinterpret_cast<const s16x8*>(tile_q + (32 * tt + column) * DK + ((2 * step + half) ^ turned_k) * 8);
+          o[tt] = product(high, qf, o[tt]);
+          o[tt] = product(low, qf, o[tt]);
+        }
+      }
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        o[tt] *= __builtin_amdgcn_exp2f(sum_hi[32 * tt + column] + sum_lo[32 * tt + column]) * a.scale;
+      }
+    }
+    s16x8 values[4];
+    float odd = 0.0f;
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      values[step] = transposed(tile_v, DV, row_v, wave, turned_v, step);
+      const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
+    }
+    if constexpr (kOutputs) {
+      lds_barrier();
+      if (__ballot(odd != odd) != 0) {
+        // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
+        for (int t = 0; t < tokens; ++t) {
+          const float keep = __builtin_amdgcn_exp2f(rate[t]);
+          const int at_v = 32 * wave + column;
+          const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
+          const float v = w * bf16_to_f32(tile_v[t * DV + ((at_v / 8) ^ turn_of<DV>(t)) * 8 + at_v % 8]);
+          const int turn = turn_of<DK>(t);
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const int row = 32 * i + 8 * (e / 4) + 4 * half;   // and the three behind
+              const uint16_t* kr = tile_k + t * DK + ((row / 8) ^ turn) * 8 + 4 * half;
+              // Row `row` of q's column order: piece 2 (row / 16) + half, its second four from row 8 of 16 on.
+              const uint16_t* qr = tile_q + t * DK + ((2 * (row / 16) + half) ^ turn) * 8 + 4 * (row / 8 % 2);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                s[i][e + j] = __builtin_fmaf(bf16_to_f32(kr[j]), v, s[i][e + j] * keep);
+                sum = __builtin_fmaf(bf16_to_f32(qr[j]), s[i][e + j], sum);
+              }
+            }
+          }
+          uint32_t low, high;
+          half_pair(__float_as_uint(sum), low, high);
+          sum = __uint_as_float(low) + __uint_as_float(high);
+          if (half == 0) a.out[((token0 + t) * a.heads + head) * DV + at_v] = f32_to_bf16(sum * a.scale);
+        }
+        lds_barrier();
+        continue;
+      }
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int step = 0; step < 2 + 2 * tt; ++step) {
+          const int frag = 2 * tt + step;
+          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[0][frag][lane]), o[tt]);
+          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[1][frag][lane]), o[tt]);
+        }
+        const int t = 32 * tt + column;
+        if (t < tokens) {
+          uint16_t* to = a.out + ((token0 + t) * a.heads + head) * DV + 32 * wave + 4 * half;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint2 packed;
+            packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
+            packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
+            *reinterpret_cast<uint2*>(to + 8 * i) = packed;
+          }
+        }
+      }
+    }
+    const float keep = __builtin_amdgcn_exp2f(sum_hi[kChunk - 1] + sum_lo[kChunk - 1]);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) s[i] *= keep;
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      float x[8];
+      unpack8(__builtin_bit_cast(u32x4, values[step]), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= left[16 * step + 8 * (e / 4) + 4 * half + e % 4];
+      const s16x8 v0 = cut(x), v1 = cut(x), v2 = cut(x);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        const s16x8 kt = transposed(tile_k, DK, row_k, i, turned_rows, step);
+        s[i] = product(kt, v0, s[i]);
+        s[i] = product(kt, v1, s[i]);
+        s[i] = product(kt, v2, s[i]);
+      }
+    }
+    lds_barrier();
+  }
+  if (kOutputs && (kind & 2) == 0) return;
+  float* to = kOutputs ? a.states + state_at : carried + a.heads * kState;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) to[mine + (32 * i + 8 * (e / 4) + e % 4) * DV] = s[i][e];
+  }
+  if (!kOutputs && threadIdx.x == 0) a.totals[static_cast<int64_t>(in + 1) * a.heads + head] = static_cast<float>(total);
+}
+
+// The states ahead of a sequence's third piece on, from what each piece before added:
+// X_p = 2^total X_{p-1} + U_p, in place.
+__global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int state) {
+  const int per_head = state / (256 * 4);   // workgroups
+  const int part = blockIdx.x % per_head;
+  const int head = blockIdx.x / per_head % a.heads, chain = blockIdx.x / per_head / a.heads;
+  const int at = a.chains[2 * chain], count = a.chains[2 * chain + 1];
+  if (at < 0 || count < 3 || count > a.pieces - at) return;
+  const int64_t between = static_cast<int64_t>(a.heads) * state;
+  float* x = a.carried + (static_cast<int64_t>(at + 1) * a.heads + head) * state + (part * 256 + threadIdx.x) * 4;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(x);
+#pragma unroll 4
+  for (int p = 2; p < count; ++p) {
+    x += between;
+    const float keep = __builtin_amdgcn_exp2f(a.totals[static_cast<int64_t>(at + p) * a.heads + head]);
+    const f32x4 own = *reinterpret_cast<const f32x4*>(x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(sum[j], keep, own[j]);
+    *reinterpret_cast<f32x4*>(x) = sum;
+  }
+}
+
+template <int DK, int DV>
+void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
+  const auto grid = [&](int64_t blocks) { return dim3(static_cast<unsigned>(blocks * a.heads)); };
+  if (steps > 0) linear_step_kernel<DK, DV><<<grid(steps), 256, 0, stream>>>(a);
+  if (handed_on > 0) linear_chunk_kernel<DK, DV, false><<<grid(handed_on), 2 * DV, 0, stream>>>(a);
+  if (chains > 0) linear_carry_kernel<<<grid(chains * (DK * DV / 1024)), 256, 0, stream>>>(a, DK * DV);
+  if (runs > 0) linear_chunk_kernel<DK, DV, true><<<grid(runs), 2 * DV, 0, stream>>>(a);
+}
+
 }  // namespace
 }  // namespace omnia
+
+extern "C" int64_t omnia_linear_attention_workspace_bytes(int64_t heads, int64_t key_dim, int64_t value_dim, int64_t pieces) {
+  if (heads <= 0 || heads > 4096 || (key_dim != 64 && key_dim != 128) || (value_dim != 64 && value_dim != 128) ||
+      pieces < 0 || pieces >= (int64_t{1} << 24)) {
+    return -EINVAL;
+  }
+  return pieces * heads * (key_dim * value_dim + 1) * static_cast<int64_t>(sizeof(float));
+}
 
 extern "C" int32_t omnia_linear_attention(const omnia_linear_attention_t* c, hipStream_t stream) {
   using namespace omnia;
@@ -103,34 +448,43 @@ extern "C" int32_t omnia_linear_attention(const omnia_linear_attention_t* c, hip
   OMNIA_REQUIRE(c->key_heads > 0 && c->heads > 0 && c->heads <= 4096 && c->heads % c->key_heads == 0,
                 "linear_attention: heads must be a multiple of key_heads");
   constexpr int64_t kMost = int64_t{1} << 24;
-  OMNIA_REQUIRE(c->tokens >= 0 && c->tokens < kMost && c->step_count >= 0 && c->step_count <= c->tokens &&
-                    c->slots >= 0 && c->slots < kMost,
-                "linear_attention: bad token, step or slot count");
-  if (c->step_count == 0) return 0;
-  OMNIA_REQUIRE(c->queries && c->keys && c->values && c->log_decay && c->states && c->steps && c->out,
+  OMNIA_REQUIRE(c->tokens >= 0 && c->tokens < kMost && c->slots >= 0 && c->slots < kMost && c->step_count >= 0 &&
+                    c->run_count >= 0 && c->step_count + c->run_count <= c->tokens,
+                "linear_attention: bad token, slot, step or run count");
+  OMNIA_REQUIRE(c->handed_on >= 0 && c->handed_on <= c->run_count && c->chain_count >= 0 && c->chain_count <= c->handed_on &&
+                    c->pieces >= c->handed_on && c->pieces <= c->run_count,
+                "linear_attention: bad piece or chain count");
+  if (c->step_count + c->run_count == 0) return 0;
+  OMNIA_REQUIRE(c->queries && c->keys && c->values && c->log_decay && c->states && c->out &&
+                    (c->steps || c->step_count == 0) && (c->runs || c->run_count == 0) && (c->chains || c->chain_count == 0),
                 "linear_attention: null pointer");
   OMNIA_REQUIRE(aligned16(c->queries) && aligned16(c->keys) && aligned16(c->values) && aligned16(c->states) &&
                     aligned16(c->out),
                 "linear_attention: pointers must be 16-byte aligned");
   OMNIA_REQUIRE(c->query_stride % 8 == 0 && c->key_stride % 8 == 0 && c->value_stride % 8 == 0 &&
                     c->query_stride >= c->key_heads * c->key_dim && c->key_stride >= c->key_heads * c->key_dim &&
-                    c->value_stride >= c->heads * c->value_dim && c->query_stride < kMost && c->key_stride < kMost &&
-                    c->value_stride < kMost,
-                "linear_attention: row strides must be multiples of 8 covering the heads, below 2^24");
+                    c->value_stride >= c->heads * c->value_dim,
+                "linear_attention: row strides must be multiples of 8 covering the heads");
   OMNIA_REQUIRE((c->decay_stride == 0 || c->decay_stride >= c->heads) &&
                     (c->strengths == nullptr || c->strength_stride >= c->heads),
                 "linear_attention: decay and strength rows must cover the heads");
-  const int64_t blocks = c->step_count * c->heads;
-  OMNIA_REQUIRE(blocks < (int64_t{1} << 31), "linear_attention: too many steps");
+  const int64_t need = omnia_linear_attention_workspace_bytes(c->heads, c->key_dim, c->value_dim, c->pieces);
+  OMNIA_REQUIRE(need == 0 || (c->workspace && c->workspace_bytes >= need && aligned16(c->workspace)),
+                "linear_attention: workspace too small (omnia_linear_attention_workspace_bytes) or not aligned");
+  constexpr int64_t kBlocks = int64_t{1} << 31;
+  OMNIA_REQUIRE(c->step_count * c->heads < kBlocks && c->run_count * c->heads < kBlocks &&
+                    c->chain_count * c->heads * 16 < kBlocks,
+                "linear_attention: too many steps or runs");
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
-  const LinearArgs a{c->queries, c->keys, c->values, c->log_decay, c->strengths, c->states, c->steps, c->out,
+  float* carried = static_cast<float*>(c->workspace);
+  const LinearArgs a{c->queries, c->keys, c->values, c->log_decay, c->strengths, c->states, c->steps, c->runs, c->chains,
+                     c->out, carried, carried + c->pieces * c->heads * c->key_dim * c->value_dim,
                      c->query_stride, c->key_stride, c->value_stride, c->decay_stride, c->strength_stride,
                      static_cast<int>(c->slots), static_cast<int>(c->tokens), static_cast<int>(c->heads),
-                     static_cast<int>(c->heads / c->key_heads), c->scale};
-  const auto kernel = c->key_dim == 64
-                          ? (c->value_dim == 64 ? linear_step_kernel<64, 64> : linear_step_kernel<64, 128>)
-                          : (c->value_dim == 64 ? linear_step_kernel<128, 64> : linear_step_kernel<128, 128>);
-  kernel<<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
+                     static_cast<int>(c->heads / c->key_heads), static_cast<int>(c->pieces), c->scale};
+  const auto launch = c->key_dim == 64 ? (c->value_dim == 64 ? launch_linear<64, 64> : launch_linear<64, 128>)
+                                       : (c->value_dim == 64 ? launch_linear<128, 64> : launch_linear<128, 128>);
+  launch(a, c->step_count, c->run_count, c->handed_on, c->chain_count, stream);
   return launched("linear_attention");
 }

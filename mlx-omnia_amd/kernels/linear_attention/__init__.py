@@ -46,7 +46,10 @@ __all__ = ["DefaultLinearAttention", "HipLinearAttention", "LinearAttention", "L
            "LinearBatch", "applies"]
 
 DIMS = (64, 128)
-CHUNK = 64   # tokens that the Core chain takes together
+CHUNK = 64         # tokens that the kernels and the Core chain take together
+STEP_TOKENS = 4    # up to which a sequence is walked a token at a time
+BLOCKS = 512       # workgroups that a call's chunks are cut into, where they give as many
+MIN_PIECE = 4      # chunks of a piece, about
 
 
 class LinearBatch:
@@ -67,18 +70,39 @@ class LinearBatch:
             raise ValueError(f"LinearBatch: {self.total} tokens, of at most {(1 << 24) - 1}")
         self.device = torch.device(device)
         self.plans: dict = {}   # what a layer's binding laid out for the batch
-        self._steps: torch.Tensor | None = None
+        self._lists: dict[int, ops.LinearLists] = {}
 
-    def steps(self) -> torch.Tensor:
-        """[n, 3] int32 on the device: slot, first token and count of every sequence with new tokens."""
-        if self._steps is None:
+    def lists(self, heads: int) -> ops.LinearLists:
+        """What a layer of so many heads does with each sequence, on the device: a token at a time, or
+        in one or several pieces (`omnia_linear_attention`'s steps, runs and chains)."""
+        held = self._lists.get(heads)
+        if held is None:
             if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise ValueError("a batch's first call cannot be captured: make one before")
-            counts = np.asarray(self.tokens, dtype=np.int64)
-            rows = np.stack([np.asarray(self.slots, dtype=np.int64), np.cumsum(counts) - counts, counts], axis=1)
-            rows = np.ascontiguousarray(rows[counts > 0], dtype=np.int32).reshape(-1, 3)
-            self._steps = torch.from_numpy(rows).to(self.device)
-        return self._steps
+            firsts = np.cumsum(self.tokens, dtype=np.int64) - np.asarray(self.tokens, dtype=np.int64)
+            steps, handed_on, last, chains, pieces = [], [], [], [], 0
+            chunks = sum(-(-n // CHUNK) for n in self.tokens if n > STEP_TOKENS)
+            longest = max(MIN_PIECE, -(-chunks * heads // BLOCKS))   # chunks of a piece, about
+            for slot, first, count in zip(self.slots, firsts.tolist(), self.tokens):
+                if count <= STEP_TOKENS:
+                    steps += [(slot, first, count)] if count else []
+                    continue
+                own = -(-count // CHUNK)
+                cut = max(1, round(own / longest))
+                size = -(-own // cut) * CHUNK
+                cut = -(-count // size)
+                for i in range(cut):
+                    at, rest = first + i * size, count - i * size
+                    (last if i == cut - 1 else handed_on).append(
+                        (slot, at, min(size, rest), pieces + i if cut > 1 else -1, (i == 0) + 2 * (i == cut - 1)))
+                if cut > 2:
+                    chains.append((pieces, cut))
+                pieces += cut if cut > 1 else 0
+            # The longest first: what is left at the end is short.
+            for runs in (handed_on, last):
+                runs.sort(key=lambda run: -run[2])
+            held = self._lists[heads] = ops.LinearLists.of(steps, handed_on, last, chains, pieces, self.device)
+        return held
 
 
 @runtime_checkable
@@ -168,7 +192,7 @@ class HipLinearAttention(LinearAttentionStrategy):
             return core(batch, queries, keys, values, log_decay, strengths)
         plan, at = batch.plans.get(self, (None, None))
         if plan is None or at != core.states.data_ptr():   # a pool that was given other memory
-            plan, at = ops.LinearAttentionPlan(core.states, batch.steps(), batch.total, key_heads=core.key_heads,
+            plan, at = ops.LinearAttentionPlan(core.states, batch.lists(core.heads), batch.total, key_heads=core.key_heads,
                                                scale=core.scale), core.states.data_ptr()
             batch.plans[self] = plan, at
         return plan(queries, keys, values, gates, strengths)

@@ -46,10 +46,12 @@ class PagedCache(ctypes.Structure):
 class LinearAttentionCall(ctypes.Structure):
     """`omnia_linear_attention_t`; must match include/omnia_hip.h."""
 
-    _fields_ = ([(name, _P) for name in ("queries", "keys", "values", "log_decay", "strengths", "states", "steps", "out")]
+    _fields_ = ([(name, _P) for name in ("queries", "keys", "values", "log_decay", "strengths", "states", "steps", "runs",
+                                         "chains", "out", "workspace")]
                 + [(name, _I64) for name in (
-                    "query_stride", "key_stride", "value_stride", "decay_stride", "strength_stride", "slots", "tokens",
-                    "heads", "key_heads", "key_dim", "value_dim", "step_count")]
+                    "workspace_bytes", "query_stride", "key_stride", "value_stride", "decay_stride", "strength_stride", "slots", "tokens",
+                    "heads", "key_heads", "key_dim", "value_dim", "step_count", "run_count", "handed_on", "chain_count",
+                    "pieces")]
                 + [("scale", _F32)])
 
 
@@ -146,6 +148,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                      _I64, _I64, _I64, _I64, _I64, _P, _F32, _P, _I64, _P, _P]),
     "omnia_attention_batch_step_bytes": (_I64, [_I64] * 8),
     "omnia_attention_batch_step": (_I32, [_P, _P]),
+    "omnia_linear_attention_workspace_bytes": (_I64, [_I64] * 4),
     "omnia_linear_attention": (_I32, [_P, _P]),
     "omnia_gated_rms_norm": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F32, _I32, _I32, _P, _P]),
     "omnia_block_norm": (_I32, [_P, _P, _P, _I64, _I32, _P, _F32, _P, _F32, _F32, _F32, _I64, _I64, _P, _P, _P]),

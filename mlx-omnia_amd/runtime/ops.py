@@ -1843,25 +1843,49 @@ def moe_down_combine_nvfp4_shared(
     return out
 
 
+@dataclass(frozen=True)
+class LinearLists:
+    """What `omnia_linear_attention` does with a batch's sequences: int32 lists on the device, steps
+    [n, 3], runs [n, 5] of which the first `handed_on` are no last pieces, chains [n, 2], and the
+    places that the pieces take in the workspace."""
+
+    steps: torch.Tensor
+    runs: torch.Tensor
+    chains: torch.Tensor
+    handed_on: int
+    pieces: int
+
+    @classmethod
+    def of(cls, steps, handed_on, last, chains, pieces: int, device) -> "LinearLists":
+        flat = [x for rows in (steps, handed_on, last, chains) for row in rows for x in row]
+        held = torch.tensor(flat, dtype=torch.int32).to(device)
+        counts = 3 * len(steps), 5 * (len(handed_on) + len(last)), 2 * len(chains)
+        parts = held.split(counts)
+        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces)
+
+
 class LinearAttentionPlan:
     """A layer's linear attention over one batch, its arguments checked and laid out once for
     `omnia_linear_attention`: what stays the same from call to call. states [slots, heads,
-    key_dim, value_dim] fp32, steps [n, 3] int32 (slot, first token, count) on their device.
+    key_dim, value_dim] fp32, the batch's lists on their device.
     Calling it with the tokens' rows gives the context [tokens, heads, value_dim] bf16. Its
     addresses are those of when it was made."""
 
-    def __init__(self, states: torch.Tensor, steps: torch.Tensor, tokens: int, *, key_heads: int, scale: float) -> None:
+    def __init__(self, states: torch.Tensor, lists: LinearLists, tokens: int, *, key_heads: int, scale: float) -> None:
         _dense(states, F32, "states")
         _require(states.dim() == 4, "linear_attention: states must be [slots, heads, key_dim, value_dim]")
-        _require(steps.dtype == torch.int32 and steps.is_contiguous() and steps.dim() == 2 and steps.shape[1] == 3,
-                 "linear_attention: steps must be contiguous int32 [n, 3]")
-        _require(on_rocm(states, steps), "linear_attention: tensors must share one ROCm device")
+        _require(on_rocm(states, lists.steps), "linear_attention: tensors must share one ROCm device")
         slots, heads, key_dim, value_dim = states.shape
-        self.held, self.index, self.device = (states.detach(), steps), states.get_device(), states.device
+        self.held, self.index, self.device = (states.detach(), lists), states.get_device(), states.device
         self.shapes = (tokens, key_heads, key_dim), (tokens, heads, value_dim), (tokens, heads)
         self.args = LinearAttentionCall(
-            states=states.data_ptr(), steps=steps.data_ptr(), slots=slots, tokens=tokens, heads=heads,
-            key_heads=key_heads, key_dim=key_dim, value_dim=value_dim, step_count=steps.shape[0], scale=scale)
+            states=states.data_ptr(), steps=lists.steps.data_ptr(), runs=lists.runs.data_ptr(),
+            chains=lists.chains.data_ptr(), slots=slots, tokens=tokens, heads=heads, key_heads=key_heads, key_dim=key_dim,
+            value_dim=value_dim, step_count=lists.steps.shape[0], run_count=lists.runs.shape[0],
+            handed_on=lists.handed_on, chain_count=lists.chains.shape[0], pieces=lists.pieces, scale=scale)
+        nbytes = library().omnia_linear_attention_workspace_bytes(heads, key_dim, value_dim, lists.pieces)
+        _require(nbytes >= 0, "linear_attention: geometry not served")
+        self.args.workspace_bytes = nbytes
         self.like = torch.empty(1, dtype=BF16, device=states.device).expand(self.shapes[1])
 
     def _rows(self, rows: torch.Tensor, shape: tuple[int, int, int], name: str) -> tuple[int, int, torch.Tensor]:
@@ -1905,6 +1929,9 @@ class LinearAttentionPlan:
             args.strengths, args.strength_stride, strengths = self._gates(strengths, "strengths")
         out = torch.empty_like(self.like, memory_format=torch.contiguous_format)
         args.out = out.data_ptr()
+        if args.workspace_bytes:
+            workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=self.device)
+            args.workspace = workspace.data_ptr()
         call("omnia_linear_attention", ctypes.addressof(args), _stream_here(self.index))
         del q, k, v, g, strengths   # held until here
         return out

@@ -84,9 +84,45 @@ def test_a_batch_refuses():
     for slots, tokens in (([0, 0], [1, 1]), ([0], [1, 2]), ([-1], [1]), ([0], [-1]), ([0], [1 << 24])):
         with pytest.raises(ValueError):
             LinearBatch(slots, tokens, device="cpu")
+
+
+def test_lists_cover_every_token_once():
+    """Whatever the lengths and heads: each token in one step or piece, pieces of a sequence in order,
+    of whole chunks but the last, and their places one behind the other."""
+    gen = torch.Generator().manual_seed(3)
+    for trial in range(60):
+        count = int(torch.randint(0, 12, (1,), generator=gen))
+        tokens = [int(2 ** (14 * float(torch.rand(1, generator=gen)))) - 1 for _ in range(count)]
+        slots = torch.randperm(count + 3, generator=gen).tolist()[:count]
+        heads = (1, 4, 32, 64)[trial % 4]
+        batch = LinearBatch(slots, tokens, device="cpu")
+        lists = batch.lists(heads)
+        assert lists is batch.lists(heads)
+        seen, places = torch.zeros(batch.total, dtype=torch.int64), []
+        for slot, first, n in lists.steps.tolist():
+            assert tokens[slots.index(slot)] == n
+            seen[first : first + n] += 1
+        by_slot: dict = {}
+        for i, (slot, first, n, place, kind) in enumerate(lists.runs.tolist()):
+            seen[first : first + n] += 1
+            assert (kind & 2 == 0) == (i < lists.handed_on) and n > 0
+            by_slot.setdefault(slot, []).append((first, n, place, kind))
+        for slot, runs in by_slot.items():
+            runs.sort()
+            assert sum(n for _, n, _, _ in runs) == tokens[slots.index(slot)]
+            assert [kind for *_, kind in runs] == [(i == 0) + 2 * (i == len(runs) - 1) for i in range(len(runs))]
+            assert all(n % 64 == 0 for _, n, _, _ in runs[:-1])
+            if len(runs) == 1:
+                assert runs[0][2] == -1
+            else:
+                assert [p for _, _, p, _ in runs] == list(range(runs[0][2], runs[0][2] + len(runs)))
+                places += [p for _, _, p, _ in runs]
+        assert (seen == 1).all() and sorted(places) == list(range(lists.pieces))
+        assert sorted(lists.chains.tolist()) == sorted(
+            [runs[0][2], len(runs)] for runs in by_slot.values() if len(runs) > 2)
     empty = LinearBatch([], [], device="cpu")
-    assert empty.total == 0 and empty.steps().shape == (0, 3)
-    assert LinearBatch([4, 2, 9], [3, 0, 2], device="cpu").steps().tolist() == [[4, 0, 3], [9, 3, 2]]
+    assert empty.total == 0 and empty.lists(4).steps.shape == (0, 3) and empty.lists(4).runs.shape == (0, 5)
+    assert LinearBatch([4, 2, 9], [3, 0, 2], device="cpu").lists(4).steps.tolist() == [[4, 0, 3], [9, 3, 2]]
 
 
 def test_a_layer_refuses():
