@@ -141,42 +141,142 @@ __device__ __forceinline__ double prefix_sum(double value, int lane) {
   return value;
 }
 
-// A piece of a sequence, for one head: a wave holds 32 columns of the state in the matrix unit's
-// accumulators over all of the piece's chunks, lane (half, c) its column c and of each 32 rows the
-// rows 8 i + 4 half + 0..3. In a chunk, with G the sums of g up to a token in it:
+// 16 bytes a lane from global memory straight to LDS: lane l's come to `to` + 16 l.
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) {
+  typedef __attribute__((address_space(1))) const void* Global;
+  typedef __attribute__((address_space(3))) void* Local;
+  __builtin_amdgcn_global_load_lds((Global)from, (Local)to, 16, 0, 0);
+}
+
+// Brings a chunk's rows of D columns to LDS, with kThreads lanes; each row's 16-byte pieces lie
+// turned (turn_of).
+template <int D, int kThreads>
+struct Rows {
+  static constexpr int kPieces = D / 8;
+  static constexpr int kPass = kThreads / kPieces;               // rows of a pass
+  static constexpr int kTurns = kPass >= 16 ? 1 : 16 / kPass;    // passes whose pieces are turned otherwise
+  static constexpr int kPasses = kChunk / kPass;
+  static_assert(kPass * kPieces == kThreads && kPasses * kPass == kChunk, "whole passes");
+  int64_t stride;
+  int offset[kTurns];   // of this lane's piece in pass i
+  __device__ __forceinline__ Rows(int64_t row_stride) : stride(row_stride) {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int row = threadIdx.x / kPieces + i * kPass;
+      offset[i] = (threadIdx.x / kPieces) * static_cast<int>(stride) + ((threadIdx.x % kPieces) ^ turn_of<D>(row)) * 8;
+    }
+  }
+  // Rows past the last of `tokens` come as the last: their weights are zeros, and where that last row
+  // is not finite, so is all that it meets.
+  __device__ __forceinline__ void ask(const uint16_t* from, int tokens, uint16_t* tile) const {
+    uint16_t* to = tile + threadIdx.x / kWave * kWave * 8;
+    if (tokens == kChunk) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) load_to_lds(from + i * kPass * stride + offset[i % kTurns], to + i * kThreads * 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int row = threadIdx.x / kPieces + i * kPass;
+        const int back = max(row - (tokens - 1), 0) * static_cast<int>(stride);
+        load_to_lds(from + i * kPass * stride + (offset[i % kTurns] - back), to + i * kThreads * 8);
+      }
+    }
+  }
+};
+
+// What a chunk's decays come to: G (in two floats, log2), w * scale, w exp(G_end - G) and g (log2).
+struct Gates {
+  float hi[kChunk], lo[kChunk], strength[kChunk], left[kChunk], rate[kChunk];
+};
+
+// A piece of a sequence, for kHeads heads of a key head: a wave holds 32 columns of a head's state in
+// the matrix unit's accumulators over all of the piece's chunks. In a chunk, with G the sums of g up
+// to a token in it:
 //   P[t, s] = exp(G_t - G_s) w_s (q_t . k_s), s <= t              each 32 x 32 of it by one wave
 //   o_t = scale (exp(G_t) q_t S + P v),   S' = exp(G_end) S + k^T (exp(G_end - G_s) w_s v_s)
-// The accumulators' order of rows is that of the products' operands over 16 rows: S is an operand
-// of q S, and the columns of P that a wave has made one of P v, as they are. S enters its product
-// as two bf16 parts (16 bits; the result is rounded to 8), P as two, the scaled v, whose sums the
-// state keeps, as three, which hold all of its 24 bits. G is summed in fp64 and held in two floats: its
-// differences are what counts, and a fast decay ahead of a slow one would swallow them.
+// The accumulators' order of rows is that of the products' operands over 16 rows once the state's
+// rows are numbered 16 j + 8 half + 0..7 (lane (half, c) holds its column c of those), for which k is
+// transposed in that order: S is an operand of q S, and the columns of P that a wave has made one of
+// P v, as they are. S enters its product as two bf16 parts (16 bits; the result is rounded to 8), P as
+// two, the scaled v, whose sums the state keeps, as three, which hold all of its 24 bits. G is summed
+// in fp64 and held in two floats: its differences are what counts, and a fast decay ahead of a slow
+// one would swallow them.
+// The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
+// tiles, q and v, which are done with after the first half, to the same. Its decays are summed by the
+// wave that has no part of P.
 // kOutputs false leaves out q, P and the context: the piece's own part of the state, for the
 // pieces behind it.
-template <int DK, int DV, bool kOutputs>
-__global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
-  constexpr int kWaves = DV / 32, kThreads = 64 * kWaves;
+template <int DK, int DV, int kHeads, bool kOutputs>
+__global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(LinearArgs a) {
+  constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
-  constexpr int kKeyPieces = DK / 8, kValuePieces = DV / 8;
   __shared__ __attribute__((aligned(16))) uint16_t tile_q[kOutputs ? kChunk * DK : 8];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_k[kChunk * DK];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * DV];
-  __shared__ u32x4 weights[kOutputs ? 2 : 1][kOutputs ? 6 : 1][kWave];   // P^T: parts, (t tile, 16 s), lanes
-  __shared__ __attribute__((aligned(16))) float sum_hi[kChunk], sum_lo[kChunk], strength[kChunk], left[kChunk], rate[kChunk];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  __shared__ __attribute__((aligned(16))) uint16_t tile_k0[kChunk * DK], tile_k1[kChunk * DK];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * kWidth];
+  __shared__ u32x4 weights[kOutputs ? kHeads : 1][kOutputs ? 2 : 1][kOutputs ? 6 : 1][kWave];   // P^T: parts, (t, 16 s), lanes
+  __shared__ __attribute__((aligned(16))) Gates gates0[kHeads], gates1[kHeads];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane / 32, column = lane % 32;
-  const int entry = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+  const int blocks = a.heads / kHeads;
+  const int entry = blockIdx.x / blocks, head0 = blockIdx.x % blocks * kHeads;
+  const int mine = wave * 32 / DV, head = head0 + mine;   // the wave's
   const int32_t* run = a.runs + 5 * entry;
   const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
   if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < -1 ||
       in + ((kind & 2) == 0) >= a.pieces || (in < 0 && kind != 3) || (!kOutputs && (kind & 2) != 0)) {
     return;
   }
-  const int shared = head / a.group;
+  const int shared = head0 / a.group;
   constexpr int64_t kState = DK * DV;
   const int64_t state_at = (static_cast<int64_t>(slot) * a.heads + head) * kState;
   float* carried = a.carried + (static_cast<int64_t>(in < 0 ? 0 : in) * a.heads + head) * kState;
-  const int64_t mine = 4 * half * DV + 32 * wave + column;   // this lane's first row and its column
+  uint32_t own = 8 * half * DV + 32 * wave % DV + column;   // this lane's first row and its column
+
+  const Rows<DK, kThreads> rows_q(a.q_stride), rows_k(a.k_stride);
+  const Rows<kWidth, kThreads> rows_v(a.v_stride);
+  auto ask = [&](int chunk, uint16_t* tile_k) {
+    const int64_t token = first + chunk;
+    const int tokens = min(kChunk, count - chunk);
+    rows_k.ask(a.k + token * a.k_stride + shared * DK, tokens, tile_k);
+    if constexpr (kOutputs) rows_q.ask(a.q + token * a.q_stride + shared * DK, tokens, tile_q);
+    rows_v.ask(a.v + token * a.v_stride + head0 * DV, tokens, tile_v);
+  };
+  ask(0, tile_k0);
+
+  // The decays of the chunk after next are asked for a chunk ahead of their sums.
+  float ahead_g[kHeads], ahead_w[kHeads];
+  auto ask_gates = [&](int chunk) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const int64_t token = first + min(chunk + lane, count - 1);
+      ahead_g[h] = a.decay[token * a.decay_stride + head0 + h];
+      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + h] : 1.0f;
+    }
+  };
+  double total[kHeads] = {};   // of the piece's log2 decays
+  auto sum_gates = [&](int chunk, Gates* gates) {
+    const bool there = lane < count - chunk;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const float g = ahead_g[h], w = there ? ahead_w[h] : 0.0f;
+      // A decay past 2^-512 leaves nothing of 32 bits, as that does; sums of -inf would differ by NaN.
+      const double log2 = !there ? 0.0 : g < -354.0f ? -512.0 : g * kLog2e;
+      const double sum = prefix_sum(log2, lane);
+      const double end = __shfl(sum, kWave - 1, kWave);
+      total[h] += end;
+      const float hi = static_cast<float>(sum);
+      gates[h].hi[lane] = hi;
+      gates[h].lo[lane] = static_cast<float>(sum - hi);
+      gates[h].strength[lane] = w * a.scale;
+      gates[h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
+      gates[h].rate[lane] = static_cast<float>(log2);
+    }
+  };
+  if (wave == kWaves - 1) {
+    ask_gates(0);
+    sum_gates(0, gates0);
+    ask_gates(kChunk);
+  }
 
   f32x16 s[kTiles];
   {
@@ -186,103 +286,73 @@ __global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
     for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int64_t at = mine + (32 * i + 8 * (e / 4) + e % 4) * DV;
+        const uint32_t at = own + (32 * i + 16 * (e / 8) + e % 8) * DV;
         s[i][e] = zero ? 0.0f : from[at];
         if (!kOutputs && !zero) carried[at] = s[i][e];   // what the first piece's context starts from
       }
     }
   }
-  double total = 0.0;   // of the piece's log2 decays (the first wave's)
 
-  // Where this lane reads: rows `column` of a piece, and transposed, rows 4 half + sub / 4 (+ 8).
+  // Where this lane reads: rows `column` of a piece, and transposed, rows 4 half + sub / 4 (+ 8), the
+  // four columns 4 (sub % 4) of 16, of k those that make the state's order.
   const int sub = lane % 16;
-  const int turned_k = turn_of<DK>(column), turned_rows = turn_of<DK>(4 * half + sub / 4);
-  const int turned_v = turn_of<DV>(4 * half + sub / 4);
-  const int piece = 2 * (lane / 16 % 2) + (sub % 4) / 2;
-  const int row_k = (4 * half + sub / 4) * DK + (sub % 2) * 4, row_v = (4 * half + sub / 4) * DV + (sub % 2) * 4;
+  const int turned = turn_of<DK>(column), turned_k = turn_of<DK>(4 * half + sub / 4);
+  const int turned_v = turn_of<kWidth>(4 * half + sub / 4);
+  const int four = (sub % 2) * 2 + sub % 4 / 2;
+  const int piece_k = 2 * (lane / 16 % 2) + four / 2, piece_v = 2 * (lane / 16 % 2) + sub % 4 / 2;
+  const int row_k = (4 * half + sub / 4) * DK + four % 2 * 4, row_v = (4 * half + sub / 4) * kWidth + sub % 2 * 4;
   typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
-  auto transposed = [&](const uint16_t* tile, int width, int row_at, int block, int turn, int step) {
-    const uint16_t* at = tile + row_at + step * 16 * width;
-    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + ((block * 4 + piece) ^ turn) * 8));
-    const s16x4_lds high =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * width + ((block * 4 + piece) ^ turn ^ 2) * 8));
+  auto transposed = [&](const uint16_t* at, int width, int piece, int turn) {   // of rows at and 8 on
+    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + (piece ^ turn) * 8));
+    const s16x4_lds high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * width + (piece ^ turn ^ 2) * 8));
     return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
   };
 
-  for (int chunk = 0; chunk < count; chunk += kChunk) {
+  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const Gates* all, Gates* next) {
     const int64_t token0 = first + chunk;
     const int tokens = min(kChunk, count - chunk);
-    // Rows past the last are zeros: they add nothing to the state, and nobody reads their context.
-    for (int i = threadIdx.x; i < kChunk * kKeyPieces; i += kThreads) {
-      const int row = i / kKeyPieces, at = i % kKeyPieces;
-      const int64_t offset = (token0 + min(row, tokens - 1));
-      u32x4 kv = *reinterpret_cast<const u32x4*>(a.k + offset * a.k_stride + shared * DK + at * 8);
-      if (row >= tokens) kv = u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(tile_k + row * DK + (at ^ turn_of<DK>(row)) * 8) = kv;
-      if constexpr (kOutputs) {
-        // q's columns in the operands' order: 16-byte piece 2 s + h has columns 16 s + 4 h + 0..3 and those 8 on.
-        const u32x4 qv = *reinterpret_cast<const u32x4*>(a.q + offset * a.q_stride + shared * DK + at * 8);
-        uint16_t* to = tile_q + row * DK + (at % 2) * 4;
-        const int turn = turn_of<DK>(row);
-        *reinterpret_cast<uint2*>(to + (((at & ~1) + 0) ^ turn) * 8) = make_uint2(qv.x, qv.y);
-        *reinterpret_cast<uint2*>(to + (((at & ~1) + 1) ^ turn) * 8) = make_uint2(qv.z, qv.w);
-      }
-    }
-    for (int i = threadIdx.x; i < kChunk * kValuePieces; i += kThreads) {
-      const int row = i / kValuePieces, at = i % kValuePieces;
-      u32x4 vv = *reinterpret_cast<const u32x4*>(a.v + (token0 + min(row, tokens - 1)) * a.v_stride + head * DV + at * 8);
-      if (row >= tokens) vv = u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(tile_v + row * DV + (at ^ turn_of<DV>(row)) * 8) = vv;
-    }
-    if (wave == 0) {
-      const bool there = lane < tokens;
-      const int64_t token = token0 + min(lane, tokens - 1);
-      const float g = there ? a.decay[token * a.decay_stride + head] : 0.0f;
-      const float w = a.strength != nullptr ? a.strength[token * a.strength_stride + head] : 1.0f;
-      // A decay past 2^-512 leaves nothing of 32 bits, as that does; sums of -inf would differ by NaN.
-      const double log2 = g < -354.0f ? -512.0 : g * kLog2e;
-      const double sum = prefix_sum(log2, lane);
-      const double end = __shfl(sum, kWave - 1, kWave);
-      total += end;
-      const float hi = static_cast<float>(sum);
-      sum_hi[lane] = hi;
-      sum_lo[lane] = static_cast<float>(sum - hi);
-      strength[lane] = w * a.scale;
-      left[lane] = __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w;
-      rate[lane] = static_cast<float>(log2);
-    }
+    const bool more = chunk + kChunk < count;
+    const Gates& gates = all[mine];
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this chunk's rows
     lds_barrier();
-
+    if (wave == kWaves - 1 && more) {
+      sum_gates(chunk + kChunk, next);
+      ask_gates(chunk + 2 * kChunk);
+    }
     f32x16 o[2] = {f32x16{}, f32x16{}};
     if constexpr (kOutputs) {
-      // P^T of 32 tokens t by 32 s: (0, 0) and (1, 1) by the waves 0 and 1, (1, 0) by the last.
+      // P^T of 32 tokens t by 32 s: (0, 0), (1, 1) and (1, 0).
       for (int tile = wave; tile < 3; tile += kWaves) {
         const int tt = tile == 0 ? 0 : 1, ts = tile == 1 ? 1 : 0;
-        const uint16_t* rows_q = tile_q + (32 * tt + column) * DK;
-        const uint16_t* rows_k = tile_k + (32 * ts + column) * DK + 4 * half;
+        const uint16_t* at_q = tile_q + (32 * tt + column) * DK;
+        const uint16_t* at_k = tile_k + (32 * ts + column) * DK;
         f32x16 p = f32x16{};
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) {
-          const s16x8 qf = *reinterpret_cast<const s16x8*>(rows_q + ((2 * step + half) ^ turned_k) * 8);
-          const s16x4 k0 = *reinterpret_cast<const s16x4*>(rows_k + ((2 * step) ^ turned_k) * 8);
-          const s16x4 k1 = *reinterpret_cast<const s16x4*>(rows_k + ((2 * step + 1) ^ turned_k) * 8);
-          p = product(__builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7), qf, p);
+          const int at = ((2 * step + half) ^ turned) * 8;
+          p = product(*reinterpret_cast<const s16x8*>(at_k + at), *reinterpret_cast<const s16x8*>(at_q + at), p);
         }
         const int t = 32 * tt + column;
-        const float hi = sum_hi[t], lo = sum_lo[t];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float x[8];
+        for (int h = 0; h < kHeads; ++h) {
+          const float hi = all[h].hi[t], lo = all[h].lo[t];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int at = 32 * ts + 16 * j + 8 * (e / 4) + 4 * half + e % 4;
-            const float apart = (hi - sum_hi[at]) + (lo - sum_lo[at]);
-            // Chosen, not multiplied by zero: a later token's key may not be finite.
-            x[e] = at <= t ? p[8 * j + e] * (__builtin_amdgcn_exp2f(apart) * strength[at]) : 0.0f;
+          for (int j = 0; j < 2; ++j) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int at = 32 * ts + 16 * j + 8 * (e / 4) + 4 * half + e % 4;
+              const float apart = (hi - all[h].hi[at]) + (lo - all[h].lo[at]);
+              float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f(apart) * all[h].strength[at]);
+              // Chosen, not multiplied by zero: a later token's key may not be finite. (Made here, or the
+              // compiler branches around each exponential.)
+              asm volatile("" : "+v"(weight));
+              x[e] = at <= t ? weight : 0.0f;
+            }
+            const int frag = 2 * tt + 2 * ts + j;
+            weights[h][0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
+            weights[h][1][frag][lane] = pack8(x);
           }
-          const int frag = (tt == 0 ? 0 : 2) + 2 * ts + j;
-          weights[0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
-          weights[1][frag][lane] = pack8(x);
         }
       }
 #pragma unroll
@@ -294,70 +364,71 @@ __global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
           const s16x8 qf =
-              *reinterpret_cast<const s16x8*>(tile_q + (32 * tt + column) * DK + ((2 * step + half) ^ turned_k) * 8);
+              *reinterpret_cast<const s16x8*>(tile_q + (32 * tt + column) * DK + ((2 * step + half) ^ turned) * 8);
           o[tt] = product(high, qf, o[tt]);
           o[tt] = product(low, qf, o[tt]);
         }
       }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        o[tt] *= __builtin_amdgcn_exp2f(sum_hi[32 * tt + column] + sum_lo[32 * tt + column]) * a.scale;
+        o[tt] *= __builtin_amdgcn_exp2f(gates.hi[32 * tt + column] + gates.lo[32 * tt + column]) * a.scale;
       }
     }
     s16x8 values[4];
     float odd = 0.0f;
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      values[step] = transposed(tile_v, DV, row_v, wave, turned_v, step);
+      values[step] = transposed(tile_v + row_v + step * 16 * kWidth, kWidth, wave * 4 + piece_v, turned_v);
       const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
     }
-    if constexpr (kOutputs) {
-      lds_barrier();
-      if (__ballot(odd != odd) != 0) {
-        // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
-        for (int t = 0; t < tokens; ++t) {
-          const float keep = __builtin_amdgcn_exp2f(rate[t]);
-          const int at_v = 32 * wave + column;
-          const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
-          const float v = w * bf16_to_f32(tile_v[t * DV + ((at_v / 8) ^ turn_of<DV>(t)) * 8 + at_v % 8]);
-          const int turn = turn_of<DK>(t);
-          float sum = 0.0f;
+    const bool slow = kOutputs && __ballot(odd != odd) != 0;   // of the wave
+    if (slow) {
+      // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
+      for (int t = 0; t < tokens; ++t) {
+        const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
+        const int at_v = 32 * wave + column;
+        const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
+        const float v = w * bf16_to_f32(tile_v[t * kWidth + ((at_v / 8) ^ turn_of<kWidth>(t)) * 8 + at_v % 8]);
+        float sum = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              const int row = 32 * i + 8 * (e / 4) + 4 * half;   // and the three behind
-              const uint16_t* kr = tile_k + t * DK + ((row / 8) ^ turn) * 8 + 4 * half;
-              // Row `row` of q's column order: piece 2 (row / 16) + half, its second four from row 8 of 16 on.
-              const uint16_t* qr = tile_q + t * DK + ((2 * (row / 16) + half) ^ turn) * 8 + 4 * (row / 8 % 2);
+          for (int j = 0; j < 2; ++j) {
+            const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
+            float k[8], q[8];
+            unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
+            unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                s[i][e + j] = __builtin_fmaf(bf16_to_f32(kr[j]), v, s[i][e + j] * keep);
-                sum = __builtin_fmaf(bf16_to_f32(qr[j]), s[i][e + j], sum);
-              }
+            for (int e = 0; e < 8; ++e) {
+              s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
+              sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
             }
           }
-          uint32_t low, high;
-          half_pair(__float_as_uint(sum), low, high);
-          sum = __uint_as_float(low) + __uint_as_float(high);
-          if (half == 0) a.out[((token0 + t) * a.heads + head) * DV + at_v] = f32_to_bf16(sum * a.scale);
         }
-        lds_barrier();
-        continue;
+        uint32_t low, high;
+        half_pair(__float_as_uint(sum), low, high);
+        sum = __uint_as_float(low) + __uint_as_float(high);
+        if (half == 0) {
+          a.out[((token0 + t) * a.heads + head) * DV + 32 * wave % DV + column] = f32_to_bf16(sum * a.scale);
+        }
       }
+    }
+    lds_barrier();   // P is there, q and v are done with
+    if (more) ask(chunk + kChunk, next_k);
+    if (slow) return;
+    if constexpr (kOutputs) {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
         for (int step = 0; step < 2 + 2 * tt; ++step) {
-          const int frag = 2 * tt + step;
-          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[0][frag][lane]), o[tt]);
-          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[1][frag][lane]), o[tt]);
+          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[mine][0][2 * tt + step][lane]), o[tt]);
+          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[mine][1][2 * tt + step][lane]), o[tt]);
         }
         const int t = 32 * tt + column;
         if (t < tokens) {
-          uint16_t* to = a.out + ((token0 + t) * a.heads + head) * DV + 32 * wave + 4 * half;
+          uint16_t* to = a.out + ((token0 + t) * a.heads + head) * DV + 32 * wave % DV + 4 * half;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint2 packed;
@@ -368,7 +439,7 @@ __global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
         }
       }
     }
-    const float keep = __builtin_amdgcn_exp2f(sum_hi[kChunk - 1] + sum_lo[kChunk - 1]);
+    const float keep = __builtin_amdgcn_exp2f(gates.hi[kChunk - 1] + gates.lo[kChunk - 1]);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) s[i] *= keep;
 #pragma unroll
@@ -376,26 +447,33 @@ __global__ __launch_bounds__(2 * DV) void linear_chunk_kernel(LinearArgs a) {
       float x[8];
       unpack8(__builtin_bit_cast(u32x4, values[step]), x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= left[16 * step + 8 * (e / 4) + 4 * half + e % 4];
+      for (int e = 0; e < 8; ++e) x[e] *= gates.left[16 * step + 8 * (e / 4) + 4 * half + e % 4];
       const s16x8 v0 = cut(x), v1 = cut(x), v2 = cut(x);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        const s16x8 kt = transposed(tile_k, DK, row_k, i, turned_rows, step);
+        const s16x8 kt = transposed(tile_k + row_k + step * 16 * DK, DK, i * 4 + piece_k, turned_k);
         s[i] = product(kt, v0, s[i]);
         s[i] = product(kt, v1, s[i]);
         s[i] = product(kt, v2, s[i]);
       }
     }
-    lds_barrier();
+  };
+  for (int chunk = 0; chunk < count; chunk += 2 * kChunk) {
+    take(chunk, tile_k0, tile_k1, gates0, gates1);
+    if (chunk + kChunk < count) take(chunk + kChunk, tile_k1, tile_k0, gates1, gates0);
+  }
+  if (!kOutputs && wave == kWaves - 1 && lane == 0) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) a.totals[static_cast<int64_t>(in + 1) * a.heads + head0 + h] = static_cast<float>(total[h]);
   }
   if (kOutputs && (kind & 2) == 0) return;
   float* to = kOutputs ? a.states + state_at : carried + a.heads * kState;
+  asm volatile("" : "+v"(own));   // the addresses made anew: kept over the walk, they were spilled
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) to[mine + (32 * i + 8 * (e / 4) + e % 4) * DV] = s[i][e];
+    for (int e = 0; e < 16; ++e) to[own + (32 * i + 16 * (e / 8) + e % 8) * DV] = s[i][e];
   }
-  if (!kOutputs && threadIdx.x == 0) a.totals[static_cast<int64_t>(in + 1) * a.heads + head] = static_cast<float>(total);
 }
 
 // The states ahead of a sequence's third piece on, from what each piece before added:
@@ -424,9 +502,14 @@ template <int DK, int DV>
 void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
   const auto grid = [&](int64_t blocks) { return dim3(static_cast<unsigned>(blocks * a.heads)); };
   if (steps > 0) linear_step_kernel<DK, DV><<<grid(steps), 256, 0, stream>>>(a);
-  if (handed_on > 0) linear_chunk_kernel<DK, DV, false><<<grid(handed_on), 2 * DV, 0, stream>>>(a);
+  // Two heads of 64 columns a workgroup where they share a key head: four waves for two.
+  const int share = DV == 64 && a.group % 2 == 0 ? 2 : 1;
+  const auto own_parts = share == 2 ? linear_chunk_kernel<DK, 64, 2, false> : linear_chunk_kernel<DK, DV, 1, false>;
+  const auto contexts = share == 2 ? linear_chunk_kernel<DK, 64, 2, true> : linear_chunk_kernel<DK, DV, 1, true>;
+  const int threads = 2 * DV * share;
+  if (handed_on > 0) own_parts<<<dim3(static_cast<unsigned>(handed_on * (a.heads / share))), threads, 0, stream>>>(a);
   if (chains > 0) linear_carry_kernel<<<grid(chains * (DK * DV / 1024)), 256, 0, stream>>>(a, DK * DV);
-  if (runs > 0) linear_chunk_kernel<DK, DV, true><<<grid(runs), 2 * DV, 0, stream>>>(a);
+  if (runs > 0) contexts<<<dim3(static_cast<unsigned>(runs * (a.heads / share))), threads, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -463,8 +546,9 @@ extern "C" int32_t omnia_linear_attention(const omnia_linear_attention_t* c, hip
                 "linear_attention: pointers must be 16-byte aligned");
   OMNIA_REQUIRE(c->query_stride % 8 == 0 && c->key_stride % 8 == 0 && c->value_stride % 8 == 0 &&
                     c->query_stride >= c->key_heads * c->key_dim && c->key_stride >= c->key_heads * c->key_dim &&
-                    c->value_stride >= c->heads * c->value_dim,
-                "linear_attention: row strides must be multiples of 8 covering the heads");
+                    c->value_stride >= c->heads * c->value_dim && c->query_stride < kMost && c->key_stride < kMost &&
+                    c->value_stride < kMost,
+                "linear_attention: row strides must be multiples of 8 covering the heads, below 2^24");
   OMNIA_REQUIRE((c->decay_stride == 0 || c->decay_stride >= c->heads) &&
                     (c->strengths == nullptr || c->strength_stride >= c->heads),
                 "linear_attention: decay and strength rows must cover the heads");
