@@ -101,8 +101,10 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;
+constexpr int kNoLds = 0x7f;   // what a scheduling barrier lets through: all but LDS's instructions
 constexpr double kLog2e = 1.4426950408889634074;
 
 // Where 16-byte piece `piece` of row `row` lies in its row of a tile of D columns: rows of one
@@ -142,11 +144,16 @@ __device__ __forceinline__ double prefix_sum(double value, int lane) {
 }
 
 // 16 bytes a lane from global memory straight to LDS: lane l's come to `to` + 16 l.
-__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint16_t* to) {
+__device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
   typedef __attribute__((address_space(1))) const void* Global;
   typedef __attribute__((address_space(3))) void* Local;
   __builtin_amdgcn_global_load_lds((Global)from, (Local)to, 16, 0, 0);
 }
+
+// A workgroup barrier for what waves exchange through LDS that leaves loads straight to LDS in flight
+// (lds_barrier's fence, to which those are writes to LDS, waits for them: 32,768 tokens of 32 heads
+// HERE us for HERE).
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Brings a chunk's rows of D columns to LDS, with kThreads lanes; each row's 16-byte pieces lie
 // turned (turn_of).
@@ -157,28 +164,28 @@ struct Rows {
   static constexpr int kTurns = kPass >= 16 ? 1 : 16 / kPass;    // passes whose pieces are turned otherwise
   static constexpr int kPasses = kChunk / kPass;
   static_assert(kPass * kPieces == kThreads && kPasses * kPass == kChunk, "whole passes");
-  int64_t stride;
-  int offset[kTurns];   // of this lane's piece in pass i
-  __device__ __forceinline__ Rows(int64_t row_stride) : stride(row_stride) {
+  int64_t stride;            // bytes
+  uint32_t offset[kTurns];   // of this lane's piece in pass i
+  __device__ __forceinline__ Rows(int64_t row_stride) : stride(2 * row_stride) {
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      const int row = threadIdx.x / kPieces + i * kPass;
-      offset[i] = (threadIdx.x / kPieces) * static_cast<int>(stride) + ((threadIdx.x % kPieces) ^ turn_of<D>(row)) * 8;
-    }
+    for (int i = 0; i < kTurns; ++i) offset[i] = threadIdx.x / kPieces * static_cast<uint32_t>(stride) + piece(i);
+  }
+  static __device__ __forceinline__ uint32_t piece(int pass) {
+    return ((threadIdx.x % kPieces) ^ turn_of<D>(threadIdx.x / kPieces + pass * kPass)) * 16;
   }
   // Rows past the last of `tokens` come as the last: their weights are zeros, and where that last row
   // is not finite, so is all that it meets.
-  __device__ __forceinline__ void ask(const uint16_t* from, int tokens, uint16_t* tile) const {
-    uint16_t* to = tile + threadIdx.x / kWave * kWave * 8;
+  __device__ __forceinline__ void ask(const uint16_t* rows, int tokens, uint16_t* tile, int wave) const {
+    const char* from = reinterpret_cast<const char*>(rows);
+    uint16_t* to = tile + wave * kWave * 8;
     if (tokens == kChunk) {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) load_to_lds(from + i * kPass * stride + offset[i % kTurns], to + i * kThreads * 8);
     } else {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        const int row = threadIdx.x / kPieces + i * kPass;
-        const int back = max(row - (tokens - 1), 0) * static_cast<int>(stride);
-        load_to_lds(from + i * kPass * stride + (offset[i % kTurns] - back), to + i * kThreads * 8);
+        const uint32_t row = min(static_cast<int>(threadIdx.x) / kPieces + i * kPass, tokens - 1);
+        load_to_lds(from + (row * static_cast<uint32_t>(stride) + piece(i)), to + i * kThreads * 8);
       }
     }
   }
@@ -202,8 +209,8 @@ struct Gates {
 // in fp64 and held in two floats: its differences are what counts, and a fast decay ahead of a slow
 // one would swallow them.
 // The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
-// tiles, q and v, which are done with after the first half, to the same. Its decays are summed by the
-// wave that has no part of P.
+// tiles, v, which is held as operands from the start, and q, done with after the first half, to the
+// same. Its decays are summed by the wave that has no part of P.
 // kOutputs false leaves out q, P and the context: the piece's own part of the state, for the
 // pieces behind it.
 template <int DK, int DV, int kHeads, bool kOutputs>
@@ -212,7 +219,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
   __shared__ __attribute__((aligned(16))) uint16_t tile_q[kOutputs ? kChunk * DK : 8];
   __shared__ __attribute__((aligned(16))) uint16_t tile_k0[kChunk * DK], tile_k1[kChunk * DK];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * kWidth];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_v0[kChunk * kWidth], tile_v1[kOutputs ? 8 : kChunk * kWidth];
   __shared__ u32x4 weights[kOutputs ? kHeads : 1][kOutputs ? 2 : 1][kOutputs ? 6 : 1][kWave];   // P^T: parts, (t, 16 s), lanes
   __shared__ __attribute__((aligned(16))) Gates gates0[kHeads], gates1[kHeads];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -234,14 +241,18 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 
   const Rows<DK, kThreads> rows_q(a.q_stride), rows_k(a.k_stride);
   const Rows<kWidth, kThreads> rows_v(a.v_stride);
-  auto ask = [&](int chunk, uint16_t* tile_k) {
-    const int64_t token = first + chunk;
-    const int tokens = min(kChunk, count - chunk);
-    rows_k.ask(a.k + token * a.k_stride + shared * DK, tokens, tile_k);
-    if constexpr (kOutputs) rows_q.ask(a.q + token * a.q_stride + shared * DK, tokens, tile_q);
-    rows_v.ask(a.v + token * a.v_stride + head0 * DV, tokens, tile_v);
+  auto ask_q = [&](int chunk) {
+    rows_q.ask(a.q + (first + chunk) * a.q_stride + shared * DK, min(kChunk, count - chunk), tile_q, wave);
   };
-  ask(0, tile_k0);
+  auto ask_k = [&](int chunk, uint16_t* tile) {
+    rows_k.ask(a.k + (first + chunk) * a.k_stride + shared * DK, min(kChunk, count - chunk), tile, wave);
+  };
+  auto ask_v = [&](int chunk, uint16_t* tile) {
+    rows_v.ask(a.v + (first + chunk) * a.v_stride + head0 * DV, min(kChunk, count - chunk), tile, wave);
+  };
+  ask_k(0, tile_k0);
+  if constexpr (kOutputs) ask_q(0);
+  ask_v(0, tile_v0);
 
   // The decays of the chunk after next are asked for a chunk ahead of their sums.
   float ahead_g[kHeads], ahead_w[kHeads];
@@ -293,174 +304,260 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     }
   }
 
-  // Where this lane reads: rows `column` of a piece, and transposed, rows 4 half + sub / 4 (+ 8), the
-  // four columns 4 (sub % 4) of 16, of k those that make the state's order.
-  const int sub = lane % 16;
-  const int turned = turn_of<DK>(column), turned_k = turn_of<DK>(4 * half + sub / 4);
-  const int turned_v = turn_of<kWidth>(4 * half + sub / 4);
+  // Where this lane reads (elements): row `column` of a tile's first 32, piece `half`, whose other
+  // pieces and columns are an xor away; transposed, rows 4 half + sub / 4 (8 rows on: their turn is
+  // another by 2), the four columns 4 (sub % 4) of 16, of k those that make the state's order.
+  const int sub = lane % 16, row = 4 * half + sub / 4;
   const int four = (sub % 2) * 2 + sub % 4 / 2;
-  const int piece_k = 2 * (lane / 16 % 2) + four / 2, piece_v = 2 * (lane / 16 % 2) + sub % 4 / 2;
-  const int row_k = (4 * half + sub / 4) * DK + four % 2 * 4, row_v = (4 * half + sub / 4) * kWidth + sub % 2 * 4;
+  const int plain = column * DK + (half ^ turn_of<DK>(column)) * 8;
+  const int turned_k = row * DK + ((2 * (lane / 16 % 2) + four / 2) ^ turn_of<DK>(row)) * 8 + four % 2 * 4;
+  const int turned_v =
+      row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
   typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
-  auto transposed = [&](const uint16_t* at, int width, int piece, int turn) {   // of rows at and 8 on
-    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + (piece ^ turn) * 8));
-    const s16x4_lds high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * width + (piece ^ turn ^ 2) * 8));
+  auto transposed = [&](const uint16_t* tile, int at, int width) {   // of rows at and 8 on
+    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + at));
+    const s16x4_lds high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + 8 * width + (at ^ 16)));
     return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
   };
+  // The part of P^T that a wave makes: 32 tokens t by 32 s, (0, 0), (1, 1) and (1, 0). (A fourth wave's is
+  // not used.)
+  const int part_t = wave == 0 ? 0 : 1, part_s = wave == 1 ? 1 : 0;
 
-  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const Gates* all, Gates* next) {
+  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const uint16_t* tile_v, uint16_t* next_v,
+                  const Gates* all, Gates* next) {
     const int64_t token0 = first + chunk;
     const int tokens = min(kChunk, count - chunk);
     const bool more = chunk + kChunk < count;
     const Gates& gates = all[mine];
+    // Pinned: what the walk's reads start from is a few numbers, and not one for each of them.
+    int at_k = turned_k, at_v = turned_v, at_s = plain + 32 * part_s * DK;
+    int at_q[2] = {plain + 32 * (1 - part_t) * DK, plain + 32 * part_t * DK};   // the part's t second
+    asm volatile("" : "+v"(at_k), "+v"(at_v), "+v"(at_s), "+v"(at_q[0]), "+v"(at_q[1]));
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this chunk's rows
     lds_barrier();
+    if (!kOutputs && more) {
+      ask_k(chunk + kChunk, next_k);
+      ask_v(chunk + kChunk, next_v);
+    }
+    s16x8 values[4];
+#pragma unroll
+    for (int step = 0; step < 4; ++step) values[step] = transposed(tile_v + step * 16 * kWidth, at_v, kWidth);
+    __builtin_amdgcn_sched_barrier(kNoLds);
+    f32x16 o[2] = {f32x16{}, f32x16{}};
+    bool slow = false;   // of the wave
+    if constexpr (kOutputs) {
+      float odd = 0.0f;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
+      }
+      slow = __ballot(odd != odd) != 0;
+      if (slow) {
+        // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
+        for (int t = 0; t < tokens; ++t) {
+          const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
+          const int column_v = 32 * wave + column;
+          const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
+          const float v = w * bf16_to_f32(tile_v[t * kWidth + ((column_v / 8) ^ turn_of<kWidth>(t)) * 8 + column_v % 8]);
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
+              float k[8], q[8];
+              unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
+              unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
+                sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
+              }
+            }
+          }
+          uint32_t low, high;
+          half_pair(__float_as_uint(sum), low, high);
+          sum = __uint_as_float(low) + __uint_as_float(high);
+          if (half == 0) {
+            a.out[((token0 + t) * a.heads + head) * DV + 32 * wave % DV + column] = f32_to_bf16(sum * a.scale);
+          }
+        }
+      }
+      meet();   // v is done with
+      if (more) {
+        ask_k(chunk + kChunk, next_k);
+        ask_v(chunk + kChunk, next_v);
+      }
+    }
     if (wave == kWaves - 1 && more) {
       sum_gates(chunk + kChunk, next);
       ask_gates(chunk + 2 * kChunk);
     }
-    f32x16 o[2] = {f32x16{}, f32x16{}};
     if constexpr (kOutputs) {
-      // P^T of 32 tokens t by 32 s: (0, 0), (1, 1) and (1, 0).
-      for (int tile = wave; tile < 3; tile += kWaves) {
-        const int tt = tile == 0 ? 0 : 1, ts = tile == 1 ? 1 : 0;
-        const uint16_t* at_q = tile_q + (32 * tt + column) * DK;
-        const uint16_t* at_k = tile_k + (32 * ts + column) * DK;
-        f32x16 p = f32x16{};
-#pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          const int at = ((2 * step + half) ^ turned) * 8;
-          p = product(*reinterpret_cast<const s16x8*>(at_k + at), *reinterpret_cast<const s16x8*>(at_q + at), p);
-        }
+      const auto weigh = [&](const f32x16& p, int tt, int ts) {
         const int t = 32 * tt + column;
+        // Past this token's place in the part: none of them where the part is not on the diagonal.
+        const int bound = tt == ts ? column - 4 * half : 32;
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
           const float hi = all[h].hi[t], lo = all[h].lo[t];
+          f32x4 his[4], los[4], strengths[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 32 * ts + 8 * i + 4 * half;
+            his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at]);
+            los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at]);
+            strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at]);
+          }
+          __builtin_amdgcn_sched_barrier(kNoLds);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const int at = 32 * ts + 16 * j + 8 * (e / 4) + 4 * half + e % 4;
-              const float apart = (hi - all[h].hi[at]) + (lo - all[h].lo[at]);
-              float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f(apart) * all[h].strength[at]);
-              // Chosen, not multiplied by zero: a later token's key may not be finite. (Made here, or the
+              const int i = 2 * j + e / 4, n = e % 4;
+              float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f((hi - his[i][n]) + (lo - los[i][n])) * strengths[i][n]);
+              // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
               // compiler branches around each exponential.)
-              asm volatile("" : "+v"(weight));
-              x[e] = at <= t ? weight : 0.0f;
+              asm("" : "+v"(weight));
+              x[e] = 8 * i + n <= bound ? weight : 0.0f;
             }
             const int frag = 2 * tt + 2 * ts + j;
             weights[h][0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
             weights[h][1][frag][lane] = pack8(x);
           }
         }
-      }
+      };
+      // q S with the products of P^T; each step's operands are asked for ahead of the last one's products.
+      s16x8 q[2][2], k[2];
+      const auto fetch = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q[step % 2][i] = *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step)));
+        k[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
+        __builtin_amdgcn_sched_barrier(kNoLds);
+      };
+      f32x16 p = f32x16{};
+      fetch(0);
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
+        const int now = step % 2;
+        if (step + 1 < kSteps) fetch(step + 1);
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
         const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
+        p = product(k[now], q[now][1], p);
+        o[0] = product(high, q[now][0], o[0]);
+        o[1] = product(high, q[now][1], o[1]);
+        o[0] = product(low, q[now][0], o[0]);
+        o[1] = product(low, q[now][1], o[1]);
+      }
+      if (wave < 3) weigh(p, part_t, part_s);
+      if (kWaves < 3 && wave == kWaves - 1) {
+        p = f32x16{};
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          const s16x8 qf =
-              *reinterpret_cast<const s16x8*>(tile_q + (32 * tt + column) * DK + ((2 * step + half) ^ turned) * 8);
-          o[tt] = product(high, qf, o[tt]);
-          o[tt] = product(low, qf, o[tt]);
+        for (int step = 0; step < kSteps; ++step) {
+          p = product(*reinterpret_cast<const s16x8*>(tile_k + (plain ^ (16 * step))),
+                      *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
         }
+        weigh(p, 1, 0);
+      }
+      if (wave == 0) {
+        const f32x16 first_rows = o[1];
+        o[1] = o[0];
+        o[0] = first_rows;
       }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
         o[tt] *= __builtin_amdgcn_exp2f(gates.hi[32 * tt + column] + gates.lo[32 * tt + column]) * a.scale;
       }
+      meet();   // P is there, q is done with
+      if (more) ask_q(chunk + kChunk);
+      if (slow) return;
     }
-    s16x8 values[4];
-    float odd = 0.0f;
+    // The first products' operands are asked for ahead of the decay, and each step's ahead of the last one's.
+    s16x8 parts[2][2][2], k[2][kTiles];   // P: t, 16 s, part
+    f32x4 left[2][2];
+    const auto fetch = [&](int step) {
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      values[step] = transposed(tile_v + row_v + step * 16 * kWidth, kWidth, wave * 4 + piece_v, turned_v);
-      const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
+      for (int i = 0; i < 2; ++i) left[step % 2][i] = *reinterpret_cast<const f32x4*>(&gates.left[16 * step + 8 * i + 4 * half]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
-    }
-    const bool slow = kOutputs && __ballot(odd != odd) != 0;   // of the wave
-    if (slow) {
-      // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
-      for (int t = 0; t < tokens; ++t) {
-        const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
-        const int at_v = 32 * wave + column;
-        const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
-        const float v = w * bf16_to_f32(tile_v[t * kWidth + ((at_v / 8) ^ turn_of<kWidth>(t)) * 8 + at_v % 8]);
-        float sum = 0.0f;
+      for (int i = 0; i < kTiles; ++i) k[step % 2][i] = transposed(tile_k + step * 16 * DK, at_k ^ (32 * i), DK);
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    const auto fetch_part = [&](int tt, int ts) {   // of P
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
-            float k[8], q[8];
-            unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
-            unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
-              sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
-            }
-          }
-        }
-        uint32_t low, high;
-        half_pair(__float_as_uint(sum), low, high);
-        sum = __uint_as_float(low) + __uint_as_float(high);
-        if (half == 0) {
-          a.out[((token0 + t) * a.heads + head) * DV + 32 * wave % DV + column] = f32_to_bf16(sum * a.scale);
+        for (int part = 0; part < 2; ++part) {
+          parts[tt][j][part] = __builtin_bit_cast(s16x8, weights[mine][part][2 * tt + 2 * ts + j][lane]);
         }
       }
-    }
-    lds_barrier();   // P is there, q and v are done with
-    if (more) ask(chunk + kChunk, next_k);
-    if (slow) return;
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    const float keep_hi = gates.hi[kChunk - 1], keep_lo = gates.lo[kChunk - 1];
     if constexpr (kOutputs) {
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-        for (int step = 0; step < 2 + 2 * tt; ++step) {
-          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[mine][0][2 * tt + step][lane]), o[tt]);
-          o[tt] = product(values[step], __builtin_bit_cast(s16x8, weights[mine][1][2 * tt + step][lane]), o[tt]);
-        }
-        const int t = 32 * tt + column;
-        if (t < tokens) {
-          uint16_t* to = a.out + ((token0 + t) * a.heads + head) * DV + 32 * wave % DV + 4 * half;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint2 packed;
-            packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
-            packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
-            *reinterpret_cast<uint2*>(to + 8 * i) = packed;
-          }
-        }
-      }
+      fetch_part(0, 0);
+      fetch_part(1, 0);
+    } else {
+      fetch(0);
     }
-    const float keep = __builtin_amdgcn_exp2f(gates.hi[kChunk - 1] + gates.lo[kChunk - 1]);
+    const float keep = __builtin_amdgcn_exp2f(keep_hi + keep_lo);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) s[i] *= keep;
+    if constexpr (kOutputs) {
+      // Rows past the last are out of the buffer, and not written.
+      const int64_t bytes = static_cast<int64_t>(a.heads) * DV * 2;   // of a row
+      const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + (token0 * a.heads + head) * DV, 0,
+                                                        static_cast<int>((tokens - 1) * bytes + DV * 2), 0x00027000);
+      const auto times = [&](int tt, int ts) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) o[tt] = product(values[2 * ts + j], parts[tt][j][part], o[tt]);
+        }
+      };
+      const auto store = [&](int tt) {
+        const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 4 * half) * 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x2 packed;
+          packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
+          packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
+          __builtin_amdgcn_raw_buffer_store_b64(packed, to, at + 16 * i, 0, 0);
+        }
+      };
+      times(0, 0);
+      times(1, 0);
+      fetch_part(1, 1);
+      fetch(0);
+      store(0);
+      times(1, 1);
+      store(1);
+    }
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
+      const int now = step % 2;
+      if (step + 1 < 4) fetch(step + 1);
       float x[8];
       unpack8(__builtin_bit_cast(u32x4, values[step]), x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= gates.left[16 * step + 8 * (e / 4) + 4 * half + e % 4];
-      const s16x8 v0 = cut(x), v1 = cut(x), v2 = cut(x);
+      for (int e = 0; e < 8; ++e) x[e] *= left[now][e / 4][e % 4];
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        const s16x8 kt = transposed(tile_k + row_k + step * 16 * DK, DK, i * 4 + piece_k, turned_k);
-        s[i] = product(kt, v0, s[i]);
-        s[i] = product(kt, v1, s[i]);
-        s[i] = product(kt, v2, s[i]);
+      for (int part = 0; part < 3; ++part) {
+        const s16x8 v = cut(x);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) s[i] = product(k[now][i], v, s[i]);
       }
     }
   };
   for (int chunk = 0; chunk < count; chunk += 2 * kChunk) {
-    take(chunk, tile_k0, tile_k1, gates0, gates1);
-    if (chunk + kChunk < count) take(chunk + kChunk, tile_k1, tile_k0, gates1, gates0);
+    take(chunk, tile_k0, tile_k1, tile_v0, kOutputs ? tile_v0 : tile_v1, gates0, gates1);
+    if (chunk + kChunk < count) {
+      take(chunk + kChunk, tile_k1, tile_k0, kOutputs ? tile_v0 : tile_v1, tile_v0, gates1, gates0);
+    }
   }
   if (!kOutputs && wave == kWaves - 1 && lane == 0) {
 #pragma unroll
