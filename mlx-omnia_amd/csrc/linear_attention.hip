@@ -133,15 +133,33 @@ __device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Inclusive sums over the lanes of a wave.
-__device__ __forceinline__ double prefix_sum(double value, int lane) {
-#pragma unroll
-  for (int step = 1; step < kWave; step *= 2) {
-    const double before = __shfl_up(value, step, kWave);
-    value += lane >= step ? before : 0.0;
-  }
+// Inclusive sums over the lanes of a wave: within rows of 16, then the rows' last onto the rows behind.
+template <int ctrl, int rows>
+__device__ __forceinline__ double moved(double value) {   // zeros where no lane is moved from
+  const uint64_t bits = __builtin_bit_cast(uint64_t, value);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), ctrl, rows, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), ctrl, rows, 0xf, false);
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ __forceinline__ double prefix_sum(double value) {
+  value += moved<0x111, 0xf>(value);   // row_shr 1, 2, 4, 8
+  value += moved<0x112, 0xf>(value);
+  value += moved<0x114, 0xf>(value);
+  value += moved<0x118, 0xf>(value);
+  value += moved<0x142, 0xa>(value);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  value += moved<0x143, 0xc>(value);
   return value;
 }
+// The last lane's value, in every lane.
+__device__ __forceinline__ double last_lane(double value) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, value);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(bits), kWave - 1);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), kWave - 1);
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+// log2 of a decay. Past 2^-512 it leaves nothing of 32 bits, as that does; sums of -inf would differ
+// by NaN.
+__device__ __forceinline__ double log2_of(float g) { return g < -354.0f ? -512.0 : g * kLog2e; }
 
 // 16 bytes a lane from global memory straight to LDS: lane l's come to `to` + 16 l.
 __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
@@ -191,6 +209,32 @@ struct Rows {
   }
 };
 
+// Sixteen rows' values of a column each lane and k's rows with them (of every 32 of the state's rows):
+// s += k^T (left v), the scaled values in three parts.
+template <int kTiles>
+__device__ __forceinline__ void add_products(f32x16 (&s)[kTiles], const s16x8& values, const f32x4 (&left)[2],
+                                             const s16x8 (&k)[kTiles]) {
+  float x[8];
+  unpack8(__builtin_bit_cast(u32x4, values), x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= left[e / 4][e % 4];
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    const s16x8 v = cut(x);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) s[i] = product(k[i], v, s[i]);
+  }
+}
+
+// Eight rows of a tile transposed, `at` in the first of them and the other four 8 rows on (whose
+// pieces' turn is another by 2).
+__device__ __forceinline__ s16x8 transposed(const uint16_t* tile, int at, int width) {
+  typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
+  const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + at));
+  const s16x4_lds high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + 8 * width + (at ^ 16)));
+  return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // What a chunk's decays come to: G (in two floats, log2), w * scale, w exp(G_end - G) and g (log2).
 struct Gates {
   float hi[kChunk], lo[kChunk], strength[kChunk], left[kChunk], rate[kChunk];
@@ -211,16 +255,13 @@ struct Gates {
 // The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
 // tiles, v, which is held as operands from the start, and q, done with after the first half, to the
 // same. Its decays are summed by the wave that has no part of P.
-// kOutputs false leaves out q, P and the context: the piece's own part of the state, for the
-// pieces behind it.
-template <int DK, int DV, int kHeads, bool kOutputs>
+template <int DK, int DV, int kHeads>
 __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(LinearArgs a) {
   constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
-  __shared__ __attribute__((aligned(16))) uint16_t tile_q[kOutputs ? kChunk * DK : 8];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_k0[kChunk * DK], tile_k1[kChunk * DK];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_v0[kChunk * kWidth], tile_v1[kOutputs ? 8 : kChunk * kWidth];
-  __shared__ u32x4 weights[kOutputs ? kHeads : 1][kOutputs ? 2 : 1][kOutputs ? 6 : 1][kWave];   // P^T: parts, (t, 16 s), lanes
+  __shared__ __attribute__((aligned(16))) uint16_t tile_q[kChunk * DK], tile_k0[kChunk * DK], tile_k1[kChunk * DK];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * kWidth];
+  __shared__ u32x4 weights[kHeads][2][6][kWave];   // P^T: parts, (t, 16 s), lanes
   __shared__ __attribute__((aligned(16))) Gates gates0[kHeads], gates1[kHeads];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane / 32, column = lane % 32;
@@ -230,13 +271,12 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   const int32_t* run = a.runs + 5 * entry;
   const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
   if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < -1 ||
-      in + ((kind & 2) == 0) >= a.pieces || (in < 0 && kind != 3) || (!kOutputs && (kind & 2) != 0)) {
+      in >= a.pieces || (in < 0 && kind != 3)) {
     return;
   }
   const int shared = head0 / a.group;
   constexpr int64_t kState = DK * DV;
   const int64_t state_at = (static_cast<int64_t>(slot) * a.heads + head) * kState;
-  float* carried = a.carried + (static_cast<int64_t>(in < 0 ? 0 : in) * a.heads + head) * kState;
   uint32_t own = 8 * half * DV + 32 * wave % DV + column;   // this lane's first row and its column
 
   const Rows<DK, kThreads> rows_q(a.q_stride), rows_k(a.k_stride);
@@ -247,12 +287,12 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   auto ask_k = [&](int chunk, uint16_t* tile) {
     rows_k.ask(a.k + (first + chunk) * a.k_stride + shared * DK, min(kChunk, count - chunk), tile, wave);
   };
-  auto ask_v = [&](int chunk, uint16_t* tile) {
-    rows_v.ask(a.v + (first + chunk) * a.v_stride + head0 * DV, min(kChunk, count - chunk), tile, wave);
+  auto ask_v = [&](int chunk) {
+    rows_v.ask(a.v + (first + chunk) * a.v_stride + head0 * DV, min(kChunk, count - chunk), tile_v, wave);
   };
   ask_k(0, tile_k0);
-  if constexpr (kOutputs) ask_q(0);
-  ask_v(0, tile_v0);
+  ask_q(0);
+  ask_v(0);
 
   // The decays of the chunk after next are asked for a chunk ahead of their sums.
   float ahead_g[kHeads], ahead_w[kHeads];
@@ -264,17 +304,14 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + h] : 1.0f;
     }
   };
-  double total[kHeads] = {};   // of the piece's log2 decays
   auto sum_gates = [&](int chunk, Gates* gates) {
     const bool there = lane < count - chunk;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
       const float g = ahead_g[h], w = there ? ahead_w[h] : 0.0f;
-      // A decay past 2^-512 leaves nothing of 32 bits, as that does; sums of -inf would differ by NaN.
-      const double log2 = !there ? 0.0 : g < -354.0f ? -512.0 : g * kLog2e;
-      const double sum = prefix_sum(log2, lane);
-      const double end = __shfl(sum, kWave - 1, kWave);
-      total[h] += end;
+      const double log2 = there ? log2_of(g) : 0.0;
+      const double sum = prefix_sum(log2);
+      const double end = last_lane(sum);
       const float hi = static_cast<float>(sum);
       gates[h].hi[lane] = hi;
       gates[h].lo[lane] = static_cast<float>(sum - hi);
@@ -291,16 +328,11 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 
   f32x16 s[kTiles];
   {
-    const float* from = kOutputs ? (in < 0 ? a.states + state_at : carried) : a.states + state_at;
-    const bool zero = !kOutputs && (kind & 1) == 0;
+    const float* from = in < 0 ? a.states + state_at : a.carried + (static_cast<int64_t>(in) * a.heads + head) * kState;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint32_t at = own + (32 * i + 16 * (e / 8) + e % 8) * DV;
-        s[i][e] = zero ? 0.0f : from[at];
-        if (!kOutputs && !zero) carried[at] = s[i][e];   // what the first piece's context starts from
-      }
+      for (int e = 0; e < 16; ++e) s[i][e] = from[own + (32 * i + 16 * (e / 8) + e % 8) * DV];
     }
   }
 
@@ -313,18 +345,11 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   const int turned_k = row * DK + ((2 * (lane / 16 % 2) + four / 2) ^ turn_of<DK>(row)) * 8 + four % 2 * 4;
   const int turned_v =
       row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
-  typedef __attribute__((address_space(3))) s16x4_lds* LdsPtr;
-  auto transposed = [&](const uint16_t* tile, int at, int width) {   // of rows at and 8 on
-    const s16x4_lds low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + at));
-    const s16x4_lds high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(tile + 8 * width + (at ^ 16)));
-    return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
   // The part of P^T that a wave makes: 32 tokens t by 32 s, (0, 0), (1, 1) and (1, 0). (A fourth wave's is
   // not used.)
   const int part_t = wave == 0 ? 0 : 1, part_s = wave == 1 ? 1 : 0;
 
-  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const uint16_t* tile_v, uint16_t* next_v,
-                  const Gates* all, Gates* next) {
+  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const Gates* all, Gates* next) {
     const int64_t token0 = first + chunk;
     const int tokens = min(kChunk, count - chunk);
     const bool more = chunk + kChunk < count;
@@ -335,156 +360,148 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     asm volatile("" : "+v"(at_k), "+v"(at_v), "+v"(at_s), "+v"(at_q[0]), "+v"(at_q[1]));
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this chunk's rows
     lds_barrier();
-    if (!kOutputs && more) {
-      ask_k(chunk + kChunk, next_k);
-      ask_v(chunk + kChunk, next_v);
-    }
     s16x8 values[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) values[step] = transposed(tile_v + step * 16 * kWidth, at_v, kWidth);
     __builtin_amdgcn_sched_barrier(kNoLds);
     f32x16 o[2] = {f32x16{}, f32x16{}};
     bool slow = false;   // of the wave
-    if constexpr (kOutputs) {
-      float odd = 0.0f;
+    float odd = 0.0f;
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
+    for (int step = 0; step < 4; ++step) {
+      const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
-      }
-      slow = __ballot(odd != odd) != 0;
-      if (slow) {
-        // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
-        for (int t = 0; t < tokens; ++t) {
-          const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
-          const int column_v = 32 * wave + column;
-          const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
-          const float v = w * bf16_to_f32(tile_v[t * kWidth + ((column_v / 8) ^ turn_of<kWidth>(t)) * 8 + column_v % 8]);
-          float sum = 0.0f;
+      for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
+    }
+    slow = __ballot(odd != odd) != 0;
+    if (slow) {
+      // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
+      for (int t = 0; t < tokens; ++t) {
+        const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
+        const int column_v = 32 * wave + column;
+        const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
+        const float v = w * bf16_to_f32(tile_v[t * kWidth + ((column_v / 8) ^ turn_of<kWidth>(t)) * 8 + column_v % 8]);
+        float sum = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
-              float k[8], q[8];
-              unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
-              unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
+          for (int j = 0; j < 2; ++j) {
+            const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
+            float k[8], q[8];
+            unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
+            unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
-                sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
-              }
+            for (int e = 0; e < 8; ++e) {
+              s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
+              sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
             }
           }
-          uint32_t low, high;
-          half_pair(__float_as_uint(sum), low, high);
-          sum = __uint_as_float(low) + __uint_as_float(high);
-          if (half == 0) {
-            a.out[((token0 + t) * a.heads + head) * DV + 32 * wave % DV + column] = f32_to_bf16(sum * a.scale);
-          }
+        }
+        uint32_t low, high;
+        half_pair(__float_as_uint(sum), low, high);
+        sum = __uint_as_float(low) + __uint_as_float(high);
+        if (half == 0) {
+          a.out[((token0 + t) * a.heads + head) * DV + 32 * wave % DV + column] = f32_to_bf16(sum * a.scale);
         }
       }
-      meet();   // v is done with
-      if (more) {
-        ask_k(chunk + kChunk, next_k);
-        ask_v(chunk + kChunk, next_v);
-      }
+    }
+    meet();   // v is done with
+    if (more) {
+      ask_k(chunk + kChunk, next_k);
+      ask_v(chunk + kChunk);
     }
     if (wave == kWaves - 1 && more) {
       sum_gates(chunk + kChunk, next);
       ask_gates(chunk + 2 * kChunk);
     }
-    if constexpr (kOutputs) {
-      const auto weigh = [&](const f32x16& p, int tt, int ts) {
-        const int t = 32 * tt + column;
-        // Past this token's place in the part: none of them where the part is not on the diagonal.
-        const int bound = tt == ts ? column - 4 * half : 32;
+    const auto weigh = [&](const f32x16& p, int tt, int ts) {
+      const int t = 32 * tt + column;
+      // Past this token's place in the part: none of them where the part is not on the diagonal.
+      const int bound = tt == ts ? column - 4 * half : 32;
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          const float hi = all[h].hi[t], lo = all[h].lo[t];
-          f32x4 his[4], los[4], strengths[4];
+      for (int h = 0; h < kHeads; ++h) {
+        const float hi = all[h].hi[t], lo = all[h].lo[t];
+        f32x4 his[4], los[4], strengths[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = 32 * ts + 8 * i + 4 * half;
-            his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at]);
-            los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at]);
-            strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at]);
-          }
-          __builtin_amdgcn_sched_barrier(kNoLds);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int i = 2 * j + e / 4, n = e % 4;
-              float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f((hi - his[i][n]) + (lo - los[i][n])) * strengths[i][n]);
-              // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
-              // compiler branches around each exponential.)
-              asm("" : "+v"(weight));
-              x[e] = 8 * i + n <= bound ? weight : 0.0f;
-            }
-            const int frag = 2 * tt + 2 * ts + j;
-            weights[h][0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
-            weights[h][1][frag][lane] = pack8(x);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int at = 32 * ts + 8 * i + 4 * half;
+          his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at]);
+          los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at]);
+          strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at]);
         }
-      };
-      // q S with the products of P^T; each step's operands are asked for ahead of the last one's products.
-      s16x8 q[2][2], k[2];
-      const auto fetch = [&](int step) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) q[step % 2][i] = *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step)));
-        k[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
         __builtin_amdgcn_sched_barrier(kNoLds);
-      };
-      f32x16 p = f32x16{};
-      fetch(0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = 2 * j + e / 4, n = e % 4;
+            float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f((hi - his[i][n]) + (lo - los[i][n])) * strengths[i][n]);
+            // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
+            // compiler branches around each exponential.)
+            asm("" : "+v"(weight));
+            x[e] = 8 * i + n <= bound ? weight : 0.0f;
+          }
+          const int frag = 2 * tt + 2 * ts + j;
+          weights[h][0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
+          weights[h][1][frag][lane] = pack8(x);
+        }
+      }
+    };
+    // q S with the products of P^T; each step's operands are asked for ahead of the last one's products.
+    s16x8 q[2][2], k[2];
+    const auto fetch = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) q[step % 2][i] = *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step)));
+      k[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    f32x16 p = f32x16{};
+    fetch(0);
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      const int now = step % 2;
+      if (step + 1 < kSteps) fetch(step + 1);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
+      const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
+      p = product(k[now], q[now][1], p);
+      o[0] = product(high, q[now][0], o[0]);
+      o[1] = product(high, q[now][1], o[1]);
+      o[0] = product(low, q[now][0], o[0]);
+      o[1] = product(low, q[now][1], o[1]);
+    }
+    if (wave < 3) weigh(p, part_t, part_s);
+    if (kWaves < 3 && wave == kWaves - 1) {
+      p = f32x16{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
-        const int now = step % 2;
-        if (step + 1 < kSteps) fetch(step + 1);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
-        const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
-        p = product(k[now], q[now][1], p);
-        o[0] = product(high, q[now][0], o[0]);
-        o[1] = product(high, q[now][1], o[1]);
-        o[0] = product(low, q[now][0], o[0]);
-        o[1] = product(low, q[now][1], o[1]);
+        p = product(*reinterpret_cast<const s16x8*>(tile_k + (plain ^ (16 * step))),
+                    *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
       }
-      if (wave < 3) weigh(p, part_t, part_s);
-      if (kWaves < 3 && wave == kWaves - 1) {
-        p = f32x16{};
-#pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          p = product(*reinterpret_cast<const s16x8*>(tile_k + (plain ^ (16 * step))),
-                      *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
-        }
-        weigh(p, 1, 0);
-      }
-      if (wave == 0) {
-        const f32x16 first_rows = o[1];
-        o[1] = o[0];
-        o[0] = first_rows;
-      }
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        o[tt] *= __builtin_amdgcn_exp2f(gates.hi[32 * tt + column] + gates.lo[32 * tt + column]) * a.scale;
-      }
-      meet();   // P is there, q is done with
-      if (more) ask_q(chunk + kChunk);
-      if (slow) return;
+      weigh(p, 1, 0);
     }
+    if (wave == 0) {
+      const f32x16 first_rows = o[1];
+      o[1] = o[0];
+      o[0] = first_rows;
+    }
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      o[tt] *= __builtin_amdgcn_exp2f(gates.hi[32 * tt + column] + gates.lo[32 * tt + column]) * a.scale;
+    }
+    meet();   // P is there, q is done with
+    if (more) ask_q(chunk + kChunk);
+    if (slow) return;
     // The first products' operands are asked for ahead of the decay, and each step's ahead of the last one's.
-    s16x8 parts[2][2][2], k[2][kTiles];   // P: t, 16 s, part
+    s16x8 parts[2][2][2], kt[2][kTiles];   // P: t, 16 s, part
     f32x4 left[2][2];
-    const auto fetch = [&](int step) {
+    const auto fetch_state = [&](int step) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) left[step % 2][i] = *reinterpret_cast<const f32x4*>(&gates.left[16 * step + 8 * i + 4 * half]);
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) k[step % 2][i] = transposed(tile_k + step * 16 * DK, at_k ^ (32 * i), DK);
+      for (int i = 0; i < kTiles; ++i) kt[step % 2][i] = transposed(tile_k + step * 16 * DK, at_k ^ (32 * i), DK);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     const auto fetch_part = [&](int tt, int ts) {   // of P
@@ -498,78 +515,194 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     const float keep_hi = gates.hi[kChunk - 1], keep_lo = gates.lo[kChunk - 1];
-    if constexpr (kOutputs) {
-      fetch_part(0, 0);
-      fetch_part(1, 0);
-    } else {
-      fetch(0);
-    }
+    fetch_part(0, 0);
+    fetch_part(1, 0);
     const float keep = __builtin_amdgcn_exp2f(keep_hi + keep_lo);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) s[i] *= keep;
-    if constexpr (kOutputs) {
-      // Rows past the last are out of the buffer, and not written.
-      const int64_t bytes = static_cast<int64_t>(a.heads) * DV * 2;   // of a row
-      const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + (token0 * a.heads + head) * DV, 0,
-                                                        static_cast<int>((tokens - 1) * bytes + DV * 2), 0x00027000);
-      const auto times = [&](int tt, int ts) {
+    // Rows past the last are out of the buffer, and not written.
+    const int64_t bytes = static_cast<int64_t>(a.heads) * DV * 2;   // of a row
+    const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + (token0 * a.heads + head) * DV, 0,
+                                                      static_cast<int>((tokens - 1) * bytes + DV * 2), 0x00027000);
+    const auto times = [&](int tt, int ts) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int part = 0; part < 2; ++part) o[tt] = product(values[2 * ts + j], parts[tt][j][part], o[tt]);
-        }
-      };
-      const auto store = [&](int tt) {
-        const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 4 * half) * 2;
+        for (int part = 0; part < 2; ++part) o[tt] = product(values[2 * ts + j], parts[tt][j][part], o[tt]);
+      }
+    };
+    const auto store = [&](int tt) {
+      const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 4 * half) * 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u32x2 packed;
-          packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
-          packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
-          __builtin_amdgcn_raw_buffer_store_b64(packed, to, at + 16 * i, 0, 0);
-        }
-      };
-      times(0, 0);
-      times(1, 0);
-      fetch_part(1, 1);
-      fetch(0);
-      store(0);
-      times(1, 1);
-      store(1);
-    }
+      for (int i = 0; i < 4; ++i) {
+        u32x2 packed;
+        packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
+        packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
+        __builtin_amdgcn_raw_buffer_store_b64(packed, to, at + 16 * i, 0, 0);
+      }
+    };
+    times(0, 0);
+    times(1, 0);
+    fetch_part(1, 1);
+    fetch_state(0);
+    store(0);
+    times(1, 1);
+    store(1);
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       const int now = step % 2;
-      if (step + 1 < 4) fetch(step + 1);
-      float x[8];
-      unpack8(__builtin_bit_cast(u32x4, values[step]), x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= left[now][e / 4][e % 4];
-#pragma unroll
-      for (int part = 0; part < 3; ++part) {
-        const s16x8 v = cut(x);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) s[i] = product(k[now][i], v, s[i]);
-      }
+      if (step + 1 < 4) fetch_state(step + 1);
+      add_products(s, values[step], left[now], kt[now]);
     }
   };
   for (int chunk = 0; chunk < count; chunk += 2 * kChunk) {
-    take(chunk, tile_k0, tile_k1, tile_v0, kOutputs ? tile_v0 : tile_v1, gates0, gates1);
-    if (chunk + kChunk < count) {
-      take(chunk + kChunk, tile_k1, tile_k0, kOutputs ? tile_v0 : tile_v1, tile_v0, gates1, gates0);
-    }
+    take(chunk, tile_k0, tile_k1, gates0, gates1);
+    if (chunk + kChunk < count) take(chunk + kChunk, tile_k1, tile_k0, gates1, gates0);
   }
-  if (!kOutputs && wave == kWaves - 1 && lane == 0) {
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) a.totals[static_cast<int64_t>(in + 1) * a.heads + head0 + h] = static_cast<float>(total[h]);
-  }
-  if (kOutputs && (kind & 2) == 0) return;
-  float* to = kOutputs ? a.states + state_at : carried + a.heads * kState;
+  if ((kind & 2) == 0) return;
+  float* to = a.states + state_at;
   asm volatile("" : "+v"(own));   // the addresses made anew: kept over the walk, they were spilled
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) to[own + (32 * i + 16 * (e / 8) + e % 8) * DV] = s[i][e];
+  }
+}
+
+// What a piece adds to the state, for the pieces behind it: k^T (exp(G_end - G_s) w_s v_s) over all of
+// its chunks, from the last to the first, so that what stands behind a chunk is known and the sums are
+// never scaled. The first piece's is the state behind it: the sequence's own, decayed, comes on top at
+// the end (and is kept for the piece's contexts, since the last piece writes over it).
+template <int DK, int DV, int kHeads>
+__global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_part_kernel(LinearArgs a) {
+  constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
+  constexpr int kTiles = DK / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t tile_k0[kChunk * DK], tile_k1[kChunk * DK];
+  __shared__ __attribute__((aligned(16))) uint16_t tile_v0[kChunk * kWidth], tile_v1[kChunk * kWidth];
+  __shared__ __attribute__((aligned(16))) float left0[kHeads][kChunk], left1[kHeads][kChunk];
+  __shared__ float whole[kHeads];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int half = lane / 32, column = lane % 32;
+  const int blocks = a.heads / kHeads;
+  const int entry = blockIdx.x / blocks, head0 = blockIdx.x % blocks * kHeads;
+  const int mine = wave * 32 / DV, head = head0 + mine;   // the wave's
+  const int32_t* run = a.runs + 5 * entry;
+  const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
+  if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < 0 ||
+      in + 1 >= a.pieces || (kind & 2) != 0) {
+    return;
+  }
+  const int shared = head0 / a.group;
+  constexpr int64_t kState = DK * DV;
+
+  const Rows<DK, kThreads> rows_k(a.k_stride);
+  const Rows<kWidth, kThreads> rows_v(a.v_stride);
+  auto ask = [&](int chunk, uint16_t* tile_k, uint16_t* tile_v) {
+    const int64_t token = first + chunk;
+    const int tokens = min(kChunk, count - chunk);
+    rows_k.ask(a.k + token * a.k_stride + shared * DK, tokens, tile_k, wave);
+    rows_v.ask(a.v + token * a.v_stride + head0 * DV, tokens, tile_v, wave);
+  };
+  const int last = (count - 1) / kChunk * kChunk;
+  ask(last, tile_k0, tile_v0);
+
+  // The decays of the chunk after next are asked for a chunk ahead of their sums.
+  float ahead_g[kHeads], ahead_w[kHeads];
+  auto ask_gates = [&](int chunk) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const int64_t token = first + min(max(chunk, 0) + lane, count - 1);
+      ahead_g[h] = a.decay[token * a.decay_stride + head0 + h];
+      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + h] : 1.0f;
+    }
+  };
+  double behind[kHeads] = {};   // the log2 decays behind the chunk
+  auto sum_gates = [&](int chunk, float (*left)[kChunk]) {
+    const bool there = lane < count - chunk;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const double sum = prefix_sum(there ? log2_of(ahead_g[h]) : 0.0);
+      behind[h] += last_lane(sum);
+      left[h][lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(behind[h] - sum)) * ahead_w[h] : 0.0f;
+    }
+  };
+  if (wave == kWaves - 1) {
+    ask_gates(last);
+    sum_gates(last, left0);
+    ask_gates(last - kChunk);
+  }
+
+  const int sub = lane % 16, row = 4 * half + sub / 4;   // as in the kernel above
+  const int four = (sub % 2) * 2 + sub % 4 / 2;
+  const int turned_k = row * DK + ((2 * (lane / 16 % 2) + four / 2) ^ turn_of<DK>(row)) * 8 + four % 2 * 4;
+  const int turned_v =
+      row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
+
+  f32x16 s[kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) s[i] = f32x16{};
+  auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const uint16_t* tile_v, uint16_t* next_v,
+                  const float (*all)[kChunk], float (*next)[kChunk]) {
+    int at_k = turned_k, at_v = turned_v;
+    asm volatile("" : "+v"(at_k), "+v"(at_v));
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this chunk's rows
+    lds_barrier();
+    if (chunk > 0) ask(chunk - kChunk, next_k, next_v);
+    s16x8 values[2], k[2][kTiles];
+    f32x4 left[2][2];
+    const auto fetch = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) left[step % 2][i] = *reinterpret_cast<const f32x4*>(&all[mine][16 * step + 8 * i + 4 * half]);
+      values[step % 2] = transposed(tile_v + step * 16 * kWidth, at_v, kWidth);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) k[step % 2][i] = transposed(tile_k + step * 16 * DK, at_k ^ (32 * i), DK);
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    fetch(0);
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const int now = step % 2;
+      if (step + 1 < 4) fetch(step + 1);
+      add_products(s, values[now], left[now], k[now]);
+    }
+    if (wave == kWaves - 1 && chunk > 0) {
+      sum_gates(chunk - kChunk, next);
+      ask_gates(chunk - 2 * kChunk);
+    }
+  };
+  for (int chunk = last; chunk >= 0; chunk -= 2 * kChunk) {
+    take(chunk, tile_k0, tile_k1, tile_v0, tile_v1, left0, left1);
+    if (chunk >= kChunk) take(chunk - kChunk, tile_k1, tile_k0, tile_v1, tile_v0, left1, left0);
+  }
+
+  if (wave == kWaves - 1 && lane == 0) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      whole[h] = static_cast<float>(behind[h]);
+      a.totals[static_cast<int64_t>(in + 1) * a.heads + head0 + h] = whole[h];
+    }
+  }
+  lds_barrier();
+  const bool opens = (kind & 1) != 0;
+  const float keep = __builtin_amdgcn_exp2f(whole[mine]);
+  const float* from = a.states + (static_cast<int64_t>(slot) * a.heads + head) * kState;
+  float* kept = a.carried + (static_cast<int64_t>(in) * a.heads + head) * kState;
+  float* to = kept + a.heads * kState;
+  const uint32_t own = 8 * half * DV + 32 * wave % DV + column;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    float before[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) before[e] = opens ? from[own + (32 * i + 16 * (e / 8) + e % 8) * DV] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t at = own + (32 * i + 16 * (e / 8) + e % 8) * DV;
+      if (opens) {
+        kept[at] = before[e];
+        s[i][e] = __builtin_fmaf(before[e], keep, s[i][e]);
+      }
+      to[at] = s[i][e];
+    }
   }
 }
 
@@ -601,10 +734,10 @@ void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t han
   if (steps > 0) linear_step_kernel<DK, DV><<<grid(steps), 256, 0, stream>>>(a);
   // Two heads of 64 columns a workgroup where they share a key head: four waves for two.
   const int share = DV == 64 && a.group % 2 == 0 ? 2 : 1;
-  const auto own_parts = share == 2 ? linear_chunk_kernel<DK, 64, 2, false> : linear_chunk_kernel<DK, DV, 1, false>;
-  const auto contexts = share == 2 ? linear_chunk_kernel<DK, 64, 2, true> : linear_chunk_kernel<DK, DV, 1, true>;
+  const auto parts = share == 2 ? linear_part_kernel<DK, 64, 2> : linear_part_kernel<DK, DV, 1>;
+  const auto contexts = share == 2 ? linear_chunk_kernel<DK, 64, 2> : linear_chunk_kernel<DK, DV, 1>;
   const int threads = 2 * DV * share;
-  if (handed_on > 0) own_parts<<<dim3(static_cast<unsigned>(handed_on * (a.heads / share))), threads, 0, stream>>>(a);
+  if (handed_on > 0) parts<<<dim3(static_cast<unsigned>(handed_on * (a.heads / share))), threads, 0, stream>>>(a);
   if (chains > 0) linear_carry_kernel<<<grid(chains * (DK * DV / 1024)), 256, 0, stream>>>(a, DK * DV);
   if (runs > 0) contexts<<<dim3(static_cast<unsigned>(runs * (a.heads / share))), threads, 0, stream>>>(a);
 }
