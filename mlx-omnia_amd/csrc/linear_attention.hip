@@ -101,7 +101,6 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;
 constexpr int kNoLds = 0x7f;   // what a scheduling barrier lets through: all but LDS's instructions
@@ -182,29 +181,25 @@ struct Rows {
   static constexpr int kTurns = kPass >= 16 ? 1 : 16 / kPass;    // passes whose pieces are turned otherwise
   static constexpr int kPasses = kChunk / kPass;
   static_assert(kPass * kPieces == kThreads && kPasses * kPass == kChunk, "whole passes");
-  int64_t stride;            // bytes
-  uint32_t offset[kTurns];   // of this lane's piece in pass i
-  __device__ __forceinline__ Rows(int64_t row_stride) : stride(2 * row_stride) {
+  uint32_t stride;   // bytes
+  uint32_t first;    // of this lane's row in the first pass
+  uint32_t piece[kTurns];
+  __device__ __forceinline__ Rows(int64_t row_stride)
+      : stride(static_cast<uint32_t>(2 * row_stride)), first(threadIdx.x / kPieces * stride) {
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) offset[i] = threadIdx.x / kPieces * static_cast<uint32_t>(stride) + piece(i);
-  }
-  static __device__ __forceinline__ uint32_t piece(int pass) {
-    return ((threadIdx.x % kPieces) ^ turn_of<D>(threadIdx.x / kPieces + pass * kPass)) * 16;
+    for (int i = 0; i < kTurns; ++i) {
+      piece[i] = ((threadIdx.x % kPieces) ^ turn_of<D>(threadIdx.x / kPieces + i * kPass)) * 16;
+    }
   }
   // Rows past the last of `tokens` come as the last: their weights are zeros, and where that last row
   // is not finite, so is all that it meets.
   __device__ __forceinline__ void ask(const uint16_t* rows, int tokens, uint16_t* tile, int wave) const {
     const char* from = reinterpret_cast<const char*>(rows);
     uint16_t* to = tile + wave * kWave * 8;
-    if (tokens == kChunk) {
+    const uint32_t last = static_cast<uint32_t>(tokens - 1) * stride;
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) load_to_lds(from + i * kPass * stride + offset[i % kTurns], to + i * kThreads * 8);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const uint32_t row = min(static_cast<int>(threadIdx.x) / kPieces + i * kPass, tokens - 1);
-        load_to_lds(from + (row * static_cast<uint32_t>(stride) + piece(i)), to + i * kThreads * 8);
-      }
+    for (int i = 0; i < kPasses; ++i) {
+      load_to_lds(from + (min(first + i * kPass * stride, last) + piece[i % kTurns]), to + i * kThreads * 8);
     }
   }
 };
@@ -363,17 +358,30 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     s16x8 values[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) values[step] = transposed(tile_v + step * 16 * kWidth, at_v, kWidth);
-    __builtin_amdgcn_sched_barrier(kNoLds);
-    f32x16 o[2] = {f32x16{}, f32x16{}};
-    bool slow = false;   // of the wave
-    float odd = 0.0f;
+    // The products of P^T; here and below each step's operands are asked for ahead of the last one's products.
+    s16x8 q[2][2], kq[2];
+    const auto q_of = [&](int i, int step) { return *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step))); };
+    const auto fetch = [&](int step) {
+      kq[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
+      q[step % 2][1] = q_of(1, step);
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    f32x16 p = f32x16{};
+    fetch(0);
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (step + 1 < kSteps) fetch(step + 1);
+      p = product(kq[step % 2], q[step % 2][1], p);
+    }
+    float odd[4] = {};
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       const u32x4 raw = __builtin_bit_cast(u32x4, values[step]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd = dot2_bf16(raw[j], 0u, odd);   // NaN behind a value that is not finite
+      for (int j = 0; j < 4; ++j) odd[j] = dot2_bf16(raw[j], 0u, odd[j]);   // NaN behind a value that is not finite
     }
-    slow = __ballot(odd != odd) != 0;
+    const float none = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+    const bool slow = __ballot(none != none) != 0;   // of the wave
     if (slow) {
       // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
       for (int t = 0; t < tokens; ++t) {
@@ -387,13 +395,13 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int at = t * DK + ((4 * i + 2 * j + half) ^ turn_of<DK>(t)) * 8;
-            float k[8], q[8];
-            unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), k);
-            unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), q);
+            float kr[8], qr[8];
+            unpack8(*reinterpret_cast<const u32x4*>(tile_k + at), kr);
+            unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), qr);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              s[i][8 * j + e] = __builtin_fmaf(k[e], v, s[i][8 * j + e] * keep);
-              sum = __builtin_fmaf(q[e], s[i][8 * j + e], sum);
+              s[i][8 * j + e] = __builtin_fmaf(kr[e], v, s[i][8 * j + e] * keep);
+              sum = __builtin_fmaf(qr[e], s[i][8 * j + e], sum);
             }
           }
         }
@@ -406,73 +414,89 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
     }
     meet();   // v is done with
-    if (more) {
-      ask_k(chunk + kChunk, next_k);
-      ask_v(chunk + kChunk);
-    }
     if (wave == kWaves - 1 && more) {
       sum_gates(chunk + kChunk, next);
       ask_gates(chunk + 2 * kChunk);
     }
-    const auto weigh = [&](const f32x16& p, int tt, int ts) {
-      const int t = 32 * tt + column;
-      // Past this token's place in the part: none of them where the part is not on the diagonal.
-      const int bound = tt == ts ? column - 4 * half : 32;
+
+    // 16 rows s of a part of P^T, weighed: a few at a time, to stand between the products.
+    struct Unit {
+      float hi, lo, x[8];
+      f32x4 his[2], los[2], strengths[2];
+    };
+    const auto look = [&](Unit& u, int h, int j, int tt, int ts) {
+      const int t = 32 * tt + column, at = 32 * ts + 16 * j + 4 * half;
+      u.hi = all[h].hi[t], u.lo = all[h].lo[t];
 #pragma unroll
-      for (int h = 0; h < kHeads; ++h) {
-        const float hi = all[h].hi[t], lo = all[h].lo[t];
-        f32x4 his[4], los[4], strengths[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = 32 * ts + 8 * i + 4 * half;
-          his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at]);
-          los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at]);
-          strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at]);
-        }
-        __builtin_amdgcn_sched_barrier(kNoLds);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = 2 * j + e / 4, n = e % 4;
-            float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f((hi - his[i][n]) + (lo - los[i][n])) * strengths[i][n]);
-            // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
-            // compiler branches around each exponential.)
-            asm("" : "+v"(weight));
-            x[e] = 8 * i + n <= bound ? weight : 0.0f;
-          }
-          const int frag = 2 * tt + 2 * ts + j;
-          weights[h][0][frag][lane] = __builtin_bit_cast(u32x4, cut(x));
-          weights[h][1][frag][lane] = pack8(x);
-        }
+      for (int i = 0; i < 2; ++i) {
+        u.his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at + 8 * i]);
+        u.los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at + 8 * i]);
+        u.strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at + 8 * i]);
       }
     };
-    // q S with the products of P^T; each step's operands are asked for ahead of the last one's products.
-    s16x8 q[2][2], k[2];
-    const auto fetch = [&](int step) {
+    const auto weigh = [&](Unit& u, int j, int tt, int ts, int from, int end) {
+      // Past this token's place in the part: none of them where the part is not on the diagonal.
+      const int bound = tt == ts ? column - 4 * half - 16 * j : 32;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) q[step % 2][i] = *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step)));
-      k[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
+      for (int e = from; e < end; ++e) {
+        const int i = e / 4, n = e % 4;
+        float weight =
+            p[8 * j + e] * (__builtin_amdgcn_exp2f((u.hi - u.his[i][n]) + (u.lo - u.los[i][n])) * u.strengths[i][n]);
+        // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
+        // compiler branches around each exponential.)
+        asm("" : "+v"(weight));
+        u.x[e] = 8 * i + n <= bound ? weight : 0.0f;
+      }
+    };
+    const auto keep_weights = [&](Unit& u, int h, int j, int tt, int ts, bool kept) {
+      const int frag = 2 * tt + 2 * ts + j;
+      const u32x4 high = __builtin_bit_cast(u32x4, cut(u.x)), low = pack8(u.x);
+      if (kept) {
+        weights[h][0][frag][lane] = high;
+        weights[h][1][frag][lane] = low;
+      }
+    };
+    // q S, in two halves with P's weights between the products and the next chunk's rows ahead of them.
+    f32x16 o[2] = {f32x16{}, f32x16{}};
+    const auto fetch_q = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) q[step % 2][i] = q_of(i, step);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
-    f32x16 p = f32x16{};
-    fetch(0);
+    fetch_q(0);
 #pragma unroll
-    for (int step = 0; step < kSteps; ++step) {
-      const int now = step % 2;
-      if (step + 1 < kSteps) fetch(step + 1);
-      float x[8];
+    for (int part = 0; part < 2; ++part) {
+      constexpr int kShare = 8 / (kSteps / 2);
+      if (more) {
+        if (part == 0) ask_k(chunk + kChunk, next_k);
+        else ask_v(chunk + kChunk);
+      }
+      Unit units[kHeads];   // kHeads * 2 of them in all
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
-      const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
-      p = product(k[now], q[now][1], p);
-      o[0] = product(high, q[now][0], o[0]);
-      o[1] = product(high, q[now][1], o[1]);
-      o[0] = product(low, q[now][0], o[0]);
-      o[1] = product(low, q[now][1], o[1]);
+      for (int n = 0; n < kHeads; ++n) look(units[n], (part * kHeads + n) / 2, (part * kHeads + n) % 2, part_t, part_s);
+      __builtin_amdgcn_sched_barrier(kNoLds);
+#pragma unroll
+      for (int i = 0; i < kSteps / 2; ++i) {
+        const int step = part * (kSteps / 2) + i, now = step % 2;
+        if (step + 1 < kSteps) fetch_q(step + 1);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
+        const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
+        o[0] = product(high, q[now][0], o[0]);
+        o[1] = product(high, q[now][1], o[1]);
+        o[0] = product(low, q[now][0], o[0]);
+        o[1] = product(low, q[now][1], o[1]);
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+          weigh(units[n], (part * kHeads + n) % 2, part_t, part_s, kShare * i, kShare * (i + 1));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kHeads; ++n) {
+        keep_weights(units[n], (part * kHeads + n) / 2, (part * kHeads + n) % 2, part_t, part_s, wave < 3);
+      }
     }
-    if (wave < 3) weigh(p, part_t, part_s);
     if (kWaves < 3 && wave == kWaves - 1) {
       p = f32x16{};
 #pragma unroll
@@ -480,7 +504,13 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
         p = product(*reinterpret_cast<const s16x8*>(tile_k + (plain ^ (16 * step))),
                     *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
       }
-      weigh(p, 1, 0);
+#pragma unroll
+      for (int n = 0; n < 2 * kHeads; ++n) {
+        Unit unit;
+        look(unit, n / 2, n % 2, 1, 0);
+        weigh(unit, n % 2, 1, 0, 0, 8);
+        keep_weights(unit, n / 2, n % 2, 1, 0, true);
+      }
     }
     if (wave == 0) {
       const f32x16 first_rows = o[1];
@@ -532,13 +562,20 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
     };
     const auto store = [&](int tt) {
-      const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 4 * half) * 2;
+      const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 8 * half) * 2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x2 packed;
-        packed.x = pack_bf16(o[tt][4 * i], o[tt][4 * i + 1]);
-        packed.y = pack_bf16(o[tt][4 * i + 2], o[tt][4 * i + 3]);
-        __builtin_amdgcn_raw_buffer_store_b64(packed, to, at + 16 * i, 0, 0);
+      for (int i = 0; i < 2; ++i) {
+        // A lane's fours 2 i and 2 i + 1 against the other half's: eight columns each.
+        u32x4 packed;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int e = 8 * i + 2 * n;
+          const auto both = __builtin_amdgcn_permlane32_swap(pack_bf16(o[tt][e], o[tt][e + 1]),
+                                                             pack_bf16(o[tt][e + 4], o[tt][e + 5]), false, false);
+          packed[n] = both[0];
+          packed[2 + n] = both[1];
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(packed, to, at + 32 * i, 0, 0);
       }
     };
     times(0, 0);
