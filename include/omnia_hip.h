@@ -851,6 +851,10 @@ typedef struct {
   int64_t step_count, run_count, handed_on, chain_count, pieces;
   float scale;
 } omnia_linear_attention_t;
+/* How many runs of single heads a card works on at once, for the caller's cut into pieces: as
+ * many as fill it and no more. -EINVAL for a bad geometry. Pure; touches no device. */
+int64_t omnia_linear_attention_places(int64_t heads, int64_t key_heads, int64_t key_dim,
+                                      int64_t value_dim);
 int64_t omnia_linear_attention_workspace_bytes(int64_t heads, int64_t key_dim, int64_t value_dim,
                                                int64_t pieces);
 int32_t omnia_linear_attention(const omnia_linear_attention_t* call, hipStream_t stream);

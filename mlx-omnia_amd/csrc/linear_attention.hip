@@ -102,6 +102,9 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
+#ifndef OMNIA_TRY_SHARE
+#define OMNIA_TRY_SHARE 0
+#endif
 constexpr int kChunk = 64;
 constexpr int kNoLds = 0x7f;   // what a scheduling barrier lets through: all but LDS's instructions
 constexpr double kLog2e = 1.4426950408889634074;
@@ -111,7 +114,7 @@ constexpr double kLog2e = 1.4426950408889634074;
 // every bank once.
 template <int D>
 __device__ __forceinline__ int turn_of(int row) {
-  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
+  return D == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
 }
 
 // Eight fp32 numbers as bf16 operands of the matrix unit: the top halves, cut off (`x` keeps what
@@ -254,6 +257,8 @@ template <int DK, int DV, int kHeads>
 __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(LinearArgs a) {
   constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
+  constexpr int kQuad = kWaves < 4 ? kWaves : 4;           // waves that make P for
+  constexpr int kOwn = kHeads / (kWaves / kQuad);          // so many heads
   __shared__ __attribute__((aligned(16))) uint16_t tile_q[kChunk * DK], tile_k0[kChunk * DK], tile_k1[kChunk * DK];
   __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * kWidth];
   __shared__ u32x4 weights[kHeads][2][6][kWave];   // P^T: parts, (t, 16 s), lanes
@@ -263,6 +268,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   const int blocks = a.heads / kHeads;
   const int entry = blockIdx.x / blocks, head0 = blockIdx.x % blocks * kHeads;
   const int mine = wave * 32 / DV, head = head0 + mine;   // the wave's
+  const int part_of = wave % kQuad, own_heads = wave / kQuad * kOwn;
   const int32_t* run = a.runs + 5 * entry;
   const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
   if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < -1 ||
@@ -290,32 +296,32 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   ask_v(0);
 
   // The decays of the chunk after next are asked for a chunk ahead of their sums.
-  float ahead_g[kHeads], ahead_w[kHeads];
+  float ahead_g[kOwn], ahead_w[kOwn];
   auto ask_gates = [&](int chunk) {
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kOwn; ++h) {
       const int64_t token = first + min(chunk + lane, count - 1);
-      ahead_g[h] = a.decay[token * a.decay_stride + head0 + h];
-      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + h] : 1.0f;
+      ahead_g[h] = a.decay[token * a.decay_stride + head0 + own_heads + h];
+      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + own_heads + h] : 1.0f;
     }
   };
   auto sum_gates = [&](int chunk, Gates* gates) {
     const bool there = lane < count - chunk;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kOwn; ++h) {
       const float g = ahead_g[h], w = there ? ahead_w[h] : 0.0f;
       const double log2 = there ? log2_of(g) : 0.0;
       const double sum = prefix_sum(log2);
       const double end = last_lane(sum);
       const float hi = static_cast<float>(sum);
-      gates[h].hi[lane] = hi;
-      gates[h].lo[lane] = static_cast<float>(sum - hi);
-      gates[h].strength[lane] = w * a.scale;
-      gates[h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
-      gates[h].rate[lane] = static_cast<float>(log2);
+      gates[own_heads + h].hi[lane] = hi;
+      gates[own_heads + h].lo[lane] = static_cast<float>(sum - hi);
+      gates[own_heads + h].strength[lane] = w * a.scale;
+      gates[own_heads + h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
+      gates[own_heads + h].rate[lane] = static_cast<float>(log2);
     }
   };
-  if (wave == kWaves - 1) {
+  if (part_of == kQuad - 1) {
     ask_gates(0);
     sum_gates(0, gates0);
     ask_gates(kChunk);
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
   // The part of P^T that a wave makes: 32 tokens t by 32 s, (0, 0), (1, 1) and (1, 0). (A fourth wave's is
   // not used.)
-  const int part_t = wave == 0 ? 0 : 1, part_s = wave == 1 ? 1 : 0;
+  const int part_t = part_of == 0 ? 0 : 1, part_s = part_of == 1 ? 1 : 0;
 
   auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const Gates* all, Gates* next) {
     const int64_t token0 = first + chunk;
@@ -414,7 +420,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
     }
     meet();   // v is done with
-    if (wave == kWaves - 1 && more) {
+    if (part_of == kQuad - 1 && more) {
       sum_gates(chunk + kChunk, next);
       ask_gates(chunk + 2 * kChunk);
     }
@@ -466,38 +472,35 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     fetch_q(0);
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      constexpr int kShare = 8 / (kSteps / 2);
+      constexpr int kUnitSteps = kSteps / 2 / kOwn, kShare = 8 / kUnitSteps;   // steps of a unit, weights of a step
       if (more) {
         if (part == 0) ask_k(chunk + kChunk, next_k);
         else ask_v(chunk + kChunk);
       }
-      Unit units[kHeads];   // kHeads * 2 of them in all
 #pragma unroll
-      for (int n = 0; n < kHeads; ++n) look(units[n], (part * kHeads + n) / 2, (part * kHeads + n) % 2, part_t, part_s);
-      __builtin_amdgcn_sched_barrier(kNoLds);
+      for (int n = 0; n < kOwn; ++n) {   // 2 kOwn units in all
+        const int h = own_heads + (part * kOwn + n) / 2, j = (part * kOwn + n) % 2;
+        Unit unit;
+        look(unit, h, j, part_t, part_s);
+        __builtin_amdgcn_sched_barrier(kNoLds);
 #pragma unroll
-      for (int i = 0; i < kSteps / 2; ++i) {
-        const int step = part * (kSteps / 2) + i, now = step % 2;
-        if (step + 1 < kSteps) fetch_q(step + 1);
-        float x[8];
+        for (int i = 0; i < kUnitSteps; ++i) {
+          const int step = (part * kOwn + n) * kUnitSteps + i, now = step % 2;
+          if (step + 1 < kSteps) fetch_q(step + 1);
+          float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
-        const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
-        o[0] = product(high, q[now][0], o[0]);
-        o[1] = product(high, q[now][1], o[1]);
-        o[0] = product(low, q[now][0], o[0]);
-        o[1] = product(low, q[now][1], o[1]);
-#pragma unroll
-        for (int n = 0; n < kHeads; ++n) {
-          weigh(units[n], (part * kHeads + n) % 2, part_t, part_s, kShare * i, kShare * (i + 1));
+          for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
+          const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
+          o[0] = product(high, q[now][0], o[0]);
+          o[1] = product(high, q[now][1], o[1]);
+          o[0] = product(low, q[now][0], o[0]);
+          o[1] = product(low, q[now][1], o[1]);
+          weigh(unit, j, part_t, part_s, kShare * i, kShare * (i + 1));
         }
-      }
-#pragma unroll
-      for (int n = 0; n < kHeads; ++n) {
-        keep_weights(units[n], (part * kHeads + n) / 2, (part * kHeads + n) % 2, part_t, part_s, wave < 3);
+        keep_weights(unit, h, j, part_t, part_s, part_of < 3);
       }
     }
-    if (kWaves < 3 && wave == kWaves - 1) {
+    if (kQuad < 3 && part_of == kQuad - 1) {
       p = f32x16{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
@@ -505,14 +508,14 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
                     *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
       }
 #pragma unroll
-      for (int n = 0; n < 2 * kHeads; ++n) {
+      for (int n = 0; n < 2 * kOwn; ++n) {
         Unit unit;
-        look(unit, n / 2, n % 2, 1, 0);
+        look(unit, own_heads + n / 2, n % 2, 1, 0);
         weigh(unit, n % 2, 1, 0, 0, 8);
-        keep_weights(unit, n / 2, n % 2, 1, 0, true);
+        keep_weights(unit, own_heads + n / 2, n % 2, 1, 0, true);
       }
     }
-    if (wave == 0) {
+    if (part_of == 0) {
       const f32x16 first_rows = o[1];
       o[1] = o[0];
       o[0] = first_rows;
@@ -765,22 +768,49 @@ __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int sta
   }
 }
 
+// Heads of a workgroup of the prompts' kernels: those that share a key head, up to 256 columns in
+// 8 waves, which then share the chunk's q and k in LDS.
+int shared_heads(int64_t group, int64_t value_dim) {
+  if (value_dim == 128) return group % 2 == 0 && OMNIA_TRY_SHARE ? 2 : 1;
+  return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+}
+
+template <int DK, int DV, int kHeads>
+void launch_runs(const LinearArgs& a, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
+  const auto grid = [&](int64_t count) { return dim3(static_cast<unsigned>(count * (a.heads / kHeads))); };
+  if (handed_on > 0) linear_part_kernel<DK, DV, kHeads><<<grid(handed_on), 2 * DV * kHeads, 0, stream>>>(a);
+  if (chains > 0) {
+    const auto blocks = static_cast<unsigned>(chains * a.heads * (DK * DV / 1024));
+    linear_carry_kernel<<<dim3(blocks), 256, 0, stream>>>(a, DK * DV);
+  }
+  linear_chunk_kernel<DK, DV, kHeads><<<grid(runs), 2 * DV * kHeads, 0, stream>>>(a);
+}
+
 template <int DK, int DV>
 void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
-  const auto grid = [&](int64_t blocks) { return dim3(static_cast<unsigned>(blocks * a.heads)); };
-  if (steps > 0) linear_step_kernel<DK, DV><<<grid(steps), 256, 0, stream>>>(a);
-  // Two heads of 64 columns a workgroup where they share a key head: four waves for two.
-  const int share = DV == 64 && a.group % 2 == 0 ? 2 : 1;
-  const auto parts = share == 2 ? linear_part_kernel<DK, 64, 2> : linear_part_kernel<DK, DV, 1>;
-  const auto contexts = share == 2 ? linear_chunk_kernel<DK, 64, 2> : linear_chunk_kernel<DK, DV, 1>;
-  const int threads = 2 * DV * share;
-  if (handed_on > 0) parts<<<dim3(static_cast<unsigned>(handed_on * (a.heads / share))), threads, 0, stream>>>(a);
-  if (chains > 0) linear_carry_kernel<<<grid(chains * (DK * DV / 1024)), 256, 0, stream>>>(a, DK * DV);
-  if (runs > 0) contexts<<<dim3(static_cast<unsigned>(runs * (a.heads / share))), threads, 0, stream>>>(a);
+  if (steps > 0) linear_step_kernel<DK, DV><<<dim3(static_cast<unsigned>(steps * a.heads)), 256, 0, stream>>>(a);
+  if (runs == 0) return;
+  const int share = shared_heads(a.group, DV);
+  if constexpr (DV == 64) {
+    if (share == 4) return launch_runs<DK, DV, 4>(a, runs, handed_on, chains, stream);
+  }
+  if (share == 2) return launch_runs<DK, DV, 2>(a, runs, handed_on, chains, stream);
+  launch_runs<DK, DV, 1>(a, runs, handed_on, chains, stream);
 }
 
 }  // namespace
 }  // namespace omnia
+
+extern "C" int64_t omnia_linear_attention_places(int64_t heads, int64_t key_heads, int64_t key_dim, int64_t value_dim) {
+  if (heads <= 0 || heads > 4096 || key_heads <= 0 || heads % key_heads != 0 || (key_dim != 64 && key_dim != 128) ||
+      (value_dim != 64 && value_dim != 128)) {
+    return -EINVAL;
+  }
+  // Workgroups that the LDS of 256 CUs holds, two of four waves or one of eight, times their heads.
+  const int share = omnia::shared_heads(heads / key_heads, value_dim);
+  const bool alone = share * value_dim > 128 || (key_dim == 128 && value_dim == 64 && share == 2);
+  return 256 * share * (alone ? 1 : 2);
+}
 
 extern "C" int64_t omnia_linear_attention_workspace_bytes(int64_t heads, int64_t key_dim, int64_t value_dim, int64_t pieces) {
   if (heads <= 0 || heads > 4096 || (key_dim != 64 && key_dim != 128) || (value_dim != 64 && value_dim != 128) ||

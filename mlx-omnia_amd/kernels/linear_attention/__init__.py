@@ -29,6 +29,7 @@ infinity or a NaN there stays with the tokens from its own on.
 
 from __future__ import annotations
 
+import heapq
 import math
 from collections.abc import Sequence
 from dataclasses import dataclass
@@ -48,8 +49,8 @@ __all__ = ["DefaultLinearAttention", "HipLinearAttention", "LinearAttention", "L
 DIMS = (64, 128)
 CHUNK = 64         # tokens that the kernels and the Core chain take together
 STEP_TOKENS = 4    # up to which a sequence is walked a token at a time
-BLOCKS = 512       # workgroups that a call's chunks are cut into, where they give as many
-MIN_PIECE = 4      # chunks of a piece, about
+MIN_PIECE = 2      # chunks of a piece
+PART, PIECE, LAUNCHES = 0.45, 0.8, 1.6
 
 
 class LinearBatch:
@@ -72,23 +73,27 @@ class LinearBatch:
         self.plans: dict = {}   # what a layer's binding laid out for the batch
         self._lists: dict[int, ops.LinearLists] = {}
 
-    def lists(self, heads: int) -> ops.LinearLists:
-        """What a layer of so many heads does with each sequence, on the device: a token at a time, or
-        in one or several pieces (`omnia_linear_attention`'s steps, runs and chains)."""
-        held = self._lists.get(heads)
+    def lists(self, heads: int, places: int) -> ops.LinearLists:
+        """What a layer of so many heads, of which the card takes `places` at once, does with each
+        sequence, on the device: a token at a time, or in one or several pieces
+        (`omnia_linear_attention`'s steps, runs and chains)."""
+        held = self._lists.get((heads, places))
         if held is None:
             if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise ValueError("a batch's first call cannot be captured: make one before")
             firsts = np.cumsum(self.tokens, dtype=np.int64) - np.asarray(self.tokens, dtype=np.int64)
             steps, handed_on, last, chains, pieces = [], [], [], [], 0
-            chunks = sum(-(-n // CHUNK) for n in self.tokens if n > STEP_TOKENS)
-            longest = max(MIN_PIECE, -(-chunks * heads // BLOCKS))   # chunks of a piece, about
+            short = sum(0 < n <= STEP_TOKENS for n in self.tokens)
+            # A launch of their own where they are all there is, or fill the card by themselves.
+            apart = short * heads >= places or all(n <= STEP_TOKENS for n in self.tokens)
+            longest = piece_chunks([-(-n // CHUNK) for n in self.tokens if n > (STEP_TOKENS if apart else 0)],
+                                   max(1, places // heads))
             for slot, first, count in zip(self.slots, firsts.tolist(), self.tokens):
-                if count <= STEP_TOKENS:
+                if count <= STEP_TOKENS and (apart or not count):
                     steps += [(slot, first, count)] if count else []
                     continue
                 own = -(-count // CHUNK)
-                cut = max(1, round(own / longest))
+                cut = -(-own // longest)
                 size = -(-own // cut) * CHUNK
                 cut = -(-count // size)
                 for i in range(cut):
@@ -101,8 +106,40 @@ class LinearBatch:
             # The longest first: what is left at the end is short.
             for runs in (handed_on, last):
                 runs.sort(key=lambda run: -run[2])
-            held = self._lists[heads] = ops.LinearLists.of(steps, handed_on, last, chains, pieces, self.device)
+            held = self._lists[heads, places] = ops.LinearLists.of(steps, handed_on, last, chains, pieces, self.device)
         return held
+
+
+def _in_turn(lengths: list[float], places: int) -> float:
+    """When the last of these is done, each taken in this order by the place that is free first."""
+    if len(lengths) <= places:
+        return max(lengths, default=0)
+    free = [0] * places
+    for n in lengths:
+        heapq.heapreplace(free, free[0] + n)
+    return max(free)
+
+
+def piece_chunks(chunks: list[int], places: int) -> int:
+    """How many chunks a piece of these sequences has at most, for the least time of all, in chunks:
+    what their contexts take with `places` sequences at a time and, where any is cut, the pieces' own
+    parts ahead of them (PART of it) and two launches (LAUNCHES); PIECE for each piece's states."""
+    if not chunks:
+        return 1
+    most, share = max(chunks), sum(chunks) / places
+    best, least = most, _in_turn(sorted((n + PIECE for n in chunks), reverse=True), places)
+    for longer in (1.0, 1.15, 1.35, 1.6, 2.0, 3.0):
+        size = max(MIN_PIECE, math.ceil(share * longer))
+        if size >= most:
+            break
+        cuts = [(-(-n // size), n) for n in chunks]
+        runs = [(-(-n // cut), cut) for cut, n in cuts]
+        all_pieces = sorted((n + PIECE for n, cut in runs for _ in range(cut)), reverse=True)
+        parts = sorted((n + PIECE for n, cut in runs for _ in range(cut - 1)), reverse=True)
+        time = _in_turn(all_pieces, places) + PART * _in_turn(parts, places) + LAUNCHES
+        if time < least:
+            best, least = size, time
+    return best
 
 
 @runtime_checkable
@@ -192,7 +229,7 @@ class HipLinearAttention(LinearAttentionStrategy):
             return core(batch, queries, keys, values, log_decay, strengths)
         plan, at = batch.plans.get(self, (None, None))
         if plan is None or at != core.states.data_ptr():   # a pool that was given other memory
-            plan, at = ops.LinearAttentionPlan(core.states, batch.lists(core.heads), batch.total, key_heads=core.key_heads,
+            plan, at = ops.LinearAttentionPlan(core.states, batch.lists(core.heads, ops.linear_attention_places(core.states, core.key_heads)), batch.total, key_heads=core.key_heads,
                                                scale=core.scale), core.states.data_ptr()
             batch.plans[self] = plan, at
         return plan(queries, keys, values, gates, strengths)

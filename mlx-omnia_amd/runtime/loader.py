@@ -149,6 +149,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "omnia_attention_batch_step_bytes": (_I64, [_I64] * 8),
     "omnia_attention_batch_step": (_I32, [_P, _P]),
     "omnia_linear_attention_workspace_bytes": (_I64, [_I64] * 4),
+    "omnia_linear_attention_places": (_I64, [_I64] * 4),
     "omnia_linear_attention": (_I32, [_P, _P]),
     "omnia_gated_rms_norm": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F32, _I32, _I32, _P, _P]),
     "omnia_block_norm": (_I32, [_P, _P, _P, _I64, _I32, _P, _F32, _P, _F32, _F32, _F32, _I64, _I64, _P, _P, _P]),

@@ -1864,6 +1864,14 @@ class LinearLists:
         return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces)
 
 
+def linear_attention_places(states: torch.Tensor, key_heads: int) -> int:
+    """How many pieces of single heads the card takes at once; see `omnia_linear_attention_places`."""
+    _, heads, key_dim, value_dim = states.shape
+    places = library().omnia_linear_attention_places(heads, key_heads, key_dim, value_dim)
+    _require(places > 0, "linear_attention: geometry not served")
+    return places
+
+
 class LinearAttentionPlan:
     """A layer's linear attention over one batch, its arguments checked and laid out once for
     `omnia_linear_attention`: what stays the same from call to call. states [slots, heads,

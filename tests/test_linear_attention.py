@@ -95,9 +95,9 @@ def test_lists_cover_every_token_once():
         tokens = [int(2 ** (14 * float(torch.rand(1, generator=gen)))) - 1 for _ in range(count)]
         slots = torch.randperm(count + 3, generator=gen).tolist()[:count]
         heads = (1, 4, 32, 64)[trial % 4]
-        batch = LinearBatch(slots, tokens, device="cpu")
-        lists = batch.lists(heads)
-        assert lists is batch.lists(heads)
+        batch, places = LinearBatch(slots, tokens, device="cpu"), (256, 512, 1024)[trial % 3]
+        lists = batch.lists(heads, places)
+        assert lists is batch.lists(heads, places)
         seen, places = torch.zeros(batch.total, dtype=torch.int64), []
         for slot, first, n in lists.steps.tolist():
             assert tokens[slots.index(slot)] == n
@@ -121,8 +121,8 @@ def test_lists_cover_every_token_once():
         assert sorted(lists.chains.tolist()) == sorted(
             [runs[0][2], len(runs)] for runs in by_slot.values() if len(runs) > 2)
     empty = LinearBatch([], [], device="cpu")
-    assert empty.total == 0 and empty.lists(4).steps.shape == (0, 3) and empty.lists(4).runs.shape == (0, 5)
-    assert LinearBatch([4, 2, 9], [3, 0, 2], device="cpu").lists(4).steps.tolist() == [[4, 0, 3], [9, 3, 2]]
+    assert empty.total == 0 and empty.lists(4, 512).steps.shape == (0, 3) and empty.lists(4, 512).runs.shape == (0, 5)
+    assert LinearBatch([4, 2, 9], [3, 0, 2], device="cpu").lists(4, 512).steps.tolist() == [[4, 0, 3], [9, 3, 2]]
 
 
 def test_a_layer_refuses():
