@@ -159,9 +159,9 @@ __device__ __forceinline__ double last_lane(double value) {
   const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), kWave - 1);
   return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
-// log2 of a decay. Past 2^-512 it leaves nothing of 32 bits, as that does; sums of -inf would differ
-// by NaN.
-__device__ __forceinline__ double log2_of(float g) { return g < -354.0f ? -512.0 : g * kLog2e; }
+// log2 of a decay. Past 2^-160 it leaves nothing of 32 bits, as that does; sums of -inf would differ
+// by NaN, and of larger ones lose more.
+__device__ __forceinline__ double log2_of(float g) { return g < -110.0f ? -160.0 : g * kLog2e; }
 
 // 16 bytes a lane from global memory straight to LDS: lane l's come to `to` + 16 l.
 __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
@@ -233,9 +233,10 @@ __device__ __forceinline__ s16x8 transposed(const uint16_t* tile, int at, int wi
   return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// What a chunk's decays come to: G (in two floats, log2), w * scale, w exp(G_end - G) and g (log2).
+// What a chunk's decays come to: G (log2), w * scale, w exp(G_end - G) and g (log2), and G_end.
 struct Gates {
-  float hi[kChunk], lo[kChunk], strength[kChunk], left[kChunk], rate[kChunk];
+  float sum[kChunk], strength[kChunk], left[kChunk], rate[kChunk], whole;
+  float pad[3];
 };
 
 // A piece of a sequence, for kHeads heads of a key head: a wave holds 32 columns of a head's state in
@@ -248,8 +249,9 @@ struct Gates {
 // transposed in that order: S is an operand of q S, and the columns of P that a wave has made one of
 // P v, as they are. S enters its product as two bf16 parts (16 bits; the result is rounded to 8), P as
 // two, the scaled v, whose sums the state keeps, as three, which hold all of its 24 bits. G is summed
-// in fp64 and held in two floats: its differences are what counts, and a fast decay ahead of a slow
-// one would swallow them.
+// in fp64, and what the state's factors are made of are its differences in fp64: a fast decay ahead of
+// a slow one would swallow the slow one's. P's are of G rounded to fp32, 2^-24 of at most 64 times the
+// fastest decay's 160: 2^-10.6 of a weight where all 64 forget everything and 2^-17 where they halve.
 // The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
 // tiles, v, which is held as operands from the start, and q, done with after the first half, to the
 // same. Its decays are summed by the wave that has no part of P.
@@ -313,9 +315,8 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       const double log2 = there ? log2_of(g) : 0.0;
       const double sum = prefix_sum(log2);
       const double end = last_lane(sum);
-      const float hi = static_cast<float>(sum);
-      gates[own_heads + h].hi[lane] = hi;
-      gates[own_heads + h].lo[lane] = static_cast<float>(sum - hi);
+      gates[own_heads + h].sum[lane] = static_cast<float>(sum);
+      gates[own_heads + h].whole = static_cast<float>(end);   // (by every lane)
       gates[own_heads + h].strength[lane] = w * a.scale;
       gates[own_heads + h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
       gates[own_heads + h].rate[lane] = static_cast<float>(log2);
@@ -337,12 +338,12 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     }
   }
 
-  // Where this lane reads (elements): row `column` of a tile's first 32, piece `half`, whose other
+  // Where this lane reads (elements; the first, in bytes): row `column` of a tile's first 32, piece `half`, whose other
   // pieces and columns are an xor away; transposed, rows 4 half + sub / 4 (8 rows on: their turn is
   // another by 2), the four columns 4 (sub % 4) of 16, of k those that make the state's order.
   const int sub = lane % 16, row = 4 * half + sub / 4;
   const int four = (sub % 2) * 2 + sub % 4 / 2;
-  const int plain = column * DK + (half ^ turn_of<DK>(column)) * 8;
+  const int plain = 2 * (column * DK + (half ^ turn_of<DK>(column)) * 8);   // bytes
   const int turned_k = row * DK + ((2 * (lane / 16 % 2) + four / 2) ^ turn_of<DK>(row)) * 8 + four % 2 * 4;
   const int turned_v =
       row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
@@ -356,20 +357,21 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     const bool more = chunk + kChunk < count;
     const Gates& gates = all[mine];
     // Pinned: what the walk's reads start from is a few numbers, and not one for each of them.
-    int at_k = turned_k, at_v = turned_v, at_s = plain + 32 * part_s * DK;
-    int at_q[2] = {plain + 32 * (1 - part_t) * DK, plain + 32 * part_t * DK};   // the part's t second
-    asm volatile("" : "+v"(at_k), "+v"(at_v), "+v"(at_s), "+v"(at_q[0]), "+v"(at_q[1]));
+    int at_k = turned_k, at_v = turned_v, at_q = plain, at_s = plain + 64 * part_s * DK, at_t = plain + 64 * part_t * DK;
+    asm volatile("" : "+v"(at_k), "+v"(at_v), "+v"(at_q), "+v"(at_s), "+v"(at_t));
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this chunk's rows
     lds_barrier();
     s16x8 values[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) values[step] = transposed(tile_v + step * 16 * kWidth, at_v, kWidth);
     // The products of P^T; here and below each step's operands are asked for ahead of the last one's products.
+    const auto read = [&](const uint16_t* tile, int at, int step) {
+      return *reinterpret_cast<const s16x8*>(reinterpret_cast<const char*>(tile) + (at ^ (32 * step)));
+    };
     s16x8 q[2][2], kq[2];
-    const auto q_of = [&](int i, int step) { return *reinterpret_cast<const s16x8*>(tile_q + (at_q[i] ^ (16 * step))); };
     const auto fetch = [&](int step) {
-      kq[step % 2] = *reinterpret_cast<const s16x8*>(tile_k + (at_s ^ (16 * step)));
-      q[step % 2][1] = q_of(1, step);
+      kq[step % 2] = read(tile_k, at_s, step);
+      q[step % 2][1] = read(tile_q, at_t, step);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     f32x16 p = f32x16{};
@@ -427,16 +429,15 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 
     // 16 rows s of a part of P^T, weighed: a few at a time, to stand between the products.
     struct Unit {
-      float hi, lo, x[8];
-      f32x4 his[2], los[2], strengths[2];
+      float sum, x[8];
+      f32x4 sums[2], strengths[2];
     };
     const auto look = [&](Unit& u, int h, int j, int tt, int ts) {
       const int t = 32 * tt + column, at = 32 * ts + 16 * j + 4 * half;
-      u.hi = all[h].hi[t], u.lo = all[h].lo[t];
+      u.sum = all[h].sum[t];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        u.his[i] = *reinterpret_cast<const f32x4*>(&all[h].hi[at + 8 * i]);
-        u.los[i] = *reinterpret_cast<const f32x4*>(&all[h].lo[at + 8 * i]);
+        u.sums[i] = *reinterpret_cast<const f32x4*>(&all[h].sum[at + 8 * i]);
         u.strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at + 8 * i]);
       }
     };
@@ -446,8 +447,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 #pragma unroll
       for (int e = from; e < end; ++e) {
         const int i = e / 4, n = e % 4;
-        float weight =
-            p[8 * j + e] * (__builtin_amdgcn_exp2f((u.hi - u.his[i][n]) + (u.lo - u.los[i][n])) * u.strengths[i][n]);
+        float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f(u.sum - u.sums[i][n]) * u.strengths[i][n]);
         // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
         // compiler branches around each exponential.)
         asm("" : "+v"(weight));
@@ -466,7 +466,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     f32x16 o[2] = {f32x16{}, f32x16{}};
     const auto fetch_q = [&](int step) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) q[step % 2][i] = q_of(i, step);
+      for (int i = 0; i < 2; ++i) q[step % 2][i] = read(tile_q + 32 * i * DK, at_q, step);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     fetch_q(0);
@@ -504,8 +504,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       p = f32x16{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
-        p = product(*reinterpret_cast<const s16x8*>(tile_k + (plain ^ (16 * step))),
-                    *reinterpret_cast<const s16x8*>(tile_q + 32 * DK + (plain ^ (16 * step))), p);
+        p = product(read(tile_k, at_q, step), read(tile_q + 32 * DK, at_q, step), p);
       }
 #pragma unroll
       for (int n = 0; n < 2 * kOwn; ++n) {
@@ -515,14 +514,9 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
         keep_weights(unit, own_heads + n / 2, n % 2, 1, 0, true);
       }
     }
-    if (part_of == 0) {
-      const f32x16 first_rows = o[1];
-      o[1] = o[0];
-      o[0] = first_rows;
-    }
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      o[tt] *= __builtin_amdgcn_exp2f(gates.hi[32 * tt + column] + gates.lo[32 * tt + column]) * a.scale;
+      o[tt] *= __builtin_amdgcn_exp2f(gates.sum[32 * tt + column]) * a.scale;
     }
     meet();   // P is there, q is done with
     if (more) ask_q(chunk + kChunk);
@@ -547,10 +541,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
-    const float keep_hi = gates.hi[kChunk - 1], keep_lo = gates.lo[kChunk - 1];
+    const float whole = gates.whole;
     fetch_part(0, 0);
     fetch_part(1, 0);
-    const float keep = __builtin_amdgcn_exp2f(keep_hi + keep_lo);
+    const float keep = __builtin_amdgcn_exp2f(whole);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) s[i] *= keep;
     // Rows past the last are out of the buffer, and not written.
