@@ -27,6 +27,7 @@ from ..resolve import record_fallback, resolve
 __all__ = ["BlockNorm", "BlockNormStrategy", "DefaultBlockNorm", "HipBlockNorm", "applies"]
 
 MAX_HIDDEN = 16384
+BF16 = torch.bfloat16
 ACTIVATIONS = (None, "sigmoid")
 
 
@@ -61,6 +62,11 @@ class DefaultBlockNorm(BlockNormStrategy):
                    0.0 if post is None else float(post.eps), residual_scale, block_scale, activation)
 
     def __call__(self, x, block, gate=None):
+        hidden = self.pre.numel()
+        if x.shape != block.shape or x.shape[-1] != hidden:
+            raise ValueError(f"block norm: x {tuple(x.shape)} and block {tuple(block.shape)} are not rows of {hidden}")
+        if gate is not None and gate.shape != x.shape and gate.shape != (hidden,):
+            raise ValueError(f"block norm: a gate {tuple(gate.shape)} for rows {tuple(x.shape)}")
         kind = torch.promote_types(x.dtype, torch.float32)
         y = block.to(kind)
         if self.post is not None:
@@ -84,15 +90,18 @@ class HipBlockNorm(BlockNormStrategy):
                                           activation=activation))
 
     def __call__(self, x, block, gate=None):
-        core = self.core
-        present = [t for t in (x, block, gate) if t is not None]
-        if any(t.dtype != torch.bfloat16 for t in present) or not unfollowed(
-                *present, core.pre, *(() if core.post is None else (core.post,))):
+        core, post = self.core, self.core.post
+        fine = x.dtype is BF16 and block.dtype is BF16
+        if gate is None:
+            fine = fine and (unfollowed(x, block, core.pre) if post is None else unfollowed(x, block, core.pre, post))
+        else:
+            fine = fine and gate.dtype is BF16 and unfollowed(x, block, gate, core.pre, *(() if post is None else (post,)))
+        if not fine:
             record_fallback(self, core)
             return core(x, block, gate)
-        return ops.block_norm(x, block, core.pre, core.post, gate, pre_eps=core.pre_eps, post_eps=core.post_eps,
+        return ops.block_norm(x, block, core.pre, post, gate, pre_eps=core.pre_eps, post_eps=core.post_eps,
                               residual_scale=core.residual_scale, block_scale=core.block_scale,
-                              sigmoid=core.activation == "sigmoid")
+                              sigmoid=core.activation is not None)
 
 
 _STRATEGIES = (HipBlockNorm, DefaultBlockNorm)
@@ -107,15 +116,10 @@ class BlockNorm(BlockNormStrategy):
             raise ValueError("BlockNorm: both norms must have one weight for each value of a row")
         if activation not in ACTIVATIONS:
             raise ValueError(f"BlockNorm: gate activation {activation!r}, not one of {ACTIVATIONS}")
-        self.hidden = pre.weight.numel()
         self.strategy: BlockNormStrategy = resolve(
             (DefaultBlockNorm,) if reference else _STRATEGIES, pre, post, residual_scale=float(residual_scale),
             block_scale=float(block_scale), activation=activation)
 
     def __call__(self, x: torch.Tensor, block: torch.Tensor,
                  gate: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        if x.shape != block.shape or x.shape[-1] != self.hidden:
-            raise ValueError(f"BlockNorm: x {tuple(x.shape)} and block {tuple(block.shape)} are not rows of {self.hidden}")
-        if gate is not None and gate.shape != x.shape and gate.shape != (self.hidden,):
-            raise ValueError(f"BlockNorm: a gate {tuple(gate.shape)} for rows {tuple(x.shape)}")
         return self.strategy(x, block, gate)

@@ -74,7 +74,7 @@ class HipGatedRmsNorm(GatedRmsNormStrategy):
 
     def __call__(self, x, gate):
         core = self.core
-        if x.dtype != torch.bfloat16 or gate.dtype != x.dtype or not unfollowed(x, gate, self.weight):
+        if x.dtype is not torch.bfloat16 or gate.dtype is not torch.bfloat16 or not unfollowed(x, gate, self.weight):
             record_fallback(self, core)
             return core(x, gate)
         return ops.gated_rms_norm(x, gate, self.weight, group=core.group, eps=core.eps, silu=core.activation == "silu",

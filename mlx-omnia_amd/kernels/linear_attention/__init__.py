@@ -73,6 +73,10 @@ class LinearBatch:
         self.plans: dict = {}   # what a layer's binding laid out for the batch
         self._lists: dict[int, ops.LinearLists] = {}
 
+    def check(self, states: torch.Tensor) -> None:
+        if self.slots and max(self.slots) >= states.shape[0]:
+            raise ValueError(f"LinearBatch: slot {max(self.slots)} of a pool of {states.shape[0]}")
+
     def lists(self, heads: int, places: int) -> ops.LinearLists:
         """What a layer of so many heads, of which the card takes `places` at once, does with each
         sequence, on the device: a token at a time, or in one or several pieces
@@ -168,12 +172,26 @@ class DefaultLinearAttention(LinearAttentionStrategy):
     def build(cls, states, *, heads, key_heads, key_dim, value_dim, scale, dtype, decay) -> "DefaultLinearAttention":
         return cls(states, heads, key_heads, scale, decay)
 
+    def _check(self, batch: LinearBatch, queries, keys, values, log_decay, strengths) -> None:
+        n, (_, heads, key_dim, value_dim) = batch.total, self.states.shape
+        of_keys, of_values = (n, self.key_heads, key_dim), (n, heads, value_dim)
+        if queries.shape != of_keys or keys.shape != of_keys or values.shape != of_values:
+            raise ValueError(f"linear attention: the batch's {n} tokens are queries and keys {of_keys} and values {of_values}, "
+                             f"not {tuple(queries.shape)}, {tuple(keys.shape)} and {tuple(values.shape)}")
+        for gates, name in ((log_decay, "log_decay"), (strengths, "strengths")):
+            if gates is not None and gates.shape != (n, heads):
+                raise ValueError(f"linear attention: {name} {(n, heads)}, not {tuple(gates.shape)}")
+        batch.check(self.states)
+
     def _gates(self, batch: LinearBatch, log_decay: torch.Tensor | None) -> torch.Tensor:
         """[N, heads], fp64: its sums lose nothing of a slow decay behind a fast one."""
         gates = self.decay if log_decay is None else log_decay
+        if gates is None:
+            raise ValueError("linear attention: neither the layer nor the call has a decay")
         return gates.double().expand(batch.total, self.heads)
 
     def __call__(self, batch, queries, keys, values, log_decay=None, strengths=None):
+        self._check(batch, queries, keys, values, log_decay, strengths)
         kind = torch.promote_types(queries.dtype, torch.float32)
         group = self.heads // self.key_heads
         q, k = (x.to(kind).repeat_interleave(group, dim=1) for x in (queries, keys))
@@ -223,15 +241,25 @@ class HipLinearAttention(LinearAttentionStrategy):
 
     def __call__(self, batch, queries, keys, values, log_decay=None, strengths=None):
         core = self.core
-        gates = core.decay if log_decay is None else log_decay
-        if not unfollowed(queries, keys, values, gates, core.states, *(() if strengths is None else (strengths,))):
+        gates = log_decay
+        if gates is None:
+            gates = core.decay
+            if gates is None:
+                raise ValueError("linear attention: neither the layer nor the call has a decay")
+        elif gates.dim() != 2:
+            raise ValueError(f"linear attention: log_decay for every token, not {tuple(gates.shape)}")
+        states = core.states
+        if not (unfollowed(queries, keys, values, gates, states) if strengths is None
+                else unfollowed(queries, keys, values, gates, states, strengths)):
             record_fallback(self, core)
             return core(batch, queries, keys, values, log_decay, strengths)
-        plan, at = batch.plans.get(self, (None, None))
-        if plan is None or at != core.states.data_ptr():   # a pool that was given other memory
-            plan, at = ops.LinearAttentionPlan(core.states, batch.lists(core.heads, ops.linear_attention_places(core.states, core.key_heads)), batch.total, key_heads=core.key_heads,
-                                               scale=core.scale), core.states.data_ptr()
-            batch.plans[self] = plan, at
+        plan, at = batch.plans.get(self, (None, 0))
+        if plan is None or at != states.data_ptr():   # a pool that was given other memory
+            batch.check(states)
+            places = ops.linear_attention_places(states, core.key_heads)
+            plan = ops.LinearAttentionPlan(states, batch.lists(core.heads, places), batch.total, key_heads=core.key_heads,
+                                           scale=core.scale)
+            batch.plans[self] = plan, states.data_ptr()
         return plan(queries, keys, values, gates, strengths)
 
 
@@ -253,26 +281,10 @@ class LinearAttention(LinearAttentionStrategy):
             raise ValueError(f"LinearAttention: states in 32 bits or more, not {states.dtype}")
         if decay is not None and decay.shape != (heads,):
             raise ValueError(f"LinearAttention: a decay for each of {heads} heads, not {tuple(decay.shape)}")
-        self.shapes = (key_heads, key_dim), (heads, value_dim), heads
-        self.slots, self.decay, self.device = states.shape[0], decay, states.device
         self.strategy: LinearAttentionStrategy = resolve(
             (DefaultLinearAttention,) if reference else _STRATEGIES, states, heads=heads, key_heads=key_heads,
             key_dim=key_dim, value_dim=value_dim, scale=scale, dtype=dtype, decay=decay)
 
     def __call__(self, batch: LinearBatch, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                  log_decay: torch.Tensor | None = None, strengths: torch.Tensor | None = None) -> torch.Tensor:
-        of_keys, of_values, heads = self.shapes
-        n = batch.total
-        if queries.shape != (n, *of_keys) or keys.shape != (n, *of_keys) or values.shape != (n, *of_values):
-            raise ValueError(f"LinearAttention: the batch's {n} tokens are queries and keys {(n, *of_keys)} and values "
-                             f"{(n, *of_values)}, not {tuple(queries.shape)}, {tuple(keys.shape)} and {tuple(values.shape)}")
-        if log_decay is None:
-            if self.decay is None:
-                raise ValueError("LinearAttention: neither the layer nor the call has a decay")
-        elif log_decay.shape != (n, heads):
-            raise ValueError(f"LinearAttention: log_decay {(n, heads)}, not {tuple(log_decay.shape)}")
-        if strengths is not None and strengths.shape != (n, heads):
-            raise ValueError(f"LinearAttention: strengths {(n, heads)}, not {tuple(strengths.shape)}")
-        if batch.slots and max(batch.slots) >= self.slots:
-            raise ValueError(f"LinearAttention: slot {max(batch.slots)} of a pool of {self.slots}")
         return self.strategy(batch, queries, keys, values, log_decay, strengths)

@@ -1885,7 +1885,8 @@ class LinearAttentionPlan:
         _require(on_rocm(states, lists.steps), "linear_attention: tensors must share one ROCm device")
         slots, heads, key_dim, value_dim = states.shape
         self.held, self.index, self.device = (states.detach(), lists), states.get_device(), states.device
-        self.shapes = (tokens, key_heads, key_dim), (tokens, heads, value_dim), (tokens, heads)
+        self.of_keys, self.of_values, self.of_gates = (tokens, key_heads, key_dim), (tokens, heads, value_dim), (tokens, heads)
+        self.key_width, self.value_width = key_heads * key_dim, heads * value_dim
         self.args = LinearAttentionCall(
             states=states.data_ptr(), steps=lists.steps.data_ptr(), runs=lists.runs.data_ptr(),
             chains=lists.chains.data_ptr(), slots=slots, tokens=tokens, heads=heads, key_heads=key_heads, key_dim=key_dim,
@@ -1893,20 +1894,19 @@ class LinearAttentionPlan:
             handed_on=lists.handed_on, chain_count=lists.chains.shape[0], pieces=lists.pieces, scale=scale)
         nbytes = library().omnia_linear_attention_workspace_bytes(heads, key_dim, value_dim, lists.pieces)
         _require(nbytes >= 0, "linear_attention: geometry not served")
-        self.args.workspace_bytes = nbytes
-        self.like = torch.empty(1, dtype=BF16, device=states.device).expand(self.shapes[1])
+        self.args.workspace_bytes = self.nbytes = nbytes
+        self.like = torch.empty(1, dtype=BF16, device=states.device).expand(self.of_values)
 
-    def _rows(self, rows: torch.Tensor, shape: tuple[int, int, int], name: str) -> tuple[int, int, torch.Tensor]:
+    def _rows(self, rows: torch.Tensor, shape: tuple[int, int, int], width: int, name: str) -> tuple[int, int, torch.Tensor]:
         """(address, row stride, the tensor that holds them) of bf16 rows [tokens, heads, dim], copied
         where the kernel could not read them in place."""
         if rows.shape != shape or rows.dtype is not BF16 or rows.get_device() != self.index:
             raise ValueError(f"{name}: expected {shape} bf16 on {self.device}, not {tuple(rows.shape)} {rows.dtype} on "
                              f"{rows.device}")
-        width = shape[1] * shape[2]
         address, (stride, between, unit) = rows.data_ptr(), rows.stride()
         if shape[0] == 1:
             stride = width   # not used, and not always the row's
-        if (unit != 1 or (between != shape[2] and shape[1] > 1) or stride % 8 or stride < width or stride >= 1 << 24
+        if (unit != 1 or (between != shape[2] and shape[1] > 1) or stride % 8 or stride < width or stride >= 16777216
                 or address % 16):
             rows = rows.clone(memory_format=torch.contiguous_format)
             address, stride = rows.data_ptr(), width
@@ -1914,22 +1914,23 @@ class LinearAttentionPlan:
 
     def _gates(self, gates: torch.Tensor, name: str) -> tuple[int, int, torch.Tensor]:
         """The same of fp32 gates [tokens, heads], or of one row [heads] for all tokens (stride 0)."""
-        shape = self.shapes[2]
-        if gates.dtype is not F32 or gates.get_device() != self.index or gates.shape not in (shape, shape[1:]):
+        shape = self.of_gates
+        if gates.dtype is not F32 or gates.get_device() != self.index or (gates.shape != shape and gates.shape != shape[1:]):
             raise ValueError(f"{name}: expected {shape} fp32 on {self.device}, not {tuple(gates.shape)} {gates.dtype} on "
                              f"{gates.device}")
-        one = gates.dim() == 1
-        if gates.stride(-1) != 1 and shape[1] > 1 or not one and gates.stride(0) < shape[1] and shape[0] > 1:
+        strides = gates.stride()
+        if strides[-1] != 1 or len(strides) == 2 and strides[0] < shape[1]:
             gates = gates.clone(memory_format=torch.contiguous_format)
-        return gates.data_ptr(), 0 if one else gates.stride(0) if shape[0] > 1 else shape[1], gates
+            strides = gates.stride()
+        return gates.data_ptr(), 0 if len(strides) == 1 else strides[0], gates
 
     def __call__(self, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_decay: torch.Tensor,
                  strengths: torch.Tensor | None = None) -> torch.Tensor:
         args = LinearAttentionCall.from_buffer_copy(self.args)   # of this call: two may be under way
-        of_keys, of_values, _ = self.shapes
-        args.queries, args.query_stride, q = self._rows(queries, of_keys, "queries")
-        args.keys, args.key_stride, k = self._rows(keys, of_keys, "keys")
-        args.values, args.value_stride, v = self._rows(values, of_values, "values")
+        of_keys, width = self.of_keys, self.key_width
+        args.queries, args.query_stride, q = self._rows(queries, of_keys, width, "queries")
+        args.keys, args.key_stride, k = self._rows(keys, of_keys, width, "keys")
+        args.values, args.value_stride, v = self._rows(values, self.of_values, self.value_width, "values")
         args.log_decay, args.decay_stride, g = self._gates(log_decay, "log_decay")
         if strengths is not None:
             if strengths.dim() != 2:
@@ -1937,8 +1938,8 @@ class LinearAttentionPlan:
             args.strengths, args.strength_stride, strengths = self._gates(strengths, "strengths")
         out = torch.empty_like(self.like, memory_format=torch.contiguous_format)
         args.out = out.data_ptr()
-        if args.workspace_bytes:
-            workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=self.device)
+        if self.nbytes:
+            workspace = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
             args.workspace = workspace.data_ptr()
         call("omnia_linear_attention", ctypes.addressof(args), _stream_here(self.index))
         del q, k, v, g, strengths   # held until here
@@ -1948,39 +1949,40 @@ class LinearAttentionPlan:
 def _flat_rows(t: torch.Tensor, width: int, name: str) -> tuple[int, int, torch.Tensor]:
     """(address, row stride, the tensor that holds them) of bf16 rows [..., width], copied where a
     kernel could not read them in place."""
-    if t.dtype is not BF16 or t.shape[-1] != width:
+    if t.dtype is not BF16:
         raise ValueError(f"{name}: expected bf16 rows of {width}, not {tuple(t.shape)} {t.dtype}")
-    if t.is_contiguous():
-        stride = width
-    elif t.dim() == 2 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= width:
-        stride = t.stride(0) if t.shape[0] > 1 else width
-    else:
-        t, stride = t.contiguous(), width
-    if t.data_ptr() % 16 and t.numel():
+    stride, address = width, t.data_ptr()
+    if not t.is_contiguous():
+        if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= width:
+            stride = t.stride(0)
+        else:
+            t = t.contiguous()
+            address = t.data_ptr()
+    if address % 16 and t.numel():
         t, stride = t.clone(memory_format=torch.contiguous_format), width
-    return t.data_ptr(), stride, t
+        address = t.data_ptr()
+    return address, stride, t
 
 
 def gated_rms_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, *, group: int, eps: float,
                    silu: bool = True, gate_first: bool = False) -> torch.Tensor:
     """RMSNorm of rows [..., width] in groups with their gate, `norm(x) * weight * act(gate)` or
     `norm(x * act(gate)) * weight`; weight [group] or [width] bf16. See `omnia_gated_rms_norm`."""
-    shape = x.shape
+    shape, index, held = x.shape, x.get_device(), weight.numel()
     if shape != gate.shape:
         raise ValueError(f"gated_rms_norm: x {tuple(shape)} and gate {tuple(gate.shape)} differ")
-    _dense(weight, BF16, "weight")
-    if not on_rocm(x, gate, weight):
+    if index < 0 or gate.get_device() != index or weight.get_device() != index:
         raise ValueError("gated_rms_norm: tensors must share one ROCm device")
-    if len(shape) == 3 and shape[2] == group == weight.numel():   # [rows, heads, group]: rows of all heads
+    _dense(weight, BF16, "weight")
+    if len(shape) == 3 and shape[2] == group == held:   # [rows, heads, group]: rows of all heads
         x, gate = x.flatten(1), gate.flatten(1)
     width = x.shape[-1]
     at, stride, x = _flat_rows(x, width, "x")
     gate_at, gate_stride, gate = _flat_rows(gate, width, "gate")
-    out = torch.empty(shape, dtype=BF16, device=x.device)
-    call("omnia_gated_rms_norm", at, stride, gate_at, gate_stride, weight.data_ptr(), weight.numel(),
-         x.numel() // width if width else 0, width, group, eps, int(silu), int(gate_first), out.data_ptr(),
-         _stream_here(x.get_device()))
-    return out
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    call("omnia_gated_rms_norm", at, stride, gate_at, gate_stride, weight.data_ptr(), held,
+         x.numel() // width if width else 0, width, group, eps, silu, gate_first, out.data_ptr(), _stream_here(index))
+    return out if out.shape == shape else out.view(shape)
 
 
 def block_norm(x: torch.Tensor, block: torch.Tensor, pre_weight: torch.Tensor, post_weight: torch.Tensor | None = None,
@@ -1988,34 +1990,29 @@ def block_norm(x: torch.Tensor, block: torch.Tensor, pre_weight: torch.Tensor, p
                block_scale: float = 1.0, sigmoid: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """`(s, norm(s) * pre_weight)` of rows [..., hidden] with `s = residual_scale * x + block_scale *
     act(gate) * norm(block) * post_weight`; gate like x, or one row [hidden]. See `omnia_block_norm`."""
-    hidden = pre_weight.numel()
-    if x.shape != block.shape or x.shape[-1] != hidden:
-        raise ValueError(f"block_norm: x {tuple(x.shape)} and block {tuple(block.shape)} are not rows of {hidden}")
-    held = [x, block, pre_weight]
-    for weight, name in ((pre_weight, "pre_weight"), (post_weight, "post_weight")):
-        if weight is not None:
-            _dense(weight, BF16, name)
-            if weight.numel() != hidden:
-                raise ValueError(f"{name}: must be [hidden]")
-    gate_at, gate_stride = None, 0
-    if post_weight is not None:
-        held.append(post_weight)
-    if gate is not None:
-        if gate.shape != x.shape and gate.shape != (hidden,):
-            raise ValueError(f"block_norm: a gate {tuple(gate.shape)} for rows {tuple(x.shape)}")
-        held.append(gate)
-    if not on_rocm(*held):
+    hidden, shape, index = pre_weight.numel(), x.shape, x.get_device()
+    if shape != block.shape or shape[-1] != hidden:
+        raise ValueError(f"block_norm: x {tuple(shape)} and block {tuple(block.shape)} are not rows of {hidden}")
+    if index < 0 or block.get_device() != index or pre_weight.get_device() != index:
         raise ValueError("block_norm: tensors must share one ROCm device")
+    _dense(pre_weight, BF16, "pre_weight")
+    post_at = gate_at = None
+    gate_stride = 0
+    if post_weight is not None:
+        _dense(post_weight, BF16, "post_weight")
+        if post_weight.numel() != hidden or post_weight.get_device() != index:
+            raise ValueError("post_weight: must be [hidden], beside the rows")
+        post_at = post_weight.data_ptr()
     if gate is not None:
-        one = gate.dim() == 1 and x.dim() != 1
+        one = gate.dim() == 1 and len(shape) != 1
+        if (gate.shape != shape and gate.shape != (hidden,)) or gate.get_device() != index:
+            raise ValueError(f"block_norm: a gate {tuple(gate.shape)} on {gate.device} for rows {tuple(shape)} on {x.device}")
         gate_at, gate_stride, gate = _flat_rows(gate, hidden, "gate")
         gate_stride = 0 if one else gate_stride
-    x, block = x.contiguous(), block.contiguous()
-    _dense(x, BF16, "x")
-    _dense(block, BF16, "block")
+    at, _, x = _flat_rows(x if x.is_contiguous() else x.contiguous(), hidden, "x")
+    block_at, _, block = _flat_rows(block if block.is_contiguous() else block.contiguous(), hidden, "block")
     summed, normalized = torch.empty_like(x), torch.empty_like(x)
-    call("omnia_block_norm", x.data_ptr(), block.data_ptr(), gate_at, gate_stride, int(sigmoid),
-         post_weight.data_ptr() if post_weight is not None else None, post_eps, pre_weight.data_ptr(), pre_eps,
+    call("omnia_block_norm", at, block_at, gate_at, gate_stride, sigmoid, post_at, post_eps, pre_weight.data_ptr(), pre_eps,
          residual_scale, block_scale, x.numel() // hidden, hidden, summed.data_ptr(), normalized.data_ptr(),
-         _stream_here(x.get_device()))
+         _stream_here(index))
     return summed, normalized
