@@ -93,7 +93,8 @@ __device__ __forceinline__ float block_sum(float v, float* parts) {
   return v;
 }
 
-// A row per workgroup of kWaves, kVectors 16-byte vectors a lane.
+// A row per workgroup of kWaves, kVectors 16-byte vectors a lane, read past the caches (8,192 rows of
+// 5,120 with a gate: 76.2 -> 71.8 us; the stores past them as well 72.0, and what follows reads those).
 template <int kWaves, int kVectors>
 __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
   constexpr int kThreads = 64 * kWaves;
@@ -106,9 +107,9 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
     const int at = threadIdx.x + i * kThreads;
     const bool there = at < a.vectors;
     const u32x4 zero = u32x4{0, 0, 0, 0};
-    bs[i] = there ? *reinterpret_cast<const u32x4*>(a.block + first + at * 8) : zero;
-    xs[i] = there ? *reinterpret_cast<const u32x4*>(a.x + first + at * 8) : zero;
-    gs[i] = there && a.gate ? *reinterpret_cast<const u32x4*>(a.gate + row * a.gate_stride + at * 8) : zero;
+    bs[i] = there ? load_nt(reinterpret_cast<const u32x4*>(a.block + first + at * 8)) : zero;
+    xs[i] = there ? load_nt(reinterpret_cast<const u32x4*>(a.x + first + at * 8)) : zero;
+    gs[i] = there && a.gate ? load_nt(reinterpret_cast<const u32x4*>(a.gate + row * a.gate_stride + at * 8)) : zero;
     posts[i] = there && a.post ? *reinterpret_cast<const u32x4*>(a.post + at * 8) : zero;
     pres[i] = there ? *reinterpret_cast<const u32x4*>(a.pre + at * 8) : zero;
   }

@@ -5,7 +5,10 @@
 //
 // Steps: a workgroup takes one head of one sequence with its whole state in registers (64 KB at
 // 128 x 128, 16 vectors of 16 bytes a lane, all asked for at once), so a step of one token reads
-// and writes the state once and is bound by that.
+// and writes the state once and is bound by that. Both go past the caches, as the states of all layers
+// do not stay in them: 64 requests of 32 heads of 128 x 128, 268 MB, 57.5 -> 50.2 us over pools in turn
+// (45 -> 50 for one of 134 MB over and over, half of which the last-level cache keeps); 200 of 64 heads
+// of 128 x 64, 839 MB, 167 -> 156 us (5.4 TB/s).
 //
 // Prompts: a workgroup takes one head of one piece of a sequence, 64 tokens at a time on the matrix
 // unit. Where the sequences are too few to fill the card each is cut into pieces: the pieces' own
@@ -43,7 +46,7 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
   float* state = a.states + (static_cast<int64_t>(slot) * a.heads + head) * (DK * DV) + row * DV + 4 * column;
   f32x4 s[kPasses];
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) s[i] = *reinterpret_cast<const f32x4*>(state + i * kRows * DV);
+  for (int i = 0; i < kPasses; ++i) s[i] = load_nt(reinterpret_cast<const f32x4*>(state + i * kRows * DV));
   const int shared = head / a.group;
   for (int t = 0; t < count; ++t) {
     const int64_t token = first + t;
@@ -94,7 +97,7 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) *reinterpret_cast<f32x4*>(state + i * kRows * DV) = s[i];
+  for (int i = 0; i < kPasses; ++i) store_nt(reinterpret_cast<f32x4*>(state + i * kRows * DV), s[i]);
 }
 
 // ---- prompts: 64 tokens at a time ---------------------------------------------------------
@@ -741,8 +744,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_part_kernel(LinearA
 }
 
 // The states ahead of a sequence's third piece on, from what each piece before added:
-// X_p = 2^total X_{p-1} + U_p, in place.
+// X_p = 2^total X_{p-1} + U_p, in place, eight pieces' asked for together. (With pieces that sum them
+// as they begin, and no launch for it, 12 sequences in up to three pieces took 94.2 us for 93.7.)
 __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int state) {
+  constexpr int kAhead = 8;
   const int per_head = state / (256 * 4);   // workgroups
   const int part = blockIdx.x % per_head;
   const int head = blockIdx.x / per_head % a.heads, chain = blockIdx.x / per_head / a.heads;
@@ -750,15 +755,25 @@ __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int sta
   if (at < 0 || count < 3 || count > a.pieces - at) return;
   const int64_t between = static_cast<int64_t>(a.heads) * state;
   float* x = a.carried + (static_cast<int64_t>(at + 1) * a.heads + head) * state + (part * 256 + threadIdx.x) * 4;
+  const float* totals = a.totals + static_cast<int64_t>(at) * a.heads + head;
   f32x4 sum = *reinterpret_cast<const f32x4*>(x);
-#pragma unroll 4
-  for (int p = 2; p < count; ++p) {
-    x += between;
-    const float keep = __builtin_amdgcn_exp2f(a.totals[static_cast<int64_t>(at + p) * a.heads + head]);
-    const f32x4 own = *reinterpret_cast<const f32x4*>(x);
+  for (int p = 2; p < count; p += kAhead) {
+    f32x4 own[kAhead];
+    float keep[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(sum[j], keep, own[j]);
-    *reinterpret_cast<f32x4*>(x) = sum;
+    for (int i = 0; i < kAhead; ++i) {
+      const int n = min(p + i, count - 1);
+      own[i] = *reinterpret_cast<const f32x4*>(x + (n - 1) * between);
+      keep[i] = totals[static_cast<int64_t>(n) * a.heads];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (p + i >= count) break;
+      const float factor = __builtin_amdgcn_exp2f(keep[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(sum[j], factor, own[i][j]);
+      *reinterpret_cast<f32x4*>(x + (p + i - 1) * between) = sum;
+    }
   }
 }
 
