@@ -56,7 +56,8 @@ PART, PIECE, LAUNCHES = 0.45, 0.8, 1.6
 class LinearBatch:
     """The sequences of a call: the slots of their states, each once, and how many new tokens each
     has (none among them). Their rows lie together in the call's tensors, in this order. Made on
-    the host and kept as long as the same slots step on."""
+    the host and kept as long as the same slots step on, or a graph that took a call of it is
+    replayed."""
 
     def __init__(self, slots: Sequence[int], tokens: Sequence[int], *, device: torch.device | str = "cuda") -> None:
         self.slots, self.tokens = tuple(int(s) for s in slots), tuple(int(n) for n in tokens)
@@ -217,8 +218,8 @@ class DefaultLinearAttention(LinearAttentionStrategy):
                 state = state * torch.exp(to[:, -1]).to(kind)[:, None, None] + (
                     ks * left[..., None]).transpose(1, 2).contiguous() @ vs
             if count:
-                # The pool itself follows no gradient.
-                self.states[slot] = state.detach().to(self.states.dtype)
+                with torch.no_grad():   # the pool itself follows no gradient
+                    self.states[slot] = state.to(self.states.dtype)
             end += count
         return torch.cat(out).to(queries.dtype) if out else torch.zeros_like(values)
 

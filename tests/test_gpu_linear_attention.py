@@ -14,6 +14,7 @@ from mlx_omnia_amd.kernels.block_norm import BlockNorm, HipBlockNorm
 from mlx_omnia_amd.kernels.gate_softplus import GateSoftplus
 from mlx_omnia_amd.kernels.gated_norm import GatedRmsNorm, HipGatedRmsNorm
 from mlx_omnia_amd.kernels.leaf import RMSNormLeaf
+from mlx_omnia_amd.kernels import linear_attention
 from mlx_omnia_amd.kernels.linear_attention import HipLinearAttention, LinearAttention, LinearBatch
 from mlx_omnia_amd.kernels.resolve import FALLBACKS
 
@@ -56,6 +57,56 @@ def test_lengths(count):
 @pytest.mark.parametrize("strengths", [False, True])
 def test_heads_and_gates(heads, key_heads, decay, strengths):
     run([1, 77], heads, key_heads, 128, 64, decay=decay, strengths=strengths, fused=True)
+
+
+GEOMETRIES = [(2, 2, 128, 128), (2, 1, 64, 128), (3, 3, 128, 64), (4, 2, 128, 64), (4, 1, 128, 64), (8, 1, 64, 64),
+              (6, 3, 64, 64), (1, 1, 64, 64)]
+
+
+@pytest.mark.parametrize("size", [1, 2, 5])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+def test_in_pieces(monkeypatch, size, heads, key_heads, key_dim, value_dim):
+    """Pieces of so many chunks: sequences of one, two, three and many, whatever the plan would do."""
+    monkeypatch.setattr(linear_attention, "piece_chunks", lambda chunks, places: size)
+    run([700, 2, 129, 64, 65, 0, 300], heads, key_heads, key_dim, value_dim, strengths=True, fused=True)
+
+
+@pytest.mark.parametrize("where", ["values", "keys", "strengths", "log_decay"])
+@pytest.mark.parametrize("at", [0, 63, 200, 449])
+def test_in_pieces_what_is_not_finite_stays_with_later_tokens(monkeypatch, where, at):
+    monkeypatch.setattr(linear_attention, "piece_chunks", lambda chunks, places: 2)
+    made, _, states, slots = inputs([450], 4, 1, 128, 64, device="cuda", strengths=True)
+    plain, _, clean, _ = inputs([450], 4, 1, 128, 64, device="cuda", strengths=True)
+    made[where].reshape(450, -1)[at, 5 if where in ("values", "keys") else 1] = math.nan
+    out = layer(states, 1)(LinearBatch(slots, [450]), **made)
+    want = layer(clean, 1)(LinearBatch(slots, [450]), **plain)
+    assert torch.isfinite(out[:at]).all()
+    torch.testing.assert_close(out[:at].float(), want[:at].float(), rtol=2 ** -7, atol=2 ** -10)
+    head, columns = (0, slice(5, 6)) if where == "values" else (slice(None), slice(None)) if where == "keys" else (
+        1, slice(None))
+    assert not torch.isfinite(out[at:, head, columns]).any() and not torch.isfinite(out[449, head, columns]).any()
+    state = states[slots[0]]
+    assert not torch.isfinite(state[head, 5 if where == "keys" else slice(None), columns]).any()
+    if where != "keys":
+        other = torch.ones_like(out, dtype=torch.bool)
+        other[:, head, columns] = False
+        assert torch.isfinite(out[other]).all()
+
+
+def test_far_offsets():
+    """States past 2^31 elements and 2^33 bytes from the first, rows 2^23 elements apart."""
+    heads, d, tokens = 8, 64, [70, 1]
+    made, _, small, slots = inputs(tokens, heads, 2, d, d, device="cuda", slots=4, strengths=True)
+    before = small.clone()
+    want = layer(small, 2)(LinearBatch(slots, tokens), **made)
+    pool = torch.empty(70000, heads, d, d, device="cuda")   # 9.2 GB
+    far = [69999 - s for s in slots]
+    pool[far] = before[slots]
+    wide = torch.empty(71, 1 << 23, dtype=torch.bfloat16, device="cuda")   # 1.2 GB, 0.6 G elements
+    rows = {name: torch.as_strided(wide, t.shape, (1 << 23, t.shape[2], 1), 1 << 12).copy_(t)
+            for name, t in (("queries", made["queries"]),)}
+    got = layer(pool, 2)(LinearBatch(far, tokens), **{**made, **rows})
+    assert torch.equal(got, want) and torch.equal(pool[far], small[slots])
 
 
 def test_sequences_of_all_lengths():
@@ -202,13 +253,37 @@ def test_followed_calls_and_other_types_run_in_torch():
         "HipLinearAttention -> DefaultLinearAttention", 0) + 1
 
 
+def test_many_batches_over_the_same_pool():
+    """Slots in turn, a fork's copy and a fresh one's zeros between calls, on one stream."""
+    heads, d = 4, 64
+    made, _, states, _ = inputs([200], heads, 2, d, d, device="cuda", slots=6)
+    other, mixer = states.clone(), layer(states, 2)
+    reference = layer(other, 2, reference=True)
+    for slots, tokens in (([0, 3], [100, 1]), ([3, 5], [1, 1]), ([1, 0], [64, 65]), ([2], [200]), ([0, 1, 2], [3, 4, 5])):
+        n = sum(tokens)
+        part = {k: None if t is None else t[:n] for k, t in made.items()}
+        for pool in (states, other):
+            pool[4].zero_()
+            pool[5] = pool[0]
+        batch = LinearBatch(slots, tokens)
+        got, want = mixer(batch, **part), reference(batch, **part)
+        torch.testing.assert_close(got.float(), want.float(), rtol=2 ** -7, atol=2 ** -8)
+        torch.testing.assert_close(states, other, rtol=2 ** -14, atol=2 ** -14)
+
+
 def test_refusals():
     made, _, states, slots = inputs([5], 4, 2, 64, 64, device="cuda")
     mixer, batch = layer(states, 2), LinearBatch(slots, [5])
     for change in (dict(queries=made["queries"].float()), dict(keys=made["keys"].cpu()),
-                   dict(log_decay=made["log_decay"].bfloat16()), dict(strengths=torch.ones(5, 4))):
+                   dict(log_decay=made["log_decay"].bfloat16()), dict(strengths=torch.ones(5, 4)), dict(log_decay=None),
+                   dict(queries=made["queries"][:4]), dict(values=made["values"][:, :2]),
+                   dict(log_decay=made["log_decay"][0]), dict(strengths=torch.ones(4, device="cuda"))):
         with pytest.raises(ValueError):
             mixer(batch, **{**made, **change})
+    with pytest.raises(ValueError):
+        mixer(LinearBatch([len(states)], [5]), **made)
+    with pytest.raises(ValueError):
+        mixer(LinearBatch(slots, [5], device="cpu"), **made)
     odd = LinearAttention(torch.zeros(2, 4, 96, 64, device="cuda"), heads=4, key_heads=2, key_dim=96, value_dim=64,
                           scale=1.0, dtype=torch.bfloat16)
     assert not isinstance(odd.strategy, HipLinearAttention)

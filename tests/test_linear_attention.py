@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from linear_cases import check, inputs
-from mlx_omnia_amd.kernels.linear_attention import DefaultLinearAttention, LinearAttention, LinearBatch, applies
+from mlx_omnia_amd.kernels.linear_attention import (DefaultLinearAttention, LinearAttention, LinearBatch, applies,
+                                                    piece_chunks)
 
 
 def layer(states, key_heads, decay=None, **more):
@@ -157,3 +158,22 @@ def test_which_geometries_the_kernels_take():
     assert applies(32, 16, 128, 128) and applies(64, 1, 128, 64) and applies(6, 2, 64, 128)
     assert not applies(32, 16, 96, 128) and not applies(32, 16, 128, 256) and not applies(5, 2, 64, 64)
     assert not applies(0, 1, 64, 64) and not applies(8192, 1, 64, 64)
+
+
+def test_a_pool_that_is_a_parameter_is_moved_on_without_gradients():
+    made, _, states, slots = inputs([70], 2, 1, 16, 8, slots=1)
+    clean, pool = states.clone(), torch.nn.Parameter(states.clone())
+    want = layer(clean, 1)(LinearBatch(slots, [70], device="cpu"), **made)
+    leaf = made["values"].clone().requires_grad_()
+    out = layer(pool, 1)(LinearBatch(slots, [70], device="cpu"), **{**made, "values": leaf})
+    assert torch.equal(out, want) and torch.equal(pool.detach(), clean)
+    out.float().sum().backward()
+    assert pool.grad is None and torch.isfinite(leaf.grad).all()
+
+
+def test_pieces_for_the_least_time():
+    assert piece_chunks([], 4) == 1 and piece_chunks([5], 1) == 5 and piece_chunks([1] * 40, 16) == 1
+    assert piece_chunks([512], 16) == 32            # as many pieces as places
+    assert piece_chunks([64] * 16, 16) == 64        # all places taken: whole
+    for chunks, places in (([24, 13, 2, 14, 1], 16), ([300, 1, 1], 8), ([7] * 50, 4)):
+        assert 1 <= piece_chunks(chunks, places) <= max(chunks)
