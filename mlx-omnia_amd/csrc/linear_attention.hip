@@ -236,6 +236,12 @@ __device__ __forceinline__ s16x8 transposed(const uint16_t* tile, int at, int wi
   return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Where a lane's i-th four of its state's rows lie in the workspace's states: lane by lane, 16 bytes each.
+template <int DK, int DV>
+__device__ __forceinline__ uint32_t held_at(int wave, int lane, int i) {
+  return ((wave % (DV / 32) * (DK / 8) + i) * kWave + lane) * 4;
+}
+
 // What a chunk's decays come to: G (log2), w * scale, w exp(G_end - G) and g (log2), and G_end.
 struct Gates {
   float sum[kChunk], strength[kChunk], left[kChunk], rate[kChunk], whole;
@@ -333,11 +339,21 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 
   f32x16 s[kTiles];
   {
-    const float* from = in < 0 ? a.states + state_at : a.carried + (static_cast<int64_t>(in) * a.heads + head) * kState;
+    if (in >= 0) {
+      const float* from = a.carried + (static_cast<int64_t>(in) * a.heads + head) * kState;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
+      for (int i = 0; i < 4 * kTiles; ++i) {
+        const f32x4 four = *reinterpret_cast<const f32x4*>(from + held_at<DK, DV>(wave, lane, i));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[i][e] = from[own + (32 * i + 16 * (e / 8) + e % 8) * DV];
+        for (int e = 0; e < 4; ++e) s[i / 4][4 * (i % 4) + e] = four[e];
+      }
+    } else {
+      const float* from = a.states + state_at;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[i][e] = from[own + (32 * i + 16 * (e / 8) + e % 8) * DV];
+      }
     }
   }
 
@@ -732,13 +748,17 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_part_kernel(LinearA
 #pragma unroll
     for (int e = 0; e < 16; ++e) before[e] = opens ? from[own + (32 * i + 16 * (e / 8) + e % 8) * DV] : 0.0f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint32_t at = own + (32 * i + 16 * (e / 8) + e % 8) * DV;
+    for (int n = 0; n < 4; ++n) {
+      const uint32_t at = held_at<DK, DV>(wave, lane, 4 * i + n);
+      f32x4 sums;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[e] = __builtin_fmaf(before[4 * n + e], keep, s[i][4 * n + e]);
       if (opens) {
-        kept[at] = before[e];
-        s[i][e] = __builtin_fmaf(before[e], keep, s[i][e]);
+        *reinterpret_cast<f32x4*>(kept + at) = f32x4{before[4 * n], before[4 * n + 1], before[4 * n + 2], before[4 * n + 3]};
+      } else {
+        sums = f32x4{s[i][4 * n], s[i][4 * n + 1], s[i][4 * n + 2], s[i][4 * n + 3]};   // (not 0 times what keep may be)
       }
-      to[at] = s[i][e];
+      *reinterpret_cast<f32x4*>(to + at) = sums;
     }
   }
 }
