@@ -105,9 +105,6 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
-#ifndef OMNIA_TRY_SHARE
-#define OMNIA_TRY_SHARE 0
-#endif
 constexpr int kChunk = 64;
 constexpr int kNoLds = 0x7f;   // what a scheduling barrier lets through: all but LDS's instructions
 constexpr double kLog2e = 1.4426950408889634074;
@@ -268,18 +265,21 @@ template <int DK, int DV, int kHeads>
 __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(LinearArgs a) {
   constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
-  constexpr int kQuad = kWaves < 4 ? kWaves : 4;           // waves that make P for
-  constexpr int kOwn = kHeads / (kWaves / kQuad);          // so many heads
   __shared__ __attribute__((aligned(16))) uint16_t tile_q[kChunk * DK], tile_k0[kChunk * DK], tile_k1[kChunk * DK];
-  __shared__ __attribute__((aligned(16))) uint16_t tile_v[kChunk * kWidth];
-  __shared__ u32x4 weights[kHeads][2][6][kWave];   // P^T: parts, (t, 16 s), lanes
+  // P^T: parts, (t, 16 s), lanes. Two heads' lies where v did, which is read first, or the LDS would hold
+  // one workgroup a CU for two; v of the next chunk is then asked for later.
+  constexpr bool kOver = DK == 128 && kHeads == 2;
+  constexpr int kWeights = kHeads * 2 * 6 * kWave;
+  __shared__ u32x4 held[kOver ? kWeights : kChunk * kWidth / 8], apart[kOver ? 1 : kWeights];
+  uint16_t* const tile_v = reinterpret_cast<uint16_t*>(held);
+  u32x4* const weights = (kOver ? held : apart) + (threadIdx.x % kWave);
+  const auto weight_at = [](int h, int part, int frag) { return ((h * 2 + part) * 6 + frag) * kWave; };
   __shared__ __attribute__((aligned(16))) Gates gates0[kHeads], gates1[kHeads];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane / 32, column = lane % 32;
   const int blocks = a.heads / kHeads;
   const int entry = blockIdx.x / blocks, head0 = blockIdx.x % blocks * kHeads;
   const int mine = wave * 32 / DV, head = head0 + mine;   // the wave's
-  const int part_of = wave % kQuad, own_heads = wave / kQuad * kOwn;
   const int32_t* run = a.runs + 5 * entry;
   const int slot = run[0], first = run[1], count = run[2], in = run[3], kind = run[4];
   if (slot < 0 || slot >= a.slots || first < 0 || count <= 0 || count > a.tokens - first || in < -1 ||
@@ -307,31 +307,31 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   ask_v(0);
 
   // The decays of the chunk after next are asked for a chunk ahead of their sums.
-  float ahead_g[kOwn], ahead_w[kOwn];
+  float ahead_g[kHeads], ahead_w[kHeads];
   auto ask_gates = [&](int chunk) {
 #pragma unroll
-    for (int h = 0; h < kOwn; ++h) {
+    for (int h = 0; h < kHeads; ++h) {
       const int64_t token = first + min(chunk + lane, count - 1);
-      ahead_g[h] = a.decay[token * a.decay_stride + head0 + own_heads + h];
-      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + own_heads + h] : 1.0f;
+      ahead_g[h] = a.decay[token * a.decay_stride + head0 + h];
+      ahead_w[h] = a.strength != nullptr ? a.strength[token * a.strength_stride + head0 + h] : 1.0f;
     }
   };
   auto sum_gates = [&](int chunk, Gates* gates) {
     const bool there = lane < count - chunk;
 #pragma unroll
-    for (int h = 0; h < kOwn; ++h) {
+    for (int h = 0; h < kHeads; ++h) {
       const float g = ahead_g[h], w = there ? ahead_w[h] : 0.0f;
       const double log2 = there ? log2_of(g) : 0.0;
       const double sum = prefix_sum(log2);
       const double end = last_lane(sum);
-      gates[own_heads + h].sum[lane] = static_cast<float>(sum);
-      gates[own_heads + h].whole = static_cast<float>(end);   // (by every lane)
-      gates[own_heads + h].strength[lane] = w * a.scale;
-      gates[own_heads + h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
-      gates[own_heads + h].rate[lane] = static_cast<float>(log2);
+      gates[h].sum[lane] = static_cast<float>(sum);
+      gates[h].whole = static_cast<float>(end);   // (by every lane)
+      gates[h].strength[lane] = w * a.scale;
+      gates[h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
+      gates[h].rate[lane] = static_cast<float>(log2);
     }
   };
-  if (part_of == kQuad - 1) {
+  if (wave == kWaves - 1) {
     ask_gates(0);
     sum_gates(0, gates0);
     ask_gates(kChunk);
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       row * kWidth + ((4 * wave + 2 * (lane / 16 % 2) + sub % 4 / 2) ^ turn_of<kWidth>(row)) * 8 + sub % 2 * 4;
   // The part of P^T that a wave makes: 32 tokens t by 32 s, (0, 0), (1, 1) and (1, 0). (A fourth wave's is
   // not used.)
-  const int part_t = part_of == 0 ? 0 : 1, part_s = part_of == 1 ? 1 : 0;
+  const int part_t = wave == 0 ? 0 : 1, part_s = wave == 1 ? 1 : 0;
 
   auto take = [&](int chunk, const uint16_t* tile_k, uint16_t* next_k, const Gates* all, Gates* next) {
     const int64_t token0 = first + chunk;
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
     }
     meet();   // v is done with
-    if (part_of == kQuad - 1 && more) {
+    if (wave == kWaves - 1 && more) {
       sum_gates(chunk + kChunk, next);
       ask_gates(chunk + 2 * kChunk);
     }
@@ -477,8 +477,8 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       const int frag = 2 * tt + 2 * ts + j;
       const u32x4 high = __builtin_bit_cast(u32x4, cut(u.x)), low = pack8(u.x);
       if (kept) {
-        weights[h][0][frag][lane] = high;
-        weights[h][1][frag][lane] = low;
+        weights[weight_at(h, 0, frag)] = high;
+        weights[weight_at(h, 1, frag)] = low;
       }
     };
     // q S, in two halves with P's weights between the products and the next chunk's rows ahead of them.
@@ -491,20 +491,20 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     fetch_q(0);
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      constexpr int kUnitSteps = kSteps / 2 / kOwn, kShare = 8 / kUnitSteps;   // steps of a unit, weights of a step
+      constexpr int kUnitSteps = kSteps / 2 / kHeads, kShare = 8 / kUnitSteps;   // steps of a unit, weights of a step
       if (more) {
         if (part == 0) ask_k(chunk + kChunk, next_k);
-        else ask_v(chunk + kChunk);
+        else if (!kOver) ask_v(chunk + kChunk);
       }
 #pragma unroll
-      for (int n = 0; n < kOwn; ++n) {   // 2 kOwn units in all
-        const int h = own_heads + (part * kOwn + n) / 2, j = (part * kOwn + n) % 2;
+      for (int n = 0; n < kHeads; ++n) {   // 2 kHeads units in all
+        const int h = (part * kHeads + n) / 2, j = (part * kHeads + n) % 2;
         Unit unit;
         look(unit, h, j, part_t, part_s);
         __builtin_amdgcn_sched_barrier(kNoLds);
 #pragma unroll
         for (int i = 0; i < kUnitSteps; ++i) {
-          const int step = (part * kOwn + n) * kUnitSteps + i, now = step % 2;
+          const int step = (part * kHeads + n) * kUnitSteps + i, now = step % 2;
           if (step + 1 < kSteps) fetch_q(step + 1);
           float x[8];
 #pragma unroll
@@ -516,21 +516,21 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
           o[1] = product(low, q[now][1], o[1]);
           weigh(unit, j, part_t, part_s, kShare * i, kShare * (i + 1));
         }
-        keep_weights(unit, h, j, part_t, part_s, part_of < 3);
+        keep_weights(unit, h, j, part_t, part_s, wave < 3);
       }
     }
-    if (kQuad < 3 && part_of == kQuad - 1) {
+    if (kWaves < 3 && wave == kWaves - 1) {
       p = f32x16{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         p = product(read(tile_k, at_q, step), read(tile_q + 32 * DK, at_q, step), p);
       }
 #pragma unroll
-      for (int n = 0; n < 2 * kOwn; ++n) {
+      for (int n = 0; n < 2 * kHeads; ++n) {
         Unit unit;
-        look(unit, own_heads + n / 2, n % 2, 1, 0);
+        look(unit, n / 2, n % 2, 1, 0);
         weigh(unit, n % 2, 1, 0, 0, 8);
-        keep_weights(unit, own_heads + n / 2, n % 2, 1, 0, true);
+        keep_weights(unit, n / 2, n % 2, 1, 0, true);
       }
     }
 #pragma unroll
@@ -539,7 +539,13 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     }
     meet();   // P is there, q is done with
     if (more) ask_q(chunk + kChunk);
-    if (slow) return;
+    if (slow) {
+      if (kOver) {
+        meet();
+        if (more) ask_v(chunk + kChunk);
+      }
+      return;
+    }
     // The first products' operands are asked for ahead of the decay, and each step's ahead of the last one's.
     s16x8 parts[2][2][2], kt[2][kTiles];   // P: t, 16 s, part
     f32x4 left[2][2];
@@ -555,7 +561,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          parts[tt][j][part] = __builtin_bit_cast(s16x8, weights[mine][part][2 * tt + 2 * ts + j][lane]);
+          parts[tt][j][part] = __builtin_bit_cast(s16x8, weights[weight_at(mine, part, 2 * tt + 2 * ts + j)]);
         }
       }
       __builtin_amdgcn_sched_barrier(kNoLds);
@@ -600,6 +606,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     fetch_state(0);
     store(0);
     times(1, 1);
+    if (kOver) {
+      meet();   // P is done with
+      if (more) ask_v(chunk + kChunk);
+    }
     store(1);
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
@@ -797,12 +807,11 @@ __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int sta
   }
 }
 
-// Heads of a workgroup of the prompts' kernels: those that share a key head, up to 256 columns in
-// 8 waves, which then share the chunk's q and k in LDS.
-int shared_heads(int64_t group, int64_t value_dim) {
-  if (value_dim == 128) return group % 2 == 0 && OMNIA_TRY_SHARE ? 2 : 1;
-  return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
-}
+// Heads of a workgroup of the prompts' kernels: two of 64 columns where they share a key head, in four
+// waves that share the chunk's q and k in LDS, else one. Two workgroups a CU, which are not in step,
+// do better than one of twice the waves and heads: HERE for four heads of 64; for two
+// of 128, 12 sequences up to 1,501 took 97.2 -> 101.1 us.
+int shared_heads(int64_t group, int64_t value_dim) { return value_dim == 64 && group % 2 == 0 ? 2 : 1; }
 
 template <int DK, int DV, int kHeads>
 void launch_runs(const LinearArgs& a, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
@@ -819,11 +828,9 @@ template <int DK, int DV>
 void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
   if (steps > 0) linear_step_kernel<DK, DV><<<dim3(static_cast<unsigned>(steps * a.heads)), 256, 0, stream>>>(a);
   if (runs == 0) return;
-  const int share = shared_heads(a.group, DV);
   if constexpr (DV == 64) {
-    if (share == 4) return launch_runs<DK, DV, 4>(a, runs, handed_on, chains, stream);
+    if (shared_heads(a.group, DV) == 2) return launch_runs<DK, DV, 2>(a, runs, handed_on, chains, stream);
   }
-  if (share == 2) return launch_runs<DK, DV, 2>(a, runs, handed_on, chains, stream);
   launch_runs<DK, DV, 1>(a, runs, handed_on, chains, stream);
 }
 
@@ -835,10 +842,7 @@ extern "C" int64_t omnia_linear_attention_places(int64_t heads, int64_t key_head
       (value_dim != 64 && value_dim != 128)) {
     return -EINVAL;
   }
-  // Workgroups that the LDS of 256 CUs holds, two of four waves or one of eight, times their heads.
-  const int share = omnia::shared_heads(heads / key_heads, value_dim);
-  const bool alone = share * value_dim > 128 || (key_dim == 128 && value_dim == 64 && share == 2);
-  return 256 * share * (alone ? 1 : 2);
+  return 2 * 256 * omnia::shared_heads(heads / key_heads, value_dim);   // two workgroups a CU
 }
 
 extern "C" int64_t omnia_linear_attention_workspace_bytes(int64_t heads, int64_t key_dim, int64_t value_dim, int64_t pieces) {
