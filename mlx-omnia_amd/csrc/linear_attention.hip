@@ -31,12 +31,19 @@ struct LinearArgs {
   float scale;
 };
 
+// Two to four vectors a lane: 200 requests of 64 heads of 128 x 64 took 156 us with eight, 64 of 32 of
+// 128 x 128 50.1 with 16 and 47.5 with four; of 64 x 64, 128 of 32 heads, 25.3 with four and 31.7 with one.
+// (The states go out at the end: right behind the last token's update it was 49.8 for 47.5.)
 template <int DK, int DV>
-__global__ __launch_bounds__(256) void linear_step_kernel(LinearArgs a) {
+constexpr int kStepThreads = DK * DV >= 64 * 128 ? 1024 : 256;
+
+template <int DK, int DV>
+__global__ __launch_bounds__((kStepThreads<DK, DV>)) void linear_step_kernel(LinearArgs a) {
+  constexpr int kThreads = kStepThreads<DK, DV>;
   constexpr int kLanes = DV / 4;              // lanes of a state row
-  constexpr int kRows = 256 / kLanes;         // rows of a pass
+  constexpr int kRows = kThreads / kLanes;    // rows of a pass
   constexpr int kPasses = DK / kRows;
-  constexpr int kWaves = 4;
+  constexpr int kWaves = kThreads / kWave;
   __shared__ float key[2][DK], query[2][DK];
   __shared__ f32x4 sums[2][kWaves][kLanes];
   const int entry = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
@@ -829,7 +836,7 @@ void launch_runs(const LinearArgs& a, int64_t runs, int64_t handed_on, int64_t c
 
 template <int DK, int DV>
 void launch_linear(const LinearArgs& a, int64_t steps, int64_t runs, int64_t handed_on, int64_t chains, hipStream_t stream) {
-  if (steps > 0) linear_step_kernel<DK, DV><<<dim3(static_cast<unsigned>(steps * a.heads)), 256, 0, stream>>>(a);
+  if (steps > 0) linear_step_kernel<DK, DV><<<dim3(static_cast<unsigned>(steps * a.heads)), kStepThreads<DK, DV>, 0, stream>>>(a);
   if (runs == 0) return;
   if constexpr (DV == 64) {
     if (shared_heads(a.group, DV) == 2) return launch_runs<DK, DV, 2>(a, runs, handed_on, chains, stream);
