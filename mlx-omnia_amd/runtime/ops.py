@@ -1854,6 +1854,7 @@ class LinearLists:
     chains: torch.Tensor
     handed_on: int
     pieces: int
+    stream: int   # that was current when they were laid out
 
     @classmethod
     def of(cls, steps, handed_on, last, chains, pieces: int, device) -> "LinearLists":
@@ -1861,7 +1862,14 @@ class LinearLists:
         held = torch.tensor(flat, dtype=torch.int32).to(device)
         counts = 3 * len(steps), 5 * (len(handed_on) + len(last)), 2 * len(chains)
         parts = held.split(counts)
-        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces)
+        stream = _raw_stream(held.get_device()) if held.is_cuda else 0
+        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces, stream)
+
+    def used_on(self, stream: int) -> None:
+        """Nobody else gets their memory, should the batch be dropped, before a call on `stream` has
+        read them. (A captured call's batch is kept as long as its graph.)"""
+        if stream != self.stream and not torch.cuda.is_current_stream_capturing():
+            self.runs.record_stream(torch.cuda.current_stream(self.runs.device))
 
 
 def linear_attention_places(states: torch.Tensor, key_heads: int) -> int:
@@ -1884,7 +1892,8 @@ class LinearAttentionPlan:
         _require(states.dim() == 4, "linear_attention: states must be [slots, heads, key_dim, value_dim]")
         _require(on_rocm(states, lists.steps), "linear_attention: tensors must share one ROCm device")
         slots, heads, key_dim, value_dim = states.shape
-        self.held, self.index, self.device = (states.detach(), lists), states.get_device(), states.device
+        self.held, self.lists = states.detach(), lists
+        self.index, self.device = states.get_device(), states.device
         self.of_keys, self.of_values, self.of_gates = (tokens, key_heads, key_dim), (tokens, heads, value_dim), (tokens, heads)
         self.key_width, self.value_width = key_heads * key_dim, heads * value_dim
         self.args = LinearAttentionCall(
@@ -1941,7 +1950,9 @@ class LinearAttentionPlan:
         if self.nbytes:
             workspace = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
             args.workspace = workspace.data_ptr()
-        call("omnia_linear_attention", ctypes.addressof(args), _stream_here(self.index))
+        stream = _stream_here(self.index)
+        call("omnia_linear_attention", ctypes.addressof(args), stream)
+        self.lists.used_on(stream)
         del q, k, v, g, strengths   # held until here
         return out
 

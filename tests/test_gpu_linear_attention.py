@@ -215,6 +215,27 @@ def test_on_another_stream():
     assert torch.equal(got, want) and torch.equal(states, clean)
 
 
+def test_a_batch_dropped_under_way_on_another_stream():
+    """Its lists' memory is nobody else's before the call has read them."""
+    made, _, states, slots = inputs([300, 1], 4, 2, 128, 128, device="cuda")
+    mixer, batch = layer(states, 2), LinearBatch(slots, [300, 1])
+    mixer(batch, **made)   # lays the lists out here
+    lists = next(iter(batch._lists.values()))
+    at, stream = lists.runs.untyped_storage().data_ptr(), torch.cuda.Stream()
+    wide = torch.randn(8192, 8192, device="cuda")
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(8):   # tens of milliseconds
+            torch.mm(wide, wide)
+        mixer(batch, **made)
+    del batch, lists
+    others = [torch.empty(64, dtype=torch.int32, device="cuda") for _ in range(64)]
+    busy = not stream.query()
+    held = {t.data_ptr() for t in others}
+    stream.synchronize()
+    assert busy and at not in held
+
+
 @pytest.mark.parametrize("tokens", [[1, 1, 1], [150, 1]])
 def test_captured_and_replayed(tokens):
     made, _, states, slots = inputs(tokens, 4, 2, 128, 128, device="cuda")
