@@ -19,11 +19,12 @@ struct GatedArgs {
   int64_t items;     // rows * groups
   int groups, vectors, weight_step;
   float inverse_group, eps;
-  int silu, gate_first;
+  int silu;
 };
 
-// A group of values per kLanes lanes, kVectors 16-byte vectors each.
-template <int kLanes, int kVectors>
+// A group of values per kLanes lanes, kVectors 16-byte vectors each. (Where the gate stands is known when
+// it is built: asked for in the kernel, groups of 512 with the gate first took 37.4 -> 41.5 us.)
+template <int kLanes, int kVectors, bool kGateFirst>
 __global__ __launch_bounds__(256) void gated_rms_norm_kernel(GatedArgs a) {
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
@@ -42,20 +43,21 @@ __global__ __launch_bounds__(256) void gated_rms_norm_kernel(GatedArgs a) {
     gs[i] = there ? *reinterpret_cast<const u32x4*>(gate + at * 8) : u32x4{0, 0, 0, 0};
     ws[i] = there ? *reinterpret_cast<const u32x4*>(weight + at * 8) : u32x4{0, 0, 0, 0};
   }
+  // The gate where the formula has it: behind the norm it may overflow with a value that the norm makes small.
   float y[kVectors][8];
+  const auto gated = [&](int i) {
+    float z[8];
+    unpack8(gs[i], z);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[i][j] *= (a.silu ? z[j] : 1.0f) * sigmoid(z[j]);
+  };
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    float z[8];
     unpack8(xs[i], y[i]);
-    unpack8(gs[i], z);
+    if constexpr (kGateFirst) gated(i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float gated = y[i][j] * (a.silu ? z[j] : 1.0f) * sigmoid(z[j]);
-      const float kept = a.gate_first ? gated : y[i][j];
-      sum = __builtin_fmaf(kept, kept, sum);
-      y[i][j] = gated;
-    }
+    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(y[i][j], y[i][j], sum);
   }
   sum = group_sum<kLanes>(sum);
   const float inverse = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, a.inverse_group, a.eps));
@@ -67,6 +69,7 @@ __global__ __launch_bounds__(256) void gated_rms_norm_kernel(GatedArgs a) {
     unpack8(ws[i], w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * inverse * w[j];
+    if constexpr (!kGateFirst) gated(i);
     if (at < a.vectors) *reinterpret_cast<u32x4*>(out + at * 8) = pack8(y[i]);
   }
 }
@@ -160,9 +163,10 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
 }
 
 template <int kLanes, int kVectors>
-void launch_gated(const GatedArgs& a, hipStream_t stream) {
+void launch_gated(const GatedArgs& a, bool gate_first, hipStream_t stream) {
   const int64_t blocks = (a.items + 256 / kLanes - 1) / (256 / kLanes);
-  gated_rms_norm_kernel<kLanes, kVectors><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
+  if (gate_first) gated_rms_norm_kernel<kLanes, kVectors, true><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
+  else gated_rms_norm_kernel<kLanes, kVectors, false><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
 }
 
 template <int kWaves, int kVectors>
@@ -194,18 +198,17 @@ extern "C" int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, con
   if (rc != 0) return rc;
   const int vectors = static_cast<int>(group / 8);
   const GatedArgs a{x, gate, weight, x_stride, gate_stride, out, rows * groups, static_cast<int>(groups), vectors,
-                    weight_width == width ? static_cast<int>(group) : 0, 1.0f / static_cast<float>(group), eps, silu,
-                    gate_first};
+                    weight_width == width ? static_cast<int>(group) : 0, 1.0f / static_cast<float>(group), eps, silu};
   // Two vectors a lane, and past a wave more: 8,192 rows of 4,096 in groups of 512 took 40.1 us with one
   // and 37.1 with two, of 128 40.2 and 38.1, of 64 38.9 and 38.1; with four 38.9, 38.5 and 38.8.
-  if (vectors <= 8) launch_gated<4, 2>(a, stream);
-  else if (vectors <= 16) launch_gated<8, 2>(a, stream);
-  else if (vectors <= 32) launch_gated<16, 2>(a, stream);
-  else if (vectors <= 64) launch_gated<32, 2>(a, stream);
-  else if (vectors <= 128) launch_gated<64, 2>(a, stream);
-  else if (vectors <= 256) launch_gated<64, 4>(a, stream);
-  else if (vectors <= 512) launch_gated<64, 8>(a, stream);
-  else launch_gated<64, 16>(a, stream);
+  if (vectors <= 8) launch_gated<4, 2>(a, gate_first != 0, stream);
+  else if (vectors <= 16) launch_gated<8, 2>(a, gate_first != 0, stream);
+  else if (vectors <= 32) launch_gated<16, 2>(a, gate_first != 0, stream);
+  else if (vectors <= 64) launch_gated<32, 2>(a, gate_first != 0, stream);
+  else if (vectors <= 128) launch_gated<64, 2>(a, gate_first != 0, stream);
+  else if (vectors <= 256) launch_gated<64, 4>(a, gate_first != 0, stream);
+  else if (vectors <= 512) launch_gated<64, 8>(a, gate_first != 0, stream);
+  else launch_gated<64, 16>(a, gate_first != 0, stream);
   return launched("gated_rms_norm");
 }
 

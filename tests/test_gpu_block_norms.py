@@ -68,6 +68,25 @@ def test_gated_edges(gate_first):
     assert out[5].isnan().all()
 
 
+@pytest.mark.parametrize("gate_first", [False, True])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_gated_at_the_ends_of_the_range(gate_first, act):
+    """Values and gates whose product is out of fp32's range where no step of the formula is."""
+    x, gate, weight = gated_case(6, 128, 128, device="cuda")
+    x[0] *= 1e15
+    gate[0, ::2] = -1e30          # times a sigmoid of zero
+    x[1] *= 1e-15
+    gate[1] = gate[1] * 1e-30
+    if not gate_first:            # (the norm of such products has no fp32 square)
+        x[2] *= 1e15
+        gate[2] = gate[2].abs() * 1e25
+    x[3, 5], gate[3, 5] = 2e18, -3e38
+    norm = GatedRmsNorm(RMSNormLeaf(weight), activation=act, gate_first=gate_first)
+    out = norm(x, gate)
+    assert torch.isfinite(out).all()
+    check_gated(out, x, gate, weight, 128, act, gate_first)
+
+
 HIDDENS = [8, 64, 504, 512, 520, 1024, 1032, 2048, 2560, 4096, 4104, 5120, 8192, 8200, 16384]
 
 
