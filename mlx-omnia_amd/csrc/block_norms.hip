@@ -199,8 +199,9 @@ extern "C" int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, con
   const int vectors = static_cast<int>(group / 8);
   const GatedArgs a{x, gate, weight, x_stride, gate_stride, out, rows * groups, static_cast<int>(groups), vectors,
                     weight_width == width ? static_cast<int>(group) : 0, 1.0f / static_cast<float>(group), eps, silu};
-  // Two vectors a lane, and past a wave more: 8,192 rows of 4,096 in groups of 512 took 40.1 us with one
-  // and 37.1 with two, of 128 40.2 and 38.1, of 64 38.9 and 38.1; with four 38.9, 38.5 and 38.8.
+  // Two vectors a lane, and past a wave more: 8,192 rows of 4,096 (201 MB) took 37.2, 36.7 and 48.2 us with
+  // one, two and four in groups of 64, 41, 35.8 and 38 of 128, 40.2, 36.4 (5.5 TB/s) and 37.8 of 512. (Read
+  // past the caches, groups of 64 43.1 for 37.2, the others as they are.)
   if (vectors <= 8) launch_gated<4, 2>(a, gate_first != 0, stream);
   else if (vectors <= 16) launch_gated<8, 2>(a, gate_first != 0, stream);
   else if (vectors <= 32) launch_gated<16, 2>(a, gate_first != 0, stream);

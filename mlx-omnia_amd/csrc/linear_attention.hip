@@ -4,15 +4,19 @@
 // over each sequence's new tokens, S [DK, DV] in fp32 read from and left in the pool of states.
 //
 // Steps: a workgroup takes one head of one sequence with its whole state in registers (64 KB at
-// 128 x 128, 16 vectors of 16 bytes a lane, all asked for at once), so a step of one token reads
-// and writes the state once and is bound by that. Both go past the caches, as the states of all layers
-// do not stay in them: 64 requests of 32 heads of 128 x 128, 268 MB, 57.5 -> 50.2 us over pools in turn
-// (45 -> 50 for one of 134 MB over and over, half of which the last-level cache keeps); 200 of 64 heads
-// of 128 x 64, 839 MB, 167 -> 156 us (5.4 TB/s).
+// 128 x 128, all asked for at once), so a step of one token reads and writes the state once and is
+// bound by that: 64 requests of 32 heads of 128 x 128, 268 MB over pools in turn, take 47.5 us (5.7 TB/s),
+// 200 of 64 heads of 128 x 64, 839 MB, 150 us (5.6 TB/s); a plain copy reaches 6.5. Both go past the
+// caches, as the states of all layers do not stay in them: 57.5 -> 50.2 us and 167 -> 156 when the lanes
+// held 16 and 8 vectors (45 -> 50 for one pool of 134 MB over and over, half of which the last-level
+// cache keeps).
 //
 // Prompts: a workgroup takes one head of one piece of a sequence, 64 tokens at a time on the matrix
 // unit. Where the sequences are too few to fill the card each is cut into pieces: the pieces' own
 // parts of the state first (k and v alone), then the states ahead of each, then the pieces' contexts.
+// 32,768 tokens of 32 heads of 128 x 128 (16 key heads) take 375 us: 120 the parts, 11 the states between,
+// 245 the contexts, at 0.86 and 0.88 PFLOP/s of products (103 and 215 GFLOP with the parts that 32-bit
+// states cost; a large product of bf16 alone reaches 1.2, and both clock the card down). 8,192 tokens of 64 heads of 128 x 64 take 116 us: 31, 11 and 69.
 #include "common.hpp"
 #include "host.hpp"
 
@@ -178,8 +182,8 @@ __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
 }
 
 // A workgroup barrier for what waves exchange through LDS that leaves loads straight to LDS in flight
-// (lds_barrier's fence, to which those are writes to LDS, waits for them: 32,768 tokens of 32 heads
-// HERE us for HERE).
+// (lds_barrier's fence, to which those are writes to LDS, waits for them: 32,768 tokens of 32 heads of
+// 128 x 128 378.5 us for 376, 8,192 of 64 heads of 128 x 64 119.5 for 118).
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Brings a chunk's rows of D columns to LDS, with kThreads lanes; each row's 16-byte pieces lie
@@ -819,8 +823,8 @@ __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int sta
 
 // Heads of a workgroup of the prompts' kernels: two of 64 columns where they share a key head, in four
 // waves that share the chunk's q and k in LDS, else one. Two workgroups a CU, which are not in step,
-// do better than one of twice the waves and heads: HERE for four heads of 64; for two
-// of 128, 12 sequences up to 1,501 took 97.2 -> 101.1 us.
+// do better than one of twice the waves and heads: 8,192 tokens of 64 heads of 128 x 64 119 us for
+// 123.5 with four of them together, 12 sequences up to 1,501 of 32 heads of 128 x 128 97.2 for 101.1 with two.
 int shared_heads(int64_t group, int64_t value_dim) { return value_dim == 64 && group % 2 == 0 ? 2 : 1; }
 
 template <int DK, int DV, int kHeads>

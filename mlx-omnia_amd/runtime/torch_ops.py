@@ -288,7 +288,35 @@ def _attention_sink_decode_fake(queries, keys, values, sinks, mask, scale):
 
 attention_sink_decode = _op("attention_sink_decode", _attention_sink_decode, _attention_sink_decode_fake)
 
+# the norms around a block ----------------------------------------------------------------
+
+def _gated_rms_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, group: int, eps: float,
+                    silu: bool = True, gate_first: bool = False) -> torch.Tensor:
+    return ops.gated_rms_norm(x, gate, weight, group=group, eps=eps, silu=silu, gate_first=gate_first)
+
+
+def _gated_rms_norm_fake(x, gate, weight, group, eps, silu=True, gate_first=False):
+    return x.new_empty(x.shape)
+
+
+gated_rms_norm = _op("gated_rms_norm", _gated_rms_norm, _gated_rms_norm_fake)
+
+
+def _block_norm(x: torch.Tensor, block: torch.Tensor, pre_weight: torch.Tensor, post_weight: torch.Tensor | None,
+                gate: torch.Tensor | None, pre_eps: float, post_eps: float, residual_scale: float, block_scale: float,
+                sigmoid: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.block_norm(x, block, pre_weight, post_weight, gate, pre_eps=pre_eps, post_eps=post_eps,
+                          residual_scale=residual_scale, block_scale=block_scale, sigmoid=sigmoid)
+
+
+def _block_norm_fake(x, block, pre_weight, post_weight, gate, pre_eps, post_eps, residual_scale, block_scale, sigmoid):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+block_norm = _op("block_norm", _block_norm, _block_norm_fake)
+
+
 REGISTERED = ("add_rms_norm", "qk_norm_rope", "rope_epilogue", "embed_atlas", "swiglu", "gate_softplus",
               "gated_activations", "softmax_topk", "sigmoid_topk", "pack_router_weight", "residual_rms_router",
               "residual_rms_router_sigmoid", "moe_gate_up", "moe_down_combine", "dense_gate_up_swiglu",
-              "dense_down_residual", "attention_sink_decode")
+              "dense_down_residual", "attention_sink_decode", "gated_rms_norm", "block_norm")

@@ -81,3 +81,17 @@ def test_refusals():
             join(*args)
     assert np.array_equal([gated_applies(n) for n in (8, 8192, 4, 8200, 0)], [True, True, False, False, False])
     assert np.array_equal([block_applies(n) for n in (8, 16384, 12, 16392, 0)], [True, True, False, False, False])
+
+
+def test_the_operators_for_compilers_give_shapes_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from mlx_omnia_amd.runtime import torch_ops
+
+    assert {"gated_rms_norm", "block_norm"} <= set(torch_ops.REGISTERED)
+    with FakeTensorMode():
+        x, w = torch.empty(3, 5, 64, dtype=torch.bfloat16), torch.empty(64, dtype=torch.bfloat16)
+        y = torch.ops.omnia.gated_rms_norm(x.transpose(0, 1), x.transpose(0, 1), w, 64, 1e-6)
+        assert y.shape == (5, 3, 64) and y.dtype == torch.bfloat16 and y.is_contiguous()
+        s, n = torch.ops.omnia.block_norm(x, x, w, None, None, 1e-6, 0.0, 1.0, 1.0, False)
+        assert s.shape == n.shape == x.shape and n.dtype == torch.bfloat16

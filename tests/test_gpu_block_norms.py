@@ -142,6 +142,24 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(held, want))
 
 
+def test_the_operators_for_compilers_equal_their_calls():
+    import mlx_omnia_amd.runtime.torch_ops  # noqa: F401
+
+    x, block, g, pre, behind = block_case(30, 512, "rows", True, device="cuda")
+    join = BlockNorm(RMSNormLeaf(pre, 1e-6), RMSNormLeaf(behind, 1e-5), residual_scale=0.5, block_scale=1.5, activation="sigmoid")
+    norm = GatedRmsNorm(RMSNormLeaf(behind, 1e-6), group=64)
+
+    def chain(x, block, g):
+        s, n = torch.ops.omnia.block_norm(x, block, pre, behind, g, 1e-6, 1e-5, 0.5, 1.5, True)
+        return s, n, torch.ops.omnia.gated_rms_norm(n, g, behind, 64, 1e-6)
+
+    s, n = join(x, block, g)
+    want = s, n, norm(n, g)
+    assert all(torch.equal(a, b) for a, b in zip(chain(x, block, g), want))
+    compiled = torch.compile(chain, fullgraph=True, backend="aot_eager")
+    assert all(torch.equal(a, b) for a, b in zip(compiled(x, block, g), want))
+
+
 def test_refusals_and_hand_offs():
     x, block, g, pre, behind = block_case(4, 64, "rows", True, device="cuda")
     join, norm = BlockNorm(RMSNormLeaf(pre)), GatedRmsNorm(RMSNormLeaf(pre))
