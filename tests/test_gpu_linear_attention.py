@@ -215,6 +215,38 @@ def test_on_another_stream():
     assert torch.equal(got, want) and torch.equal(states, clean)
 
 
+@pytest.mark.parametrize("tokens", [[1, 2], [0, 0], [], [600, 65]])
+def test_any_batch_on_another_stream_than_its_lists(tokens):
+    made, _, states, slots = inputs(tokens, 4, 2, 64, 64, device="cuda")
+    clean, batch = states.clone(), LinearBatch(slots, tokens)
+    want = layer(clean, 2)(batch, **made)   # lays the lists out here
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = layer(states, 2)(batch, **made)
+    stream.synchronize()
+    assert torch.equal(got, want) and torch.equal(states, clean)
+
+
+def test_two_layers_take_one_batch_at_once():
+    """Each call has a workspace of its own."""
+    tokens = [2000, 1, 300]
+    made, _, first, slots = inputs(tokens, 4, 2, 128, 64, device="cuda")
+    second = first.flip(0).contiguous()
+    pools, batch = [first, second], LinearBatch(slots, tokens)
+    clean = [p.clone() for p in pools]
+    want = [layer(p, 2)(batch, **made) for p in clean]
+    mixers, streams = [layer(p, 2) for p in pools], [torch.cuda.Stream() for _ in pools]
+    got = []
+    for mixer, stream in zip(mixers, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got.append(mixer(batch, **made))
+    torch.cuda.synchronize()
+    for a, b in zip(got + pools, want + clean):
+        assert torch.equal(a, b)
+
+
 def test_a_batch_dropped_under_way_on_another_stream():
     """Its lists' memory is nobody else's before the call has read them."""
     made, _, states, slots = inputs([300, 1], 4, 2, 128, 128, device="cuda")
