@@ -14,9 +14,10 @@
 // Prompts: a workgroup takes one head of one piece of a sequence, 64 tokens at a time on the matrix
 // unit. Where the sequences are too few to fill the card each is cut into pieces: the pieces' own
 // parts of the state first (k and v alone), then the states ahead of each, then the pieces' contexts.
-// 32,768 tokens of 32 heads of 128 x 128 take 375 us: 120 the parts, 11 the states between,
-// 245 the contexts, at 0.80 and 0.88 PFLOP/s of products (97 and 215 GFLOP with the parts that 32-bit
-// states cost; a large product of bf16 alone reaches 1.2, and both clock the card down). 8,192 tokens of 64 heads of 128 x 64 take 116 us: 31, 11 and 69.
+// 32,768 tokens of 32 heads of 128 x 128 take 375 us: 120 the parts, 11 the states between, 245 the
+// contexts, at 0.80 and 0.88 PFLOP/s of products (97 and 215 GFLOP with the parts that 32-bit states
+// cost; a large product of bf16 alone reaches 1.2, and both clock the card down). 8,192 tokens of 64
+// heads of 128 x 64 take 116 us: 31, 11 and 69.
 #include "common.hpp"
 #include "host.hpp"
 
