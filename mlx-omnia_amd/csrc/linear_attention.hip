@@ -36,6 +36,19 @@ struct LinearArgs {
   float scale;
 };
 
+// A token's decay, of a state s: s * factor, or a slow one's as s + s * factor (exp(g) - 1): exp(g)
+// itself, rounded next to 1, would be off the same way at every token of a sequence, as what is left by
+// a fast one would be as a difference from 1.
+struct Decay {
+  float factor;
+  bool slow;
+};
+__device__ __forceinline__ Decay decay_of(float g) {
+  const float rate = expm1f(g);
+  const bool slow = rate > -0.5f;
+  return {slow ? rate : expf(g), slow};
+}
+
 // Two to four vectors a lane: 200 requests of 64 heads of 128 x 64 took 156 us with eight, 64 of 32 of
 // 128 x 128 50.1 with 16 and 47.5 with four; of 64 x 64, 128 of 32 heads, 25.3 with four and 31.7 with one.
 // (The states go out at the end: right behind the last token's update it was 49.8 for 47.5.)
@@ -69,11 +82,7 @@ __global__ __launch_bounds__((kStepThreads<DK, DV>)) void linear_step_kernel(Lin
       query[turn][threadIdx.x - DK] = bf16_to_f32(a.q[token * a.q_stride + shared * DK + threadIdx.x - DK]);
     }
     const uint2 raw = *reinterpret_cast<const uint2*>(a.v + token * a.v_stride + head * DV + 4 * column);
-    // A slow decay is taken as S + (exp(g) - 1) S: exp(g) itself, rounded next to 1, would be off the
-    // same way at every token of a sequence.
-    const float rate = expm1f(a.decay[token * a.decay_stride + head]);
-    const bool slow = rate > -0.5f;
-    const float factor = slow ? rate : rate + 1.0f;
+    const Decay decay = decay_of(a.decay[token * a.decay_stride + head]);
     const float strength = a.strength != nullptr ? a.strength[token * a.strength_stride + head] : 1.0f;
     const float v[4] = {bf16_lo(raw.x) * strength, bf16_hi(raw.x) * strength, bf16_lo(raw.y) * strength,
                         bf16_hi(raw.y) * strength};
@@ -84,8 +93,8 @@ __global__ __launch_bounds__((kStepThreads<DK, DV>)) void linear_step_kernel(Lin
       const float kr = key[turn][row + i * kRows], qr = query[turn][row + i * kRows];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float next = __builtin_fmaf(s[i][j], factor, kr * v[j]);
-        s[i][j] = slow ? s[i][j] + next : next;
+        const float next = __builtin_fmaf(s[i][j], decay.factor, kr * v[j]);
+        s[i][j] = decay.slow ? s[i][j] + next : next;
         o[j] = __builtin_fmaf(qr, s[i][j], o[j]);
       }
     }

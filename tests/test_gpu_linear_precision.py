@@ -1,0 +1,44 @@
+"""What the linear attention's numbers are held to: inputs whose terms nearly cancel, so that a
+context shows through its own rounding to bf16 what its operands were rounded to, and states whose
+value is known to the last bit, or whose errors would add up over a sequence."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mlx_omnia_amd.kernels.linear_attention import HipLinearAttention, LinearAttention, LinearBatch
+
+pytestmark = pytest.mark.gpu
+
+HALF, STEP = 2.0 ** -8, 2.0 ** -24   # half a step of bf16 and of fp32, relative
+GEOMETRIES = [(2, 2, 128, 128), (4, 1, 128, 64), (3, 3, 128, 64), (4, 2, 64, 64), (2, 1, 64, 128), (3, 3, 64, 64)]
+
+
+def layer(states, key_heads, scale=0.125):
+    _, heads, key_dim, value_dim = states.shape
+    mixer = LinearAttention(states, heads=heads, key_heads=key_heads, key_dim=key_dim, value_dim=value_dim, scale=scale,
+                            dtype=torch.bfloat16)
+    assert isinstance(mixer.strategy, HipLinearAttention)
+    return mixer
+
+
+def one_hot(tokens, heads, dim, where=0):
+    rows = torch.zeros(tokens, heads, dim, dtype=torch.bfloat16, device="cuda")
+    rows[:, :, where] = 1
+    return rows
+
+
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+@pytest.mark.parametrize("decay", [-0.5, -0.75, -3.0, -15.0, -30.0, -80.0])
+def test_what_a_fast_decay_leaves(heads, key_heads, key_dim, value_dim, decay):
+    """A token of no strength: the state is what the decay leaves of it, to 32 bits of itself and not
+    of what it was."""
+    states = 1 + torch.rand(1, heads, key_dim, value_dim, generator=torch.Generator().manual_seed(1)).cuda()
+    want = states.double() * torch.exp(torch.tensor(decay, dtype=torch.float64))
+    rows, v = one_hot(1, key_heads, key_dim, 3), torch.ones(1, heads, value_dim, dtype=torch.bfloat16, device="cuda")
+    g = torch.full((1, heads), decay, device="cuda")
+    out = layer(states, key_heads)(LinearBatch([0], [1]), rows, rows, v, g, torch.zeros(1, heads, device="cuda"))
+    # An exponential to two steps of it, and a product (or the product and a sum).
+    assert ((states.double() - want).abs() <= 6 * STEP * want).all()
+    assert ((out.double() - 0.125 * want[:, :, 3]).abs() <= (HALF + 8 * STEP) * 0.125 * want[:, :, 3]).all()
