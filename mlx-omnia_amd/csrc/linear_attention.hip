@@ -124,6 +124,7 @@ __global__ __launch_bounds__((kStepThreads<DK, DV>)) void linear_step_kernel(Lin
 // ---- prompts: 64 tokens at a time ---------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
 constexpr int kChunk = 64;
@@ -260,9 +261,11 @@ __device__ __forceinline__ uint32_t held_at(int wave, int lane, int i) {
   return ((wave % (DV / 32) * (DK / 8) + i) * kWave + lane) * 4;
 }
 
-// What a chunk's decays come to: G (log2), w * scale, w exp(G_end - G) and g (log2), and G_end.
+// What a chunk's decays come to, with G their sums in log2: exp(G) as fraction 2^exponent, w * scale / fraction,
+// w exp(G_end - G), and G_end.
 struct Gates {
-  float sum[kChunk], strength[kChunk], left[kChunk], rate[kChunk], whole;
+  int exponent[kChunk];
+  float fraction[kChunk], strength[kChunk], left[kChunk], whole;
   float pad[3];
 };
 
@@ -277,8 +280,9 @@ struct Gates {
 // P v, as they are. S enters its product as two bf16 parts (16 bits; the result is rounded to 8), P as
 // two, the scaled v, whose sums the state keeps, as three, which hold all of its 24 bits. G is summed
 // in fp64, and what the state's factors are made of are its differences in fp64: a fast decay ahead of
-// a slow one would swallow the slow one's. P's are of G rounded to fp32, 2^-24 of at most 64 times the
-// fastest decay's 160: 2^-10.6 of a weight where all 64 forget everything and 2^-17 where they halve.
+// a slow one would swallow the slow one's. P's weights are products of exp(G_t) and exp(-G_s), each a
+// number of [1, 2) or (1/2, 1] times a power of two of its own, so that the fast decays' powers cancel
+// exactly: what is left is a few fp32 roundings, and no exponential for each of P's numbers.
 // The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
 // tiles, v, which is held as operands from the start, and q, done with after the first half, to the
 // same. Its decays are summed by the wave that has no part of P.
@@ -345,11 +349,13 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       const double log2 = there ? log2_of(g) : 0.0;
       const double sum = prefix_sum(log2);
       const double end = last_lane(sum);
-      gates[h].sum[lane] = static_cast<float>(sum);
-      gates[h].whole = static_cast<float>(end);   // (by every lane)
-      gates[h].strength[lane] = w * a.scale;
+      const double whole = __builtin_floor(sum);
+      const float rest = static_cast<float>(sum - whole);   // (NaN of a sum that is not finite)
+      gates[h].exponent[lane] = static_cast<int>(__builtin_fmin(whole, 0x1p24));
+      gates[h].fraction[lane] = __builtin_amdgcn_exp2f(rest);
+      gates[h].strength[lane] = w * a.scale * __builtin_amdgcn_exp2f(-rest);
       gates[h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
-      gates[h].rate[lane] = static_cast<float>(log2);
+      gates[h].whole = static_cast<float>(end);   // (by every lane)
     }
   };
   if (wave == kWaves - 1) {
@@ -433,7 +439,7 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     if (slow) {
       // Zero times such a value is a NaN where a token does not see it: these columns a token at a time.
       for (int t = 0; t < tokens; ++t) {
-        const float keep = __builtin_amdgcn_exp2f(gates.rate[t]);
+        const Decay decay = decay_of(a.decay[(token0 + t) * a.decay_stride + head]);
         const int column_v = 32 * wave + column;
         const float w = a.strength != nullptr ? a.strength[(token0 + t) * a.strength_stride + head] : 1.0f;
         const float v = w * bf16_to_f32(tile_v[t * kWidth + ((column_v / 8) ^ turn_of<kWidth>(t)) * 8 + column_v % 8]);
@@ -448,7 +454,8 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
             unpack8(*reinterpret_cast<const u32x4*>(tile_q + at), qr);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              s[i][8 * j + e] = __builtin_fmaf(kr[e], v, s[i][8 * j + e] * keep);
+              const float next = __builtin_fmaf(s[i][8 * j + e], decay.factor, kr[e] * v);
+              s[i][8 * j + e] = decay.slow ? s[i][8 * j + e] + next : next;
               sum = __builtin_fmaf(qr[e], s[i][8 * j + e], sum);
             }
           }
@@ -469,15 +476,18 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 
     // 16 rows s of a part of P^T, weighed: a few at a time, to stand between the products.
     struct Unit {
-      float sum, x[8];
-      f32x4 sums[2], strengths[2];
+      int exponent;
+      float fraction, x[8];
+      i32x4 exponents[2];
+      f32x4 strengths[2];
     };
     const auto look = [&](Unit& u, int h, int j, int tt, int ts) {
       const int t = 32 * tt + column, at = 32 * ts + 16 * j + 4 * half;
-      u.sum = all[h].sum[t];
+      u.exponent = all[h].exponent[t];
+      u.fraction = all[h].fraction[t];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        u.sums[i] = *reinterpret_cast<const f32x4*>(&all[h].sum[at + 8 * i]);
+        u.exponents[i] = *reinterpret_cast<const i32x4*>(&all[h].exponent[at + 8 * i]);
         u.strengths[i] = *reinterpret_cast<const f32x4*>(&all[h].strength[at + 8 * i]);
       }
     };
@@ -487,9 +497,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
 #pragma unroll
       for (int e = from; e < end; ++e) {
         const int i = e / 4, n = e % 4;
-        float weight = p[8 * j + e] * (__builtin_amdgcn_exp2f(u.sum - u.sums[i][n]) * u.strengths[i][n]);
+        const float decayed = __builtin_amdgcn_ldexpf(u.strengths[i][n], u.exponent - u.exponents[i][n]) * u.fraction;
+        float weight = p[8 * j + e] * decayed;
         // Chosen, not multiplied by zero: a later token's key may not be finite. (Pinned, or the
-        // compiler branches around each exponential.)
+        // compiler branches around each of them.)
         asm("" : "+v"(weight));
         u.x[e] = 8 * i + n <= bound ? weight : 0.0f;
       }
@@ -558,7 +569,8 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     }
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      o[tt] *= __builtin_amdgcn_exp2f(gates.sum[32 * tt + column]) * a.scale;
+      const int t = 32 * tt + column;
+      o[tt] *= __builtin_amdgcn_ldexpf(gates.fraction[t], gates.exponent[t]) * a.scale;
     }
     meet();   // P is there, q is done with
     if (more) ask_q(chunk + kChunk);

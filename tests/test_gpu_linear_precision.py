@@ -42,3 +42,25 @@ def test_what_a_fast_decay_leaves(heads, key_heads, key_dim, value_dim, decay):
     # An exponential to two steps of it, and a product (or the product and a sum).
     assert ((states.double() - want).abs() <= 6 * STEP * want).all()
     assert ((out.double() - 0.125 * want[:, :, 3]).abs() <= (HALF + 8 * STEP) * 0.125 * want[:, :, 3]).all()
+
+
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+@pytest.mark.parametrize("fast,plus,minus", [(50, 51, 61), (20, 21, 31), (20, 25, 40), (40, 41, 50)])
+def test_slow_decays_behind_fast_ones(heads, key_heads, key_dim, value_dim, fast, plus, minus):
+    """Tokens at a log decay of -109, then slow ones: a later context is the difference of two
+    weights, 1 - exp(-3e-4 n), which sums of decays in 32 bits (up to 2^-12 off here) would swallow."""
+    n, g = 64, torch.full((64, heads), -3e-4, device="cuda")
+    g[:fast] = -109.0
+    v = torch.zeros(n, heads, value_dim, dtype=torch.bfloat16, device="cuda")
+    v[plus], v[minus] = 1, -1
+    states = torch.ones(1, heads, key_dim, value_dim, device="cuda")
+    rows = one_hot(n, key_heads, key_dim)
+    out = layer(states, key_heads)(LinearBatch([0], [n]), rows, rows, v, g).double()
+    sums = torch.cumsum(g.double(), dim=0)
+    first, second = torch.exp(sums[minus:] - sums[plus]), torch.exp(sums[minus:] - sums[minus])
+    want = (0.125 * (first - second))[..., None]
+    # One rounding of the result, and 2^-15 for each weight.
+    allowed = HALF * want.abs() + 0.125 * 2 * 2.0 ** -15
+    assert (want.abs() > 30 * allowed).any() and ((out[minus:] - want).abs() <= allowed).all()
+    left = torch.exp(sums[-1] - sums[plus]) - torch.exp(sums[-1] - sums[minus])
+    assert ((states[0, :, 0].double() - left[:, None]).abs() <= 16 * STEP).all()
