@@ -277,8 +277,11 @@ struct Gates {
 // The accumulators' order of rows is that of the products' operands over 16 rows once the state's
 // rows are numbered 16 j + 8 half + 0..7 (lane (half, c) holds its column c of those), for which k is
 // transposed in that order: S is an operand of q S, and the columns of P that a wave has made one of
-// P v, as they are. S enters its product as two bf16 parts (16 bits; the result is rounded to 8), P as
-// two, the scaled v, whose sums the state keeps, as three, which hold all of its 24 bits. G is summed
+// P v, as they are. S, P and the scaled v, fp32 all of them, enter their products as three bf16 parts,
+// which hold all 24 bits, as the steps multiply them. (S and P in two parts, of 16 bits, 12 sequences up to 1,501
+// of 32 heads of 128 x 128 took 94 us for 105, 32,768 tokens 368 for 406, 8,192 of 64 heads of 128 x 64 115.5
+// for 126; the contexts then differed from those of fp32 products by 1.3e-4 of their size, and by 2 to 4e-5
+// now, as sums in another order do.) G is summed
 // in fp64, and what the state's factors are made of are its differences in fp64: a fast decay ahead of
 // a slow one would swallow the slow one's. P's weights are products of exp(G_t) and exp(-G_s), each a
 // number of [1, 2) or (1/2, 1] times a power of two of its own, so that the fast decays' powers cancel
@@ -291,14 +294,20 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
   constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;
   constexpr int kTiles = DK / 32, kSteps = DK / 16;
   __shared__ __attribute__((aligned(16))) uint16_t tile_q[kChunk * DK], tile_k0[kChunk * DK], tile_k1[kChunk * DK];
-  // P^T: parts, (t, 16 s), lanes. Two heads' lies where v did, which is read first, or the LDS would hold
-  // one workgroup a CU for two; v of the next chunk is then asked for later.
-  constexpr bool kOver = DK == 128 && kHeads == 2;
-  constexpr int kWeights = kHeads * 2 * 6 * kWave;
-  __shared__ u32x4 held[kOver ? kWeights : kChunk * kWidth / 8], apart[kOver ? 1 : kWeights];
+  // P^T: heads, parts, (t, 16 s), lanes: 1 KB each. Of 128 x 128, and of two heads, it lies where v did,
+  // which is read first, or the LDS would hold one workgroup a CU for two; v of the next chunk is then
+  // asked for later. Two heads' of 128 x 64 take the place of the next chunk's k with it: one part
+  // of each lies in either, four pieces of the third behind them and the other two apart.
+  constexpr int kWeights = kHeads * 3 * 6, kHeld = kChunk * kWidth / 8 / kWave;   // KB
+  constexpr bool kOver = kHeads == 2 || (DK == 128 && DV == 128), kOverNext = DK == 128 && kHeads == 2;
+  __shared__ u32x4 held[(kOver && !kOverNext ? kWeights : kHeld) * kWave], apart[(!kOver ? kWeights : kOverNext ? 4 : 1) * kWave];
   uint16_t* const tile_v = reinterpret_cast<uint16_t*>(held);
-  u32x4* const weights = (kOver ? held : apart) + (threadIdx.x % kWave);
-  const auto weight_at = [](int h, int part, int frag) { return ((h * 2 + part) * 6 + frag) * kWave; };
+  const auto weight_at = [&](uint16_t* next_k, int h, int part, int frag) {
+    u32x4 *const own = (kOver ? held : apart) + threadIdx.x % kWave, *const next = reinterpret_cast<u32x4*>(next_k) + threadIdx.x % kWave;
+    if (!kOverNext) return own + ((h * 3 + part) * 6 + frag) * kWave;
+    if (part < 2) return (part == 0 ? own : next) + (h * 6 + frag) * kWave;
+    return frag < 4 ? (h == 0 ? own : next) + (12 + frag) * kWave : apart + threadIdx.x % kWave + (h * 2 + frag - 4) * kWave;
+  };
   __shared__ __attribute__((aligned(16))) Gates gates0[kHeads], gates1[kHeads];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int half = lane / 32, column = lane % 32;
@@ -507,10 +516,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     };
     const auto keep_weights = [&](Unit& u, int h, int j, int tt, int ts, bool kept) {
       const int frag = 2 * tt + 2 * ts + j;
-      const u32x4 high = __builtin_bit_cast(u32x4, cut(u.x)), low = pack8(u.x);
-      if (kept) {
-        weights[weight_at(h, 0, frag)] = high;
-        weights[weight_at(h, 1, frag)] = low;
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        const u32x4 cut_off = __builtin_bit_cast(u32x4, cut(u.x));
+        if (kept) *weight_at(next_k, h, part, frag) = cut_off;
       }
     };
     // q S, in two halves with P's weights between the products and the next chunk's rows ahead of them.
@@ -527,8 +536,8 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     for (int part = 0; part < 2; ++part) {
       constexpr int kUnitSteps = kSteps / 2 / kHeads, kShare = 8 / kUnitSteps;   // steps of a unit, weights of a step
       if (more) {
-        if (part == 0) ask_k(chunk + kChunk, next_k);
-        else if (!kOver) ask_v(chunk + kChunk);
+        if (part == 0 && !kOverNext) ask_k(chunk + kChunk, next_k);
+        else if (part == 1 && !kOver) ask_v(chunk + kChunk);
       }
 #pragma unroll
       for (int n = 0; n < kHeads; ++n) {   // 2 kHeads units in all
@@ -543,11 +552,12 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = s[step / 2][8 * (step % 2) + e];
-          const s16x8 high = cut(x), low = __builtin_bit_cast(s16x8, pack8(x));
-          o[0] = product(high, q[now][0], o[0]);
-          o[1] = product(high, q[now][1], o[1]);
-          o[0] = product(low, q[now][0], o[0]);
-          o[1] = product(low, q[now][1], o[1]);
+#pragma unroll
+          for (int third = 0; third < 3; ++third) {
+            const s16x8 cut_off = cut(x);
+            o[0] = product(cut_off, q[now][0], o[0]);
+            o[1] = product(cut_off, q[now][1], o[1]);
+          }
           weigh(unit, j, part_t, part_s, kShare * i, kShare * (i + 1));
         }
         keep_weights(unit, h, j, part_t, part_s, wave < 3);
@@ -572,18 +582,20 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       const int t = 32 * tt + column;
       o[tt] *= __builtin_amdgcn_ldexpf(gates.fraction[t], gates.exponent[t]) * a.scale;
     }
+    const auto ask_rest = [&] {
+      meet();   // P is done with
+      if (kOverNext && more) ask_k(chunk + kChunk, next_k);
+      if (more) ask_v(chunk + kChunk);
+    };
     meet();   // P is there, q is done with
     if (more) ask_q(chunk + kChunk);
     if (slow) {
-      if (kOver) {
-        meet();
-        if (more) ask_v(chunk + kChunk);
-      }
+      if (kOver) ask_rest();
       return;
     }
     __builtin_amdgcn_s_setprio(0);
     // The first products' operands are asked for ahead of the decay, and each step's ahead of the last one's.
-    s16x8 parts[2][2][2], kt[2][kTiles];   // P: t, 16 s, part
+    s16x8 parts[2][3], kt[2][kTiles];   // of P's 32 t by 16 s
     f32x4 left[2][2];
     const auto fetch_state = [&](int step) {
 #pragma unroll
@@ -592,19 +604,18 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       for (int i = 0; i < kTiles; ++i) kt[step % 2][i] = transposed(tile_k + step * 16 * DK, at_k ^ (32 * i), DK);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
-    const auto fetch_part = [&](int tt, int ts) {   // of P
+    // P's parts of 32 t by 16 s in turn: (t, s / 32, s / 16 % 2).
+    constexpr int kTurn[6][3] = {{0, 0, 0}, {1, 0, 0}, {0, 0, 1}, {1, 0, 1}, {1, 1, 0}, {1, 1, 1}};
+    const auto fetch_part = [&](int turn) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          parts[tt][j][part] = __builtin_bit_cast(s16x8, weights[weight_at(mine, part, 2 * tt + 2 * ts + j)]);
-        }
+      for (int part = 0; part < 3; ++part) {
+        const int frag = 2 * kTurn[turn][0] + 2 * kTurn[turn][1] + kTurn[turn][2];
+        parts[turn % 2][part] = __builtin_bit_cast(s16x8, *weight_at(next_k, mine, part, frag));
       }
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     const float whole = gates.whole;
-    fetch_part(0, 0);
-    fetch_part(1, 0);
+    fetch_part(0);
     const float keep = __builtin_amdgcn_exp2f(whole);
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) s[i] *= keep;
@@ -612,12 +623,10 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     const int64_t bytes = static_cast<int64_t>(a.heads) * DV * 2;   // of a row
     const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + (token0 * a.heads + head) * DV, 0,
                                                       static_cast<int>((tokens - 1) * bytes + DV * 2), 0x00027000);
-    const auto times = [&](int tt, int ts) {
+    const auto times = [&](int turn) {
+      const int tt = kTurn[turn][0], step = 2 * kTurn[turn][1] + kTurn[turn][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int part = 0; part < 2; ++part) o[tt] = product(values[2 * ts + j], parts[tt][j][part], o[tt]);
-      }
+      for (int part = 0; part < 3; ++part) o[tt] = product(values[step], parts[turn % 2][part], o[tt]);
     };
     const auto store = [&](int tt) {
       const int at = (32 * tt + column) * static_cast<int>(bytes) + (32 * wave % DV + 8 * half) * 2;
@@ -636,16 +645,16 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
         __builtin_amdgcn_raw_buffer_store_b128(packed, to, at + 32 * i, 0, 0);
       }
     };
-    times(0, 0);
-    times(1, 0);
-    fetch_part(1, 1);
-    fetch_state(0);
-    store(0);
-    times(1, 1);
-    if (kOver) {
-      meet();   // P is done with
-      if (more) ask_v(chunk + kChunk);
+#pragma unroll
+    for (int turn = 0; turn < 6; ++turn) {
+      if (turn + 1 < 6) fetch_part(turn + 1);
+      if (turn == 5) {
+        fetch_state(0);
+        store(0);
+      }
+      times(turn);
     }
+    if (kOver) ask_rest();
     store(1);
 #pragma unroll
     for (int step = 0; step < 4; ++step) {

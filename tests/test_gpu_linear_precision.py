@@ -64,3 +64,48 @@ def test_slow_decays_behind_fast_ones(heads, key_heads, key_dim, value_dim, fast
     assert (want.abs() > 30 * allowed).any() and ((out[minus:] - want).abs() <= allowed).all()
     left = torch.exp(sums[-1] - sums[plus]) - torch.exp(sums[-1] - sums[minus])
     assert ((states[0, :, 0].double() - left[:, None]).abs() <= 16 * STEP).all()
+
+
+def nearly_cancelling(n, seed=3):
+    """Numbers of 24 bits in [1, 2), and others that are off by about 2^-12 of them, no two by the same."""
+    gen = torch.Generator().manual_seed(seed)
+    x = (1 + torch.rand(n, generator=gen)).float()
+    return x.cuda(), (x * (1 + 2.0 ** -12 * (1 + torch.rand(n, generator=gen)))).float().cuda()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 64, 130])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+def test_states_are_read_in_32_bits(heads, key_heads, key_dim, value_dim, tokens):
+    """Contexts that are the difference of two rows of the state, which keys of zero leave as it is."""
+    states = torch.zeros(1, heads, key_dim, value_dim, device="cuda")
+    x, y = (t.view(heads, value_dim) for t in nearly_cancelling(heads * value_dim))
+    i, j = 5, key_dim - 7
+    states[0, :, i], states[0, :, j] = x, -y
+    q = one_hot(tokens, key_heads, key_dim, i) + one_hot(tokens, key_heads, key_dim, j)
+    v = torch.ones(tokens, heads, value_dim, dtype=torch.bfloat16, device="cuda")
+    before = states.clone()
+    out = layer(states, key_heads)(LinearBatch([0], [tokens]), q, torch.zeros_like(q), v, torch.zeros(tokens, heads, device="cuda"))
+    want = 0.125 * (x.double() - y.double())
+    # One rounding of the result; a few of the sum, of terms below 2 each.
+    assert ((out.double() - want).abs() <= HALF * want.abs() + 0.125 * 8 * STEP * 2).all()
+    assert torch.equal(states, before)
+
+
+@pytest.mark.parametrize("first,second,last", [(0, 1, 64), (3, 40, 64), (33, 50, 60), (70, 71, 130), (0, 1, 5)])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+def test_weights_are_multiplied_in_32_bits(heads, key_heads, key_dim, value_dim, first, second, last):
+    """Contexts that are the difference of two tokens' values, of nearly the same strength."""
+    states = torch.zeros(1, heads, key_dim, value_dim, device="cuda")
+    x, y = nearly_cancelling(heads)
+    w = torch.zeros(last, heads, device="cuda")
+    w[first], w[second] = x, y
+    v = torch.zeros(last, heads, value_dim, dtype=torch.bfloat16, device="cuda")
+    v[first], v[second] = 1, -1
+    rows = one_hot(last, key_heads, key_dim, 9)
+    out = layer(states, key_heads)(LinearBatch([0], [last]), rows, rows, v, torch.zeros(last, heads, device="cuda"), w)
+    want = 0.125 * (x.double() - y.double())[:, None].expand(heads, value_dim)
+    # One rounding of the result; a few of each weight's factors and of the sum, of terms below 2 each.
+    allowed = HALF * want.abs() + 0.125 * 12 * STEP * 2
+    assert ((out[second:].double() - want).abs() <= allowed).all()
+    assert ((out[first:second].double() - 0.125 * x.double()[:, None]).abs() <= (HALF + 12 * STEP) * 0.125 * 2).all()
+    assert not out[:first].any()
