@@ -36,9 +36,9 @@ struct LinearArgs {
   float scale;
 };
 
-// A token's decay, of a state s: s * factor, or a slow one's as s + s * factor (exp(g) - 1): exp(g)
-// itself, rounded next to 1, would be off the same way at every token of a sequence, as what is left by
-// a fast one would be as a difference from 1.
+// A decay of a state s: s * factor, or a slow one's as s + s * factor (exp(g) - 1): exp(g) itself, rounded
+// next to 1, would be off the same way at every token or chunk of a sequence, and what a fast one leaves
+// would be as a difference from 1.
 struct Decay {
   float factor;
   bool slow;
@@ -261,12 +261,20 @@ __device__ __forceinline__ uint32_t held_at(int wave, int lane, int i) {
   return ((wave % (DV / 32) * (DK / 8) + i) * kWave + lane) * 4;
 }
 
+// The same of a decay given as log2.
+constexpr float kLn2 = 0.693147180559945f;
+__device__ __forceinline__ Decay decay_of_log2(float log2) {
+  const float rate = expm1f(log2 * kLn2);
+  const bool slow = rate > -0.5f;
+  return {slow ? rate : __builtin_amdgcn_exp2f(log2), slow};
+}
+
 // What a chunk's decays come to, with G their sums in log2: exp(G) as fraction 2^exponent, w * scale / fraction,
-// w exp(G_end - G), and G_end.
+// w exp(G_end - G), and G_end as a Decay.
 struct Gates {
   int exponent[kChunk];
-  float fraction[kChunk], strength[kChunk], left[kChunk], whole;
-  float pad[3];
+  float fraction[kChunk], strength[kChunk], left[kChunk], factor;
+  int slow, pad[2];
 };
 
 // A piece of a sequence, for kHeads heads of a key head: a wave holds 32 columns of a head's state in
@@ -364,7 +372,9 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       gates[h].fraction[lane] = __builtin_amdgcn_exp2f(rest);
       gates[h].strength[lane] = w * a.scale * __builtin_amdgcn_exp2f(-rest);
       gates[h].left[lane] = there ? __builtin_amdgcn_exp2f(static_cast<float>(end - sum)) * w : 0.0f;
-      gates[h].whole = static_cast<float>(end);   // (by every lane)
+      const Decay decay = decay_of_log2(static_cast<float>(end));
+      gates[h].factor = decay.factor;   // (by every lane)
+      gates[h].slow = decay.slow;
     }
   };
   if (wave == kWaves - 1) {
@@ -614,11 +624,9 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
       }
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
-    const float whole = gates.whole;
+    const float factor = gates.factor;
+    const bool slowly = __builtin_amdgcn_readfirstlane(gates.slow) != 0;
     fetch_part(0);
-    const float keep = __builtin_amdgcn_exp2f(whole);
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) s[i] *= keep;
     // Rows past the last are out of the buffer, and not written.
     const int64_t bytes = static_cast<int64_t>(a.heads) * DV * 2;   // of a row
     const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + (token0 * a.heads + head) * DV, 0,
@@ -656,6 +664,16 @@ __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(Linear
     }
     if (kOver) ask_rest();
     store(1);
+    if (slowly) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[i][e] = __builtin_fmaf(s[i][e], factor, s[i][e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) s[i] *= factor;
+    }
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       const int now = step % 2;
@@ -844,9 +862,12 @@ __global__ __launch_bounds__(256) void linear_carry_kernel(LinearArgs a, int sta
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (p + i >= count) break;
-      const float factor = __builtin_amdgcn_exp2f(keep[i]);
+      const Decay decay = decay_of_log2(keep[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(sum[j], factor, own[i][j]);
+      for (int j = 0; j < 4; ++j) {
+        const float next = __builtin_fmaf(sum[j], decay.factor, own[i][j]);
+        sum[j] = decay.slow ? sum[j] + next : next;
+      }
       *reinterpret_cast<f32x4*>(x + (p + i - 1) * between) = sum;
     }
   }

@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from mlx_omnia_amd.kernels import linear_attention
 from mlx_omnia_amd.kernels.linear_attention import HipLinearAttention, LinearAttention, LinearBatch
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +110,27 @@ def test_weights_are_multiplied_in_32_bits(heads, key_heads, key_dim, value_dim,
     assert ((out[second:].double() - want).abs() <= allowed).all()
     assert ((out[first:second].double() - 0.125 * x.double()[:, None]).abs() <= (HALF + 12 * STEP) * 0.125 * 2).all()
     assert not out[:first].any()
+
+
+@pytest.mark.parametrize("chunks", [1 << 20, 2, 16])   # of a piece: uncut, many pieces, some
+@pytest.mark.parametrize("decay", [-1e-4, -1.3e-5, -1e-3])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", [(2, 2, 128, 128), (2, 1, 128, 64), (1, 1, 64, 64)])
+def test_slow_decays_over_a_long_sequence(monkeypatch, chunks, decay, heads, key_heads, key_dim, value_dim):
+    """32,768 tokens of no strength and a fixed decay. What the rounding of each chunk's factor next to 1 would
+    take away is the same for every chunk and number: the mean of all numbers' errors shows it, to
+    which their own roundings, each its own, add little."""
+    monkeypatch.setattr(linear_attention, "piece_chunks", lambda own, places: chunks)
+    n = 32768
+    gen = torch.Generator().manual_seed(2)
+    states = 1 + torch.rand(1, heads, key_dim, value_dim, generator=gen).cuda()
+    g = torch.full((n, heads), decay, device="cuda")
+    want = states.double() * torch.exp(n * g[0, 0].double())
+    rows, v = one_hot(n, key_heads, key_dim), torch.ones(n, heads, value_dim, dtype=torch.bfloat16, device="cuda")
+    layer(states, key_heads)(LinearBatch([0], [n]), rows, rows, v, g, torch.zeros(n, heads, device="cuda"))
+    off = (states.double() - want) / want
+    # Each factor is off by two steps of what it takes away, or of itself (and its exponent's rounding), where it takes
+    # more than half; one, of the state as it was, may be rounded next to 1. And 512 roundings of each number, of at most
+    # a step of 2^-24, are off by 6 of their mean's deviations at most.
+    mean = (5 * abs(decay) * n + 4) * STEP + 6 * (512 / states.numel()) ** 0.5 * STEP
+    assert abs(off.mean().item()) <= mean
+    assert off.abs().max().item() <= mean + 7 * 512 ** 0.5 * STEP
