@@ -4,9 +4,11 @@ value is known to the last bit, or whose errors would add up over a sequence."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
+from linear_cases import inputs, oracle, wide
 from mlx_omnia_amd.kernels import linear_attention
 from mlx_omnia_amd.kernels.linear_attention import HipLinearAttention, LinearAttention, LinearBatch
 
@@ -134,3 +136,43 @@ def test_slow_decays_over_a_long_sequence(monkeypatch, chunks, decay, heads, key
     mean = (5 * abs(decay) * n + 4) * STEP + 6 * (512 / states.numel()) ** 0.5 * STEP
     assert abs(off.mean().item()) <= mean
     assert off.abs().max().item() <= mean + 7 * 512 ** 0.5 * STEP
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 50, 64, 100])
+@pytest.mark.parametrize("size", [1 << 20, 1])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES)
+def test_states_keep_all_bits_of_what_is_added(monkeypatch, heads, key_heads, key_dim, value_dim, size, tokens):
+    """A row of the state for each token (no more of them than rows): the token's value times its strength,
+    in 32 bits, and nothing else."""
+    monkeypatch.setattr(linear_attention, "piece_chunks", lambda own, places: size)
+    n, gen = min(tokens, key_dim), torch.Generator().manual_seed(4)
+    states = torch.zeros(1, heads, key_dim, value_dim, device="cuda")
+    order = torch.randperm(key_dim, generator=gen)[:n]
+    k = torch.zeros(n, key_heads, key_dim)
+    k[torch.arange(n), :, order] = 1
+    v = torch.randn(n, heads, value_dim, generator=gen).bfloat16().cuda()
+    w = torch.rand(n, heads, generator=gen).cuda()
+    k = k.bfloat16().cuda()
+    layer(states, key_heads)(LinearBatch([0], [n]), k, k, v, torch.zeros(n, heads, device="cuda"), w)
+    want = torch.zeros_like(states)
+    want[0, :, order.cuda()] = (v.float() * w[..., None]).transpose(0, 1)
+    assert torch.equal(states, want)
+
+
+@pytest.mark.parametrize("size", [1 << 20, 4])
+@pytest.mark.parametrize("tokens", [200, 1500])
+@pytest.mark.parametrize("heads,key_heads,key_dim,value_dim", GEOMETRIES[:4])
+def test_states_of_prompts_as_a_whole(monkeypatch, heads, key_heads, key_dim, value_dim, tokens, size):
+    """The states' error as a whole (2-norm). A chunk rounds a state at most 12 times in its products
+    and three times in its decay and its pieces, by at most a step of 2^-24 of what it comes to, one
+    way or the other: the square root of their number together. (Values in two parts, of 16 bits, would
+    be off by 2^-18.)"""
+    monkeypatch.setattr(linear_attention, "piece_chunks", lambda own, places: size)
+    made, _, states, slots = inputs([tokens], heads, key_heads, key_dim, value_dim, device="cuda", strengths=True)
+    before = wide(states)
+    layer(states, key_heads)(LinearBatch(slots, [tokens]), **made)
+    _, left, _, _ = oracle(*(wide(made[name]) for name in ("queries", "keys", "values", "log_decay", "strengths")), before,
+                           slots, [tokens], 0.125)
+    off = np.linalg.norm(wide(states)[slots[0]] - left[slots[0]]) / np.linalg.norm(left[slots[0]])
+    print(f"states off by {off:.3g}", flush=True)
+    assert off <= (15 * -(-tokens // 64)) ** 0.5 * STEP
