@@ -19,3 +19,8 @@ def hip_device(*tensors: torch.Tensor) -> bool:
         return False
     library()
     return True
+
+
+def in_place(weight: torch.Tensor) -> bool:
+    """Whether a kernel reads `weight` where it lies: a copy would not follow what is written to it."""
+    return weight.is_contiguous() and weight.data_ptr() % 16 == 0

@@ -20,7 +20,7 @@ from typing import Protocol, runtime_checkable
 import torch
 
 from ...runtime import ops
-from .._device import hip_device
+from .._device import hip_device, in_place
 from ..attention.prefill import unfollowed
 from ..resolve import record_fallback, resolve
 
@@ -85,6 +85,8 @@ class HipBlockNorm(BlockNormStrategy):
     def build(cls, pre, post, *, residual_scale, block_scale, activation) -> "HipBlockNorm | None":
         weights = [leaf.weight for leaf in (pre, post) if leaf is not None]
         if any(w.dtype != torch.bfloat16 or not applies(w.numel()) for w in weights) or not hip_device(*weights):
+            return None
+        if not all(in_place(w) for w in weights):
             return None
         return cls(DefaultBlockNorm.build(pre, post, residual_scale=residual_scale, block_scale=block_scale,
                                           activation=activation))

@@ -19,7 +19,7 @@ from typing import Protocol, runtime_checkable
 import torch
 
 from ...runtime import ops
-from .._device import hip_device
+from .._device import hip_device, in_place
 from ..attention.prefill import unfollowed
 from ..resolve import record_fallback, resolve
 
@@ -68,9 +68,12 @@ class HipGatedRmsNorm(GatedRmsNormStrategy):
 
     @classmethod
     def build(cls, leaf, *, group, activation, gate_first) -> "HipGatedRmsNorm | None":
-        if leaf.weight.dtype != torch.bfloat16 or not applies(group) or not hip_device(leaf.weight):
+        weight = leaf.weight
+        if weight.dtype != torch.bfloat16 or not applies(group) or not hip_device(weight):
             return None
-        return cls(DefaultGatedRmsNorm.build(leaf, group=group, activation=activation, gate_first=gate_first), leaf.weight)
+        if not in_place(weight):
+            return None
+        return cls(DefaultGatedRmsNorm.build(leaf, group=group, activation=activation, gate_first=gate_first), weight)
 
     def __call__(self, x, gate):
         core = self.core
