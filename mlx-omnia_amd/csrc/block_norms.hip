@@ -1,13 +1,27 @@
 // The norms around a block, with its gate and scales: the gated norm of a mixer's output in
 // groups, and the join of two blocks. Everything in fp32 from the bf16 inputs to one rounding
-// for each output; the sums of squares are fp32 (8 to 16384 terms, added in a tree over the
-// lanes: an error of a few 2^-24). Both read each tensor once and write each result once, and
+// for each output; the sums of squares are fp32 (8 to 16384 terms: of each of a lane's eight places
+// in turn, 16 at most, then in a tree over the places and the lanes and, of a row, over up to eight waves
+// in turn: under 30 roundings of 2^-24). Both read each tensor once and write each result once, and
 // are bound by that from a few hundred rows on, by the launch below.
 #include "common.hpp"
 #include "host.hpp"
 
 namespace omnia {
 namespace {
+
+// A lane's sum of squares: its vectors' first values, second and so on each by themselves, then in a tree.
+// (One by one, 128 of them, small ones behind a large one were lost.)
+template <int kVectors>
+__device__ __forceinline__ float squares(const float (&y)[kVectors][8]) {
+  float sums[8] = {};
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[j] = __builtin_fmaf(y[i][j], y[i][j], sums[j]);
+  }
+  return ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
+}
 
 // 1 / (1 + exp(-z)): exact ends (an exponential that overflows gives 0).
 __device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
@@ -51,15 +65,12 @@ __global__ __launch_bounds__(256) void gated_rms_norm_kernel(GatedArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[i][j] *= (a.silu ? z[j] : 1.0f) * sigmoid(z[j]);
   };
-  float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     unpack8(xs[i], y[i]);
     if constexpr (kGateFirst) gated(i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(y[i][j], y[i][j], sum);
   }
-  sum = group_sum<kLanes>(sum);
+  const float sum = group_sum<kLanes>(squares(y));
   const float inverse = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, a.inverse_group, a.eps));
   uint16_t* out = a.out + item * (a.vectors * 8);
 #pragma unroll
@@ -120,13 +131,7 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) unpack8(bs[i], s[i]);
   if (a.post != nullptr) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(s[i][j], s[i][j], sum);
-    }
-    const float inverse = 1.0f / __builtin_sqrtf(block_sum<kWaves>(sum, parts[0]) / a.hidden + a.post_eps);
+    const float inverse = 1.0f / __builtin_sqrtf(block_sum<kWaves>(squares(s), parts[0]) / a.hidden + a.post_eps);
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       float w[8];
@@ -135,7 +140,6 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
       for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * inverse * w[j];
     }
   }
-  float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     float x[8], g[8];
@@ -145,10 +149,9 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
     for (int j = 0; j < 8; ++j) {
       if (a.gate != nullptr) s[i][j] *= a.sigmoid ? sigmoid(g[j]) : g[j];
       s[i][j] = __builtin_fmaf(a.block_scale, s[i][j], a.residual_scale * x[j]);
-      sum = __builtin_fmaf(s[i][j], s[i][j], sum);
     }
   }
-  const float inverse = 1.0f / __builtin_sqrtf(block_sum<kWaves>(sum, parts[1]) / a.hidden + a.pre_eps);
+  const float inverse = 1.0f / __builtin_sqrtf(block_sum<kWaves>(squares(s), parts[1]) / a.hidden + a.pre_eps);
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     const int at = threadIdx.x + i * kThreads;
