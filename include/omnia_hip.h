@@ -838,7 +838,8 @@ int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hip
  * omnia_linear_attention_workspace_bytes, 16-byte aligned (null where that is 0).
  * Its input is what omnia_gate_softplus gives (models/qwen3_5/layers/deltanet.py:222-224);
  * the single-token recurrence stands where core/kernels/ssm does.
- * key_dim, value_dim 64 or 128; heads a multiple of key_heads, at most 4096. */
+ * key_dim, value_dim 64 or 128; heads a multiple of key_heads, at most 4096. Fewer than 2^32 lanes:
+ * 1024 a step and head (256 at 64 x 64), 2 value_dim a run and head. */
 typedef struct {
   const uint16_t *queries, *keys, *values;
   const float *log_decay, *strengths;
@@ -866,7 +867,8 @@ int32_t omnia_linear_attention(const omnia_linear_attention_t* call, hipStream_t
  * z / (1 + exp(-z)) (silu 1) or 1 / (1 + exp(-z)) (silu 0). x, gate bf16 [rows, width], rows
  * their strides apart; weight bf16 [group] (weight_width == group) or [width]; out [rows, width].
  * The gated norm behind the mixers of models/qwen3_5 and of core/kernels/mamba_step.
- * group a multiple of 8, at most 8192, dividing width. */
+ * group a multiple of 8, at most 8192, dividing width; fewer than 2^32 lanes (4 a group of up to 64,
+ * 8 of up to 128, 16, 32, and 64 of more than 512). */
 int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t* gate,
                              int64_t gate_stride, const uint16_t* weight, int64_t weight_width,
                              int64_t rows, int64_t width, int64_t group, float eps, int32_t silu,
@@ -881,7 +883,8 @@ int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, const uint16_t
  * bf16 [rows, hidden], rows gate_stride apart (0: one row for all); act is 1 / (1 + exp(-z))
  * (sigmoid 1) or z itself; post_weight [hidden] or null, pre_weight [hidden].
  * Beside omnia_add_rms_norm, for blocks that are normed on both sides (core/kernels/add_norm).
- * hidden a multiple of 8, at most 16384. */
+ * hidden a multiple of 8, at most 16384; fewer than 2^32 lanes (64 a row of up to 512, 128 of up to
+ * 1024, 256, and 512 of more than 2048). */
 int32_t omnia_block_norm(const uint16_t* x, const uint16_t* block, const uint16_t* gate,
                          int64_t gate_stride, int32_t sigmoid, const uint16_t* post_weight,
                          float post_eps, const uint16_t* pre_weight, float pre_eps,

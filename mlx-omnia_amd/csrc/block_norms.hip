@@ -166,8 +166,7 @@ __global__ __launch_bounds__(64 * kWaves) void block_norm_kernel(BlockArgs a) {
 }
 
 template <int kLanes, int kVectors>
-void launch_gated(const GatedArgs& a, bool gate_first, hipStream_t stream) {
-  const int64_t blocks = (a.items + 256 / kLanes - 1) / (256 / kLanes);
+void launch_gated(const GatedArgs& a, int64_t blocks, bool gate_first, hipStream_t stream) {
   if (gate_first) gated_rms_norm_kernel<kLanes, kVectors, true><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
   else gated_rms_norm_kernel<kLanes, kVectors, false><<<dim3(static_cast<unsigned>(blocks)), 256, 0, stream>>>(a);
 }
@@ -196,23 +195,21 @@ extern "C" int32_t omnia_gated_rms_norm(const uint16_t* x, int64_t x_stride, con
   OMNIA_REQUIRE(x_stride % 8 == 0 && gate_stride % 8 == 0 && x_stride >= width && gate_stride >= width,
                 "gated_rms_norm: row strides must be multiples of 8 covering the row");
   const int64_t groups = width / group;
-  OMNIA_REQUIRE(rows * groups < (int64_t{1} << 32), "gated_rms_norm: too many groups");
-  int32_t rc = check_device(stream);
-  if (rc != 0) return rc;
   const int vectors = static_cast<int>(group / 8);
-  const GatedArgs a{x, gate, weight, x_stride, gate_stride, out, rows * groups, static_cast<int>(groups), vectors,
-                    weight_width == width ? static_cast<int>(group) : 0, 1.0f / static_cast<float>(group), eps, silu};
   // Two vectors a lane, and past a wave more: 8,192 rows of 4,096 (201 MB) took 37.2, 36.7 and 48.2 us with
   // one, two and four in groups of 64, 41, 35.8 and 38 of 128, 40.2, 36.4 (5.5 TB/s) and 37.8 of 512. (Read
   // past the caches, groups of 64 43.1 for 37.2, the others as they are.)
-  if (vectors <= 8) launch_gated<4, 2>(a, gate_first != 0, stream);
-  else if (vectors <= 16) launch_gated<8, 2>(a, gate_first != 0, stream);
-  else if (vectors <= 32) launch_gated<16, 2>(a, gate_first != 0, stream);
-  else if (vectors <= 64) launch_gated<32, 2>(a, gate_first != 0, stream);
-  else if (vectors <= 128) launch_gated<64, 2>(a, gate_first != 0, stream);
-  else if (vectors <= 256) launch_gated<64, 4>(a, gate_first != 0, stream);
-  else if (vectors <= 512) launch_gated<64, 8>(a, gate_first != 0, stream);
-  else launch_gated<64, 16>(a, gate_first != 0, stream);
+  const int lanes = vectors <= 8 ? 4 : vectors <= 16 ? 8 : vectors <= 32 ? 16 : vectors <= 64 ? 32 : 64;
+  const int64_t blocks = (rows * groups + 256 / lanes - 1) / (256 / lanes);
+  OMNIA_REQUIRE(fits_launch(blocks, 256), "gated_rms_norm: too many groups for one launch");
+  int32_t rc = check_device(stream);
+  if (rc != 0) return rc;
+  const GatedArgs a{x, gate, weight, x_stride, gate_stride, out, rows * groups, static_cast<int>(groups), vectors,
+                    weight_width == width ? static_cast<int>(group) : 0, 1.0f / static_cast<float>(group), eps, silu};
+  const auto launch = lanes == 4 ? launch_gated<4, 2> : lanes == 8 ? launch_gated<8, 2> : lanes == 16 ? launch_gated<16, 2>
+                      : lanes == 32 ? launch_gated<32, 2> : vectors <= 128 ? launch_gated<64, 2>
+                      : vectors <= 256 ? launch_gated<64, 4> : vectors <= 512 ? launch_gated<64, 8> : launch_gated<64, 16>;
+  launch(a, blocks, gate_first != 0, stream);
   return launched("gated_rms_norm");
 }
 
@@ -231,15 +228,17 @@ extern "C" int32_t omnia_block_norm(const uint16_t* x, const uint16_t* block, co
                 "block_norm: pointers must be 16-byte aligned");
   OMNIA_REQUIRE(gate == nullptr || gate_stride == 0 || (gate_stride % 8 == 0 && gate_stride >= hidden),
                 "block_norm: the gate's row stride must be 0 or a multiple of 8 covering the row");
+  const int vectors = static_cast<int>(hidden / 8);
+  // The fewest waves that hold the row a vector a lane, and past eight more vectors a lane.
+  const int waves = vectors <= 64 ? 1 : vectors <= 128 ? 2 : vectors <= 256 ? 4 : 8;
+  OMNIA_REQUIRE(fits_launch(rows, 64 * waves), "block_norm: too many rows for one launch");
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
-  const int vectors = static_cast<int>(hidden / 8);
   const BlockArgs a{x, block, gate, post_weight, pre_weight, gate_stride, summed, normalized, vectors,
                     static_cast<float>(hidden), post_eps, pre_eps, residual_scale, block_scale, sigmoid};
-  // The fewest waves that hold the row a vector a lane, and past eight more vectors a lane.
-  if (vectors <= 64) launch_block<1, 1>(a, rows, stream);
-  else if (vectors <= 128) launch_block<2, 1>(a, rows, stream);
-  else if (vectors <= 256) launch_block<4, 1>(a, rows, stream);
+  if (waves == 1) launch_block<1, 1>(a, rows, stream);
+  else if (waves == 2) launch_block<2, 1>(a, rows, stream);
+  else if (waves == 4) launch_block<4, 1>(a, rows, stream);
   else if (vectors <= 512) launch_block<8, 1>(a, rows, stream);
   else if (vectors <= 1024) launch_block<8, 2>(a, rows, stream);
   else launch_block<8, 4>(a, rows, stream);

@@ -28,6 +28,9 @@ inline bool aligned16(const void* ptr) {
   return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
 }
 
+// Whether one launch carries so many workgroups of so many lanes: HIP refuses a grid of 2^32 lanes.
+inline bool fits_launch(int64_t workgroups, int64_t lanes) { return workgroups <= ((int64_t{1} << 32) - 1) / lanes; }
+
 }  // namespace omnia
 
 #define OMNIA_REQUIRE(cond, message)                         \

@@ -52,8 +52,9 @@ __device__ __forceinline__ Decay decay_of(float g) {
 // Two to four vectors a lane: 200 requests of 64 heads of 128 x 64 took 156 us with eight, 64 of 32 of
 // 128 x 128 50.1 with 16 and 47.5 with four; of 64 x 64, 128 of 32 heads, 25.3 with four and 31.7 with one.
 // (The states go out at the end: right behind the last token's update it was 49.8 for 47.5.)
+constexpr int step_threads(int64_t state) { return state >= 64 * 128 ? 1024 : 256; }
 template <int DK, int DV>
-constexpr int kStepThreads = DK * DV >= 64 * 128 ? 1024 : 256;
+constexpr int kStepThreads = step_threads(DK * DV);
 
 template <int DK, int DV>
 __global__ __launch_bounds__((kStepThreads<DK, DV>)) void linear_step_kernel(LinearArgs a) {
@@ -951,10 +952,10 @@ extern "C" int32_t omnia_linear_attention(const omnia_linear_attention_t* c, hip
   const int64_t need = omnia_linear_attention_workspace_bytes(c->heads, c->key_dim, c->value_dim, c->pieces);
   OMNIA_REQUIRE(need == 0 || (c->workspace && c->workspace_bytes >= need && aligned16(c->workspace)),
                 "linear_attention: workspace too small (omnia_linear_attention_workspace_bytes) or not aligned");
-  constexpr int64_t kBlocks = int64_t{1} << 31;
-  OMNIA_REQUIRE(c->step_count * c->heads < kBlocks && c->run_count * c->heads < kBlocks &&
-                    c->chain_count * c->heads * 16 < kBlocks,
-                "linear_attention: too many steps or runs");
+  const int64_t state = c->key_dim * c->value_dim;
+  OMNIA_REQUIRE(fits_launch(c->step_count * c->heads, step_threads(state)) && fits_launch(c->run_count * c->heads, 2 * c->value_dim) &&
+                    fits_launch(c->chain_count * c->heads, state / 4),
+                "linear_attention: too many steps or runs for one launch");
   int32_t rc = check_device(stream);
   if (rc != 0) return rc;
   float* carried = static_cast<float*>(c->workspace);
