@@ -34,6 +34,7 @@ import math
 from collections.abc import Sequence
 from dataclasses import dataclass
 from typing import Protocol, runtime_checkable
+from weakref import WeakKeyDictionary
 
 import numpy as np
 import torch
@@ -71,8 +72,9 @@ class LinearBatch:
         if self.total >= 1 << 24:
             raise ValueError(f"LinearBatch: {self.total} tokens, of at most {(1 << 24) - 1}")
         self.device = torch.device(device)
-        self.plans: dict = {}   # what a layer's binding laid out for the batch
-        self._lists: dict[int, ops.LinearLists] = {}
+        # What a layer's binding laid out for the batch, which keeps no layer, nor its pool, alive.
+        self.plans: WeakKeyDictionary = WeakKeyDictionary()
+        self._lists: dict[tuple[int, int], ops.LinearLists] = {}
 
     def check(self, states: torch.Tensor) -> None:
         if self.slots and max(self.slots) >= states.shape[0]:
