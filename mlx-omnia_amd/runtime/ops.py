@@ -1854,22 +1854,40 @@ class LinearLists:
     chains: torch.Tensor
     handed_on: int
     pieces: int
-    stream: int   # that was current when they were laid out
+    readers: set[int]   # streams that their memory is kept for, should the batch be dropped
 
     @classmethod
     def of(cls, steps, handed_on, last, chains, pieces: int, device) -> "LinearLists":
         flat = [x for rows in (steps, handed_on, last, chains) for row in rows for x in row]
-        held = torch.tensor(flat, dtype=torch.int32).to(device)
         counts = 3 * len(steps), 5 * (len(handed_on) + len(last)), 2 * len(chains)
-        parts = held.split(counts)
-        stream = _raw_stream(held.get_device()) if held.is_cuda else 0
-        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces, stream)
+        parts = _uploaded(flat, device).split(counts)
+        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces, set())
 
     def used_on(self, stream: int) -> None:
         """Nobody else gets their memory, should the batch be dropped, before a call on `stream` has
         read them. (A captured call's batch is kept as long as its graph.)"""
-        if stream != self.stream and not torch.cuda.is_current_stream_capturing():
+        if stream not in self.readers and not torch.cuda.is_current_stream_capturing():
             self.runs.record_stream(torch.cuda.current_stream(self.runs.device))
+            self.readers.add(stream)
+
+
+_upload_streams: dict[torch.device, torch.cuda.Stream] = {}
+
+
+def _uploaded(numbers: list[int], device: torch.device) -> torch.Tensor:
+    """int32 numbers on `device`, there when this returns: any stream may read them. They go up from pinned
+    memory on a stream of their own, so that the host waits for them alone and not for the work that the
+    caller's stream still has to do."""
+    if device.type != "cuda":
+        return torch.tensor(numbers, dtype=torch.int32, device=device)
+    device = torch.device(device.type, torch.cuda.current_device() if device.index is None else device.index)
+    stream = _upload_streams.get(device)
+    if stream is None:
+        stream = _upload_streams[device] = torch.cuda.Stream(device)
+    with torch.cuda.stream(stream):
+        there = torch.tensor(numbers, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
+    stream.synchronize()
+    return there
 
 
 def linear_attention_places(states: torch.Tensor, key_heads: int) -> int:

@@ -38,3 +38,59 @@ def test_a_batch_keeps_no_layer_alive(tokens):
     own = kept.strategy.core.states
     before = own.clone()
     check(kept(batch, **made), own, made, None, before, slots, tokens, 0.125)
+
+
+@pytest.mark.parametrize("tokens", [[1, 1, 1], [300, 1, 70], [2000]])
+@pytest.mark.parametrize("own", [False, True])
+def test_a_first_call_does_not_wait_for_earlier_work(tokens, own):
+    """Its lists go up while the caller's stream is busy: the host is back before that is done."""
+    made, _, states, slots = inputs(tokens, 4, 2, 64, 64, device="cuda")
+    mixer, before = layer(states, 2), states.clone()
+    warm = layer(states.clone(), 2)
+    warm(LinearBatch(slots, tokens), **made)   # what a process does once
+    wide = torch.randn(8192, 8192, device="cuda")
+    torch.mm(wide, wide)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream() if own else torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        for _ in range(8):   # tens of milliseconds
+            torch.mm(wide, wide)
+        earlier = torch.cuda.Event()
+        earlier.record(stream)
+        out = mixer(LinearBatch(slots, tokens), **made)
+        busy = not earlier.query()
+    stream.synchronize()
+    assert busy
+    check(out, states, made, None, before, slots, tokens, 0.125)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_dropped_batch_is_read_before_another_takes_its_place(own):
+    """Lists of batches that are made and dropped while the stream that reads them is behind."""
+    tokens = [130, 1, 1]
+    made, _, states, slots = inputs(tokens, 4, 2, 64, 64, device="cuda")
+    mixer = layer(states, 2)
+    wide = torch.randn(8192, 8192, device="cuda")
+    mixer(LinearBatch(slots, tokens), **made)
+    torch.mm(wide, wide)
+    torch.cuda.synchronize()
+    want, stream = states.clone(), torch.cuda.Stream() if own else torch.cuda.current_stream()
+    reference, turns = layer(want, 2), [slots, slots[::-1], slots[1:] + slots[:1]]
+    for turn in turns:
+        kept = LinearBatch(turn, tokens)
+        reference(kept, **made)
+        torch.cuda.synchronize()
+    seen = set()
+    with torch.cuda.stream(stream):
+        for _ in range(8):   # tens of milliseconds
+            torch.mm(wide, wide)
+        earlier = torch.cuda.Event()
+        earlier.record(stream)
+        for turn in turns:
+            batch = LinearBatch(turn, tokens)
+            mixer(batch, **made)
+            seen.add(next(iter(batch._lists.values())).runs.data_ptr())
+            del batch
+        busy = not earlier.query()
+    stream.synchronize()
+    assert busy and len(seen) == len(turns) and torch.equal(states, want)
