@@ -195,7 +195,7 @@ class DefaultLinearAttention(LinearAttentionStrategy):
 
     def __call__(self, batch, queries, keys, values, log_decay=None, strengths=None):
         self._check(batch, queries, keys, values, log_decay, strengths)
-        kind = torch.promote_types(queries.dtype, torch.float32)
+        kind = torch.promote_types(queries.dtype, self.states.dtype)   # 32 bits or more, as the pool holds them
         group = self.heads // self.key_heads
         q, k = (x.to(kind).repeat_interleave(group, dim=1) for x in (queries, keys))
         v, gates = values.to(kind), self._gates(batch, log_decay)
