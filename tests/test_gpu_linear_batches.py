@@ -94,3 +94,12 @@ def test_a_dropped_batch_is_read_before_another_takes_its_place(own):
         busy = not earlier.query()
     stream.synchronize()
     assert busy and len(seen) == len(turns) and torch.equal(states, want)
+
+
+def test_under_another_default_device():
+    """A batch is made and first called where tensors are made on the GPU by default."""
+    made, _, states, slots = inputs([70, 1], 4, 2, 64, 64, device="cuda")
+    before = states.clone()
+    with torch.device("cuda"):
+        out = layer(states, 2)(LinearBatch(slots, [70, 1]), **made)
+    check(out, states, made, None, before, slots, [70, 1], 0.125)
