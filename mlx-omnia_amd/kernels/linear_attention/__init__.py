@@ -58,7 +58,8 @@ class LinearBatch:
     """The sequences of a call: the slots of their states, each once, and how many new tokens each
     has (none among them). Their rows lie together in the call's tensors, in this order. Made on
     the host and kept as long as the same slots step on, or a graph that took a call of it is
-    replayed."""
+    replayed. Its first call, which is made ahead of a capture, sends its lists to the device on the call's
+    stream; calls on other streams wait for them there, and a graph's replays are ordered behind that call."""
 
     def __init__(self, slots: Sequence[int], tokens: Sequence[int], *, device: torch.device | str = "cuda") -> None:
         self.slots, self.tokens = tuple(int(s) for s in slots), tuple(int(n) for n in tokens)

@@ -1843,51 +1843,55 @@ def moe_down_combine_nvfp4_shared(
     return out
 
 
-@dataclass(frozen=True)
+@dataclass
 class LinearLists:
     """What `omnia_linear_attention` does with a batch's sequences: int32 lists on the device, steps
     [n, 3], runs [n, 5] of which the first `handed_on` are no last pieces, chains [n, 2], and the
-    places that the pieces take in the workspace."""
+    places that the pieces take in the workspace. They go up from pinned memory, in the order of the
+    stream that is current then: the host does not wait."""
 
     steps: torch.Tensor
     runs: torch.Tensor
     chains: torch.Tensor
     handed_on: int
     pieces: int
-    readers: set[int]   # streams that their memory is kept for, should the batch be dropped
+    stream: int                          # that was current when they were laid out
+    uploaded: torch.cuda.Event | None    # behind which they are there; None once that is known
+    readers: set[int]                    # streams that their memory is kept for, should the batch be dropped
 
     @classmethod
     def of(cls, steps, handed_on, last, chains, pieces: int, device) -> "LinearLists":
         flat = [x for rows in (steps, handed_on, last, chains) for row in rows for x in row]
         counts = 3 * len(steps), 5 * (len(handed_on) + len(last)), 2 * len(chains)
-        parts = _uploaded(flat, device).split(counts)
-        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces, set())
+        uploaded, stream = None, 0
+        if device.type == "cuda":
+            held = torch.tensor(flat, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
+            current = torch.cuda.current_stream(held.device)
+            uploaded, stream = torch.cuda.Event(), current.cuda_stream
+            uploaded.record(current)
+        else:
+            held = torch.tensor(flat, dtype=torch.int32, device=device)
+        parts = held.split(counts)
+        return cls(parts[0].view(-1, 3), parts[1].view(-1, 5), parts[2].view(-1, 2), len(handed_on), pieces, stream, uploaded,
+                   {stream})
 
     def used_on(self, stream: int) -> None:
-        """Nobody else gets their memory, should the batch be dropped, before a call on `stream` has
-        read them. (A captured call's batch is kept as long as its graph.)"""
-        if stream not in self.readers and not torch.cuda.is_current_stream_capturing():
-            self.runs.record_stream(torch.cuda.current_stream(self.runs.device))
+        """Ahead of a call on `stream`, the current one: it reads them when they are there, and nobody else gets
+        their memory, should the batch be dropped, before it has. (A captured call's batch is kept as long as its
+        graph, whose replays come behind the batch's first call.)"""
+        if (self.uploaded is None or stream == self.stream) and stream in self.readers:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.runs.device)
+        if self.uploaded is not None and stream != self.stream:
+            if self.uploaded.query():
+                self.uploaded = None
+            else:
+                current.wait_event(self.uploaded)
+        if stream not in self.readers:
+            self.runs.record_stream(current)
             self.readers.add(stream)
-
-
-_upload_streams: dict[torch.device, torch.cuda.Stream] = {}
-
-
-def _uploaded(numbers: list[int], device: torch.device) -> torch.Tensor:
-    """int32 numbers on `device`, there when this returns: any stream may read them. They go up from pinned
-    memory on a stream of their own, so that the host waits for them alone and not for the work that the
-    caller's stream still has to do."""
-    if device.type != "cuda":
-        return torch.tensor(numbers, dtype=torch.int32, device=device)
-    device = torch.device(device.type, torch.cuda.current_device() if device.index is None else device.index)
-    stream = _upload_streams.get(device)
-    if stream is None:
-        stream = _upload_streams[device] = torch.cuda.Stream(device)
-    with torch.cuda.stream(stream):
-        there = torch.tensor(numbers, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
-    stream.synchronize()
-    return there
 
 
 def linear_attention_places(states: torch.Tensor, key_heads: int) -> int:
@@ -1969,8 +1973,8 @@ class LinearAttentionPlan:
             workspace = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
             args.workspace = workspace.data_ptr()
         stream = _stream_here(self.index)
-        call("omnia_linear_attention", ctypes.addressof(args), stream)
         self.lists.used_on(stream)
+        call("omnia_linear_attention", ctypes.addressof(args), stream)
         del q, k, v, g, strengths   # held until here
         return out
 
