@@ -836,8 +836,10 @@ int32_t omnia_attention_batch_step(const omnia_attention_batch_step_t* step, hip
  * more: their first place and how many. No slot may be named twice; an entry outside the states,
  * the tokens or the workspace is skipped. workspace: at least
  * omnia_linear_attention_workspace_bytes, 16-byte aligned (null where that is 0).
- * Its input is what omnia_gate_softplus gives (models/qwen3_5/layers/deltanet.py:222-224);
- * the single-token recurrence stands where core/kernels/ssm does.
+ * For heads with fixed decays and for state-space layers (the single-token recurrence of
+ * core/kernels/ssm), whose g omnia_gate_softplus gives and whose w are -g exp(-A_log); the gated
+ * delta rule (models/qwen3_5/layers/deltanet.py) is another recurrence. A product of decays below
+ * 2^-126 may count as zero.
  * key_dim, value_dim 64 or 128; heads a multiple of key_heads, at most 4096. Fewer than 2^32 lanes:
  * 1024 a step and head (256 at 64 x 64), 2 value_dim a run and head. */
 typedef struct {

@@ -5,8 +5,8 @@
 //
 // Steps: a workgroup takes one head of one sequence with its whole state in registers (64 KB at
 // 128 x 128, all asked for at once), so a step of one token reads and writes the state once and is
-// bound by that: 64 requests of 32 heads of 128 x 128, 268 MB over pools in turn, take 47.5 us (5.7 TB/s),
-// 200 of 64 heads of 128 x 64, 839 MB, 150 us (5.6 TB/s); a plain copy reaches 6.5. Both go past the
+// bound by that: 64 requests of 32 heads of 128 x 128, 268 MB over pools in turn, take 47 us (5.7 TB/s),
+// 200 of 64 heads of 128 x 64, 839 MB, 149 us (5.6 TB/s); a plain copy reaches 6.5. Both go past the
 // caches, as the states of all layers do not stay in them: 57.5 -> 50.2 us and 167 -> 156 when the lanes
 // held 16 and 8 vectors (45 -> 50 for one pool of 134 MB over and over, half of which the last-level
 // cache keeps).
@@ -14,10 +14,11 @@
 // Prompts: a workgroup takes one head of one piece of a sequence, 64 tokens at a time on the matrix
 // unit. Where the sequences are too few to fill the card each is cut into pieces: the pieces' own
 // parts of the state first (k and v alone), then the states ahead of each, then the pieces' contexts.
-// 32,768 tokens of 32 heads of 128 x 128 take 375 us: 120 the parts, 11 the states between, 245 the
-// contexts, at 0.80 and 0.88 PFLOP/s of products (97 and 215 GFLOP with the parts that 32-bit states
-// cost; a large product of bf16 alone reaches 1.2, and both clock the card down). 8,192 tokens of 64
-// heads of 128 x 64 take 116 us: 31, 11 and 69.
+// 32,768 tokens of 32 heads of 128 x 128 take 422 us back to back, and in the kernel trace 126 the parts, 12 the
+// states between and 345 the contexts, at 0.77 and 0.76 PFLOP/s of products (97 and 262 GFLOP with the parts
+// that 32 bits cost; a large product of bf16 alone reaches 1.2). 8,192 tokens of 64 heads of 128 x 64 take 123 us,
+// in the trace 39, 12 and 96. By the counters the contexts' vector instructions take 63% of the cycles and the
+// matrix unit's 53 (45 of 128 x 64), the LDS 22 without a conflict, and the clock is at 1.8 to 2 of 2.4 GHz.
 #include "common.hpp"
 #include "host.hpp"
 
@@ -287,17 +288,18 @@ struct Gates {
 // rows are numbered 16 j + 8 half + 0..7 (lane (half, c) holds its column c of those), for which k is
 // transposed in that order: S is an operand of q S, and the columns of P that a wave has made one of
 // P v, as they are. S, P and the scaled v, fp32 all of them, enter their products as three bf16 parts,
-// which hold all 24 bits, as the steps multiply them. (S and P in two parts, of 16 bits, 12 sequences up to 1,501
-// of 32 heads of 128 x 128 took 94 us for 105, 32,768 tokens 368 for 406, 8,192 of 64 heads of 128 x 64 115.5
-// for 126; the contexts then differed from those of fp32 products by 1.3e-4 of their size, and by 2 to 4e-5
-// now, as sums in another order do.) G is summed
-// in fp64, and what the state's factors are made of are its differences in fp64: a fast decay ahead of
-// a slow one would swallow the slow one's. P's weights are products of exp(G_t) and exp(-G_s), each a
-// number of [1, 2) or (1/2, 1] times a power of two of its own, so that the fast decays' powers cancel
-// exactly: what is left is a few fp32 roundings, and no exponential for each of P's numbers.
+// which hold all 24 bits, as the steps multiply them. (With S and P in two parts, of 16 bits, 12 sequences
+// up to 1,501 tokens of 32 heads of 128 x 128 took 94 us for 105, 32,768 tokens 368 for 406, 8,192 of 64 heads
+// of 128 x 64 115.5 for 126; the contexts then differed from those of fp32 products by 1.3e-4 of their size,
+// and by 2 to 5e-5 now, as sums in another order do.) G is summed in fp64, and what the state's factors are made
+// of are its differences in fp64: a fast decay ahead of a slow one would swallow the slow one's. P's weights
+// are products of exp(G_t) and exp(-G_s), each a number of [1, 2) or (1/2, 1] times a power of two of its
+// own, so that the fast decays' powers cancel exactly: what is left is a few fp32 roundings, and no
+// exponential for each of P's numbers. Factors below 2^-126 are zeros.
 // The next chunk's rows go straight to LDS while this one's are multiplied: k to the other of two
 // tiles, v, which is held as operands from the start, and q, done with after the first half, to the
-// same. Its decays are summed by the wave that has no part of P.
+// same (k and v where P lies only when it is done with). Its decays are summed by the wave that has no
+// part of P.
 template <int DK, int DV, int kHeads>
 __global__ __launch_bounds__(2 * DV * kHeads, 2) void linear_chunk_kernel(LinearArgs a) {
   constexpr int kWidth = DV * kHeads, kWaves = kWidth / 32, kThreads = 64 * kWaves;

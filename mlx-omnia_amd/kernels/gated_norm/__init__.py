@@ -5,10 +5,10 @@
 
 norm(v) = v / sqrt(mean(v^2) + eps) over each `group` consecutive values of a row (a head), act
 silu or sigmoid; in fp32, rounded once. The declaration is the norm leaf (`.weight` [group] or
-[row width], `.eps`); a call takes x and the gate [..., width] or [..., heads, group], alike in
-shape, row-strided views of wider rows among them. `HipGatedRmsNorm` (`omnia_gated_rms_norm`,
-csrc/block_norms.hip) serves bf16 on a gfx950 device, `DefaultGatedRmsNorm` everything else and
-calls that autograd follows.
+[row width], `.eps`); a call takes x and the gate [..., width] or, with a weight [group],
+[..., heads, group], alike in shape, row-strided views of wider rows among them.
+`HipGatedRmsNorm` (`omnia_gated_rms_norm`, csrc/block_norms.hip) serves bf16 on a gfx950 device,
+`DefaultGatedRmsNorm` everything else and calls that autograd follows.
 """
 
 from __future__ import annotations

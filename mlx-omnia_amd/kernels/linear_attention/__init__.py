@@ -3,11 +3,14 @@
     S_t = exp(g_t) S_{t-1} + w_t k_t v_t^T,   o_t = scale * q_t S_t
 
 for each sequence's new tokens in order, S [key_dim, value_dim] fp32 of every head in a pool
-`states` [slots, heads, key_dim, value_dim]. It reads what `GateSoftplus` gives
-(models/qwen3_5/layers/deltanet.py:222-224: g = -exp(A_log) softplus(a + dt_bias)), and stands
-beside `AttentionStep` as the single-token recurrence of core/kernels/ssm stands beside
-core/kernels/attention. One call takes prompts and steps of one token alike, a batch of any
-lengths:
+`states` [slots, heads, key_dim, value_dim]. It serves mixers whose heads forget at rates of their
+own: fixed ones (`decay`), or each token's, as state-space layers have them (the single-token
+recurrence of core/kernels/ssm): g = -exp(A_log) softplus(a + dt_bias), which `GateSoftplus`
+gives, with the strengths w = softplus(a + dt_bias), which are -g exp(-A_log). It has no term that
+corrects a value by what the state holds: the gated delta rule, which
+models/qwen3_5/layers/deltanet.py makes the same decays for, is another operator. It stands beside
+`AttentionStep` as core/kernels/ssm stands beside core/kernels/attention. One call takes prompts
+and steps of one token alike, a batch of any lengths:
 
     states = torch.zeros(slots, heads, key_dim, value_dim, device="cuda")
     mixer = LinearAttention(states, heads=32, key_heads=16, key_dim=128, value_dim=128,
@@ -19,7 +22,8 @@ A fresh sequence's state is zeros and a fork's a copy of its parent's (`states[k
 states[parent]`): both are the caller's, on the stream of the calls.
 
 - `HipLinearAttention` (`omnia_linear_attention`, csrc/linear_attention.hip): bf16 rows, heads
-  of 64 or 128, any number of heads per key head, fp32 gates and states.
+  of 64 or 128, any number of heads per key head, fp32 gates and states. A layer that is made
+  with `dtype=torch.bfloat16` on the device refuses rows and gates of other types.
 - `DefaultLinearAttention` is the Core chain in torch ops, and takes everything, calls that
   autograd follows among it: gradients of the call's own inputs (the pool follows none).
 
